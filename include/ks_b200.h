@@ -226,6 +226,96 @@ int ks_indexer_noalloc(const void* q, const void* k, int64_t k_batch_rows, const
                        int32_t topk, int64_t offset, void* out, int32_t out_dtype, void* stream);
 
 /*
+ * The quantised latent cache.  A cached row has D = dq + dr columns: dq in e4m3 with
+ * one power-of-two scale per row (as ks_quant_fp8_rows, but at most 2^119), dr (the rotary part) in bf16:
+ *   kv8   e4m3 [n_slots, dq]      kv_scale fp32 [n_slots]      kv_tail bf16 [n_slots, dr]
+ * Slot s is row s % page of page s / page; position i of a sequence is row i % page of
+ * page page_table[b, i / page].
+ *
+ * ks_cache_write quantises R rows as they are written: row r (bf16, at kv + r *
+ * kv_stride elements) goes to slot slots[r] (int32 or int64, slot_dtype KS_INT32 /
+ * KS_INT64).  Negative slots store nothing; slots >= n_slots store nothing and are
+ * reported by ks_device_status.  Slots must not repeat within a call (one of the rows
+ * would win, column by column).  A row that holds a NaN or an infinity is stored with
+ * scale NaN and zero codes: it reads back as NaN.
+ * dq % 16 == 0, 16 <= dq <= 1024, dr % 8 == 0, 0 <= dr <= 1024, kv_stride >= D and a
+ * multiple of 8; kv, kv8, kv_tail 16-byte aligned.  kv_tail may be NULL when dr = 0.
+ * No counterpart in the reference.
+ */
+int ks_cache_write(const void* kv, int64_t kv_stride, const void* slots, int32_t slot_dtype,
+                   int64_t R, void* kv8, float* kv_scale, void* kv_tail, int64_t n_slots,
+                   int32_t dq, int32_t dr, void* stream);
+
+/*
+ * Positions [start, start + n) of B sequences read back as bf16 rows: out [B, n, D],
+ * e4m3 code * scale (exact in bf16).  Positions at or beyond lens[b] give zero rows;
+ * a position whose page is outside the table or the pool gives a zero row and is
+ * reported by ks_device_status.  The result is what ks_sparse_attn takes as kv.
+ *   page_table int32 [B, max_pages], lens int32 [B], B <= 65535, start + n < 2^31
+ * No counterpart in the reference.
+ */
+int ks_cache_read(const void* kv8, const float* kv_scale, const void* kv_tail, int64_t n_pages,
+                  int32_t page, int32_t dq, int32_t dr, const int32_t* page_table,
+                  int64_t max_pages, const int32_t* lens, int64_t B, int64_t n, int64_t start,
+                  void* out, void* stream);
+
+/* Workspace bytes ks_tree_attn needs. */
+size_t ks_tree_attn_workspace_size(int64_t B, int64_t T, int64_t H, int64_t dv);
+
+/*
+ * Attention of T drafted tokens per sequence over the quantised latent cache (T = 1:
+ * a decoding step).  The rows of the drafted tokens are in the cache already, at
+ * positions lens[b] .. lens[b] + T - 1 (ks_cache_write).
+ *   q    bf16 [B, T, H, D], D = dq + dr; all heads share the cached rows (MQA / MLA latent)
+ *   key  k < lens[b]: seen by every drafted token of sequence b
+ *   key  lens[b] + j: seen by token i where mask[b, i, j] != 0 (uint8 [B, T, T]; NULL:
+ *        where j <= i, a chain)
+ *   out  bf16 [B, T, H, dv] = softmax(softmax_scale * q . k) v, v = the first dv columns
+ *        of the row; attn_sink (fp32 [H], may be NULL) adds a logit that carries no value.
+ *        A token that sees no key gets zeros.
+ * A row stored with scale NaN makes every token that sees it NaN, and no other.
+ * Key positions whose page is outside the table or the pool are skipped and reported by
+ * ks_device_status.  kv_scale must hold powers of two (or NaN), as ks_cache_write writes.
+ * Requirements: dq % 64 == 0, dr 0 or 64, D <= 576, dv % 64 == 0, dv <= min(D, 512),
+ * H <= 1024, q, out, kv8, kv_tail 16-byte aligned, workspace 256-byte aligned and at
+ * least ks_tree_attn_workspace_size bytes.  No counterpart in the reference, whose
+ * attention (baseline/sparse_attention.py:5-42) reads contiguous bf16 rows.
+ */
+int ks_tree_attn(const void* q, const void* kv8, const float* kv_scale, const void* kv_tail,
+                 int64_t n_pages, int32_t page, int32_t dq, int32_t dr,
+                 const int32_t* page_table, int64_t max_pages, const int32_t* lens,
+                 const uint8_t* mask, const float* attn_sink, void* out, int64_t B, int64_t T,
+                 int64_t H, int64_t dv, float softmax_scale, void* workspace,
+                 size_t workspace_bytes, void* stream);
+
+/*
+ * Verification of T drafted tokens per sequence against the target's probabilities, from
+ * given random numbers.
+ *   p      fp32 [B, T + 1, V]: row 0 after the last accepted token, row i + 1 after
+ *          drafted token i
+ *   tokens int32 or int64 [B, T] (token_dtype KS_INT32 / KS_INT64)
+ *   u      fp32 [B, T + 1] in [0, 1): decides at row r;  noise fp32 [B, V], positive
+ *          (exponential): samples the next token
+ *   q != NULL (fp32 [B, T, V], parents NULL): a chain sampled from q.  Token i stands if
+ *     u[i] * q[i, x_i] < p[i, x_i] and all before it stand; n of them do.  The next token
+ *     is argmax_x w(x) / noise(x), w = max(p[n] - q[n], 0) (n < T) or p[T].
+ *   q == NULL: fixed candidates.  parents int32 [B, T], -1 <= parents[i] < i, gives the
+ *     tree (NULL: a chain).  At row r its children c_1, c_2, .. (in index order; one that
+ *     repeats an older sibling's token has probability 0 here) split [0, 1): c_k is taken
+ *     if sum_{j<k} p[r, x_j] <= u[r] < sum_{j<=k} p[r, x_j].  Where none is taken the next
+ *     token is argmax_x w(x) / noise(x), w = p[r] with its children's tokens set to 0.
+ *   Where w is 0 everywhere the row of p takes its place; ties go to the lowest token.
+ * Results: n_accepted int32 [B]; out [B, T + 1] (type of tokens): the accepted tokens,
+ * the next token, then -1; path int32 [B, T]: the accepted drafts' indices, then -1.
+ * A token outside [0, V) or a parent outside [-1, i) is never accepted and is reported
+ * by ks_device_status.  p, q, noise finite.  T <= 1024, V < 2^31.  No counterpart in the reference.
+ */
+int ks_verify_draft(const float* p, const float* q, const void* tokens, int32_t token_dtype,
+                    const int32_t* parents, const float* u, const float* noise, int64_t B,
+                    int64_t T, int64_t V, void* out, int32_t* n_accepted, int32_t* path,
+                    void* stream);
+
+/*
  * Synchronise `stream`, then read and clear the current device's status record:
  * KS_OK, or KS_ERR_DEVICE when a kernel reported a timed-out wait or a bounds
  * error since the last call (ks_last_error() then names the block, thread,

@@ -56,6 +56,16 @@ SIGNATURES = {
     "ks_indexer_fp8_scores": (ctypes.c_int, [_vp, _vp, _c_i64, _vp, _vp, _c_i64, _c_i64, _c_i64,
                                              _c_i64, _c_i64, _c_i64, _c_i32, _c_i32, _vp, _c_i64,
                                              _vp]),
+    "ks_cache_write": (ctypes.c_int, [_vp, _c_i64, _vp, _c_i32, _c_i64, _vp, _vp, _vp, _c_i64,
+                                      _c_i32, _c_i32, _vp]),
+    "ks_cache_read": (ctypes.c_int, [_vp, _vp, _vp, _c_i64, _c_i32, _c_i32, _c_i32, _vp, _c_i64,
+                                     _vp, _c_i64, _c_i64, _c_i64, _vp, _vp]),
+    "ks_tree_attn_workspace_size": (_sz, [_c_i64, _c_i64, _c_i64, _c_i64]),
+    "ks_tree_attn": (ctypes.c_int, [_vp, _vp, _vp, _vp, _c_i64, _c_i32, _c_i32, _c_i32, _vp,
+                                    _c_i64, _vp, _vp, _vp, _vp, _c_i64, _c_i64, _c_i64, _c_i64,
+                                    _c_f32, _vp, _sz, _vp]),
+    "ks_verify_draft": (ctypes.c_int, [_vp, _vp, _vp, _c_i32, _vp, _vp, _vp, _c_i64, _c_i64,
+                                       _c_i64, _vp, _vp, _vp, _vp]),
     "ks_device_status": (ctypes.c_int, [_vp]),
     "ks_selftest_wait_timeout": (ctypes.c_int, [_c_u64, _vp]),
 }

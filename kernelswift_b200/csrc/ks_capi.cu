@@ -13,6 +13,7 @@
 #include "ks_b200.h"
 #include "ks_device.cuh"
 #include "indexer_score.cuh"
+#include "latent_cache.cuh"
 #include "proj_gemm.cuh"
 #include "quant_fp8.cuh"
 #include "sinkhorn.cuh"
@@ -21,6 +22,8 @@
 #include "sparse_attn_tiny.cuh"
 #include "topk.cuh"
 #include "topk_small.cuh"
+#include "tree_attn.cuh"
+#include "verify_draft.cuh"
 
 namespace ks {
 
@@ -58,6 +61,7 @@ struct Device {
   // memory size it was last asked for
   int sa_clusters = 0;
   size_t sa_clusters_smem = 0;
+  bool vd_wide = false;  // the draft verification's cluster of 16 has been allowed
 };
 constexpr int kMaxDevices = 64;
 std::mutex g_mu;
@@ -567,6 +571,28 @@ int noalloc_scratch(void** out) {
   return KS_OK;
 }
 
+int cache_check(const char* op, const void* kv8, const float* scale, const void* tail, int64_t dq,
+                int64_t dr) {
+  if (!kv8 || !scale || (dr > 0 && !tail)) return fail(KS_ERR_INVALID, "%s: null cache pointer", op);
+  if (dq < 16 || dq % 16 || dr < 0 || dr % 8)
+    return fail(KS_ERR_INVALID, "%s: dq=%lld dr=%lld (dq a multiple of 16, dr of 8)", op, (long long)dq, (long long)dr);
+  if (dq > LC_MAX_DQ || dr > LC_MAX_DQ)
+    return fail(KS_ERR_UNSUPPORTED, "%s: dq=%lld dr=%lld > %d", op, (long long)dq, (long long)dr, LC_MAX_DQ);
+  if (!aligned(kv8, 16) || !aligned(scale, 4) || (dr > 0 && !aligned(tail, 16)))
+    return fail(KS_ERR_ALIGNMENT, "%s: kv8, kv_tail must be 16-byte and kv_scale 4-byte aligned", op);
+  return KS_OK;
+}
+int table_check(const char* op, const int32_t* table, int64_t max_pages, const int32_t* lens, int64_t n_pages,
+                int64_t page, int64_t B) {
+  if (!table || !lens) return fail(KS_ERR_INVALID, "%s: page_table and lens must be set", op);
+  if (!aligned(table, 4) || !aligned(lens, 4)) return fail(KS_ERR_ALIGNMENT, "%s: page_table, lens must be 4-byte aligned", op);
+  if (page < 1 || n_pages < 1 || max_pages < 1 || B < 1)
+    return fail(KS_ERR_INVALID, "%s: bad sizes B=%lld pages=%lld page=%lld max_pages=%lld", op, (long long)B, (long long)n_pages, (long long)page, (long long)max_pages);
+  if (n_pages > 0x7FFFFFFFll || max_pages > 0x7FFFFFFFll || B > 65535)
+    return fail(KS_ERR_UNSUPPORTED, "%s: too many pages or sequences", op);
+  return KS_OK;
+}
+
 }  // namespace
 }  // namespace ks
 
@@ -846,6 +872,185 @@ int ks_indexer_fp8(const void* q8, const void* k8, int64_t k_batch_rows, const f
                                    causal, ratio, workspace, ld, st, true, k_scale))
     return rc;
   return topk_impl(workspace, ld, B, S, T, pos0, causal, ratio, topk, offset, out, out_dtype, st);
+}
+
+int ks_cache_write(const void* kv, int64_t kv_stride, const void* slots, int32_t slot_dtype,
+                   int64_t R, void* kv8, float* kv_scale, void* kv_tail, int64_t n_slots,
+                   int32_t dq, int32_t dr, void* stream) {
+  Device* dev;
+  if (int rc = device(&dev)) return rc;
+  if (R < 0 || n_slots < 0) return fail(KS_ERR_INVALID, "cache_write: bad sizes");
+  if (int rc = cache_check("cache_write", kv8, kv_scale, kv_tail, dq, dr)) return rc;
+  if (slot_dtype != KS_INT32 && slot_dtype != KS_INT64) return fail(KS_ERR_INVALID, "cache_write: slot_dtype");
+  if (R == 0) return KS_OK;
+  if (!kv || !slots) return fail(KS_ERR_INVALID, "cache_write: null pointer");
+  if (kv_stride < (int64_t)dq + dr) return fail(KS_ERR_INVALID, "cache_write: kv_stride=%lld is less than a row", (long long)kv_stride);
+  if (!aligned(kv, 16) || kv_stride % 8 || !aligned(slots, slot_dtype == KS_INT64 ? 8 : 4))
+    return fail(KS_ERR_ALIGNMENT, "cache_write: the rows of kv must start on 16-byte boundaries");
+  CacheWriteParams p{};
+  p.kv = static_cast<const uint16_t*>(kv);
+  p.kv_stride = kv_stride;
+  p.slots = slots;
+  p.slots_i64 = slot_dtype == KS_INT64;
+  p.R = R; p.n_slots = n_slots;
+  p.kv8 = static_cast<uint8_t*>(kv8);
+  p.scale = kv_scale;
+  p.tail = static_cast<uint16_t*>(kv_tail);
+  p.dq = dq; p.dr = dr;
+  p.status = dev->status;
+  const int lanes = dq <= 64 ? 8 : dq <= 128 ? 16 : 32;
+  const int64_t blocks = (R + LC_THREADS / lanes - 1) / (LC_THREADS / lanes);
+  if (blocks > 0x7FFFFFFFll) return fail(KS_ERR_UNSUPPORTED, "cache_write: too many rows");
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const unsigned g = (unsigned)blocks;
+  if (lanes == 8) cache_write_kernel<8, 1><<<g, LC_THREADS, 0, st>>>(p);
+  else if (lanes == 16) cache_write_kernel<16, 1><<<g, LC_THREADS, 0, st>>>(p);
+  else if (dq <= 512) cache_write_kernel<32, 2><<<g, LC_THREADS, 0, st>>>(p);
+  else cache_write_kernel<32, 4><<<g, LC_THREADS, 0, st>>>(p);
+  return launch_check("cache_write_kernel launch");
+}
+
+int ks_cache_read(const void* kv8, const float* kv_scale, const void* kv_tail, int64_t n_pages,
+                  int32_t page, int32_t dq, int32_t dr, const int32_t* page_table,
+                  int64_t max_pages, const int32_t* lens, int64_t B, int64_t n, int64_t start,
+                  void* out, void* stream) {
+  Device* dev;
+  if (int rc = device(&dev)) return rc;
+  if (B < 0 || n < 0 || start < 0) return fail(KS_ERR_INVALID, "cache_read: bad sizes");
+  if (B == 0 || n == 0) return KS_OK;
+  if (int rc = cache_check("cache_read", kv8, kv_scale, kv_tail, dq, dr)) return rc;
+  if (int rc = table_check("cache_read", page_table, max_pages, lens, n_pages, page, B)) return rc;
+  if (!out) return fail(KS_ERR_INVALID, "cache_read: out is null");
+  if (!aligned(out, 16)) return fail(KS_ERR_ALIGNMENT, "cache_read: out must be 16-byte aligned");
+  if (start + n > 0x7FFFFFFFll) return fail(KS_ERR_UNSUPPORTED, "cache_read: start + n >= 2^31");
+  CacheReadParams p{};
+  p.kv8 = static_cast<const uint8_t*>(kv8);
+  p.scale = kv_scale;
+  p.tail = static_cast<const uint16_t*>(kv_tail);
+  p.n_pages = n_pages;
+  p.page = page; p.dq = dq; p.dr = dr;
+  p.table = page_table;
+  p.max_pages = max_pages;
+  p.lens = lens;
+  p.n = (int)n; p.start = (int)start;
+  p.out = static_cast<uint16_t*>(out);
+  p.status = dev->status;
+  const int lanes = dq <= 128 ? 8 : dq <= 256 ? 16 : 32;
+  const int rows = LC_THREADS / lanes;
+  const dim3 grid((unsigned)((n + rows - 1) / rows), (unsigned)B);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (lanes == 8) cache_read_kernel<8><<<grid, LC_THREADS, 0, st>>>(p);
+  else if (lanes == 16) cache_read_kernel<16><<<grid, LC_THREADS, 0, st>>>(p);
+  else cache_read_kernel<32><<<grid, LC_THREADS, 0, st>>>(p);
+  return launch_check("cache_read_kernel launch");
+}
+
+size_t ks_tree_attn_workspace_size(int64_t B, int64_t T, int64_t H, int64_t dv) {
+  (void)B; (void)T; (void)H; (void)dv;
+  return 256;
+}
+
+int ks_tree_attn(const void* q, const void* kv8, const float* kv_scale, const void* kv_tail,
+                 int64_t n_pages, int32_t page, int32_t dq, int32_t dr,
+                 const int32_t* page_table, int64_t max_pages, const int32_t* lens,
+                 const uint8_t* mask, const float* attn_sink, void* out, int64_t B, int64_t T,
+                 int64_t H, int64_t dv, float softmax_scale, void* workspace,
+                 size_t workspace_bytes, void* stream) {
+  Device* dev;
+  if (int rc = device(&dev)) return rc;
+  if (B < 0 || T < 0 || H < 1) return fail(KS_ERR_INVALID, "tree_attn: bad sizes B=%lld T=%lld H=%lld", (long long)B, (long long)T, (long long)H);
+  if (B == 0 || T == 0) return KS_OK;
+  if (int rc = cache_check("tree_attn", kv8, kv_scale, kv_tail, dq, dr)) return rc;
+  if (int rc = table_check("tree_attn", page_table, max_pages, lens, n_pages, page, B)) return rc;
+  if (!q || !out) return fail(KS_ERR_INVALID, "tree_attn: null pointer");
+  if (dq % 64 || (dr != 0 && dr != 64) || dq + dr > 576)
+    return fail(KS_ERR_UNSUPPORTED, "tree_attn: dq=%d dr=%d (dq a multiple of 64, dr 0 or 64, dq + dr <= 576)", dq, dr);
+  if (dv < 64 || dv % 64 || dv > 512 || dv > dq + dr)
+    return fail(KS_ERR_UNSUPPORTED, "tree_attn: dv=%lld (a multiple of 64, <= min(D, 512))", (long long)dv);
+  if (H > 1024) return fail(KS_ERR_UNSUPPORTED, "tree_attn: H=%lld > 1024", (long long)H);
+  if (B * T * H >= (1ll << 31) || T > (1 << 20)) return fail(KS_ERR_UNSUPPORTED, "tree_attn: too many rows");
+  if (!aligned(q, 16) || !aligned(out, 16) || (attn_sink && !aligned(attn_sink, 4)))
+    return fail(KS_ERR_ALIGNMENT, "tree_attn: q, out must be 16-byte aligned");
+  const size_t need = ks_tree_attn_workspace_size(B, T, H, dv);
+  if (!workspace || workspace_bytes < need)
+    return fail(KS_ERR_WORKSPACE, "tree_attn: workspace of %zu bytes needed", need);
+  if (!aligned(workspace, 256)) return fail(KS_ERR_ALIGNMENT, "tree_attn: workspace must be 256-byte aligned");
+  TreeAttnParams p{};
+  p.q = static_cast<const uint16_t*>(q);
+  p.kv8 = static_cast<const uint8_t*>(kv8);
+  p.scale = kv_scale;
+  p.tail = static_cast<const uint16_t*>(kv_tail);
+  p.n_pages = n_pages; p.max_pages = max_pages;
+  p.page = page; p.dq = dq; p.dr = dr;
+  p.table = page_table;
+  p.lens = lens;
+  p.mask = mask;
+  p.sink = attn_sink;
+  p.out = static_cast<uint16_t*>(out);
+  p.B = (int)B; p.T = (int)T; p.H = (int)H; p.dv = (int)dv;
+  p.scale_log2 = softmax_scale * 1.4426950408889634f;
+  p.status = dev->status;
+  const unsigned grid = (unsigned)(B * T * ((H + TA_HEADS - 1) / TA_HEADS));
+  tree_attn_simple_kernel<<<grid, TA_WARPS * 32, 0, static_cast<cudaStream_t>(stream)>>>(p);
+  return launch_check("tree_attn_simple_kernel launch");
+}
+
+int ks_verify_draft(const float* p, const float* q, const void* tokens, int32_t token_dtype,
+                    const int32_t* parents, const float* u, const float* noise, int64_t B,
+                    int64_t T, int64_t V, void* out, int32_t* n_accepted, int32_t* path,
+                    void* stream) {
+  Device* dev;
+  if (int rc = device(&dev)) return rc;
+  if (B < 0 || T < 0 || V < 1) return fail(KS_ERR_INVALID, "verify_draft: bad sizes B=%lld T=%lld V=%lld", (long long)B, (long long)T, (long long)V);
+  if (B == 0) return KS_OK;
+  if (!p || !u || !noise || !out || !n_accepted || (T > 0 && (!tokens || !path)))
+    return fail(KS_ERR_INVALID, "verify_draft: null pointer");
+  if (q && parents) return fail(KS_ERR_INVALID, "verify_draft: q and parents exclude each other");
+  if (token_dtype != KS_INT32 && token_dtype != KS_INT64) return fail(KS_ERR_INVALID, "verify_draft: token_dtype");
+  if (T > VD_MAX_T) return fail(KS_ERR_UNSUPPORTED, "verify_draft: T=%lld > %d", (long long)T, VD_MAX_T);
+  if (V >= 0x7FFFFFFFll - 4096 || B > (1 << 24)) return fail(KS_ERR_UNSUPPORTED, "verify_draft: too large");
+  if (!aligned(p, 4) || !aligned(u, 4) || !aligned(noise, 4) || (q && !aligned(q, 4)) ||
+      !aligned(out, token_dtype == KS_INT64 ? 8 : 4) || (T > 0 && !aligned(tokens, token_dtype == KS_INT64 ? 8 : 4)) ||
+      !aligned(path, 4) || !aligned(n_accepted, 4) || (parents && !aligned(parents, 4)))
+    return fail(KS_ERR_ALIGNMENT, "verify_draft: pointers must be aligned to their elements");
+  // As many CTAs per sequence as keep the grid within four CTAs per SM, each with at
+  // least a few thousand entries of the row.
+  int cs = VD_MAX_CLUSTER;
+  while (cs > 1 && (B * cs > 4ll * dev->num_sms || V / cs < 2048)) cs >>= 1;
+  VerifyParams vp{};
+  vp.p = p; vp.q = q; vp.tokens = tokens;
+  vp.tok_i64 = token_dtype == KS_INT64;
+  vp.parents = parents; vp.u = u; vp.noise = noise;
+  vp.out = out; vp.n_acc = n_accepted; vp.path = path;
+  vp.B = B; vp.T = (int)T; vp.V = (int)V;
+  vp.vec4 = V % 4 == 0 && aligned(p, 16) && aligned(noise, 16) && (!q || aligned(q, 16));
+  vp.per = (int)round_up((V + cs - 1) / cs, 32);
+  vp.status = dev->status;
+  // the walk's arrays and, for fixed candidates, one bit per entry of the slice
+  const size_t smem = (size_t)T * 24 + 4 + (q ? 0 : (size_t)vp.per / 8) + 16;
+  if (smem > 160 * 1024) return fail(KS_ERR_UNSUPPORTED, "verify_draft: V=%lld too large", (long long)V);
+  const void* fn = reinterpret_cast<const void*>(verify_draft_kernel);
+  if (smem > 40 * 1024)
+    if (int rc = smem_optin(dev, fn, "cudaFuncSetAttribute(verify_draft)")) return rc;
+  if (cs > 8 && !dev->vd_wide) {  // once per device
+    cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(verify_draft cluster)");
+    dev->vd_wide = true;
+  }
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = (unsigned)cs;
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  cfg.gridDim = dim3((unsigned)(B * cs));
+  cfg.blockDim = dim3(VD_THREADS);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = static_cast<cudaStream_t>(stream);
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  cudaError_t e = cudaLaunchKernelEx(&cfg, verify_draft_kernel, vp);
+  if (e != cudaSuccess) return cuda_fail(e, "verify_draft_kernel launch");
+  return launch_check("verify_draft_kernel launch");
 }
 
 int ks_device_status(void* stream) {

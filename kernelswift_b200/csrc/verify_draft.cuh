@@ -1,0 +1,240 @@
+// Verification of drafted tokens against the target's probabilities, from given
+// random numbers.
+//
+// p [B, T + 1, V]: row 0 is the target's distribution after the last accepted token,
+// row i + 1 the one after drafted token i.  u [B, T + 1] in [0, 1) decides at each row,
+// noise [B, V] (exponential) samples the next token.
+//
+//  * Sampled chain (q [B, T, V], the draft's distributions): token i stands if
+//    u_i q_i(x_i) < p_i(x_i) and every token before it stands.  n of them stand; the
+//    next token is drawn from w = max(p_n - q_n, 0), or from p_T when all stand.
+//  * Fixed candidates (parents [B, T], -1 = the root; a tree, or a chain when null):
+//    the children of a row split [0, 1) into stretches of length p_row(token), in index
+//    order, and u_row falls into one child's (taken, the walk goes on there) or into
+//    none (the next token is drawn from p_row without the children's tokens).  A
+//    sibling that repeats an older one's token has no stretch.
+//
+// Drawing: argmax_x w(x) / noise(x), ties to the lowest x.  With exponential noise
+// this picks x with probability w(x) / sum w, needs no sum, and does not depend on
+// the order of the work: every operation is one correctly rounded fp32 operation per
+// entry, and the stretches are summed in fp64.  If w is zero everywhere, p's row takes
+// its place.
+//
+// One cluster of CTAs per sequence.  Every CTA walks the draft itself (a few dependent
+// loads), then takes its slice of the one vocabulary row that matters; the slices'
+// maxima meet through distributed shared memory.  Bound by reading that row of p, q and
+// the noise (8 or 12 bytes per entry), for few sequences by the chain of load latencies
+// (token -> probability -> row).
+#pragma once
+#include "ks_device.cuh"
+
+namespace ks {
+
+constexpr int VD_THREADS = 512;
+constexpr int VD_MAX_T = 1024;
+constexpr int VD_MAX_CLUSTER = 16;
+
+struct VerifyParams {
+  const float* p;       // [B, T + 1, V]
+  const float* q;       // [B, T, V] or null
+  const void* tokens;   // int32 / int64 [B, T]
+  int32_t tok_i64;
+  const int32_t* parents;  // [B, T] or null (chain)
+  const float* u;       // [B, T + 1]
+  const float* noise;   // [B, V]
+  void* out;            // [B, T + 1], type of tokens
+  int32_t* n_acc;       // [B]
+  int32_t* path;        // [B, T]
+  int64_t B;
+  int32_t T, V;
+  int32_t vec4;         // rows and pointers are 16-byte aligned
+  int32_t per;          // entries of a slice (a multiple of 32)
+  int* status;
+};
+
+struct VdBest {
+  float val;
+  int32_t idx;
+  int32_t any;  // some w > 0
+};
+
+__device__ __forceinline__ void vd_take(VdBest& a, float val, int32_t idx) {
+  if (val > a.val || (val == a.val && idx < a.idx)) {
+    a.val = val;
+    a.idx = idx;
+  }
+}
+
+__device__ __forceinline__ int64_t vd_token(const VerifyParams& p, int64_t i) {
+  return p.tok_i64 ? static_cast<const int64_t*>(p.tokens)[i]
+                   : (int64_t)static_cast<const int32_t*>(p.tokens)[i];
+}
+
+__global__ void __launch_bounds__(VD_THREADS) verify_draft_kernel(VerifyParams p) {
+  extern __shared__ uint32_t vd_smem[];
+  // px [T] double, tok [T], par [T], next [T + 1], path [T], then the slice's bitmap
+  double* px = reinterpret_cast<double*>(vd_smem);
+  int32_t* tok = reinterpret_cast<int32_t*>(px + p.T);
+  int32_t* par = tok + p.T;
+  int32_t* next = par + p.T;
+  int32_t* path = next + p.T + 1;
+  uint32_t* gone = reinterpret_cast<uint32_t*>(path + p.T);
+  __shared__ int s_n, s_end;
+  __shared__ VdBest s_warp[VD_THREADS / 32];
+  __shared__ VdBest s_cta[VD_MAX_CLUSTER];
+  uint32_t rank, nranks;
+  asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
+  asm("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(nranks));
+  const int64_t b = blockIdx.x / nranks;
+  const int T = p.T, V = p.V, tid = threadIdx.x, lane = tid & 31;
+  const float* pb = p.p + b * (T + 1) * (int64_t)V;
+  const float* ub = p.u + b * (T + 1);
+
+  // The cluster's CTAs have all started before one writes into another's memory: arrive
+  // here, wait there.
+  asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
+
+  // ------------------------------------------------------------------ the walk
+  if (tid == 0) {
+    s_n = T;
+    s_end = 0;
+  }
+  const int words = p.per >> 5;
+  if (!p.q)
+    for (int i = tid; i < words; i += VD_THREADS) gone[i] = 0;
+  for (int i = tid; i <= T; i += VD_THREADS) next[i] = -1;
+  __syncthreads();
+  for (int i = tid; i < T; i += VD_THREADS) {
+    const int64_t x = vd_token(p, b * T + i);
+    const int32_t pa = p.parents ? p.parents[b * T + i] : i - 1;
+    const bool in = x >= 0 && x < V && pa >= -1 && pa < i;
+    if (!in && rank == 0) report_bounds(p.status, (int)b, V);
+    tok[i] = in ? (int32_t)x : -1;
+    par[i] = in ? pa : -2;
+    const float pv = in ? pb[(int64_t)(pa + 1) * V + x] : 0.f;
+    if (p.q) {
+      const float qv = in ? p.q[(b * T + i) * (int64_t)V + x] : 0.f;
+      if (!(__fmul_rn(ub[i], qv) < pv)) atomicMin(&s_n, i);
+    } else {
+      px[i] = (double)pv;
+    }
+  }
+  __syncthreads();
+  if (p.q) {
+    if (tid == 0) s_end = s_n;
+    for (int i = tid; i < T; i += VD_THREADS) path[i] = i;
+  } else {
+    // a sibling that repeats an older one's token gives up its stretch
+    for (int i = tid; i < T; i += VD_THREADS)
+      for (int j = 0; j < i; ++j)
+        if (par[j] == par[i] && tok[j] == tok[i]) px[i] = 0.0;
+    __syncthreads();
+    for (int i = tid; i < T; i += VD_THREADS) {
+      const int32_t pa = par[i];
+      if (pa < -1) continue;
+      double at = 0.0;
+      for (int j = 0; j < i; ++j)
+        if (par[j] == pa) at += px[j];
+      const double uu = (double)ub[pa + 1];
+      if (at <= uu && uu < at + px[i]) next[pa + 1] = i;
+    }
+    __syncthreads();
+    if (tid == 0) {
+      int n = 0, row = 0;
+      while (n < T && next[row] >= 0) {  // ends: a child's index is above its parent's
+        path[n++] = next[row];
+        row = next[row] + 1;
+      }
+      s_n = n;
+      s_end = row;
+    }
+    __syncthreads();
+    const int lo = (int)rank * p.per;
+    for (int i = tid; i < T; i += VD_THREADS)
+      if (par[i] == s_end - 1 && tok[i] >= lo && tok[i] < lo + p.per)
+        atomicOr(&gone[(tok[i] - lo) >> 5], 1u << ((tok[i] - lo) & 31));
+  }
+  __syncthreads();
+  const int n = s_n, end = s_end;
+
+  // ------------------------------------------------------------------ the next token
+  const float* row = pb + (int64_t)end * V;
+  const float* qrow = p.q && n < T ? p.q + (b * T + n) * (int64_t)V : nullptr;
+  const float* e = p.noise + b * (int64_t)V;
+  const int lo = (int)rank * p.per, hi = min(V, lo + p.per);
+  VdBest best;
+  for (int pass = 0; pass < 2; ++pass) {  // the second only where w is zero everywhere
+    best = {-1.f, 0x7FFFFFFF, 0};
+    const bool cut = pass == 0;
+    auto one = [&](int x, float pv, float qv, float nv, bool out) {
+      float w = pv;
+      if (cut) {
+        if (qrow) w = fmaxf(__fsub_rn(pv, qv), 0.f);
+        if (out) w = 0.f;
+      }
+      best.any |= w > 0.f;
+      vd_take(best, __fdiv_rn(w, nv), x);
+    };
+    if (p.vec4) {
+#pragma unroll 2
+      for (int x = lo + tid * 4; x < hi; x += VD_THREADS * 4) {
+        const float4 pv = __ldg(reinterpret_cast<const float4*>(row + x));
+        const float4 nv = __ldg(reinterpret_cast<const float4*>(e + x));
+        float4 qv = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (qrow) qv = __ldg(reinterpret_cast<const float4*>(qrow + x));
+        uint32_t g = 0;
+        if (!p.q) g = gone[(x - lo) >> 5] >> ((x - lo) & 31);
+        one(x, pv.x, qv.x, nv.x, g & 1);
+        one(x + 1, pv.y, qv.y, nv.y, g & 2);
+        one(x + 2, pv.z, qv.z, nv.z, g & 4);
+        one(x + 3, pv.w, qv.w, nv.w, g & 8);
+      }
+    } else {
+#pragma unroll 4
+      for (int x = lo + tid; x < hi; x += VD_THREADS) {
+        const uint32_t g = p.q ? 0u : gone[(x - lo) >> 5] >> ((x - lo) & 31);
+        one(x, __ldg(row + x), qrow ? __ldg(qrow + x) : 0.f, __ldg(e + x), g & 1);
+      }
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      const float v = __shfl_xor_sync(0xFFFFFFFFu, best.val, o);
+      const int32_t i = __shfl_xor_sync(0xFFFFFFFFu, best.idx, o);
+      best.any |= __shfl_xor_sync(0xFFFFFFFFu, best.any, o);
+      vd_take(best, v, i);
+    }
+    if (lane == 0) s_warp[tid >> 5] = best;
+    if (pass == 0) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
+    __syncthreads();
+    if (tid < (int)nranks) {  // this CTA's best into slot `rank` of CTA `tid`
+      for (int i = 0; i < VD_THREADS / 32; ++i) {
+        best.any |= s_warp[i].any;
+        vd_take(best, s_warp[i].val, s_warp[i].idx);
+      }
+      uint32_t at;
+      asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_u32(&s_cta[rank])), "r"(tid));
+      asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(at), "f"(best.val) : "memory");
+      asm volatile("st.shared::cluster.s32 [%0], %1;" ::"r"(at + 4), "r"(best.idx) : "memory");
+      asm volatile("st.shared::cluster.s32 [%0], %1;" ::"r"(at + 8), "r"(best.any) : "memory");
+    }
+    cluster_sync();
+    best = s_cta[0];
+    for (int i = 1; i < (int)nranks; ++i) {
+      best.any |= s_cta[i].any;
+      vd_take(best, s_cta[i].val, s_cta[i].idx);
+    }
+    if (best.any || pass == 1) break;
+    cluster_sync();  // every CTA has read the slots before they are written again
+  }
+  if (rank != 0) return;
+  const int32_t x = best.idx < V ? best.idx : 0;
+  for (int i = tid; i <= T; i += VD_THREADS) {
+    const int64_t v = i < n ? (int64_t)tok[path[i]] : i == n ? (int64_t)x : -1;
+    if (p.tok_i64) static_cast<int64_t*>(p.out)[b * (T + 1) + i] = v;
+    else static_cast<int32_t*>(p.out)[b * (T + 1) + i] = (int32_t)v;
+    if (i < T) p.path[b * T + i] = i < n ? path[i] : -1;
+  }
+  if (tid == 0) p.n_acc[b] = n;
+}
+
+}  // namespace ks

@@ -13,6 +13,12 @@ These are the B200 counterparts of the reference's torch extension ops
   on the tensor cores, the producer of ``indexer_topk``'s inputs.
 * ``quant_fp8_rows`` / ``indexer_topk_fp8`` / ``indexer_scores_fp8``: the FP8 indexer
   (``ModelArgs.dtype = "fp8"``), which the reference declares but does not implement.
+* ``cache_write`` / ``cache_read``: a paged latent cache in e4m3 with power-of-two row
+  scales, quantised as it is written and read back as bf16 rows.
+* ``tree_attn``: attention of drafted tokens (a tree or a chain; one token: a decoding
+  step) over that cache.
+* ``verify_draft``: drafted tokens accepted or rejected against the target's
+  probabilities, from given random numbers.  The reference has none of the four.
 
 Every op runs on the current CUDA stream of its input's device, validates its
 arguments like the reference (a ``RuntimeError`` on a bad dtype, device, shape
@@ -406,6 +412,203 @@ def topk_rows(scores: torch.Tensor, T: int, topk: int, ratio: int = 1, causal: b
                                  KS_INT64 if out_dtype == torch.int64 else KS_INT32,
                                  _stream(scores)), "ks_topk_rows")
     return out
+
+
+def _cache_args(name, kv8, kv_scale, kv_tail):
+    if kv8.dtype not in _FP8 or kv8.dim() != 3:
+        raise RuntimeError(f"{name}: kv8 must be float8_e4m3fn (or its uint8 bytes) [pages, page, dq]")
+    if kv_scale.dtype != torch.float32 or tuple(kv_scale.shape) != tuple(kv8.shape[:2]):
+        raise RuntimeError(f"{name}: kv_scale must be float32 [pages, page]")
+    pages, page, dq = kv8.shape
+    dr = 0
+    if kv_tail is not None:
+        if kv_tail.dtype != torch.bfloat16 or kv_tail.dim() != 3:
+            raise RuntimeError(f"{name}: kv_tail must be bfloat16 [pages, page, dr]")
+        if tuple(kv_tail.shape[:2]) != (pages, page):
+            raise RuntimeError(f"{name}: kv_tail shape mismatch")
+        dr = kv_tail.shape[2]
+    if pages < 1 or page < 1:
+        raise RuntimeError(f"{name}: the cache has no pages")
+    ts = [kv8, kv_scale] + ([kv_tail] if kv_tail is not None else [])
+    return pages, page, dq, dr, ts
+
+
+def _table_args(name, page_table, lens, B):
+    if page_table.dtype != torch.int32 or page_table.dim() != 2 or page_table.shape[0] != B:
+        raise RuntimeError(f"{name}: page_table must be int32 [b, max_pages]")
+    if lens.dtype != torch.int32 or tuple(lens.shape) != (B,):
+        raise RuntimeError(f"{name}: lens must be int32 [b]")
+
+
+def cache_write(kv: torch.Tensor, slots: torch.Tensor, kv8: torch.Tensor, kv_scale: torch.Tensor,
+                kv_tail: torch.Tensor | None = None) -> None:
+    """Quantise rows as they enter a paged latent cache (in place).
+
+    kv bf16 [..., D] (contiguous rows that are a constant number of elements apart, e.g.
+    a column slice of a wider projection), slots int32 / int64, one per row: row r goes
+    to ``slots[r]`` = page * page_size + offset; negative slots are skipped.  The first
+    dq = ``kv8.shape[-1]`` columns become e4m3 with one power-of-two scale per row (as
+    ``quant_fp8_rows``), the other dr columns stay bf16.  kv8 float8_e4m3fn [pages, page,
+    dq], kv_scale fp32 [pages, page], kv_tail bf16 [pages, page, dr] (None: dr = 0).  A
+    row that holds a NaN or an infinity reads back as NaN.  With dr = 0 and a page per
+    sequence, (kv8, kv_scale) are the keys ``indexer_topk_fp8`` takes."""
+    if kv.dtype != torch.bfloat16 or kv.dim() < 1:
+        raise RuntimeError("cache_write: kv must be bfloat16 [..., D]")
+    if slots.dtype not in (torch.int32, torch.int64):
+        raise RuntimeError("cache_write: slots must be int32 or int64")
+    pages, page, dq, dr, ts = _cache_args("cache_write", kv8, kv_scale, kv_tail)
+    if kv.shape[-1] != dq + dr:
+        raise RuntimeError(f"cache_write: kv rows have {kv.shape[-1]} columns, the cache {dq + dr}")
+    try:
+        rows = kv.view(-1, dq + dr)
+    except RuntimeError:
+        raise RuntimeError("cache_write: the rows of kv must be a constant stride apart") from None
+    R = rows.shape[0]
+    if slots.numel() != R:
+        raise RuntimeError(f"cache_write: {R} rows but {slots.numel()} slots")
+    _require_cuda("cache_write", slots, *ts)
+    if kv.device != kv8.device:
+        raise RuntimeError("cache_write: inputs must be on one device")
+    if R and rows.stride(1) != 1:
+        raise RuntimeError("cache_write: the columns of kv must be contiguous")
+    stride = rows.stride(0) if R > 1 else dq + dr
+    with torch.cuda.device(kv8.device):
+        check(lib().ks_cache_write(_ptr(rows), stride, _ptr(slots),
+                                   KS_INT64 if slots.dtype == torch.int64 else KS_INT32, R,
+                                   _ptr(kv8), _ptr(kv_scale), _ptr(kv_tail), pages * page, dq, dr,
+                                   _stream(kv8)), "ks_cache_write")
+
+
+def cache_read(kv8: torch.Tensor, kv_scale: torch.Tensor, kv_tail: torch.Tensor | None,
+               page_table: torch.Tensor, lens: torch.Tensor, n: int, start: int = 0,
+               out: torch.Tensor | None = None) -> torch.Tensor:
+    """Positions [start, start + n) of every sequence as bf16 rows [B, n, D], the ``kv``
+    that ``sparse_attn`` takes; zero rows from ``lens[b]`` on.  page_table int32
+    [B, max_pages], lens int32 [B].  The values are exact (e4m3 times a power of two)."""
+    pages, page, dq, dr, ts = _cache_args("cache_read", kv8, kv_scale, kv_tail)
+    B = page_table.shape[0] if page_table.dim() else 0
+    _table_args("cache_read", page_table, lens, B)
+    n, start = int(n), int(start)
+    if n < 0 or start < 0:
+        raise RuntimeError("cache_read: n and start must not be negative")
+    _require_cuda("cache_read", *ts, page_table, lens)
+    if out is None:
+        out = torch.empty((B, n, dq + dr), dtype=torch.bfloat16, device=kv8.device)
+    else:
+        _check_out("cache_read", out, (B, n, dq + dr), torch.bfloat16, kv8.device)
+    with torch.cuda.device(kv8.device):
+        check(lib().ks_cache_read(_ptr(kv8), _ptr(kv_scale), _ptr(kv_tail), pages, page, dq, dr,
+                                  _ptr(page_table), page_table.shape[1], _ptr(lens), B, n, start,
+                                  _ptr(out), _stream(kv8)), "ks_cache_read")
+    return out
+
+
+def tree_attn_workspace_size(B: int, T: int, H: int, dv: int) -> int:
+    return int(lib().ks_tree_attn_workspace_size(B, T, H, dv))
+
+
+def tree_attn(q: torch.Tensor, kv8: torch.Tensor, kv_scale: torch.Tensor,
+              kv_tail: torch.Tensor | None, page_table: torch.Tensor, lens: torch.Tensor,
+              softmax_scale: float, dv: int | None = None, mask: torch.Tensor | None = None,
+              attn_sink: torch.Tensor | None = None, out: torch.Tensor | None = None,
+              workspace: torch.Tensor | None = None) -> torch.Tensor:
+    """Attention of T drafted tokens per sequence over the quantised latent cache; T = 1
+    is a decoding step.
+
+    q bf16 [B,T,H,D]; the cache as ``cache_write`` fills it (D = dq + dr, dq a multiple
+    of 64, dr 0 or 64, D <= 576), page_table int32 [B, max_pages].  Every drafted token
+    sees the ``lens[b]`` cached positions; the drafted tokens' own rows follow at
+    positions lens[b] .. lens[b]+T-1 (already written), and token i sees row j of them
+    where ``mask[b, i, j]`` (bool [B,T,T]; None: j <= i, a chain).  attn_sink fp32 [H]
+    as in ``sparse_attn``.  Returns bf16 [B,T,H,dv], v = the first ``dv`` (default
+    min(D, 512)) columns of the cached rows; a token that sees nothing gets zeros."""
+    if q.dtype != torch.bfloat16 or q.dim() != 4:
+        raise RuntimeError("tree_attn: q must be bfloat16 [b, t, h, d]")
+    pages, page, dq, dr, ts = _cache_args("tree_attn", kv8, kv_scale, kv_tail)
+    B, T, H, D = q.shape
+    if D != dq + dr:
+        raise RuntimeError(f"tree_attn: q has {D} columns, the cache {dq + dr}")
+    _table_args("tree_attn", page_table, lens, B)
+    ts = [q] + ts + [page_table, lens]
+    if mask is not None:
+        if mask.dtype not in (torch.bool, torch.uint8) or tuple(mask.shape) != (B, T, T):
+            raise RuntimeError("tree_attn: mask must be bool [b, t, t]")
+        ts.append(mask)
+    if attn_sink is not None:
+        if attn_sink.dtype != torch.float32 or tuple(attn_sink.shape) != (H,):
+            raise RuntimeError("tree_attn: attn_sink must be float32 [h]")
+        ts.append(attn_sink)
+    _require_cuda("tree_attn", *ts)
+    dv = min(D, _DV_MAX) if dv is None else int(dv)
+    if out is None:
+        out = torch.empty((B, T, H, dv), dtype=torch.bfloat16, device=q.device)
+    else:
+        _check_out("tree_attn", out, (B, T, H, dv), torch.bfloat16, q.device)
+    need = tree_attn_workspace_size(B, T, H, dv)
+    if workspace is None:
+        workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
+    else:
+        _check_workspace("tree_attn", workspace, need, q.device)
+    with torch.cuda.device(q.device):
+        check(lib().ks_tree_attn(_ptr(q), _ptr(kv8), _ptr(kv_scale), _ptr(kv_tail), pages, page,
+                                 dq, dr, _ptr(page_table), page_table.shape[1], _ptr(lens),
+                                 _ptr(mask), _ptr(attn_sink), _ptr(out), B, T, H, dv,
+                                 float(softmax_scale), _ptr(workspace),
+                                 workspace.numel() * workspace.element_size(), _stream(q)),
+              "ks_tree_attn")
+    return out
+
+
+def verify_draft(p: torch.Tensor, tokens: torch.Tensor, u: torch.Tensor, noise: torch.Tensor,
+                 q: torch.Tensor | None = None, parents: torch.Tensor | None = None
+                 ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """Accept or reject T drafted tokens per sequence against the target's probabilities.
+
+    p fp32 [B,T+1,V]: row 0 is the target's distribution after the last accepted token,
+    row i+1 the one after drafted token i; tokens int32 / int64 [B,T]; u fp32 [B,T+1] in
+    [0, 1), one per row; noise fp32 [B,V], exponential (positive).
+
+    With ``q`` fp32 [B,T,V] the draft is a chain sampled from q: token i stands if
+    u[i] q[i, x_i] < p[i, x_i], and after the first that falls the next token is sampled
+    from max(p - q, 0).  Without q the draft is a tree of fixed candidates (``parents``
+    int32 [B,T], -1 = the root, parents[i] < i; None: a chain): u[r] falls into the
+    probability of one child of row r, or of none, and then the next token is sampled
+    from p[r] without its children's tokens.  Both give the target's distribution.
+
+    Returns (out [B,T+1] like tokens: the accepted tokens, the next token, then -1;
+    n_accepted int32 [B]; path int32 [B,T]: the accepted drafts' indices, then -1)."""
+    if tokens.dtype not in (torch.int32, torch.int64) or tokens.dim() != 2:
+        raise RuntimeError("verify_draft: tokens must be int32 or int64 [b, t]")
+    B, T = tokens.shape
+    if p.dtype != torch.float32 or p.dim() != 3 or tuple(p.shape[:2]) != (B, T + 1):
+        raise RuntimeError("verify_draft: p must be float32 [b, t + 1, v]")
+    V = p.shape[2]
+    if u.dtype != torch.float32 or tuple(u.shape) != (B, T + 1):
+        raise RuntimeError("verify_draft: u must be float32 [b, t + 1]")
+    if noise.dtype != torch.float32 or tuple(noise.shape) != (B, V):
+        raise RuntimeError("verify_draft: noise must be float32 [b, v]")
+    ts = [p, tokens, u, noise]
+    if q is not None:
+        if parents is not None:
+            raise RuntimeError("verify_draft: q (a sampled chain) and parents (fixed candidates) "
+                               "exclude each other")
+        if q.dtype != torch.float32 or tuple(q.shape) != (B, T, V):
+            raise RuntimeError("verify_draft: q must be float32 [b, t, v]")
+        ts.append(q)
+    if parents is not None:
+        if parents.dtype != torch.int32 or tuple(parents.shape) != (B, T):
+            raise RuntimeError("verify_draft: parents must be int32 [b, t]")
+        ts.append(parents)
+    _require_cuda("verify_draft", *ts)
+    out = torch.empty((B, T + 1), dtype=tokens.dtype, device=p.device)
+    n_accepted = torch.empty((B,), dtype=torch.int32, device=p.device)
+    path = torch.empty((B, T), dtype=torch.int32, device=p.device)
+    with torch.cuda.device(p.device):
+        check(lib().ks_verify_draft(_ptr(p), _ptr(q), _ptr(tokens),
+                                    KS_INT64 if tokens.dtype == torch.int64 else KS_INT32,
+                                    _ptr(parents), _ptr(u), _ptr(noise), B, T, V, _ptr(out),
+                                    _ptr(n_accepted), _ptr(path), _stream(p)), "ks_verify_draft")
+    return out, n_accepted, path
 
 
 def device_status(device: torch.device | int | None = None) -> None:

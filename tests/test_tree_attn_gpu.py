@@ -1,0 +1,297 @@
+"""tree_attn against the 64-bit restatement (oracle/cache_oracle.py).
+
+Tolerance, per element: the weights are rounded to bf16 before the product with v
+(relative 2^-9 each, so at most 2^-9 of A = sum w |v|) and the result is rounded to bf16
+(2^-9 of |out| <= A); what is left is fp32 (scores of size ~10 off by about 1e-5,
+sums of exponentials): 2^-12 of A covers it.  |got - exact| <= (2^-8 + 2^-12) A.
+"""
+import numpy as np
+import pytest
+import torch
+
+from helpers import bits_from_bf16
+from oracle import cache_oracle as C
+
+pytestmark = pytest.mark.gpu
+TOL = 2.0 ** -8 + 2.0 ** -12
+
+
+def build(B, T, H, dq, dr, page, lens, seed, spare=2, key_scale=None, q_scale=1.0):
+    """Queries and a filled paged cache; the slots no sequence reaches hold NaN."""
+    from kernelswift_b200 import ops
+
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    each = max(1, -(-(max(lens) + T) // page))
+    pages = B * each + spare
+    table = torch.randperm(pages, device="cuda", generator=g)[:B * each].view(B, each).int().contiguous()
+    kv8 = torch.full((pages, page, dq), 0x7F, dtype=torch.uint8, device="cuda").view(torch.float8_e4m3fn)
+    scale = torch.full((pages, page), float("nan"), device="cuda")
+    tail = torch.full((pages, page, dr), float("nan"), dtype=torch.bfloat16, device="cuda") if dr else None
+    for b in range(B):
+        n = lens[b] + T
+        kv = torch.randn(n, dq + dr, device="cuda", generator=g)
+        if key_scale is not None:
+            kv *= key_scale(torch.arange(n, device="cuda").float())[:, None]
+        pos = torch.arange(n, device="cuda")
+        ops.cache_write(kv.bfloat16(), table[b].long()[pos // page] * page + pos % page, kv8, scale, tail)
+    q = (q_scale * torch.randn(B, T, H, dq + dr, device="cuda", generator=g)).bfloat16()
+    return g, q, kv8, scale, tail, table, torch.tensor(lens, dtype=torch.int32, device="cuda")
+
+
+def check(q, kv8, scale, tail, table, lens, sm, dv, mask=None, sink=None, got=None, rows=None):
+    """Compare every (or a sample of) drafted token's output; returns the output."""
+    from kernelswift_b200 import ops
+
+    if got is None:
+        got = ops.tree_attn(q, kv8, scale, tail, table, lens, sm, dv=dv, mask=mask, attn_sink=sink)
+        ops.device_status()
+    B, T, H, D = q.shape
+    codes = kv8.view(torch.uint8).cpu().numpy().reshape(-1, kv8.shape[-1])
+    s = scale.double().cpu().numpy().reshape(-1)
+    t = tail.double().cpu().numpy().reshape(-1, tail.shape[-1]) if tail is not None else None
+    snk = sink.double().cpu().numpy() if sink is not None else None
+    qn, gn = q.double().cpu().numpy(), got.double().cpu().numpy()
+    assert got.shape == (B, T, H, dv) and got.dtype == torch.bfloat16
+    for b in range(B):
+        n = int(lens[b])
+        r = C.sequence_rows(codes, s, t, (table[b].cpu().numpy(), kv8.shape[1]), n + T)
+        for i in (range(T) if rows is None else rows):
+            seen = np.ones(n + T, bool)
+            seen[n:] = mask[b, i].cpu().numpy() if mask is not None else np.arange(T) <= i
+            ref, size = C.tree_attn_row(qn[b, i], r, seen, sm, snk, dv)
+            err = np.abs(gn[b, i] - ref)
+            assert (err <= TOL * size + 1e-37).all(), (b, i, float((err / np.maximum(size, 1e-30)).max()))
+    return got
+
+
+def tree_mask(g, B, T, p=0.5):
+    m = (torch.rand(B, T, T, device="cuda", generator=g) < p).tril()
+    return m | torch.eye(T, dtype=torch.bool, device="cuda")
+
+
+@pytest.mark.parametrize("B,T,H,dq,dr,dv,page,lens", [
+    (1, 1, 16, 128, 0, 128, 64, [0]),
+    (1, 1, 16, 128, 0, 128, 64, [1]),
+    (4, 1, 16, 512, 64, 512, 64, [127, 128, 126, 255]),
+    (3, 1, 128, 512, 64, 512, 64, [300, 0, 129]),
+    (2, 5, 20, 448, 64, 512, 48, [200, 77]),
+    (3, 13, 64, 448, 64, 448, 32, [60, 500, 1]),
+    (2, 33, 5, 192, 64, 192, 100, [1000, 3]),
+    (1, 64, 1, 64, 64, 64, 1, [90]),
+    (5, 2, 7, 256, 64, 320, 256, [1, 2, 3, 700, 5]),
+    (2, 3, 40, 64, 0, 64, 16, [130, 400]),
+    (1, 130, 3, 320, 0, 256, 7, [20]),
+    (2, 4, 32, 512, 0, 128, 64, [640, 641]),
+    (1, 2, 200, 128, 64, 192, 64, [333]),
+    (70, 1, 8, 128, 64, 128, 16, [3 * i for i in range(70)]),
+])
+@pytest.mark.parametrize("tree,sink", [(False, False), (True, True)])
+def test_shapes(cuda_ok, B, T, H, dq, dr, dv, page, lens, tree, sink):
+    g, *a = build(B, T, H, dq, dr, page, lens, seed=B * 100 + T * 10 + H)
+    mask = tree_mask(g, B, T) if tree else None
+    snk = torch.randn(H, device="cuda", generator=g) if sink else None
+    check(*a, (dq + dr) ** -0.5, dv, mask, snk, rows=None if T < 20 else [0, 1, T // 2, T - 1])
+
+
+@pytest.mark.parametrize("H,T,n", [(16, 1, 40000), (128, 1, 20000), (64, 8, 9001), (3, 2, 70001)])
+def test_long_context_is_split_and_joined(cuda_ok, H, T, n):
+    g, *a = build(1, T, H, 512, 64, 64, [n], seed=H)
+    check(*a, 576 ** -0.5, 512, rows=[0, T - 1])
+
+
+@pytest.mark.parametrize("tree", [False, True])
+def test_rows_of_many_sequences_at_once(cuda_ok, tree):
+    """More work items than CTAs, ragged, some sequences empty."""
+    lens = [(37 * i) % 900 if i % 5 else 0 for i in range(180)]
+    g, *a = build(180, 3, 32, 128, 64, 32, lens, seed=4)
+    check(*a, 0.07, 192, tree_mask(g, 180, 3) if tree else None)
+
+
+def test_running_maximum_grows_late(cuda_ok):
+    """Scores that grow by hundreds along the keys, shrink, and spike at single keys."""
+    for shape in (lambda x: 1 + x / 40, lambda x: torch.clamp(20 - x / 30, min=0.01),
+                  lambda x: torch.where(x % 131 == 130, 30.0, 0.1)):
+        g, *a = build(2, 3, 24, 512, 64, 64, [1500, 900], seed=9, key_scale=shape, q_scale=2.0)
+        check(*a, 576 ** -0.5, 512)
+
+
+def test_large_and_small_magnitudes(cuda_ok):
+    """Rows whose scales are far from 1, in both directions, in one sequence."""
+    g, *a = build(2, 2, 16, 448, 64, 64, [300, 200], seed=12, q_scale=2.0 ** -20,
+                  key_scale=lambda x: torch.exp2((x % 41) - 20))
+    check(*a, 1.0, 512)
+
+
+def test_masks_that_leave_nothing(cuda_ok):
+    """A token whose mask row is empty on an empty context gives zeros, with and without a
+    sink; its neighbours are untouched."""
+    from kernelswift_b200 import ops
+
+    for sink in (None, torch.randn(16, device="cuda")):
+        g, *a = build(3, 6, 16, 128, 64, 16, [0, 5, 0], seed=2)
+        mask = tree_mask(g, 3, 6)
+        mask[0, 2] = False
+        mask[1, 3] = False
+        mask[2] = False
+        got = check(*a, 0.1, 128, mask, sink)
+        assert (got[0, 2] == 0).all() and (got[2] == 0).all() and (got[1, 3] != 0).any()
+
+
+def test_nan_rows_reach_only_the_tokens_that_see_them(cuda_ok):
+    from kernelswift_b200 import ops
+
+    B, T, H = 2, 5, 16
+    g, q, kv8, scale, tail, table, lens = build(B, T, H, 128, 64, 32, [50, 70], seed=6)
+    mask = tree_mask(g, B, T)
+    mask[0, :, 2] = False
+    mask[0, 2, 2] = mask[0, 4, 2] = True
+    bad = torch.randn(1, 192, device="cuda").bfloat16()
+    bad[0, 150] = float("inf")
+    pos = 50 + 2
+    slot = table[0, pos // 32].long() * 32 + pos % 32
+    clean = ops.tree_attn(q, kv8, scale, tail, table, lens, 0.1, dv=192, mask=mask)
+    ops.cache_write(bad, slot.view(1), kv8, scale, tail)
+    got = ops.tree_attn(q, kv8, scale, tail, table, lens, 0.1, dv=192, mask=mask)
+    ops.device_status()
+    hit = torch.zeros(B, T, dtype=torch.bool, device="cuda")
+    hit[0, 2] = hit[0, 4] = True
+    assert got[hit].isnan().all()
+    assert torch.equal(got[~hit], clean[~hit])
+    # a marked row of the shared context reaches every token of its sequence, no other
+    ops.cache_write(bad, (table[1, 0].long() * 32 + 3).view(1), kv8, scale, tail)
+    got = ops.tree_attn(q, kv8, scale, tail, table, lens, 0.1, dv=192, mask=mask)
+    assert got[1].isnan().all() and torch.equal(got[0][~hit[0]], clean[0][~hit[0]])
+
+
+def test_infinite_queries_stay_in_their_rows(cuda_ok):
+    from kernelswift_b200 import ops
+
+    g, q, *rest = build(2, 3, 20, 128, 0, 32, [40, 300], seed=8)
+    clean = ops.tree_attn(q, *rest, 0.1)
+    q[0, 1, 3, 5] = float("inf")
+    q[1, 2, 19, 0] = float("nan")
+    got = ops.tree_attn(q, *rest, 0.1)
+    hit = torch.zeros(2, 3, 20, dtype=torch.bool, device="cuda")
+    hit[0, 1, 3] = hit[1, 2, 19] = True
+    assert got[hit].isnan().all() and torch.equal(got[~hit], clean[~hit])
+
+
+def test_one_token_equals_sparse_attention_over_the_same_rows(cuda_ok):
+    """T = 1 against ops.sparse_attn on the rows read back (its own rounding of the
+    weights: twice the tolerance apart)."""
+    from kernelswift_b200 import ops
+
+    g, q, kv8, scale, tail, table, lens = build(2, 1, 64, 512, 64, 64, [255, 255], seed=3)
+    sink = torch.randn(64, device="cuda", generator=g)
+    rows = ops.cache_read(kv8, scale, tail, table, lens + 1, 256)
+    idx = torch.arange(256, device="cuda").int().expand(2, 1, 256).contiguous()
+    a = ops.tree_attn(q, kv8, scale, tail, table, lens, 576 ** -0.5, dv=512, attn_sink=sink)
+    b = ops.sparse_attn(q, rows, sink, idx, 576 ** -0.5, dv=512)
+    size = ops.sparse_attn(q, rows.abs(), sink, idx, 0.0, dv=512).float().amax()
+    assert (a.float() - b.float()).abs().max() <= 2 * TOL * 3 * size
+
+
+def test_bad_pages_are_skipped_and_reported(cuda_ok):
+    from kernelswift_b200 import ops
+
+    g, q, kv8, scale, tail, table, lens = build(2, 2, 16, 128, 64, 32, [90, 90], seed=5)
+    good = ops.tree_attn(q, kv8, scale, tail, table, lens, 0.1, dv=128)
+    broken = table.clone()
+    broken[1, 1] = kv8.shape[0]
+    got = ops.tree_attn(q, kv8, scale, tail, broken, lens, 0.1, dv=128)
+    with pytest.raises(RuntimeError, match="device status"):
+        ops.device_status()
+    assert torch.equal(got[0], good[0]) and torch.isfinite(got[1].float()).all()
+    lens[0] = 10 ** 6  # longer than the table: the positions past it are skipped
+    got = ops.tree_attn(q, kv8, scale, tail, table, lens, 0.1, dv=128)
+    with pytest.raises(RuntimeError, match="device status"):
+        ops.device_status()
+    assert torch.equal(got[1], good[1])
+    ops.device_status()
+
+
+def test_repeats_streams_workspace_and_out(cuda_ok):
+    from kernelswift_b200 import ops
+
+    g, *a = build(3, 4, 48, 512, 64, 64, [5000, 100, 2500], seed=7)
+    ref = ops.tree_attn(*a, 0.05, dv=512)
+    need = ops.tree_attn_workspace_size(3, 4, 48, 512)
+    ws = torch.full((need,), 0xFF, dtype=torch.uint8, device="cuda")
+    out = torch.empty_like(ref)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(5):
+            out.fill_(7)
+            assert ops.tree_attn(*a, 0.05, dv=512, out=out, workspace=ws) is out
+    side.synchronize()
+    assert np.array_equal(bits_from_bf16(out), bits_from_bf16(ref))
+    empty = a[0][:, :0].contiguous()
+    assert ops.tree_attn(empty, *a[1:], 0.05, dv=512).shape == (3, 0, 48, 512)
+
+
+def test_captured_in_a_graph(cuda_ok):
+    """The lengths are read on the device: one captured call serves growing contexts."""
+    from kernelswift_b200 import ops
+
+    g, q, kv8, scale, tail, table, lens = build(2, 1, 16, 512, 64, 64, [700, 650], seed=10)
+    lens0 = lens.clone()
+    out = torch.empty(2, 1, 16, 512, dtype=torch.bfloat16, device="cuda")
+    ws = torch.empty(ops.tree_attn_workspace_size(2, 1, 16, 512), dtype=torch.uint8, device="cuda")
+    call = lambda: ops.tree_attn(q, kv8, scale, tail, table, lens, 0.04, dv=512, out=out, workspace=ws)  # noqa: E731
+    call()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        call()
+    for n in (700, 3, 128):
+        lens.copy_(torch.tensor([n, 650], dtype=torch.int32))
+        graph.replay()
+        torch.cuda.synchronize()
+        check(q, kv8, scale, tail, table, lens, 0.04, 512, got=out)
+    lens.copy_(lens0)
+
+
+def test_offsets_past_32_bits(cuda_ok):
+    from kernelswift_b200 import ops
+
+    pages, page = 70000, 64
+    kv8 = torch.zeros(pages, page, 512, dtype=torch.uint8, device="cuda").view(torch.float8_e4m3fn)
+    scale, tail = torch.ones(pages, page, device="cuda"), torch.zeros(pages, page, 64, dtype=torch.bfloat16, device="cuda")
+    g, q, k8, sc, tl, table, lens = build(1, 2, 16, 512, 64, 64, [300], seed=13)
+    ref = ops.tree_attn(q, k8, sc, tl, table, lens, 0.04, dv=512)
+    shift = pages - k8.shape[0]
+    kv8.view(torch.uint8)[shift:], scale[shift:], tail[shift:] = k8.view(torch.uint8), sc, tl
+    got = ops.tree_attn(q, kv8, scale, tail, table + shift, lens, 0.04, dv=512)
+    ops.device_status()
+    assert torch.equal(got, ref)
+
+
+def test_refusals(cuda_ok):
+    from kernelswift_b200 import ops
+
+    g, q, kv8, scale, tail, table, lens = build(2, 2, 16, 128, 64, 32, [20, 20], seed=5)
+    f = lambda *a, **k: (lambda: ops.tree_attn(*a, **k))  # noqa: E731
+    mask = torch.ones(2, 2, 2, dtype=torch.bool, device="cuda")
+    z = lambda *s: torch.zeros(*s, dtype=torch.uint8, device="cuda")  # noqa: E731
+    zq = lambda d: torch.zeros(2, 2, 16, d, dtype=torch.bfloat16, device="cuda")  # noqa: E731
+    for call, why in [
+        (f(q.half(), kv8, scale, tail, table, lens, 0.1), "bfloat16"),
+        (f(q[..., :128].contiguous(), kv8, scale, tail, table, lens, 0.1), "128 columns"),
+        (f(q, kv8, scale, tail, table[:1], lens, 0.1), "page_table"),
+        (f(q, kv8, scale, tail, table, lens.long(), 0.1), "lens"),
+        (f(q, kv8, scale, tail, table, lens, 0.1, dv=100), "dv=100"),
+        (f(q, kv8, scale, tail, table, lens, 0.1, dv=256), "dv=256"),
+        (f(q, kv8, scale, tail, table, lens, 0.1, mask=mask[:1]), "mask"),
+        (f(q, kv8, scale, tail, table, lens, 0.1, mask=mask.float()), "mask"),
+        (f(q, kv8, scale, tail, table, lens, 0.1, attn_sink=torch.zeros(15, device="cuda")), "attn_sink"),
+        (f(q, kv8, scale, tail, table, lens, 0.1, workspace=z(16)), "bytes needed"),
+        (f(q, kv8, scale, tail, table, lens, 0.1, out=torch.empty(2, 2, 16, 64, dtype=torch.bfloat16, device="cuda")), "shape"),
+        (f(q.cpu(), kv8, scale, tail, table, lens, 0.1), "CUDA"),
+        (f(q.transpose(1, 2), kv8, scale, tail, table, lens, 0.1), "contiguous|columns|lens|page"),
+        (f(zq(96), z(2, 4, 96), torch.ones(2, 4, device="cuda"), None, table, lens, 0.1, dv=64), "dq=96"),
+        (f(zq(640), z(2, 4, 640), torch.ones(2, 4, device="cuda"), None, table, lens, 0.1, dv=64), "dq=640"),
+    ]:
+        with pytest.raises(RuntimeError, match=why):
+            call()
+    ops.device_status()
