@@ -276,7 +276,7 @@ size_t ks_tree_attn_workspace_size(int64_t B, int64_t T, int64_t H, int64_t dv);
  * A row stored with scale NaN makes every token that sees it NaN, and no other.
  * Key positions whose page is outside the table or the pool are skipped and reported by
  * ks_device_status.  kv_scale must hold powers of two (or NaN), as ks_cache_write writes.
- * Requirements: dq % 64 == 0, dr 0 or 64, D <= 576, dv % 64 == 0, dv <= min(D, 512),
+ * Requirements: dq % 64 == 0, dq <= 512, dr 0 or 64, dv % 64 == 0, dv <= min(D, 512),
  * H <= 1024, q, out, kv8, kv_tail 16-byte aligned, workspace 256-byte aligned and at
  * least ks_tree_attn_workspace_size bytes.  No counterpart in the reference, whose
  * attention (baseline/sparse_attention.py:5-42) reads contiguous bf16 rows.

@@ -593,6 +593,27 @@ int table_check(const char* op, const int32_t* table, int64_t max_pages, const i
   return KS_OK;
 }
 
+// Rows of a row tile for a sequence's T * H query rows.
+int ta_rows(int64_t rows) { return rows <= 16 ? 16 : rows <= 32 ? 32 : 64; }
+
+template <int NR, int NQ>
+int launch_tree_attn(Device* dev, const CUtensorMap& qm, const TreeAttnParams& p, unsigned grid, size_t smem,
+                     cudaStream_t st) {
+  if (int rc = smem_optin(dev, reinterpret_cast<const void*>(tree_attn_kernel<NR, NQ>), "cudaFuncSetAttribute(tree_attn)"))
+    return rc;
+  tree_attn_kernel<NR, NQ><<<grid, TA_THREADS, smem, st>>>(qm, p);
+  if (int rc = launch_check("tree_attn_kernel launch")) return rc;
+  tree_attn_join_kernel<NR><<<dim3(grid, NR), TA_JOIN_THREADS, 0, st>>>(p);
+  return launch_check("tree_attn_join_kernel launch");
+}
+template <int NR>
+int launch_tree_attn(Device* dev, const CUtensorMap& qm, const TreeAttnParams& p, unsigned grid, size_t smem,
+                     cudaStream_t st) {
+  if (p.nq <= 2) return launch_tree_attn<NR, 2>(dev, qm, p, grid, smem, st);
+  if (p.nq <= 4) return launch_tree_attn<NR, 4>(dev, qm, p, grid, smem, st);
+  return launch_tree_attn<NR, 8>(dev, qm, p, grid, smem, st);
+}
+
 }  // namespace
 }  // namespace ks
 
@@ -946,8 +967,10 @@ int ks_cache_read(const void* kv8, const float* kv_scale, const void* kv_tail, i
 }
 
 size_t ks_tree_attn_workspace_size(int64_t B, int64_t T, int64_t H, int64_t dv) {
-  (void)B; (void)T; (void)H; (void)dv;
-  return 256;
+  if (B < 1 || T < 1 || H < 1 || dv < 1) return 256;
+  // two parts of a row tile per CTA: output, maximum and sum; and the CTA's owner record
+  const int64_t nr = ta_rows(T * H);
+  return (size_t)round_up(TA_MAX_CTAS * (2 * nr * (dv + 2) * 4 + 16), 256);
 }
 
 int ks_tree_attn(const void* q, const void* kv8, const float* kv_scale, const void* kv_tail,
@@ -963,12 +986,12 @@ int ks_tree_attn(const void* q, const void* kv8, const float* kv_scale, const vo
   if (int rc = cache_check("tree_attn", kv8, kv_scale, kv_tail, dq, dr)) return rc;
   if (int rc = table_check("tree_attn", page_table, max_pages, lens, n_pages, page, B)) return rc;
   if (!q || !out) return fail(KS_ERR_INVALID, "tree_attn: null pointer");
-  if (dq % 64 || (dr != 0 && dr != 64) || dq + dr > 576)
-    return fail(KS_ERR_UNSUPPORTED, "tree_attn: dq=%d dr=%d (dq a multiple of 64, dr 0 or 64, dq + dr <= 576)", dq, dr);
+  if (dq % 64 || dq > 512 || (dr != 0 && dr != 64))
+    return fail(KS_ERR_UNSUPPORTED, "tree_attn: dq=%d dr=%d (dq a multiple of 64 up to 512, dr 0 or 64)", dq, dr);
   if (dv < 64 || dv % 64 || dv > 512 || dv > dq + dr)
     return fail(KS_ERR_UNSUPPORTED, "tree_attn: dv=%lld (a multiple of 64, <= min(D, 512))", (long long)dv);
   if (H > 1024) return fail(KS_ERR_UNSUPPORTED, "tree_attn: H=%lld > 1024", (long long)H);
-  if (B * T * H >= (1ll << 31) || T > (1 << 20)) return fail(KS_ERR_UNSUPPORTED, "tree_attn: too many rows");
+  if (B * T * H >= (1ll << 31) || T > (1 << 20) || n_pages * page >= (1ll << 31)) return fail(KS_ERR_UNSUPPORTED, "tree_attn: too many rows");
   if (!aligned(q, 16) || !aligned(out, 16) || (attn_sink && !aligned(attn_sink, 4)))
     return fail(KS_ERR_ALIGNMENT, "tree_attn: q, out must be 16-byte aligned");
   const size_t need = ks_tree_attn_workspace_size(B, T, H, dv);
@@ -976,7 +999,6 @@ int ks_tree_attn(const void* q, const void* kv8, const float* kv_scale, const vo
     return fail(KS_ERR_WORKSPACE, "tree_attn: workspace of %zu bytes needed", need);
   if (!aligned(workspace, 256)) return fail(KS_ERR_ALIGNMENT, "tree_attn: workspace must be 256-byte aligned");
   TreeAttnParams p{};
-  p.q = static_cast<const uint16_t*>(q);
   p.kv8 = static_cast<const uint8_t*>(kv8);
   p.scale = kv_scale;
   p.tail = static_cast<const uint16_t*>(kv_tail);
@@ -988,11 +1010,45 @@ int ks_tree_attn(const void* q, const void* kv8, const float* kv_scale, const vo
   p.sink = attn_sink;
   p.out = static_cast<uint16_t*>(out);
   p.B = (int)B; p.T = (int)T; p.H = (int)H; p.dv = (int)dv;
+  p.rows = (int)(T * H);
+  const int nr = ta_rows(T * H);
+  p.row_tiles = (p.rows + nr - 1) / nr;
+  p.nq = dq / 64;
+  p.nkb = p.nq + dr / 64;
+  p.dv_tiles = (int)((dv + 127) / 128);
+  p.nka = std::max(p.nkb, 2 * p.dv_tiles);
+  // Two K tiles where they fit (D <= 256): the next tile's scores are computed while this
+  // one's softmax runs.  One otherwise; with D = 576 and 64 rows P then takes the place
+  // of the last chunk, which only the scores read.
+  const size_t tile = (size_t)p.nka * 16384, q_bytes = (size_t)p.nkb * nr * 128, limit = 232448 - 1024 - TA_HDR;
+  p.stages = 2 * (tile + 16384) + q_bytes <= limit ? 2 : 1;
+  p.p_alias = p.stages == 1 && tile + q_bytes + 16384 > limit;
+  if (p.p_alias && (p.nkb <= 2 * p.dv_tiles || tile + q_bytes > limit))
+    return fail(KS_ERR_UNSUPPORTED, "tree_attn: shared memory too small");
+  p.k_off = TA_HDR;
+  p.q_off = (uint32_t)(p.k_off + p.stages * tile);
+  p.p_off = p.p_alias ? (uint32_t)(p.k_off + (p.nkb - 1) * 16384) : (uint32_t)(p.q_off + q_bytes);
+  const size_t smem = 1024 + p.q_off + q_bytes + (p.p_alias ? 0 : (size_t)p.stages * 16384);
+  p.tmem_cols = 32;
+  while ((int)p.tmem_cols < (p.stages + p.dv_tiles) * nr) p.tmem_cols <<= 1;
   p.scale_log2 = softmax_scale * 1.4426950408889634f;
   p.status = dev->status;
-  const unsigned grid = (unsigned)(B * T * ((H + TA_HEADS - 1) / TA_HEADS));
-  tree_attn_simple_kernel<<<grid, TA_WARPS * 32, 0, static_cast<cudaStream_t>(stream)>>>(p);
-  return launch_check("tree_attn_simple_kernel launch");
+  p.budget_ns = wait_budget_ns();
+  // no more CTAs than there can be units (the lengths are known on the device only)
+  const int64_t most = B * p.row_tiles * std::max<int64_t>(1, (max_pages * page + 127) / 128);
+  const unsigned grid = (unsigned)std::min<int64_t>(most, std::min(dev->num_sms, TA_MAX_CTAS));
+  p.part_o = static_cast<float*>(workspace);
+  p.part_ml = p.part_o + 2ll * grid * nr * dv;
+  p.owner = reinterpret_cast<int32_t*>(p.part_ml + 4ll * grid * nr);
+  CUtensorMap qm;
+  if (int rc = make_map_bf16(&qm, q, (uint64_t)(dq + dr), (uint64_t)(B * p.rows), (uint64_t)(dq + dr) * 2, 64, (uint32_t)nr))
+    return rc;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  switch (nr) {
+    case 16: return launch_tree_attn<16>(dev, qm, p, grid, smem, st);
+    case 32: return launch_tree_attn<32>(dev, qm, p, grid, smem, st);
+    default: return launch_tree_attn<64>(dev, qm, p, grid, smem, st);
+  }
 }
 
 int ks_verify_draft(const float* p, const float* q, const void* tokens, int32_t token_dtype,
