@@ -20,15 +20,24 @@
 // balance.  A row tile that spans CTAs leaves (maximum, sum, unnormalised output) per
 // part in the workspace; tree_attn_join_kernel adds them up in order (no atomics).
 //
-// Warps: 8 softmax warps (thread = key = TMEM lane; two warps share a lane quarter and
-// split the rows), 8 loader warps, 1 MMA / query-TMA warp.  Two threads load a key: its
-// codes for the next tile wait in registers while this tile's are expanded, so the memory
-// latency passes behind a whole tile's work.  A 64-column chunk (16 KB) of the tile is
-// refilled as soon as the last product that reads it is done.
+// Warps: 4 softmax warps (thread = key = TMEM lane), 8 loader warps, one MMA / query-TMA
+// warp and one address warp: 14, so that four share a scheduler and a thread may hold 128
+// registers (with 18 warps, 96: the loaders spilled, and a spill waits for its load).  The
+// address warp walks the page table ahead of the loads (slot, scale factor and state of
+// each key, in shared memory).  A loader warp owns 16 keys: its codes of the next tile wait
+// in registers, so the memory latency passes behind a whole tile's work, and a pair of
+// 64-column chunks is refilled as soon as the last product that reads it is done.  No load
+// is in flight while a tile is converted: the proxy fence that hands a chunk to the tensor
+// cores waits for all of its thread's loads.  The bf16 tail goes from global to shared
+// memory directly (cp.async).
 //
-// Softmax: the running maximum of a row is only raised when a score passes it by 2^8
-// (one vote per tile); p = 2^(s - m) is then at most 256, fp32 sums are kept per thread
-// and reduced once per row tile.
+// Softmax: p = 2^(s - m) with a reference m that need not be the running maximum: p, its
+// sum and the output are floating point, so only overflow limits how far s may pass m.
+// A tile is worked on in one pass with the m it finds; if a score passed it by more than
+// TA_GROW (base 2), m is raised, and sum and output scaled, after the tile's product; only
+// a score that passes it by TA_MOST raises it before, and the tile is done again.  A row
+// tile's first tile finds its maxima first.  Sums are kept per thread in fp32 and reduced
+// once per row tile.
 #pragma once
 #include "latent_cache.cuh"
 #include "sparse_attn.cuh"
@@ -36,14 +45,16 @@
 
 namespace ks {
 
-constexpr int TA_SOFT = 256;                 // softmax threads (warps 0-7)
-constexpr int TA_LOAD = 256;                 // loader threads (warps 8-15)
-constexpr int TA_THREADS = TA_SOFT + TA_LOAD + 32;
+constexpr int TA_SOFT = 128;                 // softmax threads (warps 0-3)
+constexpr int TA_LOAD = 256;                 // loader threads (warps 4-11)
+constexpr int TA_W_LOAD = 4, TA_W_MMA = 12, TA_W_ADDR = 13;
+constexpr int TA_THREADS = TA_SOFT + TA_LOAD + 64;
 constexpr int TA_MAX_CHUNKS = 9;             // 64-column chunks of a row
 constexpr int TA_MAX_CTAS = 148;             // SMs of a B200: bounds the workspace
 constexpr int TA_MAX_ROWS = 64;
-constexpr int TA_HDR = 4096;
-constexpr float TA_GROW = 8.f;               // log2 of how far scores may pass the maximum
+constexpr int TA_HDR = 8192;
+constexpr int TA_AHEAD = 4;                  // tiles whose addresses are held
+constexpr float TA_GROW = 8.f, TA_MOST = 24.f;  // how far a score may pass m (base 2)
 
 struct TreeAttnParams {
   const uint8_t* kv8;
@@ -74,21 +85,26 @@ struct TreeAttnParams {
 };
 
 struct TaShared {
-  uint64_t full[2][TA_MAX_CHUNKS];  // a chunk has been written
+  uint64_t full[2][5];              // a pair of chunks (4: the tail) has been written
   uint64_t vfree[2][4];             // the PV products of a 128-dim tile are done
   uint64_t s_full[2];               // scores of a tile are in TMEM (and its K reads done)
   uint64_t p_full[2];               // P of a tile is in shared memory
   uint64_t pv_done[2];              // all PV products of a tile are done
+  uint64_t a_full[TA_AHEAD], a_free[TA_AHEAD];  // a tile's addresses are in place / used
   uint64_t q_full, drain;
   uint32_t tmem_base;
   int abort;
   int64_t total, per;
   int32_t b0, rt0, t0;              // where this CTA's stretch starts
-  alignas(16) float m[TA_MAX_ROWS]; // running maximum per row (base 2)
+  alignas(16) float m[TA_MAX_ROWS];     // reference of each row (base 2)
   alignas(16) float mneg[TA_MAX_ROWS];  // its negative (read as float4)
   float f[TA_MAX_ROWS];             // factor of a raise; at the end 1 / sum
   float red[4][TA_MAX_ROWS];
-  uint8_t flag[2][128];             // key: 0 fine, 1 absent, 2 marked (scale NaN)
+  int32_t slot[TA_AHEAD][128];      // row of the page pool, -1: nothing to load
+  uint32_t mul[TA_AHEAD][128];      // 2^120 * scale as two bf16 factors (low half, high half)
+  // key: 0 fine, 1 absent, 2 marked (scale NaN); read by the softmax, which is up to two
+  // tiles behind the loaders that free the addresses
+  uint8_t flag[2 * TA_AHEAD][128];
 };
 static_assert(sizeof(TaShared) <= TA_HDR, "TaShared exceeds its header");
 
@@ -143,14 +159,39 @@ __device__ __forceinline__ int ta_slot(const TreeAttnParams& p, const TaWalk& w,
   return (int)cache_row(p.table, p.max_pages, p.n_pages, p.page, w.b, pos, p.status);
 }
 
-// Two e4m3 codes (bytes of w picked by SEL) as bf16, times the powers of two in `mul`.
-// A code's exponent and mantissa moved to their places in bf16 give its value times
-// 2^-120 (bf16's bias is 120 more than e4m3's; subnormals included), so the one exact
-// product with 2^120 * scale is the value.
+// Two e4m3 codes (bytes 0, 1 of w with SEL = 0x9180, bytes 2, 3 with 0xB3A2) as bf16,
+// times the powers of two in `mul`.  A code s eeee mmm is placed in its 16-bit lane sign
+// extended, moved up by 4 and masked: s 0000 eeee mmm 0000, its value times 2^-120 (bf16's
+// bias is 120 more than e4m3's; subnormals included).  The one exact product with 2^120 *
+// scale is the value.
 template <uint32_t SEL>
 __device__ __forceinline__ uint32_t ta_expand(uint32_t w, uint32_t mul) {
-  const uint32_t t = __byte_perm(w, 0, SEL);
-  return mul_bf16x2((t & 0x80008000u) | ((t >> 4) & 0x07F007F0u), mul);
+  uint32_t t;
+  asm("prmt.b32 %0, %1, %1, %2;" : "=r"(t) : "r"(w), "n"(SEL));
+  return mul_bf16x2((t * 16u) & 0x87F087F0u, mul);
+}
+
+// ldcg_or_zero at a constant offset: one address for a whole row.
+template <int OFF>
+__device__ __forceinline__ uint4 ta_ld(const void* base, bool pred) {
+  uint4 v;
+  asm volatile(
+      "{ .reg .pred p; setp.ne.b32 p, %5, 0;"
+      " mov.b32 %0, 0; mov.b32 %1, 0; mov.b32 %2, 0; mov.b32 %3, 0;"
+      " @p ld.global.cg.v4.u32 {%0, %1, %2, %3}, [%4 + %6]; }"
+      : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+      : "l"(base), "r"((int)pred), "n"(OFF));
+  return v;
+}
+// Chunks C .. NQ - 1 of two rows.
+template <int C, int NQ>
+__device__ __forceinline__ void ta_load_rows(uint4 (&r)[NQ][2], const uint8_t* c0, const uint8_t* c1, bool ok0,
+                                             bool ok1, int nq) {
+  if constexpr (C < NQ) {
+    r[C][0] = ta_ld<C * 64>(c0, ok0 && C < nq);
+    r[C][1] = ta_ld<C * 64>(c1, ok1 && C < nq);
+    ta_load_rows<C + 1, NQ>(r, c0, c1, ok0, ok1, nq);
+  }
 }
 
 __device__ __forceinline__ void tmem_ld8(uint32_t taddr, uint32_t* r) {
@@ -196,7 +237,7 @@ __device__ __forceinline__ void ta_reduce(const float (&v)[CW], float* red, int 
 template <int NR, int NQ>
 __global__ void __launch_bounds__(TA_THREADS, 1)
     tree_attn_kernel(const __grid_constant__ CUtensorMap qm, const TreeAttnParams p) {
-  constexpr int CW = NR / 2;  // rows of a softmax thread
+  constexpr int CB = NR < 32 ? NR : 32;  // rows that a softmax thread works on at a time
   extern __shared__ uint8_t ta_raw[];
   const uint32_t raw = smem_u32(ta_raw);
   uint8_t* smem = ta_raw + (((raw + 1023u) & ~1023u) - raw);
@@ -209,11 +250,15 @@ __global__ void __launch_bounds__(TA_THREADS, 1)
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < 2; ++s) {
-      for (int c = 0; c < TA_MAX_CHUNKS; ++c) mbar_init(&sh->full[s][c], TA_LOAD / 32);
+      for (int c = 0; c < 5; ++c) mbar_init(&sh->full[s][c], TA_LOAD / 32);
       for (int m = 0; m < 4; ++m) mbar_init(&sh->vfree[s][m], 1);
       mbar_init(&sh->s_full[s], 1);
       mbar_init(&sh->p_full[s], TA_SOFT / 32);
       mbar_init(&sh->pv_done[s], 1);
+    }
+    for (int s = 0; s < TA_AHEAD; ++s) {
+      mbar_init(&sh->a_full[s], 1);
+      mbar_init(&sh->a_free[s], TA_LOAD / 32);
     }
     mbar_init(&sh->q_full, 1);
     mbar_init(&sh->drain, 1);
@@ -225,12 +270,12 @@ __global__ void __launch_bounds__(TA_THREADS, 1)
     sh->m[threadIdx.x] = -INFINITY;
     sh->mneg[threadIdx.x] = INFINITY;
   }
-  if (warp == 16) {
+  if (warp == TA_W_MMA) {
     tmem_alloc<1>(&sh->tmem_base, p.tmem_cols);
     tmem_relinquish<1>();
     if (lane == 0) tma_prefetch_desc(&qm);
   }
-  if (warp == 8) {  // the call's units, and where this CTA's stretch starts
+  if (warp == TA_W_ADDR) {  // the call's units, and where this CTA's stretch starts
     int64_t total = 0;
     for (int i = 0; i < p.B; i += 32) {
       int64_t n = 0;
@@ -281,102 +326,135 @@ __global__ void __launch_bounds__(TA_THREADS, 1)
   TaWalk w;
   w.start(p, sh);
 
-  if (warp >= 8 && warp < 16) {
+  if (warp >= TA_W_LOAD && warp < TA_W_MMA) {
     // ================================================================ loaders
-    const int lt = threadIdx.x - TA_SOFT, key = lt >> 1, half = lt & 1;
-    // r[c]: the codes of chunk c.  The bf16 tail (two chunks' worth of registers) borrows
-    // r[0] and r[1] between their use in this unit and their load for the next.
-    static_assert(NQ >= 2, "the tail borrows two chunks' registers");
+    // lane: 16 codes (part) of keys key0, key0 + 8 in each chunk; a warp's load covers
+    // 64-byte stretches of 8 rows
+    const int lw = warp - TA_W_LOAD, part = lane & 3, key0 = lw * 16 + (lane >> 2);
+    const uint32_t sw = (uint32_t)(key0 & 7), units = (uint32_t)max(w.left, 0);
+    const uint32_t at0 = (uint32_t)key0 * 128 + (((uint32_t)(part * 2) ^ sw) << 4);
+    const uint32_t at1 = (uint32_t)key0 * 128 + (((uint32_t)(part * 2 + 1) ^ sw) << 4);
     uint4 r[NQ][2];
-    const int last_free = 2 * p.dv_tiles;  // chunks from here on are read by QK only
-    TaWalk a = w;                          // the walk of the row addresses: one unit ahead
-    int slot = ta_slot(p, a, key), next;
-    auto load8 = [&](int c, int s) {
-      const uint8_t* g = p.kv8 + (int64_t)s * p.dq + c * 64 + half * 32;
-      r[c][0] = ldcg_or_zero(g, s >= 0 && c < p.nq);
-      r[c][1] = ldcg_or_zero(g + 16, s >= 0 && c < p.nq);
+    auto load = [&](uint32_t g) {
+      const int s0 = sh->slot[g % TA_AHEAD][key0], s1 = sh->slot[g % TA_AHEAD][key0 + 8];
+      const uint8_t* c0 = p.kv8 + (int64_t)s0 * p.dq + part * 16;
+      const uint8_t* c1 = p.kv8 + (int64_t)s1 * p.dq + part * 16;
+      ta_load_rows<0, NQ>(r, c0, c1, s0 >= 0, s1 >= 0, p.nq);
     };
-    auto load_scale = [&](int s) { return __float_as_uint(s >= 0 ? __ldg(p.scale + s) : 0.f); };
+    bool ok = units > 0;
+    if (ok) {
+      ok = mbar_wait_inl(&sh->a_full[0], 0, wc);
+      load(0);
+    }
+    // The tail is early where only the scores read it; it waits for the second product
+    // where that reads it too, or P takes its place (p_alias).
+    const bool tail_pv = p.nq < 2 * p.dv_tiles, tail_early = p.dr > 0 && !tail_pv && !p.p_alias;
+    for (uint32_t g = 0; g < units && ok; ++g) {
+      const int st = two ? (int)(g & 1) : 0, ad = (int)(g % TA_AHEAD);
+      const uint32_t use = two ? g >> 1 : g, last = (use - 1) & 1;
+      uint8_t* tile = ks_ + (size_t)st * p.nka * 16384;
+      const uint32_t ma = sh->mul[ad][key0], mb = sh->mul[ad][key0 + 8];
+      const uint32_t m1[2] = {(ma & 0xFFFFu) * 0x10001u, (mb & 0xFFFFu) * 0x10001u};
+      const bool big = __any_sync(0xFFFFFFFFu, (ma >> 16) != 0x3F80u || (mb >> 16) != 0x3F80u);
+      auto tail = [&] {
+        if (use > 0)
+          ok = mbar_wait_inl(tail_pv     ? &sh->vfree[st][p.nq >> 1]
+                             : p.p_alias ? &sh->pv_done[st]
+                                         : &sh->s_full[st], last, wc) && ok;
 #pragma unroll
-    for (int c = 0; c < NQ; ++c) load8(c, slot);
-    uint32_t sb = load_scale(slot);
-    a.next_unit(p);
-    next = ta_slot(p, a, key);
-    const uint32_t row = (uint32_t)(key * 128), sw = (uint32_t)(key & 7);
+        for (int j = 0; j < 4; ++j) {
+          const int key = lw * 16 + j * 4 + (lane >> 3), piece = lane & 7;
+          const int s = sh->slot[ad][key];
+          cp_async16(tile + p.nq * 16384 + key * 128 + ((piece ^ (key & 7)) << 4),
+                     p.tail + (int64_t)max(s, 0) * p.dr + piece * 8, s >= 0 ? 16u : 0u);
+        }
+      };
+      if (tail_early) tail();
+#pragma unroll
+      for (int m = 0; m < NQ / 2; ++m) {
+        if (2 * m < p.nq) {
+          const bool end = 2 * m + 2 >= p.nq;
+          if (use > 0)
+            ok = mbar_wait_inl(m < p.dv_tiles ? &sh->vfree[st][m] : &sh->s_full[st], last, wc) && ok;
+          if (end && p.dr > 0 && !tail_early) tail();
+#pragma unroll
+          for (int c = 2 * m; c < 2 * m + 2; ++c) {
+            if (c >= p.nq) continue;
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              const uint4 v = r[c][j];
+              uint4 lo, hi;
+              lo.x = ta_expand<0x9180>(v.x, m1[j]);
+              lo.y = ta_expand<0xB3A2>(v.x, m1[j]);
+              lo.z = ta_expand<0x9180>(v.y, m1[j]);
+              lo.w = ta_expand<0xB3A2>(v.y, m1[j]);
+              hi.x = ta_expand<0x9180>(v.z, m1[j]);
+              hi.y = ta_expand<0xB3A2>(v.z, m1[j]);
+              hi.z = ta_expand<0x9180>(v.w, m1[j]);
+              hi.w = ta_expand<0xB3A2>(v.w, m1[j]);
+              if (big) {  // a scale beyond 2^7
+                const uint32_t m2 = ((j ? mb : ma) >> 16) * 0x10001u;
+                lo.x = mul_bf16x2(lo.x, m2);
+                lo.y = mul_bf16x2(lo.y, m2);
+                lo.z = mul_bf16x2(lo.z, m2);
+                lo.w = mul_bf16x2(lo.w, m2);
+                hi.x = mul_bf16x2(hi.x, m2);
+                hi.y = mul_bf16x2(hi.y, m2);
+                hi.z = mul_bf16x2(hi.z, m2);
+                hi.w = mul_bf16x2(hi.w, m2);
+              }
+              *reinterpret_cast<uint4*>(tile + c * 16384 + j * 1024 + at0) = lo;
+              *reinterpret_cast<uint4*>(tile + c * 16384 + j * 1024 + at1) = hi;
+            }
+          }
+          if (p.dr > 0 && (tail_early ? m == 0 : end)) cp_async_wait_all();
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) {
+            mbar_arrive(&sh->full[st][m]);
+            if (p.dr > 0 && (tail_early ? m == 0 : end)) mbar_arrive(&sh->full[st][4]);
+            if (end) mbar_arrive(&sh->a_free[ad]);
+          }
+        }
+      }
+      if (g + 1 < units) {
+        ok = mbar_wait_inl(&sh->a_full[(g + 1) % TA_AHEAD], ((g + 1) / TA_AHEAD) & 1, wc) && ok;
+        load(g + 1);
+      }
+    }
+  } else if (warp == TA_W_ADDR) {
+    // ================================================================ addresses
     const uint32_t units = (uint32_t)max(w.left, 0);
     bool ok = true;
-    for (uint32_t g = 0; g < units && ok; ++g) {
-      const int st = two ? (int)(g & 1) : 0;
-      const uint32_t use = two ? g >> 1 : g;
-      uint8_t* tile = ks_ + (size_t)st * p.nka * 16384 + row;
-      const bool bad = (sb & 0x7F800000u) == 0x7F800000u;
-      // 2^120 * scale, or two factors where that is beyond bf16
-      const int e = (int)((sb >> 23) & 255) + 120;
-      const bool fine = slot >= 0 && !bad && (sb & 0x7F800000u) != 0;
-      const uint32_t m1 = fine ? (uint32_t)min(e, 254) * 0x00800080u : 0u;
-      const bool big = __any_sync(0xFFFFFFFFu, fine && e > 254);
-      const uint32_t m2 = (uint32_t)(max(e, 254) - 254 + 127) * 0x00800080u;
-      sb = load_scale(next);
-      auto wait_free = [&](int cc) {  // the last products that read this chunk slot are done
-        if (use > 0) {
-          uint64_t* bar = cc < last_free ? &sh->vfree[st][cc >> 1] : p.p_alias ? &sh->pv_done[st] : &sh->s_full[st];
-          ok = mbar_wait_inl(bar, (use - 1) & 1, wc) && ok;
-        }
-      };
-      auto filled = [&](int cc) {
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&sh->full[st][cc]);
-      };
+    for (uint32_t g = 0; g < units && ok; ++g, w.next_unit(p)) {
+      int s[4];
+      uint32_t sb[4];
 #pragma unroll
-      for (int c = 0; c < NQ; ++c) {
-        if (c < p.nq) {
-          wait_free(c);
-          if (c == 0 && half == 0) sh->flag[st][key] = slot < 0 ? 1 : bad ? 2 : 0;
-          uint8_t* dst = tile + c * 16384;
+      for (int i = 0; i < 4; ++i) s[i] = ta_slot(p, w, i * 32 + lane);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const uint4 v = r[c][i >> 1];
-            const uint32_t wa = i & 1 ? v.z : v.x, wb = i & 1 ? v.w : v.y;
-            uint4 o;
-            o.x = ta_expand<0x1404>(wa, m1);
-            o.y = ta_expand<0x3424>(wa, m1);
-            o.z = ta_expand<0x1404>(wb, m1);
-            o.w = ta_expand<0x3424>(wb, m1);
-            if (big) {
-              o.x = mul_bf16x2(o.x, m2);
-              o.y = mul_bf16x2(o.y, m2);
-              o.z = mul_bf16x2(o.z, m2);
-              o.w = mul_bf16x2(o.w, m2);
-            }
-            *reinterpret_cast<uint4*>(dst + (((uint32_t)(half * 4 + i) ^ sw) << 4)) = o;
-          }
-          filled(c);
-        }
-        // the next unit's codes take this chunk's registers
-        if (c >= 2) {
-          load8(c, next);
-        } else if (c == 1) {
-          const uint16_t* tg = p.tail + (int64_t)slot * p.dr + half * 32;
-#pragma unroll
-          for (int i = 0; i < 4; ++i) r[i >> 1][i & 1] = ldcg_or_zero(tg + i * 8, slot >= 0 && p.dr > 0 && !bad);
-        }
+      for (int i = 0; i < 4; ++i) {
+        sb[i] = s[i] >= 0 ? __float_as_uint(__ldg(p.scale + s[i])) : 0u;
+        if (s[i] >= 0 && p.dr > 0)  // the tail is fetched when its place is free: have it near
+          asm volatile("prefetch.global.L2 [%0];" ::"l"(p.tail + (int64_t)s[i] * p.dr));
       }
-      if (p.dr > 0) {
-        wait_free(p.nq);
-        uint8_t* dst = tile + p.nq * 16384;
+      const int ad = (int)(g % TA_AHEAD);
+      if (g >= TA_AHEAD) ok = mbar_wait_inl(&sh->a_free[ad], (g / TA_AHEAD - 1) & 1, wc);
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          *reinterpret_cast<uint4*>(dst + (((uint32_t)(half * 4 + i) ^ sw) << 4)) = r[i >> 1][i & 1];
-        filled(p.nq);
+      for (int i = 0; i < 4; ++i) {
+        const int key = i * 32 + lane;
+        const bool bad = (sb[i] & 0x7F800000u) == 0x7F800000u;
+        // 2^120 * scale, in two factors where that is beyond bf16 (0 for a scale of 0)
+        const int e = (int)((sb[i] >> 23) & 255) + 120;
+        const uint32_t m1 = (sb[i] & 0x7F800000u) && !bad ? (uint32_t)min(e, 254) << 7 : 0u;
+        const uint32_t m2 = bad ? 127u : (uint32_t)(max(e, 254) - 254 + 127);
+        sh->flag[g % (2 * TA_AHEAD)][key] = s[i] < 0 ? 1 : bad ? 2 : 0;
+        sh->slot[ad][key] = bad ? -1 : s[i];
+        sh->mul[ad][key] = m1 | (m2 << 23);
       }
-      load8(0, next);
-      load8(1, next);
-      slot = next;
-      a.next_unit(p);
-      next = ta_slot(p, a, key);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sh->a_full[ad]);
     }
-  } else if (warp == 16) {
+  } else if (warp == TA_W_MMA) {
     // ================================================================ MMA issue
     if (elect_one()) {
       const uint32_t id_qk = idesc_bf16_f32(128, NR, false, false), id_pv = idesc_bf16_f32(128, NR, true, true);
@@ -388,15 +466,20 @@ __global__ void __launch_bounds__(TA_THREADS, 1)
         const int y = x.b * p.rows + x.rt * NR;
         for (int c = 0; c < p.nkb; ++c) tma_load_2d(&qm, &sh->q_full, qs + c * NR * 128, c * 64, y);
       };
+      // descriptors: only the start address (low word, 16-byte units) changes
+      const uint64_t k_desc = sdesc_sw128(smem_u32(ks_), 16, 1024), q_desc = sdesc_sw128(smem_u32(qs), 16, 1024);
+      const uint64_t v_desc = sdesc_sw128(smem_u32(ks_), 16384, 1024), p_desc = sdesc_sw128(smem_u32(ps), 16, 1024);
+      const uint32_t stage16 = (uint32_t)p.nka * 1024;
       auto qk = [&](uint32_t g) {
         const int st = two ? (int)(g & 1) : 0;
         const uint32_t use = two ? g >> 1 : g;
-        for (int c = 0; c < p.nkb && ok; ++c) {
-          ok = mbar_wait_inl(&sh->full[st][c], use & 1, wc);
-          if (!ok) return;
-          tc_fence_after();
-          const uint64_t ad = sdesc_sw128(smem_u32(ks_ + ((size_t)st * p.nka + c) * 16384), 16, 1024);
-          const uint64_t bd = sdesc_sw128(smem_u32(qs + c * NR * 128), 16, 1024);
+        for (int c = 0; c < p.nkb; ++c) {
+          if (c == p.nq || !(c & 1)) {
+            ok = mbar_wait_inl(&sh->full[st][c == p.nq ? 4 : c >> 1], use & 1, wc);
+            if (!ok) return;
+            tc_fence_after();
+          }
+          const uint64_t ad = k_desc + st * stage16 + c * 1024, bd = q_desc + c * (NR * 8);
 #pragma unroll
           for (int k = 0; k < 4; ++k)
             umma_bf16_ss(tmem + st * NR, ad + k * 2, bd + k * 2, id_qk, c > 0 || k > 0 ? 1u : 0u);
@@ -409,9 +492,9 @@ __global__ void __launch_bounds__(TA_THREADS, 1)
         ok = mbar_wait_inl(&sh->p_full[st], use & 1, wc);
         if (!ok) return;
         tc_fence_after();
-        const uint64_t bd = sdesc_sw128(smem_u32(ps + st * 16384), 16, 1024);
+        const uint64_t bd = p_desc + st * 1024;
         for (int m = 0; m < p.dv_tiles; ++m) {
-          const uint64_t ad = sdesc_sw128(smem_u32(ks_ + ((size_t)st * p.nka + 2 * m) * 16384), 16384, 1024);
+          const uint64_t ad = v_desc + st * stage16 + m * 2048;
 #pragma unroll
           for (int k = 0; k < 8; ++k)  // 16 keys: 2048 bytes further in both
             umma_bf16_ss(tmem + o_col + m * NR, ad + k * 128, bd + k * 128, id_pv, !first || k > 0 ? 1u : 0u);
@@ -458,34 +541,33 @@ __global__ void __launch_bounds__(TA_THREADS, 1)
     // ================================================================ softmax, epilogue
     // After a wait ran out (abort) the loops run on without waiting, so the warps keep
     // meeting at their barriers; nothing here indexes by data.
-    const int quarter = warp & 3, hc = (warp >> 2) * CW;  // first row of this thread
-    const int key = quarter * 32 + lane;
-    const uint32_t lane_off = (uint32_t)(quarter * 32) << 16;
+    const int key = warp * 32 + lane;
+    const uint32_t lane_off = (uint32_t)(warp * 32) << 16;
     uint32_t g = 0;
     while (w.left > 0) {
       const int n = w.here();
       const int r0 = w.rt * NR;                      // first row of the tile in the sequence
       const int nrows = min(NR, p.rows - r0);
       const bool whole = w.t == 0 && n == w.nt;      // no other CTA has a part
-      float l[CW];
+      float l[NR];
 #pragma unroll
-      for (int i = 0; i < CW; ++i) l[i] = 0.f;
+      for (int i = 0; i < NR; ++i) l[i] = 0.f;
       for (int i = 0; i < n; ++i, ++g) {
         const int st = two ? (int)(g & 1) : 0;
         const uint32_t use = two ? g >> 1 : g;
         const int tile = w.t + i;
-        // what this key's column entries may be: ~0 everything, else a bit per row
-        uint32_t allow = 0xFFFFFFFFu;
+        // which rows see this key: all, or a bit per row
+        uint64_t allow = ~0ull;
         const int pos = tile * 128 + key, j = pos - w.len;
         if (j >= 0) {  // a drafted row, or past them (absent)
           allow = 0;
           if (j < p.T) {
-            int t = (r0 + hc) / p.H, h = (r0 + hc) - t * p.H;
+            int t = r0 / p.H, h = r0 - t * p.H;
             const uint8_t* mk = p.mask + ((int64_t)w.b * p.T) * p.T + j;
-            uint32_t bit = 0;
+            uint64_t bit = 0;
             bool fresh = true;
 #pragma unroll 1
-            for (int c = 0; c < CW; ++c) {
+            for (int c = 0; c < NR; ++c) {
               if (fresh) bit = t < p.T && (p.mask ? mk[(int64_t)t * p.T] != 0 : j <= t);
               allow |= bit << c;
               fresh = ++h == p.H;
@@ -496,102 +578,134 @@ __global__ void __launch_bounds__(TA_THREADS, 1)
             }
           }
         }
-        mbar_wait(&sh->full[st][0], use & 1, wc);  // the key's flag
-        const int flag = sh->flag[st][key];
+        mbar_wait_inl(&sh->full[st][0], use & 1, wc);  // the key's flag
+        const int flag = sh->flag[g % (2 * TA_AHEAD)][key];
         if (flag == 1) allow = 0;
-        mbar_wait(&sh->s_full[st], use & 1, wc);
+        mbar_wait_inl(&sh->s_full[st], use & 1, wc);
         tc_fence_after();
-        constexpr uint32_t ALL = CW == 32 ? 0xFFFFFFFFu : (1u << CW) - 1u;
+        constexpr uint64_t ALL = NR == 64 ? ~0ull : (1ull << NR) - 1;
         const bool plain = __all_sync(0xFFFFFFFFu, (allow & ALL) == ALL && flag == 0);
-        // exponents: scaled score minus the row's maximum
-        float d[CW];
-        auto exponents = [&] {
-          uint32_t s[CW];
-          tmem_ldn<CW>(tmem + st * NR + hc + lane_off, s);
+        // rows c0 .. c0 + CB - 1: scaled scores minus their references (raw: themselves)
+        auto exponents = [&](int c0, float (&d)[CB], bool raw) {
+          tmem_ldn<CB>(tmem + st * NR + c0 + lane_off, reinterpret_cast<uint32_t*>(d));
           tmem_wait_ld();
 #pragma unroll
-          for (int c = 0; c < CW; c += 4) {
-            const float4 mn = *reinterpret_cast<const float4*>(&sh->mneg[hc + c]);
-            d[c] = fmaf(__uint_as_float(s[c]), p.scale_log2, mn.x);
-            d[c + 1] = fmaf(__uint_as_float(s[c + 1]), p.scale_log2, mn.y);
-            d[c + 2] = fmaf(__uint_as_float(s[c + 2]), p.scale_log2, mn.z);
-            d[c + 3] = fmaf(__uint_as_float(s[c + 3]), p.scale_log2, mn.w);
+          for (int c = 0; c < CB; c += 4) {
+            const float4 mn = raw ? make_float4(0.f, 0.f, 0.f, 0.f) : *reinterpret_cast<const float4*>(&sh->mneg[c0 + c]);
+            d[c] = fmaf(d[c], p.scale_log2, mn.x);
+            d[c + 1] = fmaf(d[c + 1], p.scale_log2, mn.y);
+            d[c + 2] = fmaf(d[c + 2], p.scale_log2, mn.z);
+            d[c + 3] = fmaf(d[c + 3], p.scale_log2, mn.w);
           }
           if (!plain) {
+            const uint32_t al = (uint32_t)(allow >> c0);
 #pragma unroll
-            for (int c = 0; c < CW; ++c)
-              d[c] = !((allow >> c) & 1u) ? -INFINITY : flag == 2 ? __uint_as_float(0x7FC00000u) : d[c];
+            for (int c = 0; c < CB; ++c)
+              d[c] = !((al >> c) & 1u) ? -INFINITY : flag == 2 ? __uint_as_float(0x7FC00000u) : d[c];
           }
         };
-        exponents();
-        // a score past the row's maximum by more than TA_GROW?
-        bool need = false;
+        uint8_t* pr = ps + st * 16384 + key * 128;
+        // P of this key, its sums where `add`; returns the largest exponent
+        auto weights = [&](auto add) {
+          float most = -INFINITY;
 #pragma unroll
-        for (int c = 0; c < CW; ++c) need |= d[c] > TA_GROW;
-        if (soft_any(need)) {
-          {
-            uint32_t s[CW];
-            tmem_ldn<CW>(tmem + st * NR + hc + lane_off, s);
-            tmem_wait_ld();
+          for (int c0 = 0; c0 < NR; c0 += CB) {
+            float d[CB];
+            exponents(c0, d, false);
 #pragma unroll
-            for (int c = 0; c < CW; ++c)
-              d[c] = plain || ((allow >> c) & 1u) ? __uint_as_float(s[c]) * p.scale_log2 : -INFINITY;
+            for (int c = 0; c < CB; c += 8) {
+              uint32_t o[4];
+#pragma unroll
+              for (int k = 0; k < 4; ++k) {
+                most = fmaxf(most, fmaxf(d[c + 2 * k], d[c + 2 * k + 1]));
+                const float e0 = ex2f(d[c + 2 * k]), e1 = ex2f(d[c + 2 * k + 1]);
+                add(c0 + c + 2 * k, e0);
+                add(c0 + c + 2 * k + 1, e1);
+                o[k] = cvt_bf16x2(e0, e1);
+              }
+              *reinterpret_cast<uint4*>(pr + ((((c0 + c) >> 3) ^ (key & 7)) << 4)) = make_uint4(o[0], o[1], o[2], o[3]);
+            }
           }
-          ta_reduce<true, CW>(d, &sh->red[quarter][hc], lane);
+          return most;
+        };
+        // The tile's maxima, and references raised to them where they pass by `limit`.
+        auto raise = [&](float limit) {
+#pragma unroll
+          for (int c0 = 0; c0 < NR; c0 += CB) {
+            float d[CB];
+            exponents(c0, d, true);
+            ta_reduce<true, CB>(d, &sh->red[warp][c0], lane);
+          }
           soft_sync();
           if (threadIdx.x < NR) {
             const int c = threadIdx.x;
             const float mo = sh->m[c];
             const float tm = fmaxf(fmaxf(sh->red[0][c], sh->red[1][c]), fmaxf(sh->red[2][c], sh->red[3][c]));
-            const float mn = tm > mo + TA_GROW || mo == -INFINITY ? tm : mo;
-            sh->f[c] = mn == mo || mo == -INFINITY ? 1.f : ex2f(mo - mn);
+            const float mn = tm > mo + limit || mo == -INFINITY ? tm : mo;
+            sh->f[c] = mn == mo ? 1.f : ex2f(mo - mn);
             sh->m[c] = mn;
             sh->mneg[c] = -mn;
           }
           soft_sync();
-          exponents();
+        };
+        // The output's columns by the factors of a raise, once every product up to tile x is in them.
+        auto scale_output = [&](uint32_t x) {
+          mbar_wait_inl(&sh->pv_done[two ? x & 1 : 0], (two ? x >> 1 : x) & 1, wc);
+          tc_fence_after();
+#pragma unroll 1
+          for (int m = 0; m < p.dv_tiles; ++m) {
+#pragma unroll 1
+            for (int c = 0; c < NR; c += 8) {
+              uint32_t o[8];
+              tmem_ld8(tmem + o_col + m * NR + c + lane_off, o);
+              tmem_wait_ld();
 #pragma unroll
-          for (int c = 0; c < CW; ++c) l[c] *= sh->f[hc + c];
-          if (i > 0) {  // raise the output's columns too, once the products before are in it
-            const uint32_t lg = g - 1;
-            mbar_wait(&sh->pv_done[two ? lg & 1 : 0], (two ? lg >> 1 : lg) & 1, wc);
-            tc_fence_after();
-            for (int m = 0; m < p.dv_tiles; ++m) {
-#pragma unroll
-              for (int c = 0; c < CW; c += 8) {
-                uint32_t o[8];
-                tmem_ld8(tmem + o_col + m * NR + hc + c + lane_off, o);
-                tmem_wait_ld();
-#pragma unroll
-                for (int k = 0; k < 8; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * sh->f[hc + c + k]);
-                tmem_st8(tmem + o_col + m * NR + hc + c + lane_off, o);
-              }
+              for (int k = 0; k < 8; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * sh->f[c + k]);
+              tmem_st8(tmem + o_col + m * NR + c + lane_off, o);
             }
-            tmem_wait_st();
+          }
+          tmem_wait_st();
+        };
+        auto publish = [&] {
+          fence_proxy_async_smem();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&sh->p_full[st]);
+        };
+        auto sums = [&](int c, float e) { l[c] += e; };
+        if (i == 0) {  // no reference yet
+          raise(0.f);
+          weights(sums);
+          publish();
+        } else {
+          const float most = weights(sums);
+          if (!soft_any(most > TA_GROW)) {
+            publish();
+          } else if (!soft_any(most > TA_MOST)) {
+            raise(TA_GROW);  // (reads the scores, so before the next ones may come)
+            publish();
+#pragma unroll
+            for (int c = 0; c < NR; ++c) l[c] *= sh->f[c];
+            scale_output(g);
+          } else {
+            // Take the weights out of the sums again (to 2^-24 of the weight that passes m,
+            // which becomes 1 at most; an infinite one leaves nothing worth keeping), raise m
+            // and repeat the tile.
+            auto undo = [&](int c, float e) { l[c] = l[c] == INFINITY ? 0.f : l[c] - e; };
+            weights(undo);
+            raise(TA_GROW);
+#pragma unroll
+            for (int c = 0; c < NR; ++c) l[c] *= sh->f[c];
+            weights(sums);
+            scale_output(g - 1);
+            publish();
           }
         }
-        uint8_t* pr = ps + st * 16384 + key * 128;
-#pragma unroll
-        for (int c = 0; c < CW; c += 8) {
-          uint32_t o[4];
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const float e0 = ex2f(d[c + 2 * k]), e1 = ex2f(d[c + 2 * k + 1]);
-            l[c + 2 * k] += e0;
-            l[c + 2 * k + 1] += e1;
-            o[k] = cvt_bf16x2(e0, e1);
-          }
-          *reinterpret_cast<uint4*>(pr + ((((hc + c) >> 3) ^ (key & 7)) << 4)) = make_uint4(o[0], o[1], o[2], o[3]);
-        }
-        fence_proxy_async_smem();
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&sh->p_full[st]);
       }
       // the row tile's part is complete
       {
         const uint32_t lg = g - 1;
-        ta_reduce<false, CW>(l, &sh->red[quarter][hc], lane);
+        ta_reduce<false, NR>(l, sh->red[warp], lane);
         soft_sync();
         // a part of a longer row tile: the head of it, or a later piece
         const int slot = 2 * (int)blockIdx.x + (w.t == 0 ? 1 : 0);
@@ -617,26 +731,29 @@ __global__ void __launch_bounds__(TA_THREADS, 1)
           ow[2] = 1 + (int)((w.nt - n + sh->per - 1) / sh->per);
         }
         soft_sync();
-        mbar_wait(&sh->pv_done[two ? lg & 1 : 0], (two ? lg >> 1 : lg) & 1, wc);
+        mbar_wait_inl(&sh->pv_done[two ? lg & 1 : 0], (two ? lg >> 1 : lg) & 1, wc);
         tc_fence_after();
         for (int m = 0; m < p.dv_tiles; ++m) {
-          uint32_t o[CW];
-          tmem_ldn<CW>(tmem + o_col + m * NR + hc + lane_off, o);
-          tmem_wait_ld();
-          const int dim = m * 128 + quarter * 32 + lane;
-          if (dim < p.dv) {
-            if (whole) {
-              uint16_t* op = p.out + ((int64_t)w.b * p.rows + r0 + hc) * p.dv + dim;
+          const int dim = m * 128 + key;
 #pragma unroll
-              for (int c = 0; c < CW; ++c)
-                if (hc + c < nrows)
-                  op[(int64_t)c * p.dv] =
-                      __bfloat16_as_ushort(__float2bfloat16_rn(__uint_as_float(o[c]) * sh->f[hc + c]));
-            } else {
-              float* op = p.part_o + ((int64_t)slot * NR + hc) * p.dv + dim;
+          for (int c0 = 0; c0 < NR; c0 += CB) {
+            uint32_t o[CB];
+            tmem_ldn<CB>(tmem + o_col + m * NR + c0 + lane_off, o);
+            tmem_wait_ld();
+            if (dim < p.dv) {
+              if (whole) {
+                uint16_t* op = p.out + ((int64_t)w.b * p.rows + r0 + c0) * p.dv + dim;
 #pragma unroll
-              for (int c = 0; c < CW; ++c)
-                if (hc + c < nrows) op[(int64_t)c * p.dv] = __uint_as_float(o[c]);
+                for (int c = 0; c < CB; ++c)
+                  if (c0 + c < nrows)
+                    op[(int64_t)c * p.dv] =
+                        __bfloat16_as_ushort(__float2bfloat16_rn(__uint_as_float(o[c]) * sh->f[c0 + c]));
+              } else {
+                float* op = p.part_o + ((int64_t)slot * NR + c0) * p.dv + dim;
+#pragma unroll
+                for (int c = 0; c < CB; ++c)
+                  if (c0 + c < nrows) op[(int64_t)c * p.dv] = __uint_as_float(o[c]);
+              }
             }
           }
         }
@@ -649,7 +766,7 @@ __global__ void __launch_bounds__(TA_THREADS, 1)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (warp == 16) tmem_dealloc<1>(tmem, p.tmem_cols);
+  if (warp == TA_W_MMA) tmem_dealloc<1>(tmem, p.tmem_cols);
 }
 
 // Adds up the parts of row tiles that span CTAs, in order: the tile whose head CTA x holds
