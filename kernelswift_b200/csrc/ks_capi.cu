@@ -593,25 +593,19 @@ int table_check(const char* op, const int32_t* table, int64_t max_pages, const i
   return KS_OK;
 }
 
-// Rows of a row tile for a sequence's T * H query rows.
-int ta_rows(int64_t rows) { return rows <= 16 ? 16 : rows <= 32 ? 32 : 64; }
+// Rows of a row tile for a sequence's T * H query rows: 32 fill the tensor memory; 16 rows
+// take fewer columns of every product where there are no more.
+int ta_rows(int64_t rows) { return rows <= 16 ? 16 : 32; }
 
-template <int NR, int NQ>
-int launch_tree_attn(Device* dev, const CUtensorMap& qm, const TreeAttnParams& p, unsigned grid, size_t smem,
-                     cudaStream_t st) {
-  if (int rc = smem_optin(dev, reinterpret_cast<const void*>(tree_attn_kernel<NR, NQ>), "cudaFuncSetAttribute(tree_attn)"))
+template <int NR>
+int launch_tree_attn(Device* dev, const CUtensorMap& km, const CUtensorMap& tm, const TreeAttnParams& p, unsigned grid,
+                     size_t smem, cudaStream_t st) {
+  if (int rc = smem_optin(dev, reinterpret_cast<const void*>(tree_attn_kernel<NR>), "cudaFuncSetAttribute(tree_attn)"))
     return rc;
-  tree_attn_kernel<NR, NQ><<<grid, TA_THREADS, smem, st>>>(qm, p);
+  tree_attn_kernel<NR><<<grid, TA_THREADS, smem, st>>>(km, tm, p);
   if (int rc = launch_check("tree_attn_kernel launch")) return rc;
   tree_attn_join_kernel<NR><<<dim3(grid, NR), TA_JOIN_THREADS, 0, st>>>(p);
   return launch_check("tree_attn_join_kernel launch");
-}
-template <int NR>
-int launch_tree_attn(Device* dev, const CUtensorMap& qm, const TreeAttnParams& p, unsigned grid, size_t smem,
-                     cudaStream_t st) {
-  if (p.nq <= 2) return launch_tree_attn<NR, 2>(dev, qm, p, grid, smem, st);
-  if (p.nq <= 4) return launch_tree_attn<NR, 4>(dev, qm, p, grid, smem, st);
-  return launch_tree_attn<NR, 8>(dev, qm, p, grid, smem, st);
 }
 
 }  // namespace
@@ -999,6 +993,7 @@ int ks_tree_attn(const void* q, const void* kv8, const float* kv_scale, const vo
     return fail(KS_ERR_WORKSPACE, "tree_attn: workspace of %zu bytes needed", need);
   if (!aligned(workspace, 256)) return fail(KS_ERR_ALIGNMENT, "tree_attn: workspace must be 256-byte aligned");
   TreeAttnParams p{};
+  p.q = static_cast<const uint16_t*>(q);
   p.kv8 = static_cast<const uint8_t*>(kv8);
   p.scale = kv_scale;
   p.tail = static_cast<const uint16_t*>(kv_tail);
@@ -1013,24 +1008,29 @@ int ks_tree_attn(const void* q, const void* kv8, const float* kv_scale, const vo
   p.rows = (int)(T * H);
   const int nr = ta_rows(T * H);
   p.row_tiles = (p.rows + nr - 1) / nr;
-  p.nq = dq / 64;
-  p.nkb = p.nq + dr / 64;
-  p.dv_tiles = (int)((dv + 127) / 128);
-  p.nka = std::max(p.nkb, 2 * p.dv_tiles);
-  // Two K tiles where they fit (D <= 256): the next tile's scores are computed while this
-  // one's softmax runs.  One otherwise; with D = 576 and 64 rows P then takes the place
-  // of the last chunk, which only the scores read.
-  const size_t tile = (size_t)p.nka * 16384, q_bytes = (size_t)p.nkb * nr * 128, limit = 232448 - 1024 - TA_HDR;
-  p.stages = 2 * (tile + 16384) + q_bytes <= limit ? 2 : 1;
-  p.p_alias = p.stages == 1 && tile + q_bytes + 16384 > limit;
-  if (p.p_alias && (p.nkb <= 2 * p.dv_tiles || tile + q_bytes > limit))
-    return fail(KS_ERR_UNSUPPORTED, "tree_attn: shared memory too small");
+  p.nc = (dq + 127) / 128;
+  p.dt = (int)((std::min<int64_t>(dv, dq) + 127) / 128);
+  p.vt = dv > dq;
+  // shared memory: as many code tiles as fit (two at D = 576)
+  p.stage_bytes = (uint32_t)(p.nc + (dr ? 1 : 0)) * 16384;
+  const size_t q_bytes = (size_t)p.nc * 2 * nr * 128 + (dr ? (size_t)nr * 128 : 0);
+  const size_t fixed = 1024 + TA_HDR + q_bytes + 16384 + (p.vt ? 8192 : 0);
+  p.stages = (int)std::min<size_t>((232448 - fixed) / p.stage_bytes, TA_STAGES);
+  if (p.stages < 1) return fail(KS_ERR_UNSUPPORTED, "tree_attn: shared memory too small");
   p.k_off = TA_HDR;
-  p.q_off = (uint32_t)(p.k_off + p.stages * tile);
-  p.p_off = p.p_alias ? (uint32_t)(p.k_off + (p.nkb - 1) * 16384) : (uint32_t)(p.q_off + q_bytes);
-  const size_t smem = 1024 + p.q_off + q_bytes + (p.p_alias ? 0 : (size_t)p.stages * 16384);
+  p.q_off = p.k_off + (uint32_t)p.stages * p.stage_bytes;
+  p.p_off = p.q_off + (uint32_t)q_bytes;
+  p.pb_off = p.p_off + 16384;
+  const size_t smem = fixed + (size_t)p.stages * p.stage_bytes;
+  const int o_cols = p.dt * TA_LEVELS * nr + (p.vt ? nr : 0);
+  p.s_bufs = o_cols + 2 * 3 * nr <= 512 ? 2 : 1;
   p.tmem_cols = 32;
-  while ((int)p.tmem_cols < (p.stages + p.dv_tiles) * nr) p.tmem_cols <<= 1;
+  while ((int)p.tmem_cols < o_cols + p.s_bufs * 3 * nr) p.tmem_cols <<= 1;
+  // TMA boxes: the power of two that divides the page and the tile, of 8 rows (a swizzle
+  // atom) or more
+  p.box = 128;
+  while (p.box > 1 && page % p.box) p.box >>= 1;
+  if (p.box < 8) p.box = 0;
   p.scale_log2 = softmax_scale * 1.4426950408889634f;
   p.status = dev->status;
   p.budget_ns = wait_budget_ns();
@@ -1040,15 +1040,16 @@ int ks_tree_attn(const void* q, const void* kv8, const float* kv_scale, const vo
   p.part_o = static_cast<float*>(workspace);
   p.part_ml = p.part_o + 2ll * grid * nr * dv;
   p.owner = reinterpret_cast<int32_t*>(p.part_ml + 4ll * grid * nr);
-  CUtensorMap qm;
-  if (int rc = make_map_bf16(&qm, q, (uint64_t)(dq + dr), (uint64_t)(B * p.rows), (uint64_t)(dq + dr) * 2, 64, (uint32_t)nr))
-    return rc;
-  cudaStream_t st = static_cast<cudaStream_t>(stream);
-  switch (nr) {
-    case 16: return launch_tree_attn<16>(dev, qm, p, grid, smem, st);
-    case 32: return launch_tree_attn<32>(dev, qm, p, grid, smem, st);
-    default: return launch_tree_attn<64>(dev, qm, p, grid, smem, st);
+  CUtensorMap km{}, tm{};
+  if (p.box) {
+    const uint64_t slots = (uint64_t)n_pages * (uint64_t)page;
+    if (int rc = make_map_u8(&km, kv8, (uint64_t)dq, slots, (uint64_t)dq, 128, (uint32_t)p.box)) return rc;
+    if (dr)
+      if (int rc = make_map_bf16(&tm, kv_tail, 64, slots, 128, 64, (uint32_t)p.box)) return rc;
   }
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (nr == 16) return launch_tree_attn<16>(dev, km, tm, p, grid, smem, st);
+  return launch_tree_attn<32>(dev, km, tm, p, grid, smem, st);
 }
 
 int ks_verify_draft(const float* p, const float* q, const void* tokens, int32_t token_dtype,

@@ -7,37 +7,46 @@
 // drafted rows that follow them in the cache, those its row of the mask allows (without
 // a mask: itself and the ones before it).
 //
-// The T * H query rows of a sequence share its cached rows, so the product is run with
-// keys as the MMA's M dimension (tcgen05, bf16 operands, fp32 accumulators in TMEM):
-//   S^T[128 keys, NR rows] = K . Q^T         O^T[dv, NR rows] += V^T . P^T
-// K and V are one tile in shared memory: the e4m3 codes are expanded to bf16 (exactly,
-// their scale included) once, stored 128-byte swizzled, and read K-major by the first
-// product and MN-major (dims contiguous) by the second.  NR = 16, 32 or 64 rows.
+// The T * H query rows of a sequence share its cached rows, so the products run with keys
+// as the MMA's M dimension:
+//   S^T[128 keys, rows] = K . Q^T         O^T[dims, rows] += V^T . P^T
+// and on the cache's own e4m3 codes (tcgen05 kind::f8f6f4): a code tile is loaded once, by
+// TMA where the pages allow, and read K-major by the first product and MN-major (dims
+// contiguous) by the second.  Nothing is expanded.  What meets the codes is split into
+// e4m3 numbers, several columns per row:
+//   * a query element is 8 significant bits of bf16: q 2^-e = hi + lo / 16 exactly, hi and
+//     lo with 4 bits each (e: the row's exponent, hi below 256; elements under 2^-14 of the
+//     row's largest lose bits below 2^-21 of it).  S = S_hi + S_lo / 16.
+//   * a weight is taken to fp16 (11 bits) and split into three: P = P0 + P1 / 16 + P2 / 256,
+//     each product in columns of its own, joined at the end.  Off by 2^-12 of the weight,
+//     or 2^-24 of the row's largest weight where that is more (a bf16 weight: 2^-8).
+// A key's scale multiplies its scores (thread = key) and its weight, the latter relative to
+// the largest scale seen, so that P keeps within e4m3's range.  The rotary columns are bf16
+// and have a bf16 product of their own; where v reaches into them (dv > dq), so do they.
 //
-// Work: a unit is one 128-key tile of one (sequence, NR-row tile).  All units of the
-// call in order are cut into equal stretches, one per CTA, whatever the lengths (which
-// only the device knows), so a long context is split over the SMs and ragged batches
-// balance.  A row tile that spans CTAs leaves (maximum, sum, unnormalised output) per
-// part in the workspace; tree_attn_join_kernel adds them up in order (no atomics).
+// Why split: with bf16 operands every tile's codes are expanded in shared memory, 147 KB
+// stored and read back per tile, next to MMAs that read their operands from the same
+// memory ((4 KB + N * 32 B) / 128 B cycles for M128 N16..128: 40 at N = 16, 49 at 64, 65
+// at 128).  That form took 10.5 K cycles per 64-row tile; a code tile is half the bytes,
+// K = 32 per instruction halves the operand reads, and two tiles fit, so loads run ahead.
 //
-// Warps: 4 softmax warps (thread = key = TMEM lane), 8 loader warps, one MMA / query-TMA
-// warp and one address warp: 14, so that four share a scheduler and a thread may hold 128
-// registers (with 18 warps, 96: the loaders spilled, and a spill waits for its load).  The
-// address warp walks the page table ahead of the loads (slot, scale factor and state of
-// each key, in shared memory).  A loader warp owns 16 keys: its codes of the next tile wait
-// in registers, so the memory latency passes behind a whole tile's work, and a pair of
-// 64-column chunks is refilled as soon as the last product that reads it is done.  No load
-// is in flight while a tile is converted: the proxy fence that hands a chunk to the tensor
-// cores waits for all of its thread's loads.  The bf16 tail goes from global to shared
-// memory directly (cp.async).
+// Work: a unit is one 128-key tile of one (sequence, NR-row tile), NR = 16 or 32 (three
+// output columns per row fill TMEM at 32).  All units of the call in order are cut into
+// equal stretches, one per CTA, whatever the lengths (which only the device knows), so a
+// long context is split over the SMs and ragged batches balance.  A row tile that spans
+// CTAs leaves (maximum, sum, unnormalised output) per part in the workspace;
+// tree_attn_join_kernel adds them up in order (no atomics).
 //
-// Softmax: p = 2^(s - m) with a reference m that need not be the running maximum: p, its
-// sum and the output are floating point, so only overflow limits how far s may pass m.
-// A tile is worked on in one pass with the m it finds; if a score passed it by more than
-// TA_GROW (base 2), m is raised, and sum and output scaled, after the tile's product; only
-// a score that passes it by TA_MOST raises it before, and the tile is done again.  A row
-// tile's first tile finds its maxima first.  Sums are kept per thread in fp32 and reduced
-// once per row tile.
+// Warps: 8 softmax warps (thread = key = TMEM lane; two share a lane quarter and split the
+// rows), 4 loader warps, one MMA warp, one address warp that walks the page table ahead of
+// the loads.  A tile whose keys are all present and unmarked comes by TMA in boxes of r
+// rows (r: the power of two that divides page and 128, at least 8); others (the last of a
+// sequence, odd pages) by cp.async with absent and marked rows zeroed, so that no garbage
+// meets a zero weight.
+//
+// Softmax: p = 2^(s - m) with a reference m that is raised only when a score passes it by
+// TA_GROW (one vote per tile), together with sum and output; sums are kept per thread in
+// fp32 and reduced once per row tile.
 #pragma once
 #include "latent_cache.cuh"
 #include "sparse_attn.cuh"
@@ -45,18 +54,22 @@
 
 namespace ks {
 
-constexpr int TA_SOFT = 128;                 // softmax threads (warps 0-3)
-constexpr int TA_LOAD = 256;                 // loader threads (warps 4-11)
-constexpr int TA_W_LOAD = 4, TA_W_MMA = 12, TA_W_ADDR = 13;
-constexpr int TA_THREADS = TA_SOFT + TA_LOAD + 64;
-constexpr int TA_MAX_CHUNKS = 9;             // 64-column chunks of a row
+constexpr int TA_SOFT = 256;                 // softmax threads (warps 0-7)
+constexpr int TA_LOADERS = 4;                // loader warps (8-11)
+constexpr int TA_W_LOAD = 8, TA_W_MMA = 12, TA_W_ADDR = 13;
+constexpr int TA_THREADS = 14 * 32;
 constexpr int TA_MAX_CTAS = 148;             // SMs of a B200: bounds the workspace
-constexpr int TA_MAX_ROWS = 64;
-constexpr int TA_HDR = 8192;
+constexpr int TA_MAX_ROWS = 32;
+constexpr int TA_STAGES = 4;                 // most code tiles in shared memory
 constexpr int TA_AHEAD = 4;                  // tiles whose addresses are held
-constexpr float TA_GROW = 8.f, TA_MOST = 24.f;  // how far a score may pass m (base 2)
+constexpr int TA_HDR = 6144;
+constexpr int TA_LEVELS = 3;                 // e4m3 columns per weight
+constexpr float TA_GROW = 2.f;               // how far a score may pass m (base 2)
+constexpr float TA_HEAD = 1.f;               // a raised m lies this far above the score
+constexpr float TA_TOP = 64.f;               // P of a weight of 1 at the largest scale: 64 * 2^TA_GROW < 448
 
 struct TreeAttnParams {
+  const uint16_t* q;      // bf16 [B, T * H, dq + dr]
   const uint8_t* kv8;
   const float* scale;
   const uint16_t* tail;
@@ -70,11 +83,12 @@ struct TreeAttnParams {
   int32_t B, T, H, dv;
   int32_t rows;           // T * H
   int32_t row_tiles;      // ceil(rows / NR)
-  int32_t nq, nkb, nka;   // e4m3 chunks, all chunks, chunk slots of a stage
-  int32_t dv_tiles;       // 128-row M tiles of O^T
-  int32_t stages;         // K tiles in shared memory (1 or 2)
-  int32_t p_alias;        // P lies in the last (key-only) chunk
-  uint32_t k_off, q_off, p_off;
+  int32_t nc;             // 128-column chunks of codes
+  int32_t dt;             // 128-dim tiles of O^T from codes
+  int32_t vt;             // 1: v reaches into the bf16 columns
+  int32_t stages, s_bufs;
+  int32_t box;            // rows of a TMA box, 0: no TMA
+  uint32_t stage_bytes, k_off, q_off, p_off, pb_off;
   uint32_t tmem_cols;
   float scale_log2;
   float* part_o;          // [2 * CTAs][NR][dv]
@@ -85,26 +99,25 @@ struct TreeAttnParams {
 };
 
 struct TaShared {
-  uint64_t full[2][5];              // a pair of chunks (4: the tail) has been written
-  uint64_t vfree[2][4];             // the PV products of a 128-dim tile are done
-  uint64_t s_full[2];               // scores of a tile are in TMEM (and its K reads done)
-  uint64_t p_full[2];               // P of a tile is in shared memory
-  uint64_t pv_done[2];              // all PV products of a tile are done
-  uint64_t a_full[TA_AHEAD], a_free[TA_AHEAD];  // a tile's addresses are in place / used
+  uint64_t full[TA_STAGES], kfree[TA_STAGES];   // a tile's rows are in place / have been used
+  uint64_t s_full[2], s_free[2];                // scores are in TMEM / in registers
+  uint64_t p_full, pv_done;                     // weights are in shared memory / have been used
+  uint64_t a_full[TA_AHEAD], a_free[TA_AHEAD];  // a tile's addresses and scales
   uint64_t q_full, drain;
   uint32_t tmem_base;
   int abort;
   int64_t total, per;
-  int32_t b0, rt0, t0;              // where this CTA's stretch starts
-  alignas(16) float m[TA_MAX_ROWS];     // reference of each row (base 2)
-  alignas(16) float mneg[TA_MAX_ROWS];  // its negative (read as float4)
-  float f[TA_MAX_ROWS];             // factor of a raise; at the end 1 / sum
+  int32_t b0, rt0, t0;                          // where this CTA's stretch starts
+  float sigma, fs;                              // largest scale so far; factor of its raise
+  alignas(16) float m[TA_MAX_ROWS];             // reference of each row (base 2)
+  alignas(16) float mneg[TA_MAX_ROWS];          // its negative
+  alignas(16) float qs[TA_MAX_ROWS];            // 2^e * softmax scale of each row
+  alignas(16) float f[TA_MAX_ROWS];             // factor of a raise; at the end 1 / sum
   float red[4][TA_MAX_ROWS];
-  int32_t slot[TA_AHEAD][128];      // row of the page pool, -1: nothing to load
-  uint32_t mul[TA_AHEAD][128];      // 2^120 * scale as two bf16 factors (low half, high half)
-  // key: 0 fine, 1 absent, 2 marked (scale NaN); read by the softmax, which is up to two
-  // tiles behind the loaders that free the addresses
-  uint8_t flag[2 * TA_AHEAD][128];
+  float red_s[8];
+  int32_t whole[TA_AHEAD];                      // every key of the tile can come by TMA
+  int32_t slot[TA_AHEAD][128];                  // row of the page pool, -1: zeros
+  float sk[TA_AHEAD][128];                      // key's scale; -1: absent, NaN: marked
 };
 static_assert(sizeof(TaShared) <= TA_HDR, "TaShared exceeds its header");
 
@@ -152,46 +165,23 @@ struct TaWalk {
   }
 };
 
+// A ring position: slot and phase parity.
+struct TaRing {
+  int i = 0;
+  uint32_t ph = 0;
+  __device__ __forceinline__ void next(int n) {
+    if (++i == n) {
+      i = 0;
+      ph ^= 1;
+    }
+  }
+};
+
 // Slot of the page pool that holds this position, -1 for none (a pool has < 2^31 slots).
 __device__ __forceinline__ int ta_slot(const TreeAttnParams& p, const TaWalk& w, int key) {
   const int pos = w.t * 128 + key;
   if (w.left <= 0 || pos >= ta_keys(p, w.len)) return -1;
   return (int)cache_row(p.table, p.max_pages, p.n_pages, p.page, w.b, pos, p.status);
-}
-
-// Two e4m3 codes (bytes 0, 1 of w with SEL = 0x9180, bytes 2, 3 with 0xB3A2) as bf16,
-// times the powers of two in `mul`.  A code s eeee mmm is placed in its 16-bit lane sign
-// extended, moved up by 4 and masked: s 0000 eeee mmm 0000, its value times 2^-120 (bf16's
-// bias is 120 more than e4m3's; subnormals included).  The one exact product with 2^120 *
-// scale is the value.
-template <uint32_t SEL>
-__device__ __forceinline__ uint32_t ta_expand(uint32_t w, uint32_t mul) {
-  uint32_t t;
-  asm("prmt.b32 %0, %1, %1, %2;" : "=r"(t) : "r"(w), "n"(SEL));
-  return mul_bf16x2((t * 16u) & 0x87F087F0u, mul);
-}
-
-// ldcg_or_zero at a constant offset: one address for a whole row.
-template <int OFF>
-__device__ __forceinline__ uint4 ta_ld(const void* base, bool pred) {
-  uint4 v;
-  asm volatile(
-      "{ .reg .pred p; setp.ne.b32 p, %5, 0;"
-      " mov.b32 %0, 0; mov.b32 %1, 0; mov.b32 %2, 0; mov.b32 %3, 0;"
-      " @p ld.global.cg.v4.u32 {%0, %1, %2, %3}, [%4 + %6]; }"
-      : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-      : "l"(base), "r"((int)pred), "n"(OFF));
-  return v;
-}
-// Chunks C .. NQ - 1 of two rows.
-template <int C, int NQ>
-__device__ __forceinline__ void ta_load_rows(uint4 (&r)[NQ][2], const uint8_t* c0, const uint8_t* c1, bool ok0,
-                                             bool ok1, int nq) {
-  if constexpr (C < NQ) {
-    r[C][0] = ta_ld<C * 64>(c0, ok0 && C < nq);
-    r[C][1] = ta_ld<C * 64>(c1, ok1 && C < nq);
-    ta_load_rows<C + 1, NQ>(r, c0, c1, ok0, ok1, nq);
-  }
 }
 
 __device__ __forceinline__ void tmem_ld8(uint32_t taddr, uint32_t* r) {
@@ -205,10 +195,14 @@ __device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t* r) {
                : "memory");
 }
 template <int N>
-__device__ __forceinline__ void tmem_ldn(uint32_t taddr, uint32_t* r) {
-  if constexpr (N == 8) tmem_ld8(taddr, r);
-  else if constexpr (N == 16) tmem_ld16(taddr, r);
-  else tmem_ld32(taddr, r);
+__device__ __forceinline__ void tmem_ldn(uint32_t taddr, float* r) {
+  if constexpr (N == 8) tmem_ld8(taddr, reinterpret_cast<uint32_t*>(r));
+  else tmem_ld16(taddr, reinterpret_cast<uint32_t*>(r));
+}
+template <int N>
+__device__ __forceinline__ void tmem_stn(uint32_t taddr, const float* r) {
+  if constexpr (N == 8) tmem_st8(taddr, reinterpret_cast<const uint32_t*>(r));
+  else tmem_st16(taddr, reinterpret_cast<const uint32_t*>(r));
 }
 // Any thread of the softmax warps (also a barrier among them).
 __device__ __forceinline__ bool soft_any(bool x) {
@@ -221,48 +215,73 @@ __device__ __forceinline__ bool soft_any(bool x) {
 }
 __device__ __forceinline__ void soft_sync() { named_bar_sync(1, TA_SOFT); }
 
-// Max or sum over the warp's lanes of CW values each into red[.. + c], c < CW.
+// Max or sum over the warp's lanes of CW <= 16 values each into red[c], c < CW.
 template <bool MX, int CW>
 __device__ __forceinline__ void ta_reduce(const float (&v)[CW], float* red, int lane) {
+  float w[16];
 #pragma unroll
-  for (int g = 0; g < CW; g += 16) {
-    float w[16];
-#pragma unroll
-    for (int i = 0; i < 16; ++i) w[i] = g + i < CW ? v[(g + i) % CW] : 0.f;
-    const float r = reduce16_lanes<MX>(w, lane);  // value g + (lane >> 1)
-    if ((lane & 1) == 0 && g + (lane >> 1) < CW) red[g + (lane >> 1)] = r;
-  }
+  for (int i = 0; i < 16; ++i) w[i] = i < CW ? v[i % CW] : 0.f;
+  const float r = reduce16_lanes<MX>(w, lane);  // value lane >> 1
+  if ((lane & 1) == 0 && (lane >> 1) < CW) red[lane >> 1] = r;
 }
 
-template <int NR, int NQ>
+// MN-major operand of 64-byte rows (32 bf16) with the 64-byte swizzle: 16-byte unit u of
+// row r lies at u ^ ((r >> 1) & 3); 8 rows are 512 bytes.
+__device__ __forceinline__ uint64_t sdesc_sw64(uint32_t saddr) {
+  return (uint64_t)((saddr >> 4) & 0x3FFF) | (uint64_t)(16 >> 4) << 16 | (uint64_t)(512 >> 4) << 32 |
+         (uint64_t)1 << 46 | (uint64_t)4 << 61;
+}
+
+__device__ __forceinline__ uint32_t f16x2_of_e4m3x2(uint16_t c) {
+  uint32_t h;
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"(c));
+  return h;
+}
+// Two fp16 as e4m3 (lo in bits 0-7); `h` becomes 16 times what that leaves (exact).
+__device__ __forceinline__ uint16_t ta_split(uint32_t& h) {
+  uint16_t c;
+  asm("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;" : "=h"(c) : "r"(h));
+  const uint32_t b = f16x2_of_e4m3x2(c);
+  asm("{ .reg .b32 t; sub.rn.f16x2 t, %0, %1; mul.rn.f16x2 %0, t, %2; }" : "+r"(h) : "r"(b), "r"(0x4C004C00u));
+  return c;
+}
+
+template <int NR>
 __global__ void __launch_bounds__(TA_THREADS, 1)
-    tree_attn_kernel(const __grid_constant__ CUtensorMap qm, const TreeAttnParams p) {
-  constexpr int CB = NR < 32 ? NR : 32;  // rows that a softmax thread works on at a time
+    tree_attn_kernel(const __grid_constant__ CUtensorMap km, const __grid_constant__ CUtensorMap tm,
+                     const TreeAttnParams p) {
+  constexpr int CW = NR / 2;             // rows of a softmax thread
+  constexpr int NP = TA_LEVELS * NR;     // columns of P and of a dim tile of O^T
   extern __shared__ uint8_t ta_raw[];
   const uint32_t raw = smem_u32(ta_raw);
   uint8_t* smem = ta_raw + (((raw + 1023u) & ~1023u) - raw);
   TaShared* sh = reinterpret_cast<TaShared*>(smem);
-  uint8_t* ks_ = smem + p.k_off;  // [stages][nka][128 keys x 128 B]
-  uint8_t* qs = smem + p.q_off;   // [nkb][NR rows x 128 B]
-  uint8_t* ps = smem + p.p_off;   // [stages][128 keys x 128 B], rows contiguous (MN-major)
+  uint8_t* ks_ = smem + p.k_off;  // [stages]: [nc][128 keys x 128 B] codes, [128 keys x 128 B] bf16 tail
+  uint8_t* qs = smem + p.q_off;   // [nc][NR hi rows, NR lo rows x 128 B], [NR x 128 B] bf16 tail
+  uint8_t* ps = smem + p.p_off;   // [128 keys x 128 B]: level, row (MN-major)
+  uint8_t* pb = smem + p.pb_off;  // [128 keys x 64 B]: bf16 weights (MN-major), with vt
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   WaitCtx wc{&sh->abort, p.status, p.budget_ns};
 
   if (threadIdx.x == 0) {
-    for (int s = 0; s < 2; ++s) {
-      for (int c = 0; c < 5; ++c) mbar_init(&sh->full[s][c], TA_LOAD / 32);
-      for (int m = 0; m < 4; ++m) mbar_init(&sh->vfree[s][m], 1);
-      mbar_init(&sh->s_full[s], 1);
-      mbar_init(&sh->p_full[s], TA_SOFT / 32);
-      mbar_init(&sh->pv_done[s], 1);
+    for (int s = 0; s < TA_STAGES; ++s) {
+      mbar_init(&sh->full[s], TA_LOADERS);
+      mbar_init(&sh->kfree[s], 1);
     }
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(&sh->s_full[s], 1);
+      mbar_init(&sh->s_free[s], TA_SOFT / 32);
+    }
+    mbar_init(&sh->p_full, TA_SOFT / 32);
+    mbar_init(&sh->pv_done, 1);
     for (int s = 0; s < TA_AHEAD; ++s) {
       mbar_init(&sh->a_full[s], 1);
-      mbar_init(&sh->a_free[s], TA_LOAD / 32);
+      mbar_init(&sh->a_free[s], TA_LOADERS + TA_SOFT / 32);
     }
-    mbar_init(&sh->q_full, 1);
+    mbar_init(&sh->q_full, TA_SOFT / 32);
     mbar_init(&sh->drain, 1);
     sh->abort = 0;
+    sh->sigma = 0.f;
     fence_barrier_init();
     p.owner[(int64_t)blockIdx.x * 4 + 2] = 0;  // no row tile's head here yet
   }
@@ -273,7 +292,10 @@ __global__ void __launch_bounds__(TA_THREADS, 1)
   if (warp == TA_W_MMA) {
     tmem_alloc<1>(&sh->tmem_base, p.tmem_cols);
     tmem_relinquish<1>();
-    if (lane == 0) tma_prefetch_desc(&qm);
+    if (lane == 0 && p.box) {
+      tma_prefetch_desc(&km);
+      if (p.dr) tma_prefetch_desc(&tm);
+    }
   }
   if (warp == TA_W_ADDR) {  // the call's units, and where this CTA's stretch starts
     int64_t total = 0;
@@ -321,218 +343,161 @@ __global__ void __launch_bounds__(TA_THREADS, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = sh->tmem_base;
-  const uint32_t o_col = (uint32_t)(p.stages * NR);
-  const int two = p.stages == 2;
+  const uint32_t o_col = (uint32_t)(p.s_bufs * 3 * NR);       // S: hi, lo, tail columns
+  const uint32_t ot_col = o_col + (uint32_t)(p.dt * NP);      // O^T of the bf16 columns
   TaWalk w;
   w.start(p, sh);
 
   if (warp >= TA_W_LOAD && warp < TA_W_MMA) {
     // ================================================================ loaders
-    // lane: 16 codes (part) of keys key0, key0 + 8 in each chunk; a warp's load covers
-    // 64-byte stretches of 8 rows
-    const int lw = warp - TA_W_LOAD, part = lane & 3, key0 = lw * 16 + (lane >> 2);
-    const uint32_t sw = (uint32_t)(key0 & 7), units = (uint32_t)max(w.left, 0);
-    const uint32_t at0 = (uint32_t)key0 * 128 + (((uint32_t)(part * 2) ^ sw) << 4);
-    const uint32_t at1 = (uint32_t)key0 * 128 + (((uint32_t)(part * 2 + 1) ^ sw) << 4);
-    uint4 r[NQ][2];
-    auto load = [&](uint32_t g) {
-      const int s0 = sh->slot[g % TA_AHEAD][key0], s1 = sh->slot[g % TA_AHEAD][key0 + 8];
-      const uint8_t* c0 = p.kv8 + (int64_t)s0 * p.dq + part * 16;
-      const uint8_t* c1 = p.kv8 + (int64_t)s1 * p.dq + part * 16;
-      ta_load_rows<0, NQ>(r, c0, c1, s0 >= 0, s1 >= 0, p.nq);
-    };
-    bool ok = units > 0;
-    if (ok) {
-      ok = mbar_wait_inl(&sh->a_full[0], 0, wc);
-      load(0);
-    }
-    // The tail is early where only the scores read it; it waits for the second product
-    // where that reads it too, or P takes its place (p_alias).
-    const bool tail_pv = p.nq < 2 * p.dv_tiles, tail_early = p.dr > 0 && !tail_pv && !p.p_alias;
-    for (uint32_t g = 0; g < units && ok; ++g) {
-      const int st = two ? (int)(g & 1) : 0, ad = (int)(g % TA_AHEAD);
-      const uint32_t use = two ? g >> 1 : g, last = (use - 1) & 1;
-      uint8_t* tile = ks_ + (size_t)st * p.nka * 16384;
-      const uint32_t ma = sh->mul[ad][key0], mb = sh->mul[ad][key0 + 8];
-      const uint32_t m1[2] = {(ma & 0xFFFFu) * 0x10001u, (mb & 0xFFFFu) * 0x10001u};
-      const bool big = __any_sync(0xFFFFFFFFu, (ma >> 16) != 0x3F80u || (mb >> 16) != 0x3F80u);
-      auto tail = [&] {
-        if (use > 0)
-          ok = mbar_wait_inl(tail_pv     ? &sh->vfree[st][p.nq >> 1]
-                             : p.p_alias ? &sh->pv_done[st]
-                                         : &sh->s_full[st], last, wc) && ok;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int key = lw * 16 + j * 4 + (lane >> 3), piece = lane & 7;
-          const int s = sh->slot[ad][key];
-          cp_async16(tile + p.nq * 16384 + key * 128 + ((piece ^ (key & 7)) << 4),
-                     p.tail + (int64_t)max(s, 0) * p.dr + piece * 8, s >= 0 ? 16u : 0u);
-        }
-      };
-      if (tail_early) tail();
-#pragma unroll
-      for (int m = 0; m < NQ / 2; ++m) {
-        if (2 * m < p.nq) {
-          const bool end = 2 * m + 2 >= p.nq;
-          if (use > 0)
-            ok = mbar_wait_inl(m < p.dv_tiles ? &sh->vfree[st][m] : &sh->s_full[st], last, wc) && ok;
-          if (end && p.dr > 0 && !tail_early) tail();
-#pragma unroll
-          for (int c = 2 * m; c < 2 * m + 2; ++c) {
-            if (c >= p.nq) continue;
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-              const uint4 v = r[c][j];
-              uint4 lo, hi;
-              lo.x = ta_expand<0x9180>(v.x, m1[j]);
-              lo.y = ta_expand<0xB3A2>(v.x, m1[j]);
-              lo.z = ta_expand<0x9180>(v.y, m1[j]);
-              lo.w = ta_expand<0xB3A2>(v.y, m1[j]);
-              hi.x = ta_expand<0x9180>(v.z, m1[j]);
-              hi.y = ta_expand<0xB3A2>(v.z, m1[j]);
-              hi.z = ta_expand<0x9180>(v.w, m1[j]);
-              hi.w = ta_expand<0xB3A2>(v.w, m1[j]);
-              if (big) {  // a scale beyond 2^7
-                const uint32_t m2 = ((j ? mb : ma) >> 16) * 0x10001u;
-                lo.x = mul_bf16x2(lo.x, m2);
-                lo.y = mul_bf16x2(lo.y, m2);
-                lo.z = mul_bf16x2(lo.z, m2);
-                lo.w = mul_bf16x2(lo.w, m2);
-                hi.x = mul_bf16x2(hi.x, m2);
-                hi.y = mul_bf16x2(hi.y, m2);
-                hi.z = mul_bf16x2(hi.z, m2);
-                hi.w = mul_bf16x2(hi.w, m2);
-              }
-              *reinterpret_cast<uint4*>(tile + c * 16384 + j * 1024 + at0) = lo;
-              *reinterpret_cast<uint4*>(tile + c * 16384 + j * 1024 + at1) = hi;
-            }
+    const int lw = warp - TA_W_LOAD, piece = lane & 7;
+    TaRing st, ad;
+    uint32_t sent = 0, sent_ph = 0;  // stages whose latest load is by TMA, and its phase
+    bool ok = true;
+    for (int u = 0; u < w.left && ok; ++u, st.next(p.stages), ad.next(TA_AHEAD)) {
+      ok = mbar_wait_inl(&sh->a_full[ad.i], ad.ph, wc) && ok;
+      const bool whole = p.box && sh->whole[ad.i];
+      ok = mbar_wait_inl(&sh->kfree[st.i], st.ph ^ 1, wc) && ok;
+      if (!ok) break;
+      uint8_t* tile = ks_ + (size_t)st.i * p.stage_bytes;
+      const int32_t* sl = sh->slot[ad.i];
+      if (whole) {
+        if (lw == 0 && elect_one()) {
+          mbar_expect_tx(&sh->full[st.i], p.stage_bytes);
+          for (int r = 0; r < 128; r += p.box) {
+            const int y = sl[r];
+            for (int c = 0; c < p.nc; ++c) tma_load_2d(&km, &sh->full[st.i], tile + c * 16384 + r * 128, c * 128, y);
+            if (p.dr) tma_load_2d(&tm, &sh->full[st.i], tile + p.nc * 16384 + r * 128, 0, y);
           }
-          if (p.dr > 0 && (tail_early ? m == 0 : end)) cp_async_wait_all();
-          fence_proxy_async_smem();
-          __syncwarp();
-          if (lane == 0) {
-            mbar_arrive(&sh->full[st][m]);
-            if (p.dr > 0 && (tail_early ? m == 0 : end)) mbar_arrive(&sh->full[st][4]);
-            if (end) mbar_arrive(&sh->a_free[ad]);
-          }
+        } else if (lw != 0 && lane == 0) {
+          mbar_arrive(&sh->full[st.i]);
         }
+        __syncwarp();
+        sent |= 1u << st.i;
+        sent_ph = (sent_ph & ~(1u << st.i)) | st.ph << st.i;
+      } else {
+        sent &= ~(1u << st.i);
+        for (int i = 0; i < 8; ++i) {  // 8 lanes per row: 128 bytes of it at a time
+          const int key = lw * 32 + i * 4 + (lane >> 3), s = sl[key];
+          const uint8_t* src = p.kv8 + (int64_t)max(s, 0) * p.dq + piece * 16;
+          uint8_t* dst = tile + key * 128 + ((piece ^ (key & 7)) << 4);
+          for (int c = 0; c < p.nc; ++c) {
+            const bool in = s >= 0 && c * 128 + piece * 16 < p.dq;
+            cp_async16(dst + c * 16384, in ? src + c * 128 : p.kv8, in ? 16u : 0u);
+          }
+          if (p.dr)
+            cp_async16(dst + p.nc * 16384, p.tail + (int64_t)max(s, 0) * p.dr + piece * 8, s >= 0 ? 16u : 0u);
+        }
+        cp_async_wait_all();
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sh->full[st.i]);
       }
-      if (g + 1 < units) {
-        ok = mbar_wait_inl(&sh->a_full[(g + 1) % TA_AHEAD], ((g + 1) / TA_AHEAD) & 1, wc) && ok;
-        load(g + 1);
-      }
+      if (lane == 0) mbar_arrive(&sh->a_free[ad.i]);
     }
+    // after a timed-out wait: no load of this CTA may land once it has gone
+    if (lw == 0 && *wc.abort)
+      for (int s = 0; s < TA_STAGES; ++s)
+        if (sent >> s & 1) mbar_wait(&sh->full[s], sent_ph >> s & 1, wc, false, true);
   } else if (warp == TA_W_ADDR) {
     // ================================================================ addresses
-    const uint32_t units = (uint32_t)max(w.left, 0);
+    TaRing ad;
+    const int units = max(w.left, 0);
     bool ok = true;
-    for (uint32_t g = 0; g < units && ok; ++g, w.next_unit(p)) {
+    for (int u = 0; u < units && ok; ++u, ad.next(TA_AHEAD), w.next_unit(p)) {
       int s[4];
-      uint32_t sb[4];
+      float k[4];
+      bool whole = true;
 #pragma unroll
       for (int i = 0; i < 4; ++i) s[i] = ta_slot(p, w, i * 32 + lane);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        sb[i] = s[i] >= 0 ? __float_as_uint(__ldg(p.scale + s[i])) : 0u;
-        if (s[i] >= 0 && p.dr > 0)  // the tail is fetched when its place is free: have it near
-          asm volatile("prefetch.global.L2 [%0];" ::"l"(p.tail + (int64_t)s[i] * p.dr));
+        k[i] = s[i] >= 0 ? __ldg(p.scale + s[i]) : -1.f;
+        if ((__float_as_uint(k[i]) & 0x7F800000u) == 0x7F800000u) {  // marked: its row is not read
+          k[i] = __uint_as_float(0x7FC00000u);
+          s[i] = -1;
+        }
+        whole &= s[i] >= 0;
       }
-      const int ad = (int)(g % TA_AHEAD);
-      if (g >= TA_AHEAD) ok = mbar_wait_inl(&sh->a_free[ad], (g / TA_AHEAD - 1) & 1, wc);
+      ok = mbar_wait_inl(&sh->a_free[ad.i], ad.ph ^ 1, wc);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const int key = i * 32 + lane;
-        const bool bad = (sb[i] & 0x7F800000u) == 0x7F800000u;
-        // 2^120 * scale, in two factors where that is beyond bf16 (0 for a scale of 0)
-        const int e = (int)((sb[i] >> 23) & 255) + 120;
-        const uint32_t m1 = (sb[i] & 0x7F800000u) && !bad ? (uint32_t)min(e, 254) << 7 : 0u;
-        const uint32_t m2 = bad ? 127u : (uint32_t)(max(e, 254) - 254 + 127);
-        sh->flag[g % (2 * TA_AHEAD)][key] = s[i] < 0 ? 1 : bad ? 2 : 0;
-        sh->slot[ad][key] = bad ? -1 : s[i];
-        sh->mul[ad][key] = m1 | (m2 << 23);
+        sh->slot[ad.i][i * 32 + lane] = s[i];
+        sh->sk[ad.i][i * 32 + lane] = k[i];
       }
+      whole = __all_sync(0xFFFFFFFFu, whole);
+      if (lane == 0) sh->whole[ad.i] = whole;
       __syncwarp();
-      if (lane == 0) mbar_arrive(&sh->a_full[ad]);
+      if (lane == 0) mbar_arrive(&sh->a_full[ad.i]);
     }
   } else if (warp == TA_W_MMA) {
     // ================================================================ MMA issue
     if (elect_one()) {
-      const uint32_t id_qk = idesc_bf16_f32(128, NR, false, false), id_pv = idesc_bf16_f32(128, NR, true, true);
-      uint32_t g = 0, items = 0;
-      bool ok = true;
-      // the item's query rows (rows past it are other rows or zeros: their columns are not used)
-      auto load_q = [&](const TaWalk& x) {
-        mbar_expect_tx(&sh->q_full, (uint32_t)p.nkb * NR * 128);
-        const int y = x.b * p.rows + x.rt * NR;
-        for (int c = 0; c < p.nkb; ++c) tma_load_2d(&qm, &sh->q_full, qs + c * NR * 128, c * 64, y);
-      };
+      const uint32_t id_qk = idesc_e4m3_f32(128, 2 * NR), id_qt = idesc_bf16_f32(128, NR, false, false);
+      const uint32_t id_pv = idesc_e4m3_f32(128, NP) | (1u << 15) | (1u << 16), id_pt = idesc_bf16_f32(128, NR, true, true);
       // descriptors: only the start address (low word, 16-byte units) changes
       const uint64_t k_desc = sdesc_sw128(smem_u32(ks_), 16, 1024), q_desc = sdesc_sw128(smem_u32(qs), 16, 1024);
       const uint64_t v_desc = sdesc_sw128(smem_u32(ks_), 16384, 1024), p_desc = sdesc_sw128(smem_u32(ps), 16, 1024);
-      const uint32_t stage16 = (uint32_t)p.nka * 1024;
-      auto qk = [&](uint32_t g) {
-        const int st = two ? (int)(g & 1) : 0;
-        const uint32_t use = two ? g >> 1 : g;
-        for (int c = 0; c < p.nkb; ++c) {
-          if (c == p.nq || !(c & 1)) {
-            ok = mbar_wait_inl(&sh->full[st][c == p.nq ? 4 : c >> 1], use & 1, wc);
-            if (!ok) return;
-            tc_fence_after();
-          }
-          const uint64_t ad = k_desc + st * stage16 + c * 1024, bd = q_desc + c * (NR * 8);
-#pragma unroll
-          for (int k = 0; k < 4; ++k)
-            umma_bf16_ss(tmem + st * NR, ad + k * 2, bd + k * 2, id_qk, c > 0 || k > 0 ? 1u : 0u);
-        }
-        umma_commit(&sh->s_full[st]);
-      };
-      auto pv = [&](uint32_t g, bool first) {
-        const int st = two ? (int)(g & 1) : 0;
-        const uint32_t use = two ? g >> 1 : g;
-        ok = mbar_wait_inl(&sh->p_full[st], use & 1, wc);
+      const uint64_t pb_desc = sdesc_sw64(smem_u32(pb));
+      const uint32_t stage16 = p.stage_bytes >> 4;
+      TaRing kq, kp, sq;  // code tile of the next QK and of the next PV; score buffer
+      uint32_t n_pv = 0, items = 0;
+      bool ok = true;
+      auto qk = [&] {
+        ok = mbar_wait_inl(&sh->full[kq.i], kq.ph, wc) && mbar_wait_inl(&sh->s_free[sq.i], sq.ph ^ 1, wc);
         if (!ok) return;
         tc_fence_after();
-        const uint64_t bd = p_desc + st * 1024;
-        for (int m = 0; m < p.dv_tiles; ++m) {
-          const uint64_t ad = v_desc + st * stage16 + m * 2048;
+        const uint32_t d = tmem + sq.i * 3 * NR;
+        const uint64_t a = k_desc + kq.i * stage16;
+        for (int c = 0; c < p.nc; ++c) {
 #pragma unroll
-          for (int k = 0; k < 8; ++k)  // 16 keys: 2048 bytes further in both
-            umma_bf16_ss(tmem + o_col + m * NR, ad + k * 128, bd + k * 128, id_pv, !first || k > 0 ? 1u : 0u);
-          umma_commit(&sh->vfree[st][m]);
+          for (int k = 0; k < 4; ++k)
+            umma_f8_ss(d, a + c * 1024 + k * 2, q_desc + c * (2 * NR * 8) + k * 2, id_qk, c > 0 || k > 0 ? 1u : 0u);
         }
-        umma_commit(&sh->pv_done[st]);
+        if (p.dr) {
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            umma_bf16_ss(d + 2 * NR, a + p.nc * 1024 + k * 2, q_desc + p.nc * (2 * NR * 8) + k * 2, id_qt, k > 0 ? 1u : 0u);
+        }
+        umma_commit(&sh->s_full[sq.i]);
+        kq.next(p.stages);
+        sq.next(p.s_bufs);
       };
-      bool q_wait = false;
+      auto pv = [&](bool first) {
+        ok = mbar_wait_inl(&sh->p_full, n_pv & 1, wc);
+        if (!ok) return;
+        ++n_pv;
+        tc_fence_after();
+        const uint64_t a = v_desc + kp.i * stage16;
+        for (int m = 0; m < p.dt; ++m) {
+#pragma unroll
+          for (int k = 0; k < 4; ++k)  // 32 keys: 4096 bytes further in both
+            umma_f8_ss(tmem + o_col + m * NP, a + m * 1024 + k * 256, p_desc + k * 256, id_pv, !first || k > 0 ? 1u : 0u);
+        }
+        if (p.vt) {  // 64 dims (the other 64 lanes hold what lies behind them, unused)
+#pragma unroll
+          for (int k = 0; k < 8; ++k)  // 16 keys: 2048 and 1024 bytes further
+            umma_bf16_ss(tmem + ot_col, a + p.nc * 1024 + k * 128, pb_desc + k * 64, id_pt, !first || k > 0 ? 1u : 0u);
+        }
+        umma_commit(&sh->kfree[kp.i]);
+        umma_commit(&sh->pv_done);
+        kp.next(p.stages);
+      };
       while (w.left > 0 && ok) {
         const int n = w.here();
-        if (g > 0) {  // the previous item's QK products have read its query rows
-          const uint32_t l = g - 1;
-          ok = mbar_wait_inl(&sh->s_full[two ? l & 1 : 0], (two ? l >> 1 : l) & 1, wc);
-          if (!ok) break;
-        }
-        load_q(w);
-        q_wait = true;
         ok = mbar_wait_inl(&sh->q_full, items & 1, wc);
-        if (!ok) break;
-        q_wait = false;
-        if (two) {
-          qk(g);
-          for (int i = 0; i < n && ok; ++i) {
-            if (i + 1 < n) qk(g + i + 1);
-            if (ok) pv(g + i, i == 0);
-          }
-        } else {
-          for (int i = 0; i < n && ok; ++i) {
-            qk(g + i);
-            if (ok) pv(g + i, i == 0);
-          }
+        if (ok) {
+          tc_fence_after();
+          qk();
         }
-        g += n;
+        for (int i = 0; i < n && ok; ++i) {  // the next tile's scores while this one's weights are made
+          if (i + 1 < n) qk();
+          if (ok) pv(i == 0);
+        }
         ++items;
         w.next_item(p, n);
       }
       // nothing of this CTA is in flight when it gives its memory back
-      if (q_wait) mbar_wait(&sh->q_full, items & 1, wc, false, true);
       umma_commit(&sh->drain);
       mbar_wait(&sh->drain, 0, wc, false, true);
     }
@@ -541,33 +506,88 @@ __global__ void __launch_bounds__(TA_THREADS, 1)
     // ================================================================ softmax, epilogue
     // After a wait ran out (abort) the loops run on without waiting, so the warps keep
     // meeting at their barriers; nothing here indexes by data.
-    const int key = warp * 32 + lane;
-    const uint32_t lane_off = (uint32_t)(warp * 32) << 16;
-    uint32_t g = 0;
+    const int quarter = warp & 3, hc = (warp >> 2) * CW;  // first row of this thread
+    const int key = quarter * 32 + lane;
+    const uint32_t lane_off = (uint32_t)(quarter * 32) << 16;
+    TaRing sq, ad;
+    uint32_t g = 0;  // tiles so far: pv_done's phase g - 1 is the last tile's product
     while (w.left > 0) {
       const int n = w.here();
       const int r0 = w.rt * NR;                      // first row of the tile in the sequence
       const int nrows = min(NR, p.rows - r0);
       const bool whole = w.t == 0 && n == w.nt;      // no other CTA has a part
-      float l[NR];
+      // ---- the item's queries: hi and lo codes, bf16 tail
+#pragma unroll 1
+      for (int i = 0; i < NR / 8; ++i) {
+        const int row = warp * (NR / 8) + i;
+        const uint16_t* q = p.q + ((int64_t)w.b * p.rows + r0 + row) * (p.dq + p.dr);
+        const bool in = row < nrows && lane * 16 < p.dq;
+        uint32_t x[8], t[4];
+        *reinterpret_cast<uint4*>(x) = ldcg_or_zero(q + lane * 16, in);
+        *reinterpret_cast<uint4*>(x + 4) = ldcg_or_zero(q + lane * 16 + 8, in);
+        *reinterpret_cast<uint4*>(t) = ldcg_or_zero(q + p.dq + lane * 8, row < nrows && lane * 8 < p.dr);
+        float amax = 0.f;
+        bool bad = false;
 #pragma unroll
-      for (int i = 0; i < NR; ++i) l[i] = 0.f;
-      for (int i = 0; i < n; ++i, ++g) {
-        const int st = two ? (int)(g & 1) : 0;
-        const uint32_t use = two ? g >> 1 : g;
-        const int tile = w.t + i;
+        for (int k = 0; k < 8; ++k) {
+          amax = fmaxf(amax, fmaxf(fabsf(bf16lo_f32(x[k])), fabsf(bf16hi_f32(x[k]))));
+          bad |= bf16x2_nonfinite(x[k]);
+        }
+        bad = __any_sync(0xFFFFFFFFu, bad);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xFFFFFFFFu, amax, o));
+        // largest element into [128, 256)
+        const int e = bad ? 0 : max((int)(__float_as_uint(amax) >> 23) - 127 - 7, -100);
+        const float inv = __uint_as_float((uint32_t)(127 - e) << 23);
+        uint32_t hi[4], lo[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          uint32_t h2 = 0, l2 = 0;
+#pragma unroll
+          for (int z = 0; z < 2; ++z) {
+            const float a = bf16lo_f32(x[2 * k + z]) * inv, b = bf16hi_f32(x[2 * k + z]) * inv;
+            const uint16_t h = cvt_e4m3x2(a, b);
+            const uint32_t back = f16x2_of_e4m3x2(h);
+            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&back));
+            h2 |= (uint32_t)h << (16 * z);
+            l2 |= (uint32_t)cvt_e4m3x2((a - f.x) * 16.f, (b - f.y) * 16.f) << (16 * z);
+          }
+          hi[k] = bad ? 0x7F7F7F7Fu : h2;  // a row with a NaN or an infinity scores NaN
+          lo[k] = bad ? 0u : l2;
+        }
+        const int c = lane >> 3;
+        if (c < p.nc) {
+          uint8_t* at = qs + c * (2 * NR * 128) + row * 128 + (((lane & 7) ^ (row & 7)) << 4);
+          *reinterpret_cast<uint4*>(at) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+          *reinterpret_cast<uint4*>(at + NR * 128) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+        }
+        if (lane * 8 < p.dr) {
+          const uint32_t m2 = (uint32_t)(127 - e) * 0x00800080u;
+          *reinterpret_cast<uint4*>(qs + p.nc * (2 * NR * 128) + row * 128 + ((lane ^ (row & 7)) << 4)) =
+              make_uint4(mul_bf16x2(t[0], m2), mul_bf16x2(t[1], m2), mul_bf16x2(t[2], m2), mul_bf16x2(t[3], m2));
+        }
+        if (lane == 0) sh->qs[row] = __uint_as_float((uint32_t)(127 + e) << 23) * p.scale_log2;
+      }
+      fence_proxy_async_smem();
+      soft_sync();
+      if (lane == 0) mbar_arrive(&sh->q_full);
+
+      float l[CW];
+#pragma unroll
+      for (int c = 0; c < CW; ++c) l[c] = 0.f;
+      for (int i = 0; i < n; ++i, ++g, sq.next(p.s_bufs), ad.next(TA_AHEAD)) {
         // which rows see this key: all, or a bit per row
-        uint64_t allow = ~0ull;
-        const int pos = tile * 128 + key, j = pos - w.len;
+        uint32_t allow = 0xFFFFFFFFu;
+        const int j = (w.t + i) * 128 + key - w.len;
         if (j >= 0) {  // a drafted row, or past them (absent)
           allow = 0;
           if (j < p.T) {
-            int t = r0 / p.H, h = r0 - t * p.H;
+            int t = (r0 + hc) / p.H, h = (r0 + hc) - t * p.H;
             const uint8_t* mk = p.mask + ((int64_t)w.b * p.T) * p.T + j;
-            uint64_t bit = 0;
+            uint32_t bit = 0;
             bool fresh = true;
 #pragma unroll 1
-            for (int c = 0; c < NR; ++c) {
+            for (int c = 0; c < CW; ++c) {
               if (fresh) bit = t < p.T && (p.mask ? mk[(int64_t)t * p.T] != 0 : j <= t);
               allow |= bit << c;
               fresh = ++h == p.H;
@@ -578,134 +598,155 @@ __global__ void __launch_bounds__(TA_THREADS, 1)
             }
           }
         }
-        mbar_wait_inl(&sh->full[st][0], use & 1, wc);  // the key's flag
-        const int flag = sh->flag[g % (2 * TA_AHEAD)][key];
-        if (flag == 1) allow = 0;
-        mbar_wait_inl(&sh->s_full[st], use & 1, wc);
+        mbar_wait_inl(&sh->a_full[ad.i], ad.ph, wc);
+        float sk = sh->sk[ad.i][key];
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sh->a_free[ad.i]);
+        const bool marked = sk != sk;
+        if (sk < 0.f) allow = 0;
+        constexpr uint32_t ALL = (1u << CW) - 1u;
+        const bool plain = __all_sync(0xFFFFFFFFu, (allow & ALL) == ALL && !marked);
+        if (marked || sk < 0.f) sk = 0.f;
+
+        mbar_wait_inl(&sh->s_full[sq.i], sq.ph, wc);
         tc_fence_after();
-        constexpr uint64_t ALL = NR == 64 ? ~0ull : (1ull << NR) - 1;
-        const bool plain = __all_sync(0xFFFFFFFFu, (allow & ALL) == ALL && flag == 0);
-        // rows c0 .. c0 + CB - 1: scaled scores minus their references (raw: themselves)
-        auto exponents = [&](int c0, float (&d)[CB], bool raw) {
-          tmem_ldn<CB>(tmem + st * NR + c0 + lane_off, reinterpret_cast<uint32_t*>(d));
+        float x[CW];  // q 2^-e . k
+        {
+          float lo[CW], tl[CW];
+          const uint32_t at = tmem + sq.i * 3 * NR + hc + lane_off;
+          tmem_ldn<CW>(at, x);
+          tmem_ldn<CW>(at + NR, lo);
+          if (p.dr) tmem_ldn<CW>(at + 2 * NR, tl);
           tmem_wait_ld();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&sh->s_free[sq.i]);
 #pragma unroll
-          for (int c = 0; c < CB; c += 4) {
-            const float4 mn = raw ? make_float4(0.f, 0.f, 0.f, 0.f) : *reinterpret_cast<const float4*>(&sh->mneg[c0 + c]);
-            d[c] = fmaf(d[c], p.scale_log2, mn.x);
-            d[c + 1] = fmaf(d[c + 1], p.scale_log2, mn.y);
-            d[c + 2] = fmaf(d[c + 2], p.scale_log2, mn.z);
-            d[c + 3] = fmaf(d[c + 3], p.scale_log2, mn.w);
+          for (int c = 0; c < CW; ++c) x[c] = fmaf(fmaf(lo[c], 0.0625f, x[c]), sk, p.dr ? tl[c] : 0.f);
+        }
+        float d[CW];
+        auto exponents = [&](const float* mneg) {
+#pragma unroll
+          for (int c = 0; c < CW; c += 4) {
+            const float4 s4 = *reinterpret_cast<const float4*>(&sh->qs[hc + c]);
+            const float4 mn = mneg ? *reinterpret_cast<const float4*>(&mneg[hc + c]) : make_float4(0.f, 0.f, 0.f, 0.f);
+            d[c] = fmaf(x[c], s4.x, mn.x);
+            d[c + 1] = fmaf(x[c + 1], s4.y, mn.y);
+            d[c + 2] = fmaf(x[c + 2], s4.z, mn.z);
+            d[c + 3] = fmaf(x[c + 3], s4.w, mn.w);
           }
           if (!plain) {
-            const uint32_t al = (uint32_t)(allow >> c0);
 #pragma unroll
-            for (int c = 0; c < CB; ++c)
-              d[c] = !((al >> c) & 1u) ? -INFINITY : flag == 2 ? __uint_as_float(0x7FC00000u) : d[c];
+            for (int c = 0; c < CW; ++c)
+              d[c] = !((allow >> c) & 1u) ? -INFINITY : marked ? __uint_as_float(0x7FC00000u) : d[c];
           }
         };
-        uint8_t* pr = ps + st * 16384 + key * 128;
-        // P of this key, its sums where `add`; returns the largest exponent
-        auto weights = [&](auto add) {
-          float most = -INFINITY;
+        bool raise = i == 0;
+        if (i > 0) {
+          exponents(sh->mneg);
+          float most = d[0];
 #pragma unroll
-          for (int c0 = 0; c0 < NR; c0 += CB) {
-            float d[CB];
-            exponents(c0, d, false);
+          for (int c = 1; c < CW; ++c) most = fmaxf(most, d[c]);
+          raise = soft_any(most > TA_GROW || sk > sh->sigma);
+        }
+        if (raise) {
+          // The tile's maxima; references that they pass go up to them, and the reference of
+          // the scales to the tile's largest.
+          exponents(nullptr);
+          ta_reduce<true, CW>(d, &sh->red[quarter][hc], lane);
+          float smax = sk;
 #pragma unroll
-            for (int c = 0; c < CB; c += 8) {
-              uint32_t o[4];
-#pragma unroll
-              for (int k = 0; k < 4; ++k) {
-                most = fmaxf(most, fmaxf(d[c + 2 * k], d[c + 2 * k + 1]));
-                const float e0 = ex2f(d[c + 2 * k]), e1 = ex2f(d[c + 2 * k + 1]);
-                add(c0 + c + 2 * k, e0);
-                add(c0 + c + 2 * k + 1, e1);
-                o[k] = cvt_bf16x2(e0, e1);
-              }
-              *reinterpret_cast<uint4*>(pr + ((((c0 + c) >> 3) ^ (key & 7)) << 4)) = make_uint4(o[0], o[1], o[2], o[3]);
-            }
-          }
-          return most;
-        };
-        // The tile's maxima, and references raised to them where they pass by `limit`.
-        auto raise = [&](float limit) {
-#pragma unroll
-          for (int c0 = 0; c0 < NR; c0 += CB) {
-            float d[CB];
-            exponents(c0, d, true);
-            ta_reduce<true, CB>(d, &sh->red[warp][c0], lane);
-          }
+          for (int o = 16; o > 0; o >>= 1) smax = fmaxf(smax, __shfl_xor_sync(0xFFFFFFFFu, smax, o));
+          if (lane == 0) sh->red_s[warp] = smax;
           soft_sync();
           if (threadIdx.x < NR) {
             const int c = threadIdx.x;
             const float mo = sh->m[c];
-            const float tm = fmaxf(fmaxf(sh->red[0][c], sh->red[1][c]), fmaxf(sh->red[2][c], sh->red[3][c]));
-            const float mn = tm > mo + limit || mo == -INFINITY ? tm : mo;
+            const float tmx = fmaxf(fmaxf(sh->red[0][c], sh->red[1][c]), fmaxf(sh->red[2][c], sh->red[3][c]));
+            const float mn = tmx > mo + TA_GROW || mo == -INFINITY ? tmx + TA_HEAD : mo;
             sh->f[c] = mn == mo ? 1.f : ex2f(mo - mn);
             sh->m[c] = mn;
             sh->mneg[c] = -mn;
           }
-          soft_sync();
-        };
-        // The output's columns by the factors of a raise, once every product up to tile x is in them.
-        auto scale_output = [&](uint32_t x) {
-          mbar_wait_inl(&sh->pv_done[two ? x & 1 : 0], (two ? x >> 1 : x) & 1, wc);
-          tc_fence_after();
-#pragma unroll 1
-          for (int m = 0; m < p.dv_tiles; ++m) {
-#pragma unroll 1
-            for (int c = 0; c < NR; c += 8) {
-              uint32_t o[8];
-              tmem_ld8(tmem + o_col + m * NR + c + lane_off, o);
-              tmem_wait_ld();
-#pragma unroll
-              for (int k = 0; k < 8; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * sh->f[c + k]);
-              tmem_st8(tmem + o_col + m * NR + c + lane_off, o);
-            }
+          if (threadIdx.x == 64) {
+            const float so = sh->sigma;
+            const float sn = fmaxf(so, fmaxf(fmaxf(sh->red_s[0], sh->red_s[1]), fmaxf(sh->red_s[2], sh->red_s[3])));
+            sh->fs = so > 0.f ? so / sn : 1.f;  // (powers of two)
+            sh->sigma = sn;
           }
-          tmem_wait_st();
-        };
-        auto publish = [&] {
-          fence_proxy_async_smem();
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&sh->p_full[st]);
-        };
-        auto sums = [&](int c, float e) { l[c] += e; };
-        if (i == 0) {  // no reference yet
-          raise(0.f);
-          weights(sums);
-          publish();
-        } else {
-          const float most = weights(sums);
-          if (!soft_any(most > TA_GROW)) {
-            publish();
-          } else if (!soft_any(most > TA_MOST)) {
-            raise(TA_GROW);  // (reads the scores, so before the next ones may come)
-            publish();
+          soft_sync();
+          exponents(sh->mneg);
+          if (i > 0) {  // sums and output follow, once every product before is in it
 #pragma unroll
-            for (int c = 0; c < NR; ++c) l[c] *= sh->f[c];
-            scale_output(g);
-          } else {
-            // Take the weights out of the sums again (to 2^-24 of the weight that passes m,
-            // which becomes 1 at most; an infinite one leaves nothing worth keeping), raise m
-            // and repeat the tile.
-            auto undo = [&](int c, float e) { l[c] = l[c] == INFINITY ? 0.f : l[c] - e; };
-            weights(undo);
-            raise(TA_GROW);
+            for (int c = 0; c < CW; ++c) l[c] *= sh->f[hc + c];
+            mbar_wait_inl(&sh->pv_done, (g - 1) & 1, wc);
+            tc_fence_after();
+            float fr[CW];
+            bool same = sh->fs == 1.f;
 #pragma unroll
-            for (int c = 0; c < NR; ++c) l[c] *= sh->f[c];
-            weights(sums);
-            scale_output(g - 1);
-            publish();
+            for (int c = 0; c < CW; ++c) {
+              fr[c] = sh->f[hc + c];
+              same &= fr[c] == 1.f;
+            }
+            if (!same) {  // (the same for the whole warp)
+#pragma unroll 1
+              for (int b = 0; b < p.dt * TA_LEVELS + p.vt; ++b) {
+                const float fs = b < p.dt * TA_LEVELS ? sh->fs : 1.f;
+                float o[CW];
+                const uint32_t at = tmem + o_col + b * NR + hc + lane_off;
+                tmem_ldn<CW>(at, o);
+                tmem_wait_ld();
+#pragma unroll
+                for (int c = 0; c < CW; ++c) o[c] *= fr[c] * fs;
+                tmem_stn<CW>(at, o);
+              }
+            }
+            tmem_wait_st();
           }
         }
+        // weights, their sums, and the three codes of each
+        const float fk = marked ? 1.f : sh->sigma > 0.f ? sk * (TA_TOP / sh->sigma) : 0.f;
+        uint32_t pc[TA_LEVELS][CW / 4], pw[CW / 2];
+#pragma unroll
+        for (int c = 0; c < CW; c += 4) {
+          uint16_t q2[TA_LEVELS][2];
+#pragma unroll
+          for (int z = 0; z < 2; ++z) {
+            const float e0 = ex2f(d[c + 2 * z]), e1 = ex2f(d[c + 2 * z + 1]);
+            l[c + 2 * z] += e0;
+            l[c + 2 * z + 1] += e1;
+            pw[c / 2 + z] = cvt_bf16x2(e0, e1);
+            uint32_t h;
+            asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(h) : "f"(e1 * fk), "f"(e0 * fk));
+#pragma unroll
+            for (int v = 0; v < TA_LEVELS; ++v) q2[v][z] = ta_split(h);
+          }
+#pragma unroll
+          for (int v = 0; v < TA_LEVELS; ++v) pc[v][c / 4] = (uint32_t)q2[v][0] | ((uint32_t)q2[v][1] << 16);
+        }
+        // the previous tile's product has read P
+        if (g > 0) mbar_wait_inl(&sh->pv_done, (g - 1) & 1, wc);
+#pragma unroll
+        for (int v = 0; v < TA_LEVELS; ++v) {
+          const int byte = v * NR + hc;
+          uint8_t* at = ps + key * 128 + (((byte >> 4) ^ (key & 7)) << 4) + (byte & 15);
+          if constexpr (CW == 16) *reinterpret_cast<uint4*>(at) = make_uint4(pc[v][0], pc[v][1], pc[v][2], pc[v][3]);
+          else *reinterpret_cast<uint2*>(at) = make_uint2(pc[v][0], pc[v][1]);
+        }
+        if (p.vt) {
+#pragma unroll
+          for (int c = 0; c < CW; c += 8)
+            *reinterpret_cast<uint4*>(pb + key * 64 + ((((hc + c) >> 3) ^ ((key >> 1) & 3)) << 4)) =
+                make_uint4(pw[c / 2], pw[c / 2 + 1], pw[c / 2 + 2], pw[c / 2 + 3]);
+        }
+        fence_proxy_async_smem();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sh->p_full);
       }
-      // the row tile's part is complete
+      // ---- the row tile's part is complete
       {
-        const uint32_t lg = g - 1;
-        ta_reduce<false, NR>(l, sh->red[warp], lane);
+        ta_reduce<false, CW>(l, &sh->red[quarter][hc], lane);
         soft_sync();
         // a part of a longer row tile: the head of it, or a later piece
         const int slot = 2 * (int)blockIdx.x + (w.t == 0 ? 1 : 0);
@@ -719,9 +760,14 @@ __global__ void __launch_bounds__(TA_THREADS, 1)
             sh->f[c] = sum == 0.f ? 0.f : 1.f / sum;
           } else {
             *reinterpret_cast<float2*>(p.part_ml + ((int64_t)slot * NR + c) * 2) = make_float2(m, sum);
+            sh->f[c] = 1.f;
           }
           sh->m[c] = -INFINITY;
           sh->mneg[c] = INFINITY;
+        }
+        if (threadIdx.x == 64) {
+          sh->fs = sh->sigma * (1.f / TA_TOP);  // what a unit of P stands for
+          sh->sigma = 0.f;
         }
         if (!whole && threadIdx.x == 0 && w.t == 0) {
           int32_t* ow = p.owner + (int64_t)blockIdx.x * 4;
@@ -731,34 +777,43 @@ __global__ void __launch_bounds__(TA_THREADS, 1)
           ow[2] = 1 + (int)((w.nt - n + sh->per - 1) / sh->per);
         }
         soft_sync();
-        mbar_wait_inl(&sh->pv_done[two ? lg & 1 : 0], (two ? lg >> 1 : lg) & 1, wc);
+        mbar_wait_inl(&sh->pv_done, (g - 1) & 1, wc);
         tc_fence_after();
-        for (int m = 0; m < p.dv_tiles; ++m) {
-          const int dim = m * 128 + key;
+        const float unit = sh->fs;
+        auto store = [&](int dim, const float (&o)[CW]) {
+          if (whole) {
+            uint16_t* op = p.out + ((int64_t)w.b * p.rows + r0 + hc) * p.dv + dim;
 #pragma unroll
-          for (int c0 = 0; c0 < NR; c0 += CB) {
-            uint32_t o[CB];
-            tmem_ldn<CB>(tmem + o_col + m * NR + c0 + lane_off, o);
-            tmem_wait_ld();
-            if (dim < p.dv) {
-              if (whole) {
-                uint16_t* op = p.out + ((int64_t)w.b * p.rows + r0 + c0) * p.dv + dim;
+            for (int c = 0; c < CW; ++c)
+              if (hc + c < nrows)
+                op[(int64_t)c * p.dv] = __bfloat16_as_ushort(__float2bfloat16_rn(o[c] * sh->f[hc + c]));
+          } else {
+            float* op = p.part_o + ((int64_t)slot * NR + hc) * p.dv + dim;
 #pragma unroll
-                for (int c = 0; c < CB; ++c)
-                  if (c0 + c < nrows)
-                    op[(int64_t)c * p.dv] =
-                        __bfloat16_as_ushort(__float2bfloat16_rn(__uint_as_float(o[c]) * sh->f[c0 + c]));
-              } else {
-                float* op = p.part_o + ((int64_t)slot * NR + c0) * p.dv + dim;
-#pragma unroll
-                for (int c = 0; c < CB; ++c)
-                  if (c0 + c < nrows) op[(int64_t)c * p.dv] = __uint_as_float(o[c]);
-              }
-            }
+            for (int c = 0; c < CW; ++c)
+              if (hc + c < nrows) op[(int64_t)c * p.dv] = o[c];
           }
+        };
+#pragma unroll 1
+        for (int m = 0; m < p.dt; ++m) {
+          float o[CW], o1[CW], o2[CW];
+          const uint32_t at = tmem + o_col + m * NP + hc + lane_off;
+          tmem_ldn<CW>(at, o);
+          tmem_ldn<CW>(at + NR, o1);
+          tmem_ldn<CW>(at + 2 * NR, o2);
+          tmem_wait_ld();
+#pragma unroll
+          for (int c = 0; c < CW; ++c) o[c] = fmaf(fmaf(o2[c], 0.0625f, o1[c]), 0.0625f, o[c]) * unit;
+          if (m * 128 + key < min(p.dv, p.dq)) store(m * 128 + key, o);
+        }
+        if (p.vt) {
+          float o[CW];
+          tmem_ldn<CW>(tmem + ot_col + hc + lane_off, o);
+          tmem_wait_ld();
+          if (p.dq + key < p.dv) store(p.dq + key, o);
         }
         tc_fence_before();
-        soft_sync();  // f is read by all before the next item's raises
+        soft_sync();  // f and qs are read by all before the next item's
       }
       w.next_item(p, n);
     }
