@@ -13,15 +13,15 @@
 // and on the cache's own e4m3 codes (tcgen05 kind::f8f6f4): a code tile is loaded once, by
 // TMA where the pages allow, and read K-major by the first product and MN-major (dims
 // contiguous) by the second.  Nothing is expanded.  What meets the codes is split into
-// e4m3 numbers, several columns per row:
+// 8-bit numbers, several columns per row:
 //   * a query element is 8 significant bits of bf16: q 2^-e = hi + lo / 16 exactly, hi and
 //     lo with 4 bits each (e: the row's exponent, hi below 256; elements under 2^-14 of the
 //     row's largest lose bits below 2^-21 of it).  S = S_hi + S_lo / 16.
-//   * a weight is taken to fp16 (11 bits) and split into three: P = P0 + P1 / 16 + P2 / 256,
-//     each product in columns of its own, joined at the end.  Off by 2^-12 of the weight,
-//     or 2^-24 of the row's largest weight where that is more (a bf16 weight: 2^-8).
+//   * a weight is split into three e5m2 numbers of 3 bits each: P = P0 + P1 / 8 + P2 / 64,
+//     each product in columns of its own, joined at the end.  Off by at most 2^-9 of the
+//     weight (a bf16 weight: 2^-8), or 2^-33 of a weight of 1 where that is more.
 // A key's scale multiplies its scores (thread = key) and its weight, the latter relative to
-// the largest scale seen, so that P keeps within e4m3's range.  The rotary columns are bf16
+// the largest scale seen, so that P keeps within e5m2's range.  The rotary columns are bf16
 // and have a bf16 product of their own; where v reaches into them (dv > dq), so do they.
 //
 // Why split: with bf16 operands every tile's codes are expanded in shared memory, 147 KB
@@ -45,7 +45,9 @@
 // meets a zero weight.
 //
 // Softmax: p = 2^(s - m) with a reference m that is raised only when a score passes it by
-// TA_GROW (one vote per tile), together with sum and output; sums are kept per thread in
+// TA_GROW (one vote per tile: about a tenth of the tiles of N(0, 1) data with a limit of 3,
+// and the raise costs more than a tile, so the limit is what e5m2's range allows), together
+// with sum and output; sums are kept per thread in
 // fp32 and reduced once per row tile.
 #pragma once
 #include "latent_cache.cuh"
@@ -63,10 +65,11 @@ constexpr int TA_MAX_ROWS = 32;
 constexpr int TA_STAGES = 4;                 // most code tiles in shared memory
 constexpr int TA_AHEAD = 4;                  // tiles whose addresses are held
 constexpr int TA_HDR = 6144;
-constexpr int TA_LEVELS = 3;                 // e4m3 columns per weight
-constexpr float TA_GROW = 2.f;               // how far a score may pass m (base 2)
+constexpr int TA_LEVELS = 3;                 // e5m2 columns per weight
+constexpr float TA_STEP = 8.f;               // each is this much finer than the one before
+constexpr float TA_GROW = 5.f;               // how far a score may pass m (base 2)
 constexpr float TA_HEAD = 1.f;               // a raised m lies this far above the score
-constexpr float TA_TOP = 64.f;               // P of a weight of 1 at the largest scale: 64 * 2^TA_GROW < 448
+constexpr float TA_TOP = 1024.f;             // P of a weight of 1 at the largest scale: 2^(10 + TA_GROW) < 57344
 
 struct TreeAttnParams {
   const uint16_t* q;      // bf16 [B, T * H, dq + dr]
@@ -99,7 +102,8 @@ struct TreeAttnParams {
 };
 
 struct TaShared {
-  uint64_t full[TA_STAGES], kfree[TA_STAGES];   // a tile's rows are in place / have been used
+  uint64_t full[TA_STAGES];                     // a tile's rows are in place
+  uint64_t kfree[TA_STAGES][5];                 // a chunk of it (4: the tail) has been used
   uint64_t s_full[2], s_free[2];                // scores are in TMEM / in registers
   uint64_t p_full, pv_done;                     // weights are in shared memory / have been used
   uint64_t a_full[TA_AHEAD], a_free[TA_AHEAD];  // a tile's addresses and scales
@@ -225,6 +229,11 @@ __device__ __forceinline__ void ta_reduce(const float (&v)[CW], float* red, int 
   if ((lane & 1) == 0 && (lane >> 1) < CW) red[lane >> 1] = r;
 }
 
+// Bytes that the current phase of `bar` also waits for (no arrival).
+__device__ __forceinline__ void mbar_add_tx(uint64_t* bar, uint32_t bytes) {
+  asm volatile("mbarrier.expect_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(bar)), "r"(bytes) : "memory");
+}
+
 // MN-major operand of 64-byte rows (32 bf16) with the 64-byte swizzle: 16-byte unit u of
 // row r lies at u ^ ((r >> 1) & 3); 8 rows are 512 bytes.
 __device__ __forceinline__ uint64_t sdesc_sw64(uint32_t saddr) {
@@ -237,12 +246,13 @@ __device__ __forceinline__ uint32_t f16x2_of_e4m3x2(uint16_t c) {
   asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"(c));
   return h;
 }
-// Two fp16 as e4m3 (lo in bits 0-7); `h` becomes 16 times what that leaves (exact).
+// Two fp16 as e5m2 (lo in bits 0-7; the high byte of an fp16); `h` becomes TA_STEP = 8
+// times what that leaves (exact).
 __device__ __forceinline__ uint16_t ta_split(uint32_t& h) {
   uint16_t c;
-  asm("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;" : "=h"(c) : "r"(h));
-  const uint32_t b = f16x2_of_e4m3x2(c);
-  asm("{ .reg .b32 t; sub.rn.f16x2 t, %0, %1; mul.rn.f16x2 %0, t, %2; }" : "+r"(h) : "r"(b), "r"(0x4C004C00u));
+  asm("cvt.rn.satfinite.e5m2x2.f16x2 %0, %1;" : "=h"(c) : "r"(h));
+  const uint32_t b = __byte_perm(c, 0, 0x1404);
+  asm("{ .reg .b32 t; sub.rn.f16x2 t, %0, %1; mul.rn.f16x2 %0, t, %2; }" : "+r"(h) : "r"(b), "r"(0x48004800u));
   return c;
 }
 
@@ -266,7 +276,7 @@ __global__ void __launch_bounds__(TA_THREADS, 1)
   if (threadIdx.x == 0) {
     for (int s = 0; s < TA_STAGES; ++s) {
       mbar_init(&sh->full[s], TA_LOADERS);
-      mbar_init(&sh->kfree[s], 1);
+      for (int c = 0; c < 5; ++c) mbar_init(&sh->kfree[s][c], 1);
     }
     for (int s = 0; s < 2; ++s) {
       mbar_init(&sh->s_full[s], 1);
@@ -355,28 +365,39 @@ __global__ void __launch_bounds__(TA_THREADS, 1)
     uint32_t sent = 0, sent_ph = 0;  // stages whose latest load is by TMA, and its phase
     bool ok = true;
     for (int u = 0; u < w.left && ok; ++u, st.next(p.stages), ad.next(TA_AHEAD)) {
-      ok = mbar_wait_inl(&sh->a_full[ad.i], ad.ph, wc) && ok;
-      const bool whole = p.box && sh->whole[ad.i];
-      ok = mbar_wait_inl(&sh->kfree[st.i], st.ph ^ 1, wc) && ok;
+      ok = __all_sync(0xFFFFFFFFu, mbar_wait_inl(&sh->a_full[ad.i], ad.ph, wc));
       if (!ok) break;
+      const bool whole = p.box && sh->whole[ad.i];
+      // chunk c (nc: the tail) of the stage has been read: the second product's dim tiles
+      // free theirs one by one, chunks that only the first reads go with its end
+      auto chunk_free = [&](int c) { return mbar_wait_inl(&sh->kfree[st.i][c == p.nc ? 4 : c], st.ph ^ 1, wc); };
       uint8_t* tile = ks_ + (size_t)st.i * p.stage_bytes;
       const int32_t* sl = sh->slot[ad.i];
       if (whole) {
-        if (lw == 0 && elect_one()) {
-          mbar_expect_tx(&sh->full[st.i], p.stage_bytes);
-          for (int r = 0; r < 128; r += p.box) {
-            const int y = sl[r];
-            for (int c = 0; c < p.nc; ++c) tma_load_2d(&km, &sh->full[st.i], tile + c * 16384 + r * 128, c * 128, y);
-            if (p.dr) tma_load_2d(&tm, &sh->full[st.i], tile + p.nc * 16384 + r * 128, 0, y);
-          }
-        } else if (lw != 0 && lane == 0) {
+        // A warp per chunk, the tail with warp nc % 4.  Nothing arrives for this use of the
+        // stage before a part of it is free, when the last use's loads have landed.
+        if (elect_one()) {
+          const bool chunk = lw < p.nc, tail = p.dr && lw == (p.nc & 3);
+          auto fetch = [&](int c, const CUtensorMap* map, int x) {
+            ok = chunk_free(c) && ok;
+            mbar_add_tx(&sh->full[st.i], 16384);
+            for (int r = 0; r < 128; r += p.box) tma_load_2d(map, &sh->full[st.i], tile + c * 16384 + r * 128, x, sl[r]);
+          };
+          if (tail && !p.vt) fetch(p.nc, &tm, 0);
+          if (chunk) fetch(lw, &km, lw * 128);
+          if (tail && p.vt) fetch(p.nc, &tm, 0);
+          if (!chunk && !tail) ok = chunk_free(0) && ok;
           mbar_arrive(&sh->full[st.i]);
         }
-        __syncwarp();
+        ok = __all_sync(0xFFFFFFFFu, ok);
         sent |= 1u << st.i;
         sent_ph = (sent_ph & ~(1u << st.i)) | st.ph << st.i;
       } else {
         sent &= ~(1u << st.i);
+        for (int c = 0; c <= p.nc; ++c)
+          if (c < p.nc || p.dr) ok = chunk_free(c) && ok;
+        ok = __all_sync(0xFFFFFFFFu, ok);
+        if (!ok) break;
         for (int i = 0; i < 8; ++i) {  // 8 lanes per row: 128 bytes of it at a time
           const int key = lw * 32 + i * 4 + (lane >> 3), s = sl[key];
           const uint8_t* src = p.kv8 + (int64_t)max(s, 0) * p.dq + piece * 16;
@@ -396,7 +417,7 @@ __global__ void __launch_bounds__(TA_THREADS, 1)
       if (lane == 0) mbar_arrive(&sh->a_free[ad.i]);
     }
     // after a timed-out wait: no load of this CTA may land once it has gone
-    if (lw == 0 && *wc.abort)
+    if (*wc.abort)
       for (int s = 0; s < TA_STAGES; ++s)
         if (sent >> s & 1) mbar_wait(&sh->full[s], sent_ph >> s & 1, wc, false, true);
   } else if (warp == TA_W_ADDR) {
@@ -419,7 +440,7 @@ __global__ void __launch_bounds__(TA_THREADS, 1)
         }
         whole &= s[i] >= 0;
       }
-      ok = mbar_wait_inl(&sh->a_free[ad.i], ad.ph ^ 1, wc);
+      ok = __all_sync(0xFFFFFFFFu, mbar_wait_inl(&sh->a_free[ad.i], ad.ph ^ 1, wc));
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         sh->slot[ad.i][i * 32 + lane] = s[i];
@@ -434,68 +455,91 @@ __global__ void __launch_bounds__(TA_THREADS, 1)
     // ================================================================ MMA issue
     if (elect_one()) {
       const uint32_t id_qk = idesc_e4m3_f32(128, 2 * NR), id_qt = idesc_bf16_f32(128, NR, false, false);
-      const uint32_t id_pv = idesc_e4m3_f32(128, NP) | (1u << 15) | (1u << 16), id_pt = idesc_bf16_f32(128, NR, true, true);
+      const uint32_t id_pv = idesc_e4m3_f32(128, NP) | (1u << 10) | (1u << 15) | (1u << 16), id_pt = idesc_bf16_f32(128, NR, true, true);
       // descriptors: only the start address (low word, 16-byte units) changes
       const uint64_t k_desc = sdesc_sw128(smem_u32(ks_), 16, 1024), q_desc = sdesc_sw128(smem_u32(qs), 16, 1024);
       const uint64_t v_desc = sdesc_sw128(smem_u32(ks_), 16384, 1024), p_desc = sdesc_sw128(smem_u32(ps), 16, 1024);
       const uint64_t pb_desc = sdesc_sw64(smem_u32(pb));
       const uint32_t stage16 = p.stage_bytes >> 4;
       TaRing kq, kp, sq;  // code tile of the next QK and of the next PV; score buffer
-      uint32_t n_pv = 0, items = 0;
-      bool ok = true;
       auto qk = [&] {
-        ok = mbar_wait_inl(&sh->full[kq.i], kq.ph, wc) && mbar_wait_inl(&sh->s_free[sq.i], sq.ph ^ 1, wc);
-        if (!ok) return;
         tc_fence_after();
         const uint32_t d = tmem + sq.i * 3 * NR;
         const uint64_t a = k_desc + kq.i * stage16;
-        for (int c = 0; c < p.nc; ++c) {
-#pragma unroll
-          for (int k = 0; k < 4; ++k)
-            umma_f8_ss(d, a + c * 1024 + k * 2, q_desc + c * (2 * NR * 8) + k * 2, id_qk, c > 0 || k > 0 ? 1u : 0u);
-        }
         if (p.dr) {
 #pragma unroll
           for (int k = 0; k < 4; ++k)
             umma_bf16_ss(d + 2 * NR, a + p.nc * 1024 + k * 2, q_desc + p.nc * (2 * NR * 8) + k * 2, id_qt, k > 0 ? 1u : 0u);
         }
+        for (int c = 0; c < p.nc; ++c) {
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            umma_f8_ss(d, a + c * 1024 + k * 2, q_desc + c * (2 * NR * 8) + k * 2, id_qk, c > 0 || k > 0 ? 1u : 0u);
+        }
         umma_commit(&sh->s_full[sq.i]);
+        for (int c = p.dt; c < p.nc; ++c) umma_commit(&sh->kfree[kq.i][c]);
+        if (p.dr && !p.vt) umma_commit(&sh->kfree[kq.i][4]);
         kq.next(p.stages);
         sq.next(p.s_bufs);
       };
       auto pv = [&](bool first) {
-        ok = mbar_wait_inl(&sh->p_full, n_pv & 1, wc);
-        if (!ok) return;
-        ++n_pv;
         tc_fence_after();
         const uint64_t a = v_desc + kp.i * stage16;
         for (int m = 0; m < p.dt; ++m) {
 #pragma unroll
           for (int k = 0; k < 4; ++k)  // 32 keys: 4096 bytes further in both
             umma_f8_ss(tmem + o_col + m * NP, a + m * 1024 + k * 256, p_desc + k * 256, id_pv, !first || k > 0 ? 1u : 0u);
+          umma_commit(&sh->kfree[kp.i][m]);
         }
         if (p.vt) {  // 64 dims (the other 64 lanes hold what lies behind them, unused)
 #pragma unroll
           for (int k = 0; k < 8; ++k)  // 16 keys: 2048 and 1024 bytes further
             umma_bf16_ss(tmem + ot_col, a + p.nc * 1024 + k * 128, pb_desc + k * 64, id_pt, !first || k > 0 ? 1u : 0u);
+          umma_commit(&sh->kfree[kp.i][4]);
         }
-        umma_commit(&sh->kfree[kp.i]);
         umma_commit(&sh->pv_done);
         kp.next(p.stages);
       };
-      while (w.left > 0 && ok) {
-        const int n = w.here();
-        ok = mbar_wait_inl(&sh->q_full, items & 1, wc);
-        if (ok) {
-          tc_fence_after();
+      // Scores and outputs in the order in which their inputs come: a tile's scores may run
+      // ahead of the one before's output, which need not wait for a tile that still loads.
+      TaWalk wp = w;                                    // of the next PV
+      int q_here = w.left > 0 ? w.here() : 0, q_at = 0;  // of the item: its units, QKs issued
+      int p_here = q_here, p_at = 0;
+      uint32_t items = 0, n_pv = 0;
+      uint64_t t0 = clock64();
+      const uint64_t lim = budget_cycles(p.budget_ns);
+      while (wp.left > 0) {
+        bool did = false;
+        if (mbar_poll(smem_u32(&sh->p_full), n_pv & 1)) {
+          pv(p_at == 0);
+          did = true;
+          ++n_pv;
+          if (++p_at == p_here) {
+            wp.next_item(p, p_here);
+            p_at = 0;
+            p_here = wp.left > 0 ? wp.here() : 0;
+          }
+        }
+        if (w.left > 0 && (q_at > 0 || mbar_poll(smem_u32(&sh->q_full), items & 1)) &&
+            mbar_poll(smem_u32(&sh->s_free[sq.i]), sq.ph ^ 1) && mbar_poll(smem_u32(&sh->full[kq.i]), kq.ph)) {
           qk();
+          did = true;
+          if (++q_at == q_here) {
+            w.next_item(p, q_here);
+            q_at = 0;
+            ++items;
+            q_here = w.left > 0 ? w.here() : 0;
+          }
         }
-        for (int i = 0; i < n && ok; ++i) {  // the next tile's scores while this one's weights are made
-          if (i + 1 < n) qk();
-          if (ok) pv(i == 0);
+        if (did) {
+          t0 = clock64();
+        } else {
+          if (*wc.abort) break;
+          if ((uint64_t)clock64() - t0 > lim) {
+            raise_timeout(wc, smem_u32(&sh->p_full), n_pv & 1);
+            break;
+          }
         }
-        ++items;
-        w.next_item(p, n);
       }
       // nothing of this CTA is in flight when it gives its memory back
       umma_commit(&sh->drain);
@@ -511,27 +555,29 @@ __global__ void __launch_bounds__(TA_THREADS, 1)
     const uint32_t lane_off = (uint32_t)(quarter * 32) << 16;
     TaRing sq, ad;
     uint32_t g = 0;  // tiles so far: pv_done's phase g - 1 is the last tile's product
-    while (w.left > 0) {
-      const int n = w.here();
-      const int r0 = w.rt * NR;                      // first row of the tile in the sequence
-      const int nrows = min(NR, p.rows - r0);
-      const bool whole = w.t == 0 && n == w.nt;      // no other CTA has a part
-      // ---- the item's queries: hi and lo codes, bf16 tail
-#pragma unroll 1
-      for (int i = 0; i < NR / 8; ++i) {
-        const int row = warp * (NR / 8) + i;
-        const uint16_t* q = p.q + ((int64_t)w.b * p.rows + r0 + row) * (p.dq + p.dr);
-        const bool in = row < nrows && lane * 16 < p.dq;
-        uint32_t x[8], t[4];
-        *reinterpret_cast<uint4*>(x) = ldcg_or_zero(q + lane * 16, in);
-        *reinterpret_cast<uint4*>(x + 4) = ldcg_or_zero(q + lane * 16 + 8, in);
-        *reinterpret_cast<uint4*>(t) = ldcg_or_zero(q + p.dq + lane * 8, row < nrows && lane * 8 < p.dr);
+    // The queries of item x: hi and lo codes and the bf16 tail, scaled by a power of two
+    // per row.  The last scores of the item before are in registers.
+    auto queries = [&](const TaWalk& x) {
+      constexpr int RW = NR / 8;  // rows of a warp
+      const int first = x.rt * NR + warp * RW;
+      uint32_t v[RW][8], t[RW][4];
+#pragma unroll
+      for (int i = 0; i < RW; ++i) {
+        const bool in = first + i < p.rows;
+        const uint16_t* q = p.q + ((int64_t)x.b * p.rows + first + i) * (p.dq + p.dr);
+        *reinterpret_cast<uint4*>(v[i]) = ldcg_or_zero(q + lane * 16, in && lane * 16 < p.dq);
+        *reinterpret_cast<uint4*>(v[i] + 4) = ldcg_or_zero(q + lane * 16 + 8, in && lane * 16 < p.dq);
+        *reinterpret_cast<uint4*>(t[i]) = ldcg_or_zero(q + p.dq + lane * 8, in && lane * 8 < p.dr);
+      }
+#pragma unroll
+      for (int i = 0; i < RW; ++i) {
+        const int row = warp * RW + i;
         float amax = 0.f;
         bool bad = false;
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
-          amax = fmaxf(amax, fmaxf(fabsf(bf16lo_f32(x[k])), fabsf(bf16hi_f32(x[k]))));
-          bad |= bf16x2_nonfinite(x[k]);
+          amax = fmaxf(amax, fmaxf(fabsf(bf16lo_f32(v[i][k])), fabsf(bf16hi_f32(v[i][k]))));
+          bad |= bf16x2_nonfinite(v[i][k]);
         }
         bad = __any_sync(0xFFFFFFFFu, bad);
 #pragma unroll
@@ -545,7 +591,7 @@ __global__ void __launch_bounds__(TA_THREADS, 1)
           uint32_t h2 = 0, l2 = 0;
 #pragma unroll
           for (int z = 0; z < 2; ++z) {
-            const float a = bf16lo_f32(x[2 * k + z]) * inv, b = bf16hi_f32(x[2 * k + z]) * inv;
+            const float a = bf16lo_f32(v[i][2 * k + z]) * inv, b = bf16hi_f32(v[i][2 * k + z]) * inv;
             const uint16_t h = cvt_e4m3x2(a, b);
             const uint32_t back = f16x2_of_e4m3x2(h);
             const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&back));
@@ -564,14 +610,22 @@ __global__ void __launch_bounds__(TA_THREADS, 1)
         if (lane * 8 < p.dr) {
           const uint32_t m2 = (uint32_t)(127 - e) * 0x00800080u;
           *reinterpret_cast<uint4*>(qs + p.nc * (2 * NR * 128) + row * 128 + ((lane ^ (row & 7)) << 4)) =
-              make_uint4(mul_bf16x2(t[0], m2), mul_bf16x2(t[1], m2), mul_bf16x2(t[2], m2), mul_bf16x2(t[3], m2));
+              make_uint4(mul_bf16x2(t[i][0], m2), mul_bf16x2(t[i][1], m2), mul_bf16x2(t[i][2], m2),
+                         mul_bf16x2(t[i][3], m2));
         }
         if (lane == 0) sh->qs[row] = __uint_as_float((uint32_t)(127 + e) << 23) * p.scale_log2;
       }
       fence_proxy_async_smem();
-      soft_sync();
+      __syncwarp();
       if (lane == 0) mbar_arrive(&sh->q_full);
-
+    };
+    if (w.left > 0) queries(w);
+    soft_sync();
+    while (w.left > 0) {
+      const int n = w.here();
+      const int r0 = w.rt * NR;                      // first row of the tile in the sequence
+      const int nrows = min(NR, p.rows - r0);
+      const bool whole = w.t == 0 && n == w.nt;      // no other CTA has a part
       float l[CW];
 #pragma unroll
       for (int c = 0; c < CW; ++c) l[c] = 0.f;
@@ -704,7 +758,7 @@ __global__ void __launch_bounds__(TA_THREADS, 1)
             tmem_wait_st();
           }
         }
-        // weights, their sums, and the three codes of each
+        // weights, their sums, and the three parts of each
         const float fk = marked ? 1.f : sh->sigma > 0.f ? sk * (TA_TOP / sh->sigma) : 0.f;
         uint32_t pc[TA_LEVELS][CW / 4], pw[CW / 2];
 #pragma unroll
@@ -748,6 +802,9 @@ __global__ void __launch_bounds__(TA_THREADS, 1)
       {
         ta_reduce<false, CW>(l, &sh->red[quarter][hc], lane);
         soft_sync();
+        TaWalk x = w;
+        x.next_item(p, n);
+        if (x.left > 0) queries(x);  // their first scores run during this epilogue
         // a part of a longer row tile: the head of it, or a later piece
         const int slot = 2 * (int)blockIdx.x + (w.t == 0 ? 1 : 0);
         if (threadIdx.x < NR) {
@@ -803,7 +860,7 @@ __global__ void __launch_bounds__(TA_THREADS, 1)
           tmem_ldn<CW>(at + 2 * NR, o2);
           tmem_wait_ld();
 #pragma unroll
-          for (int c = 0; c < CW; ++c) o[c] = fmaf(fmaf(o2[c], 0.0625f, o1[c]), 0.0625f, o[c]) * unit;
+          for (int c = 0; c < CW; ++c) o[c] = fmaf(fmaf(o2[c], 1.f / TA_STEP, o1[c]), 1.f / TA_STEP, o[c]) * unit;
           if (m * 128 + key < min(p.dv, p.dq)) store(m * 128 + key, o);
         }
         if (p.vt) {
