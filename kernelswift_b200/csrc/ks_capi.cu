@@ -597,12 +597,12 @@ int table_check(const char* op, const int32_t* table, int64_t max_pages, const i
 // take fewer columns of every product where there are no more.
 int ta_rows(int64_t rows) { return rows <= 16 ? 16 : 32; }
 
-template <int NR>
+template <int NR, bool VT>
 int launch_tree_attn(Device* dev, const CUtensorMap& km, const CUtensorMap& tm, const TreeAttnParams& p, unsigned grid,
                      size_t smem, cudaStream_t st) {
-  if (int rc = smem_optin(dev, reinterpret_cast<const void*>(tree_attn_kernel<NR>), "cudaFuncSetAttribute(tree_attn)"))
+  if (int rc = smem_optin(dev, reinterpret_cast<const void*>(tree_attn_kernel<NR, VT>), "cudaFuncSetAttribute(tree_attn)"))
     return rc;
-  tree_attn_kernel<NR><<<grid, TA_THREADS, smem, st>>>(km, tm, p);
+  tree_attn_kernel<NR, VT><<<grid, TA_THREADS, smem, st>>>(km, tm, p);
   if (int rc = launch_check("tree_attn_kernel launch")) return rc;
   tree_attn_join_kernel<NR><<<dim3(grid, NR), TA_JOIN_THREADS, 0, st>>>(p);
   return launch_check("tree_attn_join_kernel launch");
@@ -1010,11 +1010,11 @@ int ks_tree_attn(const void* q, const void* kv8, const float* kv_scale, const vo
   p.row_tiles = (p.rows + nr - 1) / nr;
   p.nc = (dq + 127) / 128;
   p.dt = (int)((std::min<int64_t>(dv, dq) + 127) / 128);
-  p.vt = dv > dq;
+  const bool vt = dv > dq;  // v reaches into the bf16 columns
   // shared memory: as many code tiles as fit (two at D = 576)
   p.stage_bytes = (uint32_t)(p.nc + (dr ? 1 : 0)) * 16384;
   const size_t q_bytes = (size_t)p.nc * 2 * nr * 128 + (dr ? (size_t)nr * 128 : 0);
-  const size_t fixed = 1024 + TA_HDR + q_bytes + 16384 + (p.vt ? 8192 : 0);
+  const size_t fixed = 1024 + TA_HDR + q_bytes + 16384 + (vt ? 8192 : 0);
   p.stages = (int)std::min<size_t>((232448 - fixed) / p.stage_bytes, TA_STAGES);
   if (p.stages < 1) return fail(KS_ERR_UNSUPPORTED, "tree_attn: shared memory too small");
   p.k_off = TA_HDR;
@@ -1022,7 +1022,7 @@ int ks_tree_attn(const void* q, const void* kv8, const float* kv_scale, const vo
   p.p_off = p.q_off + (uint32_t)q_bytes;
   p.pb_off = p.p_off + 16384;
   const size_t smem = fixed + (size_t)p.stages * p.stage_bytes;
-  const int o_cols = p.dt * TA_LEVELS * nr + (p.vt ? nr : 0);
+  const int o_cols = p.dt * TA_LEVELS * nr + (vt ? nr : 0);
   p.s_bufs = o_cols + 2 * 3 * nr <= 512 ? 2 : 1;
   p.tmem_cols = 32;
   while ((int)p.tmem_cols < o_cols + p.s_bufs * 3 * nr) p.tmem_cols <<= 1;
@@ -1048,8 +1048,11 @@ int ks_tree_attn(const void* q, const void* kv8, const float* kv_scale, const vo
       if (int rc = make_map_bf16(&tm, kv_tail, 64, slots, 128, 64, (uint32_t)p.box)) return rc;
   }
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (nr == 16) return launch_tree_attn<16>(dev, km, tm, p, grid, smem, st);
-  return launch_tree_attn<32>(dev, km, tm, p, grid, smem, st);
+  if (nr == 16)
+    return vt ? launch_tree_attn<16, true>(dev, km, tm, p, grid, smem, st)
+              : launch_tree_attn<16, false>(dev, km, tm, p, grid, smem, st);
+  return vt ? launch_tree_attn<32, true>(dev, km, tm, p, grid, smem, st)
+            : launch_tree_attn<32, false>(dev, km, tm, p, grid, smem, st);
 }
 
 int ks_verify_draft(const float* p, const float* q, const void* tokens, int32_t token_dtype,

@@ -17,9 +17,10 @@
 //   * a query element is 8 significant bits of bf16: q 2^-e = hi + lo / 16 exactly, hi and
 //     lo with 4 bits each (e: the row's exponent, hi below 256; elements under 2^-14 of the
 //     row's largest lose bits below 2^-21 of it).  S = S_hi + S_lo / 16.
-//   * a weight is split into three e5m2 numbers of 3 bits each: P = P0 + P1 / 8 + P2 / 64,
-//     each product in columns of its own, joined at the end.  Off by at most 2^-9 of the
-//     weight (a bf16 weight: 2^-8), or 2^-33 of a weight of 1 where that is more.
+//   * a weight is taken to fp16 and split into three e5m2 numbers of 3 bits each, the high
+//     bytes of P, P - P0 and P - P0 - P1 as fp16, each product in columns of its own and
+//     the three added at the end.  Off by at most 2^-9 of the weight (a bf16 weight:
+//     2^-8), or 2^-27 of a weight of 1 where that is more.
 // A key's scale multiplies its scores (thread = key) and its weight, the latter relative to
 // the largest scale seen, so that P keeps within e5m2's range.  The rotary columns are bf16
 // and have a bf16 product of their own; where v reaches into them (dv > dq), so do they.
@@ -66,7 +67,6 @@ constexpr int TA_STAGES = 4;                 // most code tiles in shared memory
 constexpr int TA_AHEAD = 4;                  // tiles whose addresses are held
 constexpr int TA_HDR = 6144;
 constexpr int TA_LEVELS = 3;                 // e5m2 columns per weight
-constexpr float TA_STEP = 8.f;               // each is this much finer than the one before
 constexpr float TA_GROW = 5.f;               // how far a score may pass m (base 2)
 constexpr float TA_HEAD = 1.f;               // a raised m lies this far above the score
 constexpr float TA_TOP = 1024.f;             // P of a weight of 1 at the largest scale: 2^(10 + TA_GROW) < 57344
@@ -88,7 +88,6 @@ struct TreeAttnParams {
   int32_t row_tiles;      // ceil(rows / NR)
   int32_t nc;             // 128-column chunks of codes
   int32_t dt;             // 128-dim tiles of O^T from codes
-  int32_t vt;             // 1: v reaches into the bf16 columns
   int32_t stages, s_bufs;
   int32_t box;            // rows of a TMA box, 0: no TMA
   uint32_t stage_bytes, k_off, q_off, p_off, pb_off;
@@ -246,17 +245,40 @@ __device__ __forceinline__ uint32_t f16x2_of_e4m3x2(uint16_t c) {
   asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"(c));
   return h;
 }
-// Two fp16 as e5m2 (lo in bits 0-7; the high byte of an fp16); `h` becomes TA_STEP = 8
-// times what that leaves (exact).
-__device__ __forceinline__ uint16_t ta_split(uint32_t& h) {
-  uint16_t c;
-  asm("cvt.rn.satfinite.e5m2x2.f16x2 %0, %1;" : "=h"(c) : "r"(h));
-  const uint32_t b = __byte_perm(c, 0, 0x1404);
-  asm("{ .reg .b32 t; sub.rn.f16x2 t, %0, %1; mul.rn.f16x2 %0, t, %2; }" : "+r"(h) : "r"(b), "r"(0x48004800u));
-  return c;
+// Two fp32 per instruction.
+struct TaF2 {
+  uint64_t v;
+};
+__device__ __forceinline__ TaF2 f2(float a, float b) {
+  TaF2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void f2_get(TaF2 x, float& a, float& b) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(x.v));
+}
+__device__ __forceinline__ TaF2 fma2(TaF2 a, TaF2 b, TaF2 c) {
+  TaF2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return r;
+}
+__device__ __forceinline__ TaF2 add2(TaF2 a, TaF2 b) {
+  TaF2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ TaF2 mul2(TaF2 a, TaF2 b) {
+  TaF2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ uint32_t sub_f16x2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
 }
 
-template <int NR>
+template <int NR, bool VT>
 __global__ void __launch_bounds__(TA_THREADS, 1)
     tree_attn_kernel(const __grid_constant__ CUtensorMap km, const __grid_constant__ CUtensorMap tm,
                      const TreeAttnParams p) {
@@ -383,9 +405,9 @@ __global__ void __launch_bounds__(TA_THREADS, 1)
             mbar_add_tx(&sh->full[st.i], 16384);
             for (int r = 0; r < 128; r += p.box) tma_load_2d(map, &sh->full[st.i], tile + c * 16384 + r * 128, x, sl[r]);
           };
-          if (tail && !p.vt) fetch(p.nc, &tm, 0);
+          if (tail && !VT) fetch(p.nc, &tm, 0);
           if (chunk) fetch(lw, &km, lw * 128);
-          if (tail && p.vt) fetch(p.nc, &tm, 0);
+          if (tail && VT) fetch(p.nc, &tm, 0);
           if (!chunk && !tail) ok = chunk_free(0) && ok;
           mbar_arrive(&sh->full[st.i]);
         }
@@ -478,7 +500,7 @@ __global__ void __launch_bounds__(TA_THREADS, 1)
         }
         umma_commit(&sh->s_full[sq.i]);
         for (int c = p.dt; c < p.nc; ++c) umma_commit(&sh->kfree[kq.i][c]);
-        if (p.dr && !p.vt) umma_commit(&sh->kfree[kq.i][4]);
+        if (p.dr && !VT) umma_commit(&sh->kfree[kq.i][4]);
         kq.next(p.stages);
         sq.next(p.s_bufs);
       };
@@ -491,7 +513,7 @@ __global__ void __launch_bounds__(TA_THREADS, 1)
             umma_f8_ss(tmem + o_col + m * NP, a + m * 1024 + k * 256, p_desc + k * 256, id_pv, !first || k > 0 ? 1u : 0u);
           umma_commit(&sh->kfree[kp.i][m]);
         }
-        if (p.vt) {  // 64 dims (the other 64 lanes hold what lies behind them, unused)
+        if (VT) {  // 64 dims (the other 64 lanes hold what lies behind them, unused)
 #pragma unroll
           for (int k = 0; k < 8; ++k)  // 16 keys: 2048 and 1024 bytes further
             umma_bf16_ss(tmem + ot_col, a + p.nc * 1024 + k * 128, pb_desc + k * 64, id_pt, !first || k > 0 ? 1u : 0u);
@@ -626,9 +648,9 @@ __global__ void __launch_bounds__(TA_THREADS, 1)
       const int r0 = w.rt * NR;                      // first row of the tile in the sequence
       const int nrows = min(NR, p.rows - r0);
       const bool whole = w.t == 0 && n == w.nt;      // no other CTA has a part
-      float l[CW];
+      TaF2 l2[CW / 2];  // this key lane's sums
 #pragma unroll
-      for (int c = 0; c < CW; ++c) l[c] = 0.f;
+      for (int c = 0; c < CW / 2; ++c) l2[c] = f2(0.f, 0.f);
       for (int i = 0; i < n; ++i, ++g, sq.next(p.s_bufs), ad.next(TA_AHEAD)) {
         // which rows see this key: all, or a bit per row
         uint32_t allow = 0xFFFFFFFFu;
@@ -664,30 +686,31 @@ __global__ void __launch_bounds__(TA_THREADS, 1)
 
         mbar_wait_inl(&sh->s_full[sq.i], sq.ph, wc);
         tc_fence_after();
-        float x[CW];  // q 2^-e . k
+        TaF2 x[CW / 2];  // q 2^-e . k
         {
-          float lo[CW], tl[CW];
+          float hi[CW], lo[CW], tl[CW];
           const uint32_t at = tmem + sq.i * 3 * NR + hc + lane_off;
-          tmem_ldn<CW>(at, x);
+          tmem_ldn<CW>(at, hi);
           tmem_ldn<CW>(at + NR, lo);
           if (p.dr) tmem_ldn<CW>(at + 2 * NR, tl);
           tmem_wait_ld();
           tc_fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive(&sh->s_free[sq.i]);
+          const TaF2 sixteenth = f2(0.0625f, 0.0625f), sk2 = f2(sk, sk);
 #pragma unroll
-          for (int c = 0; c < CW; ++c) x[c] = fmaf(fmaf(lo[c], 0.0625f, x[c]), sk, p.dr ? tl[c] : 0.f);
+          for (int c = 0; c < CW; c += 2)
+            x[c / 2] = fma2(fma2(f2(lo[c], lo[c + 1]), sixteenth, f2(hi[c], hi[c + 1])), sk2,
+                            p.dr ? f2(tl[c], tl[c + 1]) : f2(0.f, 0.f));
         }
         float d[CW];
-        auto exponents = [&](const float* mneg) {
+        auto exponents = [&](bool raw) {
 #pragma unroll
           for (int c = 0; c < CW; c += 4) {
-            const float4 s4 = *reinterpret_cast<const float4*>(&sh->qs[hc + c]);
-            const float4 mn = mneg ? *reinterpret_cast<const float4*>(&mneg[hc + c]) : make_float4(0.f, 0.f, 0.f, 0.f);
-            d[c] = fmaf(x[c], s4.x, mn.x);
-            d[c + 1] = fmaf(x[c + 1], s4.y, mn.y);
-            d[c + 2] = fmaf(x[c + 2], s4.z, mn.z);
-            d[c + 3] = fmaf(x[c + 3], s4.w, mn.w);
+            const ulonglong2 s4 = *reinterpret_cast<const ulonglong2*>(&sh->qs[hc + c]);
+            const ulonglong2 mn = raw ? make_ulonglong2(0, 0) : *reinterpret_cast<const ulonglong2*>(&sh->mneg[hc + c]);
+            f2_get(fma2(x[c / 2], TaF2{s4.x}, TaF2{mn.x}), d[c], d[c + 1]);
+            f2_get(fma2(x[c / 2 + 1], TaF2{s4.y}, TaF2{mn.y}), d[c + 2], d[c + 3]);
           }
           if (!plain) {
 #pragma unroll
@@ -697,16 +720,16 @@ __global__ void __launch_bounds__(TA_THREADS, 1)
         };
         bool raise = i == 0;
         if (i > 0) {
-          exponents(sh->mneg);
-          float most = d[0];
+          exponents(false);
+          float most = fmaxf(d[0], d[1]);
 #pragma unroll
-          for (int c = 1; c < CW; ++c) most = fmaxf(most, d[c]);
+          for (int c = 2; c < CW; c += 2) most = fmaxf(most, fmaxf(d[c], d[c + 1]));
           raise = soft_any(most > TA_GROW || sk > sh->sigma);
         }
         if (raise) {
           // The tile's maxima; references that they pass go up to them, and the reference of
           // the scales to the tile's largest.
-          exponents(nullptr);
+          exponents(true);
           ta_reduce<true, CW>(d, &sh->red[quarter][hc], lane);
           float smax = sk;
 #pragma unroll
@@ -729,10 +752,10 @@ __global__ void __launch_bounds__(TA_THREADS, 1)
             sh->sigma = sn;
           }
           soft_sync();
-          exponents(sh->mneg);
+          exponents(false);
           if (i > 0) {  // sums and output follow, once every product before is in it
 #pragma unroll
-            for (int c = 0; c < CW; ++c) l[c] *= sh->f[hc + c];
+            for (int c = 0; c < CW; c += 2) l2[c / 2] = mul2(l2[c / 2], f2(sh->f[hc + c], sh->f[hc + c + 1]));
             mbar_wait_inl(&sh->pv_done, (g - 1) & 1, wc);
             tc_fence_after();
             float fr[CW];
@@ -744,7 +767,7 @@ __global__ void __launch_bounds__(TA_THREADS, 1)
             }
             if (!same) {  // (the same for the whole warp)
 #pragma unroll 1
-              for (int b = 0; b < p.dt * TA_LEVELS + p.vt; ++b) {
+              for (int b = 0; b < p.dt * TA_LEVELS + VT; ++b) {
                 const float fs = b < p.dt * TA_LEVELS ? sh->fs : 1.f;
                 float o[CW];
                 const uint32_t at = tmem + o_col + b * NR + hc + lane_off;
@@ -760,23 +783,26 @@ __global__ void __launch_bounds__(TA_THREADS, 1)
         }
         // weights, their sums, and the three parts of each
         const float fk = marked ? 1.f : sh->sigma > 0.f ? sk * (TA_TOP / sh->sigma) : 0.f;
-        uint32_t pc[TA_LEVELS][CW / 4], pw[CW / 2];
+        const TaF2 fk2 = f2(fk, fk);
+        uint32_t pc[TA_LEVELS][CW / 4], pw[VT ? CW / 2 : 1];
 #pragma unroll
         for (int c = 0; c < CW; c += 4) {
-          uint16_t q2[TA_LEVELS][2];
+          uint32_t h[2], h1[2], h2[2];
 #pragma unroll
           for (int z = 0; z < 2; ++z) {
             const float e0 = ex2f(d[c + 2 * z]), e1 = ex2f(d[c + 2 * z + 1]);
-            l[c + 2 * z] += e0;
-            l[c + 2 * z + 1] += e1;
-            pw[c / 2 + z] = cvt_bf16x2(e0, e1);
-            uint32_t h;
-            asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(h) : "f"(e1 * fk), "f"(e0 * fk));
-#pragma unroll
-            for (int v = 0; v < TA_LEVELS; ++v) q2[v][z] = ta_split(h);
+            const TaF2 e = f2(e0, e1);
+            l2[c / 2 + z] = add2(l2[c / 2 + z], e);
+            if constexpr (VT) pw[c / 2 + z] = cvt_bf16x2(e0, e1);
+            float w0, w1;
+            f2_get(mul2(e, fk2), w0, w1);
+            asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(h[z]) : "f"(w1), "f"(w0));
+            h1[z] = sub_f16x2(h[z], h[z] & 0xFF00FF00u);
+            h2[z] = sub_f16x2(h1[z], h1[z] & 0xFF00FF00u) + 0x00800080u;  // the last part rounded to nearest
           }
-#pragma unroll
-          for (int v = 0; v < TA_LEVELS; ++v) pc[v][c / 4] = (uint32_t)q2[v][0] | ((uint32_t)q2[v][1] << 16);
+          pc[0][c / 4] = __byte_perm(h[0], h[1], 0x7531);
+          pc[1][c / 4] = __byte_perm(h1[0], h1[1], 0x7531);
+          pc[2][c / 4] = __byte_perm(h2[0], h2[1], 0x7531);
         }
         // the previous tile's product has read P
         if (g > 0) mbar_wait_inl(&sh->pv_done, (g - 1) & 1, wc);
@@ -787,7 +813,7 @@ __global__ void __launch_bounds__(TA_THREADS, 1)
           if constexpr (CW == 16) *reinterpret_cast<uint4*>(at) = make_uint4(pc[v][0], pc[v][1], pc[v][2], pc[v][3]);
           else *reinterpret_cast<uint2*>(at) = make_uint2(pc[v][0], pc[v][1]);
         }
-        if (p.vt) {
+        if constexpr (VT) {
 #pragma unroll
           for (int c = 0; c < CW; c += 8)
             *reinterpret_cast<uint4*>(pb + key * 64 + ((((hc + c) >> 3) ^ ((key >> 1) & 3)) << 4)) =
@@ -800,6 +826,9 @@ __global__ void __launch_bounds__(TA_THREADS, 1)
       }
       // ---- the row tile's part is complete
       {
+        float l[CW];
+#pragma unroll
+        for (int c = 0; c < CW; c += 2) f2_get(l2[c / 2], l[c], l[c + 1]);
         ta_reduce<false, CW>(l, &sh->red[quarter][hc], lane);
         soft_sync();
         TaWalk x = w;
@@ -860,10 +889,10 @@ __global__ void __launch_bounds__(TA_THREADS, 1)
           tmem_ldn<CW>(at + 2 * NR, o2);
           tmem_wait_ld();
 #pragma unroll
-          for (int c = 0; c < CW; ++c) o[c] = fmaf(fmaf(o2[c], 1.f / TA_STEP, o1[c]), 1.f / TA_STEP, o[c]) * unit;
+          for (int c = 0; c < CW; ++c) o[c] = (o[c] + (o1[c] + o2[c])) * unit;
           if (m * 128 + key < min(p.dv, p.dq)) store(m * 128 + key, o);
         }
-        if (p.vt) {
+        if (VT) {
           float o[CW];
           tmem_ldn<CW>(tmem + ot_col + hc + lane_off, o);
           tmem_wait_ld();
