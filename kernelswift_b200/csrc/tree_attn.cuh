@@ -39,7 +39,9 @@
 // tree_attn_join_kernel adds them up in order (no atomics).
 //
 // Warps: 8 softmax warps (thread = key = TMEM lane; two share a lane quarter and split the
-// rows), 4 loader warps, one MMA warp, one address warp that walks the page table ahead of
+// rows), 4 loader warps, a warp that issues the first product and one that issues the
+// second (each waits for its own inputs; one thread for both made each wait for the
+// other's), one address warp that walks the page table ahead of
 // the loads.  A tile whose keys are all present and unmarked comes by TMA in boxes of r
 // rows (r: the power of two that divides page and 128, at least 8); others (the last of a
 // sequence, odd pages) by cp.async with absent and marked rows zeroed, so that no garbage
@@ -59,8 +61,8 @@ namespace ks {
 
 constexpr int TA_SOFT = 256;                 // softmax threads (warps 0-7)
 constexpr int TA_LOADERS = 4;                // loader warps (8-11)
-constexpr int TA_W_LOAD = 8, TA_W_MMA = 12, TA_W_ADDR = 13;
-constexpr int TA_THREADS = 14 * 32;
+constexpr int TA_W_LOAD = 8, TA_W_QK = 12, TA_W_PV = 13, TA_W_ADDR = 14;
+constexpr int TA_THREADS = 15 * 32;
 constexpr int TA_MAX_CTAS = 148;             // SMs of a B200: bounds the workspace
 constexpr int TA_MAX_ROWS = 32;
 constexpr int TA_STAGES = 4;                 // most code tiles in shared memory
@@ -101,12 +103,12 @@ struct TreeAttnParams {
 };
 
 struct TaShared {
-  uint64_t full[TA_STAGES];                     // a tile's rows are in place
-  uint64_t kfree[TA_STAGES][5];                 // a chunk of it (4: the tail) has been used
+  uint64_t full[TA_STAGES][5];                  // a chunk of a tile (4: the tail) is in place
+  uint64_t kfree[TA_STAGES][5];                 // it has been used
   uint64_t s_full[2], s_free[2];                // scores are in TMEM / in registers
   uint64_t p_full, pv_done;                     // weights are in shared memory / have been used
   uint64_t a_full[TA_AHEAD], a_free[TA_AHEAD];  // a tile's addresses and scales
-  uint64_t q_full, drain;
+  uint64_t q_full, drain[2];
   uint32_t tmem_base;
   int abort;
   int64_t total, per;
@@ -117,7 +119,7 @@ struct TaShared {
   alignas(16) float qs[TA_MAX_ROWS];            // 2^e * softmax scale of each row
   alignas(16) float f[TA_MAX_ROWS];             // factor of a raise; at the end 1 / sum
   float red[4][TA_MAX_ROWS];
-  float red_s[8];
+  float red_s[4];
   int32_t whole[TA_AHEAD];                      // every key of the tile can come by TMA
   int32_t slot[TA_AHEAD][128];                  // row of the page pool, -1: zeros
   float sk[TA_AHEAD][128];                      // key's scale; -1: absent, NaN: marked
@@ -216,6 +218,7 @@ __device__ __forceinline__ bool soft_any(bool x) {
                : "memory");
   return r != 0;
 }
+
 __device__ __forceinline__ void soft_sync() { named_bar_sync(1, TA_SOFT); }
 
 // Max or sum over the warp's lanes of CW <= 16 values each into red[c], c < CW.
@@ -297,8 +300,10 @@ __global__ void __launch_bounds__(TA_THREADS, 1)
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < TA_STAGES; ++s) {
-      mbar_init(&sh->full[s], TA_LOADERS);
-      for (int c = 0; c < 5; ++c) mbar_init(&sh->kfree[s][c], 1);
+      for (int c = 0; c < 5; ++c) {
+        mbar_init(&sh->full[s][c], 1);
+        mbar_init(&sh->kfree[s][c], 1);
+      }
     }
     for (int s = 0; s < 2; ++s) {
       mbar_init(&sh->s_full[s], 1);
@@ -311,7 +316,8 @@ __global__ void __launch_bounds__(TA_THREADS, 1)
       mbar_init(&sh->a_free[s], TA_LOADERS + TA_SOFT / 32);
     }
     mbar_init(&sh->q_full, TA_SOFT / 32);
-    mbar_init(&sh->drain, 1);
+    mbar_init(&sh->drain[0], 1);
+    mbar_init(&sh->drain[1], 1);
     sh->abort = 0;
     sh->sigma = 0.f;
     fence_barrier_init();
@@ -321,7 +327,7 @@ __global__ void __launch_bounds__(TA_THREADS, 1)
     sh->m[threadIdx.x] = -INFINITY;
     sh->mneg[threadIdx.x] = INFINITY;
   }
-  if (warp == TA_W_MMA) {
+  if (warp == TA_W_QK) {
     tmem_alloc<1>(&sh->tmem_base, p.tmem_cols);
     tmem_relinquish<1>();
     if (lane == 0 && p.box) {
@@ -380,68 +386,63 @@ __global__ void __launch_bounds__(TA_THREADS, 1)
   TaWalk w;
   w.start(p, sh);
 
-  if (warp >= TA_W_LOAD && warp < TA_W_MMA) {
+  if (warp >= TA_W_LOAD && warp < TA_W_QK) {
     // ================================================================ loaders
+    // Warp c loads chunk c, warp nc % 4 the tail too (first where only the scores read it:
+    // it is free first).
     const int lw = warp - TA_W_LOAD, piece = lane & 7;
+    const bool chunk = lw < p.nc, tail = p.dr && lw == (p.nc & 3);
     TaRing st, ad;
-    uint32_t sent = 0, sent_ph = 0;  // stages whose latest load is by TMA, and its phase
+    uint32_t sent[2] = {0, 0}, sent_ph[2] = {0, 0};  // stages whose latest load is by TMA, its phase
     bool ok = true;
     for (int u = 0; u < w.left && ok; ++u, st.next(p.stages), ad.next(TA_AHEAD)) {
       ok = __all_sync(0xFFFFFFFFu, mbar_wait_inl(&sh->a_full[ad.i], ad.ph, wc));
       if (!ok) break;
       const bool whole = p.box && sh->whole[ad.i];
-      // chunk c (nc: the tail) of the stage has been read: the second product's dim tiles
-      // free theirs one by one, chunks that only the first reads go with its end
-      auto chunk_free = [&](int c) { return mbar_wait_inl(&sh->kfree[st.i][c == p.nc ? 4 : c], st.ph ^ 1, wc); };
-      uint8_t* tile = ks_ + (size_t)st.i * p.stage_bytes;
       const int32_t* sl = sh->slot[ad.i];
-      if (whole) {
-        // A warp per chunk, the tail with warp nc % 4.  Nothing arrives for this use of the
-        // stage before a part of it is free, when the last use's loads have landed.
-        if (elect_one()) {
-          const bool chunk = lw < p.nc, tail = p.dr && lw == (p.nc & 3);
-          auto fetch = [&](int c, const CUtensorMap* map, int x) {
-            ok = chunk_free(c) && ok;
-            mbar_add_tx(&sh->full[st.i], 16384);
-            for (int r = 0; r < 128; r += p.box) tma_load_2d(map, &sh->full[st.i], tile + c * 16384 + r * 128, x, sl[r]);
-          };
-          if (tail && !VT) fetch(p.nc, &tm, 0);
-          if (chunk) fetch(lw, &km, lw * 128);
-          if (tail && VT) fetch(p.nc, &tm, 0);
-          if (!chunk && !tail) ok = chunk_free(0) && ok;
-          mbar_arrive(&sh->full[st.i]);
-        }
-        ok = __all_sync(0xFFFFFFFFu, ok);
-        sent |= 1u << st.i;
-        sent_ph = (sent_ph & ~(1u << st.i)) | st.ph << st.i;
-      } else {
-        sent &= ~(1u << st.i);
-        for (int c = 0; c <= p.nc; ++c)
-          if (c < p.nc || p.dr) ok = chunk_free(c) && ok;
-        ok = __all_sync(0xFFFFFFFFu, ok);
-        if (!ok) break;
-        for (int i = 0; i < 8; ++i) {  // 8 lanes per row: 128 bytes of it at a time
-          const int key = lw * 32 + i * 4 + (lane >> 3), s = sl[key];
-          const uint8_t* src = p.kv8 + (int64_t)max(s, 0) * p.dq + piece * 16;
-          uint8_t* dst = tile + key * 128 + ((piece ^ (key & 7)) << 4);
-          for (int c = 0; c < p.nc; ++c) {
-            const bool in = s >= 0 && c * 128 + piece * 16 < p.dq;
-            cp_async16(dst + c * 16384, in ? src + c * 128 : p.kv8, in ? 16u : 0u);
+      auto fetch = [&](bool is_tail) {
+        const int b = is_tail ? 4 : lw, x = is_tail ? 0 : lw * 128;
+        // The second product's dim tiles free their chunks one by one, chunks that only the
+        // scores read go with their end.
+        ok = __all_sync(0xFFFFFFFFu, mbar_wait_inl(&sh->kfree[st.i][b], st.ph ^ 1, wc)) && ok;
+        if (!ok) return;
+        uint8_t* dst = ks_ + (size_t)st.i * p.stage_bytes + (is_tail ? p.nc : lw) * 16384;
+        sent[is_tail] &= ~(1u << st.i);
+        if (whole) {
+          if (elect_one()) {
+            mbar_expect_tx(&sh->full[st.i][b], 16384);
+            for (int r = 0; r < 128; r += p.box)
+              tma_load_2d(is_tail ? &tm : &km, &sh->full[st.i][b], dst + r * 128, x, sl[r]);
           }
-          if (p.dr)
-            cp_async16(dst + p.nc * 16384, p.tail + (int64_t)max(s, 0) * p.dr + piece * 8, s >= 0 ? 16u : 0u);
+          __syncwarp();
+          sent[is_tail] |= 1u << st.i;
+          sent_ph[is_tail] = (sent_ph[is_tail] & ~(1u << st.i)) | st.ph << st.i;
+        } else {
+          // 8 lanes per row; rows that are not there and columns past dq become zeros
+          for (int k = lane >> 3; k < 128; k += 4) {
+            const int s = sl[k];
+            const bool in = s >= 0 && (is_tail || x + piece * 16 < p.dq);
+            const void* src = is_tail ? static_cast<const void*>(p.tail + (int64_t)s * p.dr + piece * 8)
+                                      : p.kv8 + (int64_t)s * p.dq + x + piece * 16;
+            cp_async16(dst + k * 128 + ((piece ^ (k & 7)) << 4), in ? src : p.kv8, in ? 16u : 0u);
+          }
+          cp_async_wait_all();
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&sh->full[st.i][b]);
         }
-        cp_async_wait_all();
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&sh->full[st.i]);
-      }
+      };
+      if (tail && !VT) fetch(true);
+      if (chunk && ok) fetch(false);
+      if (tail && VT && ok) fetch(true);
       if (lane == 0) mbar_arrive(&sh->a_free[ad.i]);
     }
     // after a timed-out wait: no load of this CTA may land once it has gone
     if (*wc.abort)
-      for (int s = 0; s < TA_STAGES; ++s)
-        if (sent >> s & 1) mbar_wait(&sh->full[s], sent_ph >> s & 1, wc, false, true);
+      for (int s = 0; s < TA_STAGES; ++s) {
+        if (sent[0] >> s & 1) mbar_wait(&sh->full[s][lw], sent_ph[0] >> s & 1, wc, false, true);
+        if (sent[1] >> s & 1) mbar_wait(&sh->full[s][4], sent_ph[1] >> s & 1, wc, false, true);
+      }
   } else if (warp == TA_W_ADDR) {
     // ================================================================ addresses
     TaRing ad;
@@ -473,99 +474,87 @@ __global__ void __launch_bounds__(TA_THREADS, 1)
       __syncwarp();
       if (lane == 0) mbar_arrive(&sh->a_full[ad.i]);
     }
-  } else if (warp == TA_W_MMA) {
-    // ================================================================ MMA issue
+  } else if (warp == TA_W_QK) {
+    // ================================================================ scores
     if (elect_one()) {
-      const uint32_t id_qk = idesc_e4m3_f32(128, 2 * NR), id_qt = idesc_bf16_f32(128, NR, false, false);
-      const uint32_t id_pv = idesc_e4m3_f32(128, NP) | (1u << 10) | (1u << 15) | (1u << 16), id_pt = idesc_bf16_f32(128, NR, true, true);
       // descriptors: only the start address (low word, 16-byte units) changes
       const uint64_t k_desc = sdesc_sw128(smem_u32(ks_), 16, 1024), q_desc = sdesc_sw128(smem_u32(qs), 16, 1024);
-      const uint64_t v_desc = sdesc_sw128(smem_u32(ks_), 16384, 1024), p_desc = sdesc_sw128(smem_u32(ps), 16, 1024);
-      const uint64_t pb_desc = sdesc_sw64(smem_u32(pb));
+      const uint32_t id_qk = idesc_e4m3_f32(128, 2 * NR), id_qt = idesc_bf16_f32(128, NR, false, false);
       const uint32_t stage16 = p.stage_bytes >> 4;
-      TaRing kq, kp, sq;  // code tile of the next QK and of the next PV; score buffer
-      auto qk = [&] {
-        tc_fence_after();
-        const uint32_t d = tmem + sq.i * 3 * NR;
-        const uint64_t a = k_desc + kq.i * stage16;
-        if (p.dr) {
+      TaRing st, sq;
+      uint32_t items = 0;
+      bool ok = true;
+      for (; w.left > 0 && ok; ++items) {
+        const int n = w.here();
+        ok = mbar_wait_inl(&sh->q_full, items & 1, wc);
+        for (int i = 0; i < n && ok; ++i, st.next(p.stages), sq.next(p.s_bufs)) {
+          ok = mbar_wait_inl(&sh->s_free[sq.i], sq.ph ^ 1, wc);
+          const uint32_t d = tmem + sq.i * 3 * NR;
+          const uint64_t a = k_desc + st.i * stage16;
+          if (p.dr && ok) {
+            ok = mbar_wait_inl(&sh->full[st.i][4], st.ph, wc);
+            tc_fence_after();
+            if (ok)
 #pragma unroll
-          for (int k = 0; k < 4; ++k)
-            umma_bf16_ss(d + 2 * NR, a + p.nc * 1024 + k * 2, q_desc + p.nc * (2 * NR * 8) + k * 2, id_qt, k > 0 ? 1u : 0u);
-        }
-        for (int c = 0; c < p.nc; ++c) {
-#pragma unroll
-          for (int k = 0; k < 4; ++k)
-            umma_f8_ss(d, a + c * 1024 + k * 2, q_desc + c * (2 * NR * 8) + k * 2, id_qk, c > 0 || k > 0 ? 1u : 0u);
-        }
-        umma_commit(&sh->s_full[sq.i]);
-        for (int c = p.dt; c < p.nc; ++c) umma_commit(&sh->kfree[kq.i][c]);
-        if (p.dr && !VT) umma_commit(&sh->kfree[kq.i][4]);
-        kq.next(p.stages);
-        sq.next(p.s_bufs);
-      };
-      auto pv = [&](bool first) {
-        tc_fence_after();
-        const uint64_t a = v_desc + kp.i * stage16;
-        for (int m = 0; m < p.dt; ++m) {
-#pragma unroll
-          for (int k = 0; k < 4; ++k)  // 32 keys: 4096 bytes further in both
-            umma_f8_ss(tmem + o_col + m * NP, a + m * 1024 + k * 256, p_desc + k * 256, id_pv, !first || k > 0 ? 1u : 0u);
-          umma_commit(&sh->kfree[kp.i][m]);
-        }
-        if (VT) {  // 64 dims (the other 64 lanes hold what lies behind them, unused)
-#pragma unroll
-          for (int k = 0; k < 8; ++k)  // 16 keys: 2048 and 1024 bytes further
-            umma_bf16_ss(tmem + ot_col, a + p.nc * 1024 + k * 128, pb_desc + k * 64, id_pt, !first || k > 0 ? 1u : 0u);
-          umma_commit(&sh->kfree[kp.i][4]);
-        }
-        umma_commit(&sh->pv_done);
-        kp.next(p.stages);
-      };
-      // Scores and outputs in the order in which their inputs come: a tile's scores may run
-      // ahead of the one before's output, which need not wait for a tile that still loads.
-      TaWalk wp = w;                                    // of the next PV
-      int q_here = w.left > 0 ? w.here() : 0, q_at = 0;  // of the item: its units, QKs issued
-      int p_here = q_here, p_at = 0;
-      uint32_t items = 0, n_pv = 0;
-      uint64_t t0 = clock64();
-      const uint64_t lim = budget_cycles(p.budget_ns);
-      while (wp.left > 0) {
-        bool did = false;
-        if (mbar_poll(smem_u32(&sh->p_full), n_pv & 1)) {
-          pv(p_at == 0);
-          did = true;
-          ++n_pv;
-          if (++p_at == p_here) {
-            wp.next_item(p, p_here);
-            p_at = 0;
-            p_here = wp.left > 0 ? wp.here() : 0;
+              for (int k = 0; k < 4; ++k)
+                umma_bf16_ss(d + 2 * NR, a + p.nc * 1024 + k * 2, q_desc + p.nc * (2 * NR * 8) + k * 2, id_qt, k > 0 ? 1u : 0u);
           }
-        }
-        if (w.left > 0 && (q_at > 0 || mbar_poll(smem_u32(&sh->q_full), items & 1)) &&
-            mbar_poll(smem_u32(&sh->s_free[sq.i]), sq.ph ^ 1) && mbar_poll(smem_u32(&sh->full[kq.i]), kq.ph)) {
-          qk();
-          did = true;
-          if (++q_at == q_here) {
-            w.next_item(p, q_here);
-            q_at = 0;
-            ++items;
-            q_here = w.left > 0 ? w.here() : 0;
+          for (int c = 0; c < p.nc && ok; ++c) {
+            ok = mbar_wait_inl(&sh->full[st.i][c], st.ph, wc);
+            tc_fence_after();
+            if (ok)
+#pragma unroll
+              for (int k = 0; k < 4; ++k)
+                umma_f8_ss(d, a + c * 1024 + k * 2, q_desc + c * (2 * NR * 8) + k * 2, id_qk, c > 0 || k > 0 ? 1u : 0u);
           }
+          if (!ok) break;
+          umma_commit(&sh->s_full[sq.i]);
+          for (int c = p.dt; c < p.nc; ++c) umma_commit(&sh->kfree[st.i][c]);
+          if (p.dr && !VT) umma_commit(&sh->kfree[st.i][4]);
         }
-        if (did) {
-          t0 = clock64();
-        } else {
-          if (*wc.abort) break;
-          if ((uint64_t)clock64() - t0 > lim) {
-            raise_timeout(wc, smem_u32(&sh->p_full), n_pv & 1);
-            break;
-          }
-        }
+        w.next_item(p, n);
       }
       // nothing of this CTA is in flight when it gives its memory back
-      umma_commit(&sh->drain);
-      mbar_wait(&sh->drain, 0, wc, false, true);
+      umma_commit(&sh->drain[0]);
+      mbar_wait(&sh->drain[0], 0, wc, false, true);
+    }
+    __syncwarp();
+  } else if (warp == TA_W_PV) {
+    // ================================================================ outputs
+    if (elect_one()) {
+      const uint64_t v_desc = sdesc_sw128(smem_u32(ks_), 16384, 1024), p_desc = sdesc_sw128(smem_u32(ps), 16, 1024);
+      const uint64_t pb_desc = sdesc_sw64(smem_u32(pb));
+      const uint32_t id_pv = idesc_e4m3_f32(128, NP) | (1u << 10) | (1u << 15) | (1u << 16);  // B e5m2, both MN-major
+      const uint32_t id_pt = idesc_bf16_f32(128, NR, true, true);
+      const uint32_t stage16 = p.stage_bytes >> 4;
+      TaRing st;
+      uint32_t g = 0;
+      bool ok = true;
+      while (w.left > 0 && ok) {
+        const int n = w.here();
+        for (int i = 0; i < n; ++i, ++g, st.next(p.stages)) {
+          ok = mbar_wait_inl(&sh->p_full, g & 1, wc);
+          if (!ok) break;
+          tc_fence_after();
+          const uint64_t a = v_desc + st.i * stage16;
+          for (int m = 0; m < p.dt; ++m) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k)  // 32 keys: 4096 bytes further in both
+              umma_f8_ss(tmem + o_col + m * NP, a + m * 1024 + k * 256, p_desc + k * 256, id_pv, i > 0 || k > 0 ? 1u : 0u);
+            umma_commit(&sh->kfree[st.i][m]);
+          }
+          if (VT) {  // 64 dims (the other 64 lanes hold what lies behind them, unused)
+#pragma unroll
+            for (int k = 0; k < 8; ++k)  // 16 keys: 2048 and 1024 bytes further
+              umma_bf16_ss(tmem + ot_col, a + p.nc * 1024 + k * 128, pb_desc + k * 64, id_pt, i > 0 || k > 0 ? 1u : 0u);
+            umma_commit(&sh->kfree[st.i][4]);
+          }
+          umma_commit(&sh->pv_done);
+        }
+        w.next_item(p, n);
+      }
+      umma_commit(&sh->drain[1]);
+      mbar_wait(&sh->drain[1], 0, wc, false, true);
     }
     __syncwarp();
   } else {
@@ -580,63 +569,57 @@ __global__ void __launch_bounds__(TA_THREADS, 1)
     // The queries of item x: hi and lo codes and the bf16 tail, scaled by a power of two
     // per row.  The last scores of the item before are in registers.
     auto queries = [&](const TaWalk& x) {
-      constexpr int RW = NR / 8;  // rows of a warp
-      const int first = x.rt * NR + warp * RW;
-      uint32_t v[RW][8], t[RW][4];
+      constexpr int LR = NR == 32 ? 8 : 16;  // lanes of a row, 8 columns each at a time
+      static_assert(NR / (TA_SOFT / 32) == 32 / LR, "every warp takes 32 / LR rows");
+      constexpr int QV = 64 / LR;
+      const int row = warp * (32 / LR) + lane / LR, at = lane % LR;
+      const bool in = x.rt * NR + row < p.rows;
+      const uint16_t* q = p.q + ((int64_t)x.b * p.rows + x.rt * NR + row) * (p.dq + p.dr);
+      uint4 v[QV], t;
 #pragma unroll
-      for (int i = 0; i < RW; ++i) {
-        const bool in = first + i < p.rows;
-        const uint16_t* q = p.q + ((int64_t)x.b * p.rows + first + i) * (p.dq + p.dr);
-        *reinterpret_cast<uint4*>(v[i]) = ldcg_or_zero(q + lane * 16, in && lane * 16 < p.dq);
-        *reinterpret_cast<uint4*>(v[i] + 4) = ldcg_or_zero(q + lane * 16 + 8, in && lane * 16 < p.dq);
-        *reinterpret_cast<uint4*>(t[i]) = ldcg_or_zero(q + p.dq + lane * 8, in && lane * 8 < p.dr);
+      for (int k = 0; k < QV; ++k) v[k] = ldcg_or_zero(q + (k * LR + at) * 8, in && (k * LR + at) * 8 < p.dq);
+      t = ldcg_or_zero(q + p.dq + at * 8, in && at * 8 < p.dr);
+      // the largest magnitude, as bf16 bits (in order as integers; from 0x7F80 on not finite)
+      uint32_t top = 0;
+#pragma unroll
+      for (int k = 0; k < QV; ++k) {
+        const uint32_t y[4] = {v[k].x, v[k].y, v[k].z, v[k].w};
+#pragma unroll
+        for (int z = 0; z < 4; ++z)
+          asm("max.u16x2 %0, %0, %1;" : "+r"(top) : "r"(y[z] & 0x7FFF7FFFu));
       }
+      top = max(top & 0xFFFFu, top >> 16);
 #pragma unroll
-      for (int i = 0; i < RW; ++i) {
-        const int row = warp * RW + i;
-        float amax = 0.f;
-        bool bad = false;
+      for (int o = LR / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
+      const bool bad = top >= 0x7F80u;
+      const int e = bad ? 0 : max((int)(top >> 7) - 127 - 7, -100);  // largest element into [128, 256)
+      const float inv = __uint_as_float((uint32_t)(127 - e) << 23);
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          amax = fmaxf(amax, fmaxf(fabsf(bf16lo_f32(v[i][k])), fabsf(bf16hi_f32(v[i][k]))));
-          bad |= bf16x2_nonfinite(v[i][k]);
+      for (int k = 0; k < QV; ++k) {
+        const int c8 = k * LR + at;  // columns 8 c8 .. 8 c8 + 7
+        if (c8 >= p.nc * 16) continue;
+        const uint32_t y[4] = {v[k].x, v[k].y, v[k].z, v[k].w};
+        uint32_t hi[2] = {0, 0}, lo[2] = {0, 0};
+#pragma unroll
+        for (int z = 0; z < 4; ++z) {
+          const float a = bf16lo_f32(y[z]) * inv, b = bf16hi_f32(y[z]) * inv;
+          const uint16_t h = cvt_e4m3x2(a, b);
+          const uint32_t back = f16x2_of_e4m3x2(h);
+          const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&back));
+          hi[z >> 1] |= (uint32_t)h << (16 * (z & 1));
+          lo[z >> 1] |= (uint32_t)cvt_e4m3x2((a - f.x) * 16.f, (b - f.y) * 16.f) << (16 * (z & 1));
         }
-        bad = __any_sync(0xFFFFFFFFu, bad);
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xFFFFFFFFu, amax, o));
-        // largest element into [128, 256)
-        const int e = bad ? 0 : max((int)(__float_as_uint(amax) >> 23) - 127 - 7, -100);
-        const float inv = __uint_as_float((uint32_t)(127 - e) << 23);
-        uint32_t hi[4], lo[4];
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          uint32_t h2 = 0, l2 = 0;
-#pragma unroll
-          for (int z = 0; z < 2; ++z) {
-            const float a = bf16lo_f32(v[i][2 * k + z]) * inv, b = bf16hi_f32(v[i][2 * k + z]) * inv;
-            const uint16_t h = cvt_e4m3x2(a, b);
-            const uint32_t back = f16x2_of_e4m3x2(h);
-            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&back));
-            h2 |= (uint32_t)h << (16 * z);
-            l2 |= (uint32_t)cvt_e4m3x2((a - f.x) * 16.f, (b - f.y) * 16.f) << (16 * z);
-          }
-          hi[k] = bad ? 0x7F7F7F7Fu : h2;  // a row with a NaN or an infinity scores NaN
-          lo[k] = bad ? 0u : l2;
-        }
-        const int c = lane >> 3;
-        if (c < p.nc) {
-          uint8_t* at = qs + c * (2 * NR * 128) + row * 128 + (((lane & 7) ^ (row & 7)) << 4);
-          *reinterpret_cast<uint4*>(at) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-          *reinterpret_cast<uint4*>(at + NR * 128) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-        }
-        if (lane * 8 < p.dr) {
-          const uint32_t m2 = (uint32_t)(127 - e) * 0x00800080u;
-          *reinterpret_cast<uint4*>(qs + p.nc * (2 * NR * 128) + row * 128 + ((lane ^ (row & 7)) << 4)) =
-              make_uint4(mul_bf16x2(t[i][0], m2), mul_bf16x2(t[i][1], m2), mul_bf16x2(t[i][2], m2),
-                         mul_bf16x2(t[i][3], m2));
-        }
-        if (lane == 0) sh->qs[row] = __uint_as_float((uint32_t)(127 + e) << 23) * p.scale_log2;
+        uint8_t* dst = qs + (c8 >> 4) * (2 * NR * 128) + row * 128 + ((((c8 & 15) >> 1) ^ (row & 7)) << 4) + (c8 & 1) * 8;
+        // a row with a NaN or an infinity scores NaN
+        *reinterpret_cast<uint2*>(dst) = bad ? make_uint2(0x7F7F7F7Fu, 0x7F7F7F7Fu) : make_uint2(hi[0], hi[1]);
+        *reinterpret_cast<uint2*>(dst + NR * 128) = bad ? make_uint2(0u, 0u) : make_uint2(lo[0], lo[1]);
       }
+      if (at * 8 < p.dr) {
+        const uint32_t m2 = (uint32_t)(127 - e) * 0x00800080u;
+        *reinterpret_cast<uint4*>(qs + p.nc * (2 * NR * 128) + row * 128 + ((at ^ (row & 7)) << 4)) =
+            make_uint4(mul_bf16x2(t.x, m2), mul_bf16x2(t.y, m2), mul_bf16x2(t.z, m2), mul_bf16x2(t.w, m2));
+      }
+      if (at == 0) sh->qs[row] = __uint_as_float((uint32_t)(127 + e) << 23) * p.scale_log2;
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) mbar_arrive(&sh->q_full);
@@ -734,7 +717,7 @@ __global__ void __launch_bounds__(TA_THREADS, 1)
           float smax = sk;
 #pragma unroll
           for (int o = 16; o > 0; o >>= 1) smax = fmaxf(smax, __shfl_xor_sync(0xFFFFFFFFu, smax, o));
-          if (lane == 0) sh->red_s[warp] = smax;
+          if (lane == 0 && hc == 0) sh->red_s[quarter] = smax;
           soft_sync();
           if (threadIdx.x < NR) {
             const int c = threadIdx.x;
@@ -866,18 +849,24 @@ __global__ void __launch_bounds__(TA_THREADS, 1)
         mbar_wait_inl(&sh->pv_done, (g - 1) & 1, wc);
         tc_fence_after();
         const float unit = sh->fs;
-        auto store = [&](int dim, const float (&o)[CW]) {
+        // dims `dim` (even lanes) and dim + 1 (the next lane) of a row go out together: the
+        // even lane stores row c, the odd one row c + 1
+        const bool odd = lane & 1;
+        auto store = [&](int dim, int dims, const float (&o)[CW]) {
           if (whole) {
-            uint16_t* op = p.out + ((int64_t)w.b * p.rows + r0 + hc) * p.dv + dim;
+            uint16_t* op = p.out + ((int64_t)w.b * p.rows + r0 + hc + odd) * p.dv + (dim - odd);
 #pragma unroll
-            for (int c = 0; c < CW; ++c)
-              if (hc + c < nrows)
-                op[(int64_t)c * p.dv] = __bfloat16_as_ushort(__float2bfloat16_rn(o[c] * sh->f[hc + c]));
+            for (int c = 0; c < CW; c += 2) {
+              const float a = o[c] * sh->f[hc + c], b = o[c + 1] * sh->f[hc + c + 1];
+              const float got = __shfl_xor_sync(0xFFFFFFFFu, odd ? a : b, 1);
+              if (dim < dims && hc + c + odd < nrows)
+                *reinterpret_cast<uint32_t*>(op + (int64_t)c * p.dv) = odd ? cvt_bf16x2(got, b) : cvt_bf16x2(a, got);
+            }
           } else {
             float* op = p.part_o + ((int64_t)slot * NR + hc) * p.dv + dim;
 #pragma unroll
             for (int c = 0; c < CW; ++c)
-              if (hc + c < nrows) op[(int64_t)c * p.dv] = o[c];
+              if (dim < dims && hc + c < nrows) op[(int64_t)c * p.dv] = o[c];
           }
         };
 #pragma unroll 1
@@ -890,13 +879,13 @@ __global__ void __launch_bounds__(TA_THREADS, 1)
           tmem_wait_ld();
 #pragma unroll
           for (int c = 0; c < CW; ++c) o[c] = (o[c] + (o1[c] + o2[c])) * unit;
-          if (m * 128 + key < min(p.dv, p.dq)) store(m * 128 + key, o);
+          store(m * 128 + key, min(p.dv, p.dq), o);
         }
         if (VT) {
           float o[CW];
           tmem_ldn<CW>(tmem + ot_col + hc + lane_off, o);
           tmem_wait_ld();
-          if (p.dq + key < p.dv) store(p.dq + key, o);
+          store(p.dq + key, p.dv, o);
         }
         tc_fence_before();
         soft_sync();  // f and qs are read by all before the next item's
@@ -907,7 +896,7 @@ __global__ void __launch_bounds__(TA_THREADS, 1)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (warp == TA_W_MMA) tmem_dealloc<1>(tmem, p.tmem_cols);
+  if (warp == TA_W_QK) tmem_dealloc<1>(tmem, p.tmem_cols);
 }
 
 // Adds up the parts of row tiles that span CTAs, in order: the tile whose head CTA x holds
