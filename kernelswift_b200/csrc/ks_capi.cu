@@ -604,7 +604,18 @@ int launch_tree_attn(Device* dev, const CUtensorMap& km, const CUtensorMap& tm, 
     return rc;
   tree_attn_kernel<NR, VT><<<grid, TA_THREADS, smem, st>>>(km, tm, p);
   if (int rc = launch_check("tree_attn_kernel launch")) return rc;
-  tree_attn_join_kernel<NR><<<dim3(grid, NR), TA_JOIN_THREADS, 0, st>>>(p);
+  // set up while the kernel above runs; it waits for that kernel's end itself
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.gridDim = dim3(grid, NR / TA_JOIN_ROWS);
+  cfg.blockDim = dim3(TA_JOIN_THREADS);
+  cfg.stream = st;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  cudaError_t e = cudaLaunchKernelEx(&cfg, tree_attn_join_kernel<NR>, p);
+  if (e != cudaSuccess) return cuda_fail(e, "tree_attn_join_kernel launch");
   return launch_check("tree_attn_join_kernel launch");
 }
 

@@ -39,7 +39,7 @@
 // tree_attn_join_kernel adds them up in order (no atomics).
 //
 // Warps: 8 softmax warps (thread = key = TMEM lane; two share a lane quarter and split the
-// rows), 4 loader warps, a warp that issues the first product and one that issues the
+// rows), 5 loader warps, a warp that issues the first product and one that issues the
 // second (each waits for its own inputs; one thread for both made each wait for the
 // other's), one address warp that walks the page table ahead of
 // the loads.  A tile whose keys are all present and unmarked comes by TMA in boxes of r
@@ -60,9 +60,9 @@
 namespace ks {
 
 constexpr int TA_SOFT = 256;                 // softmax threads (warps 0-7)
-constexpr int TA_LOADERS = 4;                // loader warps (8-11)
-constexpr int TA_W_LOAD = 8, TA_W_QK = 12, TA_W_PV = 13, TA_W_ADDR = 14;
-constexpr int TA_THREADS = 15 * 32;
+constexpr int TA_LOADERS = 5;                // loader warps (8-12): a chunk each, the tail
+constexpr int TA_W_LOAD = 8, TA_W_QK = 13, TA_W_PV = 14, TA_W_ADDR = 15;
+constexpr int TA_THREADS = 16 * 32;
 constexpr int TA_MAX_CTAS = 148;             // SMs of a B200: bounds the workspace
 constexpr int TA_MAX_ROWS = 32;
 constexpr int TA_STAGES = 4;                 // most code tiles in shared memory
@@ -107,12 +107,13 @@ struct TaShared {
   uint64_t kfree[TA_STAGES][5];                 // it has been used
   uint64_t s_full[2], s_free[2];                // scores are in TMEM / in registers
   uint64_t p_full, pv_done;                     // weights are in shared memory / have been used
-  uint64_t a_full[TA_AHEAD], a_free[TA_AHEAD];  // a tile's addresses and scales
+  uint64_t a_full[TA_AHEAD], a_free[TA_AHEAD];  // a tile's addresses are in place / used
+  uint64_t sk_full[TA_AHEAD];                   // its scales are in place
   uint64_t q_full, drain[2];
   uint32_t tmem_base;
   int abort;
   int64_t total, per;
-  int32_t b0, rt0, t0;                          // where this CTA's stretch starts
+  int32_t b0, rt0, t0, len0;                    // where this CTA's stretch starts
   float sigma, fs;                              // largest scale so far; factor of its raise
   alignas(16) float m[TA_MAX_ROWS];             // reference of each row (base 2)
   alignas(16) float mneg[TA_MAX_ROWS];          // its negative
@@ -143,10 +144,8 @@ struct TaWalk {
     const int64_t u0 = (int64_t)blockIdx.x * sh->per;
     left = (int)min(sh->per, sh->total - u0);
     b = sh->b0; rt = sh->rt0; t = sh->t0;
-    if (left > 0) {
-      len = ta_len(p, b);
-      nt = ta_tiles(p, len);
-    }
+    len = sh->len0;
+    nt = left > 0 ? ta_tiles(p, len) : 0;
   }
   // units of this row tile that are in the stretch, from here
   __device__ __forceinline__ int here() const { return min(nt - t, left); }
@@ -313,6 +312,7 @@ __global__ void __launch_bounds__(TA_THREADS, 1)
     mbar_init(&sh->pv_done, 1);
     for (int s = 0; s < TA_AHEAD; ++s) {
       mbar_init(&sh->a_full[s], 1);
+      mbar_init(&sh->sk_full[s], 1);
       mbar_init(&sh->a_free[s], TA_LOADERS + TA_SOFT / 32);
     }
     mbar_init(&sh->q_full, TA_SOFT / 32);
@@ -321,6 +321,7 @@ __global__ void __launch_bounds__(TA_THREADS, 1)
     sh->abort = 0;
     sh->sigma = 0.f;
     fence_barrier_init();
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the join may be set up
     p.owner[(int64_t)blockIdx.x * 4 + 2] = 0;  // no row tile's head here yet
   }
   if (threadIdx.x < TA_MAX_ROWS) {
@@ -336,14 +337,22 @@ __global__ void __launch_bounds__(TA_THREADS, 1)
     }
   }
   if (warp == TA_W_ADDR) {  // the call's units, and where this CTA's stretch starts
+    // 128 sequences at a time, their lengths loaded at once (and kept where that is all)
+    int len[4];
+    auto lengths = [&](int i) {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) len[k] = i + k * 32 + lane < p.B ? ta_len(p, i + k * 32 + lane) : -1;
+    };
     int64_t total = 0;
-    for (int i = 0; i < p.B; i += 32) {
+    for (int i = 0; i < p.B; i += 128) {
+      lengths(i);
       int64_t n = 0;
-      if (i + lane < p.B) {
-        const int len = ta_len(p, i + lane);
-        n = ta_tiles(p, len);
-        if (blockIdx.x == 0 && (int64_t)len + p.T > p.max_pages * p.page)  // past the table
-          report_bounds(p.status, i + lane, (int)p.max_pages);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        if (len[k] < 0) continue;
+        n += ta_tiles(p, len[k]);
+        if (blockIdx.x == 0 && (int64_t)len[k] + p.T > p.max_pages * p.page)  // past the table
+          report_bounds(p.status, i + k * 32 + lane, (int)p.max_pages);
       }
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) n += __shfl_xor_sync(0xFFFFFFFFu, n, o);
@@ -352,25 +361,30 @@ __global__ void __launch_bounds__(TA_THREADS, 1)
     const int64_t per = (total + gridDim.x - 1) / gridDim.x;
     const int64_t u0 = (int64_t)blockIdx.x * per;
     int64_t at = 0;
-    for (int i = 0; i < p.B && u0 < total; i += 32) {
-      const int64_t nt = i + lane < p.B ? ta_tiles(p, ta_len(p, i + lane)) : 0;
-      int64_t n = nt * p.row_tiles;  // inclusive sums of the 32 sequences
+    bool found = u0 >= total;
+    for (int i = 0; i < p.B && !found; i += 128) {
+      if (p.B > 128) lengths(i);
+#pragma unroll 1
+      for (int k = 0; k < 4 && !found; ++k) {
+        const int ln = k == 0 ? len[0] : k == 1 ? len[1] : k == 2 ? len[2] : len[3];
+        const int64_t nt = ln >= 0 ? ta_tiles(p, ln) : 0;
+        int64_t n = nt * p.row_tiles;  // inclusive sums of the 32 sequences
 #pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int64_t v = __shfl_up_sync(0xFFFFFFFFu, n, o);
-        if (lane >= o) n += v;
-      }
-      const uint32_t over = __ballot_sync(0xFFFFFFFFu, at + n > u0);
-      if (over) {
-        if (lane == __ffs(over) - 1) {
+        for (int o = 1; o < 32; o <<= 1) {
+          const int64_t v = __shfl_up_sync(0xFFFFFFFFu, n, o);
+          if (lane >= o) n += v;
+        }
+        const uint32_t over = __ballot_sync(0xFFFFFFFFu, at + n > u0);
+        if (over && lane == __ffs(over) - 1) {
           const int64_t in = u0 - (at + n - nt * p.row_tiles);
-          sh->b0 = i + lane;
+          sh->b0 = i + k * 32 + lane;
           sh->rt0 = (int)(in / nt);
           sh->t0 = (int)(in % nt);
+          sh->len0 = ln;
         }
-        break;
+        found = over != 0;
+        at += __shfl_sync(0xFFFFFFFFu, n, 31);
       }
-      at += __shfl_sync(0xFFFFFFFFu, n, 31);
     }
     if (lane == 0) {
       sh->total = total;
@@ -388,35 +402,34 @@ __global__ void __launch_bounds__(TA_THREADS, 1)
 
   if (warp >= TA_W_LOAD && warp < TA_W_QK) {
     // ================================================================ loaders
-    // Warp c loads chunk c, warp nc % 4 the tail too (first where only the scores read it:
-    // it is free first).
+    // Warp c loads chunk c, warp 4 the tail.
     const int lw = warp - TA_W_LOAD, piece = lane & 7;
-    const bool chunk = lw < p.nc, tail = p.dr && lw == (p.nc & 3);
+    const bool is_tail = lw == 4;
+    const int x = is_tail ? 0 : lw * 128;
     TaRing st, ad;
-    uint32_t sent[2] = {0, 0}, sent_ph[2] = {0, 0};  // stages whose latest load is by TMA, its phase
+    uint32_t sent = 0, sent_ph = 0;  // stages whose latest load is by TMA, its phase
     bool ok = true;
     for (int u = 0; u < w.left && ok; ++u, st.next(p.stages), ad.next(TA_AHEAD)) {
       ok = __all_sync(0xFFFFFFFFu, mbar_wait_inl(&sh->a_full[ad.i], ad.ph, wc));
       if (!ok) break;
       const bool whole = p.box && sh->whole[ad.i];
       const int32_t* sl = sh->slot[ad.i];
-      auto fetch = [&](bool is_tail) {
-        const int b = is_tail ? 4 : lw, x = is_tail ? 0 : lw * 128;
+      if (is_tail ? p.dr > 0 : lw < p.nc) {
         // The second product's dim tiles free their chunks one by one, chunks that only the
         // scores read go with their end.
-        ok = __all_sync(0xFFFFFFFFu, mbar_wait_inl(&sh->kfree[st.i][b], st.ph ^ 1, wc)) && ok;
-        if (!ok) return;
+        uint64_t* full = &sh->full[st.i][lw];
+        ok = __all_sync(0xFFFFFFFFu, mbar_wait_inl(&sh->kfree[st.i][lw], st.ph ^ 1, wc));
+        if (!ok) break;
         uint8_t* dst = ks_ + (size_t)st.i * p.stage_bytes + (is_tail ? p.nc : lw) * 16384;
-        sent[is_tail] &= ~(1u << st.i);
+        sent &= ~(1u << st.i);
         if (whole) {
           if (elect_one()) {
-            mbar_expect_tx(&sh->full[st.i][b], 16384);
-            for (int r = 0; r < 128; r += p.box)
-              tma_load_2d(is_tail ? &tm : &km, &sh->full[st.i][b], dst + r * 128, x, sl[r]);
+            mbar_expect_tx(full, 16384);
+            for (int r = 0; r < 128; r += p.box) tma_load_2d(is_tail ? &tm : &km, full, dst + r * 128, x, sl[r]);
           }
           __syncwarp();
-          sent[is_tail] |= 1u << st.i;
-          sent_ph[is_tail] = (sent_ph[is_tail] & ~(1u << st.i)) | st.ph << st.i;
+          sent |= 1u << st.i;
+          sent_ph = (sent_ph & ~(1u << st.i)) | st.ph << st.i;
         } else {
           // 8 lanes per row; rows that are not there and columns past dq become zeros
           for (int k = lane >> 3; k < 128; k += 4) {
@@ -429,20 +442,15 @@ __global__ void __launch_bounds__(TA_THREADS, 1)
           cp_async_wait_all();
           fence_proxy_async_smem();
           __syncwarp();
-          if (lane == 0) mbar_arrive(&sh->full[st.i][b]);
+          if (lane == 0) mbar_arrive(full);
         }
-      };
-      if (tail && !VT) fetch(true);
-      if (chunk && ok) fetch(false);
-      if (tail && VT && ok) fetch(true);
+      }
       if (lane == 0) mbar_arrive(&sh->a_free[ad.i]);
     }
     // after a timed-out wait: no load of this CTA may land once it has gone
     if (*wc.abort)
-      for (int s = 0; s < TA_STAGES; ++s) {
-        if (sent[0] >> s & 1) mbar_wait(&sh->full[s][lw], sent_ph[0] >> s & 1, wc, false, true);
-        if (sent[1] >> s & 1) mbar_wait(&sh->full[s][4], sent_ph[1] >> s & 1, wc, false, true);
-      }
+      for (int s = 0; s < TA_STAGES; ++s)
+        if (sent >> s & 1) mbar_wait(&sh->full[s][lw], sent_ph >> s & 1, wc, false, true);
   } else if (warp == TA_W_ADDR) {
     // ================================================================ addresses
     TaRing ad;
@@ -451,28 +459,34 @@ __global__ void __launch_bounds__(TA_THREADS, 1)
     for (int u = 0; u < units && ok; ++u, ad.next(TA_AHEAD), w.next_unit(p)) {
       int s[4];
       float k[4];
-      bool whole = true;
+      auto scales = [&] {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) k[i] = s[i] >= 0 ? __ldg(p.scale + s[i]) : -1.f;
+      };
+      auto marked = [&](int i) { return (__float_as_uint(k[i]) & 0x7F800000u) == 0x7F800000u; };
 #pragma unroll
       for (int i = 0; i < 4; ++i) s[i] = ta_slot(p, w, i * 32 + lane);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        k[i] = s[i] >= 0 ? __ldg(p.scale + s[i]) : -1.f;
-        if ((__float_as_uint(k[i]) & 0x7F800000u) == 0x7F800000u) {  // marked: its row is not read
-          k[i] = __uint_as_float(0x7FC00000u);
-          s[i] = -1;
-        }
-        whole &= s[i] >= 0;
-      }
+      // A marked row among the drafted ones is not read (it meets zero weights).  In the
+      // context, which every row sees, it may be: the loads need not wait for the scales.
+      const bool drafted = (w.t + 1) * 128 > w.len;
+      if (drafted) scales();
       ok = __all_sync(0xFFFFFFFFu, mbar_wait_inl(&sh->a_free[ad.i], ad.ph ^ 1, wc));
+      bool whole = true;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        sh->slot[ad.i][i * 32 + lane] = s[i];
-        sh->sk[ad.i][i * 32 + lane] = k[i];
+        const int at = drafted && marked(i) ? -1 : s[i];
+        whole &= at >= 0;
+        sh->slot[ad.i][i * 32 + lane] = at;
       }
       whole = __all_sync(0xFFFFFFFFu, whole);
       if (lane == 0) sh->whole[ad.i] = whole;
       __syncwarp();
       if (lane == 0) mbar_arrive(&sh->a_full[ad.i]);
+      if (!drafted) scales();
+#pragma unroll
+      for (int i = 0; i < 4; ++i) sh->sk[ad.i][i * 32 + lane] = marked(i) ? __uint_as_float(0x7FC00000u) : k[i];
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sh->sk_full[ad.i]);
     }
   } else if (warp == TA_W_QK) {
     // ================================================================ scores
@@ -491,14 +505,6 @@ __global__ void __launch_bounds__(TA_THREADS, 1)
           ok = mbar_wait_inl(&sh->s_free[sq.i], sq.ph ^ 1, wc);
           const uint32_t d = tmem + sq.i * 3 * NR;
           const uint64_t a = k_desc + st.i * stage16;
-          if (p.dr && ok) {
-            ok = mbar_wait_inl(&sh->full[st.i][4], st.ph, wc);
-            tc_fence_after();
-            if (ok)
-#pragma unroll
-              for (int k = 0; k < 4; ++k)
-                umma_bf16_ss(d + 2 * NR, a + p.nc * 1024 + k * 2, q_desc + p.nc * (2 * NR * 8) + k * 2, id_qt, k > 0 ? 1u : 0u);
-          }
           for (int c = 0; c < p.nc && ok; ++c) {
             ok = mbar_wait_inl(&sh->full[st.i][c], st.ph, wc);
             tc_fence_after();
@@ -506,6 +512,14 @@ __global__ void __launch_bounds__(TA_THREADS, 1)
 #pragma unroll
               for (int k = 0; k < 4; ++k)
                 umma_f8_ss(d, a + c * 1024 + k * 2, q_desc + c * (2 * NR * 8) + k * 2, id_qk, c > 0 || k > 0 ? 1u : 0u);
+          }
+          if (p.dr && ok) {
+            ok = mbar_wait_inl(&sh->full[st.i][4], st.ph, wc);
+            tc_fence_after();
+            if (ok)
+#pragma unroll
+              for (int k = 0; k < 4; ++k)
+                umma_bf16_ss(d + 2 * NR, a + p.nc * 1024 + k * 2, q_desc + p.nc * (2 * NR * 8) + k * 2, id_qt, k > 0 ? 1u : 0u);
           }
           if (!ok) break;
           umma_commit(&sh->s_full[sq.i]);
@@ -657,7 +671,7 @@ __global__ void __launch_bounds__(TA_THREADS, 1)
             }
           }
         }
-        mbar_wait_inl(&sh->a_full[ad.i], ad.ph, wc);
+        mbar_wait_inl(&sh->sk_full[ad.i], ad.ph, wc);
         float sk = sh->sk[ad.i][key];
         __syncwarp();
         if (lane == 0) mbar_arrive(&sh->a_free[ad.i]);
@@ -901,30 +915,48 @@ __global__ void __launch_bounds__(TA_THREADS, 1)
 
 // Adds up the parts of row tiles that span CTAs, in order: the tile whose head CTA x holds
 // has its parts in slots 2 x + 1, 2 (x + 1), 2 (x + 2), ...  blockIdx.y: TA_JOIN_ROWS rows.
+// Launched while tree_attn_kernel still runs; it waits for its end here.
 constexpr int TA_JOIN_THREADS = 128;
-constexpr int TA_JOIN_ROWS = 1;
+constexpr int TA_JOIN_ROWS = 2;
 
 template <int NR>
 __global__ void __launch_bounds__(TA_JOIN_THREADS) tree_attn_join_kernel(const TreeAttnParams p) {
+  __shared__ float fs[TA_JOIN_ROWS][TA_MAX_CTAS];  // factor of each part
+  __shared__ float inv[TA_JOIN_ROWS];
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   const int32_t* ow = p.owner + (int64_t)blockIdx.x * 4;
   const int parts = ow[2];
-  const int c = blockIdx.y;
-  const int64_t row = (int64_t)ow[1] * NR + c;
-  if (parts == 0 || row >= p.rows) return;
+  if (parts == 0) return;
   auto slot = [&](int i) { return i == 0 ? 2 * (int64_t)blockIdx.x + 1 : 2 * ((int64_t)blockIdx.x + i); };
-  float m = -INFINITY;
-  for (int i = 0; i < parts; ++i) m = fmaxf(m, p.part_ml[(slot(i) * NR + c) * 2]);
-  const float mu = m == -INFINITY ? 0.f : m;
-  float sum = p.sink && m != -INFINITY ? ex2f(__ldg(p.sink + row % p.H) * 1.4426950408889634f - m) : 0.f;
-  for (int i = 0; i < parts; ++i) {
-    const float2 v = *reinterpret_cast<const float2*>(p.part_ml + (slot(i) * NR + c) * 2);
-    sum += v.y * ex2f(v.x - mu);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (warp < TA_JOIN_ROWS) {
+    const int c = blockIdx.y * TA_JOIN_ROWS + warp;
+    const int64_t row = (int64_t)ow[1] * NR + c;
+    float m = -INFINITY, sum = 0.f;
+    for (int i = lane; i < parts; i += 32) m = fmaxf(m, p.part_ml[(slot(i) * NR + c) * 2]);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
+    const float mu = m == -INFINITY ? 0.f : m;
+    for (int i = lane; i < parts; i += 32) {
+      const float2 v = *reinterpret_cast<const float2*>(p.part_ml + (slot(i) * NR + c) * 2);
+      const float f = ex2f(v.x - mu);
+      fs[warp][i] = f;
+      sum += v.y * f;
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
+    if (p.sink && m != -INFINITY) sum += ex2f(__ldg(p.sink + row % p.H) * 1.4426950408889634f - m);
+    if (lane == 0) inv[warp] = sum == 0.f ? 0.f : 1.f / sum;
   }
-  const float inv = sum == 0.f ? 0.f : 1.f / sum;
-  for (int d = threadIdx.x * 4; d < p.dv; d += TA_JOIN_THREADS * 4) {
+  __syncthreads();
+  for (int e = threadIdx.x * 4; e < TA_JOIN_ROWS * p.dv; e += TA_JOIN_THREADS * 4) {
+    const int r = e / p.dv, d = e - r * p.dv, c = blockIdx.y * TA_JOIN_ROWS + r;
+    const int64_t row = (int64_t)ow[1] * NR + c;
+    if (row >= p.rows) continue;
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
     for (int i = 0; i < parts; ++i) {
-      const float f = ex2f(p.part_ml[(slot(i) * NR + c) * 2] - mu);
+      const float f = fs[r][i];
       const float4 v = *reinterpret_cast<const float4*>(p.part_o + (slot(i) * NR + c) * p.dv + d);
       o.x += v.x * f;
       o.y += v.y * f;
@@ -932,7 +964,7 @@ __global__ void __launch_bounds__(TA_JOIN_THREADS) tree_attn_join_kernel(const T
       o.w += v.w * f;
     }
     *reinterpret_cast<uint2*>(p.out + ((int64_t)ow[0] * p.rows + row) * p.dv + d) =
-        make_uint2(cvt_bf16x2(o.x * inv, o.y * inv), cvt_bf16x2(o.z * inv, o.w * inv));
+        make_uint2(cvt_bf16x2(o.x * inv[r], o.y * inv[r]), cvt_bf16x2(o.z * inv[r], o.w * inv[r]));
   }
 }
 
