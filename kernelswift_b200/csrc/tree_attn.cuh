@@ -181,11 +181,25 @@ struct TaRing {
   }
 };
 
-// Slot of the page pool that holds this position, -1 for none (a pool has < 2^31 slots).
-__device__ __forceinline__ int ta_slot(const TreeAttnParams& p, const TaWalk& w, int key) {
-  const int pos = w.t * 128 + key;
-  if (w.left <= 0 || pos >= ta_keys(p, w.len)) return -1;
-  return (int)cache_row(p.table, p.max_pages, p.n_pages, p.page, w.b, pos, p.status);
+// Slots of the page pool that hold this lane's four keys of a tile (lane, lane + 32, ..),
+// -1 for none.  The four table entries are loaded at once.  (A pool has < 2^31 slots.)
+__device__ __forceinline__ void ta_slots(const TreeAttnParams& p, const TaWalk& w, int lane, int (&s)[4]) {
+  const int keys = ta_keys(p, w.len);
+  const int32_t* table = p.table + (int64_t)w.b * p.max_pages;
+  int pg[4], in[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int pos = w.t * 128 + i * 32 + lane, pi = pos / p.page;  // within the table: keys is
+    in[i] = pos - pi * p.page;
+    pg[i] = ldg_s32_or(table + pi, pos < keys, -1);
+    s[i] = pos < keys;
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const bool ok = pg[i] >= 0 && pg[i] < p.n_pages;
+    if (s[i] && !ok) report_bounds(p.status, w.b, (int)p.n_pages);
+    s[i] = ok ? pg[i] * p.page + in[i] : -1;
+  }
 }
 
 __device__ __forceinline__ void tmem_ld8(uint32_t taddr, uint32_t* r) {
@@ -358,7 +372,8 @@ __global__ void __launch_bounds__(TA_THREADS, 1)
       for (int o = 16; o > 0; o >>= 1) n += __shfl_xor_sync(0xFFFFFFFFu, n, o);
       total += n * p.row_tiles;
     }
-    const int64_t per = (total + gridDim.x - 1) / gridDim.x;
+    const int64_t per = total < (1ll << 31) ? (int64_t)(((uint32_t)total + gridDim.x - 1) / gridDim.x)
+                                            : (total + gridDim.x - 1) / gridDim.x;
     const int64_t u0 = (int64_t)blockIdx.x * per;
     int64_t at = 0;
     bool found = u0 >= total;
@@ -378,8 +393,9 @@ __global__ void __launch_bounds__(TA_THREADS, 1)
         if (over && lane == __ffs(over) - 1) {
           const int64_t in = u0 - (at + n - nt * p.row_tiles);
           sh->b0 = i + k * 32 + lane;
-          sh->rt0 = (int)(in / nt);
-          sh->t0 = (int)(in % nt);
+          const int rt = in < (1ll << 31) ? (int)((uint32_t)in / (uint32_t)nt) : (int)(in / nt);
+          sh->rt0 = rt;
+          sh->t0 = (int)(in - rt * nt);
           sh->len0 = ln;
         }
         found = over != 0;
@@ -464,8 +480,7 @@ __global__ void __launch_bounds__(TA_THREADS, 1)
         for (int i = 0; i < 4; ++i) k[i] = s[i] >= 0 ? __ldg(p.scale + s[i]) : -1.f;
       };
       auto marked = [&](int i) { return (__float_as_uint(k[i]) & 0x7F800000u) == 0x7F800000u; };
-#pragma unroll
-      for (int i = 0; i < 4; ++i) s[i] = ta_slot(p, w, i * 32 + lane);
+      ta_slots(p, w, lane, s);
       // A marked row among the drafted ones is not read (it meets zero weights).  In the
       // context, which every row sees, it may be: the loads need not wait for the scales.
       const bool drafted = (w.t + 1) * 128 > w.len;

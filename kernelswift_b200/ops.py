@@ -26,6 +26,9 @@ or layout) and has no CPU fallback.
 """
 from __future__ import annotations
 
+import contextlib
+import functools
+
 import torch
 
 from ._lib import KS_INT32, KS_INT64, check, lib
@@ -34,13 +37,16 @@ _DV_MAX = 512
 
 
 def _require_cuda(name: str, *tensors: torch.Tensor) -> None:
+    dev, mixed = -1, False
     for t in tensors:
-        if not isinstance(t, torch.Tensor) or t.device.type != "cuda":
+        if not isinstance(t, torch.Tensor) or not t.is_cuda:
             raise RuntimeError(f"{name}: inputs must be CUDA tensors")
         if not t.is_contiguous():
             raise RuntimeError(f"{name}: inputs must be contiguous")
-    dev = tensors[0].device
-    if any(t.device != dev for t in tensors):
+        d = t.get_device()
+        mixed |= dev >= 0 and d != dev
+        dev = d
+    if mixed:
         raise RuntimeError(f"{name}: inputs must be on one device")
 
 
@@ -72,7 +78,17 @@ def _check_workspace(name: str, ws: torch.Tensor, need: int, device) -> None:
 
 
 def _stream(t: torch.Tensor) -> int:
-    return torch.cuda.current_stream(t.device).cuda_stream
+    return torch._C._cuda_getCurrentRawStream(t.get_device())
+
+
+_HERE = contextlib.nullcontext()
+
+
+def _on(t: torch.Tensor):
+    """t's device as the current one; entering nothing where it is already (a few
+    microseconds of a call on a decoding step's path)."""
+    d = t.get_device()
+    return _HERE if torch._C._cuda_getDevice() == d else torch.cuda.device(d)
 
 
 def _ptr(t: torch.Tensor | None) -> int | None:
@@ -459,10 +475,12 @@ def cache_write(kv: torch.Tensor, slots: torch.Tensor, kv8: torch.Tensor, kv_sca
     pages, page, dq, dr, ts = _cache_args("cache_write", kv8, kv_scale, kv_tail)
     if kv.shape[-1] != dq + dr:
         raise RuntimeError(f"cache_write: kv rows have {kv.shape[-1]} columns, the cache {dq + dr}")
-    try:
-        rows = kv.view(-1, dq + dr)
-    except RuntimeError:
-        raise RuntimeError("cache_write: the rows of kv must be a constant stride apart") from None
+    rows = kv
+    if kv.dim() != 2:
+        try:
+            rows = kv.view(-1, dq + dr)
+        except RuntimeError:
+            raise RuntimeError("cache_write: the rows of kv must be a constant stride apart") from None
     R = rows.shape[0]
     if slots.numel() != R:
         raise RuntimeError(f"cache_write: {R} rows but {slots.numel()} slots")
@@ -472,7 +490,7 @@ def cache_write(kv: torch.Tensor, slots: torch.Tensor, kv8: torch.Tensor, kv_sca
     if R and rows.stride(1) != 1:
         raise RuntimeError("cache_write: the columns of kv must be contiguous")
     stride = rows.stride(0) if R > 1 else dq + dr
-    with torch.cuda.device(kv8.device):
+    with _on(kv8):
         check(lib().ks_cache_write(_ptr(rows), stride, _ptr(slots),
                                    KS_INT64 if slots.dtype == torch.int64 else KS_INT32, R,
                                    _ptr(kv8), _ptr(kv_scale), _ptr(kv_tail), pages * page, dq, dr,
@@ -496,13 +514,14 @@ def cache_read(kv8: torch.Tensor, kv_scale: torch.Tensor, kv_tail: torch.Tensor 
         out = torch.empty((B, n, dq + dr), dtype=torch.bfloat16, device=kv8.device)
     else:
         _check_out("cache_read", out, (B, n, dq + dr), torch.bfloat16, kv8.device)
-    with torch.cuda.device(kv8.device):
+    with _on(kv8):
         check(lib().ks_cache_read(_ptr(kv8), _ptr(kv_scale), _ptr(kv_tail), pages, page, dq, dr,
                                   _ptr(page_table), page_table.shape[1], _ptr(lens), B, n, start,
                                   _ptr(out), _stream(kv8)), "ks_cache_read")
     return out
 
 
+@functools.lru_cache(maxsize=256)
 def tree_attn_workspace_size(B: int, T: int, H: int, dv: int) -> int:
     return int(lib().ks_tree_attn_workspace_size(B, T, H, dv))
 
@@ -549,7 +568,7 @@ def tree_attn(q: torch.Tensor, kv8: torch.Tensor, kv_scale: torch.Tensor,
         workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
     else:
         _check_workspace("tree_attn", workspace, need, q.device)
-    with torch.cuda.device(q.device):
+    with _on(q):
         check(lib().ks_tree_attn(_ptr(q), _ptr(kv8), _ptr(kv_scale), _ptr(kv_tail), pages, page,
                                  dq, dr, _ptr(page_table), page_table.shape[1], _ptr(lens),
                                  _ptr(mask), _ptr(attn_sink), _ptr(out), B, T, H, dv,
@@ -603,7 +622,7 @@ def verify_draft(p: torch.Tensor, tokens: torch.Tensor, u: torch.Tensor, noise: 
     out = torch.empty((B, T + 1), dtype=tokens.dtype, device=p.device)
     n_accepted = torch.empty((B,), dtype=torch.int32, device=p.device)
     path = torch.empty((B, T), dtype=torch.int32, device=p.device)
-    with torch.cuda.device(p.device):
+    with _on(p):
         check(lib().ks_verify_draft(_ptr(p), _ptr(q), _ptr(tokens),
                                     KS_INT64 if tokens.dtype == torch.int64 else KS_INT32,
                                     _ptr(parents), _ptr(u), _ptr(noise), B, T, V, _ptr(out),
