@@ -923,16 +923,16 @@ int ks_cache_write(const void* kv, int64_t kv_stride, const void* slots, int32_t
   p.scale = kv_scale;
   p.tail = static_cast<uint16_t*>(kv_tail);
   p.dq = dq; p.dr = dr;
+  p.wide = aligned(kv, 32) && kv_stride % 16 == 0;
   p.status = dev->status;
-  const int lanes = dq <= 64 ? 8 : dq <= 128 ? 16 : 32;
+  const int lanes = dq <= 128 ? 8 : dq <= 512 ? 16 : 32;
   const int64_t blocks = (R + LC_THREADS / lanes - 1) / (LC_THREADS / lanes);
   if (blocks > 0x7FFFFFFFll) return fail(KS_ERR_UNSUPPORTED, "cache_write: too many rows");
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const unsigned g = (unsigned)blocks;
   if (lanes == 8) cache_write_kernel<8, 1><<<g, LC_THREADS, 0, st>>>(p);
-  else if (lanes == 16) cache_write_kernel<16, 1><<<g, LC_THREADS, 0, st>>>(p);
-  else if (dq <= 512) cache_write_kernel<32, 2><<<g, LC_THREADS, 0, st>>>(p);
-  else cache_write_kernel<32, 4><<<g, LC_THREADS, 0, st>>>(p);
+  else if (lanes == 16) cache_write_kernel<16, 2><<<g, LC_THREADS, 0, st>>>(p);
+  else cache_write_kernel<32, 2><<<g, LC_THREADS, 0, st>>>(p);
   return launch_check("cache_write_kernel launch");
 }
 
@@ -960,14 +960,15 @@ int ks_cache_read(const void* kv8, const float* kv_scale, const void* kv_tail, i
   p.lens = lens;
   p.n = (int)n; p.start = (int)start;
   p.out = static_cast<uint16_t*>(out);
+  p.wide = aligned(out, 32) && (dq + dr) % 16 == 0;
   p.status = dev->status;
-  const int lanes = dq <= 128 ? 8 : dq <= 256 ? 16 : 32;
+  const int lanes = dq <= 512 ? 8 : 16;
   const int rows = LC_THREADS / lanes;
   const dim3 grid((unsigned)((n + rows - 1) / rows), (unsigned)B);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (lanes == 8) cache_read_kernel<8><<<grid, LC_THREADS, 0, st>>>(p);
-  else if (lanes == 16) cache_read_kernel<16><<<grid, LC_THREADS, 0, st>>>(p);
-  else cache_read_kernel<32><<<grid, LC_THREADS, 0, st>>>(p);
+  if (dq <= 128) cache_read_kernel<8, 1, 1><<<grid, LC_THREADS, 0, st>>>(p);
+  else if (dq <= 512) cache_read_kernel<8, 4, 1><<<grid, LC_THREADS, 0, st>>>(p);
+  else cache_read_kernel<16, 4, 1><<<grid, LC_THREADS, 0, st>>>(p);
   return launch_check("cache_read_kernel launch");
 }
 
