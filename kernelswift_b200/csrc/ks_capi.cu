@@ -61,7 +61,6 @@ struct Device {
   // memory size it was last asked for
   int sa_clusters = 0;
   size_t sa_clusters_smem = 0;
-  bool vd_wide = false;  // the draft verification's cluster of 16 has been allowed
 };
 constexpr int kMaxDevices = 64;
 std::mutex g_mu;
@@ -1085,10 +1084,11 @@ int ks_verify_draft(const float* p, const float* q, const void* tokens, int32_t 
       !aligned(out, token_dtype == KS_INT64 ? 8 : 4) || (T > 0 && !aligned(tokens, token_dtype == KS_INT64 ? 8 : 4)) ||
       !aligned(path, 4) || !aligned(n_accepted, 4) || (parents && !aligned(parents, 4)))
     return fail(KS_ERR_ALIGNMENT, "verify_draft: pointers must be aligned to their elements");
-  // As many CTAs per sequence as keep the grid within four CTAs per SM, each with at
-  // least a few thousand entries of the row.
+  // As many CTAs per sequence as keep the grid within two CTAs per SM, each with at least a
+  // few thousand entries of the row.  (64 chains over 129280 entries: 8, 4 and 2 CTAs a
+  // sequence 31.4, 26.4 and 36.4 us; 16 trees with 16 and 8: 19.8 and 14.3 us.)
   int cs = VD_MAX_CLUSTER;
-  while (cs > 1 && (B * cs > 4ll * dev->num_sms || V / cs < 2048)) cs >>= 1;
+  while (cs > 1 && (B * cs > 2ll * dev->num_sms || V / cs < 2048)) cs >>= 1;
   VerifyParams vp{};
   vp.p = p; vp.q = q; vp.tokens = tokens;
   vp.tok_i64 = token_dtype == KS_INT64;
@@ -1099,16 +1099,11 @@ int ks_verify_draft(const float* p, const float* q, const void* tokens, int32_t 
   vp.per = (int)round_up((V + cs - 1) / cs, 32);
   vp.status = dev->status;
   // the walk's arrays and, for fixed candidates, one bit per entry of the slice
-  const size_t smem = (size_t)T * 24 + 4 + (q ? 0 : (size_t)vp.per / 8) + 16;
+  const size_t smem = (size_t)T * 28 + 4 + (q ? 0 : (size_t)vp.per / 8) + 16;
   if (smem > 160 * 1024) return fail(KS_ERR_UNSUPPORTED, "verify_draft: V=%lld too large", (long long)V);
   const void* fn = reinterpret_cast<const void*>(verify_draft_kernel);
   if (smem > 40 * 1024)
     if (int rc = smem_optin(dev, fn, "cudaFuncSetAttribute(verify_draft)")) return rc;
-  if (cs > 8 && !dev->vd_wide) {  // once per device
-    cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-    if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(verify_draft cluster)");
-    dev->vd_wide = true;
-  }
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute at[1];
   at[0].id = cudaLaunchAttributeClusterDimension;

@@ -32,7 +32,7 @@ namespace ks {
 
 constexpr int VD_THREADS = 512;
 constexpr int VD_MAX_T = 1024;
-constexpr int VD_MAX_CLUSTER = 16;
+constexpr int VD_MAX_CLUSTER = 8;
 
 struct VerifyParams {
   const float* p;       // [B, T + 1, V]
@@ -72,9 +72,10 @@ __device__ __forceinline__ int64_t vd_token(const VerifyParams& p, int64_t i) {
 
 __global__ void __launch_bounds__(VD_THREADS) verify_draft_kernel(VerifyParams p) {
   extern __shared__ uint32_t vd_smem[];
-  // px [T] double, tok [T], par [T], next [T + 1], path [T], then the slice's bitmap
+  // px [T] double, ux, tok, par [T], next [T + 1], path [T], then the slice's bitmap
   double* px = reinterpret_cast<double*>(vd_smem);
-  int32_t* tok = reinterpret_cast<int32_t*>(px + p.T);
+  float* ux = reinterpret_cast<float*>(px + p.T);
+  int32_t* tok = reinterpret_cast<int32_t*>(ux + p.T);
   int32_t* par = tok + p.T;
   int32_t* next = par + p.T;
   int32_t* path = next + p.T + 1;
@@ -93,6 +94,10 @@ __global__ void __launch_bounds__(VD_THREADS) verify_draft_kernel(VerifyParams p
   // The cluster's CTAs have all started before one writes into another's memory: arrive
   // here, wait there.
   asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
+
+  // The noise does not depend on the walk: this slice of it comes to L2 meanwhile.
+  for (int x = (int)rank * p.per + tid * 32; x < min(V, (int)(rank + 1) * p.per); x += VD_THREADS * 32)
+    asm volatile("prefetch.global.L2 [%0];" ::"l"(p.noise + b * (int64_t)V + x));
 
   // ------------------------------------------------------------------ the walk
   if (tid == 0) {
@@ -117,6 +122,7 @@ __global__ void __launch_bounds__(VD_THREADS) verify_draft_kernel(VerifyParams p
       if (!(__fmul_rn(ub[i], qv) < pv)) atomicMin(&s_n, i);
     } else {
       px[i] = (double)pv;
+      ux[i] = in ? ub[pa + 1] : 0.f;
     }
   }
   __syncthreads();
@@ -124,19 +130,22 @@ __global__ void __launch_bounds__(VD_THREADS) verify_draft_kernel(VerifyParams p
     if (tid == 0) s_end = s_n;
     for (int i = tid; i < T; i += VD_THREADS) path[i] = i;
   } else {
-    // a sibling that repeats an older one's token gives up its stretch
-    for (int i = tid; i < T; i += VD_THREADS)
-      for (int j = 0; j < i; ++j)
-        if (par[j] == par[i] && tok[j] == tok[i]) px[i] = 0.0;
+    // A warp per candidate, lanes over the older ones.  First: a sibling that repeats an
+    // older one's token gives up its stretch.
+    for (int i = tid >> 5; i < T; i += VD_THREADS / 32) {
+      bool dup = false;
+      for (int j = lane; j < i; j += 32) dup |= par[j] == par[i] && tok[j] == tok[i];
+      if (__any_sync(0xFFFFFFFFu, dup) && lane == 0) px[i] = 0.0;
+    }
     __syncthreads();
-    for (int i = tid; i < T; i += VD_THREADS) {
-      const int32_t pa = par[i];
-      if (pa < -1) continue;
-      double at = 0.0;
-      for (int j = 0; j < i; ++j)
-        if (par[j] == pa) at += px[j];
-      const double uu = (double)ub[pa + 1];
-      if (at <= uu && uu < at + px[i]) next[pa + 1] = i;
+    for (int i = tid >> 5; i < T; i += VD_THREADS / 32) {
+      double at = 0.0;  // where its stretch begins
+      for (int j = lane; j < i; j += 32)
+        if (par[j] == par[i]) at += px[j];
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) at += __shfl_xor_sync(0xFFFFFFFFu, at, o);
+      const double uu = (double)ux[i];
+      if (lane == 0 && par[i] >= -1 && at <= uu && uu < at + px[i]) next[par[i] + 1] = i;
     }
     __syncthreads();
     if (tid == 0) {
@@ -166,6 +175,10 @@ __global__ void __launch_bounds__(VD_THREADS) verify_draft_kernel(VerifyParams p
   for (int pass = 0; pass < 2; ++pass) {  // the second only where w is zero everywhere
     best = {-1.f, 0x7FFFFFFF, 0};
     const bool cut = pass == 0;
+    // A ratio below 1 - 2^-20 of the best so far cannot win whatever its rounding, and one
+    // product shows that; the correctly rounded division is left to the few that may.
+    // (An underflowing product is 0 and filters nothing.)
+    float bar = -1.f;
     auto one = [&](int x, float pv, float qv, float nv, bool out) {
       float w = pv;
       if (cut) {
@@ -173,7 +186,10 @@ __global__ void __launch_bounds__(VD_THREADS) verify_draft_kernel(VerifyParams p
         if (out) w = 0.f;
       }
       best.any |= w > 0.f;
-      vd_take(best, __fdiv_rn(w, nv), x);
+      if (w >= bar * nv) {
+        vd_take(best, __fdiv_rn(w, nv), x);
+        bar = best.val * (1.f - 0x1p-20f);
+      }
     };
     if (p.vec4) {
 #pragma unroll 2
