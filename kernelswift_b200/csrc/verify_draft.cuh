@@ -95,10 +95,6 @@ __global__ void __launch_bounds__(VD_THREADS) verify_draft_kernel(VerifyParams p
   // here, wait there.
   asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
 
-  // The noise does not depend on the walk: this slice of it comes to L2 meanwhile.
-  for (int x = (int)rank * p.per + tid * 32; x < min(V, (int)(rank + 1) * p.per); x += VD_THREADS * 32)
-    asm volatile("prefetch.global.L2 [%0];" ::"l"(p.noise + b * (int64_t)V + x));
-
   // ------------------------------------------------------------------ the walk
   if (tid == 0) {
     s_n = T;
@@ -176,9 +172,9 @@ __global__ void __launch_bounds__(VD_THREADS) verify_draft_kernel(VerifyParams p
     best = {-1.f, 0x7FFFFFFF, 0};
     const bool cut = pass == 0;
     // A ratio below 1 - 2^-20 of the best so far cannot win whatever its rounding, and one
-    // product shows that; the correctly rounded division is left to the few that may.
-    // (An underflowing product is 0 and filters nothing.)
-    float bar = -1.f;
+    // product shows that; the correctly rounded division is left to the few that may.  The
+    // best so far is the warp's (a lane's own let most steps of a warp divide).
+    float bar = 0.f;
     auto one = [&](int x, float pv, float qv, float nv, bool out) {
       float w = pv;
       if (cut) {
@@ -186,30 +182,39 @@ __global__ void __launch_bounds__(VD_THREADS) verify_draft_kernel(VerifyParams p
         if (out) w = 0.f;
       }
       best.any |= w > 0.f;
-      if (w >= bar * nv) {
-        vd_take(best, __fdiv_rn(w, nv), x);
-        bar = best.val * (1.f - 0x1p-20f);
-      }
+      if (w >= bar * nv) vd_take(best, __fdiv_rn(w, nv), x);
+    };
+    auto share = [&] {  // non-negative floats are in order as integers
+      const uint32_t top = __reduce_max_sync(0xFFFFFFFFu, __float_as_uint(fmaxf(best.val, 0.f)));
+      bar = __uint_as_float(top) * (1.f - 0x1p-20f);
     };
     if (p.vec4) {
 #pragma unroll 2
-      for (int x = lo + tid * 4; x < hi; x += VD_THREADS * 4) {
-        const float4 pv = __ldg(reinterpret_cast<const float4*>(row + x));
-        const float4 nv = __ldg(reinterpret_cast<const float4*>(e + x));
-        float4 qv = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (qrow) qv = __ldg(reinterpret_cast<const float4*>(qrow + x));
-        uint32_t g = 0;
-        if (!p.q) g = gone[(x - lo) >> 5] >> ((x - lo) & 31);
-        one(x, pv.x, qv.x, nv.x, g & 1);
-        one(x + 1, pv.y, qv.y, nv.y, g & 2);
-        one(x + 2, pv.z, qv.z, nv.z, g & 4);
-        one(x + 3, pv.w, qv.w, nv.w, g & 8);
+      for (int x0 = lo; x0 < hi; x0 += VD_THREADS * 4) {
+        const int x = x0 + tid * 4;
+        if (x < hi) {
+          const float4 pv = __ldg(reinterpret_cast<const float4*>(row + x));
+          const float4 nv = __ldg(reinterpret_cast<const float4*>(e + x));
+          float4 qv = make_float4(0.f, 0.f, 0.f, 0.f);
+          if (qrow) qv = __ldg(reinterpret_cast<const float4*>(qrow + x));
+          uint32_t g = 0;
+          if (!p.q) g = gone[(x - lo) >> 5] >> ((x - lo) & 31);
+          one(x, pv.x, qv.x, nv.x, g & 1);
+          one(x + 1, pv.y, qv.y, nv.y, g & 2);
+          one(x + 2, pv.z, qv.z, nv.z, g & 4);
+          one(x + 3, pv.w, qv.w, nv.w, g & 8);
+        }
+        share();
       }
     } else {
 #pragma unroll 4
-      for (int x = lo + tid; x < hi; x += VD_THREADS) {
-        const uint32_t g = p.q ? 0u : gone[(x - lo) >> 5] >> ((x - lo) & 31);
-        one(x, __ldg(row + x), qrow ? __ldg(qrow + x) : 0.f, __ldg(e + x), g & 1);
+      for (int x0 = lo; x0 < hi; x0 += VD_THREADS) {
+        const int x = x0 + tid;
+        if (x < hi) {
+          const uint32_t g = p.q ? 0u : gone[(x - lo) >> 5] >> ((x - lo) & 31);
+          one(x, __ldg(row + x), qrow ? __ldg(qrow + x) : 0.f, __ldg(e + x), g & 1);
+        }
+        share();
       }
     }
 #pragma unroll
