@@ -32,11 +32,14 @@
 // K = 32 per instruction halves the operand reads, and two tiles fit, so loads run ahead.
 //
 // Work: a unit is one 128-key tile of one (sequence, NR-row tile), NR = 16 or 32 (three
-// output columns per row fill TMEM at 32).  All units of the call in order are cut into
-// equal stretches, one per CTA, whatever the lengths (which only the device knows), so a
-// long context is split over the SMs and ragged batches balance.  A row tile that spans
-// CTAs leaves (maximum, sum, unnormalised output) per part in the workspace;
-// tree_attn_join_kernel adds them up in order (no atomics).
+// output columns per row fill TMEM at 32).  Setting up a row tile's queries and storing its
+// output count as TA_SETUP units more.  The call's units in order are cut into equal
+// stretches, one per CTA, whatever the lengths (which only the device knows), so a long
+// context is split over the SMs and ragged batches balance (16 trees of 13 tokens, 64
+// heads, up to 6001 keys: 270 us with TA_SETUP = 0, when CTAs with many short sequences
+// ran twice as long as the others).  A row tile that spans CTAs leaves (maximum, sum,
+// unnormalised output) per part in the workspace; tree_attn_join_kernel adds them up in
+// order (no atomics).
 //
 // Warps: 8 softmax warps (thread = key = TMEM lane; two share a lane quarter and split the
 // rows), 5 loader warps, a warp that issues the first product and one that issues the
@@ -68,6 +71,7 @@ constexpr int TA_MAX_ROWS = 32;
 constexpr int TA_STAGES = 4;                 // most code tiles in shared memory
 constexpr int TA_AHEAD = 4;                  // tiles whose addresses are held
 constexpr int TA_HDR = 6144;
+constexpr int TA_SETUP = 4;                  // units that a row tile costs beyond its tiles
 constexpr int TA_LEVELS = 3;                 // e5m2 columns per weight
 constexpr float TA_GROW = 5.f;               // how far a score may pass m (base 2)
 constexpr float TA_HEAD = 1.f;               // a raised m lies this far above the score
@@ -112,8 +116,8 @@ struct TaShared {
   uint64_t q_full, drain[2];
   uint32_t tmem_base;
   int abort;
-  int64_t total, per;
-  int32_t b0, rt0, t0, len0;                    // where this CTA's stretch starts
+  int64_t per;                                  // units of a stretch
+  int32_t left0, b0, rt0, t0, len0;             // its first tile, see TaWalk
   float sigma, fs;                              // largest scale so far; factor of its raise
   alignas(16) float m[TA_MAX_ROWS];             // reference of each row (base 2)
   alignas(16) float mneg[TA_MAX_ROWS];          // its negative
@@ -135,22 +139,21 @@ __device__ __forceinline__ int ta_keys(const TreeAttnParams& p, int len) {
 }
 __device__ __forceinline__ int ta_tiles(const TreeAttnParams& p, int len) { return (ta_keys(p, len) + 127) >> 7; }
 
-// A CTA's stretch of units, walked by every role on its own.
+// A CTA's stretch of units, walked by every role on its own.  Tile t of a row tile lies
+// TA_SETUP + t units after the row tile's beginning.
 struct TaWalk {
-  int left;       // units from here to the end of the stretch
-  int b, rt, t;   // this unit
+  int left;       // units from here to the end of the stretch (0: no tile is left)
+  int b, rt, t;   // this tile
   int len, nt;    // of sequence b
   __device__ __forceinline__ void start(const TreeAttnParams& p, const TaShared* sh) {
-    const int64_t u0 = (int64_t)blockIdx.x * sh->per;
-    left = (int)min(sh->per, sh->total - u0);
-    b = sh->b0; rt = sh->rt0; t = sh->t0;
+    left = sh->left0; b = sh->b0; rt = sh->rt0; t = sh->t0;
     len = sh->len0;
     nt = left > 0 ? ta_tiles(p, len) : 0;
   }
-  // units of this row tile that are in the stretch, from here
+  // tiles of this row tile that are in the stretch, from here
   __device__ __forceinline__ int here() const { return min(nt - t, left); }
   __device__ __forceinline__ void next_item(const TreeAttnParams& p, int done) {
-    left -= done;
+    left = max(left - done - TA_SETUP, 0);
     t = 0;
     if (left > 0 && ++rt == p.row_tiles) {
       rt = 0;
@@ -364,7 +367,7 @@ __global__ void __launch_bounds__(TA_THREADS, 1)
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         if (len[k] < 0) continue;
-        n += ta_tiles(p, len[k]);
+        n += ta_tiles(p, len[k]) + TA_SETUP;
         if (blockIdx.x == 0 && (int64_t)len[k] + p.T > p.max_pages * p.page)  // past the table
           report_bounds(p.status, i + k * 32 + lane, (int)p.max_pages);
       }
@@ -375,6 +378,11 @@ __global__ void __launch_bounds__(TA_THREADS, 1)
     const int64_t per = total < (1ll << 31) ? (int64_t)(((uint32_t)total + gridDim.x - 1) / gridDim.x)
                                             : (total + gridDim.x - 1) / gridDim.x;
     const int64_t u0 = (int64_t)blockIdx.x * per;
+    if (lane == 0) {
+      sh->per = per;
+      sh->left0 = 0;
+    }
+    __syncwarp();
     int64_t at = 0;
     bool found = u0 >= total;
     for (int i = 0; i < p.B && !found; i += 128) {
@@ -382,8 +390,8 @@ __global__ void __launch_bounds__(TA_THREADS, 1)
 #pragma unroll 1
       for (int k = 0; k < 4 && !found; ++k) {
         const int ln = k == 0 ? len[0] : k == 1 ? len[1] : k == 2 ? len[2] : len[3];
-        const int64_t nt = ln >= 0 ? ta_tiles(p, ln) : 0;
-        int64_t n = nt * p.row_tiles;  // inclusive sums of the 32 sequences
+        const int64_t un = ln >= 0 ? ta_tiles(p, ln) + TA_SETUP : 0;  // of a row tile
+        int64_t n = un * p.row_tiles;  // inclusive sums of the 32 sequences
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
           const int64_t v = __shfl_up_sync(0xFFFFFFFFu, n, o);
@@ -391,20 +399,18 @@ __global__ void __launch_bounds__(TA_THREADS, 1)
         }
         const uint32_t over = __ballot_sync(0xFFFFFFFFu, at + n > u0);
         if (over && lane == __ffs(over) - 1) {
-          const int64_t in = u0 - (at + n - nt * p.row_tiles);
+          const int64_t in = u0 - (at + n - un * p.row_tiles);  // units into the sequence
+          const int rt = in < (1ll << 31) ? (int)((uint32_t)in / (uint32_t)un) : (int)(in / un);
+          const int into = (int)(in - rt * un);                 // and into the row tile
           sh->b0 = i + k * 32 + lane;
-          const int rt = in < (1ll << 31) ? (int)((uint32_t)in / (uint32_t)nt) : (int)(in / nt);
           sh->rt0 = rt;
-          sh->t0 = (int)(in - rt * nt);
+          sh->t0 = max(into - TA_SETUP, 0);
           sh->len0 = ln;
+          sh->left0 = (int)max(min(per, total - u0) - max(TA_SETUP - into, 0), (int64_t)0);
         }
         found = over != 0;
         at += __shfl_sync(0xFFFFFFFFu, n, 31);
       }
-    }
-    if (lane == 0) {
-      sh->total = total;
-      sh->per = per;
     }
   }
   tc_fence_before();
@@ -425,7 +431,7 @@ __global__ void __launch_bounds__(TA_THREADS, 1)
     TaRing st, ad;
     uint32_t sent = 0, sent_ph = 0;  // stages whose latest load is by TMA, its phase
     bool ok = true;
-    for (int u = 0; u < w.left && ok; ++u, st.next(p.stages), ad.next(TA_AHEAD)) {
+    for (; w.left > 0 && ok; w.next_unit(p), st.next(p.stages), ad.next(TA_AHEAD)) {
       ok = __all_sync(0xFFFFFFFFu, mbar_wait_inl(&sh->a_full[ad.i], ad.ph, wc));
       if (!ok) break;
       const bool whole = p.box && sh->whole[ad.i];
@@ -470,9 +476,8 @@ __global__ void __launch_bounds__(TA_THREADS, 1)
   } else if (warp == TA_W_ADDR) {
     // ================================================================ addresses
     TaRing ad;
-    const int units = max(w.left, 0);
     bool ok = true;
-    for (int u = 0; u < units && ok; ++u, ad.next(TA_AHEAD), w.next_unit(p)) {
+    for (; w.left > 0 && ok; ad.next(TA_AHEAD), w.next_unit(p)) {
       int s[4];
       float k[4];
       auto scales = [&] {
@@ -871,7 +876,7 @@ __global__ void __launch_bounds__(TA_THREADS, 1)
           int32_t* ow = p.owner + (int64_t)blockIdx.x * 4;
           ow[0] = w.b;
           ow[1] = w.rt;
-          // CTAs from this one to the one that holds the last unit
+          // This CTA's part ends with its stretch; the CTAs after it take `per` tiles each.
           ow[2] = 1 + (int)((w.nt - n + sh->per - 1) / sh->per);
         }
         soft_sync();
@@ -932,7 +937,7 @@ __global__ void __launch_bounds__(TA_THREADS, 1)
 // has its parts in slots 2 x + 1, 2 (x + 1), 2 (x + 2), ...  blockIdx.y: TA_JOIN_ROWS rows.
 // Launched while tree_attn_kernel still runs; it waits for its end here.
 constexpr int TA_JOIN_THREADS = 128;
-constexpr int TA_JOIN_ROWS = 2;
+constexpr int TA_JOIN_ROWS = 1;
 
 template <int NR>
 __global__ void __launch_bounds__(TA_JOIN_THREADS) tree_attn_join_kernel(const TreeAttnParams p) {
@@ -969,7 +974,7 @@ __global__ void __launch_bounds__(TA_JOIN_THREADS) tree_attn_join_kernel(const T
     const int64_t row = (int64_t)ow[1] * NR + c;
     if (row >= p.rows) continue;
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
+#pragma unroll 8
     for (int i = 0; i < parts; ++i) {
       const float f = fs[r][i];
       const float4 v = *reinterpret_cast<const float4*>(p.part_o + (slot(i) * NR + c) * p.dv + d);
