@@ -608,7 +608,7 @@ int launch_tree_attn(Device* dev, const CUtensorMap& km, const CUtensorMap& tm, 
   cudaLaunchAttribute at[1];
   at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   at[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.gridDim = dim3(grid, NR / TA_JOIN_ROWS);
+  cfg.gridDim = dim3(grid, NR);
   cfg.blockDim = dim3(TA_JOIN_THREADS);
   cfg.stream = st;
   cfg.attrs = at;

@@ -118,7 +118,7 @@ struct TaShared {
   int abort;
   int64_t per;                                  // units of a stretch
   int32_t left0, b0, rt0, t0, len0;             // its first tile, see TaWalk
-  float sigma, fs;                              // largest scale so far; factor of its raise
+  float sigma, top, fs;                         // largest scale so far, TA_TOP over it; factor of its raise
   alignas(16) float m[TA_MAX_ROWS];             // reference of each row (base 2)
   alignas(16) float mneg[TA_MAX_ROWS];          // its negative
   alignas(16) float qs[TA_MAX_ROWS];            // 2^e * softmax scale of each row
@@ -134,7 +134,7 @@ static_assert(sizeof(TaShared) <= TA_HDR, "TaShared exceeds its header");
 // Keys of sequence b: its cached positions and drafted rows, within the page table.
 __device__ __forceinline__ int ta_len(const TreeAttnParams& p, int b) { return max(0, __ldg(p.lens + b)); }
 __device__ __forceinline__ int ta_keys(const TreeAttnParams& p, int len) {
-  const int64_t cap = p.max_pages * p.page;
+  const int64_t cap = min(p.max_pages * p.page, (int64_t)0x7FFFFF00);
   return (int)min((int64_t)len + p.T, cap);
 }
 __device__ __forceinline__ int ta_tiles(const TreeAttnParams& p, int len) { return (ta_keys(p, len) + 127) >> 7; }
@@ -764,9 +764,11 @@ __global__ void __launch_bounds__(TA_THREADS, 1)
           }
           if (threadIdx.x == 64) {
             const float so = sh->sigma;
-            const float sn = fmaxf(so, fmaxf(fmaxf(sh->red_s[0], sh->red_s[1]), fmaxf(sh->red_s[2], sh->red_s[3])));
+            float sn = fmaxf(so, fmaxf(fmaxf(sh->red_s[0], sh->red_s[1]), fmaxf(sh->red_s[2], sh->red_s[3])));
+            if (sn > 0.f) sn = fmaxf(sn, 0x1p-110f);  // (TA_TOP / sn stays finite)
             sh->fs = so > 0.f ? so / sn : 1.f;  // (powers of two)
             sh->sigma = sn;
+            sh->top = sn > 0.f ? TA_TOP / sn : 0.f;
           }
           soft_sync();
           exponents(false);
@@ -799,7 +801,7 @@ __global__ void __launch_bounds__(TA_THREADS, 1)
           }
         }
         // weights, their sums, and the three parts of each
-        const float fk = marked ? 1.f : sh->sigma > 0.f ? sk * (TA_TOP / sh->sigma) : 0.f;
+        const float fk = marked ? 1.f : sk * sh->top;
         const TaF2 fk2 = f2(fk, fk);
         uint32_t pc[TA_LEVELS][CW / 4], pw[VT ? CW / 2 : 1];
 #pragma unroll
@@ -934,58 +936,63 @@ __global__ void __launch_bounds__(TA_THREADS, 1)
 }
 
 // Adds up the parts of row tiles that span CTAs, in order: the tile whose head CTA x holds
-// has its parts in slots 2 x + 1, 2 (x + 1), 2 (x + 2), ...  blockIdx.y: TA_JOIN_ROWS rows.
-// Launched while tree_attn_kernel still runs; it waits for its end here.
+// has its parts in slots 2 x + 1, 2 (x + 1), 2 (x + 2), ...  A block per CTA and row
+// (blockIdx.y); most find no parts and end at once.  Launched while tree_attn_kernel still
+// runs; it waits for its end here.  A chain of four load latencies: which tile, the parts'
+// maxima and sums, the parts (16 in flight).  Fewer blocks that take rows in turn were
+// slower (48 ragged sequences: 41.0 us with 296, 38.6 with 592, 38.1 so).
 constexpr int TA_JOIN_THREADS = 128;
-constexpr int TA_JOIN_ROWS = 1;
 
 template <int NR>
 __global__ void __launch_bounds__(TA_JOIN_THREADS) tree_attn_join_kernel(const TreeAttnParams p) {
-  __shared__ float fs[TA_JOIN_ROWS][TA_MAX_CTAS];  // factor of each part
-  __shared__ float inv[TA_JOIN_ROWS];
+  constexpr int PL = (TA_MAX_CTAS + 31) / 32;  // parts of a lane
+  __shared__ float fs[TA_JOIN_THREADS / 32][PL * 32];  // factor of each part, a copy per warp
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int32_t* ow = p.owner + (int64_t)blockIdx.x * 4;
-  const int parts = ow[2];
-  if (parts == 0) return;
-  auto slot = [&](int i) { return i == 0 ? 2 * (int64_t)blockIdx.x + 1 : 2 * ((int64_t)blockIdx.x + i); };
+  const int4 ow = *reinterpret_cast<const int4*>(p.owner + (int64_t)blockIdx.x * 4);
+  const int parts = ow.z, c = blockIdx.y;
+  const int64_t row = (int64_t)ow.y * NR + c;
+  if (parts == 0 || row >= p.rows) return;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  if (warp < TA_JOIN_ROWS) {
-    const int c = blockIdx.y * TA_JOIN_ROWS + warp;
-    const int64_t row = (int64_t)ow[1] * NR + c;
-    float m = -INFINITY, sum = 0.f;
-    for (int i = lane; i < parts; i += 32) m = fmaxf(m, p.part_ml[(slot(i) * NR + c) * 2]);
+  auto slot = [&](int i) { return i == 0 ? 2 * (int64_t)blockIdx.x + 1 : 2 * ((int64_t)blockIdx.x + i); };
+  float2 ml[PL];
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
-    const float mu = m == -INFINITY ? 0.f : m;
-    for (int i = lane; i < parts; i += 32) {
-      const float2 v = *reinterpret_cast<const float2*>(p.part_ml + (slot(i) * NR + c) * 2);
-      const float f = ex2f(v.x - mu);
-      fs[warp][i] = f;
-      sum += v.y * f;
-    }
+  for (int k = 0; k < PL; ++k) {
+    const int i = k * 32 + lane;
+    ml[k] = i < parts ? *reinterpret_cast<const float2*>(p.part_ml + (slot(i) * NR + c) * 2)
+                      : make_float2(-INFINITY, 0.f);
+  }
+  float m = ml[0].x;
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
-    if (p.sink && m != -INFINITY) sum += ex2f(__ldg(p.sink + row % p.H) * 1.4426950408889634f - m);
-    if (lane == 0) inv[warp] = sum == 0.f ? 0.f : 1.f / sum;
+  for (int k = 1; k < PL; ++k) m = fmaxf(m, ml[k].x);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
+  const float mu = m == -INFINITY ? 0.f : m;
+  float sum = 0.f;
+#pragma unroll
+  for (int k = 0; k < PL; ++k) {
+    const float f = ex2f(ml[k].x - mu);
+    fs[warp][k * 32 + lane] = f;
+    sum += ml[k].y * f;
   }
-  __syncthreads();
-  for (int e = threadIdx.x * 4; e < TA_JOIN_ROWS * p.dv; e += TA_JOIN_THREADS * 4) {
-    const int r = e / p.dv, d = e - r * p.dv, c = blockIdx.y * TA_JOIN_ROWS + r;
-    const int64_t row = (int64_t)ow[1] * NR + c;
-    if (row >= p.rows) continue;
-    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 8
-    for (int i = 0; i < parts; ++i) {
-      const float f = fs[r][i];
-      const float4 v = *reinterpret_cast<const float4*>(p.part_o + (slot(i) * NR + c) * p.dv + d);
-      o.x += v.x * f;
-      o.y += v.y * f;
-      o.z += v.z * f;
-      o.w += v.w * f;
-    }
-    *reinterpret_cast<uint2*>(p.out + ((int64_t)ow[0] * p.rows + row) * p.dv + d) =
-        make_uint2(cvt_bf16x2(o.x * inv[r], o.y * inv[r]), cvt_bf16x2(o.z * inv[r], o.w * inv[r]));
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
+  if (p.sink && m != -INFINITY) sum += ex2f(__ldg(p.sink + row % p.H) * 1.4426950408889634f - m);
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  __syncwarp();
+  const int d = threadIdx.x * 4;  // dv <= 512
+  if (d >= p.dv) return;
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 16
+  for (int i = 0; i < parts; ++i) {
+    const float f = fs[warp][i];
+    const float4 v = *reinterpret_cast<const float4*>(p.part_o + (slot(i) * NR + c) * p.dv + d);
+    o.x += v.x * f;
+    o.y += v.y * f;
+    o.z += v.z * f;
+    o.w += v.w * f;
   }
+  *reinterpret_cast<uint2*>(p.out + ((int64_t)ow.x * p.rows + row) * p.dv + d) =
+      make_uint2(cvt_bf16x2(o.x * inv, o.y * inv), cvt_bf16x2(o.z * inv, o.w * inv));
 }
 
 }  // namespace ks

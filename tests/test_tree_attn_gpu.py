@@ -2,9 +2,9 @@
 
 Tolerance, per element, A = sum w |v| (bf16 has 8 significant bits: a rounding is off by
 at most 2^-8 of the value): the result is rounded to bf16, 2^-8 of |out| <= A; the
-tensor-core kernel rounds each weight to bf16 before the product with v, at most 2^-8 of
-A; what is left is fp32 (scores of size ~10 off by about 1e-5, sums of exponentials),
-for which 2^-12 of A is room.  |got - exact| <= (2^-8 + 2^-8 + 2^-12) A.
+kernel rounds each weight before the product with v, to bf16 for v's bf16 columns (at most
+2^-8 of A) and to three e5m2 parts for its e4m3 ones (2^-9); what is left is fp32 (scores of
+size ~10 off by about 1e-5, sums of exponentials), for which 2^-12 of A is room.  |got - exact| <= (2^-8 + 2^-8 + 2^-12) A.
 """
 import numpy as np
 import pytest
@@ -121,6 +121,21 @@ def test_large_and_small_magnitudes(cuda_ok):
     g, *a = build(2, 2, 16, 448, 64, 64, [300, 200], seed=12, q_scale=2.0 ** -20,
                   key_scale=lambda x: torch.exp2((x % 41) - 20))
     check(*a, 1.0, 512)
+
+
+@pytest.mark.parametrize("big", [2.0 ** -120, 2.0 ** 60])
+def test_scales_at_the_ends_of_the_range(cuda_ok, big):
+    """A cache filled by hand, its scales (powers of two) far from 1 and some of them 0."""
+    g = torch.Generator(device="cuda").manual_seed(15)
+    pages, page, n = 6, 64, 300
+    code = torch.randint(0, 256, (pages, page, 192), device="cuda", generator=g)
+    code = torch.where((code & 127) == 127, 0x38, code).to(torch.uint8)
+    scale = big * torch.exp2(torch.randint(-3, 4, (pages, page), device="cuda", generator=g).float())
+    scale[:, ::7] = 0
+    q = (torch.randn(1, 2, 20, 192, device="cuda", generator=g) * 0.004 / big).bfloat16()
+    table = torch.arange(pages, device="cuda").int()[None].contiguous()
+    lens = torch.tensor([n], dtype=torch.int32, device="cuda")
+    check(q, code.view(torch.float8_e4m3fn), scale, None, table, lens, 0.07, 192)
 
 
 def test_masks_that_leave_nothing(cuda_ok):
