@@ -227,7 +227,8 @@ int ks_indexer_noalloc(const void* q, const void* k, int64_t k_batch_rows, const
 
 /*
  * The quantised latent cache.  A cached row has D = dq + dr columns: dq in e4m3 with
- * one power-of-two scale per row (as ks_quant_fp8_rows, but at most 2^119), dr (the rotary part) in bf16:
+ * one power-of-two scale per row (as ks_quant_fp8_rows, but at most 2^119), dr (the
+ * rotary part) in bf16:
  *   kv8   e4m3 [n_slots, dq]      kv_scale fp32 [n_slots]      kv_tail bf16 [n_slots, dr]
  * Slot s is row s % page of page s / page; position i of a sequence is row i % page of
  * page page_table[b, i / page].
@@ -308,7 +309,8 @@ int ks_tree_attn(const void* q, const void* kv8, const float* kv_scale, const vo
  * Results: n_accepted int32 [B]; out [B, T + 1] (type of tokens): the accepted tokens,
  * the next token, then -1; path int32 [B, T]: the accepted drafts' indices, then -1.
  * A token outside [0, V) or a parent outside [-1, i) is never accepted and is reported
- * by ks_device_status.  p, q, noise finite.  T <= 1024, V < 2^31.  No counterpart in the reference.
+ * by ks_device_status.  p, q, noise finite.  T <= 1024, V < 2^31.  No counterpart in the
+ * reference.
  */
 int ks_verify_draft(const float* p, const float* q, const void* tokens, int32_t token_dtype,
                     const int32_t* parents, const float* u, const float* noise, int64_t B,
