@@ -603,6 +603,7 @@ int launch_tree_attn(Device* dev, const CUtensorMap& km, const CUtensorMap& tm, 
     return rc;
   tree_attn_kernel<NR, VT><<<grid, TA_THREADS, smem, st>>>(km, tm, p);
   if (int rc = launch_check("tree_attn_kernel launch")) return rc;
+  if (p.solo) return KS_OK;
   // set up while the kernel above runs; it waits for that kernel's end itself
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute at[1];
@@ -1047,7 +1048,14 @@ int ks_tree_attn(const void* q, const void* kv8, const float* kv_scale, const vo
   p.budget_ns = wait_budget_ns();
   // no more CTAs than there can be units (the lengths are known on the device only)
   const int64_t most = B * p.row_tiles * std::max<int64_t>(1, (max_pages * page + 127) / 128);
-  const unsigned grid = (unsigned)std::min<int64_t>(most, std::min(dev->num_sms, TA_MAX_CTAS));
+  const int64_t sms = std::min(dev->num_sms, TA_MAX_CTAS);
+  // Short tables: a CTA per row tile and no join, which costs about six tiles.  (16 heads of
+  // 576 columns, split against whole: one sequence of 510 keys 12.5 and 12.9 us, 40 of them
+  // 16.9 and 13.8, 100 19.4 and 14.5; one of 1022 keys 13.1 and 18.5, 40 19.0 and 19.0,
+  // 100 28.4 and 22.9.)
+  const int64_t items = B * p.row_tiles;
+  p.solo = items <= sms && max_pages * page <= (items * 4 >= sms ? 2 * TA_SOLO : TA_SOLO);
+  const unsigned grid = (unsigned)(p.solo ? items : std::min(most, sms));
   p.part_o = static_cast<float*>(workspace);
   p.part_ml = p.part_o + 2ll * grid * nr * dv;
   p.owner = reinterpret_cast<int32_t*>(p.part_ml + 4ll * grid * nr);

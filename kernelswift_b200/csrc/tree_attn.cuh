@@ -72,6 +72,7 @@ constexpr int TA_STAGES = 4;                 // most code tiles in shared memory
 constexpr int TA_AHEAD = 4;                  // tiles whose addresses are held
 constexpr int TA_HDR = 6144;
 constexpr int TA_SETUP = 4;                  // units that a row tile costs beyond its tiles
+constexpr int TA_SOLO = 512;                 // keys of a table up to which a CTA takes a row tile whole (see the host code)
 constexpr int TA_LEVELS = 3;                 // e5m2 columns per weight
 constexpr float TA_GROW = 5.f;               // how far a score may pass m (base 2)
 constexpr float TA_HEAD = 1.f;               // a raised m lies this far above the score
@@ -96,6 +97,7 @@ struct TreeAttnParams {
   int32_t dt;             // 128-dim tiles of O^T from codes
   int32_t stages, s_bufs;
   int32_t box;            // rows of a TMA box, 0: no TMA
+  int32_t solo;           // a CTA per row tile, nothing to join
   uint32_t stage_bytes, k_off, q_off, p_off, pb_off;
   uint32_t tmem_cols;
   float scale_log2;
@@ -291,6 +293,21 @@ __device__ __forceinline__ TaF2 mul2(TaF2 a, TaF2 b) {
   asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
   return r;
 }
+__device__ __forceinline__ uint32_t f16x2_of(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+__device__ __forceinline__ uint16_t e4m3x2_of_f16x2(uint32_t x) {
+  uint16_t c;
+  asm("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;" : "=h"(c) : "r"(x));
+  return c;
+}
+__device__ __forceinline__ uint32_t mul_f16x2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
 __device__ __forceinline__ uint32_t sub_f16x2(uint32_t a, uint32_t b) {
   uint32_t r;
   asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
@@ -353,7 +370,19 @@ __global__ void __launch_bounds__(TA_THREADS, 1)
       if (p.dr) tma_prefetch_desc(&tm);
     }
   }
-  if (warp == TA_W_ADDR) {  // the call's units, and where this CTA's stretch starts
+  if (warp == TA_W_ADDR && p.solo) {
+    const int b = (int)blockIdx.x / p.row_tiles, rt = (int)blockIdx.x - b * p.row_tiles, len = ta_len(p, b);
+    if (lane == 0) {
+      sh->per = 0;
+      sh->b0 = b;
+      sh->rt0 = rt;
+      sh->t0 = 0;
+      sh->len0 = len;
+      sh->left0 = ta_tiles(p, len);
+      if (rt == 0 && (int64_t)len + p.T > p.max_pages * p.page)  // past the table
+        report_bounds(p.status, b, (int)p.max_pages);
+    }
+  } else if (warp == TA_W_ADDR) {  // the call's units, and where this CTA's stretch starts
     // 128 sequences at a time, their lengths loaded at once (and kept where that is all)
     int len[4];
     auto lengths = [&](int i) {
@@ -636,12 +665,12 @@ __global__ void __launch_bounds__(TA_THREADS, 1)
         uint32_t hi[2] = {0, 0}, lo[2] = {0, 0};
 #pragma unroll
         for (int z = 0; z < 4; ++z) {
-          const float a = bf16lo_f32(y[z]) * inv, b = bf16hi_f32(y[z]) * inv;
-          const uint16_t h = cvt_e4m3x2(a, b);
-          const uint32_t back = f16x2_of_e4m3x2(h);
-          const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&back));
+          // (in fp16: below 256 the 8 bits of a bf16 are exact down to 2^-17)
+          const uint32_t a = f16x2_of(bf16lo_f32(y[z]) * inv, bf16hi_f32(y[z]) * inv);
+          const uint16_t h = e4m3x2_of_f16x2(a);
+          const uint32_t rest = mul_f16x2(sub_f16x2(a, f16x2_of_e4m3x2(h)), 0x4C004C00u);  // x 16
           hi[z >> 1] |= (uint32_t)h << (16 * (z & 1));
-          lo[z >> 1] |= (uint32_t)cvt_e4m3x2((a - f.x) * 16.f, (b - f.y) * 16.f) << (16 * (z & 1));
+          lo[z >> 1] |= (uint32_t)e4m3x2_of_f16x2(rest) << (16 * (z & 1));
         }
         uint8_t* dst = qs + (c8 >> 4) * (2 * NR * 128) + row * 128 + ((((c8 & 15) >> 1) ^ (row & 7)) << 4) + (c8 & 1) * 8;
         // a row with a NaN or an infinity scores NaN
@@ -815,7 +844,7 @@ __global__ void __launch_bounds__(TA_THREADS, 1)
             if constexpr (VT) pw[c / 2 + z] = cvt_bf16x2(e0, e1);
             float w0, w1;
             f2_get(mul2(e, fk2), w0, w1);
-            asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(h[z]) : "f"(w1), "f"(w0));
+            h[z] = f16x2_of(w0, w1);
             h1[z] = sub_f16x2(h[z], h[z] & 0xFF00FF00u);
             h2[z] = sub_f16x2(h1[z], h1[z] & 0xFF00FF00u) + 0x00800080u;  // the last part rounded to nearest
           }

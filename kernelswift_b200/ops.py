@@ -511,7 +511,7 @@ def cache_read(kv8: torch.Tensor, kv_scale: torch.Tensor, kv_tail: torch.Tensor 
         raise RuntimeError("cache_read: n and start must not be negative")
     _require_cuda("cache_read", *ts, page_table, lens)
     if out is None:
-        out = torch.empty((B, n, dq + dr), dtype=torch.bfloat16, device=kv8.device)
+        out = torch.empty(B, n, dq + dr, dtype=torch.bfloat16, device=kv8.device)
     else:
         _check_out("cache_read", out, (B, n, dq + dr), torch.bfloat16, kv8.device)
     with _on(kv8):
@@ -560,7 +560,7 @@ def tree_attn(q: torch.Tensor, kv8: torch.Tensor, kv_scale: torch.Tensor,
     _require_cuda("tree_attn", *ts)
     dv = min(D, _DV_MAX) if dv is None else int(dv)
     if out is None:
-        out = torch.empty((B, T, H, dv), dtype=torch.bfloat16, device=q.device)
+        out = torch.empty(B, T, H, dv, dtype=torch.bfloat16, device=q.device)
     else:
         _check_out("tree_attn", out, (B, T, H, dv), torch.bfloat16, q.device)
     need = tree_attn_workspace_size(B, T, H, dv)
@@ -619,9 +619,9 @@ def verify_draft(p: torch.Tensor, tokens: torch.Tensor, u: torch.Tensor, noise: 
             raise RuntimeError("verify_draft: parents must be int32 [b, t]")
         ts.append(parents)
     _require_cuda("verify_draft", *ts)
-    out = torch.empty((B, T + 1), dtype=tokens.dtype, device=p.device)
-    n_accepted = torch.empty((B,), dtype=torch.int32, device=p.device)
-    path = torch.empty((B, T), dtype=torch.int32, device=p.device)
+    out = torch.empty(B, T + 1, dtype=tokens.dtype, device=p.device)
+    n_accepted = torch.empty(B, dtype=torch.int32, device=p.device)
+    path = torch.empty(B, T, dtype=torch.int32, device=p.device)
     with _on(p):
         check(lib().ks_verify_draft(_ptr(p), _ptr(q), _ptr(tokens),
                                     KS_INT64 if tokens.dtype == torch.int64 else KS_INT32,

@@ -100,6 +100,18 @@ def test_long_context_is_split_and_joined(cuda_ok, H, T, n):
     check(*a, 576 ** -0.5, 512, rows=[0, T - 1])
 
 
+@pytest.mark.parametrize("B,T,H,n", [(1, 1, 16, 500), (3, 5, 24, 130), (40, 1, 16, 900), (9, 7, 64, 250)])
+def test_short_contexts_in_short_and_wide_tables(cuda_ok, B, T, H, n):
+    """A short table takes a CTA per row tile, a wide one (whose entries past the context are
+    never looked at) is split: both are right."""
+    g, q, kv8, scale, tail, table, lens = build(B, T, H, 448, 64, 32, [max(0, n - 31 * b) for b in range(B)], seed=n)
+    sink = torch.randn(H, device="cuda", generator=g)
+    mask = tree_mask(g, B, T)
+    wide = torch.cat([table, torch.full((B, 300), -7, device="cuda", dtype=torch.int32)], 1)
+    for t in (table, wide):
+        check(q, kv8, scale, tail, t, lens, 512 ** -0.5, 512, mask, sink)
+
+
 @pytest.mark.parametrize("tree", [False, True])
 def test_rows_of_many_sequences_at_once(cuda_ok, tree):
     """More work items than CTAs, ragged, some sequences empty."""
