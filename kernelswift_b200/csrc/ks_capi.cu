@@ -601,7 +601,7 @@ int launch_tree_attn(Device* dev, const CUtensorMap& km, const CUtensorMap& tm, 
                      size_t smem, cudaStream_t st) {
   if (int rc = smem_optin(dev, reinterpret_cast<const void*>(tree_attn_kernel<NR, VT>), "cudaFuncSetAttribute(tree_attn)"))
     return rc;
-  tree_attn_kernel<NR, VT><<<grid, TA_THREADS, smem, st>>>(km, tm, p);
+  tree_attn_kernel<NR, VT><<<grid, TA_THREADS<NR>, smem, st>>>(km, tm, p);
   if (int rc = launch_check("tree_attn_kernel launch")) return rc;
   if (p.solo) return KS_OK;
   // set up while the kernel above runs; it waits for that kernel's end itself
@@ -1023,17 +1023,19 @@ int ks_tree_attn(const void* q, const void* kv8, const float* kv_scale, const vo
   p.nc = (dq + 127) / 128;
   p.dt = (int)((std::min<int64_t>(dv, dq) + 127) / 128);
   const bool vt = dv > dq;  // v reaches into the bf16 columns
-  // shared memory: as many code tiles as fit (two at D = 576)
-  p.stage_bytes = (uint32_t)(p.nc + (dr ? 1 : 0)) * 16384;
+  // shared memory: as many chunks of codes as fit (nine at D = 576, four a tile).  One tail
+  // chunk is enough where only the scores read it: they are done a tile before the next's.
   const size_t q_bytes = (size_t)p.nc * 2 * nr * 128 + (dr ? (size_t)nr * 128 : 0);
   const size_t fixed = 1024 + TA_HDR + q_bytes + 16384 + (vt ? 8192 : 0);
-  p.stages = (int)std::min<size_t>((232448 - fixed) / p.stage_bytes, TA_STAGES);
-  if (p.stages < 1) return fail(KS_ERR_UNSUPPORTED, "tree_attn: shared memory too small");
+  p.tails = dr ? (vt ? 2 : 1) : 0;
+  p.slots = (int)std::min<size_t>((232448 - fixed) / TA_CHUNK - p.tails, TA_SLOTS);
+  if (p.slots < p.nc) return fail(KS_ERR_UNSUPPORTED, "tree_attn: shared memory too small");
   p.k_off = TA_HDR;
-  p.q_off = p.k_off + (uint32_t)p.stages * p.stage_bytes;
+  p.t_off = p.k_off + (uint32_t)p.slots * TA_CHUNK;
+  p.q_off = p.t_off + (uint32_t)p.tails * TA_CHUNK;
   p.p_off = p.q_off + (uint32_t)q_bytes;
   p.pb_off = p.p_off + 16384;
-  const size_t smem = fixed + (size_t)p.stages * p.stage_bytes;
+  const size_t smem = fixed + (size_t)(p.slots + p.tails) * TA_CHUNK;
   const int o_cols = p.dt * TA_LEVELS * nr + (vt ? nr : 0);
   p.s_bufs = o_cols + 2 * 3 * nr <= 512 ? 2 : 1;
   p.tmem_cols = 32;

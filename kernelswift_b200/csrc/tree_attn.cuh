@@ -62,13 +62,16 @@
 
 namespace ks {
 
-constexpr int TA_SOFT = 256;                 // softmax threads (warps 0-7)
-constexpr int TA_LOADERS = 5;                // loader warps (8-12): a chunk each, the tail
-constexpr int TA_W_LOAD = 8, TA_W_QK = 13, TA_W_PV = 14, TA_W_ADDR = 15;
-constexpr int TA_THREADS = 16 * 32;
+constexpr int TA_CW = 8;                     // rows of a softmax thread
+constexpr int TA_LOADERS = 5;                // loader warps: a chunk each, the tail
+template <int NR>
+constexpr int TA_SOFT = NR / TA_CW * 128;    // softmax threads (the first ones)
+template <int NR>
+constexpr int TA_THREADS = TA_SOFT<NR> + (TA_LOADERS + 3) * 32;
 constexpr int TA_MAX_CTAS = 148;             // SMs of a B200: bounds the workspace
 constexpr int TA_MAX_ROWS = 32;
-constexpr int TA_STAGES = 4;                 // most code tiles in shared memory
+constexpr int TA_SLOTS = 12;                 // most code chunks in shared memory
+constexpr uint32_t TA_CHUNK = 16384;         // 128 keys of 128 bytes
 constexpr int TA_AHEAD = 4;                  // tiles whose addresses are held
 constexpr int TA_HDR = 6144;
 constexpr int TA_SETUP = 4;                  // units that a row tile costs beyond its tiles
@@ -95,10 +98,11 @@ struct TreeAttnParams {
   int32_t row_tiles;      // ceil(rows / NR)
   int32_t nc;             // 128-column chunks of codes
   int32_t dt;             // 128-dim tiles of O^T from codes
-  int32_t stages, s_bufs;
+  int32_t slots, tails;   // code chunks and tail chunks in shared memory
+  int32_t s_bufs;
   int32_t box;            // rows of a TMA box, 0: no TMA
   int32_t solo;           // a CTA per row tile, nothing to join
-  uint32_t stage_bytes, k_off, q_off, p_off, pb_off;
+  uint32_t k_off, t_off, q_off, p_off, pb_off;
   uint32_t tmem_cols;
   float scale_log2;
   float* part_o;          // [2 * CTAs][NR][dv]
@@ -109,8 +113,8 @@ struct TreeAttnParams {
 };
 
 struct TaShared {
-  uint64_t full[TA_STAGES][5];                  // a chunk of a tile (4: the tail) is in place
-  uint64_t kfree[TA_STAGES][5];                 // it has been used
+  uint64_t full[TA_SLOTS + 2];                  // a chunk is in place (the last two: the tail)
+  uint64_t kfree[TA_SLOTS + 2];                 // it has been used
   uint64_t s_full[2], s_free[2];                // scores are in TMEM / in registers
   uint64_t p_full, pv_done;                     // weights are in shared memory / have been used
   uint64_t a_full[TA_AHEAD], a_free[TA_AHEAD];  // a tile's addresses are in place / used
@@ -118,6 +122,7 @@ struct TaShared {
   uint64_t q_full, drain[2];
   uint32_t tmem_base;
   int abort;
+  uint32_t issued[TA_SLOTS + 2];                // loads of the chunk so far
   int64_t per;                                  // units of a stretch
   int32_t left0, b0, rt0, t0, len0;             // its first tile, see TaWalk
   float sigma, top, fs;                         // largest scale so far, TA_TOP over it; factor of its raise
@@ -228,16 +233,15 @@ __device__ __forceinline__ void tmem_stn(uint32_t taddr, const float* r) {
   else tmem_st16(taddr, reinterpret_cast<const uint32_t*>(r));
 }
 // Any thread of the softmax warps (also a barrier among them).
+template <int SOFT>
 __device__ __forceinline__ bool soft_any(bool x) {
   uint32_t r;
   asm volatile("{ .reg .pred p, q; setp.ne.u32 p, %1, 0; bar.red.or.pred q, 1, %2, p; selp.u32 %0, 1, 0, q; }"
                : "=r"(r)
-               : "r"((uint32_t)x), "n"(TA_SOFT)
+               : "r"((uint32_t)x), "n"(SOFT)
                : "memory");
   return r != 0;
 }
-
-__device__ __forceinline__ void soft_sync() { named_bar_sync(1, TA_SOFT); }
 
 // Max or sum over the warp's lanes of CW <= 16 values each into red[c], c < CW.
 template <bool MX, int CW>
@@ -315,16 +319,18 @@ __device__ __forceinline__ uint32_t sub_f16x2(uint32_t a, uint32_t b) {
 }
 
 template <int NR, bool VT>
-__global__ void __launch_bounds__(TA_THREADS, 1)
+__global__ void __launch_bounds__(TA_THREADS<NR>, 1)
     tree_attn_kernel(const __grid_constant__ CUtensorMap km, const __grid_constant__ CUtensorMap tm,
                      const TreeAttnParams p) {
-  constexpr int CW = NR / 2;             // rows of a softmax thread
+  constexpr int CW = TA_CW, SOFT = TA_SOFT<NR>;
+  constexpr int W_LOAD = SOFT / 32, W_QK = W_LOAD + TA_LOADERS, W_PV = W_QK + 1, W_ADDR = W_PV + 1;
   constexpr int NP = TA_LEVELS * NR;     // columns of P and of a dim tile of O^T
   extern __shared__ uint8_t ta_raw[];
   const uint32_t raw = smem_u32(ta_raw);
   uint8_t* smem = ta_raw + (((raw + 1023u) & ~1023u) - raw);
   TaShared* sh = reinterpret_cast<TaShared*>(smem);
-  uint8_t* ks_ = smem + p.k_off;  // [stages]: [nc][128 keys x 128 B] codes, [128 keys x 128 B] bf16 tail
+  uint8_t* ks_ = smem + p.k_off;  // [slots][128 keys x 128 B] codes: a ring of chunks, nc a tile
+  uint8_t* kt = smem + p.t_off;   // [tails][128 keys x 128 B] bf16 tail
   uint8_t* qs = smem + p.q_off;   // [nc][NR hi rows, NR lo rows x 128 B], [NR x 128 B] bf16 tail
   uint8_t* ps = smem + p.p_off;   // [128 keys x 128 B]: level, row (MN-major)
   uint8_t* pb = smem + p.pb_off;  // [128 keys x 64 B]: bf16 weights (MN-major), with vt
@@ -332,24 +338,23 @@ __global__ void __launch_bounds__(TA_THREADS, 1)
   WaitCtx wc{&sh->abort, p.status, p.budget_ns};
 
   if (threadIdx.x == 0) {
-    for (int s = 0; s < TA_STAGES; ++s) {
-      for (int c = 0; c < 5; ++c) {
-        mbar_init(&sh->full[s][c], 1);
-        mbar_init(&sh->kfree[s][c], 1);
-      }
+    for (int s = 0; s < TA_SLOTS + 2; ++s) {
+      mbar_init(&sh->full[s], 1);
+      mbar_init(&sh->kfree[s], 1);
+      sh->issued[s] = 0;
     }
     for (int s = 0; s < 2; ++s) {
       mbar_init(&sh->s_full[s], 1);
-      mbar_init(&sh->s_free[s], TA_SOFT / 32);
+      mbar_init(&sh->s_free[s], SOFT / 32);
     }
-    mbar_init(&sh->p_full, TA_SOFT / 32);
+    mbar_init(&sh->p_full, SOFT / 32);
     mbar_init(&sh->pv_done, 1);
     for (int s = 0; s < TA_AHEAD; ++s) {
       mbar_init(&sh->a_full[s], 1);
       mbar_init(&sh->sk_full[s], 1);
-      mbar_init(&sh->a_free[s], TA_LOADERS + TA_SOFT / 32);
+      mbar_init(&sh->a_free[s], TA_LOADERS + SOFT / 32);
     }
-    mbar_init(&sh->q_full, TA_SOFT / 32);
+    mbar_init(&sh->q_full, SOFT / 32);
     mbar_init(&sh->drain[0], 1);
     mbar_init(&sh->drain[1], 1);
     sh->abort = 0;
@@ -362,7 +367,7 @@ __global__ void __launch_bounds__(TA_THREADS, 1)
     sh->m[threadIdx.x] = -INFINITY;
     sh->mneg[threadIdx.x] = INFINITY;
   }
-  if (warp == TA_W_QK) {
+  if (warp == W_QK) {
     tmem_alloc<1>(&sh->tmem_base, p.tmem_cols);
     tmem_relinquish<1>();
     if (lane == 0 && p.box) {
@@ -370,7 +375,7 @@ __global__ void __launch_bounds__(TA_THREADS, 1)
       if (p.dr) tma_prefetch_desc(&tm);
     }
   }
-  if (warp == TA_W_ADDR && p.solo) {
+  if (warp == W_ADDR && p.solo) {
     const int b = (int)blockIdx.x / p.row_tiles, rt = (int)blockIdx.x - b * p.row_tiles, len = ta_len(p, b);
     if (lane == 0) {
       sh->per = 0;
@@ -382,7 +387,7 @@ __global__ void __launch_bounds__(TA_THREADS, 1)
       if (rt == 0 && (int64_t)len + p.T > p.max_pages * p.page)  // past the table
         report_bounds(p.status, b, (int)p.max_pages);
     }
-  } else if (warp == TA_W_ADDR) {  // the call's units, and where this CTA's stretch starts
+  } else if (warp == W_ADDR) {  // the call's units, and where this CTA's stretch starts
     // 128 sequences at a time, their lengths loaded at once (and kept where that is all)
     int len[4];
     auto lengths = [&](int i) {
@@ -451,36 +456,38 @@ __global__ void __launch_bounds__(TA_THREADS, 1)
   TaWalk w;
   w.start(p, sh);
 
-  if (warp >= TA_W_LOAD && warp < TA_W_QK) {
+  if (warp >= W_LOAD && warp < W_QK) {
     // ================================================================ loaders
     // Warp c loads chunk c, warp 4 the tail.
-    const int lw = warp - TA_W_LOAD, piece = lane & 7;
+    const int lw = warp - W_LOAD, piece = lane & 7;
     const bool is_tail = lw == 4;
     const int x = is_tail ? 0 : lw * 128;
-    TaRing st, ad;
-    uint32_t sent = 0, sent_ph = 0;  // stages whose latest load is by TMA, its phase
+    const bool mine = is_tail ? p.dr > 0 : lw < p.nc;
+    const int step = is_tail ? 1 : p.nc, ring = is_tail ? p.tails : p.slots;
+    int at = is_tail ? 0 : lw;  // place in the ring, its phase
+    uint32_t ph = 0;
+    TaRing ad;
     bool ok = true;
-    for (; w.left > 0 && ok; w.next_unit(p), st.next(p.stages), ad.next(TA_AHEAD)) {
+    for (; w.left > 0 && ok; w.next_unit(p), ad.next(TA_AHEAD)) {
       ok = __all_sync(0xFFFFFFFFu, mbar_wait_inl(&sh->a_full[ad.i], ad.ph, wc));
       if (!ok) break;
       const bool whole = p.box && sh->whole[ad.i];
       const int32_t* sl = sh->slot[ad.i];
-      if (is_tail ? p.dr > 0 : lw < p.nc) {
+      if (mine) {
         // The second product's dim tiles free their chunks one by one, chunks that only the
-        // scores read go with their end.
-        uint64_t* full = &sh->full[st.i][lw];
-        ok = __all_sync(0xFFFFFFFFu, mbar_wait_inl(&sh->kfree[st.i][lw], st.ph ^ 1, wc));
+        // scores read go with theirs.
+        const int bar = is_tail ? TA_SLOTS + at : at;
+        uint64_t* full = &sh->full[bar];
+        ok = __all_sync(0xFFFFFFFFu, mbar_wait_inl(&sh->kfree[bar], ph ^ 1, wc));
         if (!ok) break;
-        uint8_t* dst = ks_ + (size_t)st.i * p.stage_bytes + (is_tail ? p.nc : lw) * 16384;
-        sent &= ~(1u << st.i);
+        uint8_t* dst = (is_tail ? kt : ks_) + (size_t)at * TA_CHUNK;
+        if (lane == 0) ++sh->issued[bar];
         if (whole) {
           if (elect_one()) {
-            mbar_expect_tx(full, 16384);
+            mbar_expect_tx(full, TA_CHUNK);
             for (int r = 0; r < 128; r += p.box) tma_load_2d(is_tail ? &tm : &km, full, dst + r * 128, x, sl[r]);
           }
           __syncwarp();
-          sent |= 1u << st.i;
-          sent_ph = (sent_ph & ~(1u << st.i)) | st.ph << st.i;
         } else {
           // 8 lanes per row; rows that are not there and columns past dq become zeros
           for (int k = lane >> 3; k < 128; k += 4) {
@@ -495,14 +502,15 @@ __global__ void __launch_bounds__(TA_THREADS, 1)
           __syncwarp();
           if (lane == 0) mbar_arrive(full);
         }
+        at += step;  // (step <= ring)
+        if (at >= ring) {
+          at -= ring;
+          ph ^= 1;
+        }
       }
       if (lane == 0) mbar_arrive(&sh->a_free[ad.i]);
     }
-    // after a timed-out wait: no load of this CTA may land once it has gone
-    if (*wc.abort)
-      for (int s = 0; s < TA_STAGES; ++s)
-        if (sent >> s & 1) mbar_wait(&sh->full[s][lw], sent_ph >> s & 1, wc, false, true);
-  } else if (warp == TA_W_ADDR) {
+  } else if (warp == W_ADDR) {
     // ================================================================ addresses
     TaRing ad;
     bool ok = true;
@@ -537,43 +545,47 @@ __global__ void __launch_bounds__(TA_THREADS, 1)
       __syncwarp();
       if (lane == 0) mbar_arrive(&sh->sk_full[ad.i]);
     }
-  } else if (warp == TA_W_QK) {
+  } else if (warp == W_QK) {
     // ================================================================ scores
     if (elect_one()) {
       // descriptors: only the start address (low word, 16-byte units) changes
       const uint64_t k_desc = sdesc_sw128(smem_u32(ks_), 16, 1024), q_desc = sdesc_sw128(smem_u32(qs), 16, 1024);
       const uint32_t id_qk = idesc_e4m3_f32(128, 2 * NR), id_qt = idesc_bf16_f32(128, NR, false, false);
-      const uint32_t stage16 = p.stage_bytes >> 4;
-      TaRing st, sq;
+      const uint64_t t_desc = sdesc_sw128(smem_u32(kt), 16, 1024);
+      TaRing sl, st, sq;
       uint32_t items = 0;
       bool ok = true;
       for (; w.left > 0 && ok; ++items) {
         const int n = w.here();
         ok = mbar_wait_inl(&sh->q_full, items & 1, wc);
-        for (int i = 0; i < n && ok; ++i, st.next(p.stages), sq.next(p.s_bufs)) {
+        for (int i = 0; i < n && ok; ++i, sq.next(p.s_bufs)) {
           ok = mbar_wait_inl(&sh->s_free[sq.i], sq.ph ^ 1, wc);
           const uint32_t d = tmem + sq.i * 3 * NR;
-          const uint64_t a = k_desc + st.i * stage16;
-          for (int c = 0; c < p.nc && ok; ++c) {
-            ok = mbar_wait_inl(&sh->full[st.i][c], st.ph, wc);
+          for (int c = 0; c < p.nc && ok; ++c, sl.next(p.slots)) {
+            ok = mbar_wait_inl(&sh->full[sl.i], sl.ph, wc);
             tc_fence_after();
-            if (ok)
+            if (!ok) break;
 #pragma unroll
-              for (int k = 0; k < 4; ++k)
-                umma_f8_ss(d, a + c * 1024 + k * 2, q_desc + c * (2 * NR * 8) + k * 2, id_qk, c > 0 || k > 0 ? 1u : 0u);
+            for (int k = 0; k < 4; ++k)
+              umma_f8_ss(d, k_desc + sl.i * (TA_CHUNK >> 4) + k * 2, q_desc + c * (2 * NR * 8) + k * 2, id_qk,
+                         c > 0 || k > 0 ? 1u : 0u);
+            if (c >= p.dt) umma_commit(&sh->kfree[sl.i]);
           }
           if (p.dr && ok) {
-            ok = mbar_wait_inl(&sh->full[st.i][4], st.ph, wc);
+            ok = mbar_wait_inl(&sh->full[TA_SLOTS + st.i], st.ph, wc);
             tc_fence_after();
             if (ok)
 #pragma unroll
               for (int k = 0; k < 4; ++k)
-                umma_bf16_ss(d + 2 * NR, a + p.nc * 1024 + k * 2, q_desc + p.nc * (2 * NR * 8) + k * 2, id_qt, k > 0 ? 1u : 0u);
+                umma_bf16_ss(d + 2 * NR, t_desc + st.i * (TA_CHUNK >> 4) + k * 2, q_desc + p.nc * (2 * NR * 8) + k * 2,
+                             id_qt, k > 0 ? 1u : 0u);
           }
           if (!ok) break;
           umma_commit(&sh->s_full[sq.i]);
-          for (int c = p.dt; c < p.nc; ++c) umma_commit(&sh->kfree[st.i][c]);
-          if (p.dr && !VT) umma_commit(&sh->kfree[st.i][4]);
+          if (p.dr) {
+            if (!VT) umma_commit(&sh->kfree[TA_SLOTS + st.i]);
+            st.next(p.tails);
+          }
         }
         w.next_item(p, n);
       }
@@ -582,35 +594,38 @@ __global__ void __launch_bounds__(TA_THREADS, 1)
       mbar_wait(&sh->drain[0], 0, wc, false, true);
     }
     __syncwarp();
-  } else if (warp == TA_W_PV) {
+  } else if (warp == W_PV) {
     // ================================================================ outputs
     if (elect_one()) {
-      const uint64_t v_desc = sdesc_sw128(smem_u32(ks_), 16384, 1024), p_desc = sdesc_sw128(smem_u32(ps), 16, 1024);
+      const uint64_t v_desc = sdesc_sw128(smem_u32(ks_), TA_CHUNK, 1024), p_desc = sdesc_sw128(smem_u32(ps), 16, 1024);
       const uint64_t pb_desc = sdesc_sw64(smem_u32(pb));
       const uint32_t id_pv = idesc_e4m3_f32(128, NP) | (1u << 10) | (1u << 15) | (1u << 16);  // B e5m2, both MN-major
       const uint32_t id_pt = idesc_bf16_f32(128, NR, true, true);
-      const uint32_t stage16 = p.stage_bytes >> 4;
-      TaRing st;
+      const uint64_t vt_desc = sdesc_sw128(smem_u32(kt), TA_CHUNK, 1024);
+      TaRing sl, st;
       uint32_t g = 0;
       bool ok = true;
       while (w.left > 0 && ok) {
         const int n = w.here();
-        for (int i = 0; i < n; ++i, ++g, st.next(p.stages)) {
+        for (int i = 0; i < n; ++i, ++g) {
           ok = mbar_wait_inl(&sh->p_full, g & 1, wc);
           if (!ok) break;
           tc_fence_after();
-          const uint64_t a = v_desc + st.i * stage16;
-          for (int m = 0; m < p.dt; ++m) {
+          for (int m = 0; m < p.nc; ++m, sl.next(p.slots)) {
+            if (m >= p.dt) continue;  // read by the scores alone
 #pragma unroll
             for (int k = 0; k < 4; ++k)  // 32 keys: 4096 bytes further in both
-              umma_f8_ss(tmem + o_col + m * NP, a + m * 1024 + k * 256, p_desc + k * 256, id_pv, i > 0 || k > 0 ? 1u : 0u);
-            umma_commit(&sh->kfree[st.i][m]);
+              umma_f8_ss(tmem + o_col + m * NP, v_desc + sl.i * (TA_CHUNK >> 4) + k * 256, p_desc + k * 256, id_pv,
+                         i > 0 || k > 0 ? 1u : 0u);
+            umma_commit(&sh->kfree[sl.i]);
           }
           if (VT) {  // 64 dims (the other 64 lanes hold what lies behind them, unused)
 #pragma unroll
             for (int k = 0; k < 8; ++k)  // 16 keys: 2048 and 1024 bytes further
-              umma_bf16_ss(tmem + ot_col, a + p.nc * 1024 + k * 128, pb_desc + k * 64, id_pt, i > 0 || k > 0 ? 1u : 0u);
-            umma_commit(&sh->kfree[st.i][4]);
+              umma_bf16_ss(tmem + ot_col, vt_desc + st.i * (TA_CHUNK >> 4) + k * 128, pb_desc + k * 64, id_pt,
+                           i > 0 || k > 0 ? 1u : 0u);
+            umma_commit(&sh->kfree[TA_SLOTS + st.i]);
+            st.next(p.tails);
           }
           umma_commit(&sh->pv_done);
         }
@@ -632,8 +647,8 @@ __global__ void __launch_bounds__(TA_THREADS, 1)
     // The queries of item x: hi and lo codes and the bf16 tail, scaled by a power of two
     // per row.  The last scores of the item before are in registers.
     auto queries = [&](const TaWalk& x) {
-      constexpr int LR = NR == 32 ? 8 : 16;  // lanes of a row, 8 columns each at a time
-      static_assert(NR / (TA_SOFT / 32) == 32 / LR, "every warp takes 32 / LR rows");
+      constexpr int LR = 16;  // lanes of a row, 8 columns each at a time
+      static_assert(NR / (SOFT / 32) == 32 / LR, "every warp takes 32 / LR rows");
       constexpr int QV = 64 / LR;
       const int row = warp * (32 / LR) + lane / LR, at = lane % LR;
       const bool in = x.rt * NR + row < p.rows;
@@ -688,7 +703,7 @@ __global__ void __launch_bounds__(TA_THREADS, 1)
       if (lane == 0) mbar_arrive(&sh->q_full);
     };
     if (w.left > 0) queries(w);
-    soft_sync();
+    named_bar_sync(1, SOFT);
     while (w.left > 0) {
       const int n = w.here();
       const int r0 = w.rt * NR;                      // first row of the tile in the sequence
@@ -770,7 +785,7 @@ __global__ void __launch_bounds__(TA_THREADS, 1)
           float most = fmaxf(d[0], d[1]);
 #pragma unroll
           for (int c = 2; c < CW; c += 2) most = fmaxf(most, fmaxf(d[c], d[c + 1]));
-          raise = soft_any(most > TA_GROW || sk > sh->sigma);
+          raise = soft_any<SOFT>(most > TA_GROW || sk > sh->sigma);
         }
         if (raise) {
           // The tile's maxima; references that they pass go up to them, and the reference of
@@ -781,7 +796,7 @@ __global__ void __launch_bounds__(TA_THREADS, 1)
 #pragma unroll
           for (int o = 16; o > 0; o >>= 1) smax = fmaxf(smax, __shfl_xor_sync(0xFFFFFFFFu, smax, o));
           if (lane == 0 && hc == 0) sh->red_s[quarter] = smax;
-          soft_sync();
+          named_bar_sync(1, SOFT);
           if (threadIdx.x < NR) {
             const int c = threadIdx.x;
             const float mo = sh->m[c];
@@ -799,7 +814,7 @@ __global__ void __launch_bounds__(TA_THREADS, 1)
             sh->sigma = sn;
             sh->top = sn > 0.f ? TA_TOP / sn : 0.f;
           }
-          soft_sync();
+          named_bar_sync(1, SOFT);
           exponents(false);
           if (i > 0) {  // sums and output follow, once every product before is in it
 #pragma unroll
@@ -858,14 +873,11 @@ __global__ void __launch_bounds__(TA_THREADS, 1)
         for (int v = 0; v < TA_LEVELS; ++v) {
           const int byte = v * NR + hc;
           uint8_t* at = ps + key * 128 + (((byte >> 4) ^ (key & 7)) << 4) + (byte & 15);
-          if constexpr (CW == 16) *reinterpret_cast<uint4*>(at) = make_uint4(pc[v][0], pc[v][1], pc[v][2], pc[v][3]);
-          else *reinterpret_cast<uint2*>(at) = make_uint2(pc[v][0], pc[v][1]);
+          *reinterpret_cast<uint2*>(at) = make_uint2(pc[v][0], pc[v][1]);
         }
         if constexpr (VT) {
-#pragma unroll
-          for (int c = 0; c < CW; c += 8)
-            *reinterpret_cast<uint4*>(pb + key * 64 + ((((hc + c) >> 3) ^ ((key >> 1) & 3)) << 4)) =
-                make_uint4(pw[c / 2], pw[c / 2 + 1], pw[c / 2 + 2], pw[c / 2 + 3]);
+          *reinterpret_cast<uint4*>(pb + key * 64 + (((hc >> 3) ^ ((key >> 1) & 3)) << 4)) =
+              make_uint4(pw[0], pw[1], pw[2], pw[3]);
         }
         fence_proxy_async_smem();
         tc_fence_before();
@@ -878,7 +890,7 @@ __global__ void __launch_bounds__(TA_THREADS, 1)
 #pragma unroll
         for (int c = 0; c < CW; c += 2) f2_get(l2[c / 2], l[c], l[c + 1]);
         ta_reduce<false, CW>(l, &sh->red[quarter][hc], lane);
-        soft_sync();
+        named_bar_sync(1, SOFT);
         TaWalk x = w;
         x.next_item(p, n);
         if (x.left > 0) queries(x);  // their first scores run during this epilogue
@@ -910,7 +922,7 @@ __global__ void __launch_bounds__(TA_THREADS, 1)
           // This CTA's part ends with its stretch; the CTAs after it take `per` tiles each.
           ow[2] = 1 + (int)((w.nt - n + sh->per - 1) / sh->per);
         }
-        soft_sync();
+        named_bar_sync(1, SOFT);
         mbar_wait_inl(&sh->pv_done, (g - 1) & 1, wc);
         tc_fence_after();
         const float unit = sh->fs;
@@ -953,7 +965,7 @@ __global__ void __launch_bounds__(TA_THREADS, 1)
           store(p.dq + key, p.dv, o);
         }
         tc_fence_before();
-        soft_sync();  // f and qs are read by all before the next item's
+        named_bar_sync(1, SOFT);  // f and qs are read by all before the next item's
       }
       w.next_item(p, n);
     }
@@ -961,7 +973,11 @@ __global__ void __launch_bounds__(TA_THREADS, 1)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (warp == TA_W_QK) tmem_dealloc<1>(tmem, p.tmem_cols);
+  if (warp == W_QK) tmem_dealloc<1>(tmem, p.tmem_cols);
+  // after a timed-out wait: no load of this CTA may land once it has gone
+  if (threadIdx.x == 0 && sh->abort)
+    for (int s = 0; s < TA_SLOTS + 2; ++s)
+      if (sh->issued[s]) mbar_wait(&sh->full[s], (sh->issued[s] - 1) & 1, wc, false, true);
 }
 
 // Adds up the parts of row tiles that span CTAs, in order: the tile whose head CTA x holds
