@@ -1029,6 +1029,12 @@ int ks_tree_attn(const void* q, const void* kv8, const float* kv_scale, const vo
   const size_t fixed = 1024 + TA_HDR + q_bytes + 16384 + (vt ? 8192 : 0);
   p.tails = dr ? (vt ? 2 : 1) : 0;
   p.slots = (int)std::min<size_t>((232448 - fixed) / TA_CHUNK - p.tails, TA_SLOTS);
+  // A loader warp may wait for a slot that another warp filled last.  Its wait is by parity,
+  // so the barrier must not lag by two phases.  With chunks given back in order it cannot:
+  // the warp's chunk before was let in when the chunk slots + nc before this one was given
+  // back, and that comes after 2 slots before.  Where the scores give some chunks back ahead
+  // of others (dt < nc) every slot is one warp's: a multiple of nc.
+  if (p.dt < p.nc) p.slots -= p.slots % p.nc;
   if (p.slots < p.nc) return fail(KS_ERR_UNSUPPORTED, "tree_attn: shared memory too small");
   p.k_off = TA_HDR;
   p.t_off = p.k_off + (uint32_t)p.slots * TA_CHUNK;

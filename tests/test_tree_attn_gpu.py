@@ -112,6 +112,18 @@ def test_short_contexts_in_short_and_wide_tables(cuda_ok, B, T, H, n):
         check(q, kv8, scale, tail, t, lens, 512 ** -0.5, 512, mask, sink)
 
 
+@pytest.mark.parametrize("dq,dr,dv", [(512, 64, 128), (512, 0, 384), (384, 64, 64), (256, 0, 128), (320, 64, 256)])
+def test_values_narrower_than_the_codes(cuda_ok, dq, dr, dv):
+    """Chunks of which only the scores read go back to the loads before the others."""
+    from kernelswift_b200 import ops
+
+    g, *a = build(4, 3, 40, dq, dr, 64, [5000, 1300, 1, 257], seed=dv)
+    first = check(*a, (dq + dr) ** -0.5, dv)
+    for _ in range(20):
+        assert torch.equal(first, ops.tree_attn(*a, (dq + dr) ** -0.5, dv=dv))
+    ops.device_status()
+
+
 @pytest.mark.parametrize("tree", [False, True])
 def test_rows_of_many_sequences_at_once(cuda_ok, tree):
     """More work items than CTAs, ragged, some sequences empty."""
