@@ -37,24 +37,37 @@
 // stretches, one per CTA, whatever the lengths (which only the device knows), so a long
 // context is split over the SMs and ragged batches balance (16 trees of 13 tokens, 64
 // heads, up to 6001 keys: 270 us with TA_SETUP = 0, when CTAs with many short sequences
-// ran twice as long as the others).  A row tile that spans CTAs leaves (maximum, sum,
-// unnormalised output) per part in the workspace; tree_attn_join_kernel adds them up in
-// order (no atomics).
+// ran twice as long as the others; 179, 168 and 170 us with 3, 4 and 5).  A row tile that
+// spans CTAs leaves (maximum, sum, unnormalised output) per part in the workspace;
+// tree_attn_join_kernel adds them up in order (no atomics).  Short tables take a CTA per
+// row tile and need no join (the host code has the rule and its figures).
 //
-// Warps: 8 softmax warps (thread = key = TMEM lane; two share a lane quarter and split the
-// rows), 5 loader warps, a warp that issues the first product and one that issues the
+// Warps: a softmax warp for each lane quarter and 8 rows (thread = key = TMEM lane: 16 warps
+// at NR = 32; 8 warps of 16 rows took 1 % less on large trees and 3 % more on ragged ones),
+// 5 loader warps, a warp that issues the first product and one that issues the
 // second (each waits for its own inputs; one thread for both made each wait for the
 // other's), one address warp that walks the page table ahead of
 // the loads.  A tile whose keys are all present and unmarked comes by TMA in boxes of r
 // rows (r: the power of two that divides page and 128, at least 8); others (the last of a
 // sequence, odd pages) by cp.async with absent and marked rows zeroed, so that no garbage
-// meets a zero weight.
+// meets a zero weight.  Codes lie in a ring of chunks (128 keys of 128 columns, 16 KB), nine
+// of them at 576 columns: a chunk goes back to the loads when its dim tile's product is done.
 //
 // Softmax: p = 2^(s - m) with a reference m that is raised only when a score passes it by
 // TA_GROW (one vote per tile: about a tenth of the tiles of N(0, 1) data with a limit of 3,
 // and the raise costs more than a tile, so the limit is what e5m2's range allows), together
 // with sum and output; sums are kept per thread in
 // fp32 and reduced once per row tile.
+//
+// Measured (device time, one B200): 8 trees of 32 tokens, 128 heads, 8192 keys 737 us (585
+// GFLOP of scores and outputs: 794 TFLOP/s); 16 trees of 13 tokens, 64 heads, up to 6001 keys
+// 164 us; one token of 128 heads over 131069 keys 73 us; 48 sequences of up to 8000 keys, 16
+// heads 36.5 us (128 MB: 3.5 TB/s).  Bound: at 32 rows a tile takes about 2.8 K cycles, the
+// MMAs 1.9 K of them (counters: tensor pipe 41 %, shared memory 60 %); the rest is the chain
+// chunk given back -> load (1.3 K from L2) -> scores -> softmax (2.2 K) -> output, of which
+// two tiles are in flight, because nine chunks and a row tile's queries fill shared memory
+// and its outputs TMEM.  A row tile's beginning and end cost about 10 K cycles.  At 16 rows a
+// tile's 82 KB are the larger part: 3.4 K cycles, the rate of HBM with all SMs at work.
 #pragma once
 #include "latent_cache.cuh"
 #include "sparse_attn.cuh"
