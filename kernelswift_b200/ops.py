@@ -39,11 +39,11 @@ _DV_MAX = 512
 def _require_cuda(name: str, *tensors: torch.Tensor) -> None:
     dev, mixed = -1, False
     for t in tensors:
-        if not isinstance(t, torch.Tensor) or not t.is_cuda:
+        d = t.get_device() if isinstance(t, torch.Tensor) else -1
+        if d < 0 or not t.is_cuda:
             raise RuntimeError(f"{name}: inputs must be CUDA tensors")
         if not t.is_contiguous():
             raise RuntimeError(f"{name}: inputs must be contiguous")
-        d = t.get_device()
         mixed |= dev >= 0 and d != dev
         dev = d
     if mixed:
@@ -433,16 +433,16 @@ def topk_rows(scores: torch.Tensor, T: int, topk: int, ratio: int = 1, causal: b
 def _cache_args(name, kv8, kv_scale, kv_tail):
     if kv8.dtype not in _FP8 or kv8.dim() != 3:
         raise RuntimeError(f"{name}: kv8 must be float8_e4m3fn (or its uint8 bytes) [pages, page, dq]")
-    if kv_scale.dtype != torch.float32 or tuple(kv_scale.shape) != tuple(kv8.shape[:2]):
+    if kv_scale.dtype != torch.float32 or kv_scale.shape != kv8.shape[:2]:
         raise RuntimeError(f"{name}: kv_scale must be float32 [pages, page]")
     pages, page, dq = kv8.shape
     dr = 0
     if kv_tail is not None:
         if kv_tail.dtype != torch.bfloat16 or kv_tail.dim() != 3:
             raise RuntimeError(f"{name}: kv_tail must be bfloat16 [pages, page, dr]")
-        if tuple(kv_tail.shape[:2]) != (pages, page):
+        tail_pages, tail_page, dr = kv_tail.shape
+        if tail_pages != pages or tail_page != page:
             raise RuntimeError(f"{name}: kv_tail shape mismatch")
-        dr = kv_tail.shape[2]
     if pages < 1 or page < 1:
         raise RuntimeError(f"{name}: the cache has no pages")
     ts = [kv8, kv_scale] + ([kv_tail] if kv_tail is not None else [])
@@ -452,7 +452,7 @@ def _cache_args(name, kv8, kv_scale, kv_tail):
 def _table_args(name, page_table, lens, B):
     if page_table.dtype != torch.int32 or page_table.dim() != 2 or page_table.shape[0] != B:
         raise RuntimeError(f"{name}: page_table must be int32 [b, max_pages]")
-    if lens.dtype != torch.int32 or tuple(lens.shape) != (B,):
+    if lens.dtype != torch.int32 or lens.shape != (B,):
         raise RuntimeError(f"{name}: lens must be int32 [b]")
 
 
@@ -491,9 +491,9 @@ def cache_write(kv: torch.Tensor, slots: torch.Tensor, kv8: torch.Tensor, kv_sca
         raise RuntimeError("cache_write: the columns of kv must be contiguous")
     stride = rows.stride(0) if R > 1 else dq + dr
     with _on(kv8):
-        check(lib().ks_cache_write(_ptr(rows), stride, _ptr(slots),
+        check(lib().ks_cache_write(rows.data_ptr(), stride, slots.data_ptr(),
                                    KS_INT64 if slots.dtype == torch.int64 else KS_INT32, R,
-                                   _ptr(kv8), _ptr(kv_scale), _ptr(kv_tail), pages * page, dq, dr,
+                                   kv8.data_ptr(), kv_scale.data_ptr(), _ptr(kv_tail), pages * page, dq, dr,
                                    _stream(kv8)), "ks_cache_write")
 
 
@@ -515,9 +515,9 @@ def cache_read(kv8: torch.Tensor, kv_scale: torch.Tensor, kv_tail: torch.Tensor 
     else:
         _check_out("cache_read", out, (B, n, dq + dr), torch.bfloat16, kv8.device)
     with _on(kv8):
-        check(lib().ks_cache_read(_ptr(kv8), _ptr(kv_scale), _ptr(kv_tail), pages, page, dq, dr,
-                                  _ptr(page_table), page_table.shape[1], _ptr(lens), B, n, start,
-                                  _ptr(out), _stream(kv8)), "ks_cache_read")
+        check(lib().ks_cache_read(kv8.data_ptr(), kv_scale.data_ptr(), _ptr(kv_tail), pages, page, dq, dr,
+                                  page_table.data_ptr(), page_table.shape[1], lens.data_ptr(), B, n, start,
+                                  out.data_ptr(), _stream(kv8)), "ks_cache_read")
     return out
 
 
@@ -550,11 +550,11 @@ def tree_attn(q: torch.Tensor, kv8: torch.Tensor, kv_scale: torch.Tensor,
     _table_args("tree_attn", page_table, lens, B)
     ts = [q] + ts + [page_table, lens]
     if mask is not None:
-        if mask.dtype not in (torch.bool, torch.uint8) or tuple(mask.shape) != (B, T, T):
+        if mask.dtype not in (torch.bool, torch.uint8) or mask.shape != (B, T, T):
             raise RuntimeError("tree_attn: mask must be bool [b, t, t]")
         ts.append(mask)
     if attn_sink is not None:
-        if attn_sink.dtype != torch.float32 or tuple(attn_sink.shape) != (H,):
+        if attn_sink.dtype != torch.float32 or attn_sink.shape != (H,):
             raise RuntimeError("tree_attn: attn_sink must be float32 [h]")
         ts.append(attn_sink)
     _require_cuda("tree_attn", *ts)
@@ -569,10 +569,10 @@ def tree_attn(q: torch.Tensor, kv8: torch.Tensor, kv_scale: torch.Tensor,
     else:
         _check_workspace("tree_attn", workspace, need, q.device)
     with _on(q):
-        check(lib().ks_tree_attn(_ptr(q), _ptr(kv8), _ptr(kv_scale), _ptr(kv_tail), pages, page,
-                                 dq, dr, _ptr(page_table), page_table.shape[1], _ptr(lens),
-                                 _ptr(mask), _ptr(attn_sink), _ptr(out), B, T, H, dv,
-                                 float(softmax_scale), _ptr(workspace),
+        check(lib().ks_tree_attn(q.data_ptr(), kv8.data_ptr(), kv_scale.data_ptr(), _ptr(kv_tail), pages, page,
+                                 dq, dr, page_table.data_ptr(), page_table.shape[1], lens.data_ptr(),
+                                 _ptr(mask), _ptr(attn_sink), out.data_ptr(), B, T, H, dv,
+                                 float(softmax_scale), workspace.data_ptr(),
                                  workspace.numel() * workspace.element_size(), _stream(q)),
               "ks_tree_attn")
     return out
@@ -599,23 +599,23 @@ def verify_draft(p: torch.Tensor, tokens: torch.Tensor, u: torch.Tensor, noise: 
     if tokens.dtype not in (torch.int32, torch.int64) or tokens.dim() != 2:
         raise RuntimeError("verify_draft: tokens must be int32 or int64 [b, t]")
     B, T = tokens.shape
-    if p.dtype != torch.float32 or p.dim() != 3 or tuple(p.shape[:2]) != (B, T + 1):
+    if p.dtype != torch.float32 or p.dim() != 3 or p.shape[:2] != (B, T + 1):
         raise RuntimeError("verify_draft: p must be float32 [b, t + 1, v]")
     V = p.shape[2]
-    if u.dtype != torch.float32 or tuple(u.shape) != (B, T + 1):
+    if u.dtype != torch.float32 or u.shape != (B, T + 1):
         raise RuntimeError("verify_draft: u must be float32 [b, t + 1]")
-    if noise.dtype != torch.float32 or tuple(noise.shape) != (B, V):
+    if noise.dtype != torch.float32 or noise.shape != (B, V):
         raise RuntimeError("verify_draft: noise must be float32 [b, v]")
     ts = [p, tokens, u, noise]
     if q is not None:
         if parents is not None:
             raise RuntimeError("verify_draft: q (a sampled chain) and parents (fixed candidates) "
                                "exclude each other")
-        if q.dtype != torch.float32 or tuple(q.shape) != (B, T, V):
+        if q.dtype != torch.float32 or q.shape != (B, T, V):
             raise RuntimeError("verify_draft: q must be float32 [b, t, v]")
         ts.append(q)
     if parents is not None:
-        if parents.dtype != torch.int32 or tuple(parents.shape) != (B, T):
+        if parents.dtype != torch.int32 or parents.shape != (B, T):
             raise RuntimeError("verify_draft: parents must be int32 [b, t]")
         ts.append(parents)
     _require_cuda("verify_draft", *ts)
@@ -623,10 +623,10 @@ def verify_draft(p: torch.Tensor, tokens: torch.Tensor, u: torch.Tensor, noise: 
     n_accepted = torch.empty(B, dtype=torch.int32, device=p.device)
     path = torch.empty(B, T, dtype=torch.int32, device=p.device)
     with _on(p):
-        check(lib().ks_verify_draft(_ptr(p), _ptr(q), _ptr(tokens),
+        check(lib().ks_verify_draft(p.data_ptr(), _ptr(q), tokens.data_ptr(),
                                     KS_INT64 if tokens.dtype == torch.int64 else KS_INT32,
-                                    _ptr(parents), _ptr(u), _ptr(noise), B, T, V, _ptr(out),
-                                    _ptr(n_accepted), _ptr(path), _stream(p)), "ks_verify_draft")
+                                    _ptr(parents), u.data_ptr(), noise.data_ptr(), B, T, V, out.data_ptr(),
+                                    n_accepted.data_ptr(), path.data_ptr(), _stream(p)), "ks_verify_draft")
     return out, n_accepted, path
 
 
