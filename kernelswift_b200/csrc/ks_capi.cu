@@ -609,12 +609,13 @@ int launch_tree_attn(Device* dev, const CUtensorMap& km, const CUtensorMap& tm, 
   cudaLaunchAttribute at[1];
   at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   at[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.gridDim = dim3(grid, NR);
-  cfg.blockDim = dim3(TA_JOIN_THREADS);
+  const int groups = p.by_item ? 4 : 1;
+  cfg.gridDim = dim3(p.by_item ? (unsigned)(p.B * p.row_tiles) : grid, NR);
+  cfg.blockDim = dim3(TA_JOIN_GROUP * groups);
   cfg.stream = st;
   cfg.attrs = at;
   cfg.numAttrs = 1;
-  cudaError_t e = cudaLaunchKernelEx(&cfg, tree_attn_join_kernel<NR>, p);
+  cudaError_t e = cudaLaunchKernelEx(&cfg, groups > 1 ? tree_attn_join_kernel<NR, 4> : tree_attn_join_kernel<NR, 1>, p);
   if (e != cudaSuccess) return cuda_fail(e, "tree_attn_join_kernel launch");
   return launch_check("tree_attn_join_kernel launch");
 }
@@ -1064,6 +1065,7 @@ int ks_tree_attn(const void* q, const void* kv8, const float* kv_scale, const vo
   const int64_t items = B * p.row_tiles;
   p.solo = items <= sms && max_pages * page <= (items * 4 >= sms ? 2 * TA_SOLO : TA_SOLO);
   const unsigned grid = (unsigned)(p.solo ? items : std::min(most, sms));
+  p.by_item = items * 8 <= (int64_t)grid;  // few row tiles of many parts, see the join
   p.part_o = static_cast<float*>(workspace);
   p.part_ml = p.part_o + 2ll * grid * nr * dv;
   p.owner = reinterpret_cast<int32_t*>(p.part_ml + 4ll * grid * nr);

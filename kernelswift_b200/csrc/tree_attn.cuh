@@ -120,7 +120,8 @@ struct TreeAttnParams {
   float scale_log2;
   float* part_o;          // [2 * CTAs][NR][dv]
   float* part_ml;         // [2 * CTAs][NR][2]
-  int32_t* owner;         // [CTAs][4]: sequence, row tile, parts of the item whose head is here
+  int32_t* owner;         // [CTAs][4]: sequence, row tile, parts (0: none to join), CTA of the head
+  int32_t by_item;        // owner is indexed by row tile of the call (there are few), else by CTA
   int* status;
   uint64_t budget_ns;
 };
@@ -374,7 +375,7 @@ __global__ void __launch_bounds__(TA_THREADS<NR>, 1)
     sh->sigma = 0.f;
     fence_barrier_init();
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the join may be set up
-    p.owner[(int64_t)blockIdx.x * 4 + 2] = 0;  // no row tile's head here yet
+    if (!p.by_item) p.owner[(int64_t)blockIdx.x * 4 + 2] = 0;  // no row tile's head here yet
   }
   if (threadIdx.x < TA_MAX_ROWS) {
     sh->m[threadIdx.x] = -INFINITY;
@@ -928,12 +929,11 @@ __global__ void __launch_bounds__(TA_THREADS<NR>, 1)
           sh->fs = sh->sigma * (1.f / TA_TOP);  // what a unit of P stands for
           sh->sigma = 0.f;
         }
-        if (!whole && threadIdx.x == 0 && w.t == 0) {
-          int32_t* ow = p.owner + (int64_t)blockIdx.x * 4;
-          ow[0] = w.b;
-          ow[1] = w.rt;
+        if (threadIdx.x == 0 && w.t == 0 && !p.solo && (!whole || p.by_item)) {
           // This CTA's part ends with its stretch; the CTAs after it take `per` tiles each.
-          ow[2] = 1 + (int)((w.nt - n + sh->per - 1) / sh->per);
+          const int parts = whole ? 0 : 1 + (int)((w.nt - n + sh->per - 1) / sh->per);
+          *reinterpret_cast<int4*>(p.owner + 4 * (p.by_item ? w.b * p.row_tiles + w.rt : (int)blockIdx.x)) =
+              make_int4(w.b, w.rt, parts, (int)blockIdx.x);
         }
         named_bar_sync(1, SOFT);
         mbar_wait_inl(&sh->pv_done, (g - 1) & 1, wc);
@@ -994,24 +994,29 @@ __global__ void __launch_bounds__(TA_THREADS<NR>, 1)
 }
 
 // Adds up the parts of row tiles that span CTAs, in order: the tile whose head CTA x holds
-// has its parts in slots 2 x + 1, 2 (x + 1), 2 (x + 2), ...  A block per CTA and row
-// (blockIdx.y); most find no parts and end at once.  Launched while tree_attn_kernel still
-// runs; it waits for its end here.  A chain of four load latencies: which tile, the parts'
-// maxima and sums, the parts (16 in flight).  Fewer blocks that take rows in turn were
-// slower (48 ragged sequences: 41.0 us with 296, 38.6 with 592, 38.1 so).
-constexpr int TA_JOIN_THREADS = 128;
+// has its parts in slots 2 x + 1, 2 (x + 1), 2 (x + 2), ...  A block per row of each entry of
+// `owner`; most find no parts where entries are by CTA.  Launched while tree_attn_kernel
+// still runs; it waits for its end here.  A chain of load latencies: which tile, the parts'
+// maxima and sums, the parts.  Where few row tiles have many parts, entries are by row tile
+// and four groups of 128 threads share a row, 16 parts each in flight; else one group with
+// 4 in flight (most rows have a few; with 8, 48 ragged sequences take 1 us more).  128 rows
+// of 37 parts: 73.3 us for the call with one group, 69.0 with four.
+constexpr int TA_JOIN_GROUP = 128;  // threads of a row: dv <= 512
 
-template <int NR>
-__global__ void __launch_bounds__(TA_JOIN_THREADS) tree_attn_join_kernel(const TreeAttnParams p) {
+template <int NR, int GROUPS>
+__global__ void __launch_bounds__(TA_JOIN_GROUP* GROUPS) tree_attn_join_kernel(const TreeAttnParams p) {
+  constexpr int FLY = GROUPS > 1 ? 16 : 4;     // parts in flight
   constexpr int PL = (TA_MAX_CTAS + 31) / 32;  // parts of a lane
-  __shared__ float fs[TA_JOIN_THREADS / 32][PL * 32];  // factor of each part, a copy per warp
+  __shared__ float fs[TA_JOIN_GROUP * GROUPS / 32][PL * 32];  // factor of each part, a copy per warp
+  __shared__ float4 sums[GROUPS][TA_JOIN_GROUP];
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int4 ow = *reinterpret_cast<const int4*>(p.owner + (int64_t)blockIdx.x * 4);
   const int parts = ow.z, c = blockIdx.y;
   const int64_t row = (int64_t)ow.y * NR + c;
   if (parts == 0 || row >= p.rows) return;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  auto slot = [&](int i) { return i == 0 ? 2 * (int64_t)blockIdx.x + 1 : 2 * ((int64_t)blockIdx.x + i); };
+  const int group = threadIdx.x / TA_JOIN_GROUP;
+  auto slot = [&](int i) { return i == 0 ? 2 * (int64_t)ow.w + 1 : 2 * ((int64_t)ow.w + i); };
   float2 ml[PL];
 #pragma unroll
   for (int k = 0; k < PL; ++k) {
@@ -1037,20 +1042,43 @@ __global__ void __launch_bounds__(TA_JOIN_THREADS) tree_attn_join_kernel(const T
   if (p.sink && m != -INFINITY) sum += ex2f(__ldg(p.sink + row % p.H) * 1.4426950408889634f - m);
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
   __syncwarp();
-  const int d = threadIdx.x * 4;  // dv <= 512
-  if (d >= p.dv) return;
+  const int at = threadIdx.x % TA_JOIN_GROUP, d = at * 4;
   float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 16
-  for (int i = 0; i < parts; ++i) {
-    const float f = fs[warp][i];
-    const float4 v = *reinterpret_cast<const float4*>(p.part_o + (slot(i) * NR + c) * p.dv + d);
-    o.x += v.x * f;
-    o.y += v.y * f;
-    o.z += v.z * f;
-    o.w += v.w * f;
+  if (d < p.dv)
+    for (int base = group; base < parts; base += GROUPS * FLY) {
+      float4 v[FLY];
+#pragma unroll
+      for (int k = 0; k < FLY; ++k) {
+        const int i = base + k * GROUPS;
+        v[k] = i < parts ? *reinterpret_cast<const float4*>(p.part_o + (slot(i) * NR + c) * p.dv + d)
+                         : make_float4(0.f, 0.f, 0.f, 0.f);
+      }
+#pragma unroll
+      for (int k = 0; k < FLY; ++k) {
+        const int i = base + k * GROUPS;
+        const float f = i < parts ? fs[warp][i] : 0.f;
+        o.x += v[k].x * f;
+        o.y += v[k].y * f;
+        o.z += v[k].z * f;
+        o.w += v[k].w * f;
+      }
+    }
+  if constexpr (GROUPS > 1) {
+    if (group > 0) sums[group][at] = o;
+    __syncthreads();
+    if (group > 0) return;
+#pragma unroll
+    for (int k = 1; k < GROUPS; ++k) {
+      const float4 v = sums[k][at];
+      o.x += v.x;
+      o.y += v.y;
+      o.z += v.z;
+      o.w += v.w;
+    }
   }
-  *reinterpret_cast<uint2*>(p.out + ((int64_t)ow.x * p.rows + row) * p.dv + d) =
-      make_uint2(cvt_bf16x2(o.x * inv, o.y * inv), cvt_bf16x2(o.z * inv, o.w * inv));
+  if (d < p.dv)
+    *reinterpret_cast<uint2*>(p.out + ((int64_t)ow.x * p.rows + row) * p.dv + d) =
+        make_uint2(cvt_bf16x2(o.x * inv, o.y * inv), cvt_bf16x2(o.z * inv, o.w * inv));
 }
 
 }  // namespace ks
