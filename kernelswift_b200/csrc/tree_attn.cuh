@@ -20,9 +20,11 @@
 //   * a weight is taken to fp16 and split into three e5m2 numbers of 3 bits each, the high
 //     bytes of P, P - P0 and P - P0 - P1 as fp16, each product in columns of its own and
 //     the three added at the end.  Off by at most 2^-9 of the weight (a bf16 weight:
-//     2^-8), or 2^-27 of a weight of 1 where that is more.
+//     2^-8), or 2^-26 of the row's largest weight times scale where that is more.
 // A key's scale multiplies its scores (thread = key) and its weight, the latter relative to
-// the largest scale seen, so that P keeps within e5m2's range.  The rotary columns are bf16
+// the largest scale seen, and the reference of a row's weights is the largest weight times
+// scale: P keeps within e5m2's range, and a row of large values with no weight takes no
+// precision from the others (up to 2^TA_SPAN between the scales).  The rotary columns are bf16
 // and have a bf16 product of their own; where v reaches into them (dv > dq), so do they.
 //
 // Why split: with bf16 operands every tile's codes are expanded in shared memory, 147 KB
@@ -59,9 +61,9 @@
 // with sum and output; sums are kept per thread in
 // fp32 and reduced once per row tile.
 //
-// Measured (device time, one B200): 8 trees of 32 tokens, 128 heads, 8192 keys 737 us (585
-// GFLOP of scores and outputs: 794 TFLOP/s); 16 trees of 13 tokens, 64 heads, up to 6001 keys
-// 164 us; one token of 128 heads over 131069 keys 68 us; 48 sequences of up to 8000 keys, 16
+// Measured (device time, one B200): 8 trees of 32 tokens, 128 heads, 8192 keys 742 us (585
+// GFLOP of scores and outputs: 789 TFLOP/s); 16 trees of 13 tokens, 64 heads, up to 6001 keys
+// 167 us; one token of 128 heads over 131069 keys 70.5 us; 48 sequences of up to 8000 keys, 16
 // heads 36.2 us (128 MB: 3.5 TB/s).  Bound: at 32 rows a tile takes about 2.8 K cycles, the
 // MMAs 1.9 K of them (counters: tensor pipe 41 %, shared memory 60 %); the rest is the chain
 // chunk given back -> load (1.3 K from L2) -> scores -> softmax (2.2 K) -> output, of which
@@ -92,7 +94,8 @@ constexpr int TA_SOLO = 512;                 // keys of a table up to which a CT
 constexpr int TA_LEVELS = 3;                 // e5m2 columns per weight
 constexpr float TA_GROW = 5.f;               // how far a score may pass m (base 2)
 constexpr float TA_HEAD = 1.f;               // a raised m lies this far above the score
-constexpr float TA_TOP = 1024.f;             // P of a weight of 1 at the largest scale: 2^(10 + TA_GROW) < 57344
+constexpr float TA_TOP = 1024.f;             // P at the reference: 2^(10 + TA_GROW) < 57344
+constexpr int TA_SPAN = 40;                  // bits by which scales move references at most (e and sums stay in range)
 
 struct TreeAttnParams {
   const uint16_t* q;      // bf16 [B, T * H, dq + dr]
@@ -140,13 +143,14 @@ struct TaShared {
   int64_t per;                                  // units of a stretch
   int32_t left0, b0, rt0, t0, len0;             // its first tile, see TaWalk
   float sigma, top, fs;                         // largest scale so far, TA_TOP over it; factor of its raise
+  int sigma_e, shift;                           // its exponent; bits that its raises took off the references
   alignas(16) float m[TA_MAX_ROWS];             // reference of each row (base 2)
   alignas(16) float mneg[TA_MAX_ROWS];          // its negative
   alignas(16) float qs[TA_MAX_ROWS];            // 2^e * softmax scale of each row
   alignas(16) float f[TA_MAX_ROWS];             // factor of a raise; at the end 1 / sum
   float red[4][TA_MAX_ROWS];
-  float red_s[4];
   int32_t whole[TA_AHEAD];                      // every key of the tile can come by TMA
+  float smax[TA_AHEAD];                         // its largest scale (0: none)
   int32_t slot[TA_AHEAD][128];                  // row of the page pool, -1: zeros
   float sk[TA_AHEAD][128];                      // key's scale; -1: absent, NaN: marked
 };
@@ -373,6 +377,7 @@ __global__ void __launch_bounds__(TA_THREADS<NR>, 1)
     mbar_init(&sh->drain[1], 1);
     sh->abort = 0;
     sh->sigma = 0.f;
+    sh->sigma_e = sh->shift = 0;
     fence_barrier_init();
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the join may be set up
     if (!p.by_item) p.owner[(int64_t)blockIdx.x * 4 + 2] = 0;  // no row tile's head here yet
@@ -556,6 +561,11 @@ __global__ void __launch_bounds__(TA_THREADS<NR>, 1)
       if (!drafted) scales();
 #pragma unroll
       for (int i = 0; i < 4; ++i) sh->sk[ad.i][i * 32 + lane] = marked(i) ? __uint_as_float(0x7FC00000u) : k[i];
+      float most = 0.f;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) most = fmaxf(most, marked(i) ? 0.f : k[i]);
+      const uint32_t top = __reduce_max_sync(0xFFFFFFFFu, __float_as_uint(most));  // (not negative)
+      if (lane == 0) sh->smax[ad.i] = __uint_as_float(top);
       __syncwarp();
       if (lane == 0) mbar_arrive(&sh->sk_full[ad.i]);
     }
@@ -751,13 +761,20 @@ __global__ void __launch_bounds__(TA_THREADS<NR>, 1)
         }
         mbar_wait_inl(&sh->sk_full[ad.i], ad.ph, wc);
         float sk = sh->sk[ad.i][key];
+        const float smax = sh->smax[ad.i];
         __syncwarp();
         if (lane == 0) mbar_arrive(&sh->a_free[ad.i]);
         const bool marked = sk != sk;
         if (sk < 0.f) allow = 0;
+        // log2 of the key's scale, relative to one of exponent `e`
+        auto rel = [&](int e) {
+          return (float)(sk > 0.f ? max((int)(__float_as_uint(sk) >> 23) - e, -TA_SPAN) : -TA_SPAN);
+        };
         constexpr uint32_t ALL = (1u << CW) - 1u;
         const bool plain = __all_sync(0xFFFFFFFFu, (allow & ALL) == ALL && !marked);
         if (marked || sk < 0.f) sk = 0.f;
+        const float grow = TA_GROW - rel(sh->sigma_e);  // before the scores are there
+        const bool larger = smax > sh->sigma;
 
         mbar_wait_inl(&sh->s_full[sq.i], sq.ph, wc);
         tc_fence_after();
@@ -799,33 +816,36 @@ __global__ void __launch_bounds__(TA_THREADS<NR>, 1)
           float most = fmaxf(d[0], d[1]);
 #pragma unroll
           for (int c = 2; c < CW; c += 2) most = fmaxf(most, fmaxf(d[c], d[c + 1]));
-          raise = soft_any<SOFT>(most > TA_GROW || sk > sh->sigma);
+          raise = soft_any<SOFT>(most > grow || larger);
         }
         if (raise) {
-          // The tile's maxima; references that they pass go up to them, and the reference of
-          // the scales to the tile's largest.
+          // The reference of the scales goes up to the tile's largest, the rows' down by as
+          // much, and those that the tile's maxima (with the keys' scales) pass go up to them.
+          const float so = sh->sigma;
+          float sn = fmaxf(so, smax);
+          if (sn > 0.f) sn = fmaxf(sn, 0x1p-110f);  // (TA_TOP / sn stays finite)
+          const int ne = (int)(__float_as_uint(sn) >> 23), was = sh->shift;
+          const int down = so > 0.f ? min(ne - sh->sigma_e, TA_SPAN - was) : 0;
           exponents(true);
-          ta_reduce<true, CW>(d, &sh->red[quarter][hc], lane);
-          float smax = sk;
+          const float rl = rel(ne);
 #pragma unroll
-          for (int o = 16; o > 0; o >>= 1) smax = fmaxf(smax, __shfl_xor_sync(0xFFFFFFFFu, smax, o));
-          if (lane == 0 && hc == 0) sh->red_s[quarter] = smax;
+          for (int c = 0; c < CW; ++c) d[c] += rl;
+          ta_reduce<true, CW>(d, &sh->red[quarter][hc], lane);
           named_bar_sync(1, SOFT);
           if (threadIdx.x < NR) {
             const int c = threadIdx.x;
-            const float mo = sh->m[c];
+            const float mo = sh->m[c], md = mo - (float)down;
             const float tmx = fmaxf(fmaxf(sh->red[0][c], sh->red[1][c]), fmaxf(sh->red[2][c], sh->red[3][c]));
-            const float mn = tmx > mo + TA_GROW || mo == -INFINITY ? tmx + TA_HEAD : mo;
+            const float mn = tmx > md + TA_GROW || mo == -INFINITY ? tmx + TA_HEAD : md;
             sh->f[c] = mn == mo ? 1.f : ex2f(mo - mn);
             sh->m[c] = mn;
             sh->mneg[c] = -mn;
           }
           if (threadIdx.x == 64) {
-            const float so = sh->sigma;
-            float sn = fmaxf(so, fmaxf(fmaxf(sh->red_s[0], sh->red_s[1]), fmaxf(sh->red_s[2], sh->red_s[3])));
-            if (sn > 0.f) sn = fmaxf(sn, 0x1p-110f);  // (TA_TOP / sn stays finite)
             sh->fs = so > 0.f ? so / sn : 1.f;  // (powers of two)
             sh->sigma = sn;
+            sh->sigma_e = ne;
+            sh->shift = was + down;
             sh->top = sn > 0.f ? TA_TOP / sn : 0.f;
           }
           named_bar_sync(1, SOFT);
@@ -928,6 +948,7 @@ __global__ void __launch_bounds__(TA_THREADS<NR>, 1)
         if (threadIdx.x == 64) {
           sh->fs = sh->sigma * (1.f / TA_TOP);  // what a unit of P stands for
           sh->sigma = 0.f;
+          sh->sigma_e = sh->shift = 0;
         }
         if (threadIdx.x == 0 && w.t == 0 && !p.solo && (!whole || p.by_item)) {
           // This CTA's part ends with its stretch; the CTAs after it take `per` tiles each.
@@ -1000,7 +1021,7 @@ __global__ void __launch_bounds__(TA_THREADS<NR>, 1)
 // maxima and sums, the parts.  Where few row tiles have many parts, entries are by row tile
 // and four groups of 128 threads share a row, 16 parts each in flight; else one group with
 // 4 in flight (most rows have a few; with 8, 48 ragged sequences take 1 us more).  128 rows
-// of 37 parts: 73.3 us for the call with one group, 69.0 with four.
+// of 37 parts: 73 us for the call with one group, 69 with four.
 constexpr int TA_JOIN_GROUP = 128;  // threads of a row: dv <= 512
 
 template <int NR, int GROUPS>

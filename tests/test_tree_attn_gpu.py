@@ -147,6 +147,28 @@ def test_large_and_small_magnitudes(cuda_ok):
     check(*a, 1.0, 512)
 
 
+@pytest.mark.parametrize("at", [0, 200, 399])
+@pytest.mark.parametrize("dv", [128, 192])
+def test_large_rows_without_weight_take_no_precision(cuda_ok, at, dv):
+    """One row 2^24 times as large as the others whose score rules it out: the others are as
+    exact as without it.  And the reverse: one small row that has nearly all the weight."""
+    from kernelswift_b200 import ops
+
+    g, q, kv8, scale, tail, table, lens = build(1, 1, 1, 128, 64, 32, [400], seed=31)
+    slot = (table[0, at // 32].long() * 32 + at % 32).view(1)
+    away = (-2.0 ** 24 * q.float().view(1, 192)).bfloat16()
+    ops.cache_write(away, slot, kv8, scale, tail)
+    check(q, kv8, scale, tail, table, lens, 192 ** -0.5, dv)
+    strong = torch.full((1, 1, 1, 192), 2.0 ** 12, device="cuda").bfloat16()
+    ops.cache_write((2.0 ** -9 * torch.ones(1, 192, device="cuda")).bfloat16(), slot, kv8, scale, tail)
+    other = torch.arange(401, device="cuda")
+    other = other[other != at]
+    kv = torch.randn(400, 192, device="cuda", generator=g)
+    kv -= kv.mean(1, keepdim=True) + 0.01     # scores of -0.01 * 192 * 2^12 against 2^-9 * 192 * 2^12
+    ops.cache_write(kv.bfloat16(), table[0].long()[other // 32] * 32 + other % 32, kv8, scale, tail)
+    check(strong, kv8, scale, tail, table, lens, 2.0 ** -8, dv)
+
+
 @pytest.mark.parametrize("big", [2.0 ** -120, 2.0 ** 60])
 def test_scales_at_the_ends_of_the_range(cuda_ok, big):
     """A cache filled by hand, its scales (powers of two) far from 1 and some of them 0."""
