@@ -276,7 +276,8 @@ size_t ks_tree_attn_workspace_size(int64_t B, int64_t T, int64_t H, int64_t dv);
  *        A token that sees no key gets zeros.
  * A row stored with scale NaN makes every token that sees it NaN, and no other.
  * The weights of the e4m3 columns are kept to 2^-9 of themselves, or to 2^-26 of the
- * token's largest weight times row scale where that is more.
+ * token's largest weight times row scale where that is more, whatever the scales of rows
+ * that it does not see or weigh; a weight below 2^-100 of the token's largest is 0.
  * Key positions whose page is outside the table or the pool are skipped and reported by
  * ks_device_status.  kv_scale must hold powers of two (or NaN), as ks_cache_write writes.
  * Requirements: dq % 64 == 0, dq <= 512, dr 0 or 64, dv % 64 == 0, dv <= min(D, 512),

@@ -975,9 +975,9 @@ int ks_cache_read(const void* kv8, const float* kv_scale, const void* kv_tail, i
 
 size_t ks_tree_attn_workspace_size(int64_t B, int64_t T, int64_t H, int64_t dv) {
   if (B < 1 || T < 1 || H < 1 || dv < 1) return 256;
-  // two parts of a row tile per CTA: output, maximum and sum; and the CTA's owner record
+  // two parts of a row tile per CTA: output, references and sum; and the CTA's owner record
   const int64_t nr = ta_rows(T * H);
-  return (size_t)round_up(TA_MAX_CTAS * (2 * nr * (dv + 2) * 4 + 16), 256);
+  return (size_t)round_up(TA_MAX_CTAS * (2 * nr * (dv + 4) * 4 + 16), 256);
 }
 
 int ks_tree_attn(const void* q, const void* kv8, const float* kv_scale, const void* kv_tail,
@@ -1068,7 +1068,7 @@ int ks_tree_attn(const void* q, const void* kv8, const float* kv_scale, const vo
   p.by_item = items * 8 <= (int64_t)grid;  // few row tiles of many parts, see the join
   p.part_o = static_cast<float*>(workspace);
   p.part_ml = p.part_o + 2ll * grid * nr * dv;
-  p.owner = reinterpret_cast<int32_t*>(p.part_ml + 4ll * grid * nr);
+  p.owner = reinterpret_cast<int32_t*>(p.part_ml + 8ll * grid * nr);
   CUtensorMap km{}, tm{};
   if (p.box) {
     const uint64_t slots = (uint64_t)n_pages * (uint64_t)page;

@@ -21,10 +21,13 @@
 //     bytes of P, P - P0 and P - P0 - P1 as fp16, each product in columns of its own and
 //     the three added at the end.  Off by at most 2^-9 of the weight (a bf16 weight:
 //     2^-8), or 2^-26 of the row's largest weight times scale where that is more.
-// A key's scale multiplies its scores (thread = key) and its weight, the latter relative to
-// the largest scale seen, and the reference of a row's weights is the largest weight times
-// scale: P keeps within e5m2's range, and a row of large values with no weight takes no
-// precision from the others (up to 2^TA_SPAN between the scales).  The rotary columns are bf16
+// A key's scale multiplies its scores (thread = key) and its weight.  A row has two
+// references, both whole powers of two: m of its scores, for the weights and their sum, and
+// ms of its scores + log2 of scale, for P = 2^(TA_TOP + s - ms) * scale.  So P keeps within
+// e5m2's range by what the row itself weighs: a key that it does not see, or that has no
+// weight, takes no precision from the others, however large its values.  (One reference of
+// the scales for the CTA, the largest scale present, lost rows beside one 2^56 larger.)
+// The rotary columns are bf16
 // and have a bf16 product of their own; where v reaches into them (dv > dq), so do they.
 //
 // Why split: with bf16 operands every tile's codes are expanded in shared memory, 147 KB
@@ -40,7 +43,7 @@
 // context is split over the SMs and ragged batches balance (16 trees of 13 tokens, 64
 // heads, up to 6001 keys: 270 us with TA_SETUP = 0, when CTAs with many short sequences
 // ran twice as long as the others; 179, 168 and 170 us with 3, 4 and 5).  A row tile that
-// spans CTAs leaves (maximum, sum, unnormalised output) per part in the workspace;
+// spans CTAs leaves (references, sum, unnormalised output) per part in the workspace;
 // tree_attn_join_kernel adds them up in order (no atomics).  Short tables take a CTA per
 // row tile and need no join (the host code has the rule and its figures).
 //
@@ -55,11 +58,12 @@
 // meets a zero weight.  Codes lie in a ring of chunks (128 keys of 128 columns, 16 KB), nine
 // of them at 576 columns: a chunk goes back to the loads when its dim tile's product is done.
 //
-// Softmax: p = 2^(s - m) with a reference m that is raised only when a score passes it by
-// TA_GROW (one vote per tile: about a tenth of the tiles of N(0, 1) data with a limit of 3,
-// and the raise costs more than a tile, so the limit is what e5m2's range allows), together
-// with sum and output; sums are kept per thread in
-// fp32 and reduced once per row tile.
+// Softmax: references are raised only when some weight passes 2^TA_RISE or some P 2^(TA_TOP
+// + TA_GROW), together with sum and output (one vote per tile).  A raise costs more than a
+// tile, so the limit is what e5m2's range allows, and all rows that have grown are raised at
+// once: large trees (below) take 712 us without any raise, 749 so, 778 where only rows past
+// the limit are raised, 808 with TA_GROW = 5 too.  Sums are kept per thread in fp32 and
+// reduced once per row tile.
 //
 // Measured (device time, one B200): 8 trees of 32 tokens, 128 heads, 8192 keys 742 us (585
 // GFLOP of scores and outputs: 789 TFLOP/s); 16 trees of 13 tokens, 64 heads, up to 6001 keys
@@ -92,10 +96,10 @@ constexpr int TA_HDR = 6144;
 constexpr int TA_SETUP = 4;                  // units that a row tile costs beyond its tiles
 constexpr int TA_SOLO = 512;                 // keys of a table up to which a CTA takes a row tile whole (see the host code)
 constexpr int TA_LEVELS = 3;                 // e5m2 columns per weight
-constexpr float TA_GROW = 5.f;               // how far a score may pass m (base 2)
-constexpr float TA_HEAD = 1.f;               // a raised m lies this far above the score
-constexpr float TA_TOP = 1024.f;             // P at the reference: 2^(10 + TA_GROW) < 57344
-constexpr int TA_SPAN = 40;                  // bits by which scales move references at most (e and sums stay in range)
+constexpr float TA_TOP = 10.f;               // P at the reference ms is 2^TA_TOP
+constexpr float TA_GROW = 5.75f;             // how far it may grow past that (base 2): 2^(TA_TOP + TA_GROW) < 57344
+constexpr float TA_RISE = 7.f;               // how far a score may pass m (base 2)
+constexpr float TA_SPAN = 110.f;             // how far ms may lie below m: 2^(TA_TOP + TA_SPAN + TA_RISE) is finite
 
 struct TreeAttnParams {
   const uint16_t* q;      // bf16 [B, T * H, dq + dr]
@@ -122,7 +126,7 @@ struct TreeAttnParams {
   uint32_t tmem_cols;
   float scale_log2;
   float* part_o;          // [2 * CTAs][NR][dv]
-  float* part_ml;         // [2 * CTAs][NR][2]
+  float* part_ml;         // [2 * CTAs][NR][4]: m, sum, ms
   int32_t* owner;         // [CTAs][4]: sequence, row tile, parts (0: none to join), CTA of the head
   int32_t by_item;        // owner is indexed by row tile of the call (there are few), else by CTA
   int* status;
@@ -140,17 +144,22 @@ struct TaShared {
   uint32_t tmem_base;
   int abort;
   uint32_t issued[TA_SLOTS + 2];                // loads of the chunk so far
+  float tp_max;                                 // log2 of the largest tp
   int64_t per;                                  // units of a stretch
   int32_t left0, b0, rt0, t0, len0;             // its first tile, see TaWalk
-  float sigma, top, fs;                         // largest scale so far, TA_TOP over it; factor of its raise
-  int sigma_e, shift;                           // its exponent; bits that its raises took off the references
-  alignas(16) float m[TA_MAX_ROWS];             // reference of each row (base 2)
-  alignas(16) float mneg[TA_MAX_ROWS];          // its negative
+  alignas(16) float mneg[TA_MAX_ROWS];          // minus m, the reference of each row's scores (base 2, whole)
+  alignas(16) float ms[TA_MAX_ROWS];            // reference of its scores + log2 of the keys' scales
+  alignas(16) float tp[TA_MAX_ROWS];            // 2^(TA_TOP + m - ms): weight times scale to P
   alignas(16) float qs[TA_MAX_ROWS];            // 2^e * softmax scale of each row
-  alignas(16) float f[TA_MAX_ROWS];             // factor of a raise; at the end 1 / sum
   float red[4][TA_MAX_ROWS];
+  union {  // a row's four maxima are read by the thread that then writes its factors
+    float red_s[4][TA_MAX_ROWS];
+    struct {
+      float f[TA_MAX_ROWS];                     // factor of a raise of m; at the end 1 / sum
+      float fs[TA_MAX_ROWS];                    // of a raise of ms; at the end 1 / sum by what a unit of P stands for
+    };
+  };
   int32_t whole[TA_AHEAD];                      // every key of the tile can come by TMA
-  float smax[TA_AHEAD];                         // its largest scale (0: none)
   int32_t slot[TA_AHEAD][128];                  // row of the page pool, -1: zeros
   float sk[TA_AHEAD][128];                      // key's scale; -1: absent, NaN: marked
 };
@@ -261,14 +270,33 @@ __device__ __forceinline__ bool soft_any(bool x) {
   return r != 0;
 }
 
-// Max or sum over the warp's lanes of CW <= 16 values each into red[c], c < CW.
-template <bool MX, int CW>
+// 2^x of a whole x (0 below 2^-126; x at most 127; 1 for a NaN: what meets it is one).
+__device__ __forceinline__ float ta_pow2(float x) {
+  return __uint_as_float((uint32_t)(min(max(__float2int_rz(x), -127), 127) + 127) << 23);
+}
+
+// log2 of a power of two (-127: of less than 2^-126).
+__device__ __forceinline__ float ta_log2(float x) { return (float)((int)(__float_as_uint(x) >> 23) - 127); }
+
+// Sum over the warp's lanes of CW <= 16 values each into red[c], c < CW.
+template <int CW>
 __device__ __forceinline__ void ta_reduce(const float (&v)[CW], float* red, int lane) {
   float w[16];
 #pragma unroll
   for (int i = 0; i < 16; ++i) w[i] = i < CW ? v[i % CW] : 0.f;
-  const float r = reduce16_lanes<MX>(w, lane);  // value lane >> 1
+  const float r = reduce16_lanes<false>(w, lane);  // value lane >> 1
   if ((lane & 1) == 0 && (lane >> 1) < CW) red[lane >> 1] = r;
+}
+// Max over the warp's lanes of 8 values each into red[c], and of the values + a into red_s[c].
+__device__ __forceinline__ void ta_maxima(const float (&v)[8], float a, float* red, float* red_s, int lane) {
+  float w[16];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    w[i] = v[i];
+    w[i + 8] = v[i] + a;
+  }
+  const float r = reduce16_lanes<true>(w, lane);  // value lane >> 1
+  if ((lane & 1) == 0) (lane < 16 ? red : red_s)[(lane >> 1) & 7] = r;
 }
 
 // Bytes that the current phase of `bar` also waits for (no arrival).
@@ -376,14 +404,12 @@ __global__ void __launch_bounds__(TA_THREADS<NR>, 1)
     mbar_init(&sh->drain[0], 1);
     mbar_init(&sh->drain[1], 1);
     sh->abort = 0;
-    sh->sigma = 0.f;
-    sh->sigma_e = sh->shift = 0;
     fence_barrier_init();
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the join may be set up
     if (!p.by_item) p.owner[(int64_t)blockIdx.x * 4 + 2] = 0;  // no row tile's head here yet
   }
   if (threadIdx.x < TA_MAX_ROWS) {
-    sh->m[threadIdx.x] = -INFINITY;
+    sh->ms[threadIdx.x] = -INFINITY;
     sh->mneg[threadIdx.x] = INFINITY;
   }
   if (warp == W_QK) {
@@ -561,11 +587,6 @@ __global__ void __launch_bounds__(TA_THREADS<NR>, 1)
       if (!drafted) scales();
 #pragma unroll
       for (int i = 0; i < 4; ++i) sh->sk[ad.i][i * 32 + lane] = marked(i) ? __uint_as_float(0x7FC00000u) : k[i];
-      float most = 0.f;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) most = fmaxf(most, marked(i) ? 0.f : k[i]);
-      const uint32_t top = __reduce_max_sync(0xFFFFFFFFu, __float_as_uint(most));  // (not negative)
-      if (lane == 0) sh->smax[ad.i] = __uint_as_float(top);
       __syncwarp();
       if (lane == 0) mbar_arrive(&sh->sk_full[ad.i]);
     }
@@ -761,21 +782,15 @@ __global__ void __launch_bounds__(TA_THREADS<NR>, 1)
         }
         mbar_wait_inl(&sh->sk_full[ad.i], ad.ph, wc);
         float sk = sh->sk[ad.i][key];
-        const float smax = sh->smax[ad.i];
         __syncwarp();
         if (lane == 0) mbar_arrive(&sh->a_free[ad.i]);
         const bool marked = sk != sk;
         if (sk < 0.f) allow = 0;
-        // log2 of the key's scale, relative to one of exponent `e`
-        auto rel = [&](int e) {
-          return (float)(sk > 0.f ? max((int)(__float_as_uint(sk) >> 23) - e, -TA_SPAN) : -TA_SPAN);
-        };
         constexpr uint32_t ALL = (1u << CW) - 1u;
         const bool plain = __all_sync(0xFFFFFFFFu, (allow & ALL) == ALL && !marked);
         if (marked || sk < 0.f) sk = 0.f;
-        const float grow = TA_GROW - rel(sh->sigma_e);  // before the scores are there
-        const bool larger = smax > sh->sigma;
-
+        const float sk_log2 = sk > 0.f ? ta_log2(sk) : -INFINITY;
+        const float grow = TA_TOP + TA_GROW - sk_log2, tp_max = sh->tp_max;  // (before the scores are there)
         mbar_wait_inl(&sh->s_full[sq.i], sq.ph, wc);
         tc_fence_after();
         TaF2 x[CW / 2];  // q 2^-e . k
@@ -816,74 +831,68 @@ __global__ void __launch_bounds__(TA_THREADS<NR>, 1)
           float most = fmaxf(d[0], d[1]);
 #pragma unroll
           for (int c = 2; c < CW; c += 2) most = fmaxf(most, fmaxf(d[c], d[c + 1]));
-          raise = soft_any<SOFT>(most > grow || larger);
+          bool up = most > TA_RISE;
+          if (most + tp_max > grow) {  // some row's P may be too large: which tp has it?
+#pragma unroll
+            for (int c = 0; c < CW; ++c) up |= d[c] + ta_log2(sh->tp[hc + c]) > grow;
+          }
+          raise = soft_any<SOFT>(up);
         }
         if (raise) {
-          // The reference of the scales goes up to the tile's largest, the rows' down by as
-          // much, and those that the tile's maxima (with the keys' scales) pass go up to them.
-          const float so = sh->sigma;
-          float sn = fmaxf(so, smax);
-          if (sn > 0.f) sn = fmaxf(sn, 0x1p-110f);  // (TA_TOP / sn stays finite)
-          const int ne = (int)(__float_as_uint(sn) >> 23), was = sh->shift;
-          const int down = so > 0.f ? min(ne - sh->sigma_e, TA_SPAN - was) : 0;
+          // m goes up to the tile's largest score, ms to its largest score + log2 of scale, of
+          // every row that has a larger one
           exponents(true);
-          const float rl = rel(ne);
-#pragma unroll
-          for (int c = 0; c < CW; ++c) d[c] += rl;
-          ta_reduce<true, CW>(d, &sh->red[quarter][hc], lane);
+          ta_maxima(d, sk_log2, &sh->red[quarter][hc], &sh->red_s[quarter][hc], lane);
           named_bar_sync(1, SOFT);
-          if (threadIdx.x < NR) {
-            const int c = threadIdx.x;
-            const float mo = sh->m[c], md = mo - (float)down;
-            const float tmx = fmaxf(fmaxf(sh->red[0][c], sh->red[1][c]), fmaxf(sh->red[2][c], sh->red[3][c]));
-            const float mn = tmx > md + TA_GROW || mo == -INFINITY ? tmx + TA_HEAD : md;
-            sh->f[c] = mn == mo ? 1.f : ex2f(mo - mn);
-            sh->m[c] = mn;
+          if (warp == 0) {
+            const int c = lane & (NR - 1);
+            auto top = [&](const float (&r)[4][TA_MAX_ROWS]) {
+              return fmaxf(fmaxf(r[0][c], r[1][c]), fmaxf(r[2][c], r[3][c]));
+            };
+            const float mo = -sh->mneg[c], so = sh->ms[c], mt = top(sh->red), st = top(sh->red_s);
+            const float mn = fmaxf(mo, ceilf(mt)), sn = fmaxf(fmaxf(so, ceilf(st)), mn - TA_SPAN);
+            const float tp = ta_pow2(TA_TOP + (mn - sn));
+            const uint32_t most = __reduce_max_sync(0xFFFFFFFFu, __float_as_uint(tp));
+            if (lane == 0) sh->tp_max = ta_log2(__uint_as_float(most));
+            sh->f[c] = ta_pow2(mo - mn);
+            sh->fs[c] = ta_pow2(so - sn);
+            sh->tp[c] = tp;
             sh->mneg[c] = -mn;
-          }
-          if (threadIdx.x == 64) {
-            sh->fs = so > 0.f ? so / sn : 1.f;  // (powers of two)
-            sh->sigma = sn;
-            sh->sigma_e = ne;
-            sh->shift = was + down;
-            sh->top = sn > 0.f ? TA_TOP / sn : 0.f;
+            sh->ms[c] = sn;
           }
           named_bar_sync(1, SOFT);
           exponents(false);
           if (i > 0) {  // sums and output follow, once every product before is in it
+            bool same = true;
 #pragma unroll
-            for (int c = 0; c < CW; c += 2) l2[c / 2] = mul2(l2[c / 2], f2(sh->f[hc + c], sh->f[hc + c + 1]));
+            for (int c = 0; c < CW; c += 2) {
+              l2[c / 2] = mul2(l2[c / 2], f2(sh->f[hc + c], sh->f[hc + c + 1]));
+              same &= sh->f[hc + c] == 1.f && sh->f[hc + c + 1] == 1.f && sh->fs[hc + c] == 1.f && sh->fs[hc + c + 1] == 1.f;
+            }
             mbar_wait_inl(&sh->pv_done, (g - 1) & 1, wc);
             tc_fence_after();
-            float fr[CW];
-            bool same = sh->fs == 1.f;
-#pragma unroll
-            for (int c = 0; c < CW; ++c) {
-              fr[c] = sh->f[hc + c];
-              same &= fr[c] == 1.f;
-            }
             if (!same) {  // (the same for the whole warp)
 #pragma unroll 1
               for (int b = 0; b < p.dt * TA_LEVELS + VT; ++b) {
-                const float fs = b < p.dt * TA_LEVELS ? sh->fs : 1.f;
+                const float* fr = b < p.dt * TA_LEVELS ? sh->fs : sh->f;
                 float o[CW];
                 const uint32_t at = tmem + o_col + b * NR + hc + lane_off;
                 tmem_ldn<CW>(at, o);
                 tmem_wait_ld();
 #pragma unroll
-                for (int c = 0; c < CW; ++c) o[c] *= fr[c] * fs;
+                for (int c = 0; c < CW; ++c) o[c] *= fr[hc + c];
                 tmem_stn<CW>(at, o);
               }
             }
             tmem_wait_st();
           }
         }
-        // weights, their sums, and the three parts of each
-        const float fk = marked ? 1.f : sk * sh->top;
-        const TaF2 fk2 = f2(fk, fk);
+        // weights, their sums, and the three parts of each times scale
+        const TaF2 sk2 = f2(sk, sk);
         uint32_t pc[TA_LEVELS][CW / 4], pw[VT ? CW / 2 : 1];
 #pragma unroll
         for (int c = 0; c < CW; c += 4) {
+          const ulonglong2 tp = *reinterpret_cast<const ulonglong2*>(&sh->tp[hc + c]);
           uint32_t h[2], h1[2], h2[2];
 #pragma unroll
           for (int z = 0; z < 2; ++z) {
@@ -892,7 +901,7 @@ __global__ void __launch_bounds__(TA_THREADS<NR>, 1)
             l2[c / 2 + z] = add2(l2[c / 2 + z], e);
             if constexpr (VT) pw[c / 2 + z] = cvt_bf16x2(e0, e1);
             float w0, w1;
-            f2_get(mul2(e, fk2), w0, w1);
+            f2_get(mul2(mul2(e, TaF2{z ? tp.y : tp.x}), sk2), w0, w1);
             h[z] = f16x2_of(w0, w1);
             h1[z] = sub_f16x2(h[z], h[z] & 0xFF00FF00u);
             h2[z] = sub_f16x2(h1[z], h1[z] & 0xFF00FF00u) + 0x00800080u;  // the last part rounded to nearest
@@ -923,7 +932,7 @@ __global__ void __launch_bounds__(TA_THREADS<NR>, 1)
         float l[CW];
 #pragma unroll
         for (int c = 0; c < CW; c += 2) f2_get(l2[c / 2], l[c], l[c + 1]);
-        ta_reduce<false, CW>(l, &sh->red[quarter][hc], lane);
+        ta_reduce<CW>(l, &sh->red[quarter][hc], lane);
         named_bar_sync(1, SOFT);
         TaWalk x = w;
         x.next_item(p, n);
@@ -932,23 +941,19 @@ __global__ void __launch_bounds__(TA_THREADS<NR>, 1)
         const int slot = 2 * (int)blockIdx.x + (w.t == 0 ? 1 : 0);
         if (threadIdx.x < NR) {
           const int c = threadIdx.x;
-          const float m = sh->m[c];
+          const float m = -sh->mneg[c], ms = sh->ms[c];
           float sum = sh->red[0][c] + sh->red[1][c] + sh->red[2][c] + sh->red[3][c];
           if (whole) {
             if (p.sink && m != -INFINITY)  // (without a key the output is 0 either way)
               sum += ex2f(__ldg(p.sink + (r0 + c) % p.H) * 1.4426950408889634f - m);
-            sh->f[c] = sum == 0.f ? 0.f : 1.f / sum;
+            const float inv = sum == 0.f ? 0.f : 1.f / sum;
+            sh->f[c] = inv;
+            sh->fs[c] = inv * ta_pow2(ms - m - TA_TOP);
           } else {
-            *reinterpret_cast<float2*>(p.part_ml + ((int64_t)slot * NR + c) * 2) = make_float2(m, sum);
-            sh->f[c] = 1.f;
+            *reinterpret_cast<float4*>(p.part_ml + ((int64_t)slot * NR + c) * 4) = make_float4(m, sum, ms, 0.f);
           }
-          sh->m[c] = -INFINITY;
+          sh->ms[c] = -INFINITY;
           sh->mneg[c] = INFINITY;
-        }
-        if (threadIdx.x == 64) {
-          sh->fs = sh->sigma * (1.f / TA_TOP);  // what a unit of P stands for
-          sh->sigma = 0.f;
-          sh->sigma_e = sh->shift = 0;
         }
         if (threadIdx.x == 0 && w.t == 0 && !p.solo && (!whole || p.by_item)) {
           // This CTA's part ends with its stretch; the CTAs after it take `per` tiles each.
@@ -959,16 +964,15 @@ __global__ void __launch_bounds__(TA_THREADS<NR>, 1)
         named_bar_sync(1, SOFT);
         mbar_wait_inl(&sh->pv_done, (g - 1) & 1, wc);
         tc_fence_after();
-        const float unit = sh->fs;
         // dims `dim` (even lanes) and dim + 1 (the next lane) of a row go out together: the
         // even lane stores row c, the odd one row c + 1
         const bool odd = lane & 1;
-        auto store = [&](int dim, int dims, const float (&o)[CW]) {
+        auto store = [&](int dim, int dims, const float (&o)[CW], const float* f) {
           if (whole) {
             uint16_t* op = p.out + ((int64_t)w.b * p.rows + r0 + hc + odd) * p.dv + (dim - odd);
 #pragma unroll
             for (int c = 0; c < CW; c += 2) {
-              const float a = o[c] * sh->f[hc + c], b = o[c + 1] * sh->f[hc + c + 1];
+              const float a = o[c] * f[hc + c], b = o[c + 1] * f[hc + c + 1];
               const float got = __shfl_xor_sync(0xFFFFFFFFu, odd ? a : b, 1);
               if (dim < dims && hc + c + odd < nrows)
                 *reinterpret_cast<uint32_t*>(op + (int64_t)c * p.dv) = odd ? cvt_bf16x2(got, b) : cvt_bf16x2(a, got);
@@ -989,14 +993,14 @@ __global__ void __launch_bounds__(TA_THREADS<NR>, 1)
           tmem_ldn<CW>(at + 2 * NR, o2);
           tmem_wait_ld();
 #pragma unroll
-          for (int c = 0; c < CW; ++c) o[c] = (o[c] + (o1[c] + o2[c])) * unit;
-          store(m * 128 + key, min(p.dv, p.dq), o);
+          for (int c = 0; c < CW; ++c) o[c] += o1[c] + o2[c];
+          store(m * 128 + key, min(p.dv, p.dq), o, sh->fs);
         }
         if (VT) {
           float o[CW];
           tmem_ldn<CW>(tmem + ot_col + hc + lane_off, o);
           tmem_wait_ld();
-          store(p.dq + key, p.dv, o);
+          store(p.dq + key, p.dv, o, sh->f);
         }
         tc_fence_before();
         named_bar_sync(1, SOFT);  // f and qs are read by all before the next item's
@@ -1028,7 +1032,8 @@ template <int NR, int GROUPS>
 __global__ void __launch_bounds__(TA_JOIN_GROUP* GROUPS) tree_attn_join_kernel(const TreeAttnParams p) {
   constexpr int FLY = GROUPS > 1 ? 16 : 4;     // parts in flight
   constexpr int PL = (TA_MAX_CTAS + 31) / 32;  // parts of a lane
-  __shared__ float fs[TA_JOIN_GROUP * GROUPS / 32][PL * 32];  // factor of each part, a copy per warp
+  // factor of each part, a copy per warp: [0] of columns in units of P, [1] of the bf16 ones
+  __shared__ float fs[TA_JOIN_GROUP * GROUPS / 32][2][PL * 32];
   __shared__ float4 sums[GROUPS][TA_JOIN_GROUP];
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int4 ow = *reinterpret_cast<const int4*>(p.owner + (int64_t)blockIdx.x * 4);
@@ -1038,32 +1043,38 @@ __global__ void __launch_bounds__(TA_JOIN_GROUP* GROUPS) tree_attn_join_kernel(c
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int group = threadIdx.x / TA_JOIN_GROUP;
   auto slot = [&](int i) { return i == 0 ? 2 * (int64_t)ow.w + 1 : 2 * ((int64_t)ow.w + i); };
-  float2 ml[PL];
+  float4 ml[PL];
 #pragma unroll
   for (int k = 0; k < PL; ++k) {
     const int i = k * 32 + lane;
-    ml[k] = i < parts ? *reinterpret_cast<const float2*>(p.part_ml + (slot(i) * NR + c) * 2)
-                      : make_float2(-INFINITY, 0.f);
+    ml[k] = i < parts ? *reinterpret_cast<const float4*>(p.part_ml + (slot(i) * NR + c) * 4)
+                      : make_float4(-INFINITY, 0.f, -INFINITY, 0.f);
   }
-  float m = ml[0].x;
+  float m = ml[0].x, ms = ml[0].z;
 #pragma unroll
-  for (int k = 1; k < PL; ++k) m = fmaxf(m, ml[k].x);
+  for (int k = 1; k < PL; ++k) {
+    m = fmaxf(m, ml[k].x);
+    ms = fmaxf(ms, ml[k].z);
+  }
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
-  const float mu = m == -INFINITY ? 0.f : m;
+  for (int o = 16; o > 0; o >>= 1) {
+    m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
+    ms = fmaxf(ms, __shfl_xor_sync(0xFFFFFFFFu, ms, o));
+  }
   float sum = 0.f;
 #pragma unroll
   for (int k = 0; k < PL; ++k) {
-    const float f = ex2f(ml[k].x - mu);
-    fs[warp][k * 32 + lane] = f;
+    const float f = ta_pow2(ml[k].x - m);
+    fs[warp][0][k * 32 + lane] = ta_pow2(ml[k].z - ms);
+    fs[warp][1][k * 32 + lane] = f;
     sum += ml[k].y * f;
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
   if (p.sink && m != -INFINITY) sum += ex2f(__ldg(p.sink + row % p.H) * 1.4426950408889634f - m);
-  const float inv = sum == 0.f ? 0.f : 1.f / sum;
   __syncwarp();
-  const int at = threadIdx.x % TA_JOIN_GROUP, d = at * 4;
+  const int at = threadIdx.x % TA_JOIN_GROUP, d = at * 4, tail = d >= p.dq;  // (dq is a multiple of 4)
+  const float inv = (sum == 0.f ? 0.f : 1.f / sum) * (tail ? 1.f : ta_pow2(ms - m - TA_TOP));
   float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
   if (d < p.dv)
     for (int base = group; base < parts; base += GROUPS * FLY) {
@@ -1077,7 +1088,7 @@ __global__ void __launch_bounds__(TA_JOIN_GROUP* GROUPS) tree_attn_join_kernel(c
 #pragma unroll
       for (int k = 0; k < FLY; ++k) {
         const int i = base + k * GROUPS;
-        const float f = i < parts ? fs[warp][i] : 0.f;
+        const float f = i < parts ? fs[warp][tail][i] : 0.f;
         o.x += v[k].x * f;
         o.y += v[k].y * f;
         o.z += v[k].z * f;

@@ -357,3 +357,56 @@ def test_refusals(cuda_ok):
         with pytest.raises(RuntimeError, match=why):
             call()
     ops.device_status()
+
+
+# ---- range and precision, whatever the sizes of the rows and queries beside a token's own
+def put(kv8, scale, tail, table, b, pos, rows):
+    """Rows written at positions `pos` of sequence b."""
+    from kernelswift_b200 import ops
+
+    page = kv8.shape[1]
+    pos = torch.as_tensor(pos, device="cuda")
+    ops.cache_write(rows.bfloat16(), table[b].long()[pos // page] * page + pos % page, kv8, scale, tail)
+
+
+@pytest.mark.parametrize("n", [40, 3000])
+@pytest.mark.parametrize("dv", [128, 192])
+@pytest.mark.parametrize("big", [2.0 ** 24, 2.0 ** 56, 2.0 ** 60, 2.0 ** 80, 2.0 ** 110])
+def test_hidden_drafted_rows_of_any_size(cuda_ok, n, dv, big):
+    """A drafted row that the mask hides takes nothing from the others, however much larger
+    than they it is (n = 3000: nor through the join of parts)."""
+    g, q, kv8, scale, tail, table, lens = build(2, 4, 8, 128, 64, 32, [n, n + 90], seed=41)
+    for b in range(2):
+        put(kv8, scale, tail, table, b, [int(lens[b]) + 1], big * torch.randn(1, 192, device="cuda", generator=g))
+    mask = torch.eye(4, dtype=torch.bool, device="cuda").repeat(2, 1, 1)
+    mask[:, :, 0] = True
+    mask[:, 3, 2] = True
+    mask[:, 1, 1] = False
+    check(q, kv8, scale, tail, table, lens, 192 ** -0.5, dv, mask)
+
+
+@pytest.mark.parametrize("at", [0, 200, 1999])
+@pytest.mark.parametrize("dv", [128, 192])
+@pytest.mark.parametrize("big", [2.0 ** 56, 2.0 ** 60, 2.0 ** 80, 2.0 ** 110])
+def test_context_rows_of_any_size_without_weight(cuda_ok, at, dv, big):
+    g, q, kv8, scale, tail, table, lens = build(1, 1, 1, 128, 64, 32, [2000], seed=42)
+    put(kv8, scale, tail, table, 0, [at], -big * q.float().view(1, 192))
+    check(q, kv8, scale, tail, table, lens, 192 ** -0.5, dv)
+
+
+@pytest.mark.parametrize("n,at", [(300, 0), (300, 299), (4000, 5), (4000, 3990)])
+@pytest.mark.parametrize("dv", [128, 192])
+@pytest.mark.parametrize("bits", [30, 60, 80, 95])
+def test_large_rows_whose_weight_makes_up_for_their_size(cuda_ok, n, at, dv, bits):
+    """One row 2^bits as large as the others with about 2^-bits of their weight: both sides
+    count.  Rotary column 0 alone sets the scores."""
+    T, H = 2, 3
+    g, q, kv8, scale, tail, table, lens = build(1, T, H, 128, 64, 64, [n], seed=43)
+    q.zero_()
+    q[..., 0] = q[..., 128] = 1.0
+    rows = torch.randn(n + T, 192, device="cuda", generator=g)
+    rows[:, 0] = rows[:, 128] = 0.0
+    rows[at] *= 2.0 ** bits
+    rows[at, 128] = -round(2 * bits * np.log(2)) / 2
+    put(kv8, scale, tail, table, 0, list(range(n + T)), rows)
+    check(q, kv8, scale, tail, table, lens, 1.0, dv)
