@@ -6,6 +6,7 @@
 #include <cstdarg>
 #include <cstdio>
 #include <algorithm>
+#include <cmath>
 #include <cstdlib>
 #include <mutex>
 #include <string>
@@ -1052,7 +1053,11 @@ int ks_tree_attn(const void* q, const void* kv8, const float* kv_scale, const vo
   p.box = 128;
   while (p.box > 1 && page % p.box) p.box >>= 1;
   if (p.box < 8) p.box = 0;
-  p.scale_log2 = softmax_scale * 1.4426950408889634f;
+  const float scale_log2 = softmax_scale * 1.4426950408889634f;
+  int ex = 0;
+  if (std::isfinite(scale_log2) && scale_log2 != 0.f) ex = std::clamp(std::ilogb(scale_log2), -100, 100);
+  p.scale_in = std::ldexp(scale_log2, -ex);
+  p.scale_up = std::ldexp(1.f, TA_DOWN + ex);
   p.status = dev->status;
   p.budget_ns = wait_budget_ns();
   // no more CTAs than there can be units (the lengths are known on the device only)

@@ -23,10 +23,13 @@
 //     2^-8), or 2^-26 of the row's largest weight times scale where that is more.
 // A key's scale multiplies its scores (thread = key) and its weight.  A row has two
 // references, both whole powers of two: m of its scores, for the weights and their sum, and
-// ms of its scores + log2 of scale, for P = 2^(TA_TOP + s - ms) * scale.  So P keeps within
+// m + mr of its scores + log2 of scale, for P = 2^(TA_TOP + s - m - mr) * scale.  So P keeps within
 // e5m2's range by what the row itself weighs: a key that it does not see, or that has no
 // weight, takes no precision from the others, however large its values.  (One reference of
 // the scales for the CTA, the largest scale present, lost rows beside one 2^56 larger.)
+// Products stay finite where the result is: scores are added up 2^-TA_DOWN as large, with the
+// softmax scale's power of two put back last (exactly, so that the largest score's distance
+// to its reference is right at any size), and the weights of the bf16 columns 2^-TA_VT.
 // The rotary columns are bf16
 // and have a bf16 product of their own; where v reaches into them (dv > dq), so do they.
 //
@@ -96,10 +99,12 @@ constexpr int TA_HDR = 6144;
 constexpr int TA_SETUP = 4;                  // units that a row tile costs beyond its tiles
 constexpr int TA_SOLO = 512;                 // keys of a table up to which a CTA takes a row tile whole (see the host code)
 constexpr int TA_LEVELS = 3;                 // e5m2 columns per weight
-constexpr float TA_TOP = 10.f;               // P at the reference ms is 2^TA_TOP
+constexpr float TA_TOP = 10.f;               // P at the reference m + mr is 2^TA_TOP
 constexpr float TA_GROW = 5.75f;             // how far it may grow past that (base 2): 2^(TA_TOP + TA_GROW) < 57344
 constexpr float TA_RISE = 7.f;               // how far a score may pass m (base 2)
-constexpr float TA_SPAN = 110.f;             // how far ms may lie below m: 2^(TA_TOP + TA_SPAN + TA_RISE) is finite
+constexpr int TA_DOWN = 20;                  // scores are added up 2^20 too small: 256 * 448 * 512 * 2^(119 - 20) is finite
+constexpr int TA_VT = 24;                    // bf16 weights are 2^24 too small: 2^(TA_RISE - 24) * 2^17 keys * 2^128 is finite
+constexpr float TA_SPAN = 110.f;             // how far m + mr may lie below m: 2^(TA_TOP + TA_SPAN + TA_RISE) is finite
 
 struct TreeAttnParams {
   const uint16_t* q;      // bf16 [B, T * H, dq + dr]
@@ -124,9 +129,9 @@ struct TreeAttnParams {
   int32_t solo;           // a CTA per row tile, nothing to join
   uint32_t k_off, t_off, q_off, p_off, pb_off;
   uint32_t tmem_cols;
-  float scale_log2;
+  float scale_in, scale_up;  // product: softmax scale * log2 e * 2^TA_DOWN; scale_up is a power of two
   float* part_o;          // [2 * CTAs][NR][dv]
-  float* part_ml;         // [2 * CTAs][NR][4]: m, sum, ms
+  float* part_ml;         // [2 * CTAs][NR][4]: m, sum, mr
   int32_t* owner;         // [CTAs][4]: sequence, row tile, parts (0: none to join), CTA of the head
   int32_t by_item;        // owner is indexed by row tile of the call (there are few), else by CTA
   int* status;
@@ -145,18 +150,19 @@ struct TaShared {
   int abort;
   uint32_t issued[TA_SLOTS + 2];                // loads of the chunk so far
   float tp_max;                                 // log2 of the largest tp
+  int wide;                                     // some m is so large that m + mr would be rounded
   int64_t per;                                  // units of a stretch
   int32_t left0, b0, rt0, t0, len0;             // its first tile, see TaWalk
   alignas(16) float mneg[TA_MAX_ROWS];          // minus m, the reference of each row's scores (base 2, whole)
-  alignas(16) float ms[TA_MAX_ROWS];            // reference of its scores + log2 of the keys' scales
-  alignas(16) float tp[TA_MAX_ROWS];            // 2^(TA_TOP + m - ms): weight times scale to P
-  alignas(16) float qs[TA_MAX_ROWS];            // 2^e * softmax scale of each row
+  alignas(16) float mr[TA_MAX_ROWS];            // reference of its scores + log2 of the keys' scales, from m on
+  alignas(16) float tp[TA_MAX_ROWS];            // 2^(TA_TOP - mr): weight times scale to P
+  alignas(16) float qs[TA_MAX_ROWS];            // 2^e * scale_in of each row
   float red[4][TA_MAX_ROWS];
   union {  // a row's four maxima are read by the thread that then writes its factors
     float red_s[4][TA_MAX_ROWS];
     struct {
-      float f[TA_MAX_ROWS];                     // factor of a raise of m; at the end 1 / sum
-      float fs[TA_MAX_ROWS];                    // of a raise of ms; at the end 1 / sum by what a unit of P stands for
+      float f[TA_MAX_ROWS];                     // factor of a raise of m; at the end 2^TA_VT / sum
+      float fs[TA_MAX_ROWS];                    // of a raise of m + mr; at the end what a unit of P stands for / sum
     };
   };
   int32_t whole[TA_AHEAD];                      // every key of the tile can come by TMA
@@ -409,7 +415,6 @@ __global__ void __launch_bounds__(TA_THREADS<NR>, 1)
     if (!p.by_item) p.owner[(int64_t)blockIdx.x * 4 + 2] = 0;  // no row tile's head here yet
   }
   if (threadIdx.x < TA_MAX_ROWS) {
-    sh->ms[threadIdx.x] = -INFINITY;
     sh->mneg[threadIdx.x] = INFINITY;
   }
   if (warp == W_QK) {
@@ -715,7 +720,7 @@ __global__ void __launch_bounds__(TA_THREADS<NR>, 1)
 #pragma unroll
       for (int o = LR / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
       const bool bad = top >= 0x7F80u;
-      const int e = bad ? 0 : max((int)(top >> 7) - 127 - 7, -100);  // largest element into [128, 256)
+      const int e = bad ? 0 : max((int)(top >> 7) - 127 - 7, -126);  // largest element into [128, 256)
       const float inv = __uint_as_float((uint32_t)(127 - e) << 23);
 #pragma unroll
       for (int k = 0; k < QV; ++k) {
@@ -738,11 +743,12 @@ __global__ void __launch_bounds__(TA_THREADS<NR>, 1)
         *reinterpret_cast<uint2*>(dst + NR * 128) = bad ? make_uint2(0u, 0u) : make_uint2(lo[0], lo[1]);
       }
       if (at * 8 < p.dr) {
-        const uint32_t m2 = (uint32_t)(127 - e) * 0x00800080u;
+        const uint32_t m2 = (uint32_t)(127 - e) * 0x00800080u, down = (127u - TA_DOWN) * 0x00800080u;
+        auto scaled = [&](uint32_t x) { return mul_bf16x2(mul_bf16x2(x, m2), down); };
         *reinterpret_cast<uint4*>(qs + p.nc * (2 * NR * 128) + row * 128 + ((at ^ (row & 7)) << 4)) =
-            make_uint4(mul_bf16x2(t.x, m2), mul_bf16x2(t.y, m2), mul_bf16x2(t.z, m2), mul_bf16x2(t.w, m2));
+            make_uint4(scaled(t.x), scaled(t.y), scaled(t.z), scaled(t.w));
       }
-      if (at == 0) sh->qs[row] = __uint_as_float((uint32_t)(127 + e) << 23) * p.scale_log2;
+      if (at == 0) sh->qs[row] = __uint_as_float((uint32_t)(127 + e) << 23) * p.scale_in;
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) mbar_arrive(&sh->q_full);
@@ -793,7 +799,7 @@ __global__ void __launch_bounds__(TA_THREADS<NR>, 1)
         const float grow = TA_TOP + TA_GROW - sk_log2, tp_max = sh->tp_max;  // (before the scores are there)
         mbar_wait_inl(&sh->s_full[sq.i], sq.ph, wc);
         tc_fence_after();
-        TaF2 x[CW / 2];  // q 2^-e . k
+        TaF2 x[CW / 2];  // scores (base 2) / scale_up
         {
           float hi[CW], lo[CW], tl[CW];
           const uint32_t at = tmem + sq.i * 3 * NR + hc + lane_off;
@@ -804,20 +810,27 @@ __global__ void __launch_bounds__(TA_THREADS<NR>, 1)
           tc_fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive(&sh->s_free[sq.i]);
-          const TaF2 sixteenth = f2(0.0625f, 0.0625f), sk2 = f2(sk, sk);
-#pragma unroll
-          for (int c = 0; c < CW; c += 2)
-            x[c / 2] = fma2(fma2(f2(lo[c], lo[c + 1]), sixteenth, f2(hi[c], hi[c + 1])), sk2,
-                            p.dr ? f2(tl[c], tl[c + 1]) : f2(0.f, 0.f));
-        }
-        float d[CW];
-        auto exponents = [&](bool raw) {
+          const float down = sk * (1.f / (1 << TA_DOWN));
+          const TaF2 sixteenth = f2(0.0625f, 0.0625f), sk2 = f2(down, down);
 #pragma unroll
           for (int c = 0; c < CW; c += 4) {
             const ulonglong2 s4 = *reinterpret_cast<const ulonglong2*>(&sh->qs[hc + c]);
+#pragma unroll
+            for (int z = c; z < c + 4; z += 2)
+              x[z / 2] = mul2(fma2(fma2(f2(lo[z], lo[z + 1]), sixteenth, f2(hi[z], hi[z + 1])), sk2,
+                                   p.dr ? f2(tl[z], tl[z + 1]) : f2(0.f, 0.f)),
+                              TaF2{z == c ? s4.x : s4.y});
+          }
+        }
+        float d[CW];
+        // (scale_up * x is exact, so the difference to a maximum of it is rounded once)
+        auto exponents = [&](bool raw) {
+          const TaF2 up2 = f2(p.scale_up, p.scale_up);
+#pragma unroll
+          for (int c = 0; c < CW; c += 4) {
             const ulonglong2 mn = raw ? make_ulonglong2(0, 0) : *reinterpret_cast<const ulonglong2*>(&sh->mneg[hc + c]);
-            f2_get(fma2(x[c / 2], TaF2{s4.x}, TaF2{mn.x}), d[c], d[c + 1]);
-            f2_get(fma2(x[c / 2 + 1], TaF2{s4.y}, TaF2{mn.y}), d[c + 2], d[c + 3]);
+            f2_get(fma2(x[c / 2], up2, TaF2{mn.x}), d[c], d[c + 1]);
+            f2_get(fma2(x[c / 2 + 1], up2, TaF2{mn.y}), d[c + 2], d[c + 3]);
           }
           if (!plain) {
 #pragma unroll
@@ -839,28 +852,48 @@ __global__ void __launch_bounds__(TA_THREADS<NR>, 1)
           raise = soft_any<SOFT>(up);
         }
         if (raise) {
-          // m goes up to the tile's largest score, ms to its largest score + log2 of scale, of
-          // every row that has a larger one
+          // m goes up to the tile's largest score, m + mr to its largest score + log2 of scale,
+          // of every row that has a larger one
           exponents(true);
           ta_maxima(d, sk_log2, &sh->red[quarter][hc], &sh->red_s[quarter][hc], lane);
           named_bar_sync(1, SOFT);
+          const int row = lane & (NR - 1);  // (of warp 0, which works on the references)
+          auto most = [&](const float (&r)[4][TA_MAX_ROWS]) {
+            return fmaxf(fmaxf(r[0][row], r[1][row]), fmaxf(r[2][row], r[3][row]));
+          };
+          // mr from the tile's largest and the one before, both from the new m on; a row that
+          // has seen no key needs none
+          auto settle = [&](float tile, float before) {
+            const float mr = sh->mneg[row] == INFINITY ? TA_TOP : fmaxf(fmaxf(before, tile), -TA_SPAN);
+            const float tp = ta_pow2(TA_TOP - mr);
+            const uint32_t top = __reduce_max_sync(0xFFFFFFFFu, __float_as_uint(tp));
+            if (lane == 0) sh->tp_max = ta_log2(__uint_as_float(top));
+            sh->tp[row] = tp;
+            sh->mr[row] = mr;
+            sh->fs[row] = ta_pow2(before - mr);
+          };
+          float before = 0.f;
           if (warp == 0) {
-            const int c = lane & (NR - 1);
-            auto top = [&](const float (&r)[4][TA_MAX_ROWS]) {
-              return fmaxf(fmaxf(r[0][c], r[1][c]), fmaxf(r[2][c], r[3][c]));
-            };
-            const float mo = -sh->mneg[c], so = sh->ms[c], mt = top(sh->red), st = top(sh->red_s);
-            const float mn = fmaxf(mo, ceilf(mt)), sn = fmaxf(fmaxf(so, ceilf(st)), mn - TA_SPAN);
-            const float tp = ta_pow2(TA_TOP + (mn - sn));
-            const uint32_t most = __reduce_max_sync(0xFFFFFFFFu, __float_as_uint(tp));
-            if (lane == 0) sh->tp_max = ta_log2(__uint_as_float(most));
-            sh->f[c] = ta_pow2(mo - mn);
-            sh->fs[c] = ta_pow2(so - sn);
-            sh->tp[c] = tp;
-            sh->mneg[c] = -mn;
-            sh->ms[c] = sn;
+            const float mo = -sh->mneg[row], mt = most(sh->red), st = most(sh->red_s);
+            const float mn = fmaxf(mo, ceilf(mt));
+            before = sh->mr[row] + (mo - mn);  // (NaN without a key: taken for none)
+            const bool wide = __any_sync(0xFFFFFFFFu, fabsf(mn) > 16384.f && fabsf(mn) < INFINITY);
+            if (lane == 0) sh->wide = wide;
+            sh->f[row] = ta_pow2(mo - mn);
+            sh->mneg[row] = -mn;
+            __syncwarp();
+            if (!wide) settle(ceilf(st) - mn, before);
           }
           named_bar_sync(1, SOFT);
+          if (sh->wide) {  // the largest score + log2 of scale from the new m on, exactly
+            exponents(false);
+#pragma unroll
+            for (int c = 0; c < CW; ++c) d[c] += sk_log2;
+            ta_maxima(d, 0.f, &sh->red[quarter][hc], &sh->red[quarter][hc], lane);
+            named_bar_sync(1, SOFT);
+            if (warp == 0) settle(ceilf(most(sh->red)), before);
+            named_bar_sync(1, SOFT);
+          }
           exponents(false);
           if (i > 0) {  // sums and output follow, once every product before is in it
             bool same = true;
@@ -899,7 +932,7 @@ __global__ void __launch_bounds__(TA_THREADS<NR>, 1)
             const float e0 = ex2f(d[c + 2 * z]), e1 = ex2f(d[c + 2 * z + 1]);
             const TaF2 e = f2(e0, e1);
             l2[c / 2 + z] = add2(l2[c / 2 + z], e);
-            if constexpr (VT) pw[c / 2 + z] = cvt_bf16x2(e0, e1);
+            if constexpr (VT) pw[c / 2 + z] = cvt_bf16x2(e0 * (1.f / (1 << TA_VT)), e1 * (1.f / (1 << TA_VT)));
             float w0, w1;
             f2_get(mul2(mul2(e, TaF2{z ? tp.y : tp.x}), sk2), w0, w1);
             h[z] = f16x2_of(w0, w1);
@@ -941,18 +974,17 @@ __global__ void __launch_bounds__(TA_THREADS<NR>, 1)
         const int slot = 2 * (int)blockIdx.x + (w.t == 0 ? 1 : 0);
         if (threadIdx.x < NR) {
           const int c = threadIdx.x;
-          const float m = -sh->mneg[c], ms = sh->ms[c];
+          const float m = -sh->mneg[c], mr = sh->mr[c];
           float sum = sh->red[0][c] + sh->red[1][c] + sh->red[2][c] + sh->red[3][c];
           if (whole) {
             if (p.sink && m != -INFINITY)  // (without a key the output is 0 either way)
               sum += ex2f(__ldg(p.sink + (r0 + c) % p.H) * 1.4426950408889634f - m);
             const float inv = sum == 0.f ? 0.f : 1.f / sum;
-            sh->f[c] = inv;
-            sh->fs[c] = inv * ta_pow2(ms - m - TA_TOP);
+            sh->f[c] = inv * (float)(1 << TA_VT);
+            sh->fs[c] = inv * ta_pow2(mr - TA_TOP);
           } else {
-            *reinterpret_cast<float4*>(p.part_ml + ((int64_t)slot * NR + c) * 4) = make_float4(m, sum, ms, 0.f);
+            *reinterpret_cast<float4*>(p.part_ml + ((int64_t)slot * NR + c) * 4) = make_float4(m, sum, mr, 0.f);
           }
-          sh->ms[c] = -INFINITY;
           sh->mneg[c] = INFINITY;
         }
         if (threadIdx.x == 0 && w.t == 0 && !p.solo && (!whole || p.by_item)) {
@@ -1050,22 +1082,24 @@ __global__ void __launch_bounds__(TA_JOIN_GROUP* GROUPS) tree_attn_join_kernel(c
     ml[k] = i < parts ? *reinterpret_cast<const float4*>(p.part_ml + (slot(i) * NR + c) * 4)
                       : make_float4(-INFINITY, 0.f, -INFINITY, 0.f);
   }
-  float m = ml[0].x, ms = ml[0].z;
+  float m = ml[0].x;
 #pragma unroll
-  for (int k = 1; k < PL; ++k) {
-    m = fmaxf(m, ml[k].x);
-    ms = fmaxf(ms, ml[k].z);
+  for (int k = 1; k < PL; ++k) m = fmaxf(m, ml[k].x);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
+  float mr = -INFINITY;
+#pragma unroll
+  for (int k = 0; k < PL; ++k) {
+    ml[k].z += ml[k].x - m;
+    mr = fmaxf(mr, ml[k].z);
   }
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
-    ms = fmaxf(ms, __shfl_xor_sync(0xFFFFFFFFu, ms, o));
-  }
+  for (int o = 16; o > 0; o >>= 1) mr = fmaxf(mr, __shfl_xor_sync(0xFFFFFFFFu, mr, o));
   float sum = 0.f;
 #pragma unroll
   for (int k = 0; k < PL; ++k) {
     const float f = ta_pow2(ml[k].x - m);
-    fs[warp][0][k * 32 + lane] = ta_pow2(ml[k].z - ms);
+    fs[warp][0][k * 32 + lane] = ta_pow2(ml[k].z - mr);
     fs[warp][1][k * 32 + lane] = f;
     sum += ml[k].y * f;
   }
@@ -1074,7 +1108,7 @@ __global__ void __launch_bounds__(TA_JOIN_GROUP* GROUPS) tree_attn_join_kernel(c
   if (p.sink && m != -INFINITY) sum += ex2f(__ldg(p.sink + row % p.H) * 1.4426950408889634f - m);
   __syncwarp();
   const int at = threadIdx.x % TA_JOIN_GROUP, d = at * 4, tail = d >= p.dq;  // (dq is a multiple of 4)
-  const float inv = (sum == 0.f ? 0.f : 1.f / sum) * (tail ? 1.f : ta_pow2(ms - m - TA_TOP));
+  const float inv = (sum == 0.f ? 0.f : 1.f / sum) * (tail ? (float)(1 << TA_VT) : ta_pow2(mr - TA_TOP));
   float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
   if (d < p.dv)
     for (int base = group; base < parts; base += GROUPS * FLY) {

@@ -410,3 +410,30 @@ def test_large_rows_whose_weight_makes_up_for_their_size(cuda_ok, n, at, dv, bit
     rows[at, 128] = -round(2 * bits * np.log(2)) / 2
     put(kv8, scale, tail, table, 0, list(range(n + T)), rows)
     check(q, kv8, scale, tail, table, lens, 1.0, dv)
+
+
+@pytest.mark.parametrize("n", [300, 3000])
+@pytest.mark.parametrize("dv", [128, 192])
+@pytest.mark.parametrize("big", [2.0 ** 20, 2.0 ** 40, 2.0 ** 60, 2.0 ** 110])
+def test_scores_of_any_size(cuda_ok, n, dv, big):
+    """Large rows that are seen: scores of about `big` in either direction, so that one of
+    them, or the rest of the context, has all the weight."""
+    g, q, kv8, scale, tail, table, lens = build(2, 3, 12, 128, 64, 32, [n, n // 3], seed=49)
+    for b in range(2):
+        at = [n // 100, n // 5, int(lens[b]) + 1]
+        put(kv8, scale, tail, table, b, at, big * torch.randn(3, 192, device="cuda", generator=g))
+    check(q, kv8, scale, tail, table, lens, 192 ** -0.5, dv)
+
+
+@pytest.mark.parametrize("n", [300, 3000])
+@pytest.mark.parametrize("dq,dv", [(512, 512), (128, 128), (128, 192)])
+def test_rows_at_the_top_of_the_range(cuda_ok, n, dq, dv):
+    """Rows near the largest that the cache holds, queries so small that the scores are
+    ordinary: no product on the way overflows."""
+    g, *a = build(2, 2, 16, dq, 64, 64, [n, n // 2], seed=46, key_scale=lambda x: 0 * x + 2.0 ** 124,
+                  q_scale=2.0 ** -119)
+    check(*a, 2.0 ** -5 * (dq + 64) ** -0.5, dv)
+    # and beside ordinary rows, to which ordinary queries give all the weight
+    g, q, kv8, scale, tail, table, lens = build(1, 1, 1, dq, 64, 64, [n], seed=47)
+    put(kv8, scale, tail, table, 0, [n // 2], -2.0 ** 122 * q.float().view(1, dq + 64))
+    check(q, kv8, scale, tail, table, lens, (dq + 64) ** -0.5, dv)
