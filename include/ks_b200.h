@@ -278,6 +278,8 @@ size_t ks_tree_attn_workspace_size(int64_t B, int64_t T, int64_t H, int64_t dv);
  * The weights of the e4m3 columns are kept to 2^-9 of themselves, or to 2^-26 of the
  * token's largest weight times row scale where that is more, whatever the scales of rows
  * that it does not see or weigh; a weight below 2^-100 of the token's largest is 0.
+ * Elements of q in the e4m3 columns are exact down to 2^-14 of a row's largest there, and
+ * rounded to 2^-21 of it below; a row of q with a NaN or an infinity gives NaN.
  * Key positions whose page is outside the table or the pool are skipped and reported by
  * ks_device_status.  kv_scale must hold powers of two (or NaN), as ks_cache_write writes.
  * Requirements: dq % 64 == 0, dq <= 512, dr 0 or 64, dv % 64 == 0, dv <= min(D, 512),

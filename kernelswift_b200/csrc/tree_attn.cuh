@@ -15,8 +15,9 @@
 // contiguous) by the second.  Nothing is expanded.  What meets the codes is split into
 // 8-bit numbers, several columns per row:
 //   * a query element is 8 significant bits of bf16: q 2^-e = hi + lo / 16 exactly, hi and
-//     lo with 4 bits each (e: the row's exponent, hi below 256; elements under 2^-14 of the
-//     row's largest lose bits below 2^-21 of it).  S = S_hi + S_lo / 16.
+//     lo with 4 bits each (e: the exponent of the row's code columns, hi below 256; elements
+//     under 2^-14 of their largest are rounded to 2^-21 of it).  S = S_hi + S_lo / 16.  The
+//     rotary columns have an exponent of their own.
 //   * a weight is taken to fp16 and split into three e5m2 numbers of 3 bits each, the high
 //     bytes of P, P - P0 and P - P0 - P1 as fp16, each product in columns of its own and
 //     the three added at the end.  Off by at most 2^-9 of the weight (a bf16 weight:
@@ -155,14 +156,15 @@ struct TaShared {
   int32_t left0, b0, rt0, t0, len0;             // its first tile, see TaWalk
   alignas(16) float mneg[TA_MAX_ROWS];          // minus m, the reference of each row's scores (base 2, whole)
   alignas(16) float mr[TA_MAX_ROWS];            // reference of its scores + log2 of the keys' scales, from m on
-  alignas(16) float tp[TA_MAX_ROWS];            // 2^(TA_TOP - mr): weight times scale to P
   alignas(16) float qs[TA_MAX_ROWS];            // 2^e * scale_in of each row
+  alignas(16) float qt[TA_MAX_ROWS];            // the same for its rotary columns
   float red[4][TA_MAX_ROWS];
   union {  // a row's four maxima are read by the thread that then writes its factors
-    float red_s[4][TA_MAX_ROWS];
+    alignas(16) float red_s[4][TA_MAX_ROWS];
     struct {
       float f[TA_MAX_ROWS];                     // factor of a raise of m; at the end 2^TA_VT / sum
       float fs[TA_MAX_ROWS];                    // of a raise of m + mr; at the end what a unit of P stands for / sum
+      float tp[TA_MAX_ROWS];                    // 2^(TA_TOP - mr): weight times scale to P, until the next raise
     };
   };
   int32_t whole[TA_AHEAD];                      // every key of the tile can come by TMA
@@ -707,20 +709,29 @@ __global__ void __launch_bounds__(TA_THREADS<NR>, 1)
 #pragma unroll
       for (int k = 0; k < QV; ++k) v[k] = ldcg_or_zero(q + (k * LR + at) * 8, in && (k * LR + at) * 8 < p.dq);
       t = ldcg_or_zero(q + p.dq + at * 8, in && at * 8 < p.dr);
-      // the largest magnitude, as bf16 bits (in order as integers; from 0x7F80 on not finite)
-      uint32_t top = 0;
+      // the largest magnitudes, as bf16 bits (in order as integers; from 0x7F80 on not
+      // finite): of the code columns in the low half of `top`, of the rotary ones in the high
+      auto larger = [](uint32_t& a, uint32_t b) { asm("max.u16x2 %0, %0, %1;" : "+r"(a) : "r"(b)); };
+      constexpr uint32_t ABS = 0x7FFF7FFFu;
+      uint32_t mc = 0, mt = t.x & ABS;
 #pragma unroll
       for (int k = 0; k < QV; ++k) {
         const uint32_t y[4] = {v[k].x, v[k].y, v[k].z, v[k].w};
 #pragma unroll
-        for (int z = 0; z < 4; ++z)
-          asm("max.u16x2 %0, %0, %1;" : "+r"(top) : "r"(y[z] & 0x7FFF7FFFu));
+        for (int z = 0; z < 4; ++z) larger(mc, y[z] & ABS);
       }
-      top = max(top & 0xFFFFu, top >> 16);
+      larger(mt, t.y & ABS);
+      larger(mt, t.z & ABS);
+      larger(mt, t.w & ABS);
+      uint32_t top = __byte_perm(mc, mt, 0x5410);  // low halves, then high ones
+      larger(top, __byte_perm(mc, mt, 0x7632));
 #pragma unroll
-      for (int o = LR / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
-      const bool bad = top >= 0x7F80u;
-      const int e = bad ? 0 : max((int)(top >> 7) - 127 - 7, -126);  // largest element into [128, 256)
+      for (int o = LR / 2; o > 0; o >>= 1) larger(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
+      const uint32_t top_c = top & 0xFFFFu, top_t = top >> 16;
+      const bool bad = top_c >= 0x7F80u || top_t >= 0x7F80u;
+      // largest element into [128, 256)
+      const int e = bad ? 0 : max((int)(top_c >> 7) - 127 - 7, -126);
+      const int et = bad ? 0 : max((int)(top_t >> 7) - 127 - 7, -126);
       const float inv = __uint_as_float((uint32_t)(127 - e) << 23);
 #pragma unroll
       for (int k = 0; k < QV; ++k) {
@@ -743,12 +754,15 @@ __global__ void __launch_bounds__(TA_THREADS<NR>, 1)
         *reinterpret_cast<uint2*>(dst + NR * 128) = bad ? make_uint2(0u, 0u) : make_uint2(lo[0], lo[1]);
       }
       if (at * 8 < p.dr) {
-        const uint32_t m2 = (uint32_t)(127 - e) * 0x00800080u, down = (127u - TA_DOWN) * 0x00800080u;
-        auto scaled = [&](uint32_t x) { return mul_bf16x2(mul_bf16x2(x, m2), down); };
+        const uint32_t m2 = (uint32_t)(127 - et) * 0x00800080u, down = (127u - TA_DOWN) * 0x00800080u;
+        auto scaled = [&](uint32_t x) { return bad ? 0u : mul_bf16x2(mul_bf16x2(x, m2), down); };
         *reinterpret_cast<uint4*>(qs + p.nc * (2 * NR * 128) + row * 128 + ((at ^ (row & 7)) << 4)) =
             make_uint4(scaled(t.x), scaled(t.y), scaled(t.z), scaled(t.w));
       }
-      if (at == 0) sh->qs[row] = __uint_as_float((uint32_t)(127 + e) << 23) * p.scale_in;
+      if (at == 0) {
+        sh->qs[row] = __uint_as_float((uint32_t)(127 + e) << 23) * p.scale_in;
+        sh->qt[row] = __uint_as_float((uint32_t)(127 + et) << 23) * p.scale_in;
+      }
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) mbar_arrive(&sh->q_full);
@@ -815,11 +829,13 @@ __global__ void __launch_bounds__(TA_THREADS<NR>, 1)
 #pragma unroll
           for (int c = 0; c < CW; c += 4) {
             const ulonglong2 s4 = *reinterpret_cast<const ulonglong2*>(&sh->qs[hc + c]);
+            const ulonglong2 t4 = *reinterpret_cast<const ulonglong2*>(&sh->qt[hc + c]);
 #pragma unroll
-            for (int z = c; z < c + 4; z += 2)
-              x[z / 2] = mul2(fma2(fma2(f2(lo[z], lo[z + 1]), sixteenth, f2(hi[z], hi[z + 1])), sk2,
-                                   p.dr ? f2(tl[z], tl[z + 1]) : f2(0.f, 0.f)),
-                              TaF2{z == c ? s4.x : s4.y});
+            for (int z = c; z < c + 4; z += 2) {
+              const TaF2 u = fma2(f2(lo[z], lo[z + 1]), sixteenth, f2(hi[z], hi[z + 1]));
+              const TaF2 sc = mul2(mul2(u, sk2), TaF2{z == c ? s4.x : s4.y});
+              x[z / 2] = p.dr ? fma2(f2(tl[z], tl[z + 1]), TaF2{z == c ? t4.x : t4.y}, sc) : sc;
+            }
           }
         }
         float d[CW];

@@ -437,3 +437,33 @@ def test_rows_at_the_top_of_the_range(cuda_ok, n, dq, dv):
     g, q, kv8, scale, tail, table, lens = build(1, 1, 1, dq, 64, 64, [n], seed=47)
     put(kv8, scale, tail, table, 0, [n // 2], -2.0 ** 122 * q.float().view(1, dq + 64))
     check(q, kv8, scale, tail, table, lens, (dq + 64) ** -0.5, dv)
+
+
+@pytest.mark.parametrize("codes,rotary,keys,sm", [
+    (0.0, 2.0 ** 14, 2.0 ** 14, 2.0 ** -31),      # a query of rotary columns alone
+    (2.0 ** -110, 2.0 ** 14, 2.0 ** 14, 2.0 ** -31),
+    (0.0, 2.0 ** 100, 2.0 ** -80, 2.0 ** -23),
+    (1.0, 0.0, 1.0, 2.0 ** -4),
+    (2.0 ** -20, 1.0, 1.0, 2.0 ** -4),
+    (1.0, 2.0 ** -30, 1.0, 2.0 ** -4),
+    (2.0 ** -118, 2.0 ** -118, 2.0 ** 100, 2.0 ** 14),  # small queries keep their bits
+    (2.0 ** 110, 2.0 ** 110, 2.0 ** -10, 2.0 ** -104),
+])
+def test_queries_of_any_size_in_either_part(cuda_ok, codes, rotary, keys, sm):
+    g, q, *rest = build(2, 2, 16, 128, 64, 32, [150, 60], seed=44, key_scale=lambda x: 0 * x + keys)
+    q = torch.cat([q[..., :128].float() * codes, q[..., 128:].float() * rotary], -1).bfloat16()
+    check(q, *rest, sm, 192)
+
+
+@pytest.mark.parametrize("value", [float("inf"), float("-inf"), float("nan")])
+@pytest.mark.parametrize("column", [3, 127, 128, 191])
+def test_queries_that_are_not_finite_in_either_part(cuda_ok, value, column):
+    from kernelswift_b200 import ops
+
+    g, q, *rest = build(2, 3, 20, 128, 64, 32, [40, 300], seed=45)
+    clean = ops.tree_attn(q, *rest, 0.1, dv=192)
+    q[0, 1, 3, column] = q[1, 2, 19, column] = value
+    got = ops.tree_attn(q, *rest, 0.1, dv=192)
+    hit = torch.zeros(2, 3, 20, dtype=torch.bool, device="cuda")
+    hit[0, 1, 3] = hit[1, 2, 19] = True
+    assert got[hit].isnan().all() and torch.equal(got[~hit], clean[~hit])
