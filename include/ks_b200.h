@@ -238,7 +238,7 @@ int ks_indexer_noalloc(const void* q, const void* k, int64_t k_batch_rows, const
  * KS_INT64).  Negative slots store nothing; slots >= n_slots store nothing and are
  * reported by ks_device_status.  Slots must not repeat within a call (one of the rows
  * would win, column by column).  A row that holds a NaN or an infinity is stored with
- * scale NaN and zero codes: it reads back as NaN.
+ * scale NaN and zero codes: it reads back as NaN in every column.
  * dq % 16 == 0, 16 <= dq <= 1024, dr % 8 == 0, 0 <= dr <= 1024, kv_stride >= D and a
  * multiple of 8; kv, kv8, kv_tail 16-byte aligned.  kv_tail may be NULL when dr = 0.
  * No counterpart in the reference.

@@ -11,7 +11,8 @@
 //   4 significant bits times a power of two fit bf16's 8.
 //
 // A row that holds a NaN or an infinity (in either part) is marked by scale = NaN and
-// zero codes, so one test per row tells every reader and no code is ever e4m3's NaN.
+// zero codes, so one test per row tells every reader and no code is ever e4m3's NaN.  It
+// reads back as NaN in every column.
 //
 // Both kernels move bytes and are bound by memory (launch latency for a few rows): LANES
 // threads share a row, and each loads all its pieces before it works on the first.  The
@@ -204,6 +205,8 @@ __global__ void __launch_bounds__(LC_THREADS) cache_read_kernel(CacheReadParams 
 #pragma unroll
   for (int k = 0; k < NT; ++k) t[k] = ldcg_or_zero(ct + k * LANES * 8, ok && (lane + k * LANES) * 8 < p.dr);
   const float s = ok ? __ldg(p.scale + src) : 0.f;
+  // (zero codes times NaN are NaN; the tail of a marked row is what was written)
+  const bool marked = s != s;
   uint16_t* o = p.out + row * (p.dq + p.dr);
 #pragma unroll
   for (int k = 0; k < NV; ++k) {
@@ -218,14 +221,15 @@ __global__ void __launch_bounds__(LC_THREADS) cache_read_kernel(CacheReadParams 
     }
     st32(o + c, h, p.wide);
   }
+  const uint4 nan = make_uint4(0x7FFF7FFFu, 0x7FFF7FFFu, 0x7FFF7FFFu, 0x7FFF7FFFu);
 #pragma unroll
   for (int k = 0; k < NT; ++k) {
     const int c = (lane + k * LANES) * 8;
-    if (c < p.dr) *reinterpret_cast<uint4*>(o + p.dq + c) = t[k];
+    if (c < p.dr) *reinterpret_cast<uint4*>(o + p.dq + c) = marked ? nan : t[k];
   }
   // a tail wider than that
   for (int c = (lane + NT * LANES) * 8; c < p.dr; c += LANES * 8)
-    *reinterpret_cast<uint4*>(o + p.dq + c) = ldcg_or_zero(p.tail + src * p.dr + c, ok);
+    *reinterpret_cast<uint4*>(o + p.dq + c) = marked ? nan : ldcg_or_zero(p.tail + src * p.dr + c, ok);
 }
 
 }  // namespace ks

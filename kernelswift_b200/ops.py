@@ -466,8 +466,8 @@ def cache_write(kv: torch.Tensor, slots: torch.Tensor, kv8: torch.Tensor, kv_sca
     dq = ``kv8.shape[-1]`` columns become e4m3 with one power-of-two scale per row (as
     ``quant_fp8_rows``), the other dr columns stay bf16.  kv8 float8_e4m3fn [pages, page,
     dq], kv_scale fp32 [pages, page], kv_tail bf16 [pages, page, dr] (None: dr = 0).  A
-    row that holds a NaN or an infinity reads back as NaN.  With dr = 0 and a page per
-    sequence, (kv8, kv_scale) are the keys ``indexer_topk_fp8`` takes."""
+    row that holds a NaN or an infinity reads back as NaN in every column.  With dr = 0 and
+    a page per sequence, (kv8, kv_scale) are the keys ``indexer_topk_fp8`` takes."""
     if kv.dtype != torch.bfloat16 or kv.dim() < 1:
         raise RuntimeError("cache_write: kv must be bfloat16 [..., D]")
     if slots.dtype not in (torch.int32, torch.int64):

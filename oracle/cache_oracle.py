@@ -57,7 +57,10 @@ def sequence_rows(codes, scale, tail, table, n):
     pos = np.arange(n)
     slot = np.asarray(pages, np.int64)[pos // page] * page + pos % page
     x = e4m3_values()[codes[slot]] * scale[slot].astype(np.float64)[:, None]
-    return x if tail is None else np.concatenate([x, tail[slot].astype(np.float64)], 1)
+    if tail is not None:
+        x = np.concatenate([x, tail[slot].astype(np.float64)], 1)
+    x[np.isnan(scale[slot])] = np.nan  # a marked row, its tail too
+    return x
 
 
 def tree_attn_row(q, rows, seen, scale, sink, dv):

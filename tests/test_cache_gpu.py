@@ -231,3 +231,20 @@ def test_refusals(cuda_ok):
         with pytest.raises(RuntimeError, match=why):
             call()
     ops.device_status()
+
+
+@pytest.mark.parametrize("dq,dr", [(128, 64), (16, 8), (512, 64), (272, 40), (64, 1024), (1024, 1024)])
+def test_rows_that_are_not_finite_read_back_as_nan_whole(cuda_ok, dq, dr):
+    """Wherever the NaN or the infinity was, no column of the row reads as a number."""
+    from kernelswift_b200 import ops
+
+    kv = torch.randn(9, dq + dr, device="cuda").bfloat16()
+    kv[1, dq - 1], kv[2, dq], kv[4, dq + dr - 1], kv[7, 0] = float("nan"), float("inf"), float("nan"), float("-inf")
+    kv8, scale, tail = empty_cache(3, 3, dq, dr)
+    ops.cache_write(kv, torch.arange(9, device="cuda"), kv8, scale, tail)
+    table = torch.arange(3, dtype=torch.int32, device="cuda")[None].contiguous()
+    back = ops.cache_read(kv8, scale, tail, table, torch.tensor([9], dtype=torch.int32, device="cuda"), 9)[0]
+    bad = torch.zeros(9, dtype=torch.bool, device="cuda")
+    bad[[1, 2, 4, 7]] = True
+    assert back[bad].isnan().all() and torch.isfinite(back[~bad].float()).all()
+    assert torch.equal(back[~bad][:, dq:], kv[~bad][:, dq:])
