@@ -47,6 +47,7 @@ int fail(int code, const char* fmt, ...) {
 }
 
 int cuda_fail(cudaError_t e, const char* what) {
+  cudaGetLastError();  // reported here: the next call's launch check is not to find it
   return fail(KS_ERR_CUDA, "%s: %s", what, cudaGetErrorString(e));
 }
 

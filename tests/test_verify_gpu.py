@@ -176,3 +176,18 @@ def test_refusals(cuda_ok):
     ]:
         with pytest.raises(RuntimeError, match=why):
             call()
+
+
+def test_a_refused_call_leaves_the_next_alone(cuda_ok):
+    """Whatever a large call is told, an ordinary one after it works."""
+    from kernelswift_b200 import ops
+
+    p, noise = torch.full((1, 2, 5_000_000), 1e-7, device="cuda"), torch.ones(1, 5_000_000, device="cuda")
+    tok, u = torch.zeros(1, 1, dtype=torch.int64, device="cuda"), torch.full((1, 2), 0.5, device="cuda")
+    for _ in range(2):
+        try:
+            ops.verify_draft(p, tok, u, noise)
+        except RuntimeError:
+            pass
+        assert ops.verify_draft(p[..., :9].contiguous(), tok, u, noise[:, :9].contiguous())[1].tolist() == [0]
+        ops.device_status()
