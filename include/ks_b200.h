@@ -314,8 +314,8 @@ int ks_tree_attn(const void* q, const void* kv8, const float* kv_scale, const vo
  * Results: n_accepted int32 [B]; out [B, T + 1] (type of tokens): the accepted tokens,
  * the next token, then -1; path int32 [B, T]: the accepted drafts' indices, then -1.
  * A token outside [0, V) or a parent outside [-1, i) is never accepted and is reported
- * by ks_device_status.  p, q, noise finite.  T <= 1024, V < 2^31.  No counterpart in the
- * reference.
+ * by ks_device_status.  p, q, noise finite.  T <= 1024, V < 2^31 - 4096.  No counterpart
+ * in the reference.
  */
 int ks_verify_draft(const float* p, const float* q, const void* tokens, int32_t token_dtype,
                     const int32_t* parents, const float* u, const float* noise, int64_t B,

@@ -1122,12 +1122,9 @@ int ks_verify_draft(const float* p, const float* q, const void* tokens, int32_t 
   vp.vec4 = V % 4 == 0 && aligned(p, 16) && aligned(noise, 16) && (!q || aligned(q, 16));
   vp.per = (int)round_up((V + cs - 1) / cs, 32);
   vp.status = dev->status;
-  // the walk's arrays and, for fixed candidates, one bit per entry of the slice
-  const size_t smem = (size_t)T * 28 + 4 + (q ? 0 : (size_t)vp.per / 8) + 16;
-  if (smem > 160 * 1024) return fail(KS_ERR_UNSUPPORTED, "verify_draft: V=%lld too large", (long long)V);
-  const void* fn = reinterpret_cast<const void*>(verify_draft_kernel);
-  if (smem > 40 * 1024)
-    if (int rc = smem_optin(dev, fn, "cudaFuncSetAttribute(verify_draft)")) return rc;
+  vp.words = std::min(vp.per, VD_BITS) / 32;
+  // the walk's arrays and, for fixed candidates, the map of children's tokens: below 48 KB
+  const size_t smem = (size_t)T * 28 + 4 + (q ? 0 : (size_t)vp.words * 4) + 16;
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute at[1];
   at[0].id = cudaLaunchAttributeClusterDimension;
@@ -1139,7 +1136,7 @@ int ks_verify_draft(const float* p, const float* q, const void* tokens, int32_t 
   cfg.stream = static_cast<cudaStream_t>(stream);
   cfg.attrs = at;
   cfg.numAttrs = 1;
-  cudaError_t e = cudaLaunchKernelEx(&cfg, verify_draft_kernel, vp);
+  cudaError_t e = cudaLaunchKernelEx(&cfg, vp.per > VD_BITS ? verify_draft_kernel<true> : verify_draft_kernel<false>, vp);
   if (e != cudaSuccess) return cuda_fail(e, "verify_draft_kernel launch");
   return launch_check("verify_draft_kernel launch");
 }

@@ -191,3 +191,49 @@ def test_a_refused_call_leaves_the_next_alone(cuda_ok):
             pass
         assert ops.verify_draft(p[..., :9].contiguous(), tok, u, noise[:, :9].contiguous())[1].tolist() == [0]
         ops.device_status()
+
+
+@pytest.mark.parametrize("B,V", [(300, 1_400_000), (1, 20_000_003)])
+def test_fixed_candidates_of_large_vocabularies(cuda_ok, B, V):
+    """The batch does not limit the vocabulary.  Tokens at powers of two from a rejected
+    child stay in the draw, the child does not."""
+    from kernelswift_b200 import ops
+
+    T = 3
+    g = torch.Generator(device="cuda").manual_seed(5)
+    p = torch.rand(B, T + 1, V, device="cuda", generator=g).mul_(1e-9)
+    tokens = torch.randint(0, V // 2, (B, T), device="cuda", generator=g)
+    at = torch.arange(B, device="cuda")
+    other = tokens[:, 0] + 2 ** (14 + at % 6)
+    p[at, 0, other] = 0.25
+    p[at[:, None], 0, tokens] = 0.2       # the children of the root: likelier than all but `other`
+    p[at, 1, V - 1] = 0.5
+    u = torch.full((B, T + 1), 0.99, device="cuda")
+    u[::3, 0] = 0.1                       # taken: the first child, whose own row then gives V - 1
+    noise = torch.ones(B, V, device="cuda")
+    parents = torch.full((B, T), -1, dtype=torch.int32, device="cuda")
+    out, n, path = ops.verify_draft(p, tokens, u, noise, parents=parents)
+    ops.device_status()
+    took = at % 3 == 0
+    alike = (tokens == other[:, None]).any(1)  # (then it is a child itself)
+    assert torch.equal(n, took.int()) and torch.equal(path[:, 0], torch.where(took, 0, -1).int())
+    assert (out[took, 0] == tokens[took, 0]).all() and (out[took, 1] == V - 1).all()
+    fine = ~took & ~alike
+    assert (out[fine, 0] == other[fine]).all()
+    assert not (out[~took, :1] == tokens[~took]).any()
+
+
+def test_many_siblings_of_a_large_vocabulary(cuda_ok):
+    """1024 siblings that are the likeliest entries: the draw passes all of them over."""
+    from kernelswift_b200 import ops
+
+    V, T = 5_000_000, 1024
+    p = torch.full((1, T + 1, V), 1e-9, device="cuda")
+    tokens = (torch.arange(T, device="cuda") * 4801 + 17)[None].contiguous()
+    p[0, 0, tokens[0]] = 0.0005
+    p[0, 0, 3_000_000] = 2e-9
+    par = torch.full((1, T), -1, dtype=torch.int32, device="cuda")
+    u = torch.full((1, T + 1), 0.9, device="cuda")
+    out, n, _ = ops.verify_draft(p, tokens, u, torch.ones(1, V, device="cuda"), parents=par)
+    ops.device_status()
+    assert n.tolist() == [0] and out[0, 0].item() == 3_000_000
