@@ -308,7 +308,8 @@ int ks_tree_attn(const void* q, const void* kv8, const float* kv_scale, const vo
  *   q == NULL: fixed candidates.  parents int32 [B, T], -1 <= parents[i] < i, gives the
  *     tree (NULL: a chain).  At row r its children c_1, c_2, .. (in index order; one that
  *     repeats an older sibling's token has probability 0 here) split [0, 1): c_k is taken
- *     if sum_{j<k} p[r, x_j] <= u[r] < sum_{j<=k} p[r, x_j].  Where none is taken the next
+ *     if sum_{j<k} p[r, x_j] <= u[r] < sum_{j<=k} p[r, x_j] (sums rounded in fp64; a u[r]
+ *     below the last of them takes exactly one child).  Where none is taken the next
  *     token is argmax_x w(x) / noise(x), w = p[r] with its children's tokens set to 0.
  *   Where w is 0 everywhere the row of p takes its place; ties go to the lowest token.
  * Results: n_accepted int32 [B]; out [B, T + 1] (type of tokens): the accepted tokens,

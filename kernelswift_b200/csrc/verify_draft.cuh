@@ -17,8 +17,8 @@
 // Drawing: argmax_x w(x) / noise(x), ties to the lowest x.  With exponential noise
 // this picks x with probability w(x) / sum w, needs no sum, and does not depend on
 // the order of the work: every operation is one correctly rounded fp32 operation per
-// entry, and the stretches are summed in fp64.  If w is zero everywhere, p's row takes
-// its place.
+// entry, and the stretches are summed in fp64 in one order.  If w is zero everywhere, p's
+// row takes its place.
 //
 // One cluster of CTAs per sequence.  Every CTA walks the draft itself (a few dependent
 // loads), then takes its slice of the one vocabulary row that matters; the slices'
@@ -144,13 +144,19 @@ __global__ void __launch_bounds__(VD_THREADS) verify_draft_kernel(VerifyParams p
     }
     __syncthreads();
     for (int i = tid >> 5; i < T; i += VD_THREADS / 32) {
-      double at = 0.0;  // where its stretch begins
+      // Where its stretch begins, and where it ends: the sum that the next sibling begins
+      // at, of the same terms in the same order, so that rounding leaves no gap and no overlap.
+      double at = 0.0;
       for (int j = lane; j < i; j += 32)
         if (par[j] == par[i]) at += px[j];
+      double to = lane == (i & 31) ? at + px[i] : at;
 #pragma unroll
-      for (int o = 16; o > 0; o >>= 1) at += __shfl_xor_sync(0xFFFFFFFFu, at, o);
+      for (int o = 16; o > 0; o >>= 1) {
+        at += __shfl_xor_sync(0xFFFFFFFFu, at, o);
+        to += __shfl_xor_sync(0xFFFFFFFFu, to, o);
+      }
       const double uu = (double)ux[i];
-      if (lane == 0 && par[i] >= -1 && at <= uu && uu < at + px[i]) next[par[i] + 1] = i;
+      if (lane == 0 && par[i] >= -1 && at <= uu && uu < to) next[par[i] + 1] = i;
     }
     __syncthreads();
     if (tid == 0) {

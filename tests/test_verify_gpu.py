@@ -237,3 +237,24 @@ def test_many_siblings_of_a_large_vocabulary(cuda_ok):
     out, n, _ = ops.verify_draft(p, tokens, u, torch.ones(1, V, device="cuda"), parents=par)
     ops.device_status()
     assert n.tolist() == [0] and out[0, 0].item() == 3_000_000
+
+
+@pytest.mark.parametrize("small", [3e-17, 1e-18, 7e-17])
+@pytest.mark.parametrize("count", [1, 40, 300])
+def test_stretches_leave_no_gap(cuda_ok, small, count):
+    """Children too small for fp64 to tell their stretches' ends apart, and a u on the edge
+    before them: u is below the children's sum, so exactly one child is taken, one whose
+    stretch lies within the sum's rounding of u."""
+    from kernelswift_b200 import ops
+
+    T, V = count + 2, 400
+    p = torch.zeros(1, T + 1, V, device="cuda")
+    p[0, 0, 0], p[0, 0, 1 : count + 1], p[0, 0, count + 1] = 0.5, small, 0.25
+    p[0, 1:, 399] = 1.0
+    u = torch.full((1, T + 1), 0.5, device="cuda")
+    par = torch.full((1, T), -1, dtype=torch.int32, device="cuda")
+    for _ in range(3):
+        out, n, path = ops.verify_draft(p, torch.arange(T, device="cuda")[None], u,
+                                        torch.ones(1, V, device="cuda"), parents=par)
+        assert n.tolist() == [1] and 1 <= path[0, 0].item() <= T - 1
+        assert out[0, :2].tolist() == [path[0, 0].item(), 399]
