@@ -20,8 +20,9 @@
 //     rotary columns have an exponent of their own.
 //   * a weight is taken to fp16 and split into three e5m2 numbers of 3 bits each, the high
 //     bytes of P, P - P0 and P - P0 - P1 as fp16, each product in columns of its own and
-//     the three added at the end.  Off by at most 2^-9 of the weight (a bf16 weight:
-//     2^-8), or 2^-26 of the row's largest weight times scale where that is more.
+//     the three added at the end.  Off by at most 2^-9 (the split) + 2^-11 (fp16) of the
+//     weight (a bf16 weight: 2^-8), or 2^-26 of the row's largest weight times scale where
+//     that is more.
 // A key's scale multiplies its scores (thread = key) and its weight.  A row has two
 // references, both whole powers of two: m of its scores, for the weights and their sum, and
 // m + mr of its scores + log2 of scale, for P = 2^(TA_TOP + s - m - mr) * scale.  So P keeps within

@@ -467,3 +467,25 @@ def test_queries_that_are_not_finite_in_either_part(cuda_ok, value, column):
     hit = torch.zeros(2, 3, 20, dtype=torch.bool, device="cuda")
     hit[0, 1, 3] = hit[1, 2, 19] = True
     assert got[hit].isnan().all() and torch.equal(got[~hit], clean[~hit])
+
+
+@pytest.mark.parametrize("B,T,H,dq,dr,dv,lens", [(3, 1, 16, 512, 64, 512, [1, 127, 900]), (2, 5, 24, 448, 64, 448, [200, 77]),
+                                                 (1, 2, 128, 128, 0, 128, [3000]), (2, 1, 5, 64, 64, 64, [2, 3])])
+def test_weights_of_the_codes_within_the_stated_bound(cuda_ok, B, T, H, dq, dr, dv, lens):
+    """Where v has no bf16 columns, the weights are off by at most 2^-9 + 2^-11 of themselves
+    (three parts of 3 bits, of a number in fp16): beside the output's rounding (2^-8) and
+    fp32 work (2^-12) nothing else is allowed."""
+    bound = 2.0 ** -8 + 2.0 ** -9 + 2.0 ** -11 + 2.0 ** -12
+    g, *a = build(B, T, H, dq, dr, 64, lens, seed=48)
+    from kernelswift_b200 import ops
+
+    q, kv8, scale, tail, table, n = a
+    got = ops.tree_attn(*a, (dq + dr) ** -0.5, dv=dv).double().cpu().numpy()
+    codes, s = kv8.view(torch.uint8).cpu().numpy().reshape(-1, dq), scale.double().cpu().numpy().reshape(-1)
+    t = tail.double().cpu().numpy().reshape(-1, dr) if dr else None
+    for b in range(B):
+        rows = C.sequence_rows(codes, s, t, (table[b].cpu().numpy(), 64), lens[b] + T)
+        for i in range(T):
+            seen = np.arange(lens[b] + T) <= lens[b] + i
+            ref, size = C.tree_attn_row(q[b, i].double().cpu().numpy(), rows, seen, (dq + dr) ** -0.5, None, dv)
+            assert (np.abs(got[b, i] - ref) <= bound * size).all()
