@@ -25,7 +25,7 @@
 // maxima meet through distributed shared memory.  Bound by reading that row of p, q and
 // the noise (8 or 12 bytes per entry), for few sequences by the chain of load latencies
 // (token -> probability -> row).  Divisions are left to the few entries that may
-// beat the warp's best so far; the noise is fetched during the walk.
+// beat the warp's best so far.
 // Measured (device time, one B200): 64 chains over 129280 entries 23.0 us (99 MB: 4.3 TB/s;
 // 39.4 us with a division per entry), 16 trees of 40 candidates 12.8 us, of which the walk
 // and the launch are most, one chain over 32003 entries 6.9 us.
