@@ -24,16 +24,18 @@
 //     weight (a bf16 weight: 2^-8), or 2^-26 of the row's largest weight times scale where
 //     that is more.
 // A key's scale multiplies its scores (thread = key) and its weight.  A row has two
-// references, both whole powers of two: m of its scores, for the weights and their sum, and
-// m + mr of its scores + log2 of scale, for P = 2^(TA_TOP + s - m - mr) * scale.  So P keeps within
-// e5m2's range by what the row itself weighs: a key that it does not see, or that has no
-// weight, takes no precision from the others, however large its values.  (One reference of
-// the scales for the CTA, the largest scale present, lost rows beside one 2^56 larger.)
+// references: m of its scores, for the weights and their sum, and m + ceil(mr) of its scores
+// + log2 of scale, for P = 2^(TA_TOP + s - m - ceil(mr)) * scale.  (m is the largest score
+// itself, so that the weight that counts most is a power of two and not rounded: with m
+// rounded up, results were up to 1.6 times as far from those of exact weights.)  So P keeps
+// within e5m2's range by what the row itself weighs: a key that it does not see, or that has
+// no weight, takes no precision from the others, however large its values.  (One reference
+// of the scales for the CTA, the largest scale present, lost rows beside one 2^56 larger.)
 // Products stay finite where the result is: scores are added up 2^-TA_DOWN as large, with the
 // softmax scale's power of two put back last (exactly, so that the largest score's distance
 // to its reference is right at any size), and the weights of the bf16 columns 2^-TA_VT.
-// The rotary columns are bf16
-// and have a bf16 product of their own; where v reaches into them (dv > dq), so do they.
+// The rotary columns are bf16 and have a bf16 product of their own; where v reaches into
+// them (dv > dq), so do they.
 //
 // Why split: with bf16 operands every tile's codes are expanded in shared memory, 147 KB
 // stored and read back per tile, next to MMAs that read their operands from the same
@@ -133,7 +135,7 @@ struct TreeAttnParams {
   uint32_t tmem_cols;
   float scale_in, scale_up;  // product: softmax scale * log2 e * 2^TA_DOWN; scale_up is a power of two
   float* part_o;          // [2 * CTAs][NR][dv]
-  float* part_ml;         // [2 * CTAs][NR][4]: m, sum, mr
+  float* part_ml;         // [2 * CTAs][NR][4]: m, sum, ceil(mr)
   int32_t* owner;         // [CTAs][4]: sequence, row tile, parts (0: none to join), CTA of the head
   int32_t by_item;        // owner is indexed by row tile of the call (there are few), else by CTA
   int* status;
@@ -155,8 +157,8 @@ struct TaShared {
   int wide;                                     // some m is so large that m + mr would be rounded
   int64_t per;                                  // units of a stretch
   int32_t left0, b0, rt0, t0, len0;             // its first tile, see TaWalk
-  alignas(16) float mneg[TA_MAX_ROWS];          // minus m, the reference of each row's scores (base 2, whole)
-  alignas(16) float mr[TA_MAX_ROWS];            // reference of its scores + log2 of the keys' scales, from m on
+  alignas(16) float mneg[TA_MAX_ROWS];          // minus m, the reference of each row's scores (base 2)
+  alignas(16) float mr[TA_MAX_ROWS];            // its largest score + log2 of the key's scale, from m on
   alignas(16) float qs[TA_MAX_ROWS];            // 2^e * scale_in of each row
   alignas(16) float qt[TA_MAX_ROWS];            // the same for its rotary columns
   float red[4][TA_MAX_ROWS];
@@ -165,7 +167,7 @@ struct TaShared {
     struct {
       float f[TA_MAX_ROWS];                     // factor of a raise of m; at the end 2^TA_VT / sum
       float fs[TA_MAX_ROWS];                    // of a raise of m + mr; at the end what a unit of P stands for / sum
-      float tp[TA_MAX_ROWS];                    // 2^(TA_TOP - mr): weight times scale to P, until the next raise
+      float tp[TA_MAX_ROWS];                    // 2^(TA_TOP - ceil(mr)): weight times scale to P, until the next raise
     };
   };
   int32_t whole[TA_AHEAD];                      // every key of the tile can come by TMA
@@ -306,11 +308,6 @@ __device__ __forceinline__ void ta_maxima(const float (&v)[8], float a, float* r
   }
   const float r = reduce16_lanes<true>(w, lane);  // value lane >> 1
   if ((lane & 1) == 0) (lane < 16 ? red : red_s)[(lane >> 1) & 7] = r;
-}
-
-// Bytes that the current phase of `bar` also waits for (no arrival).
-__device__ __forceinline__ void mbar_add_tx(uint64_t* bar, uint32_t bytes) {
-  asm volatile("mbarrier.expect_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(bar)), "r"(bytes) : "memory");
 }
 
 // MN-major operand of 64-byte rows (32 bf16) with the 64-byte swizzle: 16-byte unit u of
@@ -878,28 +875,28 @@ __global__ void __launch_bounds__(TA_THREADS<NR>, 1)
           auto most = [&](const float (&r)[4][TA_MAX_ROWS]) {
             return fmaxf(fmaxf(r[0][row], r[1][row]), fmaxf(r[2][row], r[3][row]));
           };
-          // mr from the tile's largest and the one before, both from the new m on; a row that
-          // has seen no key needs none
-          auto settle = [&](float tile, float before) {
-            const float mr = sh->mneg[row] == INFINITY ? TA_TOP : fmaxf(fmaxf(before, tile), -TA_SPAN);
-            const float tp = ta_pow2(TA_TOP - mr);
+          // mr from the tile's largest, which lies `tile` above the new m, and the one before;
+          // a row that has seen no key needs none.  m fell by `down`.
+          auto settle = [&](float tile, float down) {
+            const float old = sh->mr[row];
+            const float mr = sh->mneg[row] == INFINITY ? TA_TOP : fmaxf(fmaxf(old + down, tile), -TA_SPAN);
+            const float tp = ta_pow2(TA_TOP - ceilf(mr));
             const uint32_t top = __reduce_max_sync(0xFFFFFFFFu, __float_as_uint(tp));
             if (lane == 0) sh->tp_max = ta_log2(__uint_as_float(top));
             sh->tp[row] = tp;
             sh->mr[row] = mr;
-            sh->fs[row] = ta_pow2(before - mr);
+            sh->fs[row] = ex2f(ceilf(old) + down - ceilf(mr));
           };
-          float before = 0.f;
+          float down = 0.f;
           if (warp == 0) {
-            const float mo = -sh->mneg[row], mt = most(sh->red), st = most(sh->red_s);
-            const float mn = fmaxf(mo, ceilf(mt));
-            before = sh->mr[row] + (mo - mn);  // (NaN without a key: taken for none)
+            const float mo = -sh->mneg[row], mt = most(sh->red), st = most(sh->red_s), mn = fmaxf(mo, mt);
+            down = mo == mn ? 0.f : mo - mn;
             const bool wide = __any_sync(0xFFFFFFFFu, fabsf(mn) > 16384.f && fabsf(mn) < INFINITY);
             if (lane == 0) sh->wide = wide;
-            sh->f[row] = ta_pow2(mo - mn);
+            sh->f[row] = ex2f(down);
             sh->mneg[row] = -mn;
             __syncwarp();
-            if (!wide) settle(ceilf(st) - mn, before);
+            if (!wide) settle(st - mn, down);
           }
           named_bar_sync(1, SOFT);
           if (sh->wide) {  // the largest score + log2 of scale from the new m on, exactly
@@ -908,7 +905,7 @@ __global__ void __launch_bounds__(TA_THREADS<NR>, 1)
             for (int c = 0; c < CW; ++c) d[c] += sk_log2;
             ta_maxima(d, 0.f, &sh->red[quarter][hc], &sh->red[quarter][hc], lane);
             named_bar_sync(1, SOFT);
-            if (warp == 0) settle(ceilf(most(sh->red)), before);
+            if (warp == 0) settle(most(sh->red), down);
             named_bar_sync(1, SOFT);
           }
           exponents(false);
@@ -991,7 +988,7 @@ __global__ void __launch_bounds__(TA_THREADS<NR>, 1)
         const int slot = 2 * (int)blockIdx.x + (w.t == 0 ? 1 : 0);
         if (threadIdx.x < NR) {
           const int c = threadIdx.x;
-          const float m = -sh->mneg[c], mr = sh->mr[c];
+          const float m = -sh->mneg[c], mr = ceilf(sh->mr[c]);
           float sum = sh->red[0][c] + sh->red[1][c] + sh->red[2][c] + sh->red[3][c];
           if (whole) {
             if (p.sink && m != -INFINITY)  // (without a key the output is 0 either way)
@@ -1107,7 +1104,8 @@ __global__ void __launch_bounds__(TA_JOIN_GROUP* GROUPS) tree_attn_join_kernel(c
   float mr = -INFINITY;
 #pragma unroll
   for (int k = 0; k < PL; ++k) {
-    ml[k].z += ml[k].x - m;
+    ml[k].x = ml[k].x == m ? 0.f : ml[k].x - m;
+    ml[k].z += ml[k].x;
     mr = fmaxf(mr, ml[k].z);
   }
 #pragma unroll
@@ -1115,8 +1113,8 @@ __global__ void __launch_bounds__(TA_JOIN_GROUP* GROUPS) tree_attn_join_kernel(c
   float sum = 0.f;
 #pragma unroll
   for (int k = 0; k < PL; ++k) {
-    const float f = ta_pow2(ml[k].x - m);
-    fs[warp][0][k * 32 + lane] = ta_pow2(ml[k].z - mr);
+    const float f = ex2f(ml[k].x);
+    fs[warp][0][k * 32 + lane] = ex2f(ml[k].z - mr);
     fs[warp][1][k * 32 + lane] = f;
     sum += ml[k].y * f;
   }
@@ -1125,7 +1123,7 @@ __global__ void __launch_bounds__(TA_JOIN_GROUP* GROUPS) tree_attn_join_kernel(c
   if (p.sink && m != -INFINITY) sum += ex2f(__ldg(p.sink + row % p.H) * 1.4426950408889634f - m);
   __syncwarp();
   const int at = threadIdx.x % TA_JOIN_GROUP, d = at * 4, tail = d >= p.dq;  // (dq is a multiple of 4)
-  const float inv = (sum == 0.f ? 0.f : 1.f / sum) * (tail ? (float)(1 << TA_VT) : ta_pow2(mr - TA_TOP));
+  const float inv = (sum == 0.f ? 0.f : 1.f / sum) * (tail ? (float)(1 << TA_VT) : ex2f(mr - TA_TOP));
   float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
   if (d < p.dv)
     for (int base = group; base < parts; base += GROUPS * FLY) {

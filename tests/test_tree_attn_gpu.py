@@ -489,3 +489,27 @@ def test_weights_of_the_codes_within_the_stated_bound(cuda_ok, B, T, H, dq, dr, 
             seen = np.arange(lens[b] + T) <= lens[b] + i
             ref, size = C.tree_attn_row(q[b, i].double().cpu().numpy(), rows, seen, (dq + dr) ** -0.5, None, dv)
             assert (np.abs(got[b, i] - ref) <= bound * size).all()
+
+
+@pytest.mark.parametrize("n", [90, 3000])
+@pytest.mark.parametrize("dv", [128, 192])
+def test_a_key_with_all_the_weight_is_returned_exactly(cuda_ok, n, dv):
+    """The weight that counts most is not rounded: a key 2^-30 and more ahead of the others
+    comes out as it is cached, code times scale."""
+    from kernelswift_b200 import ops
+
+    g, q, kv8, scale, tail, table, lens = build(2, 3, 5, 128, 64, 32, [n, n // 3], seed=50)
+    q = torch.randn(2, 3, 1, 192, device="cuda", generator=g).expand(2, 3, 5, 192).bfloat16().contiguous()
+    at = [n // 9, 2, n // 3 - 1]
+    for b in range(2):
+        for i in range(3):  # each token's own favourite, its scores twice any other's or more
+            put(kv8, scale, tail, table, b, [at[i]], 8 * q[b, i, :1].float())
+    mask = torch.eye(3, dtype=torch.bool, device="cuda").repeat(2, 1, 1)
+    got = ops.tree_attn(q, kv8, scale, tail, table, lens, 0.25, dv=dv, mask=mask)
+    rows = ops.cache_read(kv8, scale, tail, table, lens, n)
+    ops.device_status()
+    for b in range(2):
+        for i in range(3):
+            s = (rows[b, : int(lens[b])].double() @ q[b, i, 0].double()) * 0.25
+            assert s.topk(2).values.diff().item() < -25 and int(s.argmax()) == at[i]
+            assert torch.equal(got[b, i], rows[b, at[i], :dv].expand(5, dv))
