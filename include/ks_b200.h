@@ -275,12 +275,12 @@ size_t ks_tree_attn_workspace_size(int64_t B, int64_t T, int64_t H, int64_t dv);
  *        of the row; attn_sink (fp32 [H], may be NULL) adds a logit that carries no value.
  *        A token that sees no key gets zeros.
  * A row stored with scale NaN makes every token that sees it NaN, and no other.
- * The weights of the e4m3 columns are kept to 2^-9 + 2^-11 of themselves, or to 2^-26 of the
- * token's largest weight times row scale where that is more, whatever the scales of rows
- * that it does not see or weigh; those of the bf16 columns to 2^-8.  A weight below 2^-100
- * of the token's largest is 0.  Elements of q in the e4m3 columns are exact down to 2^-14 of
- * a row's largest there, and rounded to 2^-21 of it below; a row of q with a NaN or an
- * infinity gives NaN where it sees a key.
+ * The weights of the e4m3 columns are kept to 2^-11 of themselves, or to 2^-26 of the token's
+ * largest weight times row scale where that is more, whatever the scales of rows that it
+ * does not see or weigh; those of the bf16 columns to 2^-8.  A weight below 2^-100 of the
+ * token's largest is 0.  Elements of q in the e4m3 columns are exact down to 2^-14 of a row's
+ * largest there, and rounded to 2^-21 of it below; a row of q with a NaN or an infinity
+ * gives NaN where it sees a key.
  * Key positions whose page is outside the table or the pool are skipped and reported by
  * ks_device_status.  kv_scale must hold powers of two up to 2^119 (or NaN), as
  * ks_cache_write writes.

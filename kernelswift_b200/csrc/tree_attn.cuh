@@ -18,11 +18,12 @@
 //     lo with 4 bits each (e: the exponent of the row's code columns, hi below 256; elements
 //     under 2^-14 of their largest are rounded to 2^-21 of it).  S = S_hi + S_lo / 16.  The
 //     rotary columns have an exponent of their own.
-//   * a weight is taken to fp16 and split into three e5m2 numbers of 3 bits each, the high
-//     bytes of P, P - P0 and P - P0 - P1 as fp16, each product in columns of its own and
-//     the three added at the end.  Off by at most 2^-9 (the split) + 2^-11 (fp16) of the
-//     weight (a bf16 weight: 2^-8), or 2^-26 of the row's largest weight times scale where
-//     that is more.
+//   * a weight is taken to fp16 and split into three e5m2 numbers of 3 bits and a sign, the
+//     high bytes of P, P - P0 and P - P0 - P1 as fp16, each rounded to nearest, which
+//     together are the 11 bits exactly; each product goes to columns of its own and the
+//     three are added at the end.  Off by at most 2^-11 of the weight (fp16; a bf16 weight:
+//     2^-8), or 2^-26 of the row's largest weight times scale where that is more.  (Parts
+//     cut off instead of rounded: 2^-9 more, at the same time.)
 // A key's scale multiplies its scores (thread = key) and its weight.  A row has two
 // references: m of its scores, for the weights and their sum, and m + ceil(mr) of its scores
 // + log2 of scale, for P = 2^(TA_TOP + s - m - ceil(mr)) * scale.  (m is the largest score
@@ -949,9 +950,13 @@ __global__ void __launch_bounds__(TA_THREADS<NR>, 1)
             if constexpr (VT) pw[c / 2 + z] = cvt_bf16x2(e0 * (1.f / (1 << TA_VT)), e1 * (1.f / (1 << TA_VT)));
             float w0, w1;
             f2_get(mul2(mul2(e, TaF2{z ? tp.y : tp.x}), sk2), w0, w1);
-            h[z] = f16x2_of(w0, w1);
-            h1[z] = sub_f16x2(h[z], h[z] & 0xFF00FF00u);
-            h2[z] = sub_f16x2(h1[z], h1[z] & 0xFF00FF00u) + 0x00800080u;  // the last part rounded to nearest
+            // rounded to nearest: half a last place is added to the magnitude and the low byte
+            // dropped (a P of 55109 goes to 57344, the largest e5m2)
+            const uint32_t w = f16x2_of(w0, w1);
+            h[z] = w + 0x00800080u;
+            const uint32_t w_1 = sub_f16x2(w, h[z] & 0xFF00FF00u);
+            h1[z] = w_1 + 0x00800080u;
+            h2[z] = sub_f16x2(w_1, h1[z] & 0xFF00FF00u) + 0x00800080u;
           }
           pc[0][c / 4] = __byte_perm(h[0], h[1], 0x7531);
           pc[1][c / 4] = __byte_perm(h1[0], h1[1], 0x7531);

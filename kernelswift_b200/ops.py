@@ -541,8 +541,8 @@ def tree_attn(q: torch.Tensor, kv8: torch.Tensor, kv_scale: torch.Tensor,
     where ``mask[b, i, j]`` (bool [B,T,T]; None: j <= i, a chain).  attn_sink fp32 [H]
     as in ``sparse_attn``.  Returns bf16 [B,T,H,dv], v = the first ``dv`` (default
     min(D, 512)) columns of the cached rows; a token that sees nothing gets zeros.  The
-    weights are kept to 2^-9 + 2^-11 of themselves for the e4m3 columns, to 2^-8 for the
-    bf16 ones (scores and sums in fp32, the result rounded once)."""
+    weights are kept to 2^-11 of themselves for the e4m3 columns, to 2^-8 for the bf16 ones
+    (scores and sums in fp32, the result rounded once)."""
     if q.dtype != torch.bfloat16 or q.dim() != 4:
         raise RuntimeError("tree_attn: q must be bfloat16 [b, t, h, d]")
     pages, page, dq, dr, ts = _cache_args("tree_attn", kv8, kv_scale, kv_tail)

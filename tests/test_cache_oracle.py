@@ -97,3 +97,19 @@ def test_ops_refuse_host_tensors_and_wrong_shapes():
     ]:
         with pytest.raises(RuntimeError, match=why):
             call()
+
+
+def test_three_e5m2_parts_hold_a_half_exactly():
+    """The split of tree attention's weights, restated: parts rounded to nearest at fp16's
+    high byte (an e5m2 number) add up to every fp16 number from 2^-3 to 55109 exactly, and to
+    smaller ones within half of e5m2's smallest."""
+    half = np.arange(0x7B00, dtype=np.uint16)
+    w = half.view(np.float16).astype(np.float64)
+    half, w = half[w <= 55109], w[w <= 55109]
+    rest, parts = half.view(np.float16), 0.0
+    for _ in range(3):
+        part = ((rest.view(np.uint16).astype(np.uint32) + 0x80) & 0xFF00).astype(np.uint16).view(np.float16)
+        assert np.isfinite(part).all()
+        parts = parts + part.astype(np.float64)
+        rest = rest - part
+    assert (parts == w)[w >= 2.0 ** -3].all() and (np.abs(parts - w) <= 2.0 ** -17).all()
