@@ -1065,9 +1065,11 @@ int ks_tree_attn(const void* q, const void* kv8, const float* kv_scale, const vo
   const int64_t most = B * p.row_tiles * std::max<int64_t>(1, (max_pages * page + 127) / 128);
   const int64_t sms = std::min(dev->num_sms, TA_MAX_CTAS);
   // Short tables: a CTA per row tile and no join, which costs about six tiles.  (16 heads of
-  // 576 columns, split against whole: one sequence of 510 keys 12.5 and 12.9 us, 40 of them
-  // 16.9 and 13.8, 100 19.4 and 14.5; one of 1022 keys 13.1 and 18.5, 40 19.0 and 19.0,
-  // 100 28.4 and 22.9.)
+  // 576 columns, split against whole, on the device: one sequence of 510 keys 12.1 and 12.8 us
+  // -- but a launch less on the host: 20.8 and 19.4 us a call --, 40 of them 17.0 and 14.1,
+  // 100 21.7 and 14.6; one of 1022 keys 13.1 and 18.5, 40 20.6 and 18.6, 100 29.7 and 23.0.)
+  // The host knows the table's width only: short contexts in a table for 131072 keys are
+  // split, and take the first of each pair.
   const int64_t items = B * p.row_tiles;
   p.solo = items <= sms && max_pages * page <= (items * 4 >= sms ? 2 * TA_SOLO : TA_SOLO);
   const unsigned grid = (unsigned)(p.solo ? items : std::min(most, sms));

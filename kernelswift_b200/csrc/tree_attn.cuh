@@ -69,15 +69,15 @@
 // Softmax: references are raised only when some weight passes 2^TA_RISE or some P 2^(TA_TOP
 // + TA_GROW), together with sum and output (one vote per tile).  A raise costs more than a
 // tile, so the limit is what e5m2's range allows, and all rows that have grown are raised at
-// once: large trees (below) take 712 us without any raise, 749 so, 778 where only rows past
-// the limit are raised, 808 with TA_GROW = 5 too.  Sums are kept per thread in fp32 and
-// reduced once per row tile.
+// once: large trees (below) take 751 us so, 778 where only rows past the limit are raised,
+// 808 with TA_GROW = 5 too (one run); all raises together are 1 to 5 % of a call.  Sums are
+// kept per thread in fp32 and reduced once per row tile.
 //
-// Measured (device time, one B200): 8 trees of 32 tokens, 128 heads, 8192 keys 742 us (585
-// GFLOP of scores and outputs: 789 TFLOP/s); 16 trees of 13 tokens, 64 heads, up to 6001 keys
-// 167 us; one token of 128 heads over 131069 keys 70.5 us; 48 sequences of up to 8000 keys, 16
-// heads 36.4 us (128 MB: 3.5 TB/s).  Bound: at 32 rows a tile takes about 2.8 K cycles, the
-// MMAs 1.9 K of them (counters: tensor pipe 41 %, shared memory 60 %); the rest is the chain
+// Measured (device time, one B200): 8 trees of 32 tokens, 128 heads, 8192 keys 750 us (585
+// GFLOP of scores and outputs: 780 TFLOP/s); 16 trees of 13 tokens, 64 heads, up to 6001 keys
+// 175 us; one token of 128 heads over 131069 keys 70.8 us; 48 sequences of up to 8000 keys, 16
+// heads 37.0 us (128 MB: 3.5 TB/s).  Bound: at 32 rows a tile takes about 2.8 K cycles, the
+// MMAs 1.9 K of them (counters: tensor pipe 42 %, shared memory 61 %); the rest is the chain
 // chunk given back -> load (1.3 K from L2) -> scores -> softmax (2.2 K) -> output, of which
 // two tiles are in flight, because nine chunks and a row tile's queries fill shared memory
 // and its outputs TMEM.  A row tile's beginning and end cost about 10 K cycles.  At 16 rows a

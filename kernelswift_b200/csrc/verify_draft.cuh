@@ -26,9 +26,10 @@
 // the noise (8 or 12 bytes per entry), for few sequences by the chain of load latencies
 // (token -> probability -> row).  Divisions are left to the few entries that may
 // beat the warp's best so far.
-// Measured (device time, one B200): 64 chains over 129280 entries 23.0 us (99 MB: 4.3 TB/s;
-// 39.4 us with a division per entry), 16 trees of 40 candidates 12.8 us, of which the walk
-// and the launch are most, one chain over 32003 entries 6.9 us.
+// Measured (device time, one B200): 64 chains over 129280 entries 22.9 us (99 MB: 4.3 TB/s;
+// 39.4 us with a division per entry), 16 trees of 40 candidates 13.0 us, of which the walk
+// and the launch are most, one chain over 32003 entries 6.9 us.  With the noise prefetched to
+// L2 before the walk: 38.1, 19.6 and 7.1 us.
 #pragma once
 #include "ks_device.cuh"
 

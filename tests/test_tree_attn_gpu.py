@@ -513,3 +513,21 @@ def test_a_key_with_all_the_weight_is_returned_exactly(cuda_ok, n, dv):
             s = (rows[b, : int(lens[b])].double() @ q[b, i, 0].double()) * 0.25
             assert s.topk(2).values.diff().item() < -25 and int(s.argmax()) == at[i]
             assert torch.equal(got[b, i], rows[b, at[i], :dv].expand(5, dv))
+
+
+@pytest.mark.parametrize("sm", [0.0, -0.07, 2.0 ** -120, 1e-42, 40.0])
+def test_any_softmax_scale(cuda_ok, sm):
+    g, *a = build(2, 2, 20, 128, 64, 32, [300, 41], seed=51)
+    check(*a, float(np.float32(sm)), 192)
+
+
+@pytest.mark.parametrize("n", [60, 3000])
+def test_sinks_of_any_size(cuda_ok, n):
+    from kernelswift_b200 import ops
+
+    g, *a = build(2, 1, 6, 128, 64, 32, [n, n // 3], seed=52)
+    sink = torch.tensor([float("-inf"), -1e30, 0.0, 60.0, 1e30, float("inf")], device="cuda")
+    got = ops.tree_attn(*a, 0.07, dv=192, attn_sink=sink)
+    assert (got[:, :, 4:] == 0).all()
+    q, *rest = a
+    check(q[:, :, :4].contiguous(), *rest, 0.07, 192, None, sink[:4].contiguous(), got=got[:, :, :4])
