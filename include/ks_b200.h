@@ -279,8 +279,9 @@ size_t ks_tree_attn_workspace_size(int64_t B, int64_t T, int64_t H, int64_t dv);
  * largest weight times row scale where that is more, whatever the scales of rows that it
  * does not see or weigh; those of the bf16 columns to 2^-8.  A weight below 2^-100 of the
  * token's largest is 0.  Elements of q in the e4m3 columns are exact down to 2^-14 of a row's
- * largest there, and rounded to 2^-21 of it below; a row of q with a NaN or an infinity
- * gives NaN where it sees a key.
+ * largest there, and rounded to 2^-21 of it below (or to 2^-30 of the row's largest rotary
+ * element where that is more); a row of q with a NaN or an infinity gives NaN where it sees
+ * a key.
  * Key positions whose page is outside the table or the pool are skipped and reported by
  * ks_device_status.  kv_scale must hold powers of two up to 2^119 (or NaN), as
  * ks_cache_write writes.

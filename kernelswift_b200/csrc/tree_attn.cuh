@@ -17,7 +17,8 @@
 //   * a query element is 8 significant bits of bf16: q 2^-e = hi + lo / 16 exactly, hi and
 //     lo with 4 bits each (e: the exponent of the row's code columns, hi below 256; elements
 //     under 2^-14 of their largest are rounded to 2^-21 of it).  S = S_hi + S_lo / 16.  The
-//     rotary columns have an exponent of their own.
+//     rotary columns are scaled alike; where they are more than 2^TA_ROTARY times as large, e
+//     goes by them (an exponent of their own made ragged trees 2 % slower).
 //   * a weight is taken to fp16 and split into three e5m2 numbers of 3 bits and a sign, the
 //     high bytes of P, P - P0 and P - P0 - P1 as fp16, each rounded to nearest, which
 //     together are the 11 bits exactly; each product goes to columns of its own and the
@@ -107,7 +108,8 @@ constexpr int TA_LEVELS = 3;                 // e5m2 columns per weight
 constexpr float TA_TOP = 10.f;               // P at the reference m + mr is 2^TA_TOP
 constexpr float TA_GROW = 5.75f;             // how far it may grow past that (base 2): 2^(TA_TOP + TA_GROW) < 57344
 constexpr float TA_RISE = 7.f;               // how far a score may pass m (base 2)
-constexpr int TA_DOWN = 20;                  // scores are added up 2^20 too small: 256 * 448 * 512 * 2^(119 - 20) is finite
+constexpr int TA_DOWN = 24;                  // scores are added up 2^24 too small: 256 * 448 * 512 * 2^(119 - 24) is finite
+constexpr int TA_ROTARY = 9;                 // bits by which rotary elements may be larger: 64 * 2^(8 + 9 - 24) * 2^128 is finite
 constexpr int TA_VT = 24;                    // bf16 weights are 2^24 too small: 2^(TA_RISE - 24) * 2^17 keys * 2^128 is finite
 constexpr float TA_SPAN = 110.f;             // how far m + mr may lie below m: 2^(TA_TOP + TA_SPAN + TA_RISE) is finite
 
@@ -161,7 +163,6 @@ struct TaShared {
   alignas(16) float mneg[TA_MAX_ROWS];          // minus m, the reference of each row's scores (base 2)
   alignas(16) float mr[TA_MAX_ROWS];            // its largest score + log2 of the key's scale, from m on
   alignas(16) float qs[TA_MAX_ROWS];            // 2^e * scale_in of each row
-  alignas(16) float qt[TA_MAX_ROWS];            // the same for its rotary columns
   float red[4][TA_MAX_ROWS];
   union {  // a row's four maxima are read by the thread that then writes its factors
     alignas(16) float red_s[4][TA_MAX_ROWS];
@@ -728,9 +729,8 @@ __global__ void __launch_bounds__(TA_THREADS<NR>, 1)
       for (int o = LR / 2; o > 0; o >>= 1) larger(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
       const uint32_t top_c = top & 0xFFFFu, top_t = top >> 16;
       const bool bad = top_c >= 0x7F80u || top_t >= 0x7F80u;
-      // largest element into [128, 256)
-      const int e = bad ? 0 : max((int)(top_c >> 7) - 127 - 7, -126);
-      const int et = bad ? 0 : max((int)(top_t >> 7) - 127 - 7, -126);
+      // largest code column into [128, 256), rotary ones below 2^(8 + TA_ROTARY)
+      const int e = bad ? 0 : max(max((int)(top_c >> 7), (int)(top_t >> 7) - TA_ROTARY) - 127 - 7, -126);
       const float inv = __uint_as_float((uint32_t)(127 - e) << 23);
 #pragma unroll
       for (int k = 0; k < QV; ++k) {
@@ -753,15 +753,12 @@ __global__ void __launch_bounds__(TA_THREADS<NR>, 1)
         *reinterpret_cast<uint2*>(dst + NR * 128) = bad ? make_uint2(0u, 0u) : make_uint2(lo[0], lo[1]);
       }
       if (at * 8 < p.dr) {
-        const uint32_t m2 = (uint32_t)(127 - et) * 0x00800080u, down = (127u - TA_DOWN) * 0x00800080u;
+        const uint32_t m2 = (uint32_t)(127 - e) * 0x00800080u, down = (127u - TA_DOWN) * 0x00800080u;
         auto scaled = [&](uint32_t x) { return bad ? 0u : mul_bf16x2(mul_bf16x2(x, m2), down); };
         *reinterpret_cast<uint4*>(qs + p.nc * (2 * NR * 128) + row * 128 + ((at ^ (row & 7)) << 4)) =
             make_uint4(scaled(t.x), scaled(t.y), scaled(t.z), scaled(t.w));
       }
-      if (at == 0) {
-        sh->qs[row] = __uint_as_float((uint32_t)(127 + e) << 23) * p.scale_in;
-        sh->qt[row] = __uint_as_float((uint32_t)(127 + et) << 23) * p.scale_in;
-      }
+      if (at == 0) sh->qs[row] = __uint_as_float((uint32_t)(127 + e) << 23) * p.scale_in;
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) mbar_arrive(&sh->q_full);
@@ -828,13 +825,11 @@ __global__ void __launch_bounds__(TA_THREADS<NR>, 1)
 #pragma unroll
           for (int c = 0; c < CW; c += 4) {
             const ulonglong2 s4 = *reinterpret_cast<const ulonglong2*>(&sh->qs[hc + c]);
-            const ulonglong2 t4 = *reinterpret_cast<const ulonglong2*>(&sh->qt[hc + c]);
 #pragma unroll
-            for (int z = c; z < c + 4; z += 2) {
-              const TaF2 u = fma2(f2(lo[z], lo[z + 1]), sixteenth, f2(hi[z], hi[z + 1]));
-              const TaF2 sc = mul2(mul2(u, sk2), TaF2{z == c ? s4.x : s4.y});
-              x[z / 2] = p.dr ? fma2(f2(tl[z], tl[z + 1]), TaF2{z == c ? t4.x : t4.y}, sc) : sc;
-            }
+            for (int z = c; z < c + 4; z += 2)
+              x[z / 2] = mul2(fma2(fma2(f2(lo[z], lo[z + 1]), sixteenth, f2(hi[z], hi[z + 1])), sk2,
+                                   p.dr ? f2(tl[z], tl[z + 1]) : f2(0.f, 0.f)),
+                              TaF2{z == c ? s4.x : s4.y});
           }
         }
         float d[CW];
