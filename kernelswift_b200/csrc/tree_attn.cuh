@@ -76,8 +76,8 @@
 //
 // Measured (device time, one B200): 8 trees of 32 tokens, 128 heads, 8192 keys 750 us (585
 // GFLOP of scores and outputs: 780 TFLOP/s); 16 trees of 13 tokens, 64 heads, up to 6001 keys
-// 175 us; one token of 128 heads over 131069 keys 70.8 us; 48 sequences of up to 8000 keys, 16
-// heads 37.0 us (128 MB: 3.5 TB/s).  Bound: at 32 rows a tile takes about 2.8 K cycles, the
+// 173 us; one token of 128 heads over 131069 keys 69.8 us; 48 sequences of up to 8000 keys, 16
+// heads 36.9 us (128 MB: 3.5 TB/s).  Bound: at 32 rows a tile takes about 2.8 K cycles, the
 // MMAs 1.9 K of them (counters: tensor pipe 42 %, shared memory 61 %); the rest is the chain
 // chunk given back -> load (1.3 K from L2) -> scores -> softmax (2.2 K) -> output, of which
 // two tiles are in flight, because nine chunks and a row tile's queries fill shared memory
