@@ -274,7 +274,9 @@ size_t ks_tree_attn_workspace_size(int64_t B, int64_t T, int64_t H, int64_t dv);
  *   out  bf16 [B, T, H, dv] = softmax(softmax_scale * q . k) v, v = the first dv columns
  *        of the row; attn_sink (fp32 [H], may be NULL) adds a logit that carries no value.
  *        A token that sees no key gets zeros.
- * A row stored with scale NaN makes every token that sees it NaN, and no other.
+ * A row stored with scale NaN makes every token that sees it NaN, and no other.  Hidden rows
+ * have to have been written too, now or before: memory that never was may hold e4m3's NaN,
+ * which reaches every token of its sequence.
  * The weights of the e4m3 columns are kept to 2^-11 of themselves, or to 2^-26 of the token's
  * largest weight times row scale where that is more, whatever the scales of rows that it
  * does not see or weigh; those of the bf16 columns to 2^-8.  A weight below 2^-100 of the

@@ -537,7 +537,8 @@ def tree_attn(q: torch.Tensor, kv8: torch.Tensor, kv_scale: torch.Tensor,
     q bf16 [B,T,H,D]; the cache as ``cache_write`` fills it (D = dq + dr, dq a multiple
     of 64 up to 512, dr 0 or 64), page_table int32 [B, max_pages].  Every drafted token
     sees the ``lens[b]`` cached positions; the drafted tokens' own rows follow at
-    positions lens[b] .. lens[b]+T-1 (already written), and token i sees row j of them
+    positions lens[b] .. lens[b]+T-1 (already written, hidden ones too; a zeroed cache
+    counts as written), and token i sees row j of them
     where ``mask[b, i, j]`` (bool [B,T,T]; None: j <= i, a chain).  attn_sink fp32 [H]
     as in ``sparse_attn``.  Returns bf16 [B,T,H,dv], v = the first ``dv`` (default
     min(D, 512)) columns of the cached rows; a token that sees nothing gets zeros.  The
