@@ -329,6 +329,48 @@ int ks_verify_draft(const float* p, const float* q, const void* tokens, int32_t 
                     void* stream);
 
 /*
+ * Appends keys and values to a paged per-head cache in e4m3, rotated on the way, with one
+ * power-of-two scale for each block of tokens and head.
+ *   k, v   bf16 [B, T, heads, D]: a token's rows together, tokens *_ts and sequences *_bs
+ *          elements apart (multiples of 8)
+ *   q      bf16 [B, T, q_heads, D] laid out likewise, or NULL; q_out (contiguous) gets its
+ *          rows rotated like the keys, rounded once
+ *   freqs  fp32 [n_freqs, rope_dim / 2, 2] (cos, sin): the last rope_dim columns of a key are
+ *          rotated, as pairs (2 i, 2 i + 1), by the row of its position (positions int32
+ *          [B, T], or NULL: its place in the sequence); rope_dim 0: no rotation
+ *   k8, v8 e4m3 [n_pages, heads, page, D], k_scale, v_scale fp32 [n_pages, heads, page / block]
+ *   page_table int32 [B, max_pages], lens int32 [B]: tokens cached so far; token t of
+ *          sequence b goes to position lens[b] + t, if t < n_new[b] (NULL: T)
+ * scale = the smallest power of two >= max(amax, 1e-4) / 448 (at most 2^119) over the new rows of
+ * the block, and not less than before where the block holds rows below lens[b], which are
+ * then rounded again to it; code = e4m3(x / scale).  An element that is NaN or infinite becomes
+ * e4m3's NaN, and the lowest bit of its block's scale is set.  D 64, 128, 192 or 256; block a
+ * multiple of 16 up to 128, page of block.  Rows behind a sequence's last are left as they
+ * were.  Tokens past the table or on a page outside [0, n_pages) are not stored, positions
+ * outside freqs take its nearest row; both are reported by ks_device_status.  lens is not
+ * changed.  No counterpart in the reference.
+ */
+int ks_kv_append(const void* k, int64_t k_bs, int64_t k_ts, const void* v, int64_t v_bs,
+                 int64_t v_ts, const void* q, int64_t q_bs, int64_t q_ts, int32_t q_heads,
+                 void* q_out, const float* freqs, int64_t n_freqs, int32_t rope_dim,
+                 const int32_t* positions, void* k8, float* k_scale, void* v8, float* v_scale,
+                 int64_t n_pages, int32_t heads, int32_t page, int32_t block, int32_t D,
+                 const int32_t* page_table, int64_t max_pages, const int32_t* lens,
+                 const int32_t* n_new, int64_t B, int64_t T, void* stream);
+
+/*
+ * Log probabilities of given tokens from logits [N, V] (rows ld elements apart, bf16 where
+ * is_bf16, else fp32): logp fp32 [N] = x[token] - logsumexp(x), entropy fp32 [N] (nats), and the
+ * top (<= 32, <= V) largest as top_logp fp32 [N, top], top_ids [N, top] (type of tokens), largest
+ * first, the lowest index first among equal ones.  tokens int32 or int64 [N] (token_dtype);
+ * a negative token's logp is 0, one >= V gets NaN and is reported by ks_device_status.  A
+ * row without a finite maximum, or with a NaN, gets NaN.  No counterpart in the reference.
+ */
+int ks_token_logprobs(const void* logits, int32_t is_bf16, int64_t ld, const void* tokens,
+                      int32_t token_dtype, int64_t N, int64_t V, int32_t top, float* logp,
+                      float* entropy, float* top_logp, void* top_ids, void* stream);
+
+/*
  * Synchronise `stream`, then read and clear the current device's status record:
  * KS_OK, or KS_ERR_DEVICE when a kernel reported a timed-out wait or a bounds
  * error since the last call (ks_last_error() then names the block, thread,

@@ -66,6 +66,11 @@ SIGNATURES = {
                                     _c_f32, _vp, _sz, _vp]),
     "ks_verify_draft": (ctypes.c_int, [_vp, _vp, _vp, _c_i32, _vp, _vp, _vp, _c_i64, _c_i64,
                                        _c_i64, _vp, _vp, _vp, _vp]),
+    "ks_kv_append": (ctypes.c_int, [_vp, _c_i64, _c_i64, _vp, _c_i64, _c_i64, _vp, _c_i64, _c_i64, _c_i32,
+                                    _vp, _vp, _c_i64, _c_i32, _vp, _vp, _vp, _vp, _vp, _c_i64, _c_i32,
+                                    _c_i32, _c_i32, _c_i32, _vp, _c_i64, _vp, _vp, _c_i64, _c_i64, _vp]),
+    "ks_token_logprobs": (ctypes.c_int, [_vp, _c_i32, _c_i64, _vp, _c_i32, _c_i64, _c_i64, _c_i32, _vp,
+                                         _vp, _vp, _vp, _vp]),
     "ks_device_status": (ctypes.c_int, [_vp]),
     "ks_selftest_wait_timeout": (ctypes.c_int, [_c_u64, _vp]),
 }

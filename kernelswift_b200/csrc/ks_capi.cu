@@ -14,6 +14,7 @@
 #include "ks_b200.h"
 #include "ks_device.cuh"
 #include "indexer_score.cuh"
+#include "kv_cache.cuh"
 #include "latent_cache.cuh"
 #include "proj_gemm.cuh"
 #include "quant_fp8.cuh"
@@ -21,6 +22,7 @@
 #include "sparse_attn.cuh"
 #include "sparse_attn_small.cuh"
 #include "sparse_attn_tiny.cuh"
+#include "token_logprobs.cuh"
 #include "topk.cuh"
 #include "topk_small.cuh"
 #include "tree_attn.cuh"
@@ -594,6 +596,32 @@ int table_check(const char* op, const int32_t* table, int64_t max_pages, const i
   return KS_OK;
 }
 
+// The per-head cache (kv_append, kv_attn): checks its arguments and fills *c.
+int kv_cache_check(const char* op, KvCache* c, void* k8, float* k_scale, void* v8, float* v_scale, int64_t n_pages,
+                   int32_t heads, int32_t page, int32_t block, int32_t D, const int32_t* table, int64_t max_pages,
+                   const int32_t* lens, const int32_t* n_new, int64_t B, int64_t T) {
+  if (!k8 || !k_scale || !v8 || !v_scale) return fail(KS_ERR_INVALID, "%s: null cache pointer", op);
+  if (int rc = table_check(op, table, max_pages, lens, n_pages, page, B)) return rc;
+  if (heads < 1 || heads > 1024) return fail(KS_ERR_INVALID, "%s: kv heads=%d (1..1024)", op, heads);
+  if (D != 64 && D != 128 && D != 192 && D != 256)
+    return fail(KS_ERR_UNSUPPORTED, "%s: D=%d (64, 128, 192 or 256)", op, D);
+  if (block < 16 || block % 16 || block > KV_MAX_BLOCK || page % block)
+    return fail(KS_ERR_UNSUPPORTED, "%s: page=%d block=%d (block a multiple of 16 up to %d, page of block)", op, page, block, KV_MAX_BLOCK);
+  if (max_pages * page >= (1ll << 31)) return fail(KS_ERR_UNSUPPORTED, "%s: max_pages * page >= 2^31", op);
+  if (T > (1 << 24) || B * T >= (1ll << 31)) return fail(KS_ERR_UNSUPPORTED, "%s: too many tokens", op);
+  if (!aligned(k8, 16) || !aligned(v8, 16) || !aligned(k_scale, 4) || !aligned(v_scale, 4) || !aligned(n_new, 4))
+    return fail(KS_ERR_ALIGNMENT, "%s: k8, v8 must be 16-byte and the scales, n_new 4-byte aligned", op);
+  c->k8 = static_cast<uint8_t*>(k8);
+  c->k_scale = k_scale;
+  c->v8 = static_cast<uint8_t*>(v8);
+  c->v_scale = v_scale;
+  c->n_pages = n_pages; c->max_pages = max_pages;
+  c->table = table; c->lens = lens; c->n_new = n_new;
+  c->heads = heads; c->page = page; c->block = block; c->d = D;
+  c->B = (int)B; c->T = (int)T;
+  return KS_OK;
+}
+
 // Rows of a row tile for a sequence's T * H query rows: 32 fill the tensor memory; 16 rows
 // take fewer columns of every product where there are no more.
 int ta_rows(int64_t rows) { return rows <= 16 ? 16 : 32; }
@@ -1141,6 +1169,102 @@ int ks_verify_draft(const float* p, const float* q, const void* tokens, int32_t 
   cudaError_t e = cudaLaunchKernelEx(&cfg, vp.per > VD_BITS ? verify_draft_kernel<true> : verify_draft_kernel<false>, vp);
   if (e != cudaSuccess) return cuda_fail(e, "verify_draft_kernel launch");
   return launch_check("verify_draft_kernel launch");
+}
+
+int ks_kv_append(const void* k, int64_t k_bs, int64_t k_ts, const void* v, int64_t v_bs,
+                 int64_t v_ts, const void* q, int64_t q_bs, int64_t q_ts, int32_t q_heads,
+                 void* q_out, const float* freqs, int64_t n_freqs, int32_t rope_dim,
+                 const int32_t* positions, void* k8, float* k_scale, void* v8, float* v_scale,
+                 int64_t n_pages, int32_t heads, int32_t page, int32_t block, int32_t D,
+                 const int32_t* page_table, int64_t max_pages, const int32_t* lens,
+                 const int32_t* n_new, int64_t B, int64_t T, void* stream) {
+  Device* dev;
+  if (int rc = device(&dev)) return rc;
+  if (B < 0 || T < 0) return fail(KS_ERR_INVALID, "kv_append: bad sizes B=%lld T=%lld", (long long)B, (long long)T);
+  if (B == 0 || T == 0) return KS_OK;
+  KvAppendParams p{};
+  if (int rc = kv_cache_check("kv_append", &p.c, k8, k_scale, v8, v_scale, n_pages, heads, page, block, D, page_table, max_pages, lens, n_new, B, T)) return rc;
+  if (!k || !v || (q && !q_out)) return fail(KS_ERR_INVALID, "kv_append: null pointer");
+  if (rope_dim < 0 || rope_dim % 8 || rope_dim > D) return fail(KS_ERR_INVALID, "kv_append: rope_dim=%d (a multiple of 8 up to D)", rope_dim);
+  if (rope_dim && (!freqs || n_freqs < 1)) return fail(KS_ERR_INVALID, "kv_append: rope_dim needs freqs");
+  if (q && (q_heads < 1 || q_heads > 65536)) return fail(KS_ERR_INVALID, "kv_append: q_heads=%d", q_heads);
+  if (!aligned(k, 16) || !aligned(v, 16) || !aligned(q, 16) || !aligned(q_out, 16) || (k_bs | k_ts | v_bs | v_ts) % 8 ||
+      (q && (q_bs | q_ts) % 8))
+    return fail(KS_ERR_ALIGNMENT, "kv_append: the rows of k, v, q must start on 16-byte boundaries");
+  if ((rope_dim && !aligned(freqs, 16)) || !aligned(positions, 4))
+    return fail(KS_ERR_ALIGNMENT, "kv_append: freqs must be 16-byte and positions 4-byte aligned");
+  p.c.status = dev->status;
+  p.k = static_cast<const uint16_t*>(k);
+  p.v = static_cast<const uint16_t*>(v);
+  p.q = static_cast<const uint16_t*>(q);
+  p.q_out = static_cast<uint16_t*>(q_out);
+  p.k_bs = k_bs; p.k_ts = k_ts; p.v_bs = v_bs; p.v_ts = v_ts; p.q_bs = q_bs; p.q_ts = q_ts;
+  p.freqs = rope_dim ? freqs : nullptr;
+  p.pos = positions;
+  p.n_freqs = n_freqs;
+  p.rd = rope_dim;
+  p.q_heads = q ? q_heads : 0;
+  p.nb = (int)((block - 1 + T - 1) / block + 1);  // however the first block is filled
+  p.kv_ctas = B * p.nb * 2 * heads;
+  p.q_pieces = q ? B * T * q_heads * (D / 8) : 0;
+  // 8-column pieces of a block, up to eight per thread
+  const int pieces = block * D / 8;
+  const int threads = pieces <= 1024 ? 128 : pieces <= 2048 ? 256 : 512;
+  const int64_t q_ctas = (p.q_pieces + threads * KV_Q_PIECES - 1) / (threads * KV_Q_PIECES);
+  if (p.kv_ctas + q_ctas >= (1ll << 31)) return fail(KS_ERR_UNSUPPORTED, "kv_append: too many tokens");
+  const unsigned grid = (unsigned)(p.kv_ctas + q_ctas);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (pieces <= 128) kv_append_kernel<1><<<grid, threads, 0, st>>>(p);
+  else if (pieces <= 256) kv_append_kernel<2><<<grid, threads, 0, st>>>(p);
+  else if (pieces <= 512) kv_append_kernel<4><<<grid, threads, 0, st>>>(p);
+  else kv_append_kernel<8><<<grid, threads, 0, st>>>(p);
+  return launch_check("kv_append_kernel launch");
+}
+
+int ks_token_logprobs(const void* logits, int32_t is_bf16, int64_t ld, const void* tokens,
+                      int32_t token_dtype, int64_t N, int64_t V, int32_t top, float* logp,
+                      float* entropy, float* top_logp, void* top_ids, void* stream) {
+  Device* dev;
+  if (int rc = device(&dev)) return rc;
+  if (N < 0 || V < 1 || top < 0) return fail(KS_ERR_INVALID, "token_logprobs: bad sizes N=%lld V=%lld top=%d", (long long)N, (long long)V, top);
+  if (token_dtype != KS_INT32 && token_dtype != KS_INT64) return fail(KS_ERR_INVALID, "token_logprobs: token_dtype");
+  if (top > LP_MAX_TOP || top > V) return fail(KS_ERR_UNSUPPORTED, "token_logprobs: top=%d (at most %d, and V)", top, LP_MAX_TOP);
+  if (ld < V) return fail(KS_ERR_INVALID, "token_logprobs: ld=%lld is less than a row", (long long)ld);
+  if (N == 0) return KS_OK;
+  if (!logits || !tokens || !logp || !entropy || (top && (!top_logp || !top_ids)))
+    return fail(KS_ERR_INVALID, "token_logprobs: null pointer");
+  const int ts = token_dtype == KS_INT64 ? 8 : 4;
+  if (!aligned(logits, is_bf16 ? 2 : 4) || !aligned(tokens, ts) || !aligned(logp, 4) || !aligned(entropy, 4) ||
+      !aligned(top_logp, 4) || !aligned(top_ids, ts))
+    return fail(KS_ERR_ALIGNMENT, "token_logprobs: pointers must be aligned to their elements");
+  if (V >= 0x7FFFFFFFll - 65536 || N > (1 << 27)) return fail(KS_ERR_UNSUPPORTED, "token_logprobs: too large");
+  // As many CTAs per row as hold it in registers at once, more where there are few rows and
+  // each still has a few thousand values.
+  const int64_t pass = (int64_t)LP_THREADS * LP_PIECES * (is_bf16 ? 8 : 4);
+  int cs = 1;
+  while (cs < LP_MAX_CLUSTER && ((V + cs - 1) / cs + 8 > pass || (N * cs * 2 <= dev->num_sms && V / cs >= 8192))) cs <<= 1;
+  LogprobsParams p{};
+  p.x = logits;
+  p.ld = ld;
+  p.tokens = tokens;
+  p.tok_i64 = token_dtype == KS_INT64;
+  p.N = N; p.V = (int)V; p.top = top;
+  p.per = (int)round_up((V + cs - 1) / cs, 8);
+  p.logp = logp; p.entropy = entropy; p.top_logp = top_logp; p.top_ids = top_ids;
+  p.status = dev->status;
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = (unsigned)cs;
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  cfg.gridDim = dim3((unsigned)(N * cs));
+  cfg.blockDim = dim3(LP_THREADS);
+  cfg.stream = static_cast<cudaStream_t>(stream);
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  cudaError_t e = cudaLaunchKernelEx(&cfg, is_bf16 ? token_logprobs_kernel<true> : token_logprobs_kernel<false>, p);
+  if (e != cudaSuccess) return cuda_fail(e, "token_logprobs_kernel launch");
+  return launch_check("token_logprobs_kernel launch");
 }
 
 int ks_device_status(void* stream) {

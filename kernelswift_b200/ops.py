@@ -19,6 +19,10 @@ These are the B200 counterparts of the reference's torch extension ops
   step) over that cache.
 * ``verify_draft``: drafted tokens accepted or rejected against the target's
   probabilities, from given random numbers.  The reference has none of the four.
+* ``kv_append``: keys and values per head (grouped queries) rotated and quantised into a
+  paged e4m3 cache with a scale for each block of tokens and head.
+* ``token_logprobs``: log probabilities of given tokens, entropy and the likeliest
+  alternatives, from logits.  The reference has neither.
 
 Every op runs on the current CUDA stream of its input's device, validates its
 arguments like the reference (a ``RuntimeError`` on a bad dtype, device, shape
@@ -631,6 +635,144 @@ def verify_draft(p: torch.Tensor, tokens: torch.Tensor, u: torch.Tensor, noise: 
                                     _ptr(parents), u.data_ptr(), noise.data_ptr(), B, T, V, out.data_ptr(),
                                     n_accepted.data_ptr(), path.data_ptr(), _stream(p)), "ks_verify_draft")
     return out, n_accepted, path
+
+
+def _kv_args(name, k8, k_scale, v8, v_scale, page_table, lens, n_new, B):
+    if k8.dtype not in _FP8 or v8.dtype not in _FP8 or k8.dim() != 4 or k8.shape != v8.shape:
+        raise RuntimeError(f"{name}: k8 and v8 must be float8_e4m3fn (or their uint8 bytes) [pages, heads, page, d]")
+    pages, heads, page, D = k8.shape
+    if k_scale.dtype != torch.float32 or v_scale.dtype != torch.float32 or k_scale.dim() != 3 or \
+            k_scale.shape != v_scale.shape or k_scale.shape[:2] != k8.shape[:2]:
+        raise RuntimeError(f"{name}: k_scale and v_scale must be float32 [pages, heads, page / block]")
+    per = k_scale.shape[2]
+    if pages < 1 or heads < 1 or per < 1 or page < 1 or page % per:
+        raise RuntimeError(f"{name}: pages of {page} rows and {per} scales do not make blocks")
+    _table_args(name, page_table, lens, B)
+    ts = [k8, k_scale, v8, v_scale, page_table, lens]
+    if n_new is not None:
+        if n_new.dtype != torch.int32 or n_new.shape != (B,):
+            raise RuntimeError(f"{name}: n_new must be int32 [b]")
+        ts.append(n_new)
+    return pages, heads, page, page // per, D, ts
+
+
+def _rows_of_tokens(name, what, x, D):
+    """Elements from sequence to sequence and from token to token of [b, t, heads, D]."""
+    if x.dtype != torch.bfloat16 or x.dim() != 4 or x.shape[3] != D:
+        raise RuntimeError(f"{name}: {what} must be bfloat16 [b, t, heads, {D}]")
+    if x.numel() and (x.stride(3) != 1 or (x.shape[2] > 1 and x.stride(2) != D)):
+        raise RuntimeError(f"{name}: a token's rows of {what} must lie together")
+    B, T, H, _ = x.shape
+    # (the stride of a dimension of one element says nothing)
+    ts = x.stride(1) if T > 1 else H * D
+    return x.stride(0) if B > 1 else T * ts, ts
+
+
+def kv_append(k: torch.Tensor, v: torch.Tensor, k8: torch.Tensor, k_scale: torch.Tensor,
+              v8: torch.Tensor, v_scale: torch.Tensor, page_table: torch.Tensor, lens: torch.Tensor,
+              freqs: torch.Tensor | None = None, positions: torch.Tensor | None = None,
+              n_new: torch.Tensor | None = None, q: torch.Tensor | None = None
+              ) -> torch.Tensor | None:
+    """Append T tokens' keys and values to a paged per-head cache in 8 bits (in place), keys
+    rotated on the way.
+
+    k, v bf16 [B,T,heads,D] (a token's rows together, e.g. column slices of one
+    projection): token t of sequence b goes to position lens[b] + t, if t < n_new[b]
+    (int32 [B]; None: T).  freqs fp32 [P, rope_dim/2, 2] (cos, sin) rotates the last
+    rope_dim columns of a key, as pairs (2i, 2i+1), by row ``positions[b, t]`` (int32 [B,T];
+    None: lens[b] + t; a drafted tree's tokens have their depths'), before it is rounded.
+    With ``q`` bf16 [B,T,H,D] the queries are rotated too: returns them, bf16 [B,T,H,D] (q
+    itself without freqs), else None.
+
+    k8, v8 float8_e4m3fn [pages, heads, page, D], k_scale, v_scale fp32 [pages, heads, page /
+    block]; page_table int32 [B, max_pages]; D 64, 128, 192 or 256, block a multiple of 16 up to
+    128.  One power-of-two scale per block of tokens and head, the smallest that takes the
+    largest element (at most 448 scales); where a block holds tokens already its scale only grows, and they are rounded
+    again to it.  An element that is NaN or infinite reads as NaN, and the lowest bit of its
+    block's scale is set.  lens is not changed: add n_new to it after the last layer."""
+    if k.dim() != 4:
+        raise RuntimeError("kv_append: k must be bfloat16 [b, t, heads, d]")
+    B, T = k.shape[:2]
+    pages, heads, page, block, D, ts = _kv_args("kv_append", k8, k_scale, v8, v_scale, page_table, lens, n_new, B)
+    k_bs, k_ts = _rows_of_tokens("kv_append", "k", k, D)
+    v_bs, v_ts = _rows_of_tokens("kv_append", "v", v, D)
+    if k.shape[2] != heads or v.shape != k.shape:
+        raise RuntimeError(f"kv_append: k and v must be [b, t, {heads}, {D}]")
+    dev, rows = k8.device, [k, v]
+    H = q_bs = q_ts = rope_dim = n_freqs = 0
+    if freqs is not None:
+        if freqs.dtype != torch.float32 or freqs.dim() != 3 or freqs.shape[2] != 2:
+            raise RuntimeError("kv_append: freqs must be float32 [p, rope_dim / 2, 2]")
+        n_freqs, rope_dim = freqs.shape[0], 2 * freqs.shape[1]
+        ts.append(freqs)
+    if positions is not None:
+        if positions.dtype != torch.int32 or positions.shape != (B, T):
+            raise RuntimeError("kv_append: positions must be int32 [b, t]")
+        ts.append(positions)
+    if q is not None:
+        q_bs, q_ts = _rows_of_tokens("kv_append", "q", q, D)
+        H = q.shape[2]
+        if q.shape[:2] != k.shape[:2] or H < 1:
+            raise RuntimeError("kv_append: q must have the tokens of k")
+        rows.append(q)
+    _require_cuda("kv_append", *ts)
+    for x in rows:
+        if x.device != dev:
+            raise RuntimeError("kv_append: inputs must be on one device")
+    turn = q is not None and rope_dim > 0
+    q_out = torch.empty(B, T, H, D, dtype=torch.bfloat16, device=dev) if turn else q
+    with _on(k8):
+        check(lib().ks_kv_append(k.data_ptr(), k_bs, k_ts, v.data_ptr(), v_bs, v_ts,
+                                 q.data_ptr() if turn else None, q_bs, q_ts, H, q_out.data_ptr() if turn else None,
+                                 _ptr(freqs), n_freqs, rope_dim, _ptr(positions), k8.data_ptr(),
+                                 k_scale.data_ptr(), v8.data_ptr(), v_scale.data_ptr(), pages, heads, page, block,
+                                 D, page_table.data_ptr(), page_table.shape[1], lens.data_ptr(), _ptr(n_new), B, T,
+                                 _stream(k8)), "ks_kv_append")
+    return q_out
+
+
+def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0
+                   ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor | None, torch.Tensor | None]:
+    """Log probabilities of given tokens, the entropy of their distributions and the
+    ``top`` likeliest alternatives.
+
+    logits bf16 or fp32 [..., V] (rows contiguous and a constant number of elements apart, e.g.
+    the first V columns of a padded vocabulary), tokens int32 / int64 [...].  Returns (logp
+    fp32 [...], entropy fp32 [...] in nats, top_logp fp32 [..., top], top_ids [..., top] like
+    tokens; the last two None without top): the largest first, the lowest index first
+    among equal ones; top at most 32.  A negative token (``verify_draft``'s padding) has
+    logp 0.  Sums are in fp32.  A row with a NaN, an infinite or no finite logit gets NaN."""
+    if logits.dtype not in (torch.bfloat16, torch.float32) or logits.dim() < 1:
+        raise RuntimeError("token_logprobs: logits must be bfloat16 or float32 [..., v]")
+    if tokens.dtype not in (torch.int32, torch.int64) or tokens.shape != logits.shape[:-1]:
+        raise RuntimeError("token_logprobs: tokens must be int32 or int64 [...], one per row of logits")
+    V, top = logits.shape[-1], int(top)
+    rows = logits
+    if logits.dim() != 2:
+        try:
+            rows = logits.view(-1, V) if V else logits
+        except RuntimeError:
+            raise RuntimeError("token_logprobs: the rows of logits must be a constant stride apart") from None
+    _require_cuda("token_logprobs", tokens)
+    if logits.device != tokens.device:
+        raise RuntimeError("token_logprobs: inputs must be on one device")
+    if rows.numel() and V > 1 and rows.stride(1) != 1:
+        raise RuntimeError("token_logprobs: the columns of logits must be contiguous")
+    N = tokens.numel()
+    ld = rows.stride(0) if N > 1 else V
+    logp = torch.empty(tokens.shape, dtype=torch.float32, device=tokens.device)
+    entropy = torch.empty_like(logp)
+    top_logp = top_ids = None
+    if top:
+        shape = tuple(tokens.shape) + (max(top, 0),)
+        top_logp = torch.empty(shape, dtype=torch.float32, device=tokens.device)
+        top_ids = torch.empty(shape, dtype=tokens.dtype, device=tokens.device)
+    with _on(tokens):
+        check(lib().ks_token_logprobs(rows.data_ptr(), int(logits.dtype == torch.bfloat16), ld, tokens.data_ptr(),
+                                      KS_INT64 if tokens.dtype == torch.int64 else KS_INT32, N, V, top,
+                                      logp.data_ptr(), entropy.data_ptr(), _ptr(top_logp), _ptr(top_ids),
+                                      _stream(tokens)), "ks_token_logprobs")
+    return logp, entropy, top_logp, top_ids
 
 
 def device_status(device: torch.device | int | None = None) -> None:
