@@ -359,6 +359,28 @@ int ks_kv_append(const void* k, int64_t k_bs, int64_t k_ts, const void* v, int64
                  const int32_t* n_new, int64_t B, int64_t T, void* stream);
 
 /*
+ * Attention over the per-head cache that ks_kv_append fills (same layout and limits): decoding
+ * (T = 1), drafted tokens, a chunk of a prompt.
+ *   q, out bf16 [B, T, H, D], H a multiple of heads: query head h reads key head h / (H / heads)
+ *   lens, n_new: token t < n_new[b] (NULL: T) of sequence b sees the lens[b] cached positions and,
+ *          of the call's own tokens, cached at lens[b] .., those j < n_new[b] with mask[b, t, j]
+ *          (bytes [B, T, T]; NULL: j <= t); the others get zeros
+ *   attn_sink fp32 [H] or NULL: a logit per head that takes part in the softmax without a value
+ * Scores, sums and outputs are fp32, weights enter the product with the values in bf16, the
+ * result is rounded once.  A token that sees nothing gets zeros.  Positions past the table or
+ * on a page outside [0, n_pages) are not seen; both are reported by ks_device_status.
+ * workspace: ks_kv_attn_workspace_size bytes, 256-byte aligned, used by this call alone until it
+ * is done.  No counterpart in the reference.
+ */
+size_t ks_kv_attn_workspace_size(int64_t T, int64_t H, int64_t heads, int64_t D);
+int ks_kv_attn(const void* q, const void* k8, const float* k_scale, const void* v8,
+               const float* v_scale, int64_t n_pages, int32_t heads, int32_t page, int32_t block,
+               int32_t D, const int32_t* page_table, int64_t max_pages, const int32_t* lens,
+               const int32_t* n_new, const uint8_t* mask, const float* attn_sink, void* out,
+               int64_t B, int64_t T, int64_t H, float softmax_scale, void* workspace,
+               size_t workspace_bytes, void* stream);
+
+/*
  * Log probabilities of given tokens from logits [N, V] (rows ld elements apart, bf16 where
  * is_bf16, else fp32): logp fp32 [N] = x[token] - logsumexp(x), entropy fp32 [N] (nats), and the
  * top (<= 32, <= V) largest as top_logp fp32 [N, top], top_ids [N, top] (type of tokens), largest

@@ -69,6 +69,10 @@ SIGNATURES = {
     "ks_kv_append": (ctypes.c_int, [_vp, _c_i64, _c_i64, _vp, _c_i64, _c_i64, _vp, _c_i64, _c_i64, _c_i32,
                                     _vp, _vp, _c_i64, _c_i32, _vp, _vp, _vp, _vp, _vp, _c_i64, _c_i32,
                                     _c_i32, _c_i32, _c_i32, _vp, _c_i64, _vp, _vp, _c_i64, _c_i64, _vp]),
+    "ks_kv_attn_workspace_size": (_sz, [_c_i64, _c_i64, _c_i64, _c_i64]),
+    "ks_kv_attn": (ctypes.c_int, [_vp, _vp, _vp, _vp, _vp, _c_i64, _c_i32, _c_i32, _c_i32, _c_i32, _vp,
+                                  _c_i64, _vp, _vp, _vp, _vp, _vp, _c_i64, _c_i64, _c_i64, _c_f32, _vp,
+                                  _sz, _vp]),
     "ks_token_logprobs": (ctypes.c_int, [_vp, _c_i32, _c_i64, _vp, _c_i32, _c_i64, _c_i64, _c_i32, _vp,
                                          _vp, _vp, _vp, _vp]),
     "ks_device_status": (ctypes.c_int, [_vp]),

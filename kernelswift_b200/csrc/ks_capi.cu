@@ -14,6 +14,7 @@
 #include "ks_b200.h"
 #include "ks_device.cuh"
 #include "indexer_score.cuh"
+#include "kv_attn.cuh"
 #include "kv_cache.cuh"
 #include "latent_cache.cuh"
 #include "proj_gemm.cuh"
@@ -622,6 +623,23 @@ int kv_cache_check(const char* op, KvCache* c, void* k8, float* k_scale, void* v
   return KS_OK;
 }
 
+// Rows of a row tile of kv_attn: a sequence's T * G rows of a key head.
+int kva_rows(int64_t rows, int64_t D) { return rows <= 8 || D > 128 ? 8 : 16; }
+constexpr int KVA_MAX_CTAS = 296;  // two per SM of a B200: bounds the workspace
+
+int log2_of(int x) {  // -1: not a power of two
+  int s = 0;
+  while ((1 << s) < x) ++s;
+  return (1 << s) == x ? s : -1;
+}
+
+template <int D, int NT>
+int launch_kv_attn_few(Device* dev, const KvAttnParams& p, unsigned grid, cudaStream_t st) {
+  if (int rc = smem_optin(dev, reinterpret_cast<const void*>(kv_attn_few_kernel<D, NT>), "cudaFuncSetAttribute(kv_attn)")) return rc;
+  kv_attn_few_kernel<D, NT><<<grid, KVF_WARPS * 32, KVF_HDR + 4 * 8 * NT * D * sizeof(float), st>>>(p);
+  return launch_check("kv_attn_few_kernel launch");
+}
+
 // Rows of a row tile for a sequence's T * H query rows: 32 fill the tensor memory; 16 rows
 // take fewer columns of every product where there are no more.
 int ta_rows(int64_t rows) { return rows <= 16 ? 16 : 32; }
@@ -1219,6 +1237,65 @@ int ks_kv_append(const void* k, int64_t k_bs, int64_t k_ts, const void* v, int64
   else if (pieces <= 512) kv_append_kernel<4><<<grid, threads, 0, st>>>(p);
   else kv_append_kernel<8><<<grid, threads, 0, st>>>(p);
   return launch_check("kv_append_kernel launch");
+}
+
+size_t ks_kv_attn_workspace_size(int64_t T, int64_t H, int64_t heads, int64_t D) {
+  if (T < 1 || H < 1 || heads < 1 || H % heads || D < 1) return 256;
+  // two parts of a row tile per CTA: outputs, references and sums; and the CTA's owner record
+  const int64_t nr = kva_rows(T * (H / heads), D);
+  return (size_t)round_up(KVA_MAX_CTAS * (2 * nr * (D + 2) * 4 + 16), 256);
+}
+
+int ks_kv_attn(const void* q, const void* k8, const float* k_scale, const void* v8,
+               const float* v_scale, int64_t n_pages, int32_t heads, int32_t page, int32_t block,
+               int32_t D, const int32_t* page_table, int64_t max_pages, const int32_t* lens,
+               const int32_t* n_new, const uint8_t* mask, const float* attn_sink, void* out,
+               int64_t B, int64_t T, int64_t H, float softmax_scale, void* workspace,
+               size_t workspace_bytes, void* stream) {
+  Device* dev;
+  if (int rc = device(&dev)) return rc;
+  if (B < 0 || T < 0 || H < 1) return fail(KS_ERR_INVALID, "kv_attn: bad sizes B=%lld T=%lld H=%lld", (long long)B, (long long)T, (long long)H);
+  if (B == 0 || T == 0) return KS_OK;
+  KvAttnParams p{};
+  if (int rc = kv_cache_check("kv_attn", &p.c, const_cast<void*>(k8), const_cast<float*>(k_scale), const_cast<void*>(v8), const_cast<float*>(v_scale), n_pages, heads, page, block, D, page_table, max_pages, lens, n_new, B, T)) return rc;
+  if (!q || !out) return fail(KS_ERR_INVALID, "kv_attn: null pointer");
+  if (H % heads) return fail(KS_ERR_INVALID, "kv_attn: H=%lld is not a multiple of the %d key heads", (long long)H, heads);
+  if (H > 65536 || T * (H / heads) >= (1ll << 30)) return fail(KS_ERR_UNSUPPORTED, "kv_attn: too many rows");
+  if (!aligned(q, 16) || !aligned(out, 16) || !aligned(attn_sink, 4))
+    return fail(KS_ERR_ALIGNMENT, "kv_attn: q, out must be 16-byte aligned");
+  const size_t need = ks_kv_attn_workspace_size(T, H, heads, D);
+  if (!workspace || workspace_bytes < need) return fail(KS_ERR_WORKSPACE, "kv_attn: workspace of %zu bytes needed", need);
+  if (!aligned(workspace, 256)) return fail(KS_ERR_ALIGNMENT, "kv_attn: workspace must be 256-byte aligned");
+  p.c.status = dev->status;
+  p.q = static_cast<const uint16_t*>(q);
+  p.out = static_cast<uint16_t*>(out);
+  p.mask = mask;
+  p.sink = attn_sink;
+  p.H = (int)H;
+  p.G = (int)(H / heads);
+  p.rows = (int)(T * p.G);
+  p.nr = kva_rows(p.rows, D);
+  p.row_tiles = (p.rows + p.nr - 1) / p.nr;
+  p.page_shift = log2_of(page);
+  p.block_shift = log2_of(block);
+  p.scale_log2 = softmax_scale * 1.4426950408889634f;
+  // no more CTAs than there can be units (the lengths are known on the device only)
+  const int per_sm = D * p.nr <= 1024 ? 2 : 1;
+  const int64_t most = B * p.row_tiles * heads * (KVA_SETUP + (max_pages * page + 127) / 128);
+  const unsigned grid = (unsigned)std::min<int64_t>({most, (int64_t)dev->num_sms * per_sm, (int64_t)KVA_MAX_CTAS});
+  p.part_o = static_cast<float*>(workspace);
+  p.part_ml = reinterpret_cast<float2*>(p.part_o + 2ll * grid * p.nr * D);
+  p.owner = reinterpret_cast<int4*>(p.part_ml + 2ll * grid * p.nr);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const bool two = p.nr == 16;
+  if (int rc = D == 64    ? (two ? launch_kv_attn_few<64, 2>(dev, p, grid, st) : launch_kv_attn_few<64, 1>(dev, p, grid, st))
+               : D == 128 ? (two ? launch_kv_attn_few<128, 2>(dev, p, grid, st) : launch_kv_attn_few<128, 1>(dev, p, grid, st))
+               : D == 192 ? launch_kv_attn_few<192, 1>(dev, p, grid, st)
+                          : launch_kv_attn_few<256, 1>(dev, p, grid, st))
+    return rc;
+  const int at_once = 256 / (D / 4);
+  kv_attn_join_kernel<<<dim3(grid, (unsigned)((p.nr + at_once - 1) / at_once)), 256, 0, st>>>(p);
+  return launch_check("kv_attn_join_kernel launch");
 }
 
 int ks_token_logprobs(const void* logits, int32_t is_bf16, int64_t ld, const void* tokens,

@@ -21,8 +21,10 @@ These are the B200 counterparts of the reference's torch extension ops
   probabilities, from given random numbers.  The reference has none of the four.
 * ``kv_append``: keys and values per head (grouped queries) rotated and quantised into a
   paged e4m3 cache with a scale for each block of tokens and head.
+* ``kv_attn``: attention over that cache, from one token, a drafted tree or a chunk of a
+  prompt.
 * ``token_logprobs``: log probabilities of given tokens, entropy and the likeliest
-  alternatives, from logits.  The reference has neither.
+  alternatives, from logits.  The reference has none of the three.
 
 Every op runs on the current CUDA stream of its input's device, validates its
 arguments like the reference (a ``RuntimeError`` on a bad dtype, device, shape
@@ -729,6 +731,61 @@ def kv_append(k: torch.Tensor, v: torch.Tensor, k8: torch.Tensor, k_scale: torch
                                  D, page_table.data_ptr(), page_table.shape[1], lens.data_ptr(), _ptr(n_new), B, T,
                                  _stream(k8)), "ks_kv_append")
     return q_out
+
+
+@functools.lru_cache(maxsize=256)
+def kv_attn_workspace_size(T: int, H: int, heads: int, D: int) -> int:
+    return int(lib().ks_kv_attn_workspace_size(T, H, heads, D))
+
+
+def kv_attn(q: torch.Tensor, k8: torch.Tensor, k_scale: torch.Tensor, v8: torch.Tensor,
+            v_scale: torch.Tensor, page_table: torch.Tensor, lens: torch.Tensor, softmax_scale: float,
+            mask: torch.Tensor | None = None, attn_sink: torch.Tensor | None = None,
+            n_new: torch.Tensor | None = None, out: torch.Tensor | None = None,
+            workspace: torch.Tensor | None = None) -> torch.Tensor:
+    """Attention of T new tokens per sequence over the per-head cache that ``kv_append``
+    fills: T = 1 is a decoding step, a larger T drafted tokens or a chunk of a prompt.
+
+    q bf16 [B,T,H,D], H a multiple of the cache's heads (grouped queries: head h reads key
+    head h // (H // heads)); the cache, page_table and lens as for ``kv_append``, whose T
+    tokens are cached at lens[b] .. already.  Token t sees the lens[b] positions before and
+    of the new ones those with ``mask[b, t, j]`` (bool [B,T,T]; None: j <= t).  With n_new
+    (int32 [B]) sequence b has n_new[b] of the T tokens; the rows of the others are zeros.
+    attn_sink fp32 [H] as in ``sparse_attn``.  Returns bf16 [B,T,H,D]; a token that sees
+    nothing gets zeros.  Weights enter their product in bf16 (2^-8 of themselves), scores
+    and sums are fp32, the result is rounded once."""
+    if q.dtype != torch.bfloat16 or q.dim() != 4:
+        raise RuntimeError("kv_attn: q must be bfloat16 [b, t, h, d]")
+    B, T, H, _ = q.shape
+    pages, heads, page, block, D, ts = _kv_args("kv_attn", k8, k_scale, v8, v_scale, page_table, lens, n_new, B)
+    if q.shape[3] != D or H % heads or H < 1:
+        raise RuntimeError(f"kv_attn: q must be [b, t, h, {D}], h a multiple of {heads}")
+    ts.append(q)
+    if mask is not None:
+        if mask.dtype not in (torch.bool, torch.uint8) or mask.shape != (B, T, T):
+            raise RuntimeError("kv_attn: mask must be bool [b, t, t]")
+        ts.append(mask)
+    if attn_sink is not None:
+        if attn_sink.dtype != torch.float32 or attn_sink.shape != (H,):
+            raise RuntimeError("kv_attn: attn_sink must be float32 [h]")
+        ts.append(attn_sink)
+    _require_cuda("kv_attn", *ts)
+    if out is None:
+        out = torch.empty(B, T, H, D, dtype=torch.bfloat16, device=q.device)
+    else:
+        _check_out("kv_attn", out, (B, T, H, D), torch.bfloat16, q.device)
+    need = kv_attn_workspace_size(T, H, heads, D)
+    if workspace is None:
+        workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
+    else:
+        _check_workspace("kv_attn", workspace, need, q.device)
+    with _on(q):
+        check(lib().ks_kv_attn(q.data_ptr(), k8.data_ptr(), k_scale.data_ptr(), v8.data_ptr(), v_scale.data_ptr(),
+                               pages, heads, page, block, D, page_table.data_ptr(), page_table.shape[1],
+                               lens.data_ptr(), _ptr(n_new), _ptr(mask), _ptr(attn_sink), out.data_ptr(), B, T, H,
+                               float(softmax_scale), workspace.data_ptr(),
+                               workspace.numel() * workspace.element_size(), _stream(q)), "ks_kv_attn")
+    return out
 
 
 def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0

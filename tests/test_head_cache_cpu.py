@@ -46,6 +46,26 @@ def test_append_refuses(change, why):
         ops.kv_append(**{**append_args(), **change})
 
 
+@pytest.mark.parametrize("change,why", [
+    (dict(q=torch.zeros(1, 3, 4, 64)), "q must be bfloat16"),
+    (dict(q=torch.zeros(1, 3, 3, 64, dtype=torch.bfloat16)), "multiple of 2"),
+    (dict(q=torch.zeros(1, 3, 4, 128, dtype=torch.bfloat16)), r"q must be \[b, t, h, 64\]"),
+    (dict(mask=torch.zeros(1, 3, 4, dtype=torch.bool)), "mask"),
+    (dict(mask=torch.zeros(1, 3, 3)), "mask"),
+    (dict(attn_sink=torch.zeros(2)), "attn_sink"),
+    (dict(n_new=torch.zeros(2, dtype=torch.int32)), "n_new"),
+    (dict(lens=torch.zeros(1)), "lens"),
+    (dict(v_scale=torch.zeros(4, 2, 4)), "k_scale and v_scale"),
+    (dict(), "CUDA"),
+])
+def test_attention_refuses(change, why):
+    args = append_args()
+    del args["k"], args["v"]
+    args["q"] = torch.zeros(1, 3, 4, 64, dtype=torch.bfloat16)
+    with pytest.raises(RuntimeError, match=why):
+        ops.kv_attn(**{**args, "softmax_scale": 0.1, **change})
+
+
 @pytest.mark.parametrize("logits,tokens,why", [
     (torch.zeros(2, 5).half(), torch.zeros(2, dtype=torch.int64), "logits must be"),
     (torch.zeros(2, 5), torch.zeros(3, dtype=torch.int64), "one per row"),
