@@ -15,6 +15,7 @@
 #include "ks_device.cuh"
 #include "indexer_score.cuh"
 #include "kv_attn.cuh"
+#include "kv_attn_wide.cuh"
 #include "kv_cache.cuh"
 #include "latent_cache.cuh"
 #include "proj_gemm.cuh"
@@ -623,8 +624,13 @@ int kv_cache_check(const char* op, KvCache* c, void* k8, float* k_scale, void* v
   return KS_OK;
 }
 
-// Rows of a row tile of kv_attn: a sequence's T * G rows of a key head.
-int kva_rows(int64_t rows, int64_t D) { return rows <= 8 || D > 128 ? 8 : 16; }
+// Rows of a row tile of kv_attn: a sequence's T * G rows of a key head.  Up to 16 (8 for heads of
+// more than 128 columns) go to the kernel for few rows, whose registers hold no more.
+int kva_rows(int64_t rows, int64_t D) {
+  if (rows <= 8) return 8;
+  if (D > 128) return 128;
+  return rows <= 16 ? 16 : rows <= 128 ? 128 : 256;
+}
 constexpr int KVA_MAX_CTAS = 296;  // two per SM of a B200: bounds the workspace
 
 int log2_of(int x) {  // -1: not a power of two
@@ -638,6 +644,14 @@ int launch_kv_attn_few(Device* dev, const KvAttnParams& p, unsigned grid, cudaSt
   if (int rc = smem_optin(dev, reinterpret_cast<const void*>(kv_attn_few_kernel<D, NT>), "cudaFuncSetAttribute(kv_attn)")) return rc;
   kv_attn_few_kernel<D, NT><<<grid, KVF_WARPS * 32, KVF_HDR + 4 * 8 * NT * D * sizeof(float), st>>>(p);
   return launch_check("kv_attn_few_kernel launch");
+}
+
+template <int D>
+int launch_kv_attn_wide(Device* dev, const KvAttnParams& p, unsigned grid, cudaStream_t st) {
+  if (int rc = smem_optin(dev, reinterpret_cast<const void*>(kv_attn_wide_kernel<D>), "cudaFuncSetAttribute(kv_attn)")) return rc;
+  const size_t smem = 1024 + KVW_HDR + (size_t)(KVW_STREAM_OUT<D> + kvw_units<D>()) * KVW_TILE<D>;
+  kv_attn_wide_kernel<D><<<grid, KVW_THREADS, smem, st>>>(p);
+  return launch_check("kv_attn_wide_kernel launch");
 }
 
 // Rows of a row tile for a sequence's T * H query rows: 32 fill the tensor memory; 16 rows
@@ -1243,7 +1257,7 @@ size_t ks_kv_attn_workspace_size(int64_t T, int64_t H, int64_t heads, int64_t D)
   if (T < 1 || H < 1 || heads < 1 || H % heads || D < 1) return 256;
   // two parts of a row tile per CTA: outputs, references and sums; and the CTA's owner record
   const int64_t nr = kva_rows(T * (H / heads), D);
-  return (size_t)round_up(KVA_MAX_CTAS * (2 * nr * (D + 2) * 4 + 16), 256);
+  return (size_t)round_up((nr >= 128 ? KVA_MAX_CTAS / 2 : KVA_MAX_CTAS) * (2 * nr * (D + 2) * 4 + 16), 256);
 }
 
 int ks_kv_attn(const void* q, const void* k8, const float* k_scale, const void* v8,
@@ -1280,21 +1294,27 @@ int ks_kv_attn(const void* q, const void* k8, const float* k_scale, const void* 
   p.block_shift = log2_of(block);
   p.scale_log2 = softmax_scale * 1.4426950408889634f;
   // no more CTAs than there can be units (the lengths are known on the device only)
+  const bool wide = p.nr >= 128;
   const int per_sm = D * p.nr <= 1024 ? 2 : 1;
+  p.budget_ns = wait_budget_ns();
   const int64_t most = B * p.row_tiles * heads * (KVA_SETUP + (max_pages * page + 127) / 128);
-  const unsigned grid = (unsigned)std::min<int64_t>({most, (int64_t)dev->num_sms * per_sm, (int64_t)KVA_MAX_CTAS});
+  const unsigned grid = (unsigned)std::min<int64_t>({most, (int64_t)dev->num_sms * per_sm, (int64_t)KVA_MAX_CTAS / 2 * per_sm});
   p.part_o = static_cast<float*>(workspace);
   p.part_ml = reinterpret_cast<float2*>(p.part_o + 2ll * grid * p.nr * D);
   p.owner = reinterpret_cast<int4*>(p.part_ml + 2ll * grid * p.nr);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const bool two = p.nr == 16;
-  if (int rc = D == 64    ? (two ? launch_kv_attn_few<64, 2>(dev, p, grid, st) : launch_kv_attn_few<64, 1>(dev, p, grid, st))
+  if (int rc = wide         ? (D == 64    ? launch_kv_attn_wide<64>(dev, p, grid, st)
+                               : D == 128 ? launch_kv_attn_wide<128>(dev, p, grid, st)
+                               : D == 192 ? launch_kv_attn_wide<192>(dev, p, grid, st)
+                                          : launch_kv_attn_wide<256>(dev, p, grid, st))
+               : D == 64  ? (two ? launch_kv_attn_few<64, 2>(dev, p, grid, st) : launch_kv_attn_few<64, 1>(dev, p, grid, st))
                : D == 128 ? (two ? launch_kv_attn_few<128, 2>(dev, p, grid, st) : launch_kv_attn_few<128, 1>(dev, p, grid, st))
                : D == 192 ? launch_kv_attn_few<192, 1>(dev, p, grid, st)
                           : launch_kv_attn_few<256, 1>(dev, p, grid, st))
     return rc;
   const int at_once = 256 / (D / 4);
-  kv_attn_join_kernel<<<dim3(grid, (unsigned)((p.nr + at_once - 1) / at_once)), 256, 0, st>>>(p);
+  kv_attn_join_kernel<<<dim3(grid, (unsigned)std::min(8, (p.nr + at_once - 1) / at_once)), 256, 0, st>>>(p);
   return launch_check("kv_attn_join_kernel launch");
 }
 

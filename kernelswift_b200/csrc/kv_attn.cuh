@@ -53,6 +53,7 @@ struct KvAttnParams {
   float* part_o;          // [2 * CTAs][nr][D]
   float2* part_ml;        // [2 * CTAs][nr]: reference, sum
   int4* owner;            // [CTAs]: sequence, row tile, key head, parts (0: none to join)
+  uint64_t budget_ns;
 };
 
 struct KvaFind {

@@ -163,6 +163,15 @@ def test_long_contexts_are_split_and_joined(cuda_ok, H, heads, T, n):
     check(q, parts, table, lens, 128 ** -0.5)
 
 
+@pytest.mark.parametrize("d", [64, 128, 192, 256])
+@pytest.mark.parametrize("B,T,H,heads,n", [(4, 100, 32, 2, 3000), (1, 64, 64, 1, 10000), (3, 5, 20, 1, 50000), (20, 11, 24, 3, 2500),
+                                           (2, 150, 6, 2, 1500)])
+def test_stretches_of_many_tiles(cuda_ok, d, B, T, H, heads, n):
+    """Every CTA walks several tiles of several row tiles, in every form of the kernels."""
+    g, q, parts, table, lens = make(B, T, H, heads, d, 64, 16, [n - i for i in range(B)], d + T)
+    check(q, parts, table, lens, d ** -0.5)
+
+
 @pytest.mark.parametrize("B,T", [(200, 1), (64, 9), (700, 1)])
 def test_many_ragged_sequences(cuda_ok, B, T):
     lens = [(i * 37) % 300 for i in range(B)]
