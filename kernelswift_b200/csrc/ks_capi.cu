@@ -610,6 +610,7 @@ int kv_cache_check(const char* op, KvCache* c, void* k8, float* k_scale, void* v
   if (block < 16 || block % 16 || block > KV_MAX_BLOCK || page % block)
     return fail(KS_ERR_UNSUPPORTED, "%s: page=%d block=%d (block a multiple of 16 up to %d, page of block)", op, page, block, KV_MAX_BLOCK);
   if (max_pages * page >= (1ll << 31)) return fail(KS_ERR_UNSUPPORTED, "%s: max_pages * page >= 2^31", op);
+  if (n_pages * heads * (page / 16) >= (1ll << 32)) return fail(KS_ERR_UNSUPPORTED, "%s: n_pages * heads * page >= 2^36", op);
   if (T > (1 << 24) || B * T >= (1ll << 31)) return fail(KS_ERR_UNSUPPORTED, "%s: too many tokens", op);
   if (!aligned(k8, 16) || !aligned(v8, 16) || !aligned(k_scale, 4) || !aligned(v_scale, 4) || !aligned(n_new, 4))
     return fail(KS_ERR_ALIGNMENT, "%s: k8, v8 must be 16-byte and the scales, n_new 4-byte aligned", op);
@@ -642,7 +643,8 @@ int log2_of(int x) {  // -1: not a power of two
 template <int D, int NT>
 int launch_kv_attn_few(Device* dev, const KvAttnParams& p, unsigned grid, cudaStream_t st) {
   if (int rc = smem_optin(dev, reinterpret_cast<const void*>(kv_attn_few_kernel<D, NT>), "cudaFuncSetAttribute(kv_attn)")) return rc;
-  kv_attn_few_kernel<D, NT><<<grid, KVF_WARPS * 32, KVF_HDR + 4 * 8 * NT * D * sizeof(float), st>>>(p);
+  const size_t ring = (size_t)KVF_WARPS * KVF_STAGES * 32 * D, outputs = (size_t)4 * 8 * NT * D * sizeof(float);
+  kv_attn_few_kernel<D, NT><<<grid, KVF_WARPS * 32, KVF_HDR + std::max(ring, outputs), st>>>(p);
   return launch_check("kv_attn_few_kernel launch");
 }
 
@@ -1313,8 +1315,18 @@ int ks_kv_attn(const void* q, const void* k8, const float* k_scale, const void* 
                : D == 192 ? launch_kv_attn_few<192, 1>(dev, p, grid, st)
                           : launch_kv_attn_few<256, 1>(dev, p, grid, st))
     return rc;
-  const int at_once = 256 / (D / 4);
-  kv_attn_join_kernel<<<dim3(grid, (unsigned)std::min(8, (p.nr + at_once - 1) / at_once)), 256, 0, st>>>(p);
+  // The join's launch overlaps the kernel before it, whose end it waits for itself.
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.gridDim = dim3(grid, (unsigned)std::min(8, p.nr));
+  cfg.blockDim = dim3(256);
+  cfg.stream = st;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  cudaError_t e = cudaLaunchKernelEx(&cfg, kv_attn_join_kernel, p);
+  if (e != cudaSuccess) return cuda_fail(e, "kv_attn_join_kernel launch");
   return launch_check("kv_attn_join_kernel launch");
 }
 

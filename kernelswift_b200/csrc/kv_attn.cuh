@@ -8,14 +8,20 @@
 // positions and, of the call's tokens (cached behind them), those its mask row allows, without
 // a mask the ones up to itself.
 //
-// Numbers.  A code times its block's scale, a power of two, is exact in bf16 (4 significant
-// bits), so keys and values enter bf16 products as they are; the code's bits are moved into
-// place and one multiplication by 2^120 * scale puts the exponent right (e4m3's small numbers
-// included).  Where that factor would pass bf16's range the rest of it goes to the scores and
-// the weights.  Weights are rounded to bf16 (off by at most 2^-8 of themselves, with a random
-// sign; the result is rounded to 2^-8 once more), everything else is fp32.  They are
-// taken relative to a reference that is raised when a score passes it by 2^KVA_RISE, and
-// 2^-KVA_DOWN smaller, so that sums of values at the top of the range stay finite.
+// Numbers.  Scores, sums and outputs are fp32; what is rounded to 16 bits are the weights, and
+// what a key or value holds is exact in either 16-bit type (4 significant bits).
+//   few rows: fp16 products on the codes themselves, converted by the hardware.  A query row
+//     enters times a power of two that brings its largest element below 2^15; elements 2^-30 of
+//     that and less go into further terms (rarely: then the scores take another pass).  Weights
+//     are off by at most 2^-11 of themselves, or 2^-32 of the reference's.  A chunk's scale
+//     multiplies its scores, and its part of the output when that is added up.
+//   many rows: a tile's output is added up in tensor memory, so scales have to be in the
+//     operands: bf16, the code's bits moved into place and one multiplication by 2^120 * scale to
+//     put the exponent right (e4m3's small numbers included).  Weights are rounded to bf16, off
+//     by at most 2^-8 of themselves, with a random sign; the result is rounded by as much.
+// Weights are taken relative to a reference that is raised when a score passes it by
+// 2^KVA_RISE, and 2^-KVA_DOWN smaller in outputs and sums, so that sums of values at the top of
+// the range stay finite.
 //
 // Work: a unit is a tile of 128 keys of one (sequence, row tile, key head); setting one up counts
 // as KVA_SETUP more.  The call's units in order are cut into equal stretches, one per CTA,
@@ -23,13 +29,16 @@
 // others share goes to the workspace (reference, sum, unnormalised output), and
 // kv_attn_join_kernel adds the parts up in order (no atomics).
 //
-// kv_attn_few_kernel: up to 16 rows.  Decoding is bound by reading the cache, and here it goes
-// from global memory to registers to the product: a warp takes 16 keys at a time, loads them
-// in the layout of mma.m16n8k16's operands (keys as M, rows as N: S^T = K Q^T, then O^T = V^T P^T),
-// and no shared memory and no barrier lies between.  8 warps of a CTA take a tile's 16-key
-// chunks in turn, each with references, sums and outputs of its own, joined once per row tile.
+// kv_attn_few_kernel: up to 16 rows.  Decoding is bound by reading the cache.  Every warp works on
+// its own: it takes 16 keys at a time (their codes are one stretch of memory), has those of two
+// more such chunks on their way into its ring in shared memory (cp.async; no barrier but the
+// warp's), and reads a chunk in the layout of mma.m16n8k16's operands, keys as M, rows as N:
+// S^T = K Q^T, then O^T = V^T P^T.  8 warps of a CTA take a tile's chunks in turn, each with
+// references, sums and outputs of its own, joined once per row tile.
 // A column of a product may come from any column of the head as long as both operands agree,
-// so a lane loads 16 contiguous bytes of a key's row; for V^T, 16 bytes of four keys.
+// and a row of it from any key: a lane reads 16 contiguous bytes of a key's row, for V^T 16 bytes
+// of four keys, and keys are assigned to the product's rows (kvf_key) so that neither read has
+// bank conflicts.
 #pragma once
 #include "kv_cache.cuh"
 
@@ -39,6 +48,8 @@ constexpr int KVA_SETUP = 2;      // units that a row tile costs beyond its tile
 constexpr float KVA_RISE = 8.f;   // how far a score may pass its reference (base 2)
 constexpr float KVA_DOWN = 24.f;  // weights are 2^-24: 2^(8 - 24) * 2^14 keys * 2^128 is finite
 constexpr int KVF_WARPS = 8;
+constexpr float KVF_TOP = 7.f;    // weights of the few-row kernel are 2^7 at the reference: below 2^16 in fp16
+constexpr int KVF_TERM = 30;      // exponents of a query row that one term holds
 
 struct KvAttnParams {
   KvCache c;
@@ -215,7 +226,7 @@ __device__ __forceinline__ float kva_norm(float m, float l, float sink_log2, boo
 // ------------------------------------------------------------------ few rows
 __device__ __forceinline__ void kvf_mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
@@ -224,15 +235,65 @@ __device__ __forceinline__ uint32_t kvf_trans(uint32_t x) {
   asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
   return y;
 }
+__device__ __forceinline__ uint32_t kvf_f16x2(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+// Codes 0, 1 and codes 2, 3 of a word as fp16 pairs.
+__device__ __forceinline__ void kvf_codes(uint32_t w, uint32_t& lo, uint32_t& hi) {
+  asm("{ .reg .b16 l, h; mov.b32 {l, h}, %2; cvt.rn.f16x2.e4m3x2 %0, l; cvt.rn.f16x2.e4m3x2 %1, h; }"
+      : "=r"(lo), "=r"(hi)
+      : "r"(w));
+}
+__device__ __forceinline__ float kvf_pow2(int e) { return __uint_as_float((uint32_t)(min(max(e, -126), 127) + 127) << 23); }
+
+// A query row's 16 columns from d on, as the second operand of four steps: those elements of
+// 2^sh times the row that are in [2^-15, 2^15), the first term's also above (infinite, NaN).
+__device__ __forceinline__ void kvf_query(const uint16_t* q, bool in, int sh, bool first, uint32_t (&b)[4][2]) {
+  uint4 x = make_uint4(0, 0, 0, 0), y = x;
+  if (in) {
+    x = __ldg(reinterpret_cast<const uint4*>(q));
+    y = __ldg(reinterpret_cast<const uint4*>(q + 8));
+  }
+  const uint32_t w[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+  const float f = kvf_pow2(sh);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    float lo = bf16lo_f32(w[i]) * f, hi = bf16hi_f32(w[i]) * f;
+    if (fabsf(lo) < 0x1p-15f || (!first && fabsf(lo) >= 0x1p15f)) lo = 0.f;
+    if (fabsf(hi) < 0x1p-15f || (!first && fabsf(hi) >= 0x1p15f)) hi = 0.f;
+    b[i >> 1][i & 1] = kvf_f16x2(lo, hi);
+  }
+}
+
 template <int W>
 __device__ __forceinline__ void kvf_load(uint32_t (&v)[W], const uint8_t* ptr) {
-  if constexpr (W == 4)
-    asm volatile("ld.global.nc.L1::no_allocate.v4.b32 {%0, %1, %2, %3}, [%4];"
-                 : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3])
-                 : "l"(ptr));
-  else
-    asm volatile("ld.global.nc.L1::no_allocate.v2.b32 {%0, %1}, [%2];" : "=r"(v[0]), "=r"(v[1]) : "l"(ptr));
+  asm volatile("ld.global.nc.L1::no_allocate.v4.b32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3])
+               : "l"(ptr));
 }
+template <int W>
+__device__ __forceinline__ void kvf_lds(uint32_t (&v)[W], uint32_t addr) {
+  if constexpr (W == 4)
+    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]) : "r"(addr));
+  else
+    asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(v[0]), "=r"(v[1]) : "r"(addr));
+}
+
+// Key (of 8, and of the 8 behind) that row i of a product stands for, and where 16-byte piece u
+// of a key's row lies in a chunk.  Of a quarter warp's lanes, two product rows and four
+// pieces meet in a read of keys, four product rows (every other one) and two pieces in one of
+// values: all eight in different banks.
+template <int D>
+__device__ __forceinline__ int kvf_key(int i) {
+  return (int)((D % 128 == 0 ? 0x37156240u : 0x67324510u) >> (4 * i)) & 7;
+}
+template <int D>
+__device__ __forceinline__ int kvf_at(int key, int u) {
+  return key * D + (D % 128 == 0 ? ((u & ~7) | ((u ^ key) & 7)) : (u ^ (key & 2))) * 16;
+}
+constexpr int KVF_STAGES = 3;
 
 constexpr int KVF_HDR = 2048;
 template <int NR>
@@ -242,17 +303,11 @@ struct KvfShared {
 };
 static_assert(sizeof(KvfShared<16>) <= KVF_HDR, "KvfShared exceeds its header");
 
-// Where 16 keys lie.
+// Scales (bits) of a chunk; ks = KVF_GONE: the page is not there.
 struct KvfChunk {
-  int64_t row;      // of the page pool's rows of heads
-  uint32_t ks, vs;  // bits of the scales, 0: the page is not there
+  uint32_t ks, vs;
 };
-
-template <int D>
-__device__ __forceinline__ int kvf_page(const KvAttnParams& p, int b, int pos, int keys) {
-  const int pi = kva_div(pos, p.c.page, p.page_shift);
-  return pos < keys ? __ldg(p.c.table + (int64_t)b * p.c.max_pages + pi) : 0;
-}
+constexpr uint32_t KVF_GONE = 0xFFFFFFFFu;
 
 // D: columns of a head, NT: 8-row groups.
 template <int D, int NT>
@@ -265,13 +320,17 @@ __global__ void __launch_bounds__(KVF_WARPS * 32, D * NT <= 128 ? 2 : 1) kv_attn
   KvaFind& find = sh.find;
   auto& sm_m = sh.m;
   auto& sm_l = sh.l;
-  float* kvf_smem = reinterpret_cast<float*>(kvf_raw + KVF_HDR);  // [4][NR][D] outputs of four warps
+  float* kvf_smem = reinterpret_cast<float*>(kvf_raw + KVF_HDR);  // [4][NR][D] outputs of four warps, at the end
+  // a warp's ring: [stages][keys, values][16 keys x D]
+  const uint32_t ring = smem_u32(kvf_raw + KVF_HDR) + (threadIdx.x >> 5) * (KVF_STAGES * 32 * D);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, r = lane >> 2, c = lane & 3;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the join may be set up
   kva_find(p, &find);
   KvaWalk w;
   w.start(p, &find);
   if (tid == 0) p.owner[blockIdx.x] = make_int4(0, 0, 0, 0);
   const int per_page = p.c.page / p.c.block;
+  const int key_r = kvf_key<D>(r), key_v[2] = {kvf_key<D>(2 * c), kvf_key<D>(2 * c + 1)};
 
   for (; w.left > 0; w.next(p)) {
     const int r0 = w.rt * NR;
@@ -289,63 +348,89 @@ __global__ void __launch_bounds__(KVF_WARPS * 32, D * NT <= 128 ? 2 : 1) kv_attn
     const int chunks = min(w.t1 * 8, (w.keys + 15) >> 4);
 
     int ci = w.t0 * 8 + warp;
-    auto locate = [&](int pos, int pg, KvfChunk* k) {
-      const int in = pos - kva_div(pos, p.c.page, p.page_shift) * p.c.page;
-      const bool ok = pg >= 0 && pg < p.c.n_pages;
-      if (!ok && lane == 0) report_bounds(p.c.status, w.b, (int)p.c.n_pages);
-      const int64_t unit = (int64_t)(ok ? pg : 0) * p.c.heads + w.h;
-      k->row = unit * p.c.page + in;
-      const int64_t si = unit * per_page + kva_div(in, p.c.block, p.block_shift);
-      k->ks = __float_as_uint(__ldg(p.c.k_scale + si));
-      k->vs = __float_as_uint(__ldg(p.c.v_scale + si));
-      if (!ok) k->ks = 0xFFFFFFFFu;
+    // Lane l knows where the l-th chunk from here is and its scales, for 32 chunks at a time.
+    // (A chunk's rows lie at 16 D times its place; places fit 32 bits.)
+    uint32_t place = 0, ks32 = KVF_GONE, vs32 = 0;
+    const auto locate = [&](int first) {
+      const int pos = (first + KVF_WARPS * lane) * 16;
+      if (pos < chunks * 16) {
+        const int pi = kva_div(pos, p.c.page, p.page_shift), in = pos - pi * p.c.page;
+        const int pg = __ldg(p.c.table + (int64_t)w.b * p.c.max_pages + pi);
+        const bool ok = pg >= 0 && pg < p.c.n_pages;
+        if (!ok) report_bounds(p.c.status, w.b, (int)p.c.n_pages);
+        const int64_t unit = (int64_t)(ok ? pg : 0) * p.c.heads + w.h;
+        const int64_t si = unit * per_page + kva_div(in, p.c.block, p.block_shift);
+        place = (uint32_t)(unit * (p.c.page >> 4) + (in >> 4));
+        ks32 = ok ? __float_as_uint(__ldg(p.c.k_scale + si)) : KVF_GONE;
+        vs32 = __float_as_uint(__ldg(p.c.v_scale + si));
+      }
     };
-    uint32_t kr[2][KJ][4], vr[4][VU][VW];
-    auto load_k = [&](const KvfChunk& k) {
-      const uint8_t* base = p.c.k8 + (k.row + r) * D + c * 16;
+    // starts the copies of the n-th chunk from the first
+    const auto fetch = [&](int n, int stage, KvfChunk* k) {
+      const uint32_t at16 = __shfl_sync(0xFFFFFFFFu, place, n & 31);
+      k->ks = __shfl_sync(0xFFFFFFFFu, ks32, n & 31);
+      k->vs = __shfl_sync(0xFFFFFFFFu, vs32, n & 31);
+      const int64_t at = (int64_t)at16 * (16 * D) + lane * 16;
+      const uint8_t *ksrc = p.c.k8 + at, *vsrc = p.c.v8 + at;
+      const uint32_t dst = ring + stage * (32 * D);
 #pragma unroll
-      for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int j = 0; j < KJ; ++j) kvf_load<4>(kr[i][j], base + i * 8 * D + j * 64);
+      for (int i = 0; i < D / 32; ++i) {
+        const int e = lane + 32 * i, key = e / (D / 16), u = e - key * (D / 16);
+        const uint32_t to = dst + kvf_at<D>(key, u);
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(ksrc + 512 * i) : "memory");
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to + 16 * D), "l"(vsrc + 512 * i) : "memory");
+      }
     };
-    auto load_v = [&](const KvfChunk& k) {
-      const uint8_t* base = p.c.v8 + (k.row + 2 * c) * D + r * (4 * VW);
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < VU; ++j) kvf_load<VW>(vr[i][j], base + ((i & 1) + (i >> 1) * 8) * D + j * (32 * VW));
+    KvfChunk cur{}, n1{}, n2{};
+    int stage = 0, n_fetched = 2;
+    locate(ci);
+    if (ci < chunks) fetch(0, 0, &cur);
+    asm volatile("cp.async.commit_group;" ::: "memory");
+    if (ci + KVF_WARPS < chunks) fetch(1, 1, &n1);
+    asm volatile("cp.async.commit_group;" ::: "memory");
+    // queries as the second operand: piece j of a lane holds columns 16 (c + 4 j) ..
+    uint32_t qf[NT][KJ][4][2];
+    int sh[NT];            // exponents that the lane's rows were moved by
+    float qsc[NT][2];      // of the lane's score columns: softmax scale, back by as much
+    int terms = 1;
+    const auto query_row = [&](int g) {
+      const int row = min(r0 + g * 8 + r, p.rows - 1), t = row / p.G;
+      return p.q + (((int64_t)w.b * p.c.T + t) * p.H + w.h * p.G + (row - t * p.G)) * D + 16 * c;
     };
-
-    KvfChunk cur{}, nxt{};
-    int pg1 = 0;
-    if (ci < chunks) {
-      const int pg0 = kvf_page<D>(p, w.b, ci * 16, w.keys);
-      pg1 = kvf_page<D>(p, w.b, (ci + KVF_WARPS) * 16, chunks * 16);
-      locate(ci * 16, pg0, &cur);
-      load_k(cur);
-      load_v(cur);
-    }
-    // queries as the second operand: word i of piece j holds columns 16 (c + 4 j) + 4 i ..
-    uint32_t qf[NT][KJ * 4][2];
 #pragma unroll
     for (int g = 0; g < NT; ++g) {
-      const int row = r0 + g * 8 + r, t = row / p.G;
-      const uint16_t* qp = p.q + (((int64_t)w.b * p.c.T + t) * p.H + w.h * p.G + (row - t * p.G)) * D;
+      const uint16_t* qp = query_row(g);
+      const bool in = r0 + g * 8 + r < p.rows;
+      // exponents of the largest and the least element (bits of |x|, zeros left out)
+      uint32_t most = 0, least = 0x7F80u;
 #pragma unroll
       for (int j = 0; j < KJ; ++j) {
-        uint4 a = make_uint4(0, 0, 0, 0), b = a;
-        if (row < p.rows) {
-          a = __ldg(reinterpret_cast<const uint4*>(qp + 16 * (c + 4 * j)));
-          b = __ldg(reinterpret_cast<const uint4*>(qp + 16 * (c + 4 * j) + 8));
-        }
-        const uint32_t x[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+        const uint4 x = __ldg(reinterpret_cast<const uint4*>(qp + 64 * j)), y = __ldg(reinterpret_cast<const uint4*>(qp + 64 * j + 8));
+        const uint32_t e[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {  // codes 0 and 2 of a word go together, and 1 and 3
-          qf[g][j * 4 + i][0] = __byte_perm(x[2 * i], x[2 * i + 1], 0x5410);
-          qf[g][j * 4 + i][1] = __byte_perm(x[2 * i], x[2 * i + 1], 0x7632);
+        for (int i = 0; i < 8; ++i) {
+          const uint32_t lo = e[i] & 0x7FFFu, hi = (e[i] >> 16) & 0x7FFFu;
+          most = max(most, max(lo, hi));
+          least = min(least, min(lo ? lo : 0x7F80u, hi ? hi : 0x7F80u));
         }
       }
+#pragma unroll
+      for (int x = 1; x < 4; x <<= 1) {
+        most = max(most, __shfl_xor_sync(0xFFFFFFFFu, most, x));
+        least = min(least, __shfl_xor_sync(0xFFFFFFFFu, least, x));
+      }
+      const int top = (int)(most >> 7) - 127, low = (int)(least >> 7) - 127;
+      sh[g] = min(14 - top, 126);
+      if (in && most < 0x7F80u && low < top) terms = max(terms, (top - low) / KVF_TERM + 1);
+#pragma unroll
+      for (int j = 0; j < KJ; ++j) kvf_query(qp + 64 * j, in, sh[g], true, qf[g][j]);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int back = -__shfl_sync(0xFFFFFFFFu, sh[g], (2 * c + i) * 4);
+        qsc[g][i] = p.scale_log2 * kvf_pow2(back);
+      }
     }
+    terms = __reduce_max_sync(0xFFFFFFFFu, terms);
     float m[NT][2], mu[NT][2], l[NT][2], o[NT][D / 16][4];
     uint32_t nanv[NT][2];  // columns of the lane's outputs that are NaN
 #pragma unroll
@@ -353,7 +438,7 @@ __global__ void __launch_bounds__(KVF_WARPS * 32, D * NT <= 128 ? 2 : 1) kv_attn
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         m[g][i] = -INFINITY;
-        mu[g][i] = KVA_DOWN;
+        mu[g][i] = -KVF_TOP;
         l[g][i] = 0.f;
         nanv[g][i] = 0;
       }
@@ -365,56 +450,93 @@ __global__ void __launch_bounds__(KVF_WARPS * 32, D * NT <= 128 ? 2 : 1) kv_attn
 
     for (; ci < chunks; ci += KVF_WARPS) {
       const int pos = ci * 16;
-      // ---------------------------------------------------------- scores
-      float s[NT][4];
-#pragma unroll
-      for (int g = 0; g < NT; ++g) s[g][0] = s[g][1] = s[g][2] = s[g][3] = 0.f;
-      float rest_k, rest_v;
-      const bool there = cur.ks != 0xFFFFFFFFu;
-      const uint32_t fk = kva_factor(there ? cur.ks : 0u, &rest_k), fv = kva_factor(cur.vs, &rest_v);
-      const bool marked = there && ((cur.ks | cur.vs) & 1u);
-      uint32_t nan_k = 0;  // of the lane's two keys, bit 0 and 1
-      if (marked) {
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-#pragma unroll
-          for (int j = 0; j < KJ; ++j)
-#pragma unroll
-            for (int x = 0; x < 4; ++x) nan_k |= (kva_nan4(kr[i][j][x]) ? 1u : 0u) << i;
-        nan_k |= __shfl_xor_sync(0xFFFFFFFFu, nan_k, 1);
-        nan_k |= __shfl_xor_sync(0xFFFFFFFFu, nan_k, 2);
+      // ---------------------------------------------------------- the copies
+      __syncwarp();  // the stage that is filled next has been read
+      if (ci + 2 * KVF_WARPS < chunks) {
+        if ((n_fetched & 31) == 0) locate(ci + 2 * KVF_WARPS);
+        fetch(n_fetched++, stage == 0 ? 2 : stage - 1, &n2);
       }
+      asm volatile("cp.async.commit_group;" ::: "memory");
+      asm volatile("cp.async.wait_group 2;" ::: "memory");
+      __syncwarp();
+      const uint32_t kb = ring + stage * (32 * D), vb = kb + 16 * D;
+      uint32_t kr[2][KJ][4], vr[4][VU][VW];
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int j = 0; j < KJ; ++j) kvf_lds<4>(kr[i][j], kb + kvf_at<D>(key_r + 8 * i, c + 4 * j));
+      // ---------------------------------------------------------- scores
+      // (two sums side by side: a product waits for the one before it in its sum)
+      float s[NT][4], s_odd[NT][4];
+#pragma unroll
+      for (int g = 0; g < NT; ++g)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[g][i] = s_odd[g][i] = 0.f;
+      const bool there = cur.ks != KVF_GONE;
+      const bool marked = there && (cur.vs & 1u);
 #pragma unroll
       for (int j = 0; j < KJ; ++j)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const uint32_t x0 = kr[0][j][i], x1 = kr[1][j][i];
-          const uint32_t a[4] = {mul_bf16x2(kva_place(x0 << 8), fk), mul_bf16x2(kva_place(x1 << 8), fk),
-                                 mul_bf16x2(kva_place(x0), fk), mul_bf16x2(kva_place(x1), fk)};
+          uint32_t a[4];
+          kvf_codes(kr[0][j][i], a[0], a[2]);
+          kvf_codes(kr[1][j][i], a[1], a[3]);
 #pragma unroll
-          for (int g = 0; g < NT; ++g) kvf_mma(s[g], a, qf[g][j * 4 + i][0], qf[g][j * 4 + i][1]);
+          for (int g = 0; g < NT; ++g) kvf_mma(i & 1 ? s_odd[g] : s[g], a, qf[g][j][i][0], qf[g][j][i][1]);
         }
-      // ---------------------------------------------------------- the next keys
-      const bool more = ci + KVF_WARPS < chunks;
-      if (more) {
-        locate(pos + KVF_WARPS * 16, pg1, &nxt);
-        load_k(nxt);
-        pg1 = kvf_page<D>(p, w.b, pos + 2 * KVF_WARPS * 16, chunks * 16);
+      // (the product of the factors may pass the range where the score does not, at zero codes)
+      const float ks = __uint_as_float(cur.ks & 0x7F800000u), vs = __uint_as_float(cur.vs & 0x7F800000u) * 0x1p-31f;
+      const auto factor = [&](float back) { return fminf(fmaxf(back * ks, -3e38f), 3e38f); };
+#pragma unroll
+      for (int g = 0; g < NT; ++g)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[g][i] = (s[g][i] + s_odd[g][i]) * factor(qsc[g][i & 1]);
+#pragma unroll 1
+      for (int t = 1; t < terms; ++t) {  // elements of a query far below its largest
+#pragma unroll
+        for (int g = 0; g < NT; ++g) {
+          float s1[4] = {0.f, 0.f, 0.f, 0.f};
+          const uint16_t* qp = query_row(g);
+          const int sh1 = min(sh[g] + KVF_TERM * t, 126);
+#pragma unroll
+          for (int j = 0; j < KJ; ++j) {
+            uint32_t q1[4][2];
+            kvf_query(qp + 64 * j, r0 + g * 8 + r < p.rows, sh1, false, q1);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              uint32_t a[4];
+              kvf_codes(kr[0][j][i], a[0], a[2]);
+              kvf_codes(kr[1][j][i], a[1], a[3]);
+              kvf_mma(s1, a, q1[i][0], q1[i][1]);
+            }
+          }
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const float f = factor(p.scale_log2 * kvf_pow2(-__shfl_sync(0xFFFFFFFFu, sh1, (2 * c + i) * 4)));
+            s[g][i] += s1[i] * f;
+            s[g][i + 2] += s1[i + 2] * f;
+          }
+        }
       }
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < VU; ++j) {
+          const int u8 = r + 8 * j;  // VW words each
+          kvf_lds<VW>(vr[i][j], vb + (VW == 4 ? kvf_at<D>(key_v[i & 1] + 8 * (i >> 1), u8)
+                                              : kvf_at<D>(key_v[i & 1] + 8 * (i >> 1), u8 >> 1) + (u8 & 1) * 8));
+        }
       // ---------------------------------------------------------- weights
-      // lane: keys r and r + 8, columns 2 c and 2 c + 1 of each group
-      const float sc = p.scale_log2 * rest_k;
+      // lane: product rows r and r + 8, columns 2 c and 2 c + 1 of each group
       bool rise = false;
       const bool open = there && !marked && pos + 16 <= clear;
 #pragma unroll
       for (int g = 0; g < NT; ++g)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          s[g][i] *= sc;
           if (!open) {
             const int row = r0 + g * 8 + 2 * c + (i & 1);
-            if ((nan_k >> (i >> 1)) & 1u) s[g][i] = __uint_as_float(0x7FC00000u);
-            if (!there || !kva_sees(p, w.b, w.len, w.n, row / p.G, pos + r + (i >> 1) * 8)) s[g][i] = -INFINITY;
+            if (!there || !kva_sees(p, w.b, w.len, w.n, row / p.G, pos + key_r + (i >> 1) * 8)) s[g][i] = -INFINITY;
           }
           rise |= s[g][i] > m[g][i & 1] + KVA_RISE;
         }
@@ -429,7 +551,7 @@ __global__ void __launch_bounds__(KVF_WARPS * 32, D * NT <= 128 ? 2 : 1) kv_attn
             const float now = fmaxf(m[g][i], top);
             const float f = now == -INFINITY ? 1.f : kva_ex2(m[g][i] - now);
             m[g][i] = now;
-            mu[g][i] = (now == -INFINITY ? 0.f : now) + KVA_DOWN;
+            mu[g][i] = (now == -INFINITY ? 0.f : now) - KVF_TOP;
             l[g][i] *= f;
 #pragma unroll
             for (int y = 0; y < D / 16; ++y) {
@@ -446,15 +568,15 @@ __global__ void __launch_bounds__(KVF_WARPS * 32, D * NT <= 128 ? 2 : 1) kv_attn
         for (int i = 0; i < 4; ++i) {
           e[i] = kva_ex2(s[g][i] - mu[g][i & 1]);
           l[g][i & 1] += e[i];
-          e[i] *= rest_v;
         }
-        pb[g][0] = kvf_trans(cvt_bf16x2(e[0], e[1]));
-        pb[g][1] = kvf_trans(cvt_bf16x2(e[2], e[3]));
+        pb[g][0] = kvf_trans(kvf_f16x2(e[0], e[1]));
+        pb[g][1] = kvf_trans(kvf_f16x2(e[2], e[3]));
       }
       // ---------------------------------------------------------- outputs
-      if (marked) {
-        // codes that are NaN count as zero in the product; the rows that see them get NaN
-        uint32_t bits[4];  // of keys 2 c, 2 c + 1, 2 c + 8, 2 c + 9, by the lane's columns
+      if (!open) {
+        // codes that are NaN (also those behind the last row, of which nothing is known) count
+        // as zero in the product; the rows that see them get NaN
+        uint32_t bits[4];  // of the lane's four keys, by its columns
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           bits[i] = 0;
@@ -472,7 +594,7 @@ __global__ void __launch_bounds__(KVF_WARPS * 32, D * NT <= 128 ? 2 : 1) kv_attn
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const uint32_t of = __shfl_sync(0xFFFFFFFFu, bits[i], (lane & ~3) | y);
-            const int at = pos + 2 * y + (i & 1) + (i >> 1) * 8;
+            const int at = pos + kvf_key<D>(2 * y + (i & 1)) + (i >> 1) * 8;
             if (of) {
 #pragma unroll
               for (int g = 0; g < NT; ++g)
@@ -488,18 +610,21 @@ __global__ void __launch_bounds__(KVF_WARPS * 32, D * NT <= 128 ? 2 : 1) kv_attn
         for (int x = 0; x < VW; ++x)
 #pragma unroll
           for (int h = 0; h < 2; ++h) {  // columns 4 x + 2 h, + 1 of the piece
-            const uint32_t sel0 = h ? 0x6020u : 0x4000u, sel1 = h ? 0x7030u : 0x5010u;
-            const uint32_t a[4] = {mul_bf16x2(kva_place(__byte_perm(vr[0][j][x], vr[1][j][x], sel0)), fv),
-                                   mul_bf16x2(kva_place(__byte_perm(vr[0][j][x], vr[1][j][x], sel1)), fv),
-                                   mul_bf16x2(kva_place(__byte_perm(vr[2][j][x], vr[3][j][x], sel0)), fv),
-                                   mul_bf16x2(kva_place(__byte_perm(vr[2][j][x], vr[3][j][x], sel1)), fv)};
+            const uint32_t sel = h ? 0x7362u : 0x5140u;  // two keys' codes of a column side by side
+            uint32_t a[4];
+            kvf_codes(__byte_perm(vr[0][j][x], vr[1][j][x], sel), a[0], a[1]);
+            kvf_codes(__byte_perm(vr[2][j][x], vr[3][j][x], sel), a[2], a[3]);
 #pragma unroll
-            for (int g = 0; g < NT; ++g) kvf_mma(o[g][(j * VW + x) * 2 + h], a, pb[g][0], pb[g][1]);
+            for (int g = 0; g < NT; ++g) {
+              float t[4] = {0.f, 0.f, 0.f, 0.f};
+              kvf_mma(t, a, pb[g][0], pb[g][1]);
+#pragma unroll
+              for (int i = 0; i < 4; ++i) o[g][(j * VW + x) * 2 + h][i] = fmaf(t[i], vs, o[g][(j * VW + x) * 2 + h][i]);
+            }
           }
-      if (more) {
-        load_v(nxt);
-        cur = nxt;
-      }
+      cur = n1;
+      n1 = n2;
+      stage = stage == 2 ? 0 : stage + 1;
     }
 
     // ------------------------------------------------------------ the warps' results together
@@ -511,7 +636,7 @@ __global__ void __launch_bounds__(KVF_WARPS * 32, D * NT <= 128 ? 2 : 1) kv_attn
         for (int x = 4; x < 32; x <<= 1) l[g][i] += __shfl_xor_sync(0xFFFFFFFFu, l[g][i], x);
         if (r == 0) {
           sm_m[warp][g * 8 + 2 * c + i] = m[g][i];
-          sm_l[warp][g * 8 + 2 * c + i] = l[g][i];
+          sm_l[warp][g * 8 + 2 * c + i] = l[g][i] * 0x1p-31f;  // as the outputs (2^(KVF_TOP - 31) = 2^-KVA_DOWN)
         }
       }
     __syncthreads();
@@ -551,6 +676,7 @@ __global__ void __launch_bounds__(KVF_WARPS * 32, D * NT <= 128 ? 2 : 1) kv_attn
           if ((nanv[g][i] >> (2 * y + 1)) & 1u) o[g][y][i + 2] = __uint_as_float(0x7FC00000u);
         }
       }
+    // (every warp is past its ring, which lies where the outputs go: the barrier above)
     if (warp >= 4) put(kvf_smem + (warp - 4) * NR * D, false);
     __syncthreads();
     if (warp < 4) put(kvf_smem + warp * NR * D, true);
@@ -589,34 +715,56 @@ __global__ void __launch_bounds__(KVF_WARPS * 32, D * NT <= 128 ? 2 : 1) kv_attn
   }
 }
 
-// Parts of a row tile that several CTAs share, added up in order.  Block (c, y): rows y, y +
-// gridDim.y, .. of the row tile whose first tile CTA c has.
+// Parts of a row tile that several CTAs share, added up.  Blocks (c, y): the row tile whose first
+// tile CTA c has, some of its rows each.  D / 4 threads take a row; where there are many parts
+// (one long sequence) up to eight of such groups take every eighth part each, with a reference of
+// their own, and are added up in order.  (64 heads over 131069 keys, 37 parts a row tile, one
+// group a row: the join took 30 us of 76.)
 __global__ void __launch_bounds__(256) kv_attn_join_kernel(const __grid_constant__ KvAttnParams p) {
+  __shared__ float4 sv[256];
+  __shared__ float2 sml[256];
+  asm volatile("griddepcontrol.wait;" ::: "memory");  // until all parts are written
   const int4 own = p.owner[blockIdx.x];
   if (own.w == 0) return;
   const int b = own.x, r0 = own.y * p.nr, h = own.z, parts = own.w, d = p.c.d, per_row = d >> 2;
-  const int n = kv_new(p.c, b);
-  const int lane_row = threadIdx.x / per_row, rows = blockDim.x / per_row;  // rows of the block at once
-  for (int row = blockIdx.y * rows + lane_row; row - lane_row < p.nr; row += gridDim.y * rows) {
-    if (lane_row >= rows || row >= p.nr || r0 + row >= p.rows) continue;
-    const int t = (r0 + row) / p.G, g = (r0 + row) - t * p.G, col = (threadIdx.x - lane_row * per_row) * 4;
+  const int n = kv_new(p.c, b), at_once = blockDim.x / per_row;
+  int groups = 1;
+  while (groups * 2 <= at_once && groups * 4 < parts) groups *= 2;
+  const int rows = at_once / groups;
+  const int set = threadIdx.x / per_row, col = (threadIdx.x - set * per_row) * 4, grp = set % groups, mine = set / groups;
+  for (int first = blockIdx.y * rows; first < p.nr && r0 + first < p.rows; first += gridDim.y * rows) {
+    const int row = first + mine;
+    const bool in = mine < rows && row < p.nr && r0 + row < p.rows;
     float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
     float top = -INFINITY, sum = 0.f;
-    for (int i = 0; i < parts; ++i) {
-      const int64_t slot = i ? 2 * ((int64_t)blockIdx.x + i) : 2 * (int64_t)blockIdx.x + 1;
-      top = fmaxf(top, __ldg(&p.part_ml[slot * p.nr + row]).x);
+    const auto take = [&](const float2 ml, const float4 y) {
+      const float now = fmaxf(top, ml.x);
+      const float f0 = now == -INFINITY ? 1.f : kva_ex2(top - now), f1 = now == -INFINITY ? 1.f : kva_ex2(ml.x - now);
+      top = now;
+      sum = f0 * sum + f1 * ml.y;
+      v = make_float4(f0 * v.x + f1 * y.x, f0 * v.y + f1 * y.y, f0 * v.z + f1 * y.z, f0 * v.w + f1 * y.w);
+    };
+    if (in) {
+#pragma unroll 4
+      for (int i = grp; i < parts; i += groups) {
+        const int64_t at = (i ? 2 * ((int64_t)blockIdx.x + i) : 2 * (int64_t)blockIdx.x + 1) * p.nr + row;
+        take(p.part_ml[at], *reinterpret_cast<const float4*>(p.part_o + at * d + col));
+      }
     }
-    for (int i = 0; i < parts; ++i) {
-      const int64_t slot = i ? 2 * ((int64_t)blockIdx.x + i) : 2 * (int64_t)blockIdx.x + 1;
-      const float2 ml = __ldg(&p.part_ml[slot * p.nr + row]);
-      const float4 y = __ldg(reinterpret_cast<const float4*>(p.part_o + (slot * p.nr + row) * d + col));
-      const float f = top == -INFINITY ? 1.f : kva_ex2(ml.x - top);
-      sum += f * ml.y;
-      v.x += f * y.x; v.y += f * y.y; v.z += f * y.z; v.w += f * y.w;
+    if (groups > 1) {
+      __syncthreads();  // (the row before has been read)
+      sv[threadIdx.x] = v;
+      sml[threadIdx.x] = make_float2(top, sum);
+      __syncthreads();
+      if (grp == 0 && in)
+        for (int i = 1; i < groups; ++i) take(sml[threadIdx.x + i * per_row], sv[threadIdx.x + i * per_row]);
     }
-    const float f = kva_norm(top, sum, p.sink ? __ldg(p.sink + h * p.G + g) * 1.4426950408889634f : 0.f, p.sink);
-    *reinterpret_cast<uint2*>(p.out + (((int64_t)b * p.c.T + t) * p.H + h * p.G + g) * d + col) =
-        t < n ? make_uint2(cvt_bf16x2(v.x * f, v.y * f), cvt_bf16x2(v.z * f, v.w * f)) : make_uint2(0, 0);
+    if (grp == 0 && in) {
+      const int t = (r0 + row) / p.G, g = (r0 + row) - t * p.G;
+      const float f = kva_norm(top, sum, p.sink ? __ldg(p.sink + h * p.G + g) * 1.4426950408889634f : 0.f, p.sink);
+      *reinterpret_cast<uint2*>(p.out + (((int64_t)b * p.c.T + t) * p.H + h * p.G + g) * d + col) =
+          t < n ? make_uint2(cvt_bf16x2(v.x * f, v.y * f), cvt_bf16x2(v.z * f, v.w * f)) : make_uint2(0, 0);
+    }
   }
 }
 

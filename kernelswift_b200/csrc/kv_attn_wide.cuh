@@ -156,6 +156,7 @@ __global__ void __launch_bounds__(KVW_THREADS, 1) kv_attn_wide_kernel(const __gr
     tmem_relinquish<1>();
   }
   tc_fence_before();
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the join may be set up
   kva_find(p, &sh->find);  // (its barriers also publish the above)
   tc_fence_after();
   const uint32_t tmem = sh->tmem;

@@ -294,6 +294,31 @@ def test_large_rows_without_weight(cuda_ok, T, big):
     check(q, parts, table, lens, 0.1)
 
 
+@pytest.mark.parametrize("T", [1, 2, 40])
+@pytest.mark.parametrize("big,key", [(2.0 ** 20, 1), (2.0 ** 60, 0), (2.0 ** 100, 0), (2.0 ** 126, 0), (2.0 ** 40, 1), (2.0 ** -130, 1)])
+def test_queries_of_any_size_within_a_row(cuda_ok, T, big, key):
+    """Columns of a query that are far larger than the others, where the keys are zero (then the
+    others make the score) or where they are not."""
+    g, q, parts, table, lens = make(1, T, 8, 2, 128, 64, 16, [300], 30)
+    q[..., ::2] *= big
+    if not key:
+        parts[0].view(torch.uint8)[..., ::2] = 0
+    check(q, parts, table, lens, 0.1 if big < 1 or not key else 0.1 / big)
+    q[..., 1::4] *= 2.0 ** -20
+    check(q, parts, table, lens, 0.1 if big < 1 or not key else 0.1 / big)
+
+
+@pytest.mark.parametrize("T", [1, 40])
+@pytest.mark.parametrize("size", [2.0 ** -126, 2.0 ** -60, 2.0 ** 60, 2.0 ** 127])
+def test_queries_of_any_size(cuda_ok, T, size):
+    g, q, parts, table, lens = make(1, T, 8, 2, 64, 64, 16, [300], 31)
+    q.copy_(q.clamp(-1, 1) * size)
+    assert q.isfinite().all()
+    # (scores are sums before the softmax scale: keys of 2^-6 keep them finite)
+    parts[1].fill_(2.0 ** -14)
+    check(q, parts, table, lens, 0.1 / size if size < 2.0 ** 100 else 2.0 ** -126)
+
+
 @pytest.mark.parametrize("sm", [0.0, -0.07, 1e-30, 40.0])
 def test_any_softmax_scale(cuda_ok, sm):
     for T in (1, 40):
