@@ -640,34 +640,58 @@ def verify_draft(p: torch.Tensor, tokens: torch.Tensor, u: torch.Tensor, noise: 
 
 
 def _kv_args(name, k8, k_scale, v8, v_scale, page_table, lens, n_new, B):
-    if k8.dtype not in _FP8 or v8.dtype not in _FP8 or k8.dim() != 4 or k8.shape != v8.shape:
+    shape, scales = k8.shape, k_scale.shape
+    if k8.dtype not in _FP8 or v8.dtype not in _FP8 or len(shape) != 4 or v8.shape != shape:
         raise RuntimeError(f"{name}: k8 and v8 must be float8_e4m3fn (or their uint8 bytes) [pages, heads, page, d]")
-    pages, heads, page, D = k8.shape
-    if k_scale.dtype != torch.float32 or v_scale.dtype != torch.float32 or k_scale.dim() != 3 or \
-            k_scale.shape != v_scale.shape or k_scale.shape[:2] != k8.shape[:2]:
+    pages, heads, page, D = shape
+    if k_scale.dtype != torch.float32 or v_scale.dtype != torch.float32 or len(scales) != 3 or \
+            v_scale.shape != scales or scales[0] != pages or scales[1] != heads:
         raise RuntimeError(f"{name}: k_scale and v_scale must be float32 [pages, heads, page / block]")
-    per = k_scale.shape[2]
+    per = scales[2]
     if pages < 1 or heads < 1 or per < 1 or page < 1 or page % per:
         raise RuntimeError(f"{name}: pages of {page} rows and {per} scales do not make blocks")
-    _table_args(name, page_table, lens, B)
+    table = page_table.shape
+    if page_table.dtype != torch.int32 or len(table) != 2 or table[0] != B:
+        raise RuntimeError(f"{name}: page_table must be int32 [b, max_pages]")
+    if lens.dtype != torch.int32 or lens.shape != (B,):
+        raise RuntimeError(f"{name}: lens must be int32 [b]")
     ts = [k8, k_scale, v8, v_scale, page_table, lens]
     if n_new is not None:
         if n_new.dtype != torch.int32 or n_new.shape != (B,):
             raise RuntimeError(f"{name}: n_new must be int32 [b]")
         ts.append(n_new)
-    return pages, heads, page, page // per, D, ts
+    return pages, heads, page, page // per, D, table[1], ts
 
 
-def _rows_of_tokens(name, what, x, D):
+def _on_one_device(name, ts, rows=()):
+    """``_require_cuda`` for the common case in fewer calls; rows need not be contiguous."""
+    d = ts[0].get_device()
+    if d >= 0 and ts[0].is_cuda:
+        for t in ts:
+            if t.get_device() != d or not t.is_contiguous():
+                break
+        else:
+            for t in rows:
+                if t.get_device() != d:
+                    raise RuntimeError(f"{name}: inputs must be on one device")
+            return
+    _require_cuda(name, *ts)
+    raise RuntimeError(f"{name}: inputs must be on one device")
+
+
+def _rows_of_tokens(name, what, x, shape, D):
     """Elements from sequence to sequence and from token to token of [b, t, heads, D]."""
-    if x.dtype != torch.bfloat16 or x.dim() != 4 or x.shape[3] != D:
+    if x.dtype != torch.bfloat16 or len(shape) != 4 or shape[3] != D:
         raise RuntimeError(f"{name}: {what} must be bfloat16 [b, t, heads, {D}]")
-    if x.numel() and (x.stride(3) != 1 or (x.shape[2] > 1 and x.stride(2) != D)):
+    B, T, H, _ = shape
+    if x.is_contiguous():
+        return T * H * D, H * D
+    st = x.stride()
+    if x.numel() and (st[3] != 1 or (H > 1 and st[2] != D)):
         raise RuntimeError(f"{name}: a token's rows of {what} must lie together")
-    B, T, H, _ = x.shape
     # (the stride of a dimension of one element says nothing)
-    ts = x.stride(1) if T > 1 else H * D
-    return x.stride(0) if B > 1 else T * ts, ts
+    ts = st[1] if T > 1 else H * D
+    return st[0] if B > 1 else T * ts, ts
 
 
 def kv_append(k: torch.Tensor, v: torch.Tensor, k8: torch.Tensor, k_scale: torch.Tensor,
@@ -692,43 +716,44 @@ def kv_append(k: torch.Tensor, v: torch.Tensor, k8: torch.Tensor, k_scale: torch
     largest element (at most 448 scales); where a block holds tokens already its scale only grows, and they are rounded
     again to it.  An element that is NaN or infinite reads as NaN, and the lowest bit of its
     block's scale is set.  lens is not changed: add n_new to it after the last layer."""
-    if k.dim() != 4:
+    shape = k.shape
+    if len(shape) != 4:
         raise RuntimeError("kv_append: k must be bfloat16 [b, t, heads, d]")
-    B, T = k.shape[:2]
-    pages, heads, page, block, D, ts = _kv_args("kv_append", k8, k_scale, v8, v_scale, page_table, lens, n_new, B)
-    k_bs, k_ts = _rows_of_tokens("kv_append", "k", k, D)
-    v_bs, v_ts = _rows_of_tokens("kv_append", "v", v, D)
-    if k.shape[2] != heads or v.shape != k.shape:
+    B, T = shape[0], shape[1]
+    pages, heads, page, block, D, max_pages, ts = _kv_args("kv_append", k8, k_scale, v8, v_scale, page_table, lens,
+                                                           n_new, B)
+    k_bs, k_ts = _rows_of_tokens("kv_append", "k", k, shape, D)
+    v_bs, v_ts = _rows_of_tokens("kv_append", "v", v, v.shape, D)
+    if shape[2] != heads or v.shape != shape:
         raise RuntimeError(f"kv_append: k and v must be [b, t, {heads}, {D}]")
-    dev, rows = k8.device, [k, v]
+    rows = (k, v)
     H = q_bs = q_ts = rope_dim = n_freqs = 0
     if freqs is not None:
-        if freqs.dtype != torch.float32 or freqs.dim() != 3 or freqs.shape[2] != 2:
+        table = freqs.shape
+        if freqs.dtype != torch.float32 or len(table) != 3 or table[2] != 2:
             raise RuntimeError("kv_append: freqs must be float32 [p, rope_dim / 2, 2]")
-        n_freqs, rope_dim = freqs.shape[0], 2 * freqs.shape[1]
+        n_freqs, rope_dim = table[0], 2 * table[1]
         ts.append(freqs)
     if positions is not None:
         if positions.dtype != torch.int32 or positions.shape != (B, T):
             raise RuntimeError("kv_append: positions must be int32 [b, t]")
         ts.append(positions)
     if q is not None:
-        q_bs, q_ts = _rows_of_tokens("kv_append", "q", q, D)
-        H = q.shape[2]
-        if q.shape[:2] != k.shape[:2] or H < 1:
+        of_q = q.shape
+        q_bs, q_ts = _rows_of_tokens("kv_append", "q", q, of_q, D)
+        H = of_q[2]
+        if of_q[0] != B or of_q[1] != T or H < 1:
             raise RuntimeError("kv_append: q must have the tokens of k")
-        rows.append(q)
-    _require_cuda("kv_append", *ts)
-    for x in rows:
-        if x.device != dev:
-            raise RuntimeError("kv_append: inputs must be on one device")
+        rows = (k, v, q)
+    _on_one_device("kv_append", ts, rows)
     turn = q is not None and rope_dim > 0
-    q_out = torch.empty(B, T, H, D, dtype=torch.bfloat16, device=dev) if turn else q
+    q_out = q.new_empty(of_q) if turn else q
     with _on(k8):
         check(lib().ks_kv_append(k.data_ptr(), k_bs, k_ts, v.data_ptr(), v_bs, v_ts,
                                  q.data_ptr() if turn else None, q_bs, q_ts, H, q_out.data_ptr() if turn else None,
                                  _ptr(freqs), n_freqs, rope_dim, _ptr(positions), k8.data_ptr(),
                                  k_scale.data_ptr(), v8.data_ptr(), v_scale.data_ptr(), pages, heads, page, block,
-                                 D, page_table.data_ptr(), page_table.shape[1], lens.data_ptr(), _ptr(n_new), B, T,
+                                 D, page_table.data_ptr(), max_pages, lens.data_ptr(), _ptr(n_new), B, T,
                                  _stream(k8)), "ks_kv_append")
     return q_out
 
@@ -754,11 +779,13 @@ def kv_attn(q: torch.Tensor, k8: torch.Tensor, k_scale: torch.Tensor, v8: torch.
     attn_sink fp32 [H] as in ``sparse_attn``.  Returns bf16 [B,T,H,D]; a token that sees
     nothing gets zeros.  Weights enter their product in bf16 (2^-8 of themselves), scores
     and sums are fp32, the result is rounded once."""
-    if q.dtype != torch.bfloat16 or q.dim() != 4:
+    shape = q.shape
+    if q.dtype != torch.bfloat16 or len(shape) != 4:
         raise RuntimeError("kv_attn: q must be bfloat16 [b, t, h, d]")
-    B, T, H, _ = q.shape
-    pages, heads, page, block, D, ts = _kv_args("kv_attn", k8, k_scale, v8, v_scale, page_table, lens, n_new, B)
-    if q.shape[3] != D or H % heads or H < 1:
+    B, T, H, of_q = shape
+    pages, heads, page, block, D, max_pages, ts = _kv_args("kv_attn", k8, k_scale, v8, v_scale, page_table, lens,
+                                                           n_new, B)
+    if of_q != D or H % heads or H < 1:
         raise RuntimeError(f"kv_attn: q must be [b, t, h, {D}], h a multiple of {heads}")
     ts.append(q)
     if mask is not None:
@@ -769,22 +796,22 @@ def kv_attn(q: torch.Tensor, k8: torch.Tensor, k_scale: torch.Tensor, v8: torch.
         if attn_sink.dtype != torch.float32 or attn_sink.shape != (H,):
             raise RuntimeError("kv_attn: attn_sink must be float32 [h]")
         ts.append(attn_sink)
-    _require_cuda("kv_attn", *ts)
+    _on_one_device("kv_attn", ts)
     if out is None:
-        out = torch.empty(B, T, H, D, dtype=torch.bfloat16, device=q.device)
+        out = q.new_empty(shape)
     else:
         _check_out("kv_attn", out, (B, T, H, D), torch.bfloat16, q.device)
     need = kv_attn_workspace_size(T, H, heads, D)
     if workspace is None:
-        workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
+        workspace, size = q.new_empty(need, dtype=torch.uint8), need
     else:
         _check_workspace("kv_attn", workspace, need, q.device)
+        size = workspace.numel() * workspace.element_size()
     with _on(q):
         check(lib().ks_kv_attn(q.data_ptr(), k8.data_ptr(), k_scale.data_ptr(), v8.data_ptr(), v_scale.data_ptr(),
-                               pages, heads, page, block, D, page_table.data_ptr(), page_table.shape[1],
+                               pages, heads, page, block, D, page_table.data_ptr(), max_pages,
                                lens.data_ptr(), _ptr(n_new), _ptr(mask), _ptr(attn_sink), out.data_ptr(), B, T, H,
-                               float(softmax_scale), workspace.data_ptr(),
-                               workspace.numel() * workspace.element_size(), _stream(q)), "ks_kv_attn")
+                               softmax_scale, workspace.data_ptr(), size, _stream(q)), "ks_kv_attn")
     return out
 
 
@@ -799,34 +826,36 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0
     tokens; the last two None without top): the largest first, the lowest index first
     among equal ones; top at most 32.  A negative token (``verify_draft``'s padding) has
     logp 0.  Sums are in fp32.  A row with a NaN, an infinite or no finite logit gets NaN."""
-    if logits.dtype not in (torch.bfloat16, torch.float32) or logits.dim() < 1:
+    shape, dtype, of_tokens, ids = logits.shape, logits.dtype, tokens.shape, tokens.dtype
+    if dtype not in (torch.bfloat16, torch.float32) or len(shape) < 1:
         raise RuntimeError("token_logprobs: logits must be bfloat16 or float32 [..., v]")
-    if tokens.dtype not in (torch.int32, torch.int64) or tokens.shape != logits.shape[:-1]:
+    if ids not in (torch.int32, torch.int64) or of_tokens != shape[:-1]:
         raise RuntimeError("token_logprobs: tokens must be int32 or int64 [...], one per row of logits")
-    V, top = logits.shape[-1], int(top)
-    rows = logits
-    if logits.dim() != 2:
-        try:
-            rows = logits.view(-1, V) if V else logits
-        except RuntimeError:
-            raise RuntimeError("token_logprobs: the rows of logits must be a constant stride apart") from None
-    _require_cuda("token_logprobs", tokens)
-    if logits.device != tokens.device:
-        raise RuntimeError("token_logprobs: inputs must be on one device")
-    if rows.numel() and V > 1 and rows.stride(1) != 1:
-        raise RuntimeError("token_logprobs: the columns of logits must be contiguous")
-    N = tokens.numel()
-    ld = rows.stride(0) if N > 1 else V
-    logp = torch.empty(tokens.shape, dtype=torch.float32, device=tokens.device)
-    entropy = torch.empty_like(logp)
+    V, top, N = shape[-1], int(top), tokens.numel()
+    ld = V
+    if not logits.is_contiguous():
+        rows = logits
+        if len(shape) != 2:
+            try:
+                rows = logits.view(-1, V) if V else logits
+            except RuntimeError:
+                raise RuntimeError("token_logprobs: the rows of logits must be a constant stride apart") from None
+        if N and V > 1 and rows.stride(-1) != 1:
+            raise RuntimeError("token_logprobs: the columns of logits must be contiguous")
+        if N > 1:
+            ld = rows.stride(0)
+    _on_one_device("token_logprobs", (tokens,), (logits,))
+    if top < 0 or top > V:
+        raise RuntimeError(f"token_logprobs: top={top} must be at least 0 and at most v")
+    logp = tokens.new_empty(of_tokens, dtype=torch.float32)
+    entropy = tokens.new_empty(of_tokens, dtype=torch.float32)
     top_logp = top_ids = None
     if top:
-        shape = tuple(tokens.shape) + (max(top, 0),)
-        top_logp = torch.empty(shape, dtype=torch.float32, device=tokens.device)
-        top_ids = torch.empty(shape, dtype=tokens.dtype, device=tokens.device)
+        top_logp = tokens.new_empty((*of_tokens, top), dtype=torch.float32)
+        top_ids = tokens.new_empty((*of_tokens, top))
     with _on(tokens):
-        check(lib().ks_token_logprobs(rows.data_ptr(), int(logits.dtype == torch.bfloat16), ld, tokens.data_ptr(),
-                                      KS_INT64 if tokens.dtype == torch.int64 else KS_INT32, N, V, top,
+        check(lib().ks_token_logprobs(logits.data_ptr(), dtype == torch.bfloat16, ld, tokens.data_ptr(),
+                                      KS_INT64 if ids == torch.int64 else KS_INT32, N, V, top,
                                       logp.data_ptr(), entropy.data_ptr(), _ptr(top_logp), _ptr(top_ids),
                                       _stream(tokens)), "ks_token_logprobs")
     return logp, entropy, top_logp, top_ids
