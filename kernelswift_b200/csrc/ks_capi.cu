@@ -1347,11 +1347,12 @@ int ks_token_logprobs(const void* logits, int32_t is_bf16, int64_t ld, const voi
       !aligned(top_logp, 4) || !aligned(top_ids, ts))
     return fail(KS_ERR_ALIGNMENT, "token_logprobs: pointers must be aligned to their elements");
   if (V >= 0x7FFFFFFFll - 65536 || N > (1 << 27)) return fail(KS_ERR_UNSUPPORTED, "token_logprobs: too large");
-  // As many CTAs per row as hold it in registers at once, more where there are few rows and
-  // each still has a few thousand values.
-  const int64_t pass = (int64_t)LP_THREADS * LP_PIECES * (is_bf16 ? 8 : 4);
+  // A CTA per row where there are enough, else up to eight, as long as each has a few thousand
+  // values.  (129280 values, 20 alternatives, 1, 2, 4 and 8 CTAs a row: 512 rows 42, 50, 60 and 79 us,
+  // 64 rows 26, 21, 19 and 19 us, 8 rows 25, 19, 15 and 14 us.)
+  const int64_t batch = (int64_t)LP_THREADS * LP_PIECES * (is_bf16 ? 8 : 4);
   int cs = 1;
-  while (cs < LP_MAX_CLUSTER && ((V + cs - 1) / cs + 8 > pass || (N * cs * 2 <= dev->num_sms && V / cs >= 8192))) cs <<= 1;
+  while (cs < LP_MAX_CLUSTER && N * cs < 2ll * dev->num_sms && V / cs >= 4096) cs <<= 1;
   LogprobsParams p{};
   p.x = logits;
   p.ld = ld;
@@ -1359,6 +1360,7 @@ int ks_token_logprobs(const void* logits, int32_t is_bf16, int64_t ld, const voi
   p.tok_i64 = token_dtype == KS_INT64;
   p.N = N; p.V = (int)V; p.top = top;
   p.per = (int)round_up((V + cs - 1) / cs, 8);
+  p.together = (int)((p.per + 8 + batch - 1) / batch + LP_MAXIMA - 1) / LP_MAXIMA;
   p.logp = logp; p.entropy = entropy; p.top_logp = top_logp; p.top_ids = top_ids;
   p.status = dev->status;
   cudaLaunchConfig_t cfg = {};

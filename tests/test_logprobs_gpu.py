@@ -62,7 +62,24 @@ def test_orders_that_are_hard_to_search(cuda_ok, dtype):
                      torch.where(at % 7001 == 5, at / V, float("-inf")), torch.where(at == V - 1, 9.0, 0.0),
                      torch.where(at < 2000, 5.0, at % 5)]).to(dtype)
     check(x, torch.arange(10, device="cuda") * 13, top)
+    check(x[:, : 50001 - 8].repeat(1, 14), torch.arange(10, device="cuda") * 13, top)  # several passes
     check(x, torch.arange(10, device="cuda").int(), 1)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("low", [float("-inf"), -1e30, "min"])
+@pytest.mark.parametrize("V", [300, 20011, 129280])
+def test_masked_vocabularies(cuda_ok, dtype, low, V):
+    """All but a few tokens at -inf, or at a value that stands for it."""
+    g = torch.Generator(device="cuda").manual_seed(V)
+    low = torch.finfo(dtype).min if low == "min" else low
+    x = torch.full((6, V), low, device="cuda").to(dtype)
+    for i, n in enumerate((0, 1, 3, 20, 31, 200)):
+        at = torch.randperm(V, device="cuda", generator=g)[:n]
+        x[i, at] = torch.randn(n, device="cuda", generator=g).to(dtype)
+    if low == float("-inf"):
+        x[0, V // 2] = 0
+    check(x, torch.randint(0, V, (6,), device="cuda", generator=g), 20)
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
