@@ -4,8 +4,8 @@
 // Rows are the MMA's M: S = Q K^T and O += P V on tcgen05 in bf16, scores, weights and outputs
 // in tensor memory, the weights as the second product's A operand where the scores were. Keys
 // and values come from the cache as codes in registers and are expanded to bf16 in shared
-// memory on the way (4 KB of codes are read once per 256 rows; the expansion, ten integer
-// operations per four codes, runs beside the products and takes about a third of their time).
+// memory on the way (4 KB of codes are read once per 256 rows; the expansion, ten
+// operations per four codes on two pipes, runs beside the products).
 //
 // A CTA works on two streams of (scores, weights) so that one's softmax runs under the other's
 // products:
@@ -15,8 +15,8 @@
 //   D > 128 (tensor memory holds one output): even and odd tiles, one output; one warpgroup does
 //     the softmax of both in turn.
 // Warps: 0-3 and 4-7 softmax (thread = row = TMEM lane), also queries and results; 8 issues the
-// products; 9-16 load and expand. Codes of the next unit (the keys or the values of a tile) are in
-// flight while one is expanded; units lie in a ring in the order the products take them.
+// products; 9-15 load and expand.  Codes are loaded a unit (the keys or the values of a tile) ahead;
+// units lie in a ring in the order the products take them.
 //
 // References are raised only when a score passes them by 2^KVA_RISE (rarely after the first
 // tiles); then the row's output is scaled in place once its last product is done.
@@ -26,10 +26,11 @@
 namespace ks {
 
 constexpr int KVW_SOFT = 256;                       // softmax threads (the first ones)
-constexpr int KVW_CONV = 256;                       // expanding threads (the last ones)
+constexpr int KVW_CONV_WARPS = 7;                   // expanding warps (the last ones): 16 in all, so that a
+constexpr int KVW_CONV = 32 * KVW_CONV_WARPS;       // thread has 128 registers
 constexpr int KVW_THREADS = KVW_SOFT + 32 + KVW_CONV;
 constexpr int KVW_UNITS = 8;                        // most units of the ring
-constexpr int KVW_HDR = 6144;
+constexpr int KVW_HDR = 12288;
 
 template <int D>
 constexpr int KVW_STREAM_OUT = D <= 128 ? 2 : 1;    // outputs in tensor memory
@@ -51,7 +52,8 @@ struct KvwShared {
   int abort;
   uint32_t info[8];           // of a tile: bits 0-7 groups of 16 keys that are not there, 8-15 values marked
   float m[128], l[128];       // of the second stream, for the first
-  uint32_t nan[128][8];
+  bool nans[128];
+  uint32_t nan[2][128][8];    // columns that are NaN of a row's output, where some are
 };
 static_assert(sizeof(KvwShared) <= KVW_HDR, "KvwShared exceeds its header");
 
@@ -81,7 +83,7 @@ __device__ __forceinline__ KvwUnit kvw_unit(int i, int n, bool two) {
 // Columns of the values that are NaN in positions that a row sees.
 template <int D>
 __device__ __noinline__ void kvw_nan_columns(const KvAttnParams& p, int b, int h, int len, int n, int t, int pos0,
-                                             int keys, uint32_t groups, uint32_t (&mask)[D / 32]) {
+                                             int keys, uint32_t groups, uint32_t* mask) {
   for (int g = 0; g < 8; ++g) {
     if (!((groups >> g) & 1u)) continue;
     const int at = pos0 + 16 * g, pi = kva_div(at, p.c.page, p.page_shift);
@@ -90,16 +92,41 @@ __device__ __noinline__ void kvw_nan_columns(const KvAttnParams& p, int b, int h
     for (int k = 0; k < 16 && at + k < keys; ++k) {
       if (!kva_sees(p, b, len, n, t, at + k)) continue;
       const uint32_t* w = reinterpret_cast<const uint32_t*>(base + k * D);
-#pragma unroll
       for (int i = 0; i < D / 32; ++i) {
         uint32_t bits = 0;
-#pragma unroll
         for (int j = 0; j < 8; ++j) bits |= kva_nan4_bits(__ldg(w + i * 8 + j)) << (4 * j);
         mask[i] |= bits;
       }
     }
   }
 }
+
+__device__ __forceinline__ void tmem_ld64(uint32_t taddr, float* x) {
+  uint32_t* r = reinterpret_cast<uint32_t*>(x);
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x64.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,"
+      "%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32,%33,%34,%35,%36,%37,%38,%39,%40,%41,%42,%43,%44,%45,%46,"
+      "%47,%48,%49,%50,%51,%52,%53,%54,%55,%56,%57,%58,%59,%60,%61,%62,%63}, [%64];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31]), "=r"(r[32]),
+        "=r"(r[33]), "=r"(r[34]), "=r"(r[35]), "=r"(r[36]), "=r"(r[37]), "=r"(r[38]), "=r"(r[39]), "=r"(r[40]),
+        "=r"(r[41]), "=r"(r[42]), "=r"(r[43]), "=r"(r[44]), "=r"(r[45]), "=r"(r[46]), "=r"(r[47]), "=r"(r[48]),
+        "=r"(r[49]), "=r"(r[50]), "=r"(r[51]), "=r"(r[52]), "=r"(r[53]), "=r"(r[54]), "=r"(r[55]), "=r"(r[56]),
+        "=r"(r[57]), "=r"(r[58]), "=r"(r[59]), "=r"(r[60]), "=r"(r[61]), "=r"(r[62]), "=r"(r[63])
+      : "r"(taddr));
+}
+
+__device__ __forceinline__ float kvw_max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+// Two e4m3 codes in the low bytes of two halves to bf16 2^-120 times as large: exponent and
+// mantissa move up by four bits and the sign by eight.  (As multiplications, which leave the
+// integer pipe to the softmax: shifts and masks there took 4 of every 10 of its cycles.)
+__device__ __forceinline__ uint32_t kvw_place(uint32_t x) { return (x & 0x00800080u) * 0xF0u + x * 16u; }
 
 __device__ __forceinline__ float2 kvw_fma2(float2 a, float2 b, float2 c) {
   float2 r;
@@ -134,7 +161,7 @@ __global__ void __launch_bounds__(KVW_THREADS, 1) kv_attn_wide_kernel(const __gr
 
   if (tid == 0) {
     for (int i = 0; i < UNITS; ++i) {
-      mbar_init(&sh->full[i], KVW_CONV / 32);
+      mbar_init(&sh->full[i], KVW_CONV_WARPS);
       mbar_init(&sh->free[i], 1);
     }
     for (int i = 0; i < 2; ++i) {
@@ -174,6 +201,9 @@ __global__ void __launch_bounds__(KVW_THREADS, 1) kv_attn_wide_kernel(const __gr
     // is ever waited for, and its parity tells it.
     uint32_t o_count[2] = {0, 0};
     bool first = true;
+    // the scale's sign goes into the queries; times 2^-149 instead of zero, unseen scores stay -inf
+    const uint32_t turn = p.scale_log2 < 0.f ? 0x80008000u : 0u;
+    const float scale = fmaxf(fabsf(p.scale_log2), __uint_as_float(1u));
     uint32_t item = 0, tiles_before = 0, pair_ph = 0;
     for (; w.left > 0; w.next(p)) {
       const int r0 = w.rt * p.nr;
@@ -206,7 +236,8 @@ __global__ void __launch_bounds__(KVW_THREADS, 1) kv_attn_wide_kernel(const __gr
             if (row < p.rows)
               x = __ldg(reinterpret_cast<const uint4*>(
                   p.q + (((int64_t)w.b * p.c.T + t) * p.H + w.h * p.G + (row - t * p.G)) * D + u * 8));
-            *reinterpret_cast<uint4*>(dst + (u >> 3) * 16384 + rr * 128 + (((u & 7) ^ (rr & 7)) << 4)) = x;
+            *reinterpret_cast<uint4*>(dst + (u >> 3) * 16384 + rr * 128 + (((u & 7) ^ (rr & 7)) << 4)) =
+                make_uint4(x.x ^ turn, x.y ^ turn, x.z ^ turn, x.w ^ turn);
           }
           fence_proxy_async_smem();
         }
@@ -225,9 +256,7 @@ __global__ void __launch_bounds__(KVW_THREADS, 1) kv_attn_wide_kernel(const __gr
       const int step = ONE_OUT || two ? 1 : 2;
       const bool idle = rows256 && !two && wg == 1;
       float m = -INFINITY, l = 0.f;
-      uint32_t nan[D / 32];
-#pragma unroll
-      for (int i = 0; i < D / 32; ++i) nan[i] = 0;
+      bool nans = false;  // sh->nan is in use
       int done = 0, last = wg;  // buffer of the last tile
       const uint32_t o_col = tmem + 256 + (ONE_OUT ? 0 : wg * D) + lanes;
       bool ok = true;
@@ -248,10 +277,7 @@ __global__ void __launch_bounds__(KVW_THREADS, 1) kv_attn_wide_kernel(const __gr
         const uint32_t info = sh->info[(tiles_before + j) & 7];
         const bool open = pos0 + 128 <= cl && (info & 255u) == 0;
         // ---------------------------------------------------------- maximum
-        // (a negative softmax scale makes the least product the largest score)
-        float top = -INFINITY;
         uint32_t see[4] = {~0u, ~0u, ~0u, ~0u};
-        const float sign = p.scale_log2 < 0.f ? -1.f : 1.f;
         if (!open) {
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
@@ -264,21 +290,32 @@ __global__ void __launch_bounds__(KVW_THREADS, 1) kv_attn_wide_kernel(const __gr
             if ((info >> (2 * c + 1)) & 1u) see[c] &= 0x0000FFFFu;
           }
         }
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          float x[32];
-          tmem_ld32(s_col + 32 * c, reinterpret_cast<uint32_t*>(x));
+        // half a row's scores at a time.  The second half stays in registers: its weights go where
+        // its last scores were, and the first half, read again, gets the columns before.
+        float x[64];
+        const auto read = [&](int half) {
+          tmem_ld64(s_col + 64 * half, x);
           tmem_wait_ld();
-          if (open && sign > 0.f) {
+          if (!open) {
+            const uint32_t lo = half ? see[2] : see[0], hi = half ? see[3] : see[1];
 #pragma unroll
-            for (int i = 0; i < 32; ++i) top = fmaxf(top, x[i]);
-          } else {
-#pragma unroll
-            for (int i = 0; i < 32; ++i)
-              if ((see[c] >> i) & 1u) top = fmaxf(top, x[i] * sign);
+            for (int i = 0; i < 64; ++i)
+              if (!(((i < 32 ? lo : hi) >> (i % 32)) & 1u)) x[i] = -INFINITY;
           }
+        };
+        float top = -INFINITY;
+#pragma unroll 1
+        for (int half = 0; half < 2; ++half) {
+          read(half);
+          float a = kvw_max3(x[0], x[1], x[2]), b = kvw_max3(x[3], x[4], x[5]);
+#pragma unroll
+          for (int i = 6; i < 62; i += 4) {
+            a = kvw_max3(a, x[i], x[i + 1]);
+            b = kvw_max3(b, x[i + 2], x[i + 3]);
+          }
+          top = kvw_max3(kvw_max3(a, x[62], x[63]), b, top);
         }
-        top = top == -INFINITY ? top : top * fabsf(p.scale_log2);
+        top = top == -INFINITY ? top : top * scale;
         // ---------------------------------------------------------- raise the reference
         if (__any_sync(0xFFFFFFFFu, top > m + KVA_RISE)) {
           const float now = fmaxf(m, top);
@@ -286,44 +323,40 @@ __global__ void __launch_bounds__(KVW_THREADS, 1) kv_attn_wide_kernel(const __gr
           m = now;
           l *= f;
           if (done > 0) {
-            ok = __all_sync(0xFFFFFFFFu, mbar_wait(&sh->o_done[last], (o_count[last] - 1) & 1, wc));
+            ok = __all_sync(0xFFFFFFFFu, mbar_wait_inl(&sh->o_done[last], (o_count[last] - 1) & 1, wc));
             if (!ok) break;
             tc_fence_after();
 #pragma unroll 1
-            for (int c = 0; c < D; c += 32) {
-              float x[32];
-              tmem_ld32(o_col + c, reinterpret_cast<uint32_t*>(x));
+            for (int c = 0; c < D; c += 16) {
+              float y[16];
+              tmem_ld16(o_col + c, reinterpret_cast<uint32_t*>(y));
               tmem_wait_ld();
 #pragma unroll
-              for (int i = 0; i < 32; ++i) x[i] *= f;
-              tmem_st16(o_col + c, reinterpret_cast<uint32_t*>(x));
-              tmem_st16(o_col + c + 16, reinterpret_cast<uint32_t*>(x) + 16);
+              for (int i = 0; i < 16; ++i) y[i] *= f;
+              tmem_st16(o_col + c, reinterpret_cast<uint32_t*>(y));
             }
             tmem_wait_st();
           }
         }
         // ---------------------------------------------------------- weights
         const float mu = (m == -INFINITY ? 0.f : m) + KVA_DOWN;
-        const float2 sc = make_float2(p.scale_log2, p.scale_log2), minus = make_float2(-mu, -mu);
+        const float2 sc = make_float2(scale, scale), minus = make_float2(-mu, -mu);
         float2 sum = make_float2(0.f, 0.f);
+#pragma unroll 1
+        for (int half = 1; half >= 0; --half) {
+          if (half == 0) read(0);
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          float x[32];
-          tmem_ld32(s_col + 32 * c, reinterpret_cast<uint32_t*>(x));
-          tmem_wait_ld();
-          uint32_t e[16];
+          for (int c = 0; c < 2; ++c) {
+            uint32_t e[16];
 #pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            float2 y = kvw_fma2(make_float2(x[2 * i], x[2 * i + 1]), sc, minus);
-            if (!open) {
-              if (!((see[c] >> (2 * i)) & 1u)) y.x = -INFINITY;
-              if (!((see[c] >> (2 * i + 1)) & 1u)) y.y = -INFINITY;
+            for (int i = 0; i < 16; ++i) {
+              float2 y = kvw_fma2(make_float2(x[32 * c + 2 * i], x[32 * c + 2 * i + 1]), sc, minus);
+              y = make_float2(kva_ex2(y.x), kva_ex2(y.y));
+              sum = kvw_add2(sum, y);
+              e[i] = cvt_bf16x2(y.x, y.y);
             }
-            y = make_float2(kva_ex2(y.x), kva_ex2(y.y));
-            sum = kvw_add2(sum, y);
-            e[i] = cvt_bf16x2(y.x, y.y);
+            tmem_st16(s_col + 64 + 32 * half + 16 * c, e);
           }
-          tmem_st16(s_col + 16 * c, e);
         }
         tmem_wait_st();
         tc_fence_before();
@@ -332,7 +365,12 @@ __global__ void __launch_bounds__(KVW_THREADS, 1) kv_attn_wide_kernel(const __gr
         ++o_count[buf];
         last = buf;
         l += sum.x + sum.y;
-        if (info >> 8) kvw_nan_columns<D>(p, w.b, w.h, w.len, w.n, tk, pos0, w.keys, info >> 8, nan);
+        if (info >> 8) {
+          if (!nans)
+            for (int i = 0; i < D / 32; ++i) sh->nan[wg][t128][i] = 0;
+          nans = true;
+          kvw_nan_columns<D>(p, w.b, w.h, w.len, w.n, tk, pos0, w.keys, info >> 8, sh->nan[wg][t128]);
+        }
       }
       if (!ok) break;
       tiles_before += n;
@@ -346,8 +384,7 @@ __global__ void __launch_bounds__(KVW_THREADS, 1) kv_attn_wide_kernel(const __gr
         if (wg == 1) {
           sh->m[t128] = m;
           sh->l[t128] = l;
-#pragma unroll
-          for (int i = 0; i < D / 32; ++i) sh->nan[t128][i] = nan[i];
+          sh->nans[t128] = nans;
           tc_fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive(&sh->pair_full);
@@ -369,8 +406,10 @@ __global__ void __launch_bounds__(KVW_THREADS, 1) kv_attn_wide_kernel(const __gr
           f1 = now == -INFINITY ? 1.f : kva_ex2(m1 - now);
           l = l * f0 + l1 * f1;
           m = now;
-#pragma unroll
-          for (int i = 0; i < D / 32; ++i) nan[i] |= sh->nan[t128][i];
+          if (sh->nans[t128]) {
+            for (int i = 0; i < D / 32; ++i) sh->nan[0][t128][i] = (nans ? sh->nan[0][t128][i] : 0u) | sh->nan[1][t128][i];
+            nans = true;
+          }
         }
         const bool whole = w.whole(), in = row < p.rows;
         const int g = row - tk * p.G;
@@ -379,7 +418,7 @@ __global__ void __launch_bounds__(KVW_THREADS, 1) kv_attn_wide_kernel(const __gr
           f = kva_norm(m, l, in && p.sink ? __ldg(p.sink + w.h * p.G + g) * 1.4426950408889634f : 0.f, in && p.sink);
         uint16_t* orow = p.out + (((int64_t)w.b * p.c.T + tk) * p.H + w.h * p.G + g) * D;
         const int64_t prow = (int64_t)w.slot() * p.nr + (row - r0);
-#pragma unroll
+#pragma unroll 1
         for (int c = 0; c < D; c += 32) {
           float x[32];
           tmem_ld32(o_col + c, reinterpret_cast<uint32_t*>(x));
@@ -391,10 +430,11 @@ __global__ void __launch_bounds__(KVW_THREADS, 1) kv_attn_wide_kernel(const __gr
 #pragma unroll
             for (int i = 0; i < 32; ++i) x[i] = x[i] * f0 + y[i] * f1;
           }
-          if (nan[c / 32]) {
+          if (nans) {
+            const uint32_t nan = sh->nan[wg][t128][c / 32];
 #pragma unroll
             for (int i = 0; i < 32; ++i)
-              if ((nan[c / 32] >> i) & 1u) x[i] = __uint_as_float(0x7FC00000u);
+              if ((nan >> i) & 1u) x[i] = __uint_as_float(0x7FC00000u);
           }
           if (whole) {
             if (in) {
@@ -454,7 +494,7 @@ __global__ void __launch_bounds__(KVW_THREADS, 1) kv_attn_wide_kernel(const __gr
         const uint32_t b = smem_u32(ring + slot * TILE);
 #pragma unroll
         for (int ks = 0; ks < 8; ++ks)
-          kvw_mma_ts(tmem + 256 + out * D, tmem + buf * 128 + ks * 8, sdesc_sw128(b + ks * 2048, 16384, 1024), idesc_o,
+          kvw_mma_ts(tmem + 256 + out * D, tmem + buf * 128 + 64 + ks * 8, sdesc_sw128(b + ks * 2048, 16384, 1024), idesc_o,
                      acc || ks > 0);
         umma_commit(&sh->o_done[buf]);
       }
@@ -531,9 +571,17 @@ __global__ void __launch_bounds__(KVW_THREADS, 1) kv_attn_wide_kernel(const __gr
     mbar_wait(&sh->drain, 0, wc, false, true);
   } else {
     // -------------------------------------------------------------- keys and values
-    constexpr int P16 = D / 16;                    // 16-code pieces of a row
-    constexpr int NP = 128 * P16 / KVW_CONV;       // pieces of a thread per unit
-    const int ct = tid - (KVW_SOFT + 32), cw = ct >> 5;
+    // A warp takes KEYS keys of 16-code pieces at a time, every KVW_CONV_WARPS-th such step of a unit.
+    // Codes are loaded AHEAD steps before they are expanded, into the registers just used.
+    constexpr int P16 = D / 16, KEYS = D == 64 ? 8 : D == 128 ? 4 : 2;
+    constexpr int STEPS = 128 / KEYS, NP = (STEPS + KVW_CONV_WARPS - 1) / KVW_CONV_WARPS;
+    constexpr int AHEAD = NP > 5 ? 5 : NP;
+    static_assert(NP % AHEAD == 0, "whole rounds");
+    // lane's key and piece: eight lanes that store together have four pieces of two keys, whose
+    // swizzles differ in the lowest bit, so they meet no bank twice
+    const int cw = warp - 9, k0 = D == 64 ? lane >> 2 : ((lane >> 2) & 1) + (D == 128 ? 2 * (lane >> 4) : 0);
+    const int c = D == 64 ? lane & 3 : (lane & 3) + 4 * (D == 128 ? (lane >> 3) & 1 : lane >> 3);
+    const bool on = c < P16;                       // (D = 192: 24 lanes of a warp)
     const int per_page = p.c.page / p.c.block;
     uint32_t unit = 0, tiles_before = 0;
     bool ok = true;
@@ -541,107 +589,127 @@ __global__ void __launch_bounds__(KVW_THREADS, 1) kv_attn_wide_kernel(const __gr
       if (!w.any()) continue;
       const int n = w.t1 - w.t0;
       const bool two = rows256 && w.rt * 256 + 128 < p.rows;
-      // lanes 0-7: a group of 16 keys of the tile each
-      struct Group {
-        int64_t row;      // of the page pool's rows of heads
-        uint32_t scale;   // bits, 0: not there
+      // what is known of a unit; lanes 0-7 have a group of 16 of its keys each
+      struct Unit {
+        KvwUnit u;
+        uint32_t place;           // of the group, in 16 rows
+        uint32_t scale, v_scale;  // bits of its scale (keys: and of the values'); 0: not there
+        uint32_t gone;            // groups that are not there
       };
       const auto page_of = [&](int tile) {
         const int pos = (w.t0 + tile) * 128 + 16 * lane;
         return lane < 8 && tile < n && pos < w.keys
                    ? __ldg(p.c.table + (int64_t)w.b * p.c.max_pages + kva_div(pos, p.c.page, p.page_shift)) : -2;
       };
-      uint32_t info_next = 0;
-      const auto locate = [&](const KvwUnit& u, int pg, Group* g) {
-        const int pos = (w.t0 + u.tile) * 128 + 16 * lane;
-        const bool ok_pg = pg >= 0 && pg < p.c.n_pages;
-        if (pg != -2 && !ok_pg && cw == 0) report_bounds(p.c.status, w.b, (int)p.c.n_pages);
-        const int in = ok_pg ? pos - kva_div(pos, p.c.page, p.page_shift) * p.c.page : 0;
-        const int64_t at = (int64_t)(ok_pg ? pg : 0) * p.c.heads + w.h;
-        g->row = at * p.c.page + in;
+      int pg0 = page_of(0), pg1 = page_of(1);  // page numbers of the tiles to come, by tile parity
+      const auto locate = [&](int i, Unit& a) {
+        a.u = kvw_unit(i, n, two);
+        const int page = (a.u.tile & 1) ? pg1 : pg0, pos = (w.t0 + a.u.tile) * 128 + 16 * lane;
+        const bool there = page >= 0 && page < p.c.n_pages;
+        if (page != -2 && !there && cw == 0) report_bounds(p.c.status, w.b, (int)p.c.n_pages);
+        const int in = there ? pos - kva_div(pos, p.c.page, p.page_shift) * p.c.page : 0;
+        const int64_t at = (int64_t)(there ? page : 0) * p.c.heads + w.h;
+        a.place = (uint32_t)(at * (p.c.page >> 4) + (in >> 4));
         const int64_t si = at * per_page + kva_div(in, p.c.block, p.block_shift);
-        const uint32_t vs = ok_pg ? __float_as_uint(__ldg(p.c.v_scale + si)) : 0u;
-        if (u.v) {
-          g->scale = vs;
-        } else {
-          g->scale = ok_pg ? __float_as_uint(__ldg(p.c.k_scale + si)) : 0u;
-          info_next = (__ballot_sync(0xFFFFFFFFu, !ok_pg) & 255u) | (__ballot_sync(0xFFFFFFFFu, ok_pg && (vs & 1u)) & 255u) << 8;
+        a.scale = a.v_scale = 0;
+        if (there) {
+          a.v_scale = __float_as_uint(__ldg(p.c.v_scale + si));
+          if (!a.u.v) a.scale = __float_as_uint(__ldg(p.c.k_scale + si));
+        }
+        a.gone = __ballot_sync(0xFFFFFFFFu, !there) & 255u;
+        if (a.u.v) {  // a tile's values come after its keys
+          if (a.u.tile & 1) pg1 = page_of(a.u.tile + 2);
+          else pg0 = page_of(a.u.tile + 2);
         }
       };
-      uint32_t code[NP][4];
-      const auto load = [&](const KvwUnit& u, const Group& g) {
-        const uint8_t* src = u.v ? p.c.v8 : p.c.k8;
+      uint32_t code[AHEAD][4];
+      const auto load = [&](int q, const Unit& a, uint32_t (&v)[4]) {
+        const int step = cw + q * KVW_CONV_WARPS, key = step * KEYS;
+        const uint32_t row16 = __shfl_sync(0xFFFFFFFFu, a.place, (key >> 4) & 7);
+        const uint8_t* src = (a.u.v ? p.c.v8 : p.c.k8) + (k0 * D + c * 16);
+        if (step < STEPS && on) kvf_load<4>(v, src + (int64_t)row16 * (16 * D) + (key & 15) * D);
+      };
+      Unit cur, nxt;
+      locate(0, cur);
 #pragma unroll
-        for (int i = 0; i < NP; ++i) {
-          const int e = ct + i * KVW_CONV, key = e / P16, c = e - key * P16;
-          const int64_t row = __shfl_sync(0xFFFFFFFFu, g.row, key >> 4);
-          kvf_load<4>(code[i], src + (row + (key & 15)) * D + c * 16);
-        }
-      };
-      KvwUnit u = kvw_unit(0, n, two), v{};
-      // page numbers of the tiles to come, by tile parity
-      int pg[2] = {page_of(0), page_of(1)};
-      Group g{}, gn{};
-      locate(u, pg[0], &g);
-      uint32_t info = info_next;
-      load(u, g);
+      for (int q = 0; q < AHEAD; ++q) load(q, cur, code[q]);
+      locate(1, nxt);
       for (int i = 0; i < 2 * n; ++i) {
         const uint32_t slot = (unit + i) % UNITS, ph = ((unit + i) / UNITS) & 1;
         if (unit + i >= UNITS) {
           ok = __all_sync(0xFFFFFFFFu, mbar_wait_inl(&sh->free[slot], ph ^ 1, wc));
           if (!ok) break;
         }
-        uint8_t* dst = ring + slot * TILE;
         const bool more = i + 1 < 2 * n;
-        if (more) {
-          v = kvw_unit(i + 1, n, two);
-          locate(v, pg[v.tile & 1], &gn);
-          if (v.v) pg[v.tile & 1] = page_of(v.tile + 2);  // a tile's values come after its keys
-        }
-#pragma unroll
-        for (int q = 0; q < NP; ++q) {
-          const int e = ct + q * KVW_CONV, key = e / P16, c = e - key * P16;
-          const uint32_t sb = __shfl_sync(0xFFFFFFFFu, g.scale, key >> 4);
-          float rest;
-          const uint32_t f = kva_factor(sb, &rest);
-          uint32_t x[8];
+        const uint32_t scale = cur.u.v ? cur.v_scale : cur.scale;
+        float rest;
+        const uint32_t factor = kva_factor(scale, &rest);
+        const bool plain = !__any_sync(0xFFFFFFFFu, rest != 1.f || (scale & 1u));
+        uint8_t* dst = ring + slot * TILE + (c >> 2) * 16384;
+        const auto store = [&](int key, const uint32_t (&x)[8]) {
+          uint8_t* at = dst + key * 128;
+          const int b = 2 * (c & 3);
+          *reinterpret_cast<uint4*>(at + ((b ^ (key & 7)) << 4)) = make_uint4(x[0], x[1], x[2], x[3]);
+          *reinterpret_cast<uint4*>(at + (((b + 1) ^ (key & 7)) << 4)) = make_uint4(x[4], x[5], x[6], x[7]);
+        };
+        const auto expand = [&](const uint32_t (&v)[4], uint32_t f, uint32_t (&x)[8]) {
 #pragma unroll
           for (int h = 0; h < 4; ++h) {
-            const uint32_t wd = code[q][h];
-            x[2 * h] = mul_bf16x2(kva_place(__byte_perm(wd, 0, 0x1404)), f);
-            x[2 * h + 1] = mul_bf16x2(kva_place(__byte_perm(wd, 0, 0x3424)), f);
+            x[2 * h] = mul_bf16x2(kvw_place(__byte_perm(v[h], 0, 0x4140)), f);
+            x[2 * h + 1] = mul_bf16x2(kvw_place(__byte_perm(v[h], 0, 0x4342)), f);
           }
-          if (rest != 1.f || (sb & 1u)) {
-            const uint32_t r2 = cvt_bf16x2(rest, rest);
+        };
+        if (plain) {
+#pragma unroll
+          for (int q = 0; q < NP; ++q) {
+            const int step = cw + q * KVW_CONV_WARPS;
+            uint32_t x[8];
+            expand(code[q % AHEAD], __shfl_sync(0xFFFFFFFFu, factor, (step * KEYS >> 4) & 7), x);
+            if (step < STEPS && on) store(step * KEYS + k0, x);
+            if (q + AHEAD < NP) load(q + AHEAD, cur, code[q % AHEAD]);
+            else if (more) load(q + AHEAD - NP, nxt, code[q % AHEAD]);
+          }
+        } else {
+          // large scales and marked blocks: rare, and read (again) one step at a time
+#pragma unroll 1
+          for (int q = 0; q < NP; ++q) {
+            const int step = cw + q * KVW_CONV_WARPS;
+            uint32_t v[4] = {0, 0, 0, 0}, x[8];
+            load(q, cur, v);
+            expand(v, __shfl_sync(0xFFFFFFFFu, factor, (step * KEYS >> 4) & 7), x);
+            const uint32_t sb = __shfl_sync(0xFFFFFFFFu, scale, (step * KEYS >> 4) & 7);
+            float r1;
+            kva_factor(sb, &r1);
+            const uint32_t r2 = cvt_bf16x2(r1, r1);
 #pragma unroll
             for (int h = 0; h < 4; ++h) {
-              const uint32_t bits = (sb & 1u) ? kva_nan4_bits(code[q][h]) : 0u;
+              const uint32_t bits = (sb & 1u) ? kva_nan4_bits(v[h]) : 0u;
 #pragma unroll
               for (int y = 0; y < 2; ++y) {
                 uint32_t z = mul_bf16x2(x[2 * h + y], r2);
                 // a key's NaN goes into the scores, a value's is put into the outputs at the end
-                const uint32_t nan = u.v ? 0u : 0x7FC0u;
+                const uint32_t nan = cur.u.v ? 0u : 0x7FC0u;
                 if ((bits >> (2 * y)) & 1u) z = (z & 0xFFFF0000u) | nan;
                 if ((bits >> (2 * y + 1)) & 1u) z = (z & 0x0000FFFFu) | nan << 16;
                 x[2 * h + y] = z;
               }
             }
+            if (step < STEPS && on) store(step * KEYS + k0, x);
           }
-          // (neighbouring lanes' halves the other way round: no two of a phase meet a bank)
-          uint8_t* at = dst + (c >> 2) * 16384 + key * 128;
-          const int a = 2 * (c & 3), flip = (c >> 2) & 1;
-          const uint4 lo = make_uint4(x[0], x[1], x[2], x[3]), hi = make_uint4(x[4], x[5], x[6], x[7]);
-          *reinterpret_cast<uint4*>(at + (((a + flip) ^ (key & 7)) << 4)) = flip ? hi : lo;
-          *reinterpret_cast<uint4*>(at + (((a + 1 - flip) ^ (key & 7)) << 4)) = flip ? lo : hi;
+          if (more) {
+#pragma unroll
+            for (int q = 0; q < AHEAD; ++q) load(q, nxt, code[q]);
+          }
         }
-        if (!u.v && cw == 0 && lane == 0) sh->info[(tiles_before + u.tile) & 7] = info;
-        if (more) load(v, gn);
+        if (!cur.u.v && cw == 0) {
+          const uint32_t marks = __ballot_sync(0xFFFFFFFFu, cur.v_scale & 1u) & 255u;
+          if (lane == 0) sh->info[(tiles_before + cur.u.tile) & 7] = cur.gone | marks << 8;
+        }
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(&sh->full[slot]);
-        u = v;
-        g = gn;
-        info = info_next;
+        cur = nxt;
+        if (i + 2 < 2 * n) locate(i + 2, nxt);
       }
       unit += 2 * n;
       tiles_before += n;
