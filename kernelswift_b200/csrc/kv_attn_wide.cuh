@@ -15,8 +15,11 @@
 //   D > 128 (tensor memory holds one output): even and odd tiles, one output; one warpgroup does
 //     the softmax of both in turn.
 // Warps: 0-3 and 4-7 softmax (thread = row = TMEM lane), also queries and results; 8 issues the
-// products; 9-15 load and expand.  Codes are loaded a unit (the keys or the values of a tile) ahead;
-// units lie in a ring in the order the products take them.
+// products; 9 walks the page table and the scales; 10-16 and 17-23 load and expand, every other
+// unit (the keys or the values of a tile) each.  Units lie in a ring in the order the products
+// take them; a warp's codes are loaded a unit of its own ahead, into the registers just used.
+// (Expansion is a chain of latencies: with seven warps that also found the addresses themselves it
+// took 3700 cycles a unit, two units a tile, and was what everything waited for.)
 //
 // References are raised only when a score passes them by 2^KVA_RISE (rarely after the first
 // tiles); then the row's output is scaled in place once its last product is done.
@@ -26,9 +29,12 @@
 namespace ks {
 
 constexpr int KVW_SOFT = 256;                       // softmax threads (the first ones)
-constexpr int KVW_CONV_WARPS = 7;                   // expanding warps (the last ones): 16 in all, so that a
-constexpr int KVW_CONV = 32 * KVW_CONV_WARPS;       // thread has 128 registers
-constexpr int KVW_THREADS = KVW_SOFT + 32 + KVW_CONV;
+constexpr int KVW_CONV_WARPS = 7;                   // of either group of expanding warps (the last ones)
+constexpr int KVW_THREADS = KVW_SOFT + 64 + 2 * 32 * KVW_CONV_WARPS;
+// 768 threads start with 80 registers; the softmax warpgroups take theirs from the other four.
+constexpr int KVW_REGS_SOFT = 128, KVW_REGS_REST = 56;
+static_assert(KVW_THREADS == 768 && 2 * KVW_REGS_SOFT + 4 * KVW_REGS_REST <= 6 * 80, "register split");
+constexpr int KVW_META = 8;                         // units whose addresses are held
 constexpr int KVW_UNITS = 8;                        // most units of the ring
 constexpr int KVW_HDR = 12288;
 
@@ -42,15 +48,25 @@ __host__ __device__ constexpr int kvw_units() {
   return n < KVW_UNITS ? n : KVW_UNITS;
 }
 
+struct KvwMeta {
+  uint32_t place[8];          // of the unit's groups of 16 keys, in 16 rows of the page pool
+  uint32_t scale[8];          // their scales' bits, 0: not there
+  uint32_t factor[8];         // 2^120 times those, twice
+  uint32_t flags;
+};
+enum : uint32_t { KVW_VALUES = 1, KVW_PLAIN = 2, KVW_END = 4 };  // PLAIN: no larger scale, no mark
+
 struct KvwShared {
   KvaFind find;
+  KvwMeta meta[KVW_META];
+  uint64_t meta_full[KVW_META], meta_free[KVW_META];
   uint64_t full[KVW_UNITS], free[KVW_UNITS];
   uint64_t s_full[2], p_full[2], o_done[2];
   uint64_t q_full, q_free, drain;
   uint64_t pair_full, pair_free;  // the second stream's results are there / have been taken
   uint32_t tmem;
   int abort;
-  uint32_t info[8];           // of a tile: bits 0-7 groups of 16 keys that are not there, 8-15 values marked
+  uint32_t info[16];          // of a tile: bits 0-7 groups of 16 keys that are not there, 8-15 values marked
   float m[128], l[128];       // of the second stream, for the first
   bool nans[128];
   uint32_t nan[2][128][8];    // columns that are NaN of a row's output, where some are
@@ -82,7 +98,7 @@ __device__ __forceinline__ KvwUnit kvw_unit(int i, int n, bool two) {
 
 // Columns of the values that are NaN in positions that a row sees.
 template <int D>
-__device__ __noinline__ void kvw_nan_columns(const KvAttnParams& p, int b, int h, int len, int n, int t, int pos0,
+__device__ __forceinline__ void kvw_nan_columns(const KvAttnParams& p, int b, int h, int len, int n, int t, int pos0,
                                              int keys, uint32_t groups, uint32_t* mask) {
   for (int g = 0; g < 8; ++g) {
     if (!((groups >> g) & 1u)) continue;
@@ -99,23 +115,6 @@ __device__ __noinline__ void kvw_nan_columns(const KvAttnParams& p, int b, int h
       }
     }
   }
-}
-
-__device__ __forceinline__ void tmem_ld64(uint32_t taddr, float* x) {
-  uint32_t* r = reinterpret_cast<uint32_t*>(x);
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x64.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,"
-      "%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32,%33,%34,%35,%36,%37,%38,%39,%40,%41,%42,%43,%44,%45,%46,"
-      "%47,%48,%49,%50,%51,%52,%53,%54,%55,%56,%57,%58,%59,%60,%61,%62,%63}, [%64];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
-        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
-        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31]), "=r"(r[32]),
-        "=r"(r[33]), "=r"(r[34]), "=r"(r[35]), "=r"(r[36]), "=r"(r[37]), "=r"(r[38]), "=r"(r[39]), "=r"(r[40]),
-        "=r"(r[41]), "=r"(r[42]), "=r"(r[43]), "=r"(r[44]), "=r"(r[45]), "=r"(r[46]), "=r"(r[47]), "=r"(r[48]),
-        "=r"(r[49]), "=r"(r[50]), "=r"(r[51]), "=r"(r[52]), "=r"(r[53]), "=r"(r[54]), "=r"(r[55]), "=r"(r[56]),
-        "=r"(r[57]), "=r"(r[58]), "=r"(r[59]), "=r"(r[60]), "=r"(r[61]), "=r"(r[62]), "=r"(r[63])
-      : "r"(taddr));
 }
 
 __device__ __forceinline__ float kvw_max3(float a, float b, float c) {
@@ -164,6 +163,10 @@ __global__ void __launch_bounds__(KVW_THREADS, 1) kv_attn_wide_kernel(const __gr
       mbar_init(&sh->full[i], KVW_CONV_WARPS);
       mbar_init(&sh->free[i], 1);
     }
+    for (int i = 0; i < KVW_META; ++i) {
+      mbar_init(&sh->meta_full[i], 1);
+      mbar_init(&sh->meta_free[i], KVW_CONV_WARPS);
+    }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&sh->s_full[i], 1);
       mbar_init(&sh->p_full[i], 4);
@@ -193,6 +196,7 @@ __global__ void __launch_bounds__(KVW_THREADS, 1) kv_attn_wide_kernel(const __gr
 
   if (warp < 8) {
     // -------------------------------------------------------------- softmax
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(KVW_REGS_SOFT));
     const int wg = warp >> 2, t128 = tid & 127;
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
     uint32_t s_ph[2] = {0, 0};  // phases of the score buffers
@@ -222,7 +226,7 @@ __global__ void __launch_bounds__(KVW_THREADS, 1) kv_attn_wide_kernel(const __gr
       const bool two = rows256 && r0 + 128 < p.rows;  // both streams on every tile
       // ------------------------------------------------------------ queries
       if (!first) {
-        if (!mbar_wait(&sh->q_free, (item - 1) & 1, wc)) break;
+        if (!mbar_wait_inl(&sh->q_free, (item - 1) & 1, wc)) break;
       }
       first = false;
       if (!ONE_OUT || wg == 0) {
@@ -269,12 +273,12 @@ __global__ void __launch_bounds__(KVW_THREADS, 1) kv_attn_wide_kernel(const __gr
       for (int j = step == 2 ? wg : 0; j < n; j += step, ++done) {
         const int buf = ONE_OUT ? (j & 1) : wg;
         const uint32_t s_col = tmem + buf * 128 + lanes;
-        ok = __all_sync(0xFFFFFFFFu, mbar_wait(&sh->s_full[buf], s_ph[buf], wc));
+        ok = __all_sync(0xFFFFFFFFu, mbar_wait_inl(&sh->s_full[buf], s_ph[buf], wc));
         if (!ok) break;
         s_ph[buf] ^= 1;
         tc_fence_after();
         const int pos0 = (w.t0 + j) * 128;
-        const uint32_t info = sh->info[(tiles_before + j) & 7];
+        const uint32_t info = sh->info[(tiles_before + j) & 15];
         const bool open = pos0 + 128 <= cl && (info & 255u) == 0;
         // ---------------------------------------------------------- maximum
         uint32_t see[4] = {~0u, ~0u, ~0u, ~0u};
@@ -294,7 +298,8 @@ __global__ void __launch_bounds__(KVW_THREADS, 1) kv_attn_wide_kernel(const __gr
         // its last scores were, and the first half, read again, gets the columns before.
         float x[64];
         const auto read = [&](int half) {
-          tmem_ld64(s_col + 64 * half, x);
+          tmem_ld32(s_col + 64 * half, reinterpret_cast<uint32_t*>(x));
+          tmem_ld32(s_col + 64 * half + 32, reinterpret_cast<uint32_t*>(x + 32));
           tmem_wait_ld();
           if (!open) {
             const uint32_t lo = half ? see[2] : see[0], hi = half ? see[3] : see[1];
@@ -376,7 +381,7 @@ __global__ void __launch_bounds__(KVW_THREADS, 1) kv_attn_wide_kernel(const __gr
       tiles_before += n;
       // ------------------------------------------------------------ results
       if (done > 0) {
-        ok = __all_sync(0xFFFFFFFFu, mbar_wait(&sh->o_done[last], (o_count[last] - 1) & 1, wc));
+        ok = __all_sync(0xFFFFFFFFu, mbar_wait_inl(&sh->o_done[last], (o_count[last] - 1) & 1, wc));
         tc_fence_after();
       }
       if (!ONE_OUT && !two) {
@@ -389,9 +394,9 @@ __global__ void __launch_bounds__(KVW_THREADS, 1) kv_attn_wide_kernel(const __gr
           __syncwarp();
           if (lane == 0) mbar_arrive(&sh->pair_full);
           // its output is the first warpgroup's to read until here
-          ok = ok && __all_sync(0xFFFFFFFFu, mbar_wait(&sh->pair_free, pair_ph, wc));
+          ok = ok && __all_sync(0xFFFFFFFFu, mbar_wait_inl(&sh->pair_free, pair_ph, wc));
         } else {
-          ok = ok && __all_sync(0xFFFFFFFFu, mbar_wait(&sh->pair_full, pair_ph, wc));
+          ok = ok && __all_sync(0xFFFFFFFFu, mbar_wait_inl(&sh->pair_full, pair_ph, wc));
           tc_fence_after();
         }
         pair_ph ^= 1;
@@ -467,13 +472,14 @@ __global__ void __launch_bounds__(KVW_THREADS, 1) kv_attn_wide_kernel(const __gr
     }
   } else if (warp == 8) {
     // -------------------------------------------------------------- products
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(KVW_REGS_REST));
     const bool leader = elect_one();
     uint32_t unit = 0, q_ph = 0, p_ph[2] = {0, 0};
     constexpr uint32_t idesc_s = idesc_bf16_f32(128, 128, false, false);
     constexpr uint32_t idesc_o = idesc_bf16_f32(128, D, false, true);
     bool ok = true;
     const auto wait = [&](uint64_t* bar, uint32_t ph) {
-      ok = ok && __all_sync(0xFFFFFFFFu, mbar_wait(bar, ph, wc));
+      ok = ok && __all_sync(0xFFFFFFFFu, mbar_wait_inl(bar, ph, wc));
       tc_fence_after();
       return ok;
     };
@@ -568,151 +574,193 @@ __global__ void __launch_bounds__(KVW_THREADS, 1) kv_attn_wide_kernel(const __gr
     }
     // every product and arrival in flight has landed before the CTA gives its memory back
     commit(&sh->drain);
-    mbar_wait(&sh->drain, 0, wc, false, true);
-  } else {
-    // -------------------------------------------------------------- keys and values
-    // A warp takes KEYS keys of 16-code pieces at a time, every KVW_CONV_WARPS-th such step of a unit.
-    // Codes are loaded AHEAD steps before they are expanded, into the registers just used.
-    constexpr int P16 = D / 16, KEYS = D == 64 ? 8 : D == 128 ? 4 : 2;
-    constexpr int STEPS = 128 / KEYS, NP = (STEPS + KVW_CONV_WARPS - 1) / KVW_CONV_WARPS;
-    constexpr int AHEAD = NP > 5 ? 5 : NP;
-    static_assert(NP % AHEAD == 0, "whole rounds");
-    // lane's key and piece: eight lanes that store together have four pieces of two keys, whose
-    // swizzles differ in the lowest bit, so they meet no bank twice
-    const int cw = warp - 9, k0 = D == 64 ? lane >> 2 : ((lane >> 2) & 1) + (D == 128 ? 2 * (lane >> 4) : 0);
-    const int c = D == 64 ? lane & 3 : (lane & 3) + 4 * (D == 128 ? (lane >> 3) & 1 : lane >> 3);
-    const bool on = c < P16;                       // (D = 192: 24 lanes of a warp)
-    const int per_page = p.c.page / p.c.block;
+    mbar_wait_body(&sh->drain, 0, wc, false, true);
+  } else if (warp == 9) {
+    // -------------------------------------------------------------- addresses
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(KVW_REGS_REST));
+    const uint32_t per_page = (uint32_t)(p.c.page / p.c.block), page16 = (uint32_t)(p.c.page >> 4);
     uint32_t unit = 0, tiles_before = 0;
     bool ok = true;
+    // a unit whose scales are on their way; lanes 0-7: a group of 16 of its keys each
+    struct Unit {
+      uint32_t place, scale, v_scale, gone;
+      int tile;  // of all
+      bool v;
+    } last{};
+    const auto publish = [&](const Unit& a, uint32_t u) {
+      const uint32_t slot = u % KVW_META;
+      if (u >= KVW_META) ok = ok && __all_sync(0xFFFFFFFFu, mbar_wait_inl(&sh->meta_free[slot], ((u / KVW_META) & 1) ^ 1, wc));
+      if (!ok) return;
+      KvwMeta& m = sh->meta[slot];
+      float rest;
+      const uint32_t scale = a.v ? a.v_scale : a.scale, factor = kva_factor(scale, &rest);
+      const bool plain = !__any_sync(0xFFFFFFFFu, rest != 1.f || (scale & 1u));
+      const uint32_t marks = __ballot_sync(0xFFFFFFFFu, a.v_scale & 1u) & 255u;
+      if (lane < 8) {
+        m.place[lane] = a.place;
+        m.scale[lane] = scale;
+        m.factor[lane] = factor;
+      }
+      if (lane == 0) {
+        m.flags = (a.v ? KVW_VALUES : 0u) | (plain ? KVW_PLAIN : 0u);
+        if (!a.v) sh->info[a.tile & 15] = a.gone | marks << 8;
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sh->meta_full[slot]);
+    };
     for (; w.left > 0 && ok; w.next(p)) {
       if (!w.any()) continue;
       const int n = w.t1 - w.t0;
       const bool two = rows256 && w.rt * 256 + 128 < p.rows;
-      // what is known of a unit; lanes 0-7 have a group of 16 of its keys each
-      struct Unit {
-        KvwUnit u;
-        uint32_t place;           // of the group, in 16 rows
-        uint32_t scale, v_scale;  // bits of its scale (keys: and of the values'); 0: not there
-        uint32_t gone;            // groups that are not there
-      };
       const auto page_of = [&](int tile) {
         const int pos = (w.t0 + tile) * 128 + 16 * lane;
         return lane < 8 && tile < n && pos < w.keys
                    ? __ldg(p.c.table + (int64_t)w.b * p.c.max_pages + kva_div(pos, p.c.page, p.page_shift)) : -2;
       };
       int pg0 = page_of(0), pg1 = page_of(1);  // page numbers of the tiles to come, by tile parity
-      const auto locate = [&](int i, Unit& a) {
-        a.u = kvw_unit(i, n, two);
-        const int page = (a.u.tile & 1) ? pg1 : pg0, pos = (w.t0 + a.u.tile) * 128 + 16 * lane;
+      for (int i = 0; i < 2 * n && ok; ++i) {
+        const KvwUnit u = kvw_unit(i, n, two);
+        const int page = (u.tile & 1) ? pg1 : pg0, pos = (w.t0 + u.tile) * 128 + 16 * lane;
         const bool there = page >= 0 && page < p.c.n_pages;
-        if (page != -2 && !there && cw == 0) report_bounds(p.c.status, w.b, (int)p.c.n_pages);
-        const int in = there ? pos - kva_div(pos, p.c.page, p.page_shift) * p.c.page : 0;
-        const int64_t at = (int64_t)(there ? page : 0) * p.c.heads + w.h;
-        a.place = (uint32_t)(at * (p.c.page >> 4) + (in >> 4));
-        const int64_t si = at * per_page + kva_div(in, p.c.block, p.block_shift);
-        a.scale = a.v_scale = 0;
+        if (page != -2 && !there) report_bounds(p.c.status, w.b, (int)p.c.n_pages);
+        const uint32_t in = there ? (uint32_t)(pos - kva_div(pos, p.c.page, p.page_shift) * p.c.page) : 0u;
+        const uint32_t at = (there ? (uint32_t)page : 0u) * (uint32_t)p.c.heads + (uint32_t)w.h;
+        Unit now;
+        now.place = at * page16 + (in >> 4);  // (the host has checked that it fits)
+        const uint32_t si = at * per_page + (uint32_t)kva_div((int)in, p.c.block, p.block_shift);
+        now.scale = now.v_scale = 0;
         if (there) {
-          a.v_scale = __float_as_uint(__ldg(p.c.v_scale + si));
-          if (!a.u.v) a.scale = __float_as_uint(__ldg(p.c.k_scale + si));
+          now.v_scale = __float_as_uint(__ldg(p.c.v_scale + si));
+          if (!u.v) now.scale = __float_as_uint(__ldg(p.c.k_scale + si));
         }
-        a.gone = __ballot_sync(0xFFFFFFFFu, !there) & 255u;
-        if (a.u.v) {  // a tile's values come after its keys
-          if (a.u.tile & 1) pg1 = page_of(a.u.tile + 2);
-          else pg0 = page_of(a.u.tile + 2);
+        now.gone = __ballot_sync(0xFFFFFFFFu, !there) & 255u;
+        now.tile = (int)tiles_before + u.tile;
+        now.v = u.v;
+        if (u.v) {  // a tile's values come after its keys
+          if (u.tile & 1) pg1 = page_of(u.tile + 2);
+          else pg0 = page_of(u.tile + 2);
         }
-      };
-      uint32_t code[AHEAD][4];
-      const auto load = [&](int q, const Unit& a, uint32_t (&v)[4]) {
-        const int step = cw + q * KVW_CONV_WARPS, key = step * KEYS;
-        const uint32_t row16 = __shfl_sync(0xFFFFFFFFu, a.place, (key >> 4) & 7);
-        const uint8_t* src = (a.u.v ? p.c.v8 : p.c.k8) + (k0 * D + c * 16);
-        if (step < STEPS && on) kvf_load<4>(v, src + (int64_t)row16 * (16 * D) + (key & 15) * D);
-      };
-      Unit cur, nxt;
-      locate(0, cur);
-#pragma unroll
-      for (int q = 0; q < AHEAD; ++q) load(q, cur, code[q]);
-      locate(1, nxt);
-      for (int i = 0; i < 2 * n; ++i) {
-        const uint32_t slot = (unit + i) % UNITS, ph = ((unit + i) / UNITS) & 1;
-        if (unit + i >= UNITS) {
-          ok = __all_sync(0xFFFFFFFFu, mbar_wait_inl(&sh->free[slot], ph ^ 1, wc));
-          if (!ok) break;
-        }
-        const bool more = i + 1 < 2 * n;
-        const uint32_t scale = cur.u.v ? cur.v_scale : cur.scale;
-        float rest;
-        const uint32_t factor = kva_factor(scale, &rest);
-        const bool plain = !__any_sync(0xFFFFFFFFu, rest != 1.f || (scale & 1u));
-        uint8_t* dst = ring + slot * TILE + (c >> 2) * 16384;
-        const auto store = [&](int key, const uint32_t (&x)[8]) {
-          uint8_t* at = dst + key * 128;
-          const int b = 2 * (c & 3);
-          *reinterpret_cast<uint4*>(at + ((b ^ (key & 7)) << 4)) = make_uint4(x[0], x[1], x[2], x[3]);
-          *reinterpret_cast<uint4*>(at + (((b + 1) ^ (key & 7)) << 4)) = make_uint4(x[4], x[5], x[6], x[7]);
-        };
-        const auto expand = [&](const uint32_t (&v)[4], uint32_t f, uint32_t (&x)[8]) {
-#pragma unroll
-          for (int h = 0; h < 4; ++h) {
-            x[2 * h] = mul_bf16x2(kvw_place(__byte_perm(v[h], 0, 0x4140)), f);
-            x[2 * h + 1] = mul_bf16x2(kvw_place(__byte_perm(v[h], 0, 0x4342)), f);
-          }
-        };
-        if (plain) {
-#pragma unroll
-          for (int q = 0; q < NP; ++q) {
-            const int step = cw + q * KVW_CONV_WARPS;
-            uint32_t x[8];
-            expand(code[q % AHEAD], __shfl_sync(0xFFFFFFFFu, factor, (step * KEYS >> 4) & 7), x);
-            if (step < STEPS && on) store(step * KEYS + k0, x);
-            if (q + AHEAD < NP) load(q + AHEAD, cur, code[q % AHEAD]);
-            else if (more) load(q + AHEAD - NP, nxt, code[q % AHEAD]);
-          }
-        } else {
-          // large scales and marked blocks: rare, and read (again) one step at a time
-#pragma unroll 1
-          for (int q = 0; q < NP; ++q) {
-            const int step = cw + q * KVW_CONV_WARPS;
-            uint32_t v[4] = {0, 0, 0, 0}, x[8];
-            load(q, cur, v);
-            expand(v, __shfl_sync(0xFFFFFFFFu, factor, (step * KEYS >> 4) & 7), x);
-            const uint32_t sb = __shfl_sync(0xFFFFFFFFu, scale, (step * KEYS >> 4) & 7);
-            float r1;
-            kva_factor(sb, &r1);
-            const uint32_t r2 = cvt_bf16x2(r1, r1);
-#pragma unroll
-            for (int h = 0; h < 4; ++h) {
-              const uint32_t bits = (sb & 1u) ? kva_nan4_bits(v[h]) : 0u;
-#pragma unroll
-              for (int y = 0; y < 2; ++y) {
-                uint32_t z = mul_bf16x2(x[2 * h + y], r2);
-                // a key's NaN goes into the scores, a value's is put into the outputs at the end
-                const uint32_t nan = cur.u.v ? 0u : 0x7FC0u;
-                if ((bits >> (2 * y)) & 1u) z = (z & 0xFFFF0000u) | nan;
-                if ((bits >> (2 * y + 1)) & 1u) z = (z & 0x0000FFFFu) | nan << 16;
-                x[2 * h + y] = z;
-              }
-            }
-            if (step < STEPS && on) store(step * KEYS + k0, x);
-          }
-          if (more) {
-#pragma unroll
-            for (int q = 0; q < AHEAD; ++q) load(q, nxt, code[q]);
-          }
-        }
-        if (!cur.u.v && cw == 0) {
-          const uint32_t marks = __ballot_sync(0xFFFFFFFFu, cur.v_scale & 1u) & 255u;
-          if (lane == 0) sh->info[(tiles_before + cur.u.tile) & 7] = cur.gone | marks << 8;
-        }
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&sh->full[slot]);
-        cur = nxt;
-        if (i + 2 < 2 * n) locate(i + 2, nxt);
+        if (unit + i > 0) publish(last, unit + i - 1);
+        last = now;
       }
       unit += 2 * n;
       tiles_before += n;
+    }
+    if (unit > 0) publish(last, unit - 1);
+    // an end for either group
+    for (int i = 0; i < 2 && ok; ++i, ++unit) {
+      const uint32_t slot = unit % KVW_META;
+      if (unit >= KVW_META) ok = __all_sync(0xFFFFFFFFu, mbar_wait_inl(&sh->meta_free[slot], ((unit / KVW_META) & 1) ^ 1, wc));
+      if (!ok) break;
+      if (lane == 0) {
+        sh->meta[slot].flags = KVW_END;
+        mbar_arrive(&sh->meta_full[slot]);
+      }
+      __syncwarp();
+    }
+  } else {
+    // -------------------------------------------------------------- keys and values
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(KVW_REGS_REST));
+    // A warp takes KEYS keys of 16-code pieces at a time, every KVW_CONV_WARPS-th such step of a unit.
+    // Codes are loaded AHEAD steps before they are expanded.
+    constexpr int P16 = D / 16, KEYS = D == 64 ? 8 : D == 128 ? 4 : 2;
+    constexpr int STEPS = 128 / KEYS, NP = (STEPS + KVW_CONV_WARPS - 1) / KVW_CONV_WARPS;
+    constexpr int AHEAD = NP > 5 ? 5 : NP;
+    static_assert(NP % AHEAD == 0, "whole rounds");
+    // lane's key and piece: eight lanes that store together have four pieces of two keys, whose
+    // swizzles differ in the lowest bit, so they meet no bank twice
+    const int group = (warp - 10) / KVW_CONV_WARPS, cw = (warp - 10) % KVW_CONV_WARPS;
+    const int k0 = D == 64 ? lane >> 2 : ((lane >> 2) & 1) + (D == 128 ? 2 * (lane >> 4) : 0);
+    const int c = D == 64 ? lane & 3 : (lane & 3) + 4 * (D == 128 ? (lane >> 3) & 1 : lane >> 3);
+    const bool on = c < P16;                       // (D = 192: 24 lanes of a warp)
+    uint32_t code[AHEAD][4];
+    const auto load = [&](int q, const KvwMeta& m, const uint8_t* src, uint32_t (&v)[4]) {
+      const int step = cw + q * KVW_CONV_WARPS, key = step * KEYS;
+      if (step < STEPS && on) kvf_load<4>(v, src + (int64_t)m.place[(key >> 4) & 7] * (16 * D) + (key & 15) * D);
+    };
+    const auto source = [&](uint32_t flags) { return (flags & KVW_VALUES ? p.c.v8 : p.c.k8) + (k0 * D + c * 16); };
+    const auto known = [&](uint32_t u, uint32_t* flags) {
+      const bool ok = __all_sync(0xFFFFFFFFu, mbar_wait_inl(&sh->meta_full[u % KVW_META], (u / KVW_META) & 1, wc));
+      *flags = ok ? sh->meta[u % KVW_META].flags : KVW_END;
+    };
+    uint32_t unit = group, flags;
+    known(unit, &flags);
+    if (!(flags & KVW_END)) {
+#pragma unroll
+      for (int q = 0; q < AHEAD; ++q) load(q, sh->meta[unit % KVW_META], source(flags), code[q]);
+    }
+    while (!(flags & KVW_END)) {
+      const KvwMeta &m = sh->meta[unit % KVW_META], &next = sh->meta[(unit + 2) % KVW_META];
+      uint32_t flags_next;
+      known(unit + 2, &flags_next);
+      const bool more = !(flags_next & KVW_END);
+      const uint8_t *src = source(flags), *src_next = source(flags_next);
+      const uint32_t slot = unit % UNITS;
+      if (unit >= UNITS && !__all_sync(0xFFFFFFFFu, mbar_wait_inl(&sh->free[slot], ((unit / UNITS) & 1) ^ 1, wc))) break;
+      uint8_t* dst = ring + slot * TILE + (c >> 2) * 16384 + k0 * 128;
+      const auto store = [&](int step, const uint32_t (&x)[8]) {
+        const int key = step * KEYS + k0, b = 2 * (c & 3);
+        uint8_t* at = dst + step * KEYS * 128;
+        *reinterpret_cast<uint4*>(at + ((b ^ (key & 7)) << 4)) = make_uint4(x[0], x[1], x[2], x[3]);
+        *reinterpret_cast<uint4*>(at + (((b + 1) ^ (key & 7)) << 4)) = make_uint4(x[4], x[5], x[6], x[7]);
+      };
+      const auto expand = [&](const uint32_t (&v)[4], uint32_t f, uint32_t (&x)[8]) {
+#pragma unroll
+        for (int h = 0; h < 4; ++h) {
+          x[2 * h] = mul_bf16x2(kvw_place(__byte_perm(v[h], 0, 0x4140)), f);
+          x[2 * h + 1] = mul_bf16x2(kvw_place(__byte_perm(v[h], 0, 0x4342)), f);
+        }
+      };
+      if (flags & KVW_PLAIN) {
+#pragma unroll
+        for (int q = 0; q < NP; ++q) {
+          const int step = cw + q * KVW_CONV_WARPS;
+          uint32_t x[8];
+          expand(code[q % AHEAD], m.factor[(step * KEYS >> 4) & 7], x);
+          if (step < STEPS && on) store(step, x);
+          if (q + AHEAD < NP) load(q + AHEAD, m, src, code[q % AHEAD]);
+          else if (more) load(q + AHEAD - NP, next, src_next, code[q % AHEAD]);
+        }
+      } else {
+        // large scales and marked blocks: rare, and read (again) one step at a time
+#pragma unroll 1
+        for (int q = 0; q < NP; ++q) {
+          const int step = cw + q * KVW_CONV_WARPS;
+          uint32_t v[4] = {0, 0, 0, 0}, x[8];
+          load(q, m, src, v);
+          expand(v, m.factor[(step * KEYS >> 4) & 7], x);
+          const uint32_t sb = m.scale[(step * KEYS >> 4) & 7];
+          float r1;
+          kva_factor(sb, &r1);
+          const uint32_t r2 = cvt_bf16x2(r1, r1);
+#pragma unroll
+          for (int h = 0; h < 4; ++h) {
+            const uint32_t bits = (sb & 1u) ? kva_nan4_bits(v[h]) : 0u;
+#pragma unroll
+            for (int y = 0; y < 2; ++y) {
+              uint32_t z = mul_bf16x2(x[2 * h + y], r2);
+              // a key's NaN goes into the scores, a value's is put into the outputs at the end
+              const uint32_t nan = flags & KVW_VALUES ? 0u : 0x7FC0u;
+              if ((bits >> (2 * y)) & 1u) z = (z & 0xFFFF0000u) | nan;
+              if ((bits >> (2 * y + 1)) & 1u) z = (z & 0x0000FFFFu) | nan << 16;
+              x[2 * h + y] = z;
+            }
+          }
+          if (step < STEPS && on) store(step, x);
+        }
+        if (more) {
+#pragma unroll
+          for (int q = 0; q < AHEAD; ++q) load(q, next, src_next, code[q]);
+        }
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) {
+        mbar_arrive(&sh->full[slot]);
+        mbar_arrive(&sh->meta_free[unit % KVW_META]);
+      }
+      unit += 2;
+      flags = flags_next;
     }
   }
   tc_fence_before();
