@@ -7,8 +7,11 @@
 // memory on the way (4 KB of codes are read once per 256 rows; the expansion, ten
 // operations per four codes on two pipes, runs beside the products).
 //
-// A CTA works on two streams of (scores, weights) so that one's softmax runs under the other's
-// products:
+// Scores come in buffers of 64 keys, two per stream, so that a row's stay in registers from the
+// maximum to the weights and the next are there when it is done with them (with one buffer of 128
+// the chain scores -> softmax -> output -> scores took 6700 cycles, 5000 of them softmax).  The
+// weights of a buffer go where its scores were.
+// A CTA works on two streams, so that one's softmax runs under the other's products:
 //   D <= 128, more than 128 rows: a stream per 128 rows, on the same keys;
 //   D <= 128, up to 128 rows: even and odd tiles of keys, each stream with references, sums and
 //     outputs of its own, added up at the end of the row tile;
@@ -61,7 +64,7 @@ struct KvwShared {
   KvwMeta meta[KVW_META];
   uint64_t meta_full[KVW_META], meta_free[KVW_META];
   uint64_t full[KVW_UNITS], free[KVW_UNITS];
-  uint64_t s_full[2], p_full[2], o_done[2];
+  uint64_t s_full[4], p_full[4], o_done[4];  // buffer 2 * stream + half of the tile
   uint64_t q_full, q_free, drain;
   uint64_t pair_full, pair_free;  // the second stream's results are there / have been taken
   uint32_t tmem;
@@ -167,7 +170,7 @@ __global__ void __launch_bounds__(KVW_THREADS, 1) kv_attn_wide_kernel(const __gr
       mbar_init(&sh->meta_full[i], 1);
       mbar_init(&sh->meta_free[i], KVW_CONV_WARPS);
     }
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < 4; ++i) {
       mbar_init(&sh->s_full[i], 1);
       mbar_init(&sh->p_full[i], 4);
       mbar_init(&sh->o_done[i], 1);
@@ -199,11 +202,11 @@ __global__ void __launch_bounds__(KVW_THREADS, 1) kv_attn_wide_kernel(const __gr
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(KVW_REGS_SOFT));
     const int wg = warp >> 2, t128 = tid & 127;
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-    uint32_t s_ph[2] = {0, 0};  // phases of the score buffers
-    // products with the weights of either buffer so far.  A tile's scores come after the product
-    // with the weights that were in their buffer before, so at most one of a buffer's products
-    // is ever waited for, and its parity tells it.
-    uint32_t o_count[2] = {0, 0};
+    uint32_t s_ph = 0;  // phases of the score buffers, a bit each
+    // products with the weights of each buffer so far, modulo two.  A buffer's scores come after the
+    // product with the weights that were in it before, so at most one of its products is ever
+    // waited for, and its parity tells it.
+    uint32_t o_ph = 0;
     bool first = true;
     // the scale's sign goes into the queries; times 2^-149 instead of zero, unseen scores stay -inf
     const uint32_t turn = p.scale_log2 < 0.f ? 0x80008000u : 0u;
@@ -251,17 +254,17 @@ __global__ void __launch_bounds__(KVW_THREADS, 1) kv_attn_wide_kernel(const __gr
       ++item;
       if (ONE_OUT && wg == 1) continue;
       // ------------------------------------------------------------ tiles of this warpgroup
-      // two: all of them, in buffer wg; else every other one in buffer wg; one output: all, in
-      // buffers by turns
+      // two: all of them, in the buffers of stream wg; else every other one; one output: all, in the
+      // streams' buffers by turns
       const int my_row = r0 + (rows256 ? wg * 128 : 0) + t128;
       const int tok = my_row / p.G;
       const int clear = w.len + (p.mask ? 0 : (my_row - t128) / p.G + 1);
       const int limit = tok < w.n ? (int)min((int64_t)w.len + (p.mask ? 0 : tok + 1), (int64_t)w.keys) : 0;
-      const int step = ONE_OUT || two ? 1 : 2;
+      const int step = ONE_OUT || two ? 1 : 2;  // tiles
       const bool idle = rows256 && !two && wg == 1;
       float m = -INFINITY, l = 0.f;
       bool nans = false;  // sh->nan is in use
-      int done = 0, last = wg;  // buffer of the last tile
+      int last = -1;  // buffer of the last weights
       const uint32_t o_col = tmem + 256 + (ONE_OUT ? 0 : wg * D) + lanes;
       bool ok = true;
       // (a row tile of 256 rows whose second half is empty is done by even and odd tiles too:
@@ -270,56 +273,43 @@ __global__ void __launch_bounds__(KVW_THREADS, 1) kv_attn_wide_kernel(const __gr
       const int tk = idle ? row / p.G : tok;
       const int cl = idle ? w.len + (p.mask ? 0 : r0 / p.G + 1) : clear;
       const int lm = idle ? (tk < w.n ? (int)min((int64_t)w.len + (p.mask ? 0 : tk + 1), (int64_t)w.keys) : 0) : limit;
-      for (int j = step == 2 ? wg : 0; j < n; j += step, ++done) {
-        const int buf = ONE_OUT ? (j & 1) : wg;
-        const uint32_t s_col = tmem + buf * 128 + lanes;
-        ok = __all_sync(0xFFFFFFFFu, mbar_wait_inl(&sh->s_full[buf], s_ph[buf], wc));
+      for (int q = step == 2 ? 2 * wg : 0; q < 2 * n; q += (q & 1) ? 2 * step - 1 : 1) {
+        const int j = q >> 1, h = q & 1, buf = 2 * (ONE_OUT ? j & 1 : wg) + h;
+        const uint32_t s_col = tmem + buf * 64 + lanes;
+        ok = __all_sync(0xFFFFFFFFu, mbar_wait_inl(&sh->s_full[buf], (s_ph >> buf) & 1, wc));
         if (!ok) break;
-        s_ph[buf] ^= 1;
+        s_ph ^= 1u << buf;
         tc_fence_after();
-        const int pos0 = (w.t0 + j) * 128;
-        const uint32_t info = sh->info[(tiles_before + j) & 15];
-        const bool open = pos0 + 128 <= cl && (info & 255u) == 0;
-        // ---------------------------------------------------------- maximum
-        uint32_t see[4] = {~0u, ~0u, ~0u, ~0u};
-        if (!open) {
+        float x[64];
+        tmem_ld32(s_col, reinterpret_cast<uint32_t*>(x));
+        tmem_ld32(s_col + 32, reinterpret_cast<uint32_t*>(x + 32));
+        const int pos0 = (w.t0 + j) * 128 + 64 * h;
+        const uint32_t info = sh->info[(tiles_before + j) & 15], gone = (info >> (4 * h)) & 15u;
+        tmem_wait_ld();
+        if (pos0 + 64 > cl || gone) {
+          // some rows do not see some of the keys
 #pragma unroll
-          for (int c = 0; c < 4; ++c) {
+          for (int c = 0; c < 2; ++c) {
             const int at = pos0 + 32 * c, k = lm - at;
-            see[c] = k >= 32 ? ~0u : k <= 0 ? 0u : (1u << k) - 1u;
+            uint32_t see = k >= 32 ? ~0u : k <= 0 ? 0u : (1u << k) - 1u;
             if (p.mask && tk < w.n)
               for (int i = max(w.len - at, 0); i < 32 && at + i < w.keys; ++i)
-                if (kva_sees(p, w.b, w.len, w.n, tk, at + i)) see[c] |= 1u << i;
-            if ((info >> (2 * c)) & 1u) see[c] &= 0xFFFF0000u;
-            if ((info >> (2 * c + 1)) & 1u) see[c] &= 0x0000FFFFu;
+                if (kva_sees(p, w.b, w.len, w.n, tk, at + i)) see |= 1u << i;
+            if ((gone >> (2 * c)) & 1u) see &= 0xFFFF0000u;
+            if ((gone >> (2 * c + 1)) & 1u) see &= 0x0000FFFFu;
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              if (!((see >> i) & 1u)) x[32 * c + i] = -INFINITY;
           }
         }
-        // half a row's scores at a time.  The second half stays in registers: its weights go where
-        // its last scores were, and the first half, read again, gets the columns before.
-        float x[64];
-        const auto read = [&](int half) {
-          tmem_ld32(s_col + 64 * half, reinterpret_cast<uint32_t*>(x));
-          tmem_ld32(s_col + 64 * half + 32, reinterpret_cast<uint32_t*>(x + 32));
-          tmem_wait_ld();
-          if (!open) {
-            const uint32_t lo = half ? see[2] : see[0], hi = half ? see[3] : see[1];
+        // ---------------------------------------------------------- maximum
+        float top = kvw_max3(x[0], x[1], x[2]), top1 = kvw_max3(x[3], x[4], x[5]);
 #pragma unroll
-            for (int i = 0; i < 64; ++i)
-              if (!(((i < 32 ? lo : hi) >> (i % 32)) & 1u)) x[i] = -INFINITY;
-          }
-        };
-        float top = -INFINITY;
-#pragma unroll 1
-        for (int half = 0; half < 2; ++half) {
-          read(half);
-          float a = kvw_max3(x[0], x[1], x[2]), b = kvw_max3(x[3], x[4], x[5]);
-#pragma unroll
-          for (int i = 6; i < 62; i += 4) {
-            a = kvw_max3(a, x[i], x[i + 1]);
-            b = kvw_max3(b, x[i + 2], x[i + 3]);
-          }
-          top = kvw_max3(kvw_max3(a, x[62], x[63]), b, top);
+        for (int i = 6; i < 62; i += 4) {
+          top = kvw_max3(top, x[i], x[i + 1]);
+          top1 = kvw_max3(top1, x[i + 2], x[i + 3]);
         }
+        top = fmaxf(kvw_max3(kvw_max3(top, x[62], x[63]), top1, -INFINITY), -INFINITY);
         top = top == -INFINITY ? top : top * scale;
         // ---------------------------------------------------------- raise the reference
         if (__any_sync(0xFFFFFFFFu, top > m + KVA_RISE)) {
@@ -327,8 +317,8 @@ __global__ void __launch_bounds__(KVW_THREADS, 1) kv_attn_wide_kernel(const __gr
           const float f = now == -INFINITY ? 1.f : kva_ex2(m - now);
           m = now;
           l *= f;
-          if (done > 0) {
-            ok = __all_sync(0xFFFFFFFFu, mbar_wait_inl(&sh->o_done[last], (o_count[last] - 1) & 1, wc));
+          if (last >= 0) {
+            ok = __all_sync(0xFFFFFFFFu, mbar_wait_inl(&sh->o_done[last], ((o_ph >> last) & 1) ^ 1, wc));
             if (!ok) break;
             tc_fence_after();
 #pragma unroll 1
@@ -347,41 +337,37 @@ __global__ void __launch_bounds__(KVW_THREADS, 1) kv_attn_wide_kernel(const __gr
         const float mu = (m == -INFINITY ? 0.f : m) + KVA_DOWN;
         const float2 sc = make_float2(scale, scale), minus = make_float2(-mu, -mu);
         float2 sum = make_float2(0.f, 0.f);
-#pragma unroll 1
-        for (int half = 1; half >= 0; --half) {
-          if (half == 0) read(0);
 #pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            uint32_t e[16];
+        for (int c = 0; c < 2; ++c) {
+          uint32_t e[16];
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-              float2 y = kvw_fma2(make_float2(x[32 * c + 2 * i], x[32 * c + 2 * i + 1]), sc, minus);
-              y = make_float2(kva_ex2(y.x), kva_ex2(y.y));
-              sum = kvw_add2(sum, y);
-              e[i] = cvt_bf16x2(y.x, y.y);
-            }
-            tmem_st16(s_col + 64 + 32 * half + 16 * c, e);
+          for (int i = 0; i < 16; ++i) {
+            float2 y = kvw_fma2(make_float2(x[32 * c + 2 * i], x[32 * c + 2 * i + 1]), sc, minus);
+            y = make_float2(kva_ex2(y.x), kva_ex2(y.y));
+            sum = kvw_add2(sum, y);
+            e[i] = cvt_bf16x2(y.x, y.y);
           }
+          tmem_st16(s_col + 16 * c, e);
         }
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&sh->p_full[buf]);
-        ++o_count[buf];
+        o_ph ^= 1u << buf;
         last = buf;
         l += sum.x + sum.y;
-        if (info >> 8) {
+        if ((info >> 8) && h == 1) {
           if (!nans)
             for (int i = 0; i < D / 32; ++i) sh->nan[wg][t128][i] = 0;
           nans = true;
-          kvw_nan_columns<D>(p, w.b, w.h, w.len, w.n, tk, pos0, w.keys, info >> 8, sh->nan[wg][t128]);
+          kvw_nan_columns<D>(p, w.b, w.h, w.len, w.n, tk, pos0 - 64, w.keys, info >> 8, sh->nan[wg][t128]);
         }
       }
       if (!ok) break;
       tiles_before += n;
       // ------------------------------------------------------------ results
-      if (done > 0) {
-        ok = __all_sync(0xFFFFFFFFu, mbar_wait_inl(&sh->o_done[last], (o_count[last] - 1) & 1, wc));
+      if (last >= 0) {
+        ok = __all_sync(0xFFFFFFFFu, mbar_wait_inl(&sh->o_done[last], ((o_ph >> last) & 1) ^ 1, wc));
         tc_fence_after();
       }
       if (!ONE_OUT && !two) {
@@ -474,8 +460,8 @@ __global__ void __launch_bounds__(KVW_THREADS, 1) kv_attn_wide_kernel(const __gr
     // -------------------------------------------------------------- products
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(KVW_REGS_REST));
     const bool leader = elect_one();
-    uint32_t unit = 0, q_ph = 0, p_ph[2] = {0, 0};
-    constexpr uint32_t idesc_s = idesc_bf16_f32(128, 128, false, false);
+    uint32_t unit = 0, q_ph = 0, p_ph = 0;
+    constexpr uint32_t idesc_s = idesc_bf16_f32(128, 64, false, false);
     constexpr uint32_t idesc_o = idesc_bf16_f32(128, D, false, true);
     bool ok = true;
     const auto wait = [&](uint64_t* bar, uint32_t ph) {
@@ -483,28 +469,51 @@ __global__ void __launch_bounds__(KVW_THREADS, 1) kv_attn_wide_kernel(const __gr
       tc_fence_after();
       return ok;
     };
-    const auto qk = [&](int buf, int qt, uint32_t slot) {
+    // scores of half h of the tile whose keys are in `slot`, into the stream's buffer
+    const auto qk = [&](int stream, int h, int qt, uint32_t slot) {
       if (leader) {
-        const uint32_t a = smem_u32(qs + qt * TILE), b = smem_u32(ring + slot * TILE);
+        const uint32_t a = smem_u32(qs + qt * TILE), b = smem_u32(ring + slot * TILE) + h * 8192;
 #pragma unroll
         for (int ks = 0; ks < D / 16; ++ks) {
           const uint32_t off = (ks >> 2) * 16384 + (ks & 3) * 32;
-          umma_bf16_ss(tmem + buf * 128, sdesc_sw128(a + off, 16, 1024), sdesc_sw128(b + off, 16, 1024), idesc_s, ks > 0);
+          umma_bf16_ss(tmem + (2 * stream + h) * 64, sdesc_sw128(a + off, 16, 1024), sdesc_sw128(b + off, 16, 1024), idesc_s,
+                       ks > 0);
         }
-        umma_commit(&sh->s_full[buf]);
+        umma_commit(&sh->s_full[2 * stream + h]);
       }
       __syncwarp();
     };
-    const auto pv = [&](int buf, int out, uint32_t slot, bool acc) {
+    // a whole tile's, into both of the stream's buffers, which lie side by side
+    const auto qk_tile = [&](int stream, uint32_t slot) {
       if (leader) {
-        const uint32_t b = smem_u32(ring + slot * TILE);
+        const uint32_t a = smem_u32(qs), b = smem_u32(ring + slot * TILE);
 #pragma unroll
-        for (int ks = 0; ks < 8; ++ks)
-          kvw_mma_ts(tmem + 256 + out * D, tmem + buf * 128 + 64 + ks * 8, sdesc_sw128(b + ks * 2048, 16384, 1024), idesc_o,
-                     acc || ks > 0);
-        umma_commit(&sh->o_done[buf]);
+        for (int ks = 0; ks < D / 16; ++ks) {
+          const uint32_t off = (ks >> 2) * 16384 + (ks & 3) * 32;
+          umma_bf16_ss(tmem + stream * 128, sdesc_sw128(a + off, 16, 1024), sdesc_sw128(b + off, 16, 1024),
+                       idesc_bf16_f32(128, 128, false, false), ks > 0);
+        }
+        umma_commit(&sh->s_full[2 * stream]);
+        umma_commit(&sh->s_full[2 * stream + 1]);
       }
       __syncwarp();
+    };
+    const auto pv = [&](int stream, int h, int out, uint32_t slot, bool acc) {
+      if (leader) {
+        const uint32_t b = smem_u32(ring + slot * TILE) + h * 8192;
+#pragma unroll
+        for (int ks = 0; ks < 4; ++ks)
+          kvw_mma_ts(tmem + 256 + out * D, tmem + (2 * stream + h) * 64 + ks * 8, sdesc_sw128(b + ks * 2048, 16384, 1024),
+                     idesc_o, acc || ks > 0);
+        umma_commit(&sh->o_done[2 * stream + h]);
+      }
+      __syncwarp();
+    };
+    const auto weights = [&](int stream, int h) {
+      const int buf = 2 * stream + h;
+      const bool there = wait(&sh->p_full[buf], (p_ph >> buf) & 1);
+      p_ph ^= 1u << buf;
+      return there;
     };
     const auto commit = [&](uint64_t* bar) {
       if (leader) umma_commit(bar);
@@ -523,49 +532,59 @@ __global__ void __launch_bounds__(KVW_THREADS, 1) kv_attn_wide_kernel(const __gr
         *slot = u % UNITS;
         return wait(&sh->full[*slot], (u / UNITS) & 1);
       };
-      uint32_t s0, s1;
+      uint32_t vs, ks;
       if (two) {
-        if (!take(0, &s0)) break;
-        qk(0, 0, s0);
-        qk(1, 1, s0);
-        commit(&sh->free[s0]);
+        if (!take(0, &ks)) break;
+        for (int q = 0; q < 4; ++q) qk(q & 1, q >> 1, q & 1, ks);
+        commit(&sh->free[ks]);
         if (n == 1) commit(&sh->q_free);
         for (int j = 0; j < n && ok; ++j) {
-          if (!take(2 * j + 1, &s0)) break;
-          for (int s = 0; s < 2; ++s) {
-            if (!wait(&sh->p_full[s], p_ph[s])) break;
-            p_ph[s] ^= 1;
-            pv(s, s, s0, j > 0);
-            if (s == 1) commit(&sh->free[s0]);
+          if (!take(2 * j + 1, &vs)) break;
+          for (int q = 0; q < 4; ++q) {
+            const int s = q & 1, h = q >> 1;
+            if (!weights(s, h)) break;
+            pv(s, h, s, vs, j > 0 || h > 0);
+            if (q == 3) commit(&sh->free[vs]);
             if (j + 1 < n) {
-              if (s == 0 && !take(2 * j + 2, &s1)) break;
-              qk(s, s, s1);
-              if (s == 1) {
-                commit(&sh->free[s1]);
-                if (j + 2 == n) commit(&sh->q_free);
-              }
+              if (q == 0 && !take(2 * j + 2, &ks)) break;
+              qk(s, h, s, ks);
             }
+          }
+          if (ok && j + 1 < n) {
+            commit(&sh->free[ks]);
+            if (j + 2 == n) commit(&sh->q_free);
           }
         }
       } else {
         for (int j = 0; j < min(n, 2) && ok; ++j) {
-          if (!take(j, &s0)) break;
-          qk(j, 0, s0);
-          commit(&sh->free[s0]);
+          if (!take(j, &ks)) break;
+          // (wide heads wait for the tensor cores, which 64 keys at a time would feed from shared
+          // memory at two thirds of their rate)
+          if constexpr (ONE_OUT) {
+            qk_tile(j, ks);
+          } else {
+            qk(j, 0, 0, ks);
+            qk(j, 1, 0, ks);
+          }
+          commit(&sh->free[ks]);
           if (j + 1 == n) commit(&sh->q_free);
         }
         for (int j = 0; j < n && ok; ++j) {
           const int s = j & 1;
           // values of tile j: unit 1 of a single tile; else 2 + 2 j, the last one 2 n - 1
-          if (!take(n == 1 ? 1 : j + 1 == n ? 2 * n - 1 : 2 + 2 * j, &s0)) break;
-          if (!wait(&sh->p_full[s], p_ph[s])) break;
-          p_ph[s] ^= 1;
-          pv(s, ONE_OUT ? 0 : s, s0, ONE_OUT ? j > 0 : j > 1);
-          commit(&sh->free[s0]);
-          if (j + 2 < n) {
-            if (!take(2 * j + 3, &s0)) break;
-            qk(s, 0, s0);
-            commit(&sh->free[s0]);
+          if (!take(n == 1 ? 1 : j + 1 == n ? 2 * n - 1 : 2 + 2 * j, &vs)) break;
+          for (int h = 0; h < 2; ++h) {
+            if (!weights(s, h)) break;
+            pv(s, h, ONE_OUT ? 0 : s, vs, h > 0 || (ONE_OUT ? j > 0 : j > 1));
+            if (h == 1) commit(&sh->free[vs]);
+            if (j + 2 < n) {
+              if (h == (ONE_OUT ? 1 : 0) && !take(2 * j + 3, &ks)) break;
+              if constexpr (!ONE_OUT) qk(s, h, 0, ks);
+              else if (h == 1) qk_tile(s, ks);
+            }
+          }
+          if (ok && j + 2 < n) {
+            commit(&sh->free[ks]);
             if (j + 3 == n) commit(&sh->q_free);
           }
         }
