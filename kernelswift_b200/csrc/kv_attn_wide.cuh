@@ -76,12 +76,25 @@ struct KvwShared {
 };
 static_assert(sizeof(KvwShared) <= KVW_HDR, "KvwShared exceeds its header");
 
-// D[tmem] (+)= A[tmem] * B[smem]^T, bf16 inputs, fp32 accumulate.
-__device__ __forceinline__ void kvw_mma_ts(uint32_t d, uint32_t a, uint64_t bdesc, uint32_t idesc, uint32_t acc) {
+// Products in bf16 with fp32 sums; A in shared memory or in tensor memory, B in shared memory.
+// Descriptors as words: the high one (8 rows 1024 bytes apart, 128-byte swizzle) is always the
+// same, and the start address sits in the low bits of the low one, so that an operand's steps are
+// additions.  (With 64-bit descriptors put together for each product, the one thread that issues
+// them took 90 cycles a product, more than the tensor cores.)
+constexpr uint32_t KVW_DESC_HI = (1024u >> 4) | 1u << 14 | 1u << 30;
+__device__ __forceinline__ uint32_t kvw_desc(uint32_t saddr, uint32_t lbo_bytes) { return saddr >> 4 | lbo_bytes >> 4 << 16; }
+__device__ __forceinline__ void kvw_mma_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t acc) {
   asm volatile(
-      "{ .reg .pred p; setp.ne.b32 p, %4, 0;"
-      " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p; }" ::"r"(d),
-      "r"(a), "l"(bdesc), "r"(idesc), "r"(acc)
+      "{ .reg .pred p; .reg .b64 ad, bd; setp.ne.b32 p, %4, 0; mov.b64 ad, {%1, %5}; mov.b64 bd, {%2, %5};"
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], ad, bd, %3, p; }" ::"r"(d),
+      "r"(a), "r"(b), "r"(idesc), "r"(acc), "r"(KVW_DESC_HI)
+      : "memory");
+}
+__device__ __forceinline__ void kvw_mma_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{ .reg .pred p; .reg .b64 bd; setp.ne.b32 p, %4, 0; mov.b64 bd, {%2, %5};"
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], bd, %3, p; }" ::"r"(d),
+      "r"(a), "r"(b), "r"(idesc), "r"(acc), "r"(KVW_DESC_HI)
       : "memory");
 }
 
@@ -459,55 +472,53 @@ __global__ void __launch_bounds__(KVW_THREADS, 1) kv_attn_wide_kernel(const __gr
   } else if (warp == 8) {
     // -------------------------------------------------------------- products
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(KVW_REGS_REST));
-    const bool leader = elect_one();
+    // One thread does all of it: every instruction of this warp is in the chain of products.
+    if (elect_one()) {
     uint32_t unit = 0, q_ph = 0, p_ph = 0;
     constexpr uint32_t idesc_s = idesc_bf16_f32(128, 64, false, false);
     constexpr uint32_t idesc_o = idesc_bf16_f32(128, D, false, true);
+    const uint32_t q_desc = kvw_desc(smem_u32(qs), 16), k_desc = kvw_desc(smem_u32(ring), 16),
+                   v_desc = kvw_desc(smem_u32(ring), 16384);
     bool ok = true;
     const auto wait = [&](uint64_t* bar, uint32_t ph) {
-      ok = ok && __all_sync(0xFFFFFFFFu, mbar_wait_inl(bar, ph, wc));
+      ok = ok && mbar_wait_inl(bar, ph, wc);
       tc_fence_after();
       return ok;
     };
     // scores of half h of the tile whose keys are in `slot`, into the stream's buffer
     const auto qk = [&](int stream, int h, int qt, uint32_t slot) {
-      if (leader) {
-        const uint32_t a = smem_u32(qs + qt * TILE), b = smem_u32(ring + slot * TILE) + h * 8192;
+      {
+        const uint32_t a = q_desc + qt * (TILE >> 4), b = k_desc + slot * (TILE >> 4) + h * (8192 >> 4);
 #pragma unroll
         for (int ks = 0; ks < D / 16; ++ks) {
-          const uint32_t off = (ks >> 2) * 16384 + (ks & 3) * 32;
-          umma_bf16_ss(tmem + (2 * stream + h) * 64, sdesc_sw128(a + off, 16, 1024), sdesc_sw128(b + off, 16, 1024), idesc_s,
-                       ks > 0);
+          const uint32_t off = ((ks >> 2) * 16384 + (ks & 3) * 32) >> 4;
+          kvw_mma_ss(tmem + (2 * stream + h) * 64, a + off, b + off, idesc_s, ks > 0);
         }
         umma_commit(&sh->s_full[2 * stream + h]);
       }
-      __syncwarp();
     };
     // a whole tile's, into both of the stream's buffers, which lie side by side
     const auto qk_tile = [&](int stream, uint32_t slot) {
-      if (leader) {
-        const uint32_t a = smem_u32(qs), b = smem_u32(ring + slot * TILE);
+      {
+        const uint32_t b = k_desc + slot * (TILE >> 4);
 #pragma unroll
         for (int ks = 0; ks < D / 16; ++ks) {
-          const uint32_t off = (ks >> 2) * 16384 + (ks & 3) * 32;
-          umma_bf16_ss(tmem + stream * 128, sdesc_sw128(a + off, 16, 1024), sdesc_sw128(b + off, 16, 1024),
-                       idesc_bf16_f32(128, 128, false, false), ks > 0);
+          const uint32_t off = ((ks >> 2) * 16384 + (ks & 3) * 32) >> 4;
+          kvw_mma_ss(tmem + stream * 128, q_desc + off, b + off, idesc_bf16_f32(128, 128, false, false), ks > 0);
         }
         umma_commit(&sh->s_full[2 * stream]);
         umma_commit(&sh->s_full[2 * stream + 1]);
       }
-      __syncwarp();
     };
     const auto pv = [&](int stream, int h, int out, uint32_t slot, bool acc) {
-      if (leader) {
-        const uint32_t b = smem_u32(ring + slot * TILE) + h * 8192;
+      {
+        const uint32_t b = v_desc + slot * (TILE >> 4) + h * (8192 >> 4);
 #pragma unroll
         for (int ks = 0; ks < 4; ++ks)
-          kvw_mma_ts(tmem + 256 + out * D, tmem + (2 * stream + h) * 64 + ks * 8, sdesc_sw128(b + ks * 2048, 16384, 1024),
-                     idesc_o, acc || ks > 0);
+          kvw_mma_ts(tmem + 256 + out * D, tmem + (2 * stream + h) * 64 + ks * 8, b + ks * (2048 >> 4), idesc_o,
+                     acc || ks > 0);
         umma_commit(&sh->o_done[2 * stream + h]);
       }
-      __syncwarp();
     };
     const auto weights = [&](int stream, int h) {
       const int buf = 2 * stream + h;
@@ -516,8 +527,7 @@ __global__ void __launch_bounds__(KVW_THREADS, 1) kv_attn_wide_kernel(const __gr
       return there;
     };
     const auto commit = [&](uint64_t* bar) {
-      if (leader) umma_commit(bar);
-      __syncwarp();
+      umma_commit(bar);
     };
     for (; w.left > 0 && ok; w.next(p)) {
       if (!w.any()) continue;
@@ -594,6 +604,8 @@ __global__ void __launch_bounds__(KVW_THREADS, 1) kv_attn_wide_kernel(const __gr
     // every product and arrival in flight has landed before the CTA gives its memory back
     commit(&sh->drain);
     mbar_wait_body(&sh->drain, 0, wc, false, true);
+    }
+    __syncwarp();
   } else if (warp == 9) {
     // -------------------------------------------------------------- addresses
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(KVW_REGS_REST));
