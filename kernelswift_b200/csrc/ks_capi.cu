@@ -1300,10 +1300,13 @@ int ks_kv_attn(const void* q, const void* k8, const float* k_scale, const void* 
   const int per_sm = D * p.nr <= 1024 ? 2 : 1;
   p.budget_ns = wait_budget_ns();
   const int64_t most = B * p.row_tiles * heads * (KVA_SETUP + (max_pages * page + 127) / 128);
+  if (most >= (1ll << 31)) return fail(KS_ERR_UNSUPPORTED, "kv_attn: too many rows times keys");
   const unsigned grid = (unsigned)std::min<int64_t>({most, (int64_t)dev->num_sms * per_sm, (int64_t)KVA_MAX_CTAS / 2 * per_sm});
   p.part_o = static_cast<float*>(workspace);
   p.part_ml = reinterpret_cast<float2*>(p.part_o + 2ll * grid * p.nr * D);
   p.owner = reinterpret_cast<int4*>(p.part_ml + 2ll * grid * p.nr);
+  const int64_t items = B * p.row_tiles * heads;
+  p.by_item = items < (int64_t)grid;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const bool two = p.nr == 16;
   if (int rc = wide         ? (D == 64    ? launch_kv_attn_wide<64>(dev, p, grid, st)
@@ -1320,7 +1323,9 @@ int ks_kv_attn(const void* q, const void* k8, const float* k_scale, const void* 
   cudaLaunchAttribute at[1];
   at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   at[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.gridDim = dim3(grid, (unsigned)std::min(8, p.nr));
+  const unsigned shared = p.by_item ? (unsigned)items : grid;
+  cfg.gridDim = dim3(shared, (unsigned)std::min(p.nr, std::max(8, 256 / (int)shared)));  // of rows
+  if (p.nr >= 128) cfg.gridDim.y = 16;
   cfg.blockDim = dim3(256);
   cfg.stream = st;
   cfg.attrs = at;

@@ -63,13 +63,14 @@ struct KvAttnParams {
   float scale_log2;       // softmax scale * log2 e
   float* part_o;          // [2 * CTAs][nr][D]
   float2* part_ml;        // [2 * CTAs][nr]: reference, sum
-  int4* owner;            // [CTAs]: sequence, row tile, key head, parts (0: none to join)
+  int4* owner;            // sequence, row tile, key head, parts << 10 | CTA of the first one (0: none to join)
+  int32_t by_item;        // owner is indexed by row tile of the call (they are fewer), else by CTA
   uint64_t budget_ns;
 };
 
 struct KvaFind {
-  int64_t warp_sum[32];
-  int64_t total, per;
+  uint32_t warp_sum[32];
+  uint32_t per;
   int32_t left, b, rt, h, u;
 };
 
@@ -87,49 +88,47 @@ __device__ __forceinline__ int kva_tiles(const KvAttnParams& p, int len, int n, 
 // This CTA's stretch: its first row tile, the unit in it, and how many units.  All threads.
 __device__ __forceinline__ void kva_find(const KvAttnParams& p, KvaFind* f) {
   const int tid = threadIdx.x, threads = blockDim.x, lane = tid & 31, warp = tid >> 5;
-  const int64_t pairs = (int64_t)p.c.B * p.row_tiles;
-  const int64_t each = (pairs + threads - 1) / threads;
-  const int64_t i0 = min(tid * each, pairs), i1 = min(i0 + each, pairs);
-  int64_t sum = 0;
-  for (int64_t i = i0; i < i1; ++i) {
-    const int b = (int)(i / p.row_tiles), rt = (int)(i - (int64_t)b * p.row_tiles);
-    sum += (int64_t)p.c.heads * (KVA_SETUP + kva_tiles(p, kv_len(p.c, b), kv_new(p.c, b), rt));
-  }
-  int64_t incl = sum;
+  // (sequence, row tile) pairs, so many per thread; all units together are below 2^31
+  const uint32_t tiles = (uint32_t)p.row_tiles, pairs = (uint32_t)p.c.B * tiles;
+  const uint32_t each = (pairs + threads - 1) / threads, i0 = min(tid * each, pairs), i1 = min(i0 + each, pairs);
+  const auto cost = [&](uint32_t i) {
+    const int b = (int)(i / tiles), rt = (int)(i - b * tiles);
+    return (uint32_t)(KVA_SETUP + kva_tiles(p, kv_len(p.c, b), kv_new(p.c, b), rt));
+  };
+  uint32_t sum = 0;
+  for (uint32_t i = i0; i < i1; ++i) sum += p.c.heads * cost(i);
+  uint32_t incl = sum;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const int64_t v = __shfl_up_sync(0xFFFFFFFFu, incl, o);
+    const uint32_t v = __shfl_up_sync(0xFFFFFFFFu, incl, o);
     if (lane >= o) incl += v;
   }
   if (lane == 31) f->warp_sum[warp] = incl;
   if (tid == 0) f->left = 0;
   __syncthreads();
-  int64_t total = 0, before = 0;
+  uint32_t total = 0, before = 0;
   for (int w = 0; w < threads >> 5; ++w) {
     if (w < warp) before += f->warp_sum[w];
     total += f->warp_sum[w];
   }
-  const int64_t per = (total + gridDim.x - 1) / gridDim.x, start = (int64_t)blockIdx.x * per;
-  int64_t at = before + incl - sum;
-  if (start >= at && start < at + sum) {
-    for (int64_t i = i0; i < i1; ++i) {
-      const int b = (int)(i / p.row_tiles), rt = (int)(i - (int64_t)b * p.row_tiles);
-      const int cost = KVA_SETUP + kva_tiles(p, kv_len(p.c, b), kv_new(p.c, b), rt);
-      if (start < at + (int64_t)p.c.heads * cost) {
-        f->b = b;
-        f->rt = rt;
-        f->h = (int)((start - at) / cost);
-        f->u = (int)((start - at) % cost);
-        f->left = (int)min(per, total - start);
+  const uint32_t per = (total + gridDim.x - 1) / gridDim.x;
+  const uint64_t start = (uint64_t)blockIdx.x * per;
+  uint32_t at = before + incl - sum;
+  if (start >= at && start < (uint64_t)at + sum) {
+    for (uint32_t i = i0; i < i1; ++i) {
+      const uint32_t c = cost(i), in = (uint32_t)start - at;
+      if (in < p.c.heads * c) {
+        f->b = (int)(i / tiles);
+        f->rt = (int)(i % tiles);
+        f->h = (int)(in / c);
+        f->u = (int)(in % c);
+        f->left = (int)min(per, total - (uint32_t)start);
         break;
       }
-      at += (int64_t)p.c.heads * cost;
+      at += p.c.heads * c;
     }
   }
-  if (tid == 0) {
-    f->total = total;
-    f->per = per;
-  }
+  if (tid == 0) f->per = per;
   __syncthreads();
 }
 
@@ -176,11 +175,22 @@ struct KvaWalk {
   // where a part goes: a CTA shares its first row tile with the CTAs before it, its last one
   // with those behind
   __device__ __forceinline__ int slot() const { return 2 * (int)blockIdx.x + (t0 > 0 ? 0 : 1); }
-  // parts of the row tile, seen from the CTA that has its first tile
-  __device__ __forceinline__ int parts(int64_t per) const {
-    return (int)((at + KVA_SETUP + nt - 1) / per) - (int)blockIdx.x + 1;
+  // what the CTA that has a shared row tile's first tile leaves for the join
+  __device__ __forceinline__ void share(const KvAttnParams& p, uint32_t per) const {
+    const int parts = (int)((at + KVA_SETUP + nt - 1) / per) - (int)blockIdx.x + 1;
+    p.owner[p.by_item ? (b * p.row_tiles + rt) * p.c.heads + h : (int)blockIdx.x] = make_int4(b, rt, h, parts << 10 | (int)blockIdx.x);
   }
 };
+// Nothing to join yet.  A thread clears what it alone may set later: its CTA's entry, or those of
+// the row tiles whose first tile (or nothing at all) is in its stretch.
+__device__ __forceinline__ void kva_clear(const KvAttnParams& p, KvaWalk w) {
+  if (!p.by_item) {
+    p.owner[blockIdx.x] = make_int4(0, 0, 0, 0);
+    return;
+  }
+  for (; w.left > 0; w.next(p))
+    if (w.empty() || (w.any() && w.t0 == 0)) p.owner[(w.b * p.row_tiles + w.rt) * p.c.heads + w.h] = make_int4(0, 0, 0, 0);
+}
 
 __device__ __forceinline__ bool kva_sees(const KvAttnParams& p, int b, int len, int n, int t, int pos) {
   const int j = pos - len;
@@ -328,7 +338,7 @@ __global__ void __launch_bounds__(KVF_WARPS * 32, D * NT <= 128 ? 2 : 1) kv_attn
   kva_find(p, &find);
   KvaWalk w;
   w.start(p, &find);
-  if (tid == 0) p.owner[blockIdx.x] = make_int4(0, 0, 0, 0);
+  if (tid == 0) kva_clear(p, w);
   const int per_page = p.c.page / p.c.block;
   const int key_r = kvf_key<D>(r), key_v[2] = {kvf_key<D>(2 * c), kvf_key<D>(2 * c + 1)};
 
@@ -358,9 +368,9 @@ __global__ void __launch_bounds__(KVF_WARPS * 32, D * NT <= 128 ? 2 : 1) kv_attn
         const int pg = __ldg(p.c.table + (int64_t)w.b * p.c.max_pages + pi);
         const bool ok = pg >= 0 && pg < p.c.n_pages;
         if (!ok) report_bounds(p.c.status, w.b, (int)p.c.n_pages);
-        const int64_t unit = (int64_t)(ok ? pg : 0) * p.c.heads + w.h;
-        const int64_t si = unit * per_page + kva_div(in, p.c.block, p.block_shift);
-        place = (uint32_t)(unit * (p.c.page >> 4) + (in >> 4));
+        const uint32_t unit = (ok ? (uint32_t)pg : 0u) * (uint32_t)p.c.heads + (uint32_t)w.h;
+        const uint32_t si = unit * (uint32_t)per_page + (uint32_t)kva_div(in, p.c.block, p.block_shift);
+        place = unit * (uint32_t)(p.c.page >> 4) + (uint32_t)(in >> 4);
         ks32 = ok ? __float_as_uint(__ldg(p.c.k_scale + si)) : KVF_GONE;
         vs32 = __float_as_uint(__ldg(p.c.v_scale + si));
       }
@@ -710,23 +720,24 @@ __global__ void __launch_bounds__(KVF_WARPS * 32, D * NT <= 128 ? 2 : 1) kv_attn
         if (col == 0) p.part_ml[slot * NR + row] = make_float2(top, sum);
       }
     }
-    if (tid == 0 && !whole && w.t0 == 0) p.owner[blockIdx.x] = make_int4(w.b, w.rt, w.h, w.parts(find.per));
+    if (tid == 0 && !whole && w.t0 == 0) w.share(p, find.per);
     __syncthreads();
   }
 }
 
-// Parts of a row tile that several CTAs share, added up.  Blocks (c, y): the row tile whose first
-// tile CTA c has, some of its rows each.  D / 4 threads take a row; where there are many parts
-// (one long sequence) up to eight of such groups take every eighth part each, with a reference of
-// their own, and are added up in order.  (64 heads over 131069 keys, 37 parts a row tile, one
-// group a row: the join took 30 us of 76.)
+// Parts of a row tile that several CTAs share, added up.  Blocks (x, y): a row tile, or the one whose
+// first tile CTA x has where there are more row tiles than CTAs; some of its rows each.  D / 4
+// threads take a row; where there are many parts (one long sequence) up to eight of such groups
+// take every eighth part each, with a reference of their own, and are added up in order.  (64
+// heads over 131069 keys, 37 parts a row tile, one group a row: the join took 30 us of 76.)
 __global__ void __launch_bounds__(256) kv_attn_join_kernel(const __grid_constant__ KvAttnParams p) {
   __shared__ float4 sv[256];
   __shared__ float2 sml[256];
   asm volatile("griddepcontrol.wait;" ::: "memory");  // until all parts are written
   const int4 own = p.owner[blockIdx.x];
   if (own.w == 0) return;
-  const int b = own.x, r0 = own.y * p.nr, h = own.z, parts = own.w, d = p.c.d, per_row = d >> 2;
+  const int b = own.x, r0 = own.y * p.nr, h = own.z, parts = own.w >> 10, d = p.c.d, per_row = d >> 2;
+  const int64_t cta = own.w & 1023;
   const int n = kv_new(p.c, b), at_once = blockDim.x / per_row;
   int groups = 1;
   while (groups * 2 <= at_once && groups * 4 < parts) groups *= 2;
@@ -747,7 +758,7 @@ __global__ void __launch_bounds__(256) kv_attn_join_kernel(const __grid_constant
     if (in) {
 #pragma unroll 4
       for (int i = grp; i < parts; i += groups) {
-        const int64_t at = (i ? 2 * ((int64_t)blockIdx.x + i) : 2 * (int64_t)blockIdx.x + 1) * p.nr + row;
+        const int64_t at = (i ? 2 * (cta + i) : 2 * cta + 1) * p.nr + row;
         take(p.part_ml[at], *reinterpret_cast<const float4*>(p.part_o + at * d + col));
       }
     }

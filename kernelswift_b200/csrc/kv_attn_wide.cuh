@@ -195,7 +195,6 @@ __global__ void __launch_bounds__(KVW_THREADS, 1) kv_attn_wide_kernel(const __gr
     mbar_init(&sh->pair_free, 4);
     sh->abort = 0;
     fence_barrier_init();
-    p.owner[blockIdx.x] = make_int4(0, 0, 0, 0);
   }
   if (warp == 8) {
     tmem_alloc<1>(&sh->tmem, 512);
@@ -208,6 +207,7 @@ __global__ void __launch_bounds__(KVW_THREADS, 1) kv_attn_wide_kernel(const __gr
   const uint32_t tmem = sh->tmem;
   KvaWalk w;
   w.start(p, &sh->find);
+  if (tid == 0) kva_clear(p, w);
   const bool rows256 = p.nr == 256;
 
   if (warp < 8) {
@@ -459,7 +459,7 @@ __global__ void __launch_bounds__(KVW_THREADS, 1) kv_attn_wide_kernel(const __gr
         }
         if (!whole) {
           p.part_ml[prow] = make_float2(m, l);
-          if (tid == 0 && w.t0 == 0) p.owner[blockIdx.x] = make_int4(w.b, w.rt, w.h, w.parts(sh->find.per));
+          if (tid == 0 && w.t0 == 0) w.share(p, sh->find.per);
         }
         tc_fence_before();
       }
