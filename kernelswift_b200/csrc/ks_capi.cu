@@ -1235,23 +1235,29 @@ int ks_kv_append(const void* k, int64_t k_bs, int64_t k_ts, const void* v, int64
   p.k_bs = k_bs; p.k_ts = k_ts; p.v_bs = v_bs; p.v_ts = v_ts; p.q_bs = q_bs; p.q_ts = q_ts;
   p.freqs = rope_dim ? freqs : nullptr;
   p.pos = positions;
-  p.n_freqs = n_freqs;
+  p.n_freqs = (int)std::min<int64_t>(n_freqs, 0x7FFFFFFF);
+  p.page_shift = log2_of(page);
+  p.block_shift = log2_of(block);
+  p.row_shift = log2_of(D / 8);
   p.rd = rope_dim;
   p.q_heads = q ? q_heads : 0;
   p.nb = (int)((block - 1 + T - 1) / block + 1);  // however the first block is filled
   p.kv_ctas = B * p.nb * 2 * heads;
   p.q_pieces = q ? B * T * q_heads * (D / 8) : 0;
-  // 8-column pieces of a block, up to eight per thread
+  if (p.q_pieces >= (1ll << 32) - 65536) return fail(KS_ERR_UNSUPPORTED, "kv_append: too many queries");
+  // 8-column pieces of a block: two per thread, as far as threads go
   const int pieces = block * D / 8;
-  const int threads = pieces <= 1024 ? 128 : pieces <= 2048 ? 256 : 512;
+  const int threads = pieces <= 256 ? 128 : pieces <= 512 ? 256 : 512;
   const int64_t q_ctas = (p.q_pieces + threads * KV_Q_PIECES - 1) / (threads * KV_Q_PIECES);
   if (p.kv_ctas + q_ctas >= (1ll << 31)) return fail(KS_ERR_UNSUPPORTED, "kv_append: too many tokens");
   const unsigned grid = (unsigned)(p.kv_ctas + q_ctas);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (pieces <= 128) kv_append_kernel<1><<<grid, threads, 0, st>>>(p);
-  else if (pieces <= 256) kv_append_kernel<2><<<grid, threads, 0, st>>>(p);
-  else if (pieces <= 512) kv_append_kernel<4><<<grid, threads, 0, st>>>(p);
-  else kv_append_kernel<8><<<grid, threads, 0, st>>>(p);
+  if (pieces <= 128) kv_append_kernel<1, 128><<<grid, threads, 0, st>>>(p);
+  else if (pieces <= 256) kv_append_kernel<2, 128><<<grid, threads, 0, st>>>(p);
+  else if (pieces <= 512) kv_append_kernel<2, 256><<<grid, threads, 0, st>>>(p);
+  else if (pieces <= 1024) kv_append_kernel<2, 512><<<grid, threads, 0, st>>>(p);
+  else if (pieces <= 2048) kv_append_kernel<4, 512><<<grid, threads, 0, st>>>(p);
+  else kv_append_kernel<8, 512><<<grid, threads, 0, st>>>(p);
   return launch_check("kv_append_kernel launch");
 }
 

@@ -58,7 +58,8 @@ struct KvAppendParams {
   int64_t k_bs, k_ts, v_bs, v_ts, q_bs, q_ts;  // elements from sequence to sequence, token to token
   const float* freqs;    // [n_freqs, rd / 2, 2] or null
   const int32_t* pos;    // [B, T] or null: positions of the rotation
-  int64_t n_freqs;
+  int32_t n_freqs;
+  int32_t page_shift, block_shift, row_shift;  // of page, block and D / 8; -1: not a power of two
   int32_t rd, q_heads;
   int32_t nb;            // blocks that T tokens may touch
   int64_t kv_ctas;
@@ -75,8 +76,7 @@ __device__ __forceinline__ float kv_power(float amax) {
 
 // Eight columns from column c0 on, in fp32, rotated where they are among the last rd.  Each
 // product and sum is rounded on its own, so results do not depend on how they are fused.
-__device__ __forceinline__ void kv_rotate8(const uint4& raw, float (&y)[8], const float* freqs, int64_t row, int rd,
-                                           int c0) {
+__device__ __forceinline__ void kv_rotate8(const uint4& raw, float (&y)[8], const float* freqs, int row, int rd, int c0) {
   const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
@@ -84,7 +84,7 @@ __device__ __forceinline__ void kv_rotate8(const uint4& raw, float (&y)[8], cons
     y[2 * i + 1] = bf16hi_f32(w[i]);
   }
   if (c0 >= 0 && freqs) {  // c0: column among the rotated ones
-    const float4* f = reinterpret_cast<const float4*>(freqs + row * rd + c0);
+    const float4* f = reinterpret_cast<const float4*>(freqs + (int64_t)row * rd + c0);
     const float4 f0 = __ldg(f), f1 = __ldg(f + 1);
     const float cs[4] = {f0.x, f0.z, f1.x, f1.z}, sn[4] = {f0.y, f0.w, f1.y, f1.w};
 #pragma unroll
@@ -96,11 +96,18 @@ __device__ __forceinline__ void kv_rotate8(const uint4& raw, float (&y)[8], cons
   }
 }
 
-// Row of freqs for token t of sequence b; false where there is none.
-__device__ __forceinline__ bool kv_freq_row(const KvAppendParams& p, int b, int t, int at, int64_t* row) {
-  const int64_t r = p.pos ? (int64_t)__ldg(p.pos + (int64_t)b * p.c.T + t) : (int64_t)at;
-  *row = r < 0 ? 0 : r >= p.n_freqs ? p.n_freqs - 1 : r;
+// Row of freqs for token t of sequence b, at position `at`; false where there is none.
+__device__ __forceinline__ bool kv_freq_row(const KvAppendParams& p, int b, int t, int at, int* row) {
+  const int r = p.pos ? __ldg(p.pos + (int64_t)b * p.c.T + t) : at;
+  *row = min(max(r, 0), p.n_freqs - 1);
   return r == *row;
+}
+__device__ __forceinline__ uint32_t kv_div(uint32_t x, int d, int shift) { return shift >= 0 ? x >> shift : x / (uint32_t)d; }
+// The larger, NaN where either is.
+__device__ __forceinline__ float kv_max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
 }
 
 __device__ __forceinline__ float e4m3_f32(uint32_t code) {
@@ -109,36 +116,45 @@ __device__ __forceinline__ float e4m3_f32(uint32_t code) {
   return __half2float(__ushort_as_half((unsigned short)h));
 }
 
-// NP: 8-column pieces of the block per thread (block * D / 8 <= NP * threads).
-template <int NP>
-__global__ void __launch_bounds__(512) kv_append_kernel(KvAppendParams p) {
+// NP: 8-column pieces of the block per thread (block * D / 8 <= NP * THREADS).
+template <int NP, int THREADS>
+__global__ void __launch_bounds__(THREADS, NP <= 2 ? 1280 / THREADS : 1) kv_append_kernel(const __grid_constant__ KvAppendParams p) {
   const KvCache& c = p.c;
-  const int per_row = c.d >> 3, tid = threadIdx.x, threads = blockDim.x;
+  constexpr int threads = THREADS;
+  const int per_row = c.d >> 3, tid = threadIdx.x;
   if (blockIdx.x >= p.kv_ctas) {
     // ------------------------------------------------------------ queries
-    const int64_t first = (int64_t)(blockIdx.x - p.kv_ctas) * threads * KV_Q_PIECES + tid;
-    const uint32_t per_token = (uint32_t)(p.q_heads * per_row);
+    // (pieces of all queries are below 2^32)
+    const uint32_t first = (uint32_t)(blockIdx.x - p.kv_ctas) * (threads * KV_Q_PIECES) + tid;
+    const uint32_t per_token = (uint32_t)(p.q_heads * per_row), pieces = (uint32_t)p.q_pieces;
+    uint32_t token = first / per_token, at = first - token * per_token;
+    int b = (int)(token / (uint32_t)c.T), t = (int)(token - (uint32_t)b * (uint32_t)c.T);
     uint4 raw[KV_Q_PIECES];
-    int64_t frow[KV_Q_PIECES];
+    int frow[KV_Q_PIECES];
     int col[KV_Q_PIECES];
 #pragma unroll
     for (int i = 0; i < KV_Q_PIECES; ++i) {
-      const int64_t e = first + (int64_t)i * threads;
       raw[i] = make_uint4(0, 0, 0, 0);
       frow[i] = 0;
       col[i] = -1;
-      if (e < p.q_pieces) {
-        const uint32_t token = (uint32_t)((uint64_t)e / per_token), at = (uint32_t)(e - (int64_t)token * per_token);
-        const int b = (int)(token / (uint32_t)c.T), t = (int)(token - (uint32_t)b * c.T);
-        raw[i] = __ldg(reinterpret_cast<const uint4*>(p.q + b * p.q_bs + t * p.q_ts + (int64_t)at * 8));
-        col[i] = (int)(at % (uint32_t)per_row) * 8 - (c.d - p.rd);
+      if (first + i * threads < pieces) {
+        raw[i] = __ldcs(reinterpret_cast<const uint4*>(p.q + b * p.q_bs + t * p.q_ts + (int64_t)at * 8));
+        col[i] = (int)(at - kv_div(at, per_row, p.row_shift) * per_row) * 8 - (c.d - p.rd);
         if (col[i] >= 0) kv_freq_row(p, b, t, kv_len(c, b) + t, &frow[i]);
+      }
+      at += threads;
+      while (at >= per_token) {
+        at -= per_token;
+        if (++t == c.T) {
+          t = 0;
+          ++b;
+        }
       }
     }
 #pragma unroll
     for (int i = 0; i < KV_Q_PIECES; ++i) {
-      const int64_t e = first + (int64_t)i * threads;
-      if (e >= p.q_pieces) break;
+      const uint32_t e = first + i * threads;
+      if (e >= pieces) break;
       float y[8];
       kv_rotate8(raw[i], y, p.freqs, frow[i], p.rd, col[i]);
       reinterpret_cast<uint4*>(p.q_out)[e] =
@@ -162,7 +178,25 @@ __global__ void __launch_bounds__(512) kv_append_kernel(KvAppendParams p) {
   const int lo = (int)max((int64_t)0, len - start);
   const int hi = (int)min((int64_t)c.block, (int64_t)len + n - start);
   if (hi <= lo) return;
-  const int64_t pi = start / c.page;
+  // the rows are on their way while the page is looked up
+  const uint16_t* x = is_k ? p.k + b * p.k_bs : p.v + b * p.v_bs;
+  const int64_t ts = is_k ? p.k_ts : p.v_ts;
+  const float* freqs = is_k ? p.freqs : nullptr;
+
+  uint4 raw[NP];
+  int row[NP], col[NP];  // of the piece in the block; -1: not the call's
+#pragma unroll
+  for (int i = 0; i < NP; ++i) {
+    const int e = tid + i * threads;
+    row[i] = (int)kv_div(e, per_row, p.row_shift);
+    col[i] = (e - row[i] * per_row) * 8;
+    raw[i] = make_uint4(0, 0, 0, 0);
+    if (row[i] >= lo && row[i] < hi)
+      raw[i] = __ldcs(reinterpret_cast<const uint4*>(x + (start + row[i] - len) * ts + (int64_t)head * c.d + col[i]));
+    else
+      row[i] = -1;
+  }
+  const uint32_t pi = kv_div((uint32_t)min(start, (int64_t)0x7FFFFFFF), c.page, p.page_shift);
   const int32_t pg = pi < c.max_pages ? __ldg(c.table + (int64_t)b * c.max_pages + pi) : -1;
   if (pg < 0 || pg >= c.n_pages) {
     if (tid == 0 && head == 0)
@@ -170,56 +204,44 @@ __global__ void __launch_bounds__(512) kv_append_kernel(KvAppendParams p) {
     return;
   }
   const int64_t unit = (int64_t)pg * c.heads + head;
-  const int in_page = (int)(start - pi * c.page);
+  const int in_page = (int)(start - (int64_t)pi * c.page), in_block = (int)kv_div(in_page, c.block, p.block_shift);
   uint8_t* codes = (is_k ? c.k8 : c.v8) + (unit * c.page + in_page) * c.d;
-  float* scale = (is_k ? c.k_scale : c.v_scale) + unit * (c.page / c.block) + in_page / c.block;
+  float* scale = (is_k ? c.k_scale : c.v_scale) + unit * kv_div(c.page, c.block, p.block_shift) + in_block;
   const float old_raw = lo > 0 ? *scale : 0.f;
-  const uint16_t* x = is_k ? p.k + b * p.k_bs : p.v + b * p.v_bs;
-  const int64_t ts = is_k ? p.k_ts : p.v_ts;
-  const float* freqs = is_k ? p.freqs : nullptr;
-
-  uint4 raw[NP];
-  int row[NP], col[NP];
+  float y[NP][8], amax = 0.f;
 #pragma unroll
   for (int i = 0; i < NP; ++i) {
-    const int e = tid + i * threads;
-    row[i] = e / per_row;
-    col[i] = (e - row[i] * per_row) * 8;
-    const int t = (int)(start + row[i] - len);
-    raw[i] = make_uint4(0, 0, 0, 0);
-    if (row[i] >= lo && row[i] < hi)
-      raw[i] = __ldg(reinterpret_cast<const uint4*>(x + t * ts + (int64_t)head * c.d + col[i]));
-    else
-      row[i] = -1;
+    int fr = 0;
+    const int rc = row[i] < 0 || !freqs ? -1 : col[i] - (c.d - p.rd);
+    if (rc >= 0 && !kv_freq_row(p, b, (int)(start + row[i] - len), (int)start + row[i], &fr))
+      report_bounds(c.status, b, p.n_freqs);
+    kv_rotate8(raw[i], y[i], freqs, fr, p.rd, rc);  // (zeros where the row is not the call's)
+#pragma unroll
+    for (int j = 0; j < 8; ++j) amax = kv_max_nan(amax, fabsf(y[i][j]));
   }
-  float amax = 0.f;
-  bool bad = false;
+  __shared__ float red[2][THREADS / 32];
+  const auto largest = [&](float (&r)[THREADS / 32], float a) {
 #pragma unroll
-  for (int i = 0; i < NP; ++i) {
-    if (row[i] < 0) continue;
-    float y[8];
-    int64_t fr = 0;
-    const int rc = col[i] - (c.d - p.rd);
-    if (freqs && rc >= 0) {
-      const int t = (int)(start + row[i] - len);
-      if (!kv_freq_row(p, b, t, (int)(start + row[i]), &fr)) {
-        report_bounds(c.status, b, (int)min(p.n_freqs, (int64_t)0x7FFFFFFF));
+    for (int o = 16; o > 0; o >>= 1) a = kv_max_nan(a, __shfl_xor_sync(0xFFFFFFFFu, a, o));
+    if ((tid & 31) == 0) r[tid >> 5] = a;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < THREADS / 32; ++w) a = kv_max_nan(a, r[w]);
+    return a;
+  };
+  amax = largest(red[0], amax);
+  bool bad = !(amax < INFINITY);
+  if (bad) {  // (the whole block) the finite ones' largest; the others become NaN
+    amax = 0.f;
+#pragma unroll
+    for (int i = 0; i < NP; ++i)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        if (fabsf(y[i][j]) < INFINITY) amax = fmaxf(amax, fabsf(y[i][j]));
+        else y[i][j] = __uint_as_float(0x7FC00000u);
       }
-    }
-    kv_rotate8(raw[i], y, freqs, fr, p.rd, rc);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const float a = fabsf(y[j]);
-      if (a < INFINITY) amax = fmaxf(amax, a);
-      else bad = true;
-    }
+    amax = largest(red[1], amax);
   }
-  __shared__ float red[16];
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xFFFFFFFFu, amax, o));
-  if ((tid & 31) == 0) red[tid >> 5] = amax;
-  bad = __syncthreads_or(bad);
-  for (int w = 0; w < threads >> 5; ++w) amax = fmaxf(amax, red[w]);
   const uint32_t old_bits = __float_as_uint(old_raw);
   bad |= (old_bits & 1u) != 0;
   const float old = __uint_as_float(old_bits & ~1u);
@@ -243,17 +265,11 @@ __global__ void __launch_bounds__(512) kv_append_kernel(KvAppendParams p) {
 #pragma unroll
   for (int i = 0; i < NP; ++i) {
     if (row[i] < 0) continue;
-    float y[8];
-    int64_t fr = 0;
-    const int rc = col[i] - (c.d - p.rd);
-    if (freqs && rc >= 0) kv_freq_row(p, b, (int)(start + row[i] - len), (int)(start + row[i]), &fr);
-    kv_rotate8(raw[i], y, freqs, fr, p.rd, rc);
 #pragma unroll
-    for (int j = 0; j < 8; ++j)
-      y[j] = fabsf(y[j]) < INFINITY ? y[j] * inv : __uint_as_float(0x7FC00000u);
-    const uint32_t a = cvt_e4m3x2(y[0], y[1]) | (uint32_t)cvt_e4m3x2(y[2], y[3]) << 16;
-    const uint32_t d = cvt_e4m3x2(y[4], y[5]) | (uint32_t)cvt_e4m3x2(y[6], y[7]) << 16;
-    *reinterpret_cast<uint2*>(codes + (int64_t)row[i] * c.d + col[i]) = make_uint2(a, d);
+    for (int j = 0; j < 8; ++j) y[i][j] *= inv;
+    const uint32_t a = cvt_e4m3x2(y[i][0], y[i][1]) | (uint32_t)cvt_e4m3x2(y[i][2], y[i][3]) << 16;
+    const uint32_t d = cvt_e4m3x2(y[i][4], y[i][5]) | (uint32_t)cvt_e4m3x2(y[i][6], y[i][7]) << 16;
+    *reinterpret_cast<uint2*>(codes + row[i] * c.d + col[i]) = make_uint2(a, d);
   }
   if (tid == 0) *scale = __uint_as_float(__float_as_uint(s) | (bad ? 1u : 0u));
 }
