@@ -24,6 +24,15 @@
 // (Expansion is a chain of latencies: with seven warps that also found the addresses themselves it
 // took 3700 cycles a unit, two units a tile, and was what everything waited for.)
 //
+// Bound by the chain scores -> weights -> output and by the expansion, no unit being full (4096
+// tokens of 64 heads of 128 over 12288 keys, under a profiler: tensor cores 36 % of their cycles,
+// issue 57 %, ALU 38 %, exponentials 37 %).  Measured (one B200): that chunk 2240 us, 860 TFLOP/s, in
+// short runs, 2.5-2.6 ms when runs are long enough for the power limit; 2048 tokens of heads of 256
+// 2.5 ms (714 TFLOP/s, expansion bound: a unit is twice as large); 16 trees of 13 tokens, 64 heads
+// on 8, up to 6001 keys 97 us (5 K cycles a tile, 10 us of it the join).  The steps that made
+// the chunk faster, in short runs: 3240 us; codes loaded a unit ahead and no rare path unrolled 2560;
+// buffers of 64 keys 2320; one issuing thread 2265 to 2339; more registers for the expansion 2240.
+//
 // References are raised only when a score passes them by 2^KVA_RISE (rarely after the first
 // tiles); then the row's output is scaled in place once its last product is done.
 #pragma once
@@ -35,7 +44,9 @@ constexpr int KVW_SOFT = 256;                       // softmax threads (the firs
 constexpr int KVW_CONV_WARPS = 7;                   // of either group of expanding warps (the last ones)
 constexpr int KVW_THREADS = KVW_SOFT + 64 + 2 * 32 * KVW_CONV_WARPS;
 // 768 threads start with 80 registers; the softmax warpgroups take theirs from the other four.
-constexpr int KVW_REGS_SOFT = 128, KVW_REGS_REST = 56;
+// (4096 tokens of 64 heads over 12288 keys, softmax / others: 128 / 56 2339 us, 112 / 64 2237 us;
+// 2048 tokens at heads of 192 3806 and 3244 us, of 256 2674 and 2503 us; 96 / 72 is 10 % slower.)
+constexpr int KVW_REGS_SOFT = 112, KVW_REGS_REST = 64;
 static_assert(KVW_THREADS == 768 && 2 * KVW_REGS_SOFT + 4 * KVW_REGS_REST <= 6 * 80, "register split");
 constexpr int KVW_META = 8;                         // units whose addresses are held
 constexpr int KVW_UNITS = 8;                        // most units of the ring
@@ -474,20 +485,19 @@ __global__ void __launch_bounds__(KVW_THREADS, 1) kv_attn_wide_kernel(const __gr
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(KVW_REGS_REST));
     // One thread does all of it: every instruction of this warp is in the chain of products.
     if (elect_one()) {
-    uint32_t unit = 0, q_ph = 0, p_ph = 0;
-    constexpr uint32_t idesc_s = idesc_bf16_f32(128, 64, false, false);
-    constexpr uint32_t idesc_o = idesc_bf16_f32(128, D, false, true);
-    const uint32_t q_desc = kvw_desc(smem_u32(qs), 16), k_desc = kvw_desc(smem_u32(ring), 16),
-                   v_desc = kvw_desc(smem_u32(ring), 16384);
-    bool ok = true;
-    const auto wait = [&](uint64_t* bar, uint32_t ph) {
-      ok = ok && mbar_wait_inl(bar, ph, wc);
-      tc_fence_after();
-      return ok;
-    };
-    // scores of half h of the tile whose keys are in `slot`, into the stream's buffer
-    const auto qk = [&](int stream, int h, int qt, uint32_t slot) {
-      {
+      uint32_t unit = 0, q_ph = 0, p_ph = 0;
+      constexpr uint32_t idesc_s = idesc_bf16_f32(128, 64, false, false);
+      constexpr uint32_t idesc_o = idesc_bf16_f32(128, D, false, true);
+      const uint32_t q_desc = kvw_desc(smem_u32(qs), 16), k_desc = kvw_desc(smem_u32(ring), 16),
+                     v_desc = kvw_desc(smem_u32(ring), 16384);
+      bool ok = true;
+      const auto wait = [&](uint64_t* bar, uint32_t ph) {
+        ok = ok && mbar_wait_inl(bar, ph, wc);
+        tc_fence_after();
+        return ok;
+      };
+      // scores of half h of the tile whose keys are in `slot`, into the stream's buffer
+      const auto qk = [&](int stream, int h, int qt, uint32_t slot) {
         const uint32_t a = q_desc + qt * (TILE >> 4), b = k_desc + slot * (TILE >> 4) + h * (8192 >> 4);
 #pragma unroll
         for (int ks = 0; ks < D / 16; ++ks) {
@@ -495,11 +505,9 @@ __global__ void __launch_bounds__(KVW_THREADS, 1) kv_attn_wide_kernel(const __gr
           kvw_mma_ss(tmem + (2 * stream + h) * 64, a + off, b + off, idesc_s, ks > 0);
         }
         umma_commit(&sh->s_full[2 * stream + h]);
-      }
-    };
-    // a whole tile's, into both of the stream's buffers, which lie side by side
-    const auto qk_tile = [&](int stream, uint32_t slot) {
-      {
+      };
+      // a whole tile's, into both of the stream's buffers, which lie side by side
+      const auto qk_tile = [&](int stream, uint32_t slot) {
         const uint32_t b = k_desc + slot * (TILE >> 4);
 #pragma unroll
         for (int ks = 0; ks < D / 16; ++ks) {
@@ -508,102 +516,96 @@ __global__ void __launch_bounds__(KVW_THREADS, 1) kv_attn_wide_kernel(const __gr
         }
         umma_commit(&sh->s_full[2 * stream]);
         umma_commit(&sh->s_full[2 * stream + 1]);
-      }
-    };
-    const auto pv = [&](int stream, int h, int out, uint32_t slot, bool acc) {
-      {
+      };
+      const auto pv = [&](int stream, int h, int out, uint32_t slot, bool acc) {
         const uint32_t b = v_desc + slot * (TILE >> 4) + h * (8192 >> 4);
 #pragma unroll
         for (int ks = 0; ks < 4; ++ks)
           kvw_mma_ts(tmem + 256 + out * D, tmem + (2 * stream + h) * 64 + ks * 8, b + ks * (2048 >> 4), idesc_o,
                      acc || ks > 0);
         umma_commit(&sh->o_done[2 * stream + h]);
-      }
-    };
-    const auto weights = [&](int stream, int h) {
-      const int buf = 2 * stream + h;
-      const bool there = wait(&sh->p_full[buf], (p_ph >> buf) & 1);
-      p_ph ^= 1u << buf;
-      return there;
-    };
-    const auto commit = [&](uint64_t* bar) {
-      umma_commit(bar);
-    };
-    for (; w.left > 0 && ok; w.next(p)) {
-      if (!w.any()) continue;
-      const int n = w.t1 - w.t0;
-      const bool two = rows256 && w.rt * 256 + 128 < p.rows;
-      if (!wait(&sh->q_full, q_ph)) break;
-      q_ph ^= 1;
-      // unit i of the row tile: waits for it and gives its slot
-      const uint32_t base = unit;
-      const auto take = [&](int i, uint32_t* slot) {
-        const uint32_t u = base + i;
-        *slot = u % UNITS;
-        return wait(&sh->full[*slot], (u / UNITS) & 1);
       };
-      uint32_t vs, ks;
-      if (two) {
-        if (!take(0, &ks)) break;
-        for (int q = 0; q < 4; ++q) qk(q & 1, q >> 1, q & 1, ks);
-        commit(&sh->free[ks]);
-        if (n == 1) commit(&sh->q_free);
-        for (int j = 0; j < n && ok; ++j) {
-          if (!take(2 * j + 1, &vs)) break;
-          for (int q = 0; q < 4; ++q) {
-            const int s = q & 1, h = q >> 1;
-            if (!weights(s, h)) break;
-            pv(s, h, s, vs, j > 0 || h > 0);
-            if (q == 3) commit(&sh->free[vs]);
-            if (j + 1 < n) {
-              if (q == 0 && !take(2 * j + 2, &ks)) break;
-              qk(s, h, s, ks);
+      const auto weights = [&](int stream, int h) {
+        const int buf = 2 * stream + h;
+        const bool there = wait(&sh->p_full[buf], (p_ph >> buf) & 1);
+        p_ph ^= 1u << buf;
+        return there;
+      };
+      for (; w.left > 0 && ok; w.next(p)) {
+        if (!w.any()) continue;
+        const int n = w.t1 - w.t0;
+        const bool two = rows256 && w.rt * 256 + 128 < p.rows;
+        if (!wait(&sh->q_full, q_ph)) break;
+        q_ph ^= 1;
+        // unit i of the row tile: waits for it and gives its slot
+        const uint32_t base = unit;
+        const auto take = [&](int i, uint32_t* slot) {
+          const uint32_t u = base + i;
+          *slot = u % UNITS;
+          return wait(&sh->full[*slot], (u / UNITS) & 1);
+        };
+        uint32_t vs, ks;
+        if (two) {
+          if (!take(0, &ks)) break;
+          for (int q = 0; q < 4; ++q) qk(q & 1, q >> 1, q & 1, ks);
+          umma_commit(&sh->free[ks]);
+          if (n == 1) umma_commit(&sh->q_free);
+          for (int j = 0; j < n && ok; ++j) {
+            if (!take(2 * j + 1, &vs)) break;
+            for (int q = 0; q < 4; ++q) {
+              const int s = q & 1, h = q >> 1;
+              if (!weights(s, h)) break;
+              pv(s, h, s, vs, j > 0 || h > 0);
+              if (q == 3) umma_commit(&sh->free[vs]);
+              if (j + 1 < n) {
+                if (q == 0 && !take(2 * j + 2, &ks)) break;
+                qk(s, h, s, ks);
+              }
+            }
+            if (ok && j + 1 < n) {
+              umma_commit(&sh->free[ks]);
+              if (j + 2 == n) umma_commit(&sh->q_free);
             }
           }
-          if (ok && j + 1 < n) {
-            commit(&sh->free[ks]);
-            if (j + 2 == n) commit(&sh->q_free);
+        } else {
+          for (int j = 0; j < min(n, 2) && ok; ++j) {
+            if (!take(j, &ks)) break;
+            // (wide heads wait for the tensor cores, which 64 keys at a time would feed from shared
+            // memory at two thirds of their rate)
+            if constexpr (ONE_OUT) {
+              qk_tile(j, ks);
+            } else {
+              qk(j, 0, 0, ks);
+              qk(j, 1, 0, ks);
+            }
+            umma_commit(&sh->free[ks]);
+            if (j + 1 == n) umma_commit(&sh->q_free);
           }
-        }
-      } else {
-        for (int j = 0; j < min(n, 2) && ok; ++j) {
-          if (!take(j, &ks)) break;
-          // (wide heads wait for the tensor cores, which 64 keys at a time would feed from shared
-          // memory at two thirds of their rate)
-          if constexpr (ONE_OUT) {
-            qk_tile(j, ks);
-          } else {
-            qk(j, 0, 0, ks);
-            qk(j, 1, 0, ks);
-          }
-          commit(&sh->free[ks]);
-          if (j + 1 == n) commit(&sh->q_free);
-        }
-        for (int j = 0; j < n && ok; ++j) {
-          const int s = j & 1;
-          // values of tile j: unit 1 of a single tile; else 2 + 2 j, the last one 2 n - 1
-          if (!take(n == 1 ? 1 : j + 1 == n ? 2 * n - 1 : 2 + 2 * j, &vs)) break;
-          for (int h = 0; h < 2; ++h) {
-            if (!weights(s, h)) break;
-            pv(s, h, ONE_OUT ? 0 : s, vs, h > 0 || (ONE_OUT ? j > 0 : j > 1));
-            if (h == 1) commit(&sh->free[vs]);
-            if (j + 2 < n) {
-              if (h == (ONE_OUT ? 1 : 0) && !take(2 * j + 3, &ks)) break;
-              if constexpr (!ONE_OUT) qk(s, h, 0, ks);
-              else if (h == 1) qk_tile(s, ks);
+          for (int j = 0; j < n && ok; ++j) {
+            const int s = j & 1;
+            // values of tile j: unit 1 of a single tile; else 2 + 2 j, the last one 2 n - 1
+            if (!take(n == 1 ? 1 : j + 1 == n ? 2 * n - 1 : 2 + 2 * j, &vs)) break;
+            for (int h = 0; h < 2; ++h) {
+              if (!weights(s, h)) break;
+              pv(s, h, ONE_OUT ? 0 : s, vs, h > 0 || (ONE_OUT ? j > 0 : j > 1));
+              if (h == 1) umma_commit(&sh->free[vs]);
+              if (j + 2 < n) {
+                if (h == (ONE_OUT ? 1 : 0) && !take(2 * j + 3, &ks)) break;
+                if constexpr (!ONE_OUT) qk(s, h, 0, ks);
+                else if (h == 1) qk_tile(s, ks);
+              }
+            }
+            if (ok && j + 2 < n) {
+              umma_commit(&sh->free[ks]);
+              if (j + 3 == n) umma_commit(&sh->q_free);
             }
           }
-          if (ok && j + 2 < n) {
-            commit(&sh->free[ks]);
-            if (j + 3 == n) commit(&sh->q_free);
-          }
         }
+        unit += 2 * n;
       }
-      unit += 2 * n;
-    }
-    // every product and arrival in flight has landed before the CTA gives its memory back
-    commit(&sh->drain);
-    mbar_wait_body(&sh->drain, 0, wc, false, true);
+      // every product and arrival in flight has landed before the CTA gives its memory back
+      umma_commit(&sh->drain);
+      mbar_wait_body(&sh->drain, 0, wc, false, true);
     }
     __syncwarp();
   } else if (warp == 9) {
