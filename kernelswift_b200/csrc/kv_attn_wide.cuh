@@ -45,7 +45,7 @@ constexpr int KVW_CONV_WARPS = 7;                   // of either group of expand
 constexpr int KVW_THREADS = KVW_SOFT + 64 + 2 * 32 * KVW_CONV_WARPS;
 // 768 threads start with 80 registers; the softmax warpgroups take theirs from the other four.
 // (4096 tokens of 64 heads over 12288 keys, softmax / others: 128 / 56 2339 us, 112 / 64 2237 us;
-// 2048 tokens at heads of 192 3806 and 3244 us, of 256 2674 and 2503 us; 96 / 72 is 10 % slower.)
+// 2048 tokens at heads of 256 2674 and 2503 us; 96 / 72 is 10 % slower.)
 constexpr int KVW_REGS_SOFT = 112, KVW_REGS_REST = 64;
 static_assert(KVW_THREADS == 768 && 2 * KVW_REGS_SOFT + 4 * KVW_REGS_REST <= 6 * 80, "register split");
 constexpr int KVW_META = 8;                         // units whose addresses are held
@@ -59,6 +59,8 @@ constexpr uint32_t KVW_TILE = 128u * D * 2;         // bytes of a unit, and of 1
 template <int D>
 __host__ __device__ constexpr int kvw_units() {
   const int n = (int)((232448 - 1024 - KVW_HDR - KVW_STREAM_OUT<D> * KVW_TILE<D>) / KVW_TILE<D>);
+  // (an odd number, three for D = 192, gives a slot's units to the expanding groups by turns; a group
+  // is then at most a phase ahead because units are given back in order.  Two: 8 % slower)
   return n < KVW_UNITS ? n : KVW_UNITS;
 }
 
@@ -704,12 +706,13 @@ __global__ void __launch_bounds__(KVW_THREADS, 1) kv_attn_wide_kernel(const __gr
     // swizzles differ in the lowest bit, so they meet no bank twice
     const int group = (warp - 10) / KVW_CONV_WARPS, cw = (warp - 10) % KVW_CONV_WARPS;
     const int k0 = D == 64 ? lane >> 2 : ((lane >> 2) & 1) + (D == 128 ? 2 * (lane >> 4) : 0);
-    const int c = D == 64 ? lane & 3 : (lane & 3) + 4 * (D == 128 ? (lane >> 3) & 1 : lane >> 3);
-    const bool on = c < P16;                       // (D = 192: 24 lanes of a warp)
+    // (D = 192: the last eight lanes do what the eight before them do; left out, they made every
+    // step a branch of its own: 2048 tokens, 64 heads over 12288 keys 3244 us, so 2446)
+    const int c = D == 64 ? lane & 3 : (lane & 3) + 4 * (D == 128 ? (lane >> 3) & 1 : min(lane >> 3, P16 / 4 - 1));
     uint32_t code[AHEAD][4];
     const auto load = [&](int q, const KvwMeta& m, const uint8_t* src, uint32_t (&v)[4]) {
       const int step = cw + q * KVW_CONV_WARPS, key = step * KEYS;
-      if (step < STEPS && on) kvf_load<4>(v, src + (int64_t)m.place[(key >> 4) & 7] * (16 * D) + (key & 15) * D);
+      if (step < STEPS) kvf_load<4>(v, src + (int64_t)m.place[(key >> 4) & 7] * (16 * D) + (key & 15) * D);
     };
     const auto source = [&](uint32_t flags) { return (flags & KVW_VALUES ? p.c.v8 : p.c.k8) + (k0 * D + c * 16); };
     const auto known = [&](uint32_t u, uint32_t* flags) {
@@ -750,7 +753,7 @@ __global__ void __launch_bounds__(KVW_THREADS, 1) kv_attn_wide_kernel(const __gr
           const int step = cw + q * KVW_CONV_WARPS;
           uint32_t x[8];
           expand(code[q % AHEAD], m.factor[(step * KEYS >> 4) & 7], x);
-          if (step < STEPS && on) store(step, x);
+          if (step < STEPS) store(step, x);
           if (q + AHEAD < NP) load(q + AHEAD, m, src, code[q % AHEAD]);
           else if (more) load(q + AHEAD - NP, next, src_next, code[q % AHEAD]);
         }
@@ -779,7 +782,7 @@ __global__ void __launch_bounds__(KVW_THREADS, 1) kv_attn_wide_kernel(const __gr
               x[2 * h + y] = z;
             }
           }
-          if (step < STEPS && on) store(step, x);
+          if (step < STEPS) store(step, x);
         }
         if (more) {
 #pragma unroll
