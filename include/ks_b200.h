@@ -344,7 +344,8 @@ int ks_verify_draft(const float* p, const float* q, const void* tokens, int32_t 
  * scale = the smallest power of two >= max(amax, 1e-4) / 448 (at most 2^119) over the new rows of
  * the block, and not less than before where the block holds rows below lens[b], which are
  * then rounded again to it; code = e4m3(x / scale).  An element that is NaN or infinite becomes
- * e4m3's NaN, and the lowest bit of its block's scale is set.  D 64, 128, 192 or 256; block a
+ * e4m3's NaN, and the lowest bit of its block's scale is set.  A block that is written belongs to
+ * one sequence of the call (full ones before it may be shared).  D 64, 128, 192 or 256; block a
  * multiple of 16 up to 128, page of block.  Rows behind a sequence's last are left as they
  * were.  Tokens past the table or on a page outside [0, n_pages) are not stored, positions
  * outside freqs take its nearest row; both are reported by ks_device_status.  lens is not
@@ -366,8 +367,8 @@ int ks_kv_append(const void* k, int64_t k_bs, int64_t k_ts, const void* v, int64
  *          of the call's own tokens, cached at lens[b] .., those j < n_new[b] with mask[b, t, j]
  *          (bytes [B, T, T]; NULL: j <= t); the others get zeros
  *   attn_sink fp32 [H] or NULL: a logit per head that takes part in the softmax without a value
- * Scores, sums and outputs are fp32, weights enter the product with the values in bf16, the
- * result is rounded once.  A token that sees nothing gets zeros.  Positions past the table or
+ * Scores, sums and outputs are fp32; weights enter the product with the values in 16 bits, off by
+ * at most 2^-8 of themselves or 2^-32 of the row's largest; the result is rounded once.  A token that sees nothing gets zeros.  Positions past the table or
  * on a page outside [0, n_pages) are not seen; both are reported by ks_device_status.
  * workspace: ks_kv_attn_workspace_size bytes, 256-byte aligned, used by this call alone until it
  * is done.  No counterpart in the reference.

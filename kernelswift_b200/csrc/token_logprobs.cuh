@@ -21,12 +21,12 @@
 // Sums are in fp32 relative to the thread's maximum, merged by the usual rescaling.
 //
 // Bound by reading the logits; per value about 5 instructions, one of them an exponential (16 a
-// cycle and SM).  Measured (device time, one B200): 2048 rows of 129280 bf16 values 100 us (530 MB:
-// 5.3 TB/s, 0.82 of a copy's rate), with 20 alternatives 126 us; 4096 rows of 32003 fp32 values 100
-// us; 8 rows of 129280 values with 5 alternatives 13 us.  Forms that held a slice of the row per
-// CTA in registers and met in barriers before and after the search took 342 us (a bound per
-// slice, so k values of each to rank) and 406 us (a bound per row) with 20 alternatives; each
-// thread reading its own batches again, 164 us.
+// cycle and SM).  Measured (one B200): 2048 rows of 129280 bf16 values with 20 alternatives 119
+// us (530 MB: 4.5 TB/s, 0.69 of a copy's rate), without 100; 4096 rows of 32003 fp32 values 92
+// us (5.7 TB/s); 8 rows of 129280 values with 5 alternatives 9 us on the device.  Forms that held
+// a slice of the row per CTA in registers and met in barriers before and after the search took 342
+// us (a bound per slice, so k values of each to rank) and 406 us (a bound per row) with 20
+// alternatives; each thread reading its own batches again, 164 us.
 #pragma once
 #include "ks_device.cuh"
 

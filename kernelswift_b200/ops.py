@@ -713,9 +713,11 @@ def kv_append(k: torch.Tensor, v: torch.Tensor, k8: torch.Tensor, k_scale: torch
     k8, v8 float8_e4m3fn [pages, heads, page, D], k_scale, v_scale fp32 [pages, heads, page /
     block]; page_table int32 [B, max_pages]; D 64, 128, 192 or 256, block a multiple of 16 up to
     128.  One power-of-two scale per block of tokens and head, the smallest that takes the
-    largest element (at most 448 scales); where a block holds tokens already its scale only grows, and they are rounded
-    again to it.  An element that is NaN or infinite reads as NaN, and the lowest bit of its
-    block's scale is set.  lens is not changed: add n_new to it after the last layer."""
+    largest element (at most 448 scales); where a block holds tokens already its scale only
+    grows, and they are rounded again to it.  An element that is NaN or infinite reads as NaN,
+    and the lowest bit of its block's scale is set.  A block that is written belongs to one
+    sequence of the call; full ones before it (a common prefix) may be shared.  lens is not
+    changed: add n_new to it after the last layer."""
     shape = k.shape
     if len(shape) != 4:
         raise RuntimeError("kv_append: k must be bfloat16 [b, t, heads, d]")
@@ -777,8 +779,11 @@ def kv_attn(q: torch.Tensor, k8: torch.Tensor, k_scale: torch.Tensor, v8: torch.
     of the new ones those with ``mask[b, t, j]`` (bool [B,T,T]; None: j <= t).  With n_new
     (int32 [B]) sequence b has n_new[b] of the T tokens; the rows of the others are zeros.
     attn_sink fp32 [H] as in ``sparse_attn``.  Returns bf16 [B,T,H,D]; a token that sees
-    nothing gets zeros.  Weights enter their product in bf16 (2^-8 of themselves), scores
-    and sums are fp32, the result is rounded once."""
+    nothing gets zeros.  Weights enter their product in 16 bits (off by at most 2^-8 of
+    themselves or 2^-32 of the row's largest), scores and sums are fp32, the result is
+    rounded once.  workspace: ``kv_attn_workspace_size(T, H, heads, D)`` bytes, 256-byte
+    aligned, used by this call alone until it is done (None: allocated); out: where the
+    result goes."""
     shape = q.shape
     if q.dtype != torch.bfloat16 or len(shape) != 4:
         raise RuntimeError("kv_attn: q must be bfloat16 [b, t, h, d]")

@@ -294,6 +294,28 @@ def test_large_rows_without_weight(cuda_ok, T, big):
     check(q, parts, table, lens, 0.1)
 
 
+@pytest.mark.parametrize("T", [1, 40])
+@pytest.mark.parametrize("down", [5.0, 21.0, 24.0, 60.0])
+def test_weights_far_below_the_largest(cuda_ok, T, down):
+    """Rows whose largest weights meet zeros only: what shows is weights of e^-down.  Each may be
+    off by 2^-32 of the largest, so an output by 2^-32 sum |v| more than elsewhere."""
+    from kernelswift_b200 import ops
+
+    g, q, parts, table, lens = make(1, T, 8, 2, 128, 64, 16, [200], 40)
+    q.fill_(1.0)
+    first = table[0, 0].long()
+    parts[1].fill_(2.0 ** -7)
+    parts[0].view(torch.uint8).fill_(0xB8)  # -1: scores of -128 * 2^-7 times the softmax scale
+    for x in (parts[0], parts[2]):
+        x.view(torch.uint8)[first] = 0  # 64 keys with scores of 0 and no values
+    got = ops.kv_attn(q, *parts, table, lens, down).double()
+    ops.device_status()
+    ref, size, off = reference(q, parts, table, lens, down)
+    most = sum(head_rows(parts[2], parts[3], table[0], h, 200 + T).abs().sum(0).max() for h in range(2))
+    lim = 2.0 ** -8 * ref.abs() + (2.0 ** -8 + 2.0 ** -16 + off) * size + 2.0 ** -32 * most
+    assert ((got - ref).abs() <= lim).all()
+
+
 @pytest.mark.parametrize("T", [1, 2, 40])
 @pytest.mark.parametrize("big,key", [(2.0 ** 20, 1), (2.0 ** 60, 0), (2.0 ** 100, 0), (2.0 ** 126, 0), (2.0 ** 40, 1), (2.0 ** -130, 1)])
 def test_queries_of_any_size_within_a_row(cuda_ok, T, big, key):
