@@ -24,14 +24,15 @@
 // (Expansion is a chain of latencies: with seven warps that also found the addresses themselves it
 // took 3700 cycles a unit, two units a tile, and was what everything waited for.)
 //
-// Bound by the chain scores -> weights -> output and by the expansion, no unit being full (4096
-// tokens of 64 heads of 128 over 12288 keys, under a profiler: tensor cores 36 % of their cycles,
-// issue 57 %, ALU 38 %, exponentials 37 %).  Measured (one B200): that chunk 2240 us, 860 TFLOP/s, in
-// short runs, 2.5-2.6 ms when runs are long enough for the power limit; 2048 tokens of heads of 256
-// 2.5 ms (714 TFLOP/s, expansion bound: a unit is twice as large); 16 trees of 13 tokens, 64 heads
-// on 8, up to 6001 keys 97 us (5 K cycles a tile, 10 us of it the join).  The steps that made
-// the chunk faster, in short runs: 3240 us; codes loaded a unit ahead and no rare path unrolled 2560;
-// buffers of 64 keys 2320; one issuing thread 2265 to 2339; more registers for the expansion 2240.
+// Bound by the chain scores -> weights -> output and by the expansion, no unit being full (1024
+// tokens of 64 heads of 128 on 8 behind 12288, under a profiler: tensor cores 41 % of their cycles,
+// issue 59 %, ALU 44 %, exponentials 41 %).  Measured (one B200): 4096 such tokens 2240 us, 860
+// TFLOP/s, in short runs, 2443 us in runs long enough for the power limit; 2048 tokens of heads of
+// 256 2.5 ms (714 TFLOP/s, expansion bound: a unit is twice as large); 16 trees of 13 tokens, 64
+// heads on 8, up to 6001 keys 92 us (5 K cycles a tile, 10 us of it the join).  The steps that made
+// the 4096 tokens faster, in short runs: 3240 us; codes loaded a unit ahead and no rare path unrolled
+// 2560; buffers of 64 keys 2320; one issuing thread 2265 to 2339; more registers for the expansion
+// 2240.
 //
 // References are raised only when a score passes them by 2^KVA_RISE (rarely after the first
 // tiles); then the row's output is scaled in place once its last product is done.
