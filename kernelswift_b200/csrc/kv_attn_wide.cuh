@@ -255,11 +255,11 @@ __global__ void __launch_bounds__(KVW_THREADS, 1) kv_attn_wide_kernel(const __gr
       const int n = w.t1 - w.t0;
       const bool two = rows256 && r0 + 128 < p.rows;  // both streams on every tile
       // ------------------------------------------------------------ queries
-      if (!first) {
-        if (!mbar_wait_inl(&sh->q_free, (item - 1) & 1, wc)) break;
-      }
-      first = false;
+      // (with one output the second warpgroup writes no queries, so nothing waits for it and q_free may
+      // complete twice before it looks: it has no part in that barrier)
       if (!ONE_OUT || wg == 0) {
+        if (!first && !mbar_wait_inl(&sh->q_free, (item - 1) & 1, wc)) break;
+        first = false;
         const int base = !rows256 ? 0 : wg * 128;  // rows of this warpgroup's queries
         if (rows256 || ONE_OUT || wg == 0) {
           uint8_t* dst = qs + (rows256 ? wg : 0) * TILE;

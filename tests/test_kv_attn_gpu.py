@@ -445,3 +445,19 @@ def test_empty_calls(cuda_ok):
     with pytest.raises(RuntimeError, match="64, 128, 192 or 256"):
         ops.kv_attn(q[..., :32].contiguous(), parts[0][..., :32].contiguous(), parts[1], parts[2][..., :32].contiguous(),
                     parts[3], table, lens, 0.1)
+
+
+@pytest.mark.parametrize("d", [192, 256])
+@pytest.mark.parametrize("T,longest", [(3, 40), (9, 300)])
+def test_many_short_row_tiles_of_wide_heads(cuda_ok, d, T, longest):
+    """Every CTA of the kernel for many rows goes through a dozen row tiles of one to three tiles each,
+    call after call: its warpgroups stay in step, and no wait runs out."""
+    from kernelswift_b200 import ops
+
+    lens = [(i * 37) % longest for i in range(450)]
+    g, q, parts, table, lens = make(450, T, 16, 4, d, 64, 16, lens, d + T)
+    want = check(q, parts, table, lens, d ** -0.5)
+    for _ in range(100):
+        got = ops.kv_attn(q, *parts, table, lens, d ** -0.5)
+    assert torch.equal(got, want)
+    ops.device_status()
