@@ -258,7 +258,8 @@ __global__ void __launch_bounds__(KVW_THREADS, 1) kv_attn_wide_kernel(const __gr
       // (with one output the second warpgroup writes no queries, so nothing waits for it and q_free may
       // complete twice before it looks: it has no part in that barrier)
       if (!ONE_OUT || wg == 0) {
-        if (!first && !mbar_wait_inl(&sh->q_free, (item - 1) & 1, wc)) break;
+        // (a warp gives up as one: a lane that left alone would be missed at the warp's next barrier)
+        if (!first && !__all_sync(0xFFFFFFFFu, mbar_wait_inl(&sh->q_free, (item - 1) & 1, wc))) break;
         first = false;
         const int base = !rows256 ? 0 : wg * 128;  // rows of this warpgroup's queries
         if (rows256 || ONE_OUT || wg == 0) {
