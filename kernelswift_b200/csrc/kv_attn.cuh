@@ -320,7 +320,8 @@ struct KvfShared {
 };
 static_assert(sizeof(KvfShared<16>) <= KVF_HDR, "KvfShared exceeds its header");
 
-// Scales (bits) of a chunk; ks = KVF_GONE: the page is not there.
+// Scales (bits) of a chunk; ks = KVF_GONE: the page is not there (the first page's codes stand in for
+// it, in bounds, with weights and a value scale of zero).
 struct KvfChunk {
   uint32_t ks, vs;
 };
@@ -379,7 +380,7 @@ __global__ void __launch_bounds__(KVF_WARPS * 32, D * NT <= 128 ? 2 : 1) kv_attn
         const uint32_t si = unit * (uint32_t)per_page + (uint32_t)kva_div(in, p.c.block, p.block_shift);
         place = unit * (uint32_t)(p.c.page >> 4) + (uint32_t)(in >> 4);
         ks32 = ok ? __float_as_uint(__ldg(p.c.k_scale + si)) : KVF_GONE;
-        vs32 = __float_as_uint(__ldg(p.c.v_scale + si));
+        vs32 = ok ? __float_as_uint(__ldg(p.c.v_scale + si)) : 0u;
       }
     };
     // starts the copies of the n-th chunk from the first
@@ -592,7 +593,7 @@ __global__ void __launch_bounds__(KVF_WARPS * 32, D * NT <= 128 ? 2 : 1) kv_attn
       // ---------------------------------------------------------- outputs
       if (!open) {
         // codes that are NaN (also those behind the last row, of which nothing is known) count
-        // as zero in the product; the rows that see them get NaN
+        // as zero in the product; the rows that see them get NaN (none sees a page that is not there)
         uint32_t bits[4];  // of the lane's four keys, by its columns
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -612,7 +613,7 @@ __global__ void __launch_bounds__(KVF_WARPS * 32, D * NT <= 128 ? 2 : 1) kv_attn
           for (int i = 0; i < 4; ++i) {
             const uint32_t of = __shfl_sync(0xFFFFFFFFu, bits[i], (lane & ~3) | y);
             const int at = pos + kvf_key<D>(2 * y + (i & 1)) + (i >> 1) * 8;
-            if (of) {
+            if (of && there) {
 #pragma unroll
               for (int g = 0; g < NT; ++g)
 #pragma unroll

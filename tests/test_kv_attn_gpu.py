@@ -461,3 +461,29 @@ def test_many_short_row_tiles_of_wide_heads(cuda_ok, d, T, longest):
         got = ops.kv_attn(q, *parts, table, lens, d ** -0.5)
     assert torch.equal(got, want)
     ops.device_status()
+
+
+@pytest.mark.parametrize("T", [1, 4, 40])
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("codes,bits", [(0x7F, 0x7F800000), (0xFF, 0x7FC00001), (0x7F, 0x3C000001)])
+def test_missing_pages_are_not_seen_whatever_the_first_page_holds(cuda_ok, T, d, codes, bits):
+    """Pages outside the pool: the result is that of the sequence without them.  The pool's first
+    page is nobody's, all NaN codes, its scales infinite, NaN or marked."""
+    from kernelswift_b200 import ops
+
+    g, q, parts, table, lens = make(2, T, 8, 2, d, 64, 16, [200, 90], 44 + T + d)
+    spare = next(p for p in range(parts[0].shape[0]) if p and not (table == p).any())
+    table[table == 0] = spare
+    for i in (0, 2):
+        parts[i].view(torch.uint8)[0] = codes
+        parts[i + 1].view(torch.int32)[0] = bits
+    # the first sequence loses two pages in its middle, the second its last ones, its own tokens' among them
+    bad, left = table.clone(), table.clone()
+    bad[0, 1], bad[0, 2], bad[1, 1:] = -1, 10 ** 7, parts[0].shape[0]
+    left[0, 1:-2] = table[0, 3:]
+    mask = torch.ones(2, T, T, device="cuda").tril().bool()
+    mask[1] = False
+    got = ops.kv_attn(q, *parts, bad, lens, 0.1)
+    with pytest.raises(RuntimeError, match="index"):
+        ops.device_status()
+    check(q, parts, left, torch.tensor([200 - 128, 64], device="cuda"), 0.1, got=got, mask=mask)
