@@ -418,7 +418,6 @@ __global__ void __launch_bounds__(KVF_WARPS * 32, D * NT <= 128 ? 2 : 1) kv_attn
 #pragma unroll
     for (int g = 0; g < NT; ++g) {
       const uint16_t* qp = query_row(g);
-      const bool in = r0 + g * 8 + r < p.rows;
       // exponents of the largest and the least element (bits of |x|, zeros left out)
       uint32_t most = 0, least = 0x7F80u;
 #pragma unroll
@@ -437,18 +436,26 @@ __global__ void __launch_bounds__(KVF_WARPS * 32, D * NT <= 128 ? 2 : 1) kv_attn
         most = max(most, __shfl_xor_sync(0xFFFFFFFFu, most, x));
         least = min(least, __shfl_xor_sync(0xFFFFFFFFu, least, x));
       }
-      const int top = (int)(most >> 7) - 127, low = (int)(least >> 7) - 127;
-      sh[g] = min(14 - top, 126);
-      if (in && most < 0x7F80u && low < top) terms = max(terms, (top - low) / KVF_TERM + 1);
+      // (numbers below 2^-126 have the exponent of their first bit)
+      const int top = (int)(most >> 7) - 127, low = least < 128u ? -102 - __clz(least) : (int)(least >> 7) - 127;
+      sh[g] = 14 - top;
+      if (r0 + g * 8 + r < p.rows && most < 0x7F80u && low < top) terms = max(terms, (top - low) / KVF_TERM + 1);
+    }
+    terms = __reduce_max_sync(0xFFFFFFFFu, terms);
 #pragma unroll
-      for (int j = 0; j < KJ; ++j) kvf_query(qp + 64 * j, in, sh[g], true, qf[g][j]);
+    for (int g = 0; g < NT; ++g) {
+      // Every row goes through as many terms as the one that needs most.  Their windows follow each
+      // other without overlap: a row's first factor is small enough for its last one to be at most
+      // 2^126, whose window reaches down to 2^-141, below bf16's least number.
+      sh[g] = min(sh[g], 126 - KVF_TERM * (terms - 1));
+#pragma unroll
+      for (int j = 0; j < KJ; ++j) kvf_query(query_row(g) + 64 * j, r0 + g * 8 + r < p.rows, sh[g], true, qf[g][j]);
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         const int back = -__shfl_sync(0xFFFFFFFFu, sh[g], (2 * c + i) * 4);
         qsc[g][i] = p.scale_log2 * kvf_pow2(back);
       }
     }
-    terms = __reduce_max_sync(0xFFFFFFFFu, terms);
     float m[NT][2], mu[NT][2], l[NT][2], o[NT][D / 16][4];
     uint32_t nanv[NT][2];  // columns of the lane's outputs that are NaN
 #pragma unroll
@@ -515,7 +522,7 @@ __global__ void __launch_bounds__(KVF_WARPS * 32, D * NT <= 128 ? 2 : 1) kv_attn
         for (int g = 0; g < NT; ++g) {
           float s1[4] = {0.f, 0.f, 0.f, 0.f};
           const uint16_t* qp = query_row(g);
-          const int sh1 = min(sh[g] + KVF_TERM * t, 126);
+          const int sh1 = sh[g] + KVF_TERM * t;
 #pragma unroll
           for (int j = 0; j < KJ; ++j) {
             uint32_t q1[4][2];

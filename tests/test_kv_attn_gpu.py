@@ -487,3 +487,32 @@ def test_missing_pages_are_not_seen_whatever_the_first_page_holds(cuda_ok, T, d,
     with pytest.raises(RuntimeError, match="index"):
         ops.device_status()
     check(q, parts, left, torch.tensor([200 - 128, 64], device="cuda"), 0.1, got=got, mask=mask)
+
+
+@pytest.mark.parametrize("T", [1, 4])
+@pytest.mark.parametrize("top", [0, 14, 40, 97, 120])
+@pytest.mark.parametrize("small", [112, 115, 118, 121, 124, 127, 130, 132])
+def test_small_elements_of_a_query_count_once(cuda_ok, T, top, small):
+    """Elements of 2^-small, down to bf16's least numbers, beside ones of 2^-top that meet zero keys, in
+    every other head; the heads between have small ones alone.  The keys and the softmax scale
+    bring the small ones back."""
+    g, q, parts, table, lens = make(1, T, 8, 2, 64, 64, 16, [300], small * 100 + top)
+    e = torch.full((8, 64), -float(small), dtype=torch.float64, device="cuda")
+    e[::2, ::4] = -float(top)
+    q = (q.double() * torch.exp2(e)).bfloat16()
+    parts[0].view(torch.uint8)[..., ::4] = 0
+    parts[1].mul_(2.0 ** 20)
+    check(q, parts, table, lens, 2.0 ** (small - 22))
+
+
+@pytest.mark.parametrize("T", [1, 4])
+@pytest.mark.parametrize("d", [64, 256])
+def test_rows_beside_a_widely_spread_one_lose_nothing(cuda_ok, T, d):
+    """Every other head has elements of 2^120, which meet zero keys, and of 2^-130; the heads between have
+    ordinary ones, and some of 2^-25."""
+    g, q, parts, table, lens = make(1, T, 8, 2, d, 64, 16, [300], 45 + T)
+    q[..., ::2, ::4] *= 2.0 ** 120
+    q[..., ::2, 1::4] *= 2.0 ** -130
+    q[..., 1::2, 2::4] *= 2.0 ** -25
+    parts[0].view(torch.uint8)[..., ::4] = 0
+    check(q, parts, table, lens, 0.1)
