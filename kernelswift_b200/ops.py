@@ -707,8 +707,9 @@ def kv_append(k: torch.Tensor, v: torch.Tensor, k8: torch.Tensor, k_scale: torch
     (int32 [B]; None: T).  freqs fp32 [P, rope_dim/2, 2] (cos, sin) rotates the last
     rope_dim columns of a key, as pairs (2i, 2i+1), by row ``positions[b, t]`` (int32 [B,T];
     None: lens[b] + t; a drafted tree's tokens have their depths'), before it is rounded.
-    With ``q`` bf16 [B,T,H,D] the queries are rotated too: returns them, bf16 [B,T,H,D] (q
-    itself without freqs), else None.
+    With ``q`` bf16 [B,T,H,D] the queries are rotated too: returns them, contiguous as
+    ``kv_attn`` takes them, bf16 [B,T,H,D] (without freqs q itself, or its copy where it is a
+    slice), else None.
 
     k8, v8 float8_e4m3fn [pages, heads, page, D], k_scale, v_scale fp32 [pages, heads, page /
     block]; page_table int32 [B, max_pages]; D 64, 128, 192 or 256, block a multiple of 16 up to
@@ -749,7 +750,7 @@ def kv_append(k: torch.Tensor, v: torch.Tensor, k8: torch.Tensor, k_scale: torch
         rows = (k, v, q)
     _on_one_device("kv_append", ts, rows)
     turn = q is not None and rope_dim > 0
-    q_out = q.new_empty(of_q) if turn else q
+    q_out = q.new_empty(of_q) if turn else None if q is None else q.contiguous()
     with _on(k8):
         check(lib().ks_kv_append(k.data_ptr(), k_bs, k_ts, v.data_ptr(), v_bs, v_ts,
                                  q.data_ptr() if turn else None, q_bs, q_ts, H, q_out.data_ptr() if turn else None,

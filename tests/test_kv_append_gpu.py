@@ -251,3 +251,20 @@ def test_streams_and_graphs(cuda_ok):
     assert torch.equal(out, out2)
     graph.replay()  # the same rows again change nothing
     same(parts, want)
+
+
+def test_queries_that_are_not_rotated_go_on_to_attention(cuda_ok):
+    """Without freqs, slices of one projection: what comes back is what kv_attn takes."""
+    from kernelswift_b200 import ops
+
+    B, T, H, heads, d = 2, 3, 8, 2, 128
+    g, table, n, parts = make(B, heads, d, 64, 16, [30, 7], T, 23)
+    wide = rows(g, B, T, H + 2 * heads, d, 0)
+    q, k, v = wide.split([H, heads, heads], 2)
+    want = expect(k, v, parts, table, n, None)
+    out = ops.kv_append(k, v, *parts, table, n, q=q)
+    same(parts, want)
+    assert out.is_contiguous() and torch.equal(out, q)
+    whole = ops.kv_attn(out, *parts, table, n, d ** -0.5)
+    assert torch.equal(whole, ops.kv_attn(q.clone(memory_format=torch.contiguous_format), *parts, table, n, d ** -0.5))
+    assert ops.kv_append(k, v, *parts, table, n, q=out) is out
