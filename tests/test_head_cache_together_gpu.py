@@ -133,3 +133,47 @@ def test_a_captured_step_decodes_as_an_eager_one(cuda_ok):
         assert torch.equal(token, a) and torch.equal(logp, b)
     assert all(torch.equal(x, y) for x, y in zip(m.cache[1::2] + [m.lens], eager.cache[1::2] + [eager.lens]))
     ops.device_status()
+
+
+def test_a_captured_step_leaves_the_cache_of_an_eager_one(cuda_ok):
+    """Codes and scales, byte by byte, and the log probabilities' alternatives."""
+    from kernelswift_b200 import ops
+
+    def begin():
+        m = Layer(seed=5)
+        m.step(torch.arange(B * 20, device="cuda").view(B, 20))
+        m.lens += 20
+        return m, torch.arange(B, device="cuda")[:, None].contiguous()
+
+    def decode(m, token, top):
+        _, _, logits = m.step(token)
+        token.copy_(logits[:, 0].argmax(-1, keepdim=True))
+        for x, y in zip(top, ops.token_logprobs(logits, token, top=4)):
+            x.copy_(y)
+        m.lens += 1
+
+    def outputs():
+        at = (B, 1)
+        return [torch.zeros(at, device="cuda"), torch.zeros(at, device="cuda"), torch.zeros(*at, 4, device="cuda"),
+                torch.zeros(*at, 4, dtype=torch.int64, device="cuda")]
+
+    (eager, token), top = begin(), outputs()
+    want = []
+    for _ in range(20):
+        decode(eager, token, top)
+        want.append([x.clone() for x in top])
+    (m, token), top = begin(), outputs()
+    start = [x.clone() for x in (*m.cache, m.lens, token)]
+    decode(m, token, top)  # a pass before the capture, taken back below
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        decode(m, token, top)
+    for x, y in zip((*m.cache, m.lens, token), start):
+        x.copy_(y)
+    for step in want:
+        graph.replay()
+        assert all(torch.equal(x, y) for x, y in zip(top, step))
+    for x, y in zip((*m.cache, m.lens), (*eager.cache, eager.lens)):
+        assert torch.equal(x.view(torch.uint8), y.view(torch.uint8))
+    assert any(int((x.view(torch.uint8) != y.view(torch.uint8)).sum()) for x, y in zip(m.cache, start))
+    ops.device_status()

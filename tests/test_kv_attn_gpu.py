@@ -516,3 +516,25 @@ def test_rows_beside_a_widely_spread_one_lose_nothing(cuda_ok, T, d):
     q[..., 1::2, 2::4] *= 2.0 ** -25
     parts[0].view(torch.uint8)[..., ::4] = 0
     check(q, parts, table, lens, 0.1)
+
+
+@pytest.mark.parametrize("d,T,H", [(64, 1, 16), (64, 2, 16), (128, 1, 16), (128, 2, 16), (192, 1, 16), (256, 1, 16)])
+def test_weights_of_few_rows_are_good_to_half_a_step_of_fp16(cuda_ok, d, T, H):
+    """Values that cancel, so that the weights' rounding shows: two keys, the second one's values the
+    negative of the first one's.  Each weight is off by at most 2^-11 of itself (2^-32 of the largest
+    where it is smaller than fp16's normal numbers), the sum of them by no rounding but fp32's."""
+    from kernelswift_b200 import ops
+
+    B = 64
+    g, q, parts, table, lens = make(B, T, H, 2, d, 16, 16, [1] * B, 50 + d + T)
+    codes = parts[2].view(torch.uint8)
+    codes[:, :, 1] = codes[:, :, 0] ^ 0x80
+    mask = torch.zeros(B, T, T, dtype=torch.bool, device="cuda")
+    mask[:, :, 0] = True  # every token sees the cached row and the first new one
+    got = ops.kv_attn(q, *parts, table, lens, d ** -0.5, mask=mask).double()
+    ops.device_status()
+    ref, size, off = reference(q, parts, table, lens, d ** -0.5, mask=mask)
+    most = size.amax()
+    lim = 2.0 ** -8 * ref.abs() + (2.0 ** -11 + 2.0 ** -16 + off) * size + 2.0 ** -32 * most
+    assert ((got - ref).abs() <= lim).all()
+    assert float((ref.abs() < 0.1 * size).double().mean()) > 0.05  # many do cancel

@@ -169,3 +169,26 @@ def test_no_rows(cuda_ok):
 
     logp, ent, tl, ti = ops.token_logprobs(torch.empty(0, 100, device="cuda"), torch.empty(0, dtype=torch.int64, device="cuda"), top=3)
     assert logp.shape == (0,) and tl.shape == (0, 3) and ti.shape == (0, 3)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_a_replay_on_other_logits_gives_theirs(cuda_ok, dtype):
+    """The captured call, replayed on other logits and tokens: all four outputs are those of a call of
+    its own, which the restatement confirms."""
+    from kernelswift_b200 import ops
+
+    g = torch.Generator(device="cuda").manual_seed(19)
+    x = torch.randn(5, 70000, device="cuda", generator=g).to(dtype)
+    tokens = torch.randint(0, 70000, (5,), device="cuda", generator=g)
+    graph = torch.cuda.CUDAGraph()
+    ops.token_logprobs(x, tokens, top=20)
+    with torch.cuda.graph(graph):
+        got = ops.token_logprobs(x, tokens, top=20)
+    for i in range(3):
+        x.copy_(torch.randn(5, 70000, device="cuda", generator=g) * (i + 1))
+        tokens.copy_(torch.randint(0, 70000, (5,), device="cuda", generator=g))
+        for out in got:
+            out.fill_(-7)
+        graph.replay()
+        for a, b in zip(got, check(x, tokens, 20)):
+            assert torch.equal(a, b)
