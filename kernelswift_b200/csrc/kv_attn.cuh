@@ -215,14 +215,6 @@ __device__ __forceinline__ uint32_t kva_factor(uint32_t scale_bits, float* rest)
   *rest = __uint_as_float((e + 120u > 254u ? e + 120u - 254u + 127u : 127u) << 23);
   return (f << 7) * 0x00010001u;
 }
-// Bits of e4m3 codes in the high bytes of two halves to bf16 2^-120 times as large.
-__device__ __forceinline__ uint32_t kva_place(uint32_t x) { return ((x >> 4) & 0x07F007F0u) | (x & 0x80008000u); }
-
-__device__ __forceinline__ float kva_ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
 
 // Codes that are NaN among four, as bits 7, 15, 23, 31.
 __device__ __forceinline__ uint32_t kva_nan4(uint32_t w) {
@@ -236,7 +228,7 @@ __device__ __forceinline__ uint32_t kva_nan4_bits(uint32_t w) {
 
 // A row's result: bf16 of o / den, zeros where nothing is seen.
 __device__ __forceinline__ float kva_norm(float m, float l, float sink_log2, bool has_sink) {
-  if (has_sink) l += kva_ex2(sink_log2 - (m == -INFINITY ? 0.f : m) - KVA_DOWN);
+  if (has_sink) l += ex2f(sink_log2 - (m == -INFINITY ? 0.f : m) - KVA_DOWN);
   return l == 0.f ? 0.f : 1.f / l;  // (a NaN stays one)
 }
 
@@ -284,12 +276,6 @@ __device__ __forceinline__ void kvf_query(const uint16_t* q, bool in, int sh, bo
   }
 }
 
-template <int W>
-__device__ __forceinline__ void kvf_load(uint32_t (&v)[W], const uint8_t* ptr) {
-  asm volatile("ld.global.nc.L1::no_allocate.v4.b32 {%0, %1, %2, %3}, [%4];"
-               : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3])
-               : "l"(ptr));
-}
 template <int W>
 __device__ __forceinline__ void kvf_lds(uint32_t (&v)[W], uint32_t addr) {
   if constexpr (W == 4)
@@ -574,7 +560,7 @@ __global__ void __launch_bounds__(KVF_WARPS * 32, D * NT <= 128 ? 2 : 1) kv_attn
 #pragma unroll
             for (int x = 4; x < 32; x <<= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, x));
             const float now = fmaxf(m[g][i], top);
-            const float f = now == -INFINITY ? 1.f : kva_ex2(m[g][i] - now);
+            const float f = now == -INFINITY ? 1.f : ex2f(m[g][i] - now);
             m[g][i] = now;
             mu[g][i] = (now == -INFINITY ? 0.f : now) - KVF_TOP;
             l[g][i] *= f;
@@ -591,7 +577,7 @@ __global__ void __launch_bounds__(KVF_WARPS * 32, D * NT <= 128 ? 2 : 1) kv_attn
         float e[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          e[i] = kva_ex2(s[g][i] - mu[g][i & 1]);
+          e[i] = ex2f(s[g][i] - mu[g][i & 1]);
           l[g][i & 1] += e[i];
         }
         pb[g][0] = kvf_trans(kvf_f16x2(e[0], e[1]));
@@ -691,7 +677,7 @@ __global__ void __launch_bounds__(KVF_WARPS * 32, D * NT <= 128 ? 2 : 1) kv_attn
         float top = -INFINITY;
 #pragma unroll
         for (int x = 0; x < KVF_WARPS; ++x) top = fmaxf(top, sm_m[x][g * 8 + 2 * c + i]);
-        const float f = top == -INFINITY ? 1.f : kva_ex2(m[g][i] - top);
+        const float f = top == -INFINITY ? 1.f : ex2f(m[g][i] - top);
 #pragma unroll
         for (int y = 0; y < D / 16; ++y) {
           o[g][y][i] *= f;
@@ -721,7 +707,7 @@ __global__ void __launch_bounds__(KVF_WARPS * 32, D * NT <= 128 ? 2 : 1) kv_attn
       for (int x = 0; x < KVF_WARPS; ++x) top = fmaxf(top, sm_m[x][row]);
 #pragma unroll
       for (int x = 0; x < KVF_WARPS; ++x)
-        sum += top == -INFINITY ? sm_l[x][row] : sm_l[x][row] * kva_ex2(sm_m[x][row] - top);
+        sum += top == -INFINITY ? sm_l[x][row] : sm_l[x][row] * ex2f(sm_m[x][row] - top);
       if (whole) {
         const int t = (r0 + row) / p.G, g = (r0 + row) - t * p.G;
         if (r0 + row < p.rows) {
@@ -766,7 +752,7 @@ __global__ void __launch_bounds__(256) kv_attn_join_kernel(const __grid_constant
     float top = -INFINITY, sum = 0.f;
     const auto take = [&](const float2 ml, const float4 y) {
       const float now = fmaxf(top, ml.x);
-      const float f0 = now == -INFINITY ? 1.f : kva_ex2(top - now), f1 = now == -INFINITY ? 1.f : kva_ex2(ml.x - now);
+      const float f0 = now == -INFINITY ? 1.f : ex2f(top - now), f1 = now == -INFINITY ? 1.f : ex2f(ml.x - now);
       top = now;
       sum = f0 * sum + f1 * ml.y;
       v = make_float4(f0 * v.x + f1 * y.x, f0 * v.y + f1 * y.y, f0 * v.z + f1 * y.z, f0 * v.w + f1 * y.w);

@@ -152,26 +152,15 @@ __device__ __forceinline__ float kvw_max3(float a, float b, float c) {
   asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
 }
+__device__ __forceinline__ void kvw_load(uint32_t (&v)[4], const uint8_t* ptr) {
+  asm volatile("ld.global.nc.L1::no_allocate.v4.b32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3])
+               : "l"(ptr));
+}
 // Two e4m3 codes in the low bytes of two halves to bf16 2^-120 times as large: exponent and
 // mantissa move up by four bits and the sign by eight.  (As multiplications, which leave the
 // integer pipe to the softmax: shifts and masks there took 4 of every 10 of its cycles.)
 __device__ __forceinline__ uint32_t kvw_place(uint32_t x) { return (x & 0x00800080u) * 0xF0u + x * 16u; }
-
-__device__ __forceinline__ float2 kvw_fma2(float2 a, float2 b, float2 c) {
-  float2 r;
-  asm("{ .reg .b64 w, x, y, z; mov.b64 w, {%2, %3}; mov.b64 x, {%4, %5}; mov.b64 y, {%6, %7};"
-      " fma.rn.f32x2 z, w, x, y; mov.b64 {%0, %1}, z; }"
-      : "=f"(r.x), "=f"(r.y)
-      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
-  return r;
-}
-__device__ __forceinline__ float2 kvw_add2(float2 a, float2 b) {
-  float2 r;
-  asm("{ .reg .b64 x, y, z; mov.b64 x, {%2, %3}; mov.b64 y, {%4, %5}; add.rn.f32x2 z, x, y; mov.b64 {%0, %1}, z; }"
-      : "=f"(r.x), "=f"(r.y)
-      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
-  return r;
-}
 
 template <int D>
 __global__ void __launch_bounds__(KVW_THREADS, 1) kv_attn_wide_kernel(const __grid_constant__ KvAttnParams p) {
@@ -342,7 +331,7 @@ __global__ void __launch_bounds__(KVW_THREADS, 1) kv_attn_wide_kernel(const __gr
         // ---------------------------------------------------------- raise the reference
         if (__any_sync(0xFFFFFFFFu, top > m + KVA_RISE)) {
           const float now = fmaxf(m, top);
-          const float f = now == -INFINITY ? 1.f : kva_ex2(m - now);
+          const float f = now == -INFINITY ? 1.f : ex2f(m - now);
           m = now;
           l *= f;
           if (last >= 0) {
@@ -370,9 +359,9 @@ __global__ void __launch_bounds__(KVW_THREADS, 1) kv_attn_wide_kernel(const __gr
           uint32_t e[16];
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
-            float2 y = kvw_fma2(make_float2(x[32 * c + 2 * i], x[32 * c + 2 * i + 1]), sc, minus);
-            y = make_float2(kva_ex2(y.x), kva_ex2(y.y));
-            sum = kvw_add2(sum, y);
+            float2 y = fma2(make_float2(x[32 * c + 2 * i], x[32 * c + 2 * i + 1]), sc, minus);
+            y = make_float2(ex2f(y.x), ex2f(y.y));
+            sum = add2(sum, y);
             e[i] = cvt_bf16x2(y.x, y.y);
           }
           tmem_st16(s_col + 16 * c, e);
@@ -421,8 +410,8 @@ __global__ void __launch_bounds__(KVW_THREADS, 1) kv_attn_wide_kernel(const __gr
         if (both) {
           const float m1 = sh->m[t128], l1 = sh->l[t128];
           const float now = fmaxf(m, m1);
-          f0 = now == -INFINITY ? 1.f : kva_ex2(m - now);
-          f1 = now == -INFINITY ? 1.f : kva_ex2(m1 - now);
+          f0 = now == -INFINITY ? 1.f : ex2f(m - now);
+          f1 = now == -INFINITY ? 1.f : ex2f(m1 - now);
           l = l * f0 + l1 * f1;
           m = now;
           if (sh->nans[t128]) {
@@ -714,7 +703,7 @@ __global__ void __launch_bounds__(KVW_THREADS, 1) kv_attn_wide_kernel(const __gr
     uint32_t code[AHEAD][4];
     const auto load = [&](int q, const KvwMeta& m, const uint8_t* src, uint32_t (&v)[4]) {
       const int step = cw + q * KVW_CONV_WARPS, key = step * KEYS;
-      if (step < STEPS) kvf_load<4>(v, src + (int64_t)m.place[(key >> 4) & 7] * (16 * D) + (key & 15) * D);
+      if (step < STEPS) kvw_load(v, src + (int64_t)m.place[(key >> 4) & 7] * (16 * D) + (key & 15) * D);
     };
     const auto source = [&](uint32_t flags) { return (flags & KVW_VALUES ? p.c.v8 : p.c.k8) + (k0 * D + c * 16); };
     const auto known = [&](uint32_t u, uint32_t* flags) {

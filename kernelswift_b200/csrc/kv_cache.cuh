@@ -107,12 +107,6 @@ __device__ __forceinline__ bool kv_freq_row(const KvAppendParams& p, int b, int 
   return r == *row;
 }
 __device__ __forceinline__ uint32_t kv_div(uint32_t x, int d, int shift) { return shift >= 0 ? x >> shift : x / (uint32_t)d; }
-// The larger, NaN where either is.
-__device__ __forceinline__ float kv_max_nan(float a, float b) {
-  float r;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
-  return r;
-}
 
 __device__ __forceinline__ float e4m3_f32(uint32_t code) {
   uint32_t h;
@@ -221,16 +215,16 @@ __global__ void __launch_bounds__(THREADS, NP <= 2 ? 1280 / THREADS : 1) kv_appe
       report_bounds(c.status, b, p.n_freqs);
     kv_rotate8(raw[i], y[i], freqs, fr, p.rd, rc);  // (zeros where the row is not the call's)
 #pragma unroll
-    for (int j = 0; j < 8; ++j) amax = kv_max_nan(amax, fabsf(y[i][j]));
+    for (int j = 0; j < 8; ++j) amax = max_nan(amax, fabsf(y[i][j]));
   }
   __shared__ float red[2][THREADS / 32];
   const auto largest = [&](float (&r)[THREADS / 32], float a) {
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) a = kv_max_nan(a, __shfl_xor_sync(0xFFFFFFFFu, a, o));
+    for (int o = 16; o > 0; o >>= 1) a = max_nan(a, __shfl_xor_sync(0xFFFFFFFFu, a, o));
     if ((tid & 31) == 0) r[tid >> 5] = a;
     __syncthreads();
 #pragma unroll
-    for (int w = 0; w < THREADS / 32; ++w) a = kv_max_nan(a, r[w]);
+    for (int w = 0; w < THREADS / 32; ++w) a = max_nan(a, r[w]);
     return a;
   };
   amax = largest(red[0], amax);

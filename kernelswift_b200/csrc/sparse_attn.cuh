@@ -122,12 +122,6 @@ struct SaShared {
 };
 static_assert(sizeof(SaShared) <= SA_HDR, "SaShared exceeds the header");
 
-__device__ __forceinline__ float ex2f(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
 // One warp's "my part of this chunk is in shared memory" for the leader CTA's
 // barrier: every lane fences its own stores for the tensor core (async proxy),
 // then one lane arrives, locally in CTA 0 or remotely (release, cluster scope)

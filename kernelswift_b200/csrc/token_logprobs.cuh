@@ -101,44 +101,9 @@ __device__ __forceinline__ void lp_merge(float& m, float& s, float& t, float m2,
   m = M;
 }
 
-__device__ __forceinline__ float lp_ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
-// Two fp32 operations in one instruction.
-__device__ __forceinline__ float2 lp_add2(float2 a, float2 b) {
-  float2 r;
-  asm("{ .reg .b64 x, y, z; mov.b64 x, {%2, %3}; mov.b64 y, {%4, %5}; add.rn.f32x2 z, x, y; mov.b64 {%0, %1}, z; }"
-      : "=f"(r.x), "=f"(r.y)
-      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
-  return r;
-}
-__device__ __forceinline__ float2 lp_mul2(float2 a, float2 b) {
-  float2 r;
-  asm("{ .reg .b64 x, y, z; mov.b64 x, {%2, %3}; mov.b64 y, {%4, %5}; mul.rn.f32x2 z, x, y; mov.b64 {%0, %1}, z; }"
-      : "=f"(r.x), "=f"(r.y)
-      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
-  return r;
-}
-__device__ __forceinline__ float2 lp_fma2(float2 a, float2 b, float2 c) {
-  float2 r;
-  asm("{ .reg .b64 w, x, y, z; mov.b64 w, {%2, %3}; mov.b64 x, {%4, %5}; mov.b64 y, {%6, %7};"
-      " fma.rn.f32x2 z, w, x, y; mov.b64 {%0, %1}, z; }"
-      : "=f"(r.x), "=f"(r.y)
-      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
-  return r;
-}
 __device__ __forceinline__ uint32_t lp_max_nan_bf16x2(uint32_t a, uint32_t b) {
   uint32_t r;
   asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
-  return r;
-}
-// The larger, a NaN where a is one.
-__device__ __forceinline__ float lp_max_nan(float a, float b) {
-  float r;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
   return r;
 }
 __device__ __forceinline__ uint32_t lp_max_bf16x2(uint32_t a, uint32_t b) {
@@ -333,10 +298,10 @@ __global__ void __launch_bounds__(LP_THREADS, 4) token_logprobs_kernel(LogprobsP
     if (near) {
       const float2 minus = make_float2(-h, -h), log2e = make_float2(C, C);
       const auto add = [&](float a, float c) {
-        const float2 y = lp_fma2(make_float2(a, c), log2e, minus);
-        const float2 e = make_float2(lp_ex2(y.x), lp_ex2(y.y));
-        s2 = lp_add2(s2, e);
-        t2 = lp_fma2(e, y, t2);
+        const float2 y = fma2(make_float2(a, c), log2e, minus);
+        const float2 e = make_float2(ex2f(y.x), ex2f(y.y));
+        s2 = add2(s2, e);
+        t2 = fma2(e, y, t2);
       };
       // (values below -1e37, -inf among them, count as that: e = 0 and e y = 0; NaN stays)
 #pragma unroll
@@ -350,7 +315,7 @@ __global__ void __launch_bounds__(LP_THREADS, 4) token_logprobs_kernel(LogprobsP
           }
         } else {
 #pragma unroll
-          for (int j = 0; j < 4; j += 2) add(lp_max_nan(v[i].at(j), -1e37f), lp_max_nan(v[i].at(j + 1), -1e37f));
+          for (int j = 0; j < 4; j += 2) add(max_nan(v[i].at(j), -1e37f), max_nan(v[i].at(j + 1), -1e37f));
         }
       }
     } else {
@@ -360,20 +325,20 @@ __global__ void __launch_bounds__(LP_THREADS, 4) token_logprobs_kernel(LogprobsP
         for (int j = 0; j < E; ++j) {
           const float x = v[i].at(j);
           // nothing but -inf: 0, and NaN where it is one
-          const float y = m == -INFINITY ? x - x : lp_max_nan((x - m) * C, -200.f);
-          const float z = m == -INFINITY ? (x != x ? x : 0.f) : lp_ex2(y);
+          const float y = m == -INFINITY ? x - x : max_nan((x - m) * C, -200.f);
+          const float z = m == -INFINITY ? (x != x ? x : 0.f) : ex2f(y);
           s2.x += z;
           if (m > -INFINITY) t2.x = fmaf(z, y, t2.x);
         }
     }
     float s = s2.x + s2.y, t = t2.x + t2.y;
     if (near) {
-      const float f = lp_ex2(-err);
+      const float f = ex2f(-err);
       t = f * (t - err * s);
       s *= f;
     }
     // raise what is there to the new maximum
-    const float d = M == m ? 0.f : (M - m) * C, f = lp_ex2(d);
+    const float d = M == m ? 0.f : (M - m) * C, f = ex2f(d);
     Tt = (f > 0.f ? f * (Tt + S * d) : 0.f) + t;
     S = S * f + s;
     M = m;
@@ -389,7 +354,7 @@ __global__ void __launch_bounds__(LP_THREADS, 4) token_logprobs_kernel(LogprobsP
   }
   const bool nan = __any_sync(0xFFFFFFFFu, bad);
   {
-    const float d = M == wm ? 0.f : (M - wm) * C, f = lp_ex2(d);
+    const float d = M == wm ? 0.f : (M - wm) * C, f = ex2f(d);
     Tt = f > 0.f ? f * (Tt + S * d) : 0.f;
     S *= f;
 #pragma unroll
