@@ -337,7 +337,8 @@ int ks_verify_draft(const float* p, const float* q, const void* tokens, int32_t 
  *          rows rotated like the keys, rounded once
  *   freqs  fp32 [n_freqs, rope_dim / 2, 2] (cos, sin): the last rope_dim columns of a key are
  *          rotated, as pairs (2 i, 2 i + 1), by the row of its position (positions int32
- *          [B, T], or NULL: its place in the sequence); rope_dim 0: no rotation
+ *          [B, T], or NULL: its place in the sequence); rope_dim 0: no rotation.  (Models that
+ *          rotate halves, or the first columns, permute the rows of both projections once.)
  *   k8, v8 e4m3 [n_pages, heads, page, D], k_scale, v_scale fp32 [n_pages, heads, page / block]
  *   page_table int32 [B, max_pages], lens int32 [B]: tokens cached so far; token t of
  *          sequence b goes to position lens[b] + t, if t < n_new[b] (NULL: T)
@@ -367,9 +368,11 @@ int ks_kv_append(const void* k, int64_t k_bs, int64_t k_ts, const void* v, int64
  *          of the call's own tokens, cached at lens[b] .., those j < n_new[b] with mask[b, t, j]
  *          (bytes [B, T, T]; NULL: j <= t); the others get zeros
  *   attn_sink fp32 [H] or NULL: a logit per head that takes part in the softmax without a value
- * Scores, sums and outputs are fp32; weights enter the product with the values in 16 bits, off by
- * at most 2^-8 of themselves or 2^-32 of the row's largest; the result is rounded once.  A token that sees nothing gets zeros.  Positions past the table or
- * on a page outside [0, n_pages) are not seen; both are reported by ks_device_status.
+ * Scores, sums and outputs are fp32; weights enter the product with the values in 16 bits: fp16 for
+ * T * H / heads up to 16 (8 for D above 128), off by at most 2^-11 of themselves or 2^-32 of the
+ * row's largest, else bf16, off by at most 2^-8; the result is rounded once.  A token that sees
+ * nothing gets zeros.  Positions past the table or on a page outside [0, n_pages) are not seen; both
+ * are reported by ks_device_status.
  * workspace: ks_kv_attn_workspace_size bytes, 256-byte aligned, used by this call alone until it
  * is done.  No counterpart in the reference.
  */
@@ -387,7 +390,9 @@ int ks_kv_attn(const void* q, const void* k8, const float* k_scale, const void* 
  * top (<= 32, <= V) largest as top_logp fp32 [N, top], top_ids [N, top] (type of tokens), largest
  * first, the lowest index first among equal ones.  tokens int32 or int64 [N] (token_dtype);
  * a negative token's logp is 0, one >= V gets NaN and is reported by ks_device_status.  A
- * row without a finite maximum, or with a NaN, gets NaN.  No counterpart in the reference.
+ * row without a finite maximum, or with a NaN, gets NaN.  With top, rows whose largest values lie
+ * side by side (sorted ones, a stretch of some 600 allowed tokens) and rows with a NaN take top
+ * passes of one CTA.  No counterpart in the reference.
  */
 int ks_token_logprobs(const void* logits, int32_t is_bf16, int64_t ld, const void* tokens,
                       int32_t token_dtype, int64_t N, int64_t V, int32_t top, float* logp,

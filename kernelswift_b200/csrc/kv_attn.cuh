@@ -41,8 +41,12 @@
 // of four keys, and keys are assigned to the product's rows (kvf_key) so that neither read has
 // bank conflicts.
 // Measured (one B200, join included): 64 heads on 8 key heads of 128, one token over 131069 keys
-// (268 MB) 67 us, 4.0 TB/s: the loop alone runs at 0.84 of a copy's rate, and 25 us are start, ends
-// and join.  48 sequences up to 8000 keys, 40 heads on 8 (403 MB) 109-114 us, 3.6 TB/s.  The first
+// (268 MB) 66 us, 4.1 TB/s: the loop alone runs at 0.84 of a copy's rate, and 25 us are start, ends
+// and join.  48 sequences up to 8000 keys, 40 heads on 8 (403 MB) 108 to 112 us, 3.7 TB/s; with 128
+// heads (16 rows a key head: 254 registers, one CTA an SM) 184.  Short contexts are bound by row tiles
+// taken one after the other, each a chain of lookups and loads, and four barriers: 300 sequences up
+// to 60 keys, 2400 row tiles, 78 us for 24 MB.  At heads of 128 (and of 64 with 16 rows) the cap of 128
+// registers, which two CTAs an SM need, spills 60 bytes of stores and 88 of loads (44 and 76).  The first
 // form (operands from global memory to registers, bf16 by integer operations, one join group a
 // row) took 82 us: ALU 60 % of its cycles, now 45 %.  Not taken: the next row tile's queries and
 // places fetched ahead (spills: 109 us), the rare further terms of a query out of line (68 us).
@@ -51,7 +55,13 @@
 
 namespace ks {
 
-constexpr int KVA_SETUP = 2;      // units that a row tile costs beyond its tiles
+// Units that a row tile costs beyond its tiles, for both kernels.  Measured (us, L2 flushed) with 1, 2, 4, 6,
+// 10: one sequence of 509 keys 16.5, 16.5, 16.6, 18.2, 18.4, since CTAs of nothing but setting up come
+// on top of the parts; 40 sequences up to 500 keys 31.8, 31.6, 32.8, 33.4, 32.7; 48 up to 8000 keys 129,
+// 118, 105, 100, 100; 16 trees of 13 129, 108, 102, 97, 99; one of 131069 keys 82, 79, 78, 78, 77; a chunk
+// of 4096 tokens the same with all.  Two keeps the small calls; a value for each kernel and size,
+// which the ragged ones ask for, is not built.
+constexpr int KVA_SETUP = 2;
 constexpr float KVA_RISE = 8.f;   // how far a score may pass its reference (base 2)
 constexpr float KVA_DOWN = 24.f;  // weights are 2^-24: 2^(8 - 24) * 2^14 keys * 2^128 is finite
 constexpr int KVF_WARPS = 8;

@@ -26,13 +26,15 @@
 //
 // Bound by the chain scores -> weights -> output and by the expansion, no unit being full (1024
 // tokens of 64 heads of 128 on 8 behind 12288, under a profiler: tensor cores 41 % of their cycles,
-// issue 59 %, ALU 44 %, exponentials 41 %).  Measured (one B200): 4096 such tokens 2240 us, 860
-// TFLOP/s, in short runs, 2443 us in runs long enough for the power limit; 2048 tokens of heads of
-// 256 2.5 ms (714 TFLOP/s, expansion bound: a unit is twice as large); 16 trees of 13 tokens, 64
-// heads on 8, up to 6001 keys 92 us (5 K cycles a tile, 10 us of it the join).  The steps that made
-// the 4096 tokens faster, in short runs: 3240 us; codes loaded a unit ahead and no rare path unrolled
-// 2560; buffers of 64 keys 2320; one issuing thread 2265 to 2339; more registers for the expansion
-// 2240.
+// issue 59 %, ALU 44 %, exponentials 41 %).  Measured (one B200): 4096 such tokens 2470 us, 779
+// TFLOP/s (2255 in runs too short for the power limit); 2048 tokens of heads of 256 2.5 ms in short
+// runs (714 TFLOP/s, expansion bound: a unit is twice as large); 16 trees of 13 tokens, 64 heads on
+// 8, up to 6001 keys 92 to 96 us (5 K cycles a tile, 10 us of it the join), chains of 3 tokens 83: a
+// product has 128 rows whatever the call has.  The steps that made the 4096 tokens faster, in short
+// runs: 3240 us; codes loaded a unit ahead and no rare path unrolled 2560; buffers of 64 keys 2320;
+// one issuing thread 2265 to 2339; more registers for the expansion 2240.
+// 80 registers at launch make the softmax's code spill: 212 bytes of stores and 420 of loads at heads
+// of 256, 228 and 488 at 128, 184 and 384 at 64.
 //
 // References are raised only when a score passes them by 2^KVA_RISE (rarely after the first
 // tiles); then the row's output is scaled in place once its last product is done.

@@ -20,10 +20,11 @@
 // writes the block, so there are no races and no atomics; every row is read once and kept in
 // registers between the maximum and the conversion.  Further CTAs rotate the queries.
 // Bound by memory, for few rows by launch latency.  Measured (one B200): two prompts of 16384 tokens,
-// 32 query and 8 key heads of 128, all columns rotated, blocks of 16: 168 us (755 MB, 4.5 TB/s, 0.70 of
-// a copy's rate; issue slots 80 %, so the rotation and the conversion count: with values held in bf16
-// between maximum and conversion, and rotated twice, 238 us); blocks of 64 230 us (more registers a
-// thread, fewer CTAs an SM); one token of 8 sequences 5.5 us on the device.
+// 32 query and 8 key heads of 128, all columns rotated, blocks of 16: 165 to 168 us (755 MB, 4.5 TB/s,
+// 0.70 of a copy's rate; issue slots 80 %, so the rotation and the conversion count: with values held
+// in bf16 between maximum and conversion, and rotated twice, 238 us; cos and sin, 512 bytes a token, are
+// read again for every head); blocks of 64 231 us (more registers a thread, fewer CTAs an SM); one
+// token of 8 sequences 5.5 us on the device.
 #pragma once
 #include <cuda_fp16.h>
 

@@ -124,3 +124,28 @@ def test_logprob_restatement_agrees_with_torch():
         p = lp[i].exp()
         assert np.isclose(a, lp[i, 3]) and np.isclose(b, -(torch.where(p > 0, p * lp[i], 0.0)).sum())
         assert np.allclose(c, lp[i].topk(4).values) and d.tolist() == lp[i].topk(4).indices.tolist()
+
+
+@pytest.mark.parametrize("first", [False, True])
+def test_models_that_rotate_halves_permute_their_projections(first):
+    """Rotation of halves (i, i + rd/2), of a head's last or first columns: with the columns of queries
+    and keys permuted alike, the rotation of pairs at the end gives the same scores."""
+    rng = np.random.default_rng(3)
+    d, rd, n = 24, 16, 7
+    q, k = rng.standard_normal((2, n, 1, d)).astype(np.float32)
+    ang = np.outer(np.arange(n), 0.3 ** np.arange(rd // 2))
+    fr = np.stack([np.cos(ang), np.sin(ang)], -1)
+    at = 0 if first else d - rd
+
+    def halves(x):
+        y = x.astype(np.float64)
+        a, b = x[..., at:at + rd // 2], x[..., at + rd // 2:at + rd]
+        c, s = fr[:, None, :, 0], fr[:, None, :, 1]
+        y[..., at:at + rd // 2], y[..., at + rd // 2:at + rd] = a * c - b * s, a * s + b * c
+        return y[:, 0]
+
+    rest = [i for i in range(d) if not at <= i < at + rd]
+    order = rest + [at + i // 2 + (i % 2) * (rd // 2) for i in range(rd)]
+    pairs = [O.rotate(x[..., order], fr, np.arange(n)).astype(np.float64)[:, 0] for x in (q, k)]
+    # (fp32 rotation: 2^-22 of the sums' terms)
+    assert np.allclose(pairs[0] @ pairs[1].T, halves(q) @ halves(k).T, atol=2.0 ** -22 * d * 20)
