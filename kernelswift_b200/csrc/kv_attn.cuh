@@ -505,7 +505,9 @@ __global__ void __launch_bounds__(KVF_WARPS * 32, D * NT <= 128 ? 2 : 1) kv_attn
 #pragma unroll
           for (int g = 0; g < NT; ++g) kvf_mma(i & 1 ? s_odd[g] : s[g], a, qf[g][j][i][0], qf[g][j][i][1]);
         }
-      // (the product of the factors may pass the range where the score does not, at zero codes)
+      // (The product of the factors may pass the range where the score does not, at zero codes; scores
+      // beyond 2^103 may come out smaller.  A softmax scale and a power that are below 2^-126 together put
+      // a score off by at most 2^-118 times the key scale, which shows for keys above 2^100 alone.)
       const float ks = __uint_as_float(cur.ks & 0x7F800000u), vs = __uint_as_float(cur.vs & 0x7F800000u) * 0x1p-31f;
       const auto factor = [&](float back) { return fminf(fmaxf(back * ks, -3e38f), 3e38f); };
 #pragma unroll
