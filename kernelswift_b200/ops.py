@@ -786,9 +786,9 @@ def kv_attn(q: torch.Tensor, k8: torch.Tensor, k_scale: torch.Tensor, v8: torch.
     nothing gets zeros.  Weights enter their product in 16 bits: fp16 where T * H / heads is
     at most 16 (8 for D above 128), off by at most 2^-11 of themselves or 2^-32 of the row's
     largest; else bf16, off by at most 2^-8, so a token's last bits depend on how many share its
-    call.  Scores and sums are fp32, the result is rounded once.  workspace: ``kv_attn_workspace_size(T, H, heads, D)`` bytes, 256-byte
-    aligned, used by this call alone until it is done (None: allocated); out: where the
-    result goes."""
+    call.  Scores and sums are fp32, the result is rounded once.
+    workspace: ``kv_attn_workspace_size(T, H, heads, D)`` bytes, 256-byte aligned, used by this
+    call alone until it is done (None: allocated); out: where the result goes."""
     shape = q.shape
     if q.dtype != torch.bfloat16 or len(shape) != 4:
         raise RuntimeError("kv_attn: q must be bfloat16 [b, t, h, d]")
